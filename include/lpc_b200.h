@@ -357,6 +357,111 @@ LPC_API int lpc_qkv_rope_append(const void* x, const void* packed_w, const int64
                                 float norm_eps, void* stream);
 
 /*
+ * 4-bit KV cache.  No counterpart in the reference, whose INT4 precision
+ * (config.py:27-60) sizes a cache but runs nothing.  A row (one position of
+ * one KV head) is head_dim / 2 bytes of codes -- byte j holds dim j in its low
+ * and dim j + head_dim/2 in its high four bits -- and four numbers of the
+ * data type, s0 m0 s1 m1: a code c of the lower half of the dims stands for
+ * s0 * c + m0, one of the upper half for s1 * c + m1.
+ *   dense  (seq_base NULL): codes [max_batch, kv_heads, max_seq_len, head_dim/2],
+ *          scales [max_batch, kv_heads, max_seq_len, 4];
+ *   ragged: codes [kv_heads, total_rows, head_dim/2], scales [kv_heads,
+ *          total_rows, 4]; sequence b owns rows [seq_base[b], seq_base[b] +
+ *          seq_cap[b]) of every head, max_seq_len bounds every seq_cap.
+ * Codes 16-byte, scales 8-byte aligned.  head_dim 32, 64 or 128; bf16 or fp16.
+ */
+typedef struct lpc_kv4 {
+  void* key_codes;
+  void* key_scales;
+  void* value_codes;
+  void* value_scales;
+  const int64_t* seq_base; /* device, ragged only */
+  const int32_t* seq_cap;  /* device, ragged only */
+  int64_t max_batch;       /* dense only */
+  int64_t max_seq_len;
+  int64_t total_rows;      /* ragged only */
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  int32_t reserved;
+} lpc_kv4;
+
+/*
+ * lpc_rope_kv_append (and _ragged) into a 4-bit cache: q rotated into q_out
+ * [batch, heads, seq, head_dim]; rotated k, rounded to the data type, and v
+ * quantised into the row of (b, positions[b, s]).  Per half of the dims:
+ *   m = min, s = T((max - min) / 15), c = clamp(rint((x - m) * (1/s)), 0, 15),
+ * each operation rounded once in fp32; s below 2^-126 becomes 0, and so do its
+ * codes.  A half with a non-finite value, or whose s overflows the type, holds
+ * s = m = NaN and reads as NaN.  A negative position is skipped (its q rows
+ * become zero); one outside the sequence's rows or the tables is skipped and
+ * flagged in lpc_device_status().  Positions of one sequence must differ.
+ * cos/sin [table_rows, head_dim] in the data type or fp32.
+ */
+LPC_API int lpc_rope_kv_append_int4(const lpc_kv4* kv, const void* qkv, const int64_t* positions,
+                                    const void* cos, const void* sin, int64_t table_rows,
+                                    void* q_out, int64_t batch, int64_t seq, int num_heads,
+                                    int table_dtype, void* stream);
+
+/*
+ * The values of the rows at positions [batch, seq] (int64, device), T(s*c + m):
+ * k_out, v_out [batch, kv_heads, seq, head_dim].  Rows of negative positions
+ * are zero; so are those outside the sequence's rows, which are flagged too.
+ * What a prompt chunk after the first needs for lpc_flash_attention.
+ */
+LPC_API int lpc_kv_read_int4(const lpc_kv4* kv, const int64_t* positions, void* k_out, void* v_out,
+                             int64_t batch, int64_t seq, void* stream);
+
+/*
+ * lpc_decode_attention (and _ragged) over a 4-bit cache: q and out [batch,
+ * heads, head_dim], keys [0, seq_lens[b]) of sequence b; an empty sequence
+ * gives zeros, a length beyond the sequence's rows is cut to them and flagged.
+ * Any number of query heads per KV head.  workspace: the split partials,
+ * lpc_decode_attention_int4_workspace_bytes() bytes always suffice (NULL when
+ * one split covers the cache).  One kernel then, else two.  The partials of
+ * calls that overlap need workspaces of their own.
+ */
+LPC_API int64_t lpc_decode_attention_int4_workspace_bytes(const lpc_kv4* kv, int64_t batch,
+                                                          int heads);
+LPC_API int lpc_decode_attention_int4(const lpc_kv4* kv, const void* q, const int32_t* seq_lens,
+                                      void* out, void* workspace, int64_t workspace_bytes,
+                                      int64_t batch, int heads, float sm_scale, void* stream);
+
+/*
+ * 4-bit weights with group scales.  No counterpart in the reference.  Column k
+ * of row n stands for scales[n, g] * c + mins[n, g], c in 0..15, g = k / group,
+ * group 32, 64 or 128.  `packed` (lpc_int4_weight_bytes bytes, 16-byte
+ * aligned) is filled by lpc_int4_pack from row-major codes [rows, k/2] (column
+ * 2j in the low, 2j + 1 in the high four bits of byte j), scales and mins
+ * [rows, k/group] in the data type.  layout 0: rows = n_out.  layout 1: the
+ * SwiGLU pair, rows = 2 * n_out, gate rows first.  k a multiple of 64 and of
+ * group; n_out <= 2^24.  lpc_int4_pack returns after the copy is complete (it
+ * synchronises `stream`): lpc_int4_linear reads the weight before it waits on
+ * the kernel before it.  lpc_int4_unpack writes the values T(s*c + m), [rows,
+ * k] row-major.
+ */
+typedef struct lpc_w4 {
+  void* packed;
+  int64_t n_out;
+  int32_t k;
+  int32_t group;
+  int32_t layout;
+  int32_t dtype;
+} lpc_w4;
+LPC_API int64_t lpc_int4_weight_bytes(int64_t n_out, int k, int group, int layout);
+LPC_API int lpc_int4_pack(const lpc_w4* w, const void* codes, const void* scales, const void* mins,
+                          void* stream);
+LPC_API int lpc_int4_unpack(const lpc_w4* w, void* out, void* stream);
+
+/*
+ * out[t, n] = epilogue(sum_k x[t, k] * W[n, k]) for x [tokens, k], tokens <= 64:
+ * epilogue 0 store, 1 resid + (resid may equal out), 2 silu(gate) * up (layout 1
+ * and only it).  fp32 accumulation, one rounding.  No workspace.
+ */
+LPC_API int lpc_int4_linear(const lpc_w4* w, const void* x, void* out, const void* resid,
+                            int64_t tokens, int epilogue, void* stream);
+
+/*
  * HBM read-rate probe (a measurement utility; no reference counterpart).
  * Reads `bytes` (a positive multiple of 131072) of `buf` the way the decode
  * attention reads its cache rows: one CTA per 128 KB, 16 KB 1-D bulk copies

@@ -30,6 +30,21 @@ _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
 
+
+class Kv4(ctypes.Structure):
+    """``lpc_kv4`` of include/lpc_b200.h: where a 4-bit KV cache lives."""
+    _fields_ = [("key_codes", _P), ("key_scales", _P), ("value_codes", _P), ("value_scales", _P),
+                ("seq_base", _P), ("seq_cap", _P), ("max_batch", _I64), ("max_seq_len", _I64),
+                ("total_rows", _I64), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class W4(ctypes.Structure):
+    """``lpc_w4`` of include/lpc_b200.h: a packed 4-bit weight."""
+    _fields_ = [("packed", _P), ("n_out", _I64), ("k", ctypes.c_int32), ("group", ctypes.c_int32),
+                ("layout", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); kept in the order of include/lpc_b200.h
 SIGNATURES = {
     "lpc_version": (_I, []),
@@ -60,6 +75,14 @@ SIGNATURES = {
     "lpc_wsgemm": (_I, [_P, _P, _P, _P, _I64, _I64, _I, _I, _I, _F, _P]),
     "lpc_qkv_rope_append": (_I, [_P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I, _I,
                                  _I, _I, _I64, _I64, _I64, _I, _I, _F, _P]),
+    "lpc_rope_kv_append_int4": (_I, [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I, _I, _P]),
+    "lpc_kv_read_int4": (_I, [_P, _P, _P, _P, _I64, _I64, _P]),
+    "lpc_decode_attention_int4_workspace_bytes": (_I64, [_P, _I64, _I]),
+    "lpc_decode_attention_int4": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I, _F, _P]),
+    "lpc_int4_weight_bytes": (_I64, [_I64, _I, _I, _I]),
+    "lpc_int4_pack": (_I, [_P, _P, _P, _P, _P]),
+    "lpc_int4_unpack": (_I, [_P, _P, _P]),
+    "lpc_int4_linear": (_I, [_P, _P, _P, _P, _I64, _I, _P]),
     "lpc_hbm_read_probe": (_I, [_P, _I64, _P]),
 }
 
@@ -73,6 +96,8 @@ KERNELS_PER_CALL = {
     "lpc_decode_attention": 2, "lpc_decode_attention_noalloc": 2,
     "lpc_pack_weights": 1, "lpc_wsgemm": 1, "lpc_qkv_rope_append": 1, "lpc_rope_kv_append_ragged": 1,
     "lpc_decode_attention_ragged": 2, "lpc_rmsswiglu_folded_forward": 1, "lpc_hbm_read_probe": 1,
+    "lpc_rope_kv_append_int4": 1, "lpc_kv_read_int4": 1, "lpc_decode_attention_int4": 2,
+    "lpc_int4_pack": 2, "lpc_int4_unpack": 1, "lpc_int4_linear": 1,
 }
 launch_count = 0
 

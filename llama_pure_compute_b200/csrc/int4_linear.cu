@@ -1,0 +1,552 @@
+// Decode-sized products with 4-bit weights and group scales:
+//
+//   y[t, n] = sum_g ( s[n, g] * sum_{k in g} x[t, k] c[n, k] + m[n, g] * sum_{k in g} x[t, k] ),
+//
+// epilogues: store, residual (+ resid), SwiGLU (silu(gate) * up).
+//
+// Bound: HBM, by the weight stream of k/2 + 4 k/group bytes a row; a byte of
+// codes has 4 FLOPs a token, so up to about 30 tokens the tensor cores are not
+// the limit even on mma.sync, and what has to be kept small is the number of
+// instructions a code costs.  mma.sync m16n8k16 takes 16 weight rows (A) by 8
+// tokens (B); a packed 32-bit word holds exactly the lane's 8 codes of one
+// product, in the order in which masks pick them:
+//   fp16: (w & 0x000F000F) is a pair of subnormal halves c * 2^-24, exactly;
+//         0x00F000F0 picks rows r + 8, 16-fold.  5 instructions a word.
+//   bf16: (w & 0x000F000F) | 0x43004300 is the pair 128 + c, exactly (a bf16
+//         subnormal times x would underflow the fp32 sum).  7 instructions;
+//         the 128 is taken out again with the group's sum of x, which
+//         costs the fp32 accumulator about 5 of its 24 bits and leaves an error
+//         some hundred times below the output's rounding.
+// The sum of x over a group is one more product, of a row of ones.
+// tcgen05 would want the weights converted into shared memory for 128-row
+// tiles: at these token counts more work than the products themselves.
+//
+// Packed weight: tiles of 16 rows x 64 columns, 512 contiguous bytes, 16 a
+// lane, read with cp.async into the lane's own slots (no barrier), followed by
+// the group numbers, 64 bytes per tile row and group.  The 8 warps of a CTA
+// share a tile row's k range and add their partial sums through shared memory;
+// CTAs walk over the tile rows, and the weight stream runs on across them.
+#include <algorithm>
+#include <atomic>
+#include <cstdlib>
+
+#include "lpc_common.cuh"
+
+namespace {
+
+using lpc::Num;
+
+constexpr int WARPS = 8;
+constexpr int THREADS = WARPS * 32;
+constexpr int MAX_TOKENS = 64;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                    uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The 8 codes of a word as the A operand: rows r, r + 8 of columns 2t.., then
+// the same rows of columns 2t + 8...
+template <typename T>
+__device__ __forceinline__ void operand(uint32_t w, uint32_t (&a)[4]) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const uint32_t v = w >> 8;
+    a[0] = w & 0x000F000Fu;
+    a[1] = w & 0x00F000F0u;
+    a[2] = v & 0x000F000Fu;
+    a[3] = v & 0x00F000F0u;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float2 pair_f(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else
+    return make_float2(lpc::bf16lo(w), lpc::bf16hi(w));
+}
+
+template <int GS, int MT, int NT>
+struct Cfg {
+  static constexpr int CK = GS > 64 ? GS : 64;  // columns of a pipeline stage
+  static constexpr int TILES = CK / 64;
+  static constexpr int SG = CK / GS;            // groups of a stage
+  static constexpr int STAGE = MT * (TILES * 512 + SG * 256);
+  static constexpr int NST = (MT * TILES == 4) ? 4 : (MT * TILES == 2) ? 8 : 12;
+  static constexpr int RING = NST * STAGE;
+  static constexpr int RED = MT * 16 * NT * 8;  // fp32 partial sums of a warp
+  static constexpr int SMEM = WARPS * (RING + 2 * RED * 4);
+};
+
+enum { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_SWIGLU = 2 };
+
+template <typename T, int GS, int MT, int NT>
+__global__ void __launch_bounds__(THREADS)
+    int4_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ numbers,
+                       const T* __restrict__ x, const T* resid, T* out, int tokens, int64_t n_out,
+                       int k, int items, int epi) {
+  using C = Cfg<GS, MT, NT>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, t = lane & 3;
+  const int nchunks = k / C::CK;
+  const int kb = k / 64, ng = k / GS;
+  const int c0 = warp * nchunks / WARPS, nc = (warp + 1) * nchunks / WARPS - c0;
+  const int tok0 = blockIdx.y * (NT * 8);
+  const int ntok = min(NT * 8, tokens - tok0);
+  uint8_t* ring = smem + warp * C::RING;
+  const uint32_t ring_u = lpc::smem_u32(ring);
+  float* red = reinterpret_cast<float*>(smem + WARPS * C::RING);
+
+  auto fetch = [&](int item, int chunk, int st) {
+    const uint32_t dst = ring_u + st * C::STAGE;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int64_t tile = (int64_t)item * MT + m;
+#pragma unroll
+      for (int i = 0; i < C::TILES; ++i)
+        cp16(dst + (m * C::TILES + i) * 512 + lane * 16,
+             codes + ((tile * kb + chunk * C::TILES + i) * 512 + lane * 16));
+#pragma unroll
+      for (int g = 0; g < C::SG; ++g)
+        cp8(dst + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8,
+            numbers + ((tile * ng + chunk * C::SG + g) * 64 + r * 8));
+    }
+  };
+
+  lpc::pdl_trigger();
+  // the weights belong to no earlier kernel of the stream: their first stages
+  // are requested before the kernel that writes x is waited for
+  int fi = blockIdx.x, fc = 0, fst = 0;
+  auto advance = [&]() {
+    if (nc > 0 && fi < items) {
+      fetch(fi, c0 + fc, fst);
+      if (++fc == nc) {
+        fc = 0;
+        fi += gridDim.x;
+      }
+    }
+    cp_commit();
+    if (++fst == C::NST) fst = 0;
+  };
+#pragma unroll
+  for (int i = 0; i < C::NST - 1; ++i) advance();
+  lpc::pdl_wait();
+
+  // x of token tok0 + 8 j + r: 8 columns at 32 h + 8 t of every 64
+  const T* xp[NT];
+  bool has[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    has[j] = 8 * j + r < ntok;
+    xp[j] = x + (int64_t)(tok0 + (has[j] ? 8 * j + r : 0)) * k + 8 * t;
+  }
+  constexpr uint32_t ONES = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
+
+  int st = 0, buf = 0;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    float sum[MT][NT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[m][j][i] = 0.f;
+    for (int c = 0; c < nc; ++c) {
+      advance();
+      cp_wait<C::NST - 1>();
+      const uint8_t* s = ring + st * C::STAGE;
+      if (++st == C::NST) st = 0;
+      const int64_t col = (int64_t)(c0 + c) * C::CK;
+#pragma unroll
+      for (int g = 0; g < C::SG; ++g) {
+        float acc[MT][NT][4], ones[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ones[j][i] = 0.f;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[m][j][i] = 0.f;
+          }
+        // 32-column halves of this group: GS 128 has 4, 64 has 2, 32 has 1
+#pragma unroll
+        for (int hh = 0; hh < GS / 32; ++hh) {
+          const int half = g * (GS / 32) + hh;
+          uint4 xv[NT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            xv[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (has[j]) xv[j] = *reinterpret_cast<const uint4*>(xp[j] + col + 32 * half);
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const uint2 w = *reinterpret_cast<const uint2*>(
+                s + (m * C::TILES + (half >> 1)) * 512 + lane * 16 + (half & 1) * 8);
+            uint32_t a[4], b[4];
+            operand<T>(w.x, a);
+            operand<T>(w.y, b);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              mma<T>(acc[m][j], a[0], a[1], a[2], a[3], xv[j].x, xv[j].y);
+              mma<T>(acc[m][j], b[0], b[1], b[2], b[3], xv[j].z, xv[j].w);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            mma<T>(ones[j], ONES, ONES, ONES, ONES, xv[j].x, xv[j].y);
+            mma<T>(ones[j], ONES, ONES, ONES, ONES, xv[j].z, xv[j].w);
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint2 w = *reinterpret_cast<const uint2*>(
+              s + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8);
+          const float2 lo = pair_f<T>(w.x), hi = pair_f<T>(w.y);
+          float s0, m0, s1, m1;
+          if constexpr (std::is_same<T, __half>::value) {
+            s0 = lo.x * 16777216.f;
+            m0 = lo.y;
+            s1 = hi.x * 1048576.f;
+            m1 = hi.y;
+          } else {
+            s0 = lo.x;
+            m0 = fmaf(-128.f, lo.x, lo.y);
+            s1 = hi.x;
+            m1 = fmaf(-128.f, hi.x, hi.y);
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            sum[m][j][0] = fmaf(s0, acc[m][j][0], fmaf(m0, ones[j][0], sum[m][j][0]));
+            sum[m][j][1] = fmaf(s0, acc[m][j][1], fmaf(m0, ones[j][1], sum[m][j][1]));
+            sum[m][j][2] = fmaf(s1, acc[m][j][2], fmaf(m1, ones[j][0], sum[m][j][2]));
+            sum[m][j][3] = fmaf(s1, acc[m][j][3], fmaf(m1, ones[j][1], sum[m][j][3]));
+          }
+        }
+      }
+    }
+    // partial sums of the 8 warps, [token][row] of the item, added in warp order
+    float* mine = red + (buf * WARPS + warp) * C::RED;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float* p = mine + (8 * j + 2 * t) * (MT * 16) + m * 16 + r;
+        p[0] = sum[m][j][0];
+        p[MT * 16] = sum[m][j][1];
+        p[8] = sum[m][j][2];
+        p[MT * 16 + 8] = sum[m][j][3];
+      }
+    __syncthreads();
+    const float* all = red + buf * WARPS * C::RED;
+    auto total = [&](int at) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) v += all[w * C::RED + at];
+      return v;
+    };
+    if (epi == EPI_SWIGLU) {
+      if constexpr (MT == 2)
+        for (int i = threadIdx.x; i < ntok * 16; i += THREADS) {
+          const int tk = i >> 4, row = i & 15;
+          const int64_t n = (int64_t)item * 16 + row;
+          if (n >= n_out) continue;
+          const float gate = total(tk * 32 + row), upv = total(tk * 32 + 16 + row);
+          out[(int64_t)(tok0 + tk) * n_out + n] =
+              Num<T>::from_f(__fdividef(gate, 1.f + __expf(-gate)) * upv);
+        }
+    } else {
+      for (int i = threadIdx.x; i < ntok * (MT * 16); i += THREADS) {
+        const int tk = i / (MT * 16), row = i % (MT * 16);
+        const int64_t n = (int64_t)item * (MT * 16) + row;
+        if (n >= n_out) continue;
+        float v = total(i);
+        const int64_t o = (int64_t)(tok0 + tk) * n_out + n;
+        if (epi == EPI_RESIDUAL) v += Num<T>::to_f(resid[o]);
+        out[o] = Num<T>::from_f(v);
+      }
+    }
+    buf ^= 1;
+  }
+  cp_wait<0>();
+}
+
+// ---------------------------------------------------------------------------
+// layout
+// ---------------------------------------------------------------------------
+// Tile rows of 16: of the weight (layout 0), or gate tile i, up tile i, ...
+// (layout 1, gate rows first in the source).  An even number of them.
+__host__ __device__ inline int64_t tile_rows(int64_t n_out, int layout) {
+  const int64_t t = (n_out + 15) / 16;
+  return layout == 1 ? 2 * t : (t + 1) / 2 * 2;
+}
+// Source row of row `i` of tile row `p`, or -1 for padding.
+__device__ __forceinline__ int64_t source_row(int64_t p, int i, int64_t n_out, int layout) {
+  const int64_t n = (layout == 1 ? p >> 1 : p) * 16 + i;
+  if (n >= n_out) return -1;
+  return layout == 1 && (p & 1) ? n_out + n : n;
+}
+// Row and column (in the 64) of nibble `i`, half `p` of word j of lane (r, t).
+__device__ __forceinline__ int nibble_row(int r, int i) { return r + 8 * (i & 1); }
+__device__ __forceinline__ int nibble_col(int t, int j, int i, int p) {
+  return 32 * (j >> 1) + 8 * t + 4 * (j & 1) + 2 * (i >> 1) + p;
+}
+
+// One thread: one packed word.
+__global__ void int4_pack_kernel(const uint8_t* __restrict__ src, uint32_t* __restrict__ dst,
+                                 int64_t words, int64_t n_out, int k, int layout) {
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (at >= words) return;
+  const int j = (int)(at & 3), lane = (int)((at >> 2) & 31);
+  const int64_t tk = at >> 7;
+  const int64_t p = tk / (k / 64);
+  const int kb = (int)(tk - p * (k / 64));
+  const int r = lane >> 2, t = lane & 3;
+  uint32_t w = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = source_row(p, nibble_row(r, i), n_out, layout);
+    if (row < 0) continue;
+    const int col = kb * 64 + nibble_col(t, j, i, 0);  // even: the pair shares a byte
+    const uint32_t byte = src[row * (k / 2) + col / 2];
+    w |= (byte & 15u) << (4 * i);
+    w |= (byte >> 4) << (4 * i + 16);
+  }
+  dst[at] = w;
+}
+
+template <typename T>
+__global__ void int4_pack_numbers_kernel(const T* __restrict__ s, const T* __restrict__ m,
+                                         T* __restrict__ dst, int64_t count, int64_t n_out, int ng,
+                                         int layout) {
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;  // (tile row, group, r)
+  if (at >= count) return;
+  const int r = (int)(at & 7);
+  const int64_t pg = at >> 3;
+  const int64_t p = pg / ng;
+  const int g = (int)(pg - p * ng);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t row = source_row(p, r + 8 * h, n_out, layout);
+    dst[at * 4 + 2 * h] = row < 0 ? Num<T>::from_f(0.f) : s[row * ng + g];
+    dst[at * 4 + 2 * h + 1] = row < 0 ? Num<T>::from_f(0.f) : m[row * ng + g];
+  }
+}
+
+// One thread: one packed word, 8 values written as 4 pairs.
+template <typename T>
+__global__ void int4_unpack_kernel(const uint32_t* __restrict__ codes, const T* __restrict__ numbers,
+                                   T* __restrict__ out, int64_t words, int64_t n_out, int k,
+                                   int group, int layout) {
+  lpc::pdl_trigger();
+  lpc::pdl_wait();
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (at >= words) return;
+  const int j = (int)(at & 3), lane = (int)((at >> 2) & 31);
+  const int64_t tk = at >> 7;
+  const int64_t p = tk / (k / 64);
+  const int kb = (int)(tk - p * (k / 64));
+  const int r = lane >> 2, t = lane & 3;
+  const uint32_t w = codes[at];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = source_row(p, nibble_row(r, i), n_out, layout);
+    if (row < 0) continue;
+    const int col = kb * 64 + nibble_col(t, j, i, 0);
+    const T* nb = numbers + ((p * (k / group) + col / group) * 8 + r) * 4 + 2 * (i & 1);
+    const float s = Num<T>::to_f(nb[0]), m = Num<T>::to_f(nb[1]);
+    __align__(4) T v[2];
+    v[0] = Num<T>::from_f(fmaf((float)((w >> (4 * i)) & 15u), s, m));
+    v[1] = Num<T>::from_f(fmaf((float)((w >> (4 * i + 16)) & 15u), s, m));
+    *reinterpret_cast<uint32_t*>(out + row * k + col) = *reinterpret_cast<const uint32_t*>(v);
+  }
+}
+
+bool use_pdl() {
+  static const bool on = [] {
+    const char* e = getenv("LPC_PDL");
+    return !(e && e[0] == '0');
+  }();
+  return on;
+}
+
+template <typename T, int GS, int MT, int NT>
+int launch(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
+           cudaStream_t s) {
+  using C = Cfg<GS, MT, NT>;
+  static std::atomic<uint64_t> mask{0};
+  int rc = lpc::once_per_device_smem((const void*)int4_linear_kernel<T, GS, MT, NT>, C::SMEM, mask);
+  if (rc) return rc;
+  const int64_t tr = tile_rows(w->n_out, w->layout);
+  const int items = (int)(w->layout == 1 ? tr / 2 : (w->n_out + 16 * MT - 1) / (16 * MT));
+  const int slots = lpc::current_device_sms() * std::max(1, (int)(227 * 1024 / (C::SMEM + 1024)));
+  const int rounds = (items + slots - 1) / slots;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((items + rounds - 1) / rounds),
+                     (unsigned)((tokens + NT * 8 - 1) / (NT * 8)));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const uint8_t* codes = (const uint8_t*)w->packed;
+  cudaLaunchKernelEx(&cfg, int4_linear_kernel<T, GS, MT, NT>, codes,
+                     codes + tr * 16 * (int64_t)(w->k / 2), (const T*)x, (const T*)resid, (T*)out,
+                     (int)tokens, w->n_out, w->k, items, epi);
+  return lpc::check_launch("int4_linear");
+}
+
+template <typename T, int GS>
+int launch_nt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
+              cudaStream_t s) {
+  if (tokens <= 8) {
+    if (w->layout == 1) return launch<T, GS, 2, 1>(w, x, out, resid, tokens, epi, s);
+    return launch<T, GS, 1, 1>(w, x, out, resid, tokens, epi, s);
+  }
+  if (tokens <= 16) return launch<T, GS, 2, 2>(w, x, out, resid, tokens, epi, s);
+  return launch<T, GS, 2, 4>(w, x, out, resid, tokens, epi, s);
+}
+
+template <typename T>
+int launch_gs(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
+              cudaStream_t s) {
+  if (w->group == 128) return launch_nt<T, 128>(w, x, out, resid, tokens, epi, s);
+  if (w->group == 64) return launch_nt<T, 64>(w, x, out, resid, tokens, epi, s);
+  return launch_nt<T, 32>(w, x, out, resid, tokens, epi, s);
+}
+
+bool shape_ok(int64_t n_out, int k, int group, int layout) {
+  return n_out > 0 && n_out <= (1 << 24) && k > 0 && k <= (1 << 20) && k % 64 == 0 &&
+         (group == 32 || group == 64 || group == 128) && k % group == 0 &&
+         (layout == 0 || layout == 1);
+}
+
+int weight_check(const lpc_w4* w, const char* what) {
+  if (!w || !w->packed || !lpc::aligned16(w->packed) ||
+      !shape_ok(w->n_out, w->k, w->group, w->layout)) {
+    lpc::set_error("%s: invalid packed weight", what);
+    return LPC_ERR_INVALID;
+  }
+  if (w->dtype != LPC_DTYPE_BF16 && w->dtype != LPC_DTYPE_F16) {
+    lpc::set_error("%s: only bf16 and fp16 are supported", what);
+    return LPC_ERR_UNSUPPORTED;
+  }
+  return LPC_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t lpc_int4_weight_bytes(int64_t n_out, int k, int group, int layout) {
+  if (!shape_ok(n_out, k, group, layout)) return 0;
+  const int64_t tr = tile_rows(n_out, layout);
+  return tr * 16 * (int64_t)(k / 2) + tr * 64 * (int64_t)(k / group);
+}
+
+extern "C" int lpc_int4_pack(const lpc_w4* w, const void* codes, const void* scales,
+                             const void* mins, void* stream) {
+  using namespace lpc;
+  int rc = weight_check(w, "int4_pack");
+  if (rc) return rc;
+  if (!codes || !scales || !mins) {
+    set_error("int4_pack: null pointer");
+    return LPC_ERR_INVALID;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int64_t tr = tile_rows(w->n_out, w->layout);
+  const int64_t words = tr * (w->k / 64) * 128;
+  const int ng = w->k / w->group;
+  const int64_t count = tr * ng * 8;
+  uint8_t* base = (uint8_t*)w->packed;
+  int4_pack_kernel<<<(unsigned)((words + 255) / 256), 256, 0, s>>>(
+      (const uint8_t*)codes, (uint32_t*)base, words, w->n_out, w->k, w->layout);
+  // 16-bit numbers are moved, not computed with: one type serves both
+  int4_pack_numbers_kernel<__half><<<(unsigned)((count + 255) / 256), 256, 0, s>>>(
+      (const __half*)scales, (const __half*)mins, (__half*)(base + tr * 16 * (int64_t)(w->k / 2)),
+      count, w->n_out, ng, w->layout);
+  if ((rc = check_launch("int4_pack"))) return rc;
+  // the products read the weight before they wait on the kernel before them
+  if (cudaStreamSynchronize(s) != cudaSuccess) {
+    set_error("int4_pack: synchronisation failed");
+    return LPC_ERR_CUDA;
+  }
+  return LPC_OK;
+}
+
+extern "C" int lpc_int4_unpack(const lpc_w4* w, void* out, void* stream) {
+  using namespace lpc;
+  int rc = weight_check(w, "int4_unpack");
+  if (rc) return rc;
+  if (!out || !aligned16(out)) {
+    set_error("int4_unpack: out must be given and 16-byte aligned");
+    return LPC_ERR_INVALID;
+  }
+  const int64_t tr = tile_rows(w->n_out, w->layout);
+  const int64_t words = tr * (w->k / 64) * 128;
+  const uint8_t* base = (const uint8_t*)w->packed;
+  const uint8_t* nb = base + tr * 16 * (int64_t)(w->k / 2);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)((words + 255) / 256);
+  if (w->dtype == LPC_DTYPE_BF16)
+    int4_unpack_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>((const uint32_t*)base,
+                                                           (const __nv_bfloat16*)nb,
+                                                           (__nv_bfloat16*)out, words, w->n_out,
+                                                           w->k, w->group, w->layout);
+  else
+    int4_unpack_kernel<__half><<<grid, 256, 0, s>>>((const uint32_t*)base, (const __half*)nb,
+                                                    (__half*)out, words, w->n_out, w->k, w->group,
+                                                    w->layout);
+  return check_launch("int4_unpack");
+}
+
+extern "C" int lpc_int4_linear(const lpc_w4* w, const void* x, void* out, const void* resid,
+                               int64_t tokens, int epilogue, void* stream) {
+  using namespace lpc;
+  int rc = weight_check(w, "int4_linear");
+  if (rc) return rc;
+  if (tokens < 0 || tokens > MAX_TOKENS) {
+    set_error("int4_linear: takes at most %d tokens, got %lld", MAX_TOKENS, (long long)tokens);
+    return LPC_ERR_INVALID;
+  }
+  if (epilogue < 0 || epilogue > 2 || (epilogue == EPI_SWIGLU) != (w->layout == 1)) {
+    set_error("int4_linear: epilogue %d does not fit a weight of layout %d", epilogue, w->layout);
+    return LPC_ERR_INVALID;
+  }
+  if (tokens == 0) return LPC_OK;
+  if (!x || !out || !aligned16(x) || (epilogue == EPI_RESIDUAL && !resid)) {
+    set_error("int4_linear: x (16-byte aligned), out and, for the residual epilogue, resid must be "
+              "given");
+    return LPC_ERR_INVALID;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return w->dtype == LPC_DTYPE_BF16
+             ? launch_gs<__nv_bfloat16>(w, x, out, resid, tokens, epilogue, s)
+             : launch_gs<__half>(w, x, out, resid, tokens, epilogue, s);
+}

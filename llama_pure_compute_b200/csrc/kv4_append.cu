@@ -1,0 +1,432 @@
+// RoPE + append into a 4-bit KV cache, and its read-back (row format: kv4.cuh).
+//
+// Append: qkv [B, S, (H + 2 Hkv) D] -> q rotated into q_out [B, H, S, D]; k
+// rotated and rounded to the data type as the 16-bit append does, v as given,
+// both held as
+//   m = min of the group,  s = T(fl(fl(max - min) / 15)),
+//   c = clamp(rint(fl(fl(x - m) * fl(1 / s))), 0, 15),
+// every operation one fp32 rounding, so that the same bytes come out of any
+// correct evaluation.  m is exact in T.  A scale below 2^-126 (whose inverse
+// fp32 does not hold) becomes 0 and its codes 0; a group with a non-finite
+// value, or with a range whose scale T does not hold, holds s = m = NaN: it
+// reads as NaN and not as some finite number.
+//
+// Bound: HBM.  A thread owns 8 rotation pairs of one (token, head): two 16-byte
+// loads, and for k and v one 8-byte store of codes; the D / 16 threads of a
+// row find min and max of its two groups in 4 * log2(D / 16) shuffles.
+#include <algorithm>
+#include <cstdlib>
+
+#include "kv4.cuh"
+
+LPC_DECLARE_STATUS(g_kv4_append_status)
+
+unsigned int lpc_status_kv4_append(bool clear) {
+  unsigned int v = 0;
+  cudaMemcpyFromSymbol(&v, g_kv4_append_status, sizeof(v));
+  if (clear && v) {
+    unsigned int z = 0;
+    cudaMemcpyToSymbol(g_kv4_append_status, &z, sizeof(z));
+  }
+  return v;
+}
+
+namespace lpc {
+
+int kv4_check(const lpc_kv4* kv, const char* what) {
+  if (!kv || !kv->key_codes || !kv->key_scales || !kv->value_codes || !kv->value_scales) {
+    set_error("%s: null cache pointer", what);
+    return LPC_ERR_INVALID;
+  }
+  if (kv->dtype != LPC_DTYPE_BF16 && kv->dtype != LPC_DTYPE_F16) {
+    set_error("%s: only bf16 and fp16 are supported", what);
+    return LPC_ERR_UNSUPPORTED;
+  }
+  if (kv->head_dim != 32 && kv->head_dim != 64 && kv->head_dim != 128) {
+    set_error("%s: head_dim must be 32, 64 or 128, got %d", what, kv->head_dim);
+    return LPC_ERR_UNSUPPORTED;
+  }
+  if (kv->kv_heads <= 0 || kv->kv_heads > 65535 || kv->max_seq_len <= 0 ||
+      kv->max_seq_len > 0x7fffffffLL ||
+      (kv->seq_base ? (!kv->seq_cap || kv->total_rows <= 0) : kv->max_batch <= 0)) {
+    set_error("%s: invalid cache sizes (kv_heads=%d max_seq_len=%lld max_batch=%lld "
+              "total_rows=%lld)", what, kv->kv_heads, (long long)kv->max_seq_len,
+              (long long)kv->max_batch, (long long)kv->total_rows);
+    return LPC_ERR_INVALID;
+  }
+  if (!aligned16(kv->key_codes) || !aligned16(kv->value_codes) ||
+      (reinterpret_cast<uintptr_t>(kv->key_scales) & 7u) ||
+      (reinterpret_cast<uintptr_t>(kv->value_scales) & 7u)) {
+    set_error("%s: codes must be 16-byte and scales 8-byte aligned", what);
+    return LPC_ERR_INVALID;
+  }
+  return LPC_OK;
+}
+
+}  // namespace lpc
+
+namespace {
+
+using lpc::Num;
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(uint4 u, float (&f)[8]) {
+  const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = Num<T>::to_f(e[i]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  uint4 u;
+  T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = Num<T>::from_f(f[i]);
+  return u;
+}
+template <typename TT>
+__device__ __forceinline__ void load8(const TT* p, float (&f)[8]) {
+  if constexpr (sizeof(TT) == 4) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
+    unpack8<TT>(__ldg(reinterpret_cast<const uint4*>(p)), f);
+  }
+}
+
+// Scale, minimum (as T) and the factor that turns x - m into a code.
+template <typename T>
+__device__ __forceinline__ void group_numbers(float lo, float hi, T& s, T& m, float& inv) {
+  s = Num<T>::from_f(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+  m = Num<T>::from_f(lo);
+  const float sf = Num<T>::to_f(s);
+  inv = 0.f;
+  if (!(sf < INFINITY)) {
+    s = m = Num<T>::from_f(__int_as_float(0x7fffffff));
+  } else if (sf < 1.17549435e-38f) {
+    s = Num<T>::from_f(0.f);
+  } else {
+    inv = __frcp_rn(sf);
+  }
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, float m, float inv) {
+  const float t = __fmul_rn(__fsub_rn(x, m), inv);
+  return (uint32_t)__float2int_rn(fminf(fmaxf(t, 0.f), 15.f));
+}
+
+constexpr int THREADS = 256;
+
+// One CTA: one token, K * (threads / chunks) of its heads; thread t owns chunk
+// t % chunks of head t / chunks + k * hpb, as in the 16-bit append.
+template <typename T, typename TT, int D, int K>
+__global__ void __launch_bounds__(THREADS) kv4_append_kernel(
+    const T* __restrict__ qkv, const int64_t* __restrict__ positions, const TT* __restrict__ cosb,
+    const TT* __restrict__ sinb, int64_t table_rows, T* __restrict__ q_out, uint8_t* kcodes,
+    uint8_t* kscales, uint8_t* vcodes, uint8_t* vscales, int64_t seq, int H, lpc::Kv4Rows rows) {
+  constexpr int C = D / 16;  // threads of a row
+  lpc::pdl_trigger();
+  lpc::pdl_wait();
+  const int Hkv = rows.kv_heads;
+  const int all = H + 2 * Hkv;
+  const int hpb = (int)blockDim.x / C;
+  const int64_t tok = blockIdx.x;
+  const int c = (int)threadIdx.x % C;
+  const int hh0 = (int)threadIdx.x / C + (int)blockIdx.y * K * hpb;
+  const int d = c * 8;
+  const T* src = qkv + tok * (int64_t)all * D + d;
+  uint4 x0[K], x1[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int hh = hh0 + k * hpb;
+    x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (hh < all) {
+      const T* p = src + (int64_t)hh * D;
+      x0[k] = __ldg(reinterpret_cast<const uint4*>(p));
+      x1[k] = __ldg(reinterpret_cast<const uint4*>(p + D / 2));
+    }
+  }
+  const int64_t pos = __ldg(positions + tok);
+  const int64_t b = tok / seq;
+  const int64_t q_row = b * H * seq + (tok - b * seq);  // q_out row of (b, head 0, s)
+  int64_t row0 = 0, head_rows = 0, cap = 0;
+  const bool inside = rows.locate(b, &row0, &head_rows, &cap);
+  if (pos < 0 || !inside || pos >= cap || pos >= table_rows) {  // the same for the whole CTA
+    if (pos >= 0 && threadIdx.x == 0) atomicOr(&g_kv4_append_status, LPC_DEV_ERR_BOUNDS);
+    // a skipped token leaves the cache as it is; its q rows become zero
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int hh = hh0 + k * hpb;
+      if (hh < H) {
+        T* dst = q_out + (q_row + (int64_t)hh * seq) * D + d;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(dst + D / 2) = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+    return;
+  }
+  float c0[8], s0[8], c1[8], s1[8];
+  if (hh0 < H + Hkv) {  // the thread's first head is its lowest; v heads are not rotated
+    const TT* cr = cosb + pos * D + d;
+    const TT* sr = sinb + pos * D + d;
+    load8<TT>(cr, c0);
+    load8<TT>(sr, s0);
+    load8<TT>(cr + D / 2, c1);
+    load8<TT>(sr + D / 2, s1);
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int hh = hh0 + k * hpb;
+    uint4 u0 = x0[k], u1 = x1[k];
+    float a0[8], a1[8];
+    unpack8<T>(u0, a0);
+    unpack8<T>(u1, a1);
+    if (hh < H + Hkv) {
+      float o0[8], o1[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        o0[i] = __fsub_rn(__fmul_rn(a0[i], c0[i]), __fmul_rn(a1[i], s0[i]));
+        o1[i] = __fadd_rn(__fmul_rn(a1[i], c1[i]), __fmul_rn(a0[i], s1[i]));
+      }
+      u0 = pack8<T>(o0);
+      u1 = pack8<T>(o1);
+      if (hh < H) {
+        T* dst = q_out + (q_row + (int64_t)hh * seq) * D + d;
+        *reinterpret_cast<uint4*>(dst) = u0;
+        *reinterpret_cast<uint4*>(dst + D / 2) = u1;
+      }
+      unpack8<T>(u0, a0);  // the values that the 16-bit cache would hold
+      unpack8<T>(u1, a1);
+    }
+    if (!__any_sync(0xffffffffu, hh >= H && hh < all)) continue;
+    float lo0 = a0[0], hi0 = a0[0], lo1 = a1[0], hi1 = a1[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      lo0 = min_nan(lo0, a0[i]);
+      hi0 = max_nan(hi0, a0[i]);
+      lo1 = min_nan(lo1, a1[i]);
+      hi1 = max_nan(hi1, a1[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < C; o <<= 1) {
+      lo0 = min_nan(lo0, __shfl_xor_sync(0xffffffffu, lo0, o));
+      hi0 = max_nan(hi0, __shfl_xor_sync(0xffffffffu, hi0, o));
+      lo1 = min_nan(lo1, __shfl_xor_sync(0xffffffffu, lo1, o));
+      hi1 = max_nan(hi1, __shfl_xor_sync(0xffffffffu, hi1, o));
+    }
+    if (hh < H || hh >= all) continue;
+    __align__(8) T sc[4];
+    float i0, i1;
+    group_numbers<T>(lo0, hi0, sc[0], sc[1], i0);
+    group_numbers<T>(lo1, hi1, sc[2], sc[3], i1);
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t byte = code_of(a0[i], lo0, i0) | code_of(a1[i], lo1, i1) << 4;
+      w[i >> 2] |= byte << (8 * (i & 3));
+    }
+    const bool key = hh < H + Hkv;
+    const int64_t row = row0 + pos + (int64_t)(hh - H - (key ? 0 : Hkv)) * head_rows;
+    uint8_t* codes = key ? kcodes : vcodes;
+    uint8_t* scales = key ? kscales : vscales;
+    *reinterpret_cast<uint2*>(codes + row * (D / 2) + d) = make_uint2(w[0], w[1]);
+    if (c == 0)
+      *reinterpret_cast<uint2*>(scales + row * 8) = *reinterpret_cast<const uint2*>(sc);
+  }
+}
+
+// K and V of (b, head, positions[b, s]) as T: thread = 8 code bytes of one row,
+// of K and of V; rows run along s, so both sides are contiguous where the
+// positions are.
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS) kv4_read_kernel(
+    const uint8_t* __restrict__ kcodes, const uint8_t* __restrict__ kscales,
+    const uint8_t* __restrict__ vcodes, const uint8_t* __restrict__ vscales,
+    const int64_t* __restrict__ positions, T* __restrict__ k_out, T* __restrict__ v_out,
+    int64_t seq, lpc::Kv4Rows rows) {
+  constexpr int C = D / 16;
+  lpc::pdl_trigger();
+  lpc::pdl_wait();
+  const int64_t s = (int64_t)blockIdx.x * (THREADS / C) + threadIdx.x / C;
+  if (s >= seq) return;
+  const int c = threadIdx.x % C;
+  const int h = blockIdx.y;
+  const int64_t b = blockIdx.z;
+  const int64_t pos = __ldg(positions + b * seq + s);
+  int64_t row0, head_rows, cap;
+  const bool inside = rows.locate(b, &row0, &head_rows, &cap);
+  const int64_t o = ((b * rows.kv_heads + h) * seq + s) * D + c * 8;
+  if (pos < 0 || !inside || pos >= cap) {
+    if (pos >= 0) atomicOr(&g_kv4_append_status, LPC_DEV_ERR_BOUNDS);
+    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+    *reinterpret_cast<uint4*>(k_out + o) = z;
+    *reinterpret_cast<uint4*>(k_out + o + D / 2) = z;
+    *reinterpret_cast<uint4*>(v_out + o) = z;
+    *reinterpret_cast<uint4*>(v_out + o + D / 2) = z;
+    return;
+  }
+  const int64_t row = row0 + (int64_t)h * head_rows + pos;
+  const uint2 cw[2] = {*reinterpret_cast<const uint2*>(kcodes + row * (D / 2) + c * 8),
+                       *reinterpret_cast<const uint2*>(vcodes + row * (D / 2) + c * 8)};
+  const uint2 sw[2] = {*reinterpret_cast<const uint2*>(kscales + row * 8),
+                       *reinterpret_cast<const uint2*>(vscales + row * 8)};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const T* sm = reinterpret_cast<const T*>(&sw[i]);
+    const float s0 = Num<T>::to_f(sm[0]), m0 = Num<T>::to_f(sm[1]);
+    const float s1 = Num<T>::to_f(sm[2]), m1 = Num<T>::to_f(sm[3]);
+    float lo[8], hi[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t byte = (j < 4 ? cw[i].x : cw[i].y) >> (8 * (j & 3));
+      lo[j] = fmaf((float)(byte & 15u), s0, m0);
+      hi[j] = fmaf((float)((byte >> 4) & 15u), s1, m1);
+    }
+    T* dst = (i ? v_out : k_out) + o;
+    *reinterpret_cast<uint4*>(dst) = pack8<T>(lo);
+    *reinterpret_cast<uint4*>(dst + D / 2) = pack8<T>(hi);
+  }
+}
+
+bool use_pdl() {
+  static const bool on = [] {
+    const char* e = getenv("LPC_PDL");
+    return !(e && e[0] == '0');
+  }();
+  return on;
+}
+
+struct Launch {
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg = {};
+  Launch(dim3 grid, int threads, cudaStream_t s) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+};
+
+template <typename T, typename TT, int D>
+int append(const lpc_kv4* kv, const void* qkv, const int64_t* pos, const void* cosb,
+           const void* sinb, int64_t table_rows, void* q_out, int64_t batch, int64_t seq, int H,
+           cudaStream_t s) {
+  constexpr int C = D / 16;
+  const int all = H + 2 * kv->kv_heads;
+  // whole warps, no more threads than the token has chunks
+  const int threads = std::min(THREADS, (all * C + 31) / 32 * 32);
+  const int hpb = threads / C;
+  const int steps = (all + hpb - 1) / hpb;
+  const int K = steps < 2 ? 1 : 2;
+  Launch l(dim3((unsigned)(batch * seq), (unsigned)((all + K * hpb - 1) / (K * hpb))), threads, s);
+  const lpc::Kv4Rows rows = lpc::kv4_rows(kv);
+#define LPC_APPEND(KK)                                                                          \
+  cudaLaunchKernelEx(&l.cfg, kv4_append_kernel<T, TT, D, KK>, (const T*)qkv, pos,               \
+                     (const TT*)cosb, (const TT*)sinb, table_rows, (T*)q_out,                   \
+                     (uint8_t*)kv->key_codes, (uint8_t*)kv->key_scales,                         \
+                     (uint8_t*)kv->value_codes, (uint8_t*)kv->value_scales, seq, H, rows)
+  if (K == 1) LPC_APPEND(1); else LPC_APPEND(2);
+#undef LPC_APPEND
+  return lpc::check_launch("rope_kv_append_int4");
+}
+
+template <typename T, int D>
+int read(const lpc_kv4* kv, const int64_t* pos, void* k_out, void* v_out, int64_t batch,
+         int64_t seq, cudaStream_t s) {
+  constexpr int RPB = THREADS / (D / 16);
+  Launch l(dim3((unsigned)((seq + RPB - 1) / RPB), (unsigned)kv->kv_heads, (unsigned)batch),
+           THREADS, s);
+  cudaLaunchKernelEx(&l.cfg, kv4_read_kernel<T, D>, (const uint8_t*)kv->key_codes,
+                     (const uint8_t*)kv->key_scales, (const uint8_t*)kv->value_codes,
+                     (const uint8_t*)kv->value_scales, pos, (T*)k_out, (T*)v_out, seq,
+                     lpc::kv4_rows(kv));
+  return lpc::check_launch("kv_read_int4");
+}
+
+}  // namespace
+
+extern "C" int lpc_rope_kv_append_int4(const lpc_kv4* kv, const void* qkv,
+                                       const int64_t* positions, const void* cos, const void* sin,
+                                       int64_t table_rows, void* q_out, int64_t batch, int64_t seq,
+                                       int num_heads, int table_dtype, void* stream) {
+  using namespace lpc;
+  int rc = kv4_check(kv, "rope_kv_append_int4");
+  if (rc) return rc;
+  if (batch < 0 || seq < 0 || num_heads <= 0 || num_heads > 65535 || table_rows <= 0 ||
+      batch > 0x7fffffffLL || seq > 0x7fffffffLL || batch * seq > 0x7fffffffLL ||
+      (!kv->seq_base && batch > kv->max_batch)) {
+    set_error("rope_kv_append_int4: invalid sizes (batch=%lld seq=%lld heads=%d max_batch=%lld)",
+              (long long)batch, (long long)seq, num_heads, (long long)kv->max_batch);
+    return LPC_ERR_INVALID;
+  }
+  if (batch == 0 || seq == 0) return LPC_OK;
+  if (!qkv || !positions || !cos || !sin || !q_out || !aligned16(qkv) || !aligned16(cos) ||
+      !aligned16(sin) || !aligned16(q_out)) {
+    set_error("rope_kv_append_int4: tensors must be given and 16-byte aligned");
+    return LPC_ERR_INVALID;
+  }
+  if (table_dtype != kv->dtype && table_dtype != LPC_DTYPE_F32) {
+    set_error("rope_kv_append_int4: table dtype must match activations or be fp32");
+    return LPC_ERR_UNSUPPORTED;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool wide = table_dtype == LPC_DTYPE_F32;
+#define LPC_A(T, DD)                                                                              \
+  return wide ? append<T, float, DD>(kv, qkv, positions, cos, sin, table_rows, q_out, batch, seq, \
+                                     num_heads, s)                                                \
+              : append<T, T, DD>(kv, qkv, positions, cos, sin, table_rows, q_out, batch, seq,     \
+                                 num_heads, s)
+  if (kv->dtype == LPC_DTYPE_BF16) {
+    if (kv->head_dim == 128) LPC_A(__nv_bfloat16, 128);
+    if (kv->head_dim == 64) LPC_A(__nv_bfloat16, 64);
+    LPC_A(__nv_bfloat16, 32);
+  }
+  if (kv->head_dim == 128) LPC_A(__half, 128);
+  if (kv->head_dim == 64) LPC_A(__half, 64);
+  LPC_A(__half, 32);
+#undef LPC_A
+}
+
+extern "C" int lpc_kv_read_int4(const lpc_kv4* kv, const int64_t* positions, void* k_out,
+                                void* v_out, int64_t batch, int64_t seq, void* stream) {
+  using namespace lpc;
+  int rc = kv4_check(kv, "kv_read_int4");
+  if (rc) return rc;
+  if (batch < 0 || batch > 65535 || seq < 0 || seq > 0x7fffffffLL ||
+      (!kv->seq_base && batch > kv->max_batch)) {
+    set_error("kv_read_int4: invalid sizes (batch=%lld seq=%lld max_batch=%lld)", (long long)batch,
+              (long long)seq, (long long)kv->max_batch);
+    return LPC_ERR_INVALID;
+  }
+  if (batch == 0 || seq == 0) return LPC_OK;
+  if (!positions || !k_out || !v_out || !aligned16(k_out) || !aligned16(v_out)) {
+    set_error("kv_read_int4: tensors must be given and 16-byte aligned");
+    return LPC_ERR_INVALID;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define LPC_R(T, DD) return read<T, DD>(kv, positions, k_out, v_out, batch, seq, s)
+  if (kv->dtype == LPC_DTYPE_BF16) {
+    if (kv->head_dim == 128) LPC_R(__nv_bfloat16, 128);
+    if (kv->head_dim == 64) LPC_R(__nv_bfloat16, 64);
+    LPC_R(__nv_bfloat16, 32);
+  }
+  if (kv->head_dim == 128) LPC_R(__half, 128);
+  if (kv->head_dim == 64) LPC_R(__half, 64);
+  LPC_R(__half, 32);
+#undef LPC_R
+}

@@ -1,0 +1,667 @@
+// Split-KV decode attention over a 4-bit KV cache (row format: kv4.cuh).
+//
+//   out[b, h] = softmax_j(scale * q . k_j) v_j,   k_j = s c_j + m (per group),
+// one query per sequence, keys j < L_b = seq_lens[b].
+//
+// Bound: HBM.  A key of one KV head is D + 16 bytes (144 at D = 128, against 512
+// in 16 bits) for 4 D G FLOPs.  On CUDA cores the unpacking and the FMAs would
+// cost about 4 instructions a value, more than the issue slots that HBM's rate
+// leaves (3.2 lane operations a value), so both products run on tensor cores
+// (mma.sync m16n8k16; 8 columns = the query heads that share the KV head, and
+// a single query token cannot fill a tcgen05 tile) and the codes enter them
+// without being converted: a 4-bit code in the low bits of an fp16 word is the
+// subnormal number c * 2^-24, exactly, so one AND makes an operand.  The codes
+// of the upper half of the dims sit 4 bits higher and count 16-fold; q (for
+// K) and the final factor (for V) undo that with powers of two.
+//   scores  S^T[key, head] = s0 * acc0 + s1 * acc1 + m0 * sum(q0) + m1 * sum(q1)
+//           with acc_g the fp32 accumulator of group g's dims;
+//   output  O^T[dim, head] of group g += codes^T (P s_g), and one number per
+//           head and group, sum_j P_j m_g[j], is added to every dim at the end.
+// q enters as fp16 scaled per head by a power of two so that its largest value
+// is about 2^14: a bf16 or fp16 q then loses nothing but what lies 2^-38 below
+// that value.  P s_g enters as fp16 (rounded to 2^-11, finer than the bf16
+// that P is usually held in); the running reference M of the softmax includes
+// the exponent of the tile's largest V scale, so that P s_g stays near 2^5 for
+// the heaviest key whatever the scales are.  Sums, maxima and statistics are fp32.
+//
+// Each warp walks its own 32-key tiles through a ring of shared-memory stages
+// filled by cp.async, with no barrier between warps until the end; the warps
+// merge through shared memory, the splits through the workspace and a second
+// kernel (none when one split covers the cache).
+#include <atomic>
+#include <cstdlib>
+
+#include "kv4.cuh"
+
+LPC_DECLARE_STATUS(g_kv4_attn_status)
+
+unsigned int lpc_status_kv4_attention(bool clear) {
+  unsigned int v = 0;
+  cudaMemcpyFromSymbol(&v, g_kv4_attn_status, sizeof(v));
+  if (clear && v) {
+    unsigned int z = 0;
+    cudaMemcpyToSymbol(g_kv4_attn_status, &z, sizeof(z));
+  }
+  return v;
+}
+
+namespace {
+
+using lpc::Num;
+
+constexpr int W = 4;          // warps
+constexpr int TK = 32;        // keys per warp tile
+constexpr int NST = 4;        // stages per warp
+constexpr int HB = 8;         // query heads per CTA (columns of the products)
+constexpr int UNIT = 128;     // shortest split: one tile per warp; workspace granularity
+constexpr float LOG2E = 1.4426950408889634f;
+// The reference M is set RISE below the heaviest key and moved when a key
+// exceeds it by LIFT: fp16 holds 2^(LIFT + 1), and a tile that stays below
+// costs one vote instead of a rescaling of the accumulators.
+constexpr float RISE = 5.f, LIFT = 13.f;
+
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
+               : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 8 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Transpose of an 8x8 matrix of 16-bit values spread over the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack_sm(uint32_t w, float& s, float& m);
+template <>
+__device__ __forceinline__ void unpack_sm<__nv_bfloat16>(uint32_t w, float& s, float& m) {
+  s = lpc::bf16lo(w);
+  m = lpc::bf16hi(w);
+}
+template <>
+__device__ __forceinline__ void unpack_sm<__half>(uint32_t w, float& s, float& m) {
+  const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w));
+  s = f.x;
+  m = f.y;
+}
+
+// Exponent of the larger of a row's two V scales as an integer key (its bits,
+// 0 for a non-finite scale, which must not move the other keys' reference).
+template <typename T>
+__device__ __forceinline__ uint32_t scale_bits(uint2 row) {
+  constexpr uint32_t INF = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+  uint32_t a = row.x & 0x7FFFu, b = row.y & 0x7FFFu;
+  a = a >= INF ? 0u : a;
+  b = b >= INF ? 0u : b;
+  return a > b ? a : b;
+}
+template <typename T>
+__device__ __forceinline__ float scale_exponent(uint32_t bits) {
+  if constexpr (std::is_same<T, __half>::value) return (float)((int)(bits >> 10) - 15);
+  // below 2^-60 the scales no longer move the reference: the sum of the P
+  // themselves, up to 2^60 times larger than P s, has to stay in fp32
+  return fmaxf((float)((int)(bits >> 7) - 127), -60.f);
+}
+
+template <int D>
+struct Layout {
+  static constexpr int CB = D / 2;                 // code bytes of a row
+  static constexpr int CODES = TK * CB;            // of a tile, K or V
+  static constexpr int SCALES = TK * 8;
+  static constexpr int STAGE = 2 * CODES + 2 * SCALES;
+  static constexpr int RED = HB * (D + 2) * 4;     // merge buffer of a warp
+  static constexpr int SMEM = W * (NST * STAGE > RED ? NST * STAGE : RED);
+};
+
+template <typename T, int D, int NH>
+__global__ void __launch_bounds__(W * 32)
+    kv4_split_kernel(const T* __restrict__ q, const uint8_t* __restrict__ kcodes,
+                     const uint8_t* __restrict__ kscales, const uint8_t* __restrict__ vcodes,
+                     const uint8_t* __restrict__ vscales, const int32_t* __restrict__ seq_lens,
+                     T* __restrict__ out, float* __restrict__ part_o, float* __restrict__ part_ml,
+                     int H, int G, int head_blocks, int max_splits, int chunk, float scale_log2,
+                     lpc::Kv4Rows rows) {
+  using L = Layout<D>;
+  constexpr int CB = L::CB;
+  constexpr int KW = D / 32;              // K words of a lane and key
+  constexpr int VM = D / 32;              // V products per group: 16 dims each
+  extern __shared__ __align__(16) uint8_t smem[];
+
+  lpc::pdl_trigger();
+  lpc::pdl_wait();
+  const int split = blockIdx.x;
+  const int kvh = blockIdx.y / head_blocks;
+  const int hb = blockIdx.y - kvh * head_blocks;
+  const int64_t b = blockIdx.z;
+  const int heads = min(HB, G - hb * HB);             // query heads of this CTA
+  const int64_t h0 = (int64_t)kvh * G + hb * HB;      // the first of them
+  int64_t row0, head_rows, cap;
+  const bool inside = rows.locate(b, &row0, &head_rows, &cap);
+  int len = __ldg(seq_lens + b);
+  if (!inside || len > cap) {
+    if (split == 0 && threadIdx.x == 0) atomicOr(&g_kv4_attn_status, LPC_DEV_ERR_BOUNDS);
+    len = inside ? (int)cap : 0;
+  }
+  const int nsplits = len > 0 ? (len + chunk - 1) / chunk : 0;
+  if (split >= nsplits) {
+    if (len <= 0 && split == 0)  // an empty context attends to nothing
+      for (int i = threadIdx.x; i < heads * D; i += blockDim.x)
+        out[(b * H + h0) * D + i] = Num<T>::from_f(0.f);
+    return;
+  }
+  const int start = split * chunk;
+  const int end = min(start + chunk, len);
+  const int ntiles = (end - start + TK - 1) / TK;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, t = lane & 3;
+
+  const int64_t head_row = row0 + kvh * head_rows;
+  const uint8_t* kc = kcodes + head_row * CB;
+  const uint8_t* vc = vcodes + head_row * CB;
+  const uint8_t* ks = kscales + head_row * 8;
+  const uint8_t* vs = vscales + head_row * 8;
+  uint8_t* ring = smem + warp * (NST * L::STAGE);
+  const uint32_t ring_u = lpc::smem_u32(ring);
+
+  // stage `st` <- tile `tile` of this CTA; rows past `end` become zeros
+  auto fetch = [&](int tile, int st) {
+    const int k0 = start + tile * TK;
+    const uint32_t dst = ring_u + st * L::STAGE;
+#pragma unroll
+    for (int c = 0; c < L::CODES / 512; ++c) {
+      const int off = (c * 32 + lane) * 16;
+      const int key = k0 + off / CB;
+      const bool ok = key < end;
+      const int64_t src = (int64_t)(ok ? key : start) * CB + off % CB;
+      cp16(dst + off, kc + src, ok);
+      cp16(dst + L::CODES + off, vc + src, ok);
+    }
+    const int key = k0 + lane;
+    const bool ok = key < end;
+    const int64_t src = (int64_t)(ok ? key : start) * 8;
+    cp8(dst + 2 * L::CODES + lane * 8, ks + src, ok);
+    cp8(dst + 2 * L::CODES + L::SCALES + lane * 8, vs + src, ok);
+  };
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i) {
+    const int tile = warp + i * W;
+    if (tile < ntiles) fetch(tile, i);
+    cp_commit();
+  }
+
+  // q as the products' column operand.  Lane (r, t) holds head r's dims of
+  // words t*KW .. t*KW + KW - 1: word w covers dims 4w..4w+3 of each group.
+  uint32_t qb[KW][2][2];
+  float qs0 = 0.f, qs1 = 0.f, amax = 0.f;
+  float qv[KW][8];
+  {
+    const T* qp = q + (b * H + h0 + (r < heads ? r : 0)) * D;
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int d = 4 * (t * KW + w) + i + g * (D / 2);
+          const float f = r < heads ? Num<T>::to_f(qp[d]) : 0.f;
+          qv[w][g * 4 + i] = f;
+          amax = fmaxf(amax, fabsf(f));
+          if (g == 0) qs0 += f; else qs1 += f;
+        }
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    qs0 += __shfl_xor_sync(0xffffffffu, qs0, o);
+    qs1 += __shfl_xor_sync(0xffffffffu, qs1, o);
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  }
+  int e = 0;
+  if (amax > 0.f && amax < INFINITY) e = 14 - ((int)(__float_as_uint(amax) >> 23) - 127);
+  e = max(-100, min(100, e));
+  const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+  for (int w = 0; w < KW; ++w)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const float f = g ? up * 0.0625f : up;
+      qb[w][g][0] = pack_half2(qv[w][g * 4 + 0] * f, qv[w][g * 4 + 2] * f);
+      qb[w][g][1] = pack_half2(qv[w][g * 4 + 1] * f, qv[w][g * 4 + 3] * f);
+    }
+  // what this lane needs of its two score columns, heads 2t and 2t + 1
+  float cs[NH], z0[NH], z1[NH], M[NH], l[NH], a0s[NH], a1s[NH];
+#pragma unroll
+  for (int n = 0; n < NH; ++n) {
+    const int from = (2 * t + n) * 4;
+    const int eh = __shfl_sync(0xffffffffu, e, from);
+    cs[n] = __uint_as_float((uint32_t)(127 + 24 - eh) << 23) * scale_log2;
+    z0[n] = __shfl_sync(0xffffffffu, qs0, from) * scale_log2;
+    z1[n] = __shfl_sync(0xffffffffu, qs1, from) * scale_log2;
+    M[n] = -INFINITY;
+    l[n] = a0s[n] = a1s[n] = 0.f;
+  }
+  float acc[2][VM][4];
+#pragma unroll
+  for (int g = 0; g < 2; ++g)
+#pragma unroll
+    for (int i = 0; i < VM; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[g][i][j] = 0.f;
+
+  constexpr uint32_t LOW = 0x000F000Fu, HIGH = 0x00F000F0u;
+  int st = 0;
+  for (int tile = warp; tile < ntiles; tile += W) {
+    {
+      const int next = tile + (NST - 1) * W;
+      int to = st + NST - 1;
+      if (to >= NST) to -= NST;
+      __syncwarp();  // every lane has read that stage's last tile
+      if (next < ntiles) fetch(next, to);
+      cp_commit();
+    }
+    cp_wait<NST - 1>();
+    __syncwarp();
+    const uint8_t* sk = ring + st * L::STAGE;
+    const uint8_t* sv = sk + L::CODES;
+    const uint8_t* sks = sk + 2 * L::CODES;
+    const uint8_t* svs = sks + L::SCALES;
+    if (++st == NST) st = 0;
+
+    // scores of keys 16u + r and 16u + r + 8
+    float x[2][2][NH];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uint32_t wa[KW], wb[KW];
+      const uint8_t* pa = sk + (16 * u + r) * CB + t * (KW * 4);
+      const uint8_t* pb = pa + 8 * CB;
+      if constexpr (KW == 4) {
+        const uint4 a = *reinterpret_cast<const uint4*>(pa), c = *reinterpret_cast<const uint4*>(pb);
+        wa[0] = a.x; wa[1] = a.y; wa[2] = a.z; wa[3] = a.w;
+        wb[0] = c.x; wb[1] = c.y; wb[2] = c.z; wb[3] = c.w;
+      } else if constexpr (KW == 2) {
+        const uint2 a = *reinterpret_cast<const uint2*>(pa), c = *reinterpret_cast<const uint2*>(pb);
+        wa[0] = a.x; wa[1] = a.y;
+        wb[0] = c.x; wb[1] = c.y;
+      } else {
+        wa[0] = *reinterpret_cast<const uint32_t*>(pa);
+        wb[0] = *reinterpret_cast<const uint32_t*>(pb);
+      }
+      float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const uint32_t a8 = wa[w] >> 8, b8 = wb[w] >> 8;
+        mma_f16(c0, wa[w] & LOW, wb[w] & LOW, a8 & LOW, b8 & LOW, qb[w][0][0], qb[w][0][1]);
+        mma_f16(c1, wa[w] & HIGH, wb[w] & HIGH, a8 & HIGH, b8 & HIGH, qb[w][1][0], qb[w][1][1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint2 w = *reinterpret_cast<const uint2*>(sks + (16 * u + r + 8 * i) * 8);
+        float s0, m0, s1, m1;
+        unpack_sm<T>(w.x, s0, m0);
+        unpack_sm<T>(w.y, s1, m1);
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+          const float sc = fmaf(s1, c1[2 * i + n], s0 * c0[2 * i + n]);
+          x[u][i][n] = fmaf(sc, cs[n], fmaf(m1, z1[n], m0 * z0[n]));
+        }
+      }
+    }
+    const int left = end - (start + tile * TK);
+    if (left < TK) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (16 * u + 8 * i + r >= left)
+#pragma unroll
+            for (int n = 0; n < NH; ++n) x[u][i][n] = -INFINITY;
+    }
+    // the reference M, moved only when a key rises far above it
+    const float ev = scale_exponent<T>(__reduce_max_sync(
+        0xffffffffu, scale_bits<T>(*reinterpret_cast<const uint2*>(svs + lane * 8))));
+    float top[NH];
+    bool rise = false;
+#pragma unroll
+    for (int n = 0; n < NH; ++n) {
+      top[n] = fmaxf(fmaxf(x[0][0][n], x[0][1][n]), fmaxf(x[1][0][n], x[1][1][n])) + ev;
+      rise |= top[n] > M[n] + LIFT;
+    }
+    if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+      for (int n = 0; n < NH; ++n) {
+        float v = top[n];
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+        const float next = fmaxf(fmaxf(M[n], v - RISE), -1e30f);
+        const float f = fast_exp2(M[n] - next);
+        M[n] = next;
+        l[n] *= f;
+        a0s[n] *= f;
+        a1s[n] *= f;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int i = 0; i < VM; ++i) {
+            acc[g][i][n] *= f;
+            acc[g][i][2 + n] *= f;
+          }
+      }
+    }
+    // weights, then the output products
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uint32_t pb[2][2];  // [group][keys 0-7 / 8-15]
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint2 w = *reinterpret_cast<const uint2*>(svs + (16 * u + r + 8 * i) * 8);
+        float s0, m0, s1, m1;
+        unpack_sm<T>(w.x, s0, m0);
+        unpack_sm<T>(w.y, s1, m1);
+        float p[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < NH; ++n) {
+          p[n] = fast_exp2(x[u][i][n] - M[n]);
+          l[n] += p[n];
+          a0s[n] = fmaf(p[n], m0, a0s[n]);
+          a1s[n] = fmaf(p[n], m1, a1s[n]);
+        }
+        pb[0][i] = transpose8(pack_half2(p[0] * s0, NH > 1 ? p[1] * s0 : 0.f));
+        pb[1][i] = transpose8(pack_half2(p[0] * s1, NH > 1 ? p[1] * s1 : 0.f));
+      }
+      // lane (r, t): keys 2t, 2t+1, 2t+8, 2t+9; for D = 128 words 2r, 2r+1
+      const uint8_t* pv = sv + (16 * u + 2 * t) * CB;
+      if constexpr (D == 32) {  // bytes 2r, 2r+1
+        const uint32_t k0 = *reinterpret_cast<const uint16_t*>(pv + 2 * r);
+        const uint32_t k1 = *reinterpret_cast<const uint16_t*>(pv + CB + 2 * r);
+        const uint32_t k2 = *reinterpret_cast<const uint16_t*>(pv + 8 * CB + 2 * r);
+        const uint32_t k3 = *reinterpret_cast<const uint16_t*>(pv + 9 * CB + 2 * r);
+        const uint32_t lo = __byte_perm(k0, k1, 0x5410), hi = __byte_perm(k2, k3, 0x5410);
+        mma_f16(acc[0][0], lo & LOW, (lo >> 8) & LOW, hi & LOW, (hi >> 8) & LOW, pb[0][0], pb[0][1]);
+        mma_f16(acc[1][0], lo & HIGH, (lo >> 8) & HIGH, hi & HIGH, (hi >> 8) & HIGH, pb[1][0],
+                pb[1][1]);
+      } else {
+        constexpr int VW = D / 64;
+        uint32_t kw[4][VW];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint8_t* p = pv + ((k & 1) + (k >> 1) * 8) * CB + r * (VW * 4);
+          if constexpr (VW == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            kw[k][0] = v.x;
+            kw[k][1] = v.y;
+          } else {
+            kw[k][0] = *reinterpret_cast<const uint32_t*>(p);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {  // bytes 0, 1 or 2, 3 of the word
+            const uint32_t sel = hf ? 0x7632 : 0x5410;
+            const uint32_t lo = __byte_perm(kw[0][w], kw[1][w], sel);
+            const uint32_t hi = __byte_perm(kw[2][w], kw[3][w], sel);
+            const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+            mma_f16(acc[0][2 * w + hf], lo & LOW, lo8 & LOW, hi & LOW, hi8 & LOW, pb[0][0], pb[0][1]);
+            mma_f16(acc[1][2 * w + hf], lo & HIGH, lo8 & HIGH, hi & HIGH, hi8 & HIGH, pb[1][0],
+                    pb[1][1]);
+          }
+      }
+    }
+  }
+  cp_wait<0>();
+  // a head's sums over the 8 lanes that hold its keys
+#pragma unroll
+  for (int n = 0; n < NH; ++n)
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      l[n] += __shfl_xor_sync(0xffffffffu, l[n], o);
+      a0s[n] += __shfl_xor_sync(0xffffffffu, a0s[n], o);
+      a1s[n] += __shfl_xor_sync(0xffffffffu, a1s[n], o);
+    }
+  __syncthreads();  // the rings become the merge buffer: [W][HB][D + 2]
+  float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int n = 0; n < NH; ++n) {
+    const int h = 2 * t + n;
+    if (h >= heads) continue;
+    float* p = red + (warp * HB + h) * (D + 2);
+#pragma unroll
+    for (int i = 0; i < VM; ++i) {
+      // row r of product i is dim 4 * word + 2 * half of its group, row r + 8 the next one
+      const int d = D == 32 ? 2 * r : 4 * (r * (D / 64) + (i >> 1)) + 2 * (i & 1);
+      p[d] = fmaf(acc[0][i][n], 16777216.f, a0s[n]);
+      p[d + 1] = fmaf(acc[0][i][2 + n], 16777216.f, a0s[n]);
+      p[d + D / 2] = fmaf(acc[1][i][n], 1048576.f, a1s[n]);
+      p[d + D / 2 + 1] = fmaf(acc[1][i][2 + n], 1048576.f, a1s[n]);
+    }
+    if (r == 0) {
+      p[D] = M[n];
+      p[D + 1] = l[n];
+    }
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < heads * D; idx += W * 32) {
+    const int h = idx / D, d = idx - h * D;
+    float Mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) Mx = fmaxf(Mx, red[(w * HB + h) * (D + 2) + D]);
+    const float Mu = Mx == -INFINITY ? 0.f : Mx;
+    float O = 0.f, Ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float* p = red + (w * HB + h) * (D + 2);
+      const float f = fast_exp2(p[D] - Mu);
+      O = fmaf(f, p[d], O);
+      Ls = fmaf(f, p[D + 1], Ls);
+    }
+    const int64_t bh = b * H + h0 + h;
+    if (nsplits == 1) {
+      out[bh * D + d] = Num<T>::from_f(Ls == 0.f ? 0.f : O / Ls);
+    } else {
+      const int64_t pi = bh * max_splits + split;
+      part_o[pi * D + d] = O;
+      if (d == 0) {
+        part_ml[2 * pi] = Mx;
+        part_ml[2 * pi + 1] = Ls;
+      }
+    }
+  }
+}
+
+// One warp per (sequence, head): the splits' partials, in split order.
+constexpr int CWARPS = 4;
+template <typename T, int D>
+__global__ void __launch_bounds__(CWARPS * 32)
+    kv4_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
+                       const int32_t* __restrict__ seq_lens, T* __restrict__ out, int H,
+                       int max_splits, int chunk, lpc::Kv4Rows rows, int64_t bh_total) {
+  lpc::pdl_trigger();
+  lpc::pdl_wait();
+  constexpr int DPL = D / 32;
+  const int64_t bh = (int64_t)blockIdx.x * CWARPS + (threadIdx.x >> 5);
+  if (bh >= bh_total) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t b = bh / H;
+  int64_t row0, head_rows, cap;
+  const bool inside = rows.locate(b, &row0, &head_rows, &cap);
+  int len = __ldg(seq_lens + b);
+  if (len > cap) len = (int)cap;
+  const int ns = inside && len > 0 ? (len + chunk - 1) / chunk : 0;
+  if (ns <= 1) return;  // written by the split kernel
+  const float* ml = part_ml + bh * max_splits * 2;
+  const float* po = part_o + bh * max_splits * D + lane * DPL;
+  float mx = -INFINITY;
+  for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml[2 * s]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float Mu = mx == -INFINITY ? 0.f : mx;
+  float O[DPL], Ls = 0.f;
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) O[i] = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < ns; ++s) {
+    const float f = fast_exp2(ml[2 * s] - Mu);
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) O[i] = fmaf(f, po[(int64_t)s * D + i], O[i]);
+    Ls = fmaf(f, ml[2 * s + 1], Ls);
+  }
+  T* o = out + bh * D + lane * DPL;
+#pragma unroll
+  for (int i = 0; i < DPL; ++i) o[i] = Num<T>::from_f(Ls == 0.f ? 0.f : O[i] / Ls);
+}
+
+bool use_pdl() {
+  static const bool on = [] {
+    const char* e = getenv("LPC_PDL");
+    return !(e && e[0] == '0');
+  }();
+  return on;
+}
+
+template <typename T, int D, int NH>
+int launch(const lpc_kv4* kv, const void* q, const int32_t* lens, void* out, float* po, float* pml,
+           int64_t batch, int heads, int max_splits, int chunk, float scale_log2, cudaStream_t s) {
+  using L = Layout<D>;
+  static std::atomic<uint64_t> mask{0};
+  int rc = lpc::once_per_device_smem((const void*)kv4_split_kernel<T, D, NH>, L::SMEM, mask);
+  if (rc) return rc;
+  const int G = heads / kv->kv_heads;
+  const int blocks = (G + HB - 1) / HB;
+  const int grid_splits = (int)((kv->max_seq_len + chunk - 1) / chunk);
+  const lpc::Kv4Rows rows = lpc::kv4_rows(kv);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid_splits, (unsigned)(kv->kv_heads * blocks), (unsigned)batch);
+  cfg.blockDim = dim3(W * 32);
+  cfg.dynamicSmemBytes = L::SMEM;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kv4_split_kernel<T, D, NH>, (const T*)q,
+                         (const uint8_t*)kv->key_codes, (const uint8_t*)kv->key_scales,
+                         (const uint8_t*)kv->value_codes, (const uint8_t*)kv->value_scales, lens,
+                         (T*)out, po, pml, heads, G, blocks, max_splits, chunk, scale_log2,
+                         rows) != cudaSuccess)
+    return lpc::check_launch("decode_attention_int4 (split)");
+  if ((rc = lpc::check_launch("decode_attention_int4 (split)"))) return rc;
+  if (grid_splits == 1) return LPC_OK;
+  const int64_t bh_total = batch * heads;
+  cfg.gridDim = dim3((unsigned)((bh_total + CWARPS - 1) / CWARPS));
+  cfg.blockDim = dim3(CWARPS * 32);
+  cfg.dynamicSmemBytes = 0;
+  if (cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D>, (const float*)po, (const float*)pml, lens,
+                         (T*)out, heads, max_splits, chunk, rows, bh_total) != cudaSuccess)
+    return lpc::check_launch("decode_attention_int4 (combine)");
+  return lpc::check_launch("decode_attention_int4 (combine)");
+}
+
+constexpr int64_t MAX_BATCH = 65535;
+constexpr int64_t MAX_SEQ = 65535LL * UNIT;
+constexpr int MAX_HEADS = 65535;
+
+// Split length: the longest of the candidates that still gives the launch
+// enough CTAs to fill the GPU several times over (592 run at once).
+int split_keys(const lpc_kv4* kv, int64_t batch, int heads) {
+  const int64_t G = heads / kv->kv_heads, blocks = (G + HB - 1) / HB;
+  const int64_t pairs = batch * kv->kv_heads * blocks;
+  for (int c : {1024, 512, 256})
+    if (pairs * (kv->max_seq_len / c) >= 2048) return c;
+  return UNIT;
+}
+
+bool sizes_ok(const lpc_kv4* kv, int64_t batch, int heads) {
+  return batch >= 0 && batch <= MAX_BATCH && heads > 0 && heads <= MAX_HEADS &&
+         heads % kv->kv_heads == 0 && kv->max_seq_len <= MAX_SEQ;
+}
+
+}  // namespace
+
+extern "C" int64_t lpc_decode_attention_int4_workspace_bytes(const lpc_kv4* kv, int64_t batch,
+                                                             int heads) {
+  if (lpc::kv4_check(kv, "decode_attention_int4") || !sizes_ok(kv, batch, heads)) return 0;
+  const int64_t splits = (kv->max_seq_len + UNIT - 1) / UNIT;
+  return batch * heads * splits * (int64_t)(kv->head_dim + 2) * 4;
+}
+
+extern "C" int lpc_decode_attention_int4(const lpc_kv4* kv, const void* q, const int32_t* seq_lens,
+                                         void* out, void* workspace, int64_t workspace_bytes,
+                                         int64_t batch, int heads, float sm_scale, void* stream) {
+  using namespace lpc;
+  int rc = kv4_check(kv, "decode_attention_int4");
+  if (rc) return rc;
+  if (!sizes_ok(kv, batch, heads) || (!kv->seq_base && batch > kv->max_batch)) {
+    set_error("decode_attention_int4: invalid sizes (batch=%lld heads=%d kv_heads=%d "
+              "max_batch=%lld max_seq_len=%lld)", (long long)batch, heads, kv->kv_heads,
+              (long long)kv->max_batch, (long long)kv->max_seq_len);
+    return LPC_ERR_INVALID;
+  }
+  if (batch == 0) return LPC_OK;
+  if (!q || !seq_lens || !out || !aligned16(q) || !aligned16(out)) {
+    set_error("decode_attention_int4: q, seq_lens and out must be given, q and out 16-byte aligned");
+    return LPC_ERR_INVALID;
+  }
+  const int chunk = split_keys(kv, batch, heads);
+  const int64_t splits = (kv->max_seq_len + chunk - 1) / chunk;
+  const int64_t need = splits > 1 ? batch * heads * splits * (int64_t)(kv->head_dim + 2) * 4 : 0;
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
+    set_error("decode_attention_int4: workspace of %lld bytes required, got %lld", (long long)need,
+              (long long)workspace_bytes);
+    return LPC_ERR_INVALID;
+  }
+  if ((int64_t)kv->kv_heads * ((heads / kv->kv_heads + HB - 1) / HB) > 65535) {
+    set_error("decode_attention_int4: too many heads");
+    return LPC_ERR_UNSUPPORTED;
+  }
+  float* po = static_cast<float*>(workspace);
+  float* pml = po ? po + batch * heads * splits * kv->head_dim : nullptr;
+  const float sl2 = sm_scale * LOG2E;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool one = heads == kv->kv_heads;
+#define LPC_KV4(T, DD)                                                                            \
+  return one ? launch<T, DD, 1>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits, chunk,  \
+                                sl2, s)                                                           \
+             : launch<T, DD, 2>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits, chunk,  \
+                                sl2, s)
+  if (kv->dtype == LPC_DTYPE_BF16) {
+    if (kv->head_dim == 128) LPC_KV4(__nv_bfloat16, 128);
+    if (kv->head_dim == 64) LPC_KV4(__nv_bfloat16, 64);
+    LPC_KV4(__nv_bfloat16, 32);
+  }
+  if (kv->head_dim == 128) LPC_KV4(__half, 128);
+  if (kv->head_dim == 64) LPC_KV4(__half, 64);
+  LPC_KV4(__half, 32);
+#undef LPC_KV4
+}

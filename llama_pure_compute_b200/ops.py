@@ -13,9 +13,13 @@ arguments raise ValueError.
 
 Extra ops used by the model's fused attention block (not in the reference's
 ops module): ``rmsnorm_forward``, ``rope_kv_append`` and ``decode_attention``.
+
+4-bit KV cache: ``Int4KV`` (the cache's tensors), ``rope_kv_append_int4``,
+``decode_attention_int4`` and ``kv_read_int4``.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -33,6 +37,11 @@ __all__ = [
     "rope_kv_append_ragged",
     "qkv_rope_append",
     "decode_attention_ragged",
+    "Int4KV",
+    "rope_kv_append_int4",
+    "decode_attention_int4",
+    "decode_attention_int4_workspace",
+    "kv_read_int4",
 ]
 
 
@@ -554,4 +563,291 @@ def decode_attention_ragged(
     _lib.check(rc, "decode_attention_ragged")
     _lib.count_launch("lpc_decode_attention_ragged",
                       _lib.decode_kernels(B, Hkv, max_seq_len, total_rows))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# 4-bit KV cache
+# ---------------------------------------------------------------------------
+class Int4KV:
+    """The tensors of a 4-bit KV cache, checked once and handed to the ops below.
+
+    A row (one position of one KV head, D = 32, 64 or 128 dims) is D/2 code
+    bytes -- byte j holds dim j in its low and dim j + D/2 in its high four
+    bits -- and four numbers of the data type, ``(s0, m0, s1, m1)``: a code c
+    of the lower half of the dims stands for ``s0 * c + m0``, one of the upper
+    half for ``s1 * c + m1``.  At D = 128 a row takes 72 bytes, 256 in 16 bits.
+
+    dense:  codes uint8 ``[max_batch, kv_heads, max_seq_len, D/2]``, scales
+            (bf16 or fp16) ``[max_batch, kv_heads, max_seq_len, 4]``;
+    ragged: ``[kv_heads, total_rows, D/2]`` and ``[kv_heads, total_rows, 4]`` with
+            ``seq_base`` int64 and ``seq_cap`` int32 (device, one entry per
+            sequence of the batch) and ``max_seq_len``, which bounds every
+            ``seq_cap``.
+    """
+
+    __slots__ = ("key_codes", "key_scales", "value_codes", "value_scales", "seq_base", "seq_cap",
+                 "max_seq_len", "kv_heads", "head_dim", "dtype", "device", "max_batch", "_c", "ref")
+
+    def __init__(self, key_codes: torch.Tensor, key_scales: torch.Tensor,
+                 value_codes: torch.Tensor, value_scales: torch.Tensor,
+                 seq_base: Optional[torch.Tensor] = None, seq_cap: Optional[torch.Tensor] = None,
+                 max_seq_len: Optional[int] = None):
+        named = ((key_codes, "key_codes"), (key_scales, "key_scales"),
+                 (value_codes, "value_codes"), (value_scales, "value_scales"))
+        for t, n in named:
+            _require_cuda(t, n)
+            if not t.is_contiguous():
+                raise ValueError(f"LlamaPureComputeError: {n} must be memory-contiguous.")
+            if t.device != key_codes.device:
+                raise ValueError("LlamaPureComputeError: the cache's tensors must share a device.")
+        if key_codes.dtype != torch.uint8 or value_codes.dtype != torch.uint8:
+            raise TypeError("LlamaPureComputeError: codes must be uint8.")
+        self.dtype = key_scales.dtype
+        if self.dtype not in (torch.bfloat16, torch.float16) or value_scales.dtype != self.dtype:
+            raise TypeError("LlamaPureComputeError: scales must be bf16 or fp16, keys' and values' alike.")
+        ragged = seq_base is not None or seq_cap is not None
+        lead = tuple(key_codes.shape[:-1])
+        if key_codes.dim() != (3 if ragged else 4) or value_codes.shape != key_codes.shape \
+                or tuple(key_scales.shape) != (*lead, 4) or value_scales.shape != key_scales.shape:
+            raise ValueError("LlamaPureComputeError: codes must be matching [B, H, S, D/2] (dense) or "
+                             "[H, rows, D/2] (ragged) tensors and scales [..., 4].")
+        self.head_dim = 2 * key_codes.shape[-1]
+        if self.head_dim not in (32, 64, 128):
+            raise ValueError("LlamaPureComputeError: Supported head dimensions: 32, 64, 128.")
+        if key_codes.numel() == 0:
+            raise ValueError("LlamaPureComputeError: the cache is empty.")
+        if ragged:
+            if seq_base is None or seq_cap is None or max_seq_len is None:
+                raise ValueError("LlamaPureComputeError: a ragged cache needs seq_base, seq_cap and "
+                                 "max_seq_len.")
+            _check_ragged_index(seq_base, seq_cap, 0)
+            if seq_base.numel() != seq_cap.numel() or seq_base.device != key_codes.device \
+                    or seq_cap.device != key_codes.device:
+                raise ValueError("LlamaPureComputeError: seq_base and seq_cap must have the same "
+                                 "entries, on the cache's device.")
+            self.kv_heads, total_rows = lead
+            self.max_batch = seq_base.numel()
+            self.max_seq_len = int(max_seq_len)
+            if self.max_seq_len <= 0:
+                raise ValueError("LlamaPureComputeError: max_seq_len must be positive.")
+        else:
+            self.max_batch, self.kv_heads, self.max_seq_len = lead
+            total_rows = 0
+            if max_seq_len is not None and int(max_seq_len) != self.max_seq_len:
+                raise ValueError("LlamaPureComputeError: a dense cache's max_seq_len is its shape's.")
+        self.key_codes, self.key_scales = key_codes, key_scales
+        self.value_codes, self.value_scales = value_codes, value_scales
+        self.seq_base, self.seq_cap = seq_base, seq_cap
+        self.device = key_codes.device
+        self._c = _lib.Kv4(key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(),
+                           value_scales.data_ptr(), _lib.ptr(seq_base), _lib.ptr(seq_cap),
+                           self.max_batch, self.max_seq_len, total_rows, self.kv_heads,
+                           self.head_dim, _lib.DTYPE_CODE[self.dtype], 0)
+        self.ref = ctypes.addressof(self._c)
+
+    @classmethod
+    def empty(cls, max_batch: int, kv_heads: int, max_seq_len: int, head_dim: int,
+              dtype: torch.dtype = torch.bfloat16, device="cuda") -> "Int4KV":
+        """A new dense cache (its rows hold nothing until they are appended)."""
+        lead = (max_batch, kv_heads, max_seq_len)
+        return cls(*cls._allocate(lead, head_dim, dtype, device))
+
+    @classmethod
+    def empty_ragged(cls, kv_heads: int, total_rows: int, head_dim: int, seq_base: torch.Tensor,
+                     seq_cap: torch.Tensor, max_seq_len: int, dtype: torch.dtype = torch.bfloat16,
+                     device="cuda") -> "Int4KV":
+        """A new ragged cache of ``total_rows`` rows per head."""
+        return cls(*cls._allocate((kv_heads, total_rows), head_dim, dtype, device), seq_base,
+                   seq_cap, max_seq_len)
+
+    @staticmethod
+    def _allocate(lead, head_dim, dtype, device):
+        got = []
+        for _ in range(2):
+            got.append(torch.empty((*lead, head_dim // 2), dtype=torch.uint8, device=device))
+            got.append(torch.empty((*lead, 4), dtype=dtype, device=device))
+        return got
+
+    @property
+    def ragged(self) -> bool:
+        return self.seq_base is not None
+
+    def memory_footprint_bytes(self) -> int:
+        return 2 * (self.key_codes.numel() + 2 * self.key_scales.numel())
+
+    def rows(self, start: int, count: int) -> "Int4KV":
+        """Sequences ``[start, start + count)`` of a dense cache, in place."""
+        if self.ragged or start < 0 or count <= 0 or start + count > self.max_batch:
+            raise ValueError("LlamaPureComputeError: rows outside the dense cache.")
+        part = slice(start, start + count)
+        return Int4KV(self.key_codes[part], self.key_scales[part], self.value_codes[part],
+                      self.value_scales[part])
+
+    def select(self, seq_base: torch.Tensor, seq_cap: torch.Tensor) -> "Int4KV":
+        """The same ragged cache with other sequences in the batch."""
+        if not self.ragged:
+            raise ValueError("LlamaPureComputeError: select needs a ragged cache.")
+        return Int4KV(self.key_codes, self.key_scales, self.value_codes, self.value_scales,
+                      seq_base, seq_cap, self.max_seq_len)
+
+
+def _on_device(device: torch.device, name: str, *args) -> int:
+    """Calls a C entry point, its stream argument appended, with the tensors'
+    device current."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == device.index:
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _int4_out(out: Optional[torch.Tensor], name: str, shape, kv: Int4KV) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=kv.dtype, device=kv.device)
+    if out.shape != torch.Size(shape) or out.dtype != kv.dtype or out.device != kv.device \
+            or not out.is_contiguous():
+        raise ValueError(f"LlamaPureComputeError: {name} must be a contiguous {tuple(shape)} tensor "
+                         "of the cache's dtype and device.")
+    return out
+
+
+def _int4_positions(positions: torch.Tensor, B: int, S: int, kv: Int4KV) -> torch.Tensor:
+    if tuple(positions.shape) != (B, S):
+        raise ValueError("LlamaPureComputeError: positions must be [batch, seq].")
+    if positions.device != kv.device:
+        raise ValueError("LlamaPureComputeError: positions must be on the cache's device.")
+    if positions.dtype.is_floating_point or positions.dtype == torch.bool:
+        raise TypeError("LlamaPureComputeError: positions must be integers.")
+    if B > kv.max_batch:
+        raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
+    return positions.to(torch.int64).contiguous()
+
+
+def rope_kv_append_int4(
+    qkv: torch.Tensor,
+    positions: torch.Tensor,
+    cos_table: torch.Tensor,
+    sin_table: torch.Tensor,
+    kv: Int4KV,
+    num_heads: int,
+    q_out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``rope_kv_append`` / ``rope_kv_append_ragged`` into a 4-bit cache: rotate
+    q/k of ``qkv`` [B, S, (H+2Hkv)*D] at ``positions`` [B, S], quantise the
+    rotated k and v into the cache rows of those positions, return q as
+    [B, H, S, D].
+
+    Each half of a row's dims is held with its own minimum m and scale
+    ``s = (max - m) / 15`` (rounded to the data type), codes rounded to nearest.
+    A half with a non-finite value, or whose scale overflows the type, reads as
+    NaN.  A negative position skips its token (its q is zero); a position
+    outside the sequence's rows or the tables skips it and sets the device
+    status.  The positions of one sequence must differ."""
+    for t, n in ((qkv, "qkv"), (positions, "positions"), (cos_table, "cos"), (sin_table, "sin")):
+        _require_cuda(t, n)
+    D = kv.head_dim
+    if qkv.dim() != 3 or qkv.shape[-1] != (num_heads + 2 * kv.kv_heads) * D or num_heads <= 0:
+        raise ValueError("LlamaPureComputeError: qkv width does not match heads * head_dim.")
+    B, S, _ = qkv.shape
+    if qkv.dtype != kv.dtype:
+        raise TypeError("LlamaPureComputeError: qkv and cache dtypes differ.")
+    if qkv.device != kv.device or cos_table.device != kv.device or sin_table.device != kv.device:
+        raise ValueError("LlamaPureComputeError: qkv and the rope tables must be on the cache's device.")
+    if cos_table.dim() != 2 or cos_table.shape[-1] != D or sin_table.shape != cos_table.shape \
+            or sin_table.dtype != cos_table.dtype:
+        raise ValueError("LlamaPureComputeError: rope tables must be matching [max_pos, head_dim].")
+    pos = _int4_positions(positions, B, S, kv)
+    qkv = qkv.contiguous()
+    cos_table, sin_table = cos_table.contiguous(), sin_table.contiguous()
+    q_out = _int4_out(q_out, "q_out", (B, num_heads, S, D), kv)
+    rc = _on_device(kv.device, "lpc_rope_kv_append_int4", kv.ref, qkv.data_ptr(), pos.data_ptr(),
+                    cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0],
+                    q_out.data_ptr(), B, S, num_heads,
+                    _lib.dtype_code(cos_table.dtype, "rope_kv_append_int4"))
+    _lib.check(rc, "rope_kv_append_int4")
+    if B and S:
+        _lib.count_launch("lpc_rope_kv_append_int4")
+    return q_out
+
+
+def kv_read_int4(
+    kv: Int4KV,
+    positions: torch.Tensor,
+    k_out: Optional[torch.Tensor] = None,
+    v_out: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values that a 4-bit cache holds at ``positions`` [B, S], as
+    two [B, Hkv, S, D] tensors of the data type (``s * c + m``, rounded once):
+    what ``flash_attention_v2`` needs of the context before a prompt chunk.
+    Rows of negative positions are zero; so are those of positions outside the
+    sequence's rows, which set the device status as well."""
+    _require_cuda(positions, "positions")
+    if positions.dim() != 2:
+        raise ValueError("LlamaPureComputeError: positions must be [batch, seq].")
+    B, S = positions.shape
+    pos = _int4_positions(positions, B, S, kv)
+    shape = (B, kv.kv_heads, S, kv.head_dim)
+    k_out = _int4_out(k_out, "k_out", shape, kv)
+    v_out = _int4_out(v_out, "v_out", shape, kv)
+    rc = _on_device(kv.device, "lpc_kv_read_int4", kv.ref, pos.data_ptr(), k_out.data_ptr(),
+                    v_out.data_ptr(), B, S)
+    _lib.check(rc, "kv_read_int4")
+    if B and S:
+        _lib.count_launch("lpc_kv_read_int4")
+    return k_out, v_out
+
+
+def decode_attention_int4_workspace(kv: Int4KV, batch: int, heads: int) -> torch.Tensor:
+    """Workspace for ``decode_attention_int4`` calls of these sizes.  Calls that
+    may overlap (other streams, other graphs) need one each."""
+    n = _lib.load().lpc_decode_attention_int4_workspace_bytes(kv.ref, batch, heads)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=kv.device)
+
+
+def decode_attention_int4(
+    q: torch.Tensor,
+    kv: Int4KV,
+    seq_lens: torch.Tensor,
+    sm_scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``decode_attention`` / ``decode_attention_ragged`` over a 4-bit cache:
+    one query per sequence, q [B, H, D] (or [B, H, 1, D]), keys
+    ``[0, seq_lens[b])`` of sequence b (int32, device).  Any number of query
+    heads per KV head.  An empty sequence gives zeros; a length beyond the
+    sequence's rows is cut to them and sets the device status.  fp32 softmax
+    and accumulation; returns q's shape."""
+    _require_cuda(q, "q")
+    _require_cuda(seq_lens, "seq_lens")
+    if seq_lens.dtype != torch.int32:
+        raise TypeError("LlamaPureComputeError: seq_lens must be int32.")
+    if q.dtype != kv.dtype:
+        raise TypeError("LlamaPureComputeError: q and cache dtypes differ.")
+    D = kv.head_dim
+    if q.dim() not in (3, 4) or q.shape[-1] != D or (q.dim() == 4 and q.shape[2] != 1):
+        raise ValueError("LlamaPureComputeError: q must be [B, H, D] with the cache's head_dim.")
+    B, H = q.shape[0], q.shape[1]
+    if H == 0 or H % kv.kv_heads:
+        raise ValueError("LlamaPureComputeError: heads must be a multiple of the cache's KV heads.")
+    if B > kv.max_batch:
+        raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
+    if seq_lens.numel() < B or not seq_lens.is_contiguous():
+        raise ValueError("LlamaPureComputeError: seq_lens must have a contiguous entry per sequence.")
+    if q.device != kv.device or seq_lens.device != kv.device:
+        raise ValueError("LlamaPureComputeError: q and seq_lens must be on the cache's device.")
+    qc = q.contiguous()
+    out = _int4_out(out, "out", q.shape, kv)
+    if workspace is None:
+        workspace = decode_attention_int4_workspace(kv, B, H)
+    elif workspace.device != kv.device or not workspace.is_contiguous():
+        raise ValueError("LlamaPureComputeError: workspace must be contiguous on the cache's device.")
+    rc = _on_device(kv.device, "lpc_decode_attention_int4", kv.ref, qc.data_ptr(),
+                    seq_lens.data_ptr(), out.data_ptr(), workspace.data_ptr(),
+                    workspace.numel() * workspace.element_size(), B, H,
+                    D ** -0.5 if sm_scale is None else float(sm_scale))
+    _lib.check(rc, "decode_attention_int4")
+    if B:
+        _lib.count_launch("lpc_decode_attention_int4")
     return out
