@@ -36,8 +36,6 @@ namespace {
 
 using lpc::Num;
 
-constexpr int WARPS = 8;
-constexpr int THREADS = WARPS * 32;
 constexpr int MAX_TOKENS = 64;
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -68,9 +66,17 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 }
 
 // The 8 codes of a word as the A operand: rows r, r + 8 of columns 2t.., then
-// the same rows of columns 2t + 8...
+// the same rows of columns 2t + 8...  The bf16 shifts are products by a power
+// of two that the compiler does not see (`sh` = 2^28): LOP3 and SHF share the
+// half-rate ALU pipe, which 7 of them a word would fill, the products run on
+// the FMA pipe beside it.
+__device__ __forceinline__ uint32_t shift4(uint32_t w, uint32_t sh) {
+  uint64_t p;
+  asm("mul.wide.u32 %0, %1, %2;" : "=l"(p) : "r"(w), "r"(sh));
+  return (uint32_t)(p >> 32);
+}
 template <typename T>
-__device__ __forceinline__ void operand(uint32_t w, uint32_t (&a)[4]) {
+__device__ __forceinline__ void operand(uint32_t w, uint32_t sh, uint32_t (&a)[4]) {
   if constexpr (std::is_same<T, __half>::value) {
     const uint32_t v = w >> 8;
     a[0] = w & 0x000F000Fu;
@@ -79,7 +85,10 @@ __device__ __forceinline__ void operand(uint32_t w, uint32_t (&a)[4]) {
     a[3] = v & 0x00F000F0u;
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+    for (int i = 0; i < 4; ++i) {
+      a[i] = (w & 0x000F000Fu) | 0x43004300u;
+      if (i < 3) w = shift4(w, sh);
+    }
   }
 }
 
@@ -91,84 +100,96 @@ __device__ __forceinline__ float2 pair_f(uint32_t w) {
     return make_float2(lpc::bf16lo(w), lpc::bf16hi(w));
 }
 
-template <int GS, int MT, int NT>
+template <int GS, int MT, int NT, int NW>
 struct Cfg {
   static constexpr int CK = GS > 64 ? GS : 64;  // columns of a pipeline stage
   static constexpr int TILES = CK / 64;
   static constexpr int SG = CK / GS;            // groups of a stage
   static constexpr int STAGE = MT * (TILES * 512 + SG * 256);
-  static constexpr int NST = (MT * TILES == 4) ? 4 : (MT * TILES == 2) ? 8 : 12;
+  static constexpr int NST = (MT * TILES == 4 ? 4 : MT * TILES == 2 ? 8 : 12) * 8 / NW + (NW > 8);
   static constexpr int RING = NST * STAGE;
   static constexpr int RED = MT * 16 * NT * 8;  // fp32 partial sums of a warp
-  static constexpr int SMEM = WARPS * (RING + 2 * RED * 4);
+  static constexpr int SMEM = NW * (RING + 2 * RED * 4);
+  // bytes for the sums of x, beside the above
+  static constexpr int XS_MAX = 232448 - SMEM < 24576 ? 232448 - SMEM : 24576;
+  static_assert(XS_MAX >= 0, "shared memory");
 };
 
 enum { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_SWIGLU = 2 };
 
-template <typename T, int GS, int MT, int NT>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, int GS, int MT, int NT, int NW>
+__global__ void __launch_bounds__(NW * 32)
     int4_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ numbers,
                        const T* __restrict__ x, const T* resid, T* out, int tokens, int64_t n_out,
-                       int k, int items, int epi) {
-  using C = Cfg<GS, MT, NT>;
+                       int k, int items, int epi, int keep_sums, uint32_t sh) {
+  using C = Cfg<GS, MT, NT, NW>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
   const int nchunks = k / C::CK;
-  const int kb = k / 64, ng = k / GS;
-  const int c0 = warp * nchunks / WARPS, nc = (warp + 1) * nchunks / WARPS - c0;
+  const int64_t tile_codes = (int64_t)(k / 64) * 512, tile_numbers = (int64_t)(k / GS) * 64;
+  const int c0 = warp * nchunks / NW, nc = (warp + 1) * nchunks / NW - c0;
   const int tok0 = blockIdx.y * (NT * 8);
   const int ntok = min(NT * 8, tokens - tok0);
   uint8_t* ring = smem + warp * C::RING;
   const uint32_t ring_u = lpc::smem_u32(ring);
-  float* red = reinterpret_cast<float*>(smem + WARPS * C::RING);
+  float* red = reinterpret_cast<float*>(smem + NW * C::RING);
+  // sums of x of this warp's groups, [group][token]
+  float* xs = reinterpret_cast<float*>(smem + C::SMEM) +
+              warp * ((nchunks + NW - 1) / NW) * C::SG * NT * 8;
 
-  auto fetch = [&](int item, int chunk, int st) {
-    const uint32_t dst = ring_u + st * C::STAGE;
+  // the weight stream: this warp's chunks of item blockIdx.x, then of the next
+  const uint8_t* fcode = codes + (int64_t)blockIdx.x * MT * tile_codes + c0 * (C::TILES * 512) + lane * 16;
+  const uint8_t* fnum = numbers + (int64_t)blockIdx.x * MT * tile_numbers + c0 * (C::SG * 64) + r * 8;
+  const int64_t jump_code = gridDim.x * MT * tile_codes - nc * (C::TILES * 512);
+  const int64_t jump_num = gridDim.x * MT * tile_numbers - nc * (C::SG * 64);
+  int fleft = nc > 0 ? nc * ((items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) : 0;
+  int fc = nc;
+  uint32_t fdst = ring_u;
+  auto advance = [&]() {
+    if (fleft > 0) {
+      --fleft;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int64_t tile = (int64_t)item * MT + m;
+      for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int i = 0; i < C::TILES; ++i)
-        cp16(dst + (m * C::TILES + i) * 512 + lane * 16,
-             codes + ((tile * kb + chunk * C::TILES + i) * 512 + lane * 16));
+        for (int i = 0; i < C::TILES; ++i)
+          cp16(fdst + (m * C::TILES + i) * 512 + lane * 16, fcode + m * tile_codes + i * 512);
 #pragma unroll
-      for (int g = 0; g < C::SG; ++g)
-        cp8(dst + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8,
-            numbers + ((tile * ng + chunk * C::SG + g) * 64 + r * 8));
+        for (int g = 0; g < C::SG; ++g)
+          cp8(fdst + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8,
+              fnum + m * tile_numbers + g * 64);
+      }
+      fcode += C::TILES * 512;
+      fnum += C::SG * 64;
+      if (--fc == 0) {
+        fc = nc;
+        fcode += jump_code;
+        fnum += jump_num;
+      }
     }
+    cp_commit();
+    fdst += C::STAGE;
+    if (fdst == ring_u + C::RING) fdst = ring_u;
   };
 
   lpc::pdl_trigger();
   // the weights belong to no earlier kernel of the stream: their first stages
   // are requested before the kernel that writes x is waited for
-  int fi = blockIdx.x, fc = 0, fst = 0;
-  auto advance = [&]() {
-    if (nc > 0 && fi < items) {
-      fetch(fi, c0 + fc, fst);
-      if (++fc == nc) {
-        fc = 0;
-        fi += gridDim.x;
-      }
-    }
-    cp_commit();
-    if (++fst == C::NST) fst = 0;
-  };
 #pragma unroll
   for (int i = 0; i < C::NST - 1; ++i) advance();
   lpc::pdl_wait();
 
-  // x of token tok0 + 8 j + r: 8 columns at 32 h + 8 t of every 64
+  // x of token tok0 + 8 j + r: 8 columns at 32 h + 8 t of every 64.  A column
+  // without a token repeats the first one; its sums are not stored.
   const T* xp[NT];
-  bool has[NT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    has[j] = 8 * j + r < ntok;
-    xp[j] = x + (int64_t)(tok0 + (has[j] ? 8 * j + r : 0)) * k + 8 * t;
-  }
+  for (int j = 0; j < NT; ++j)
+    xp[j] = x + (int64_t)(tok0 + (8 * j + r < ntok ? 8 * j + r : 0)) * k + c0 * C::CK + 8 * t;
   constexpr uint32_t ONES = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
 
-  int st = 0, buf = 0;
+  const uint8_t* s = ring;
+  int buf = 0;
+  bool fresh = true;  // the sums of x are not in xs
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
     float sum[MT][NT][4];
 #pragma unroll
@@ -177,81 +198,104 @@ __global__ void __launch_bounds__(THREADS)
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[m][j][i] = 0.f;
-    for (int c = 0; c < nc; ++c) {
-      advance();
-      cp_wait<C::NST - 1>();
-      const uint8_t* s = ring + st * C::STAGE;
-      if (++st == C::NST) st = 0;
-      const int64_t col = (int64_t)(c0 + c) * C::CK;
+
+    auto chunks = [&](auto with_sums) {
+      constexpr bool SUMS = decltype(with_sums)::value;
+      for (int c = 0; c < nc; ++c) {
+        advance();
+        cp_wait<C::NST - 1>();
+        const int col = c * C::CK;
 #pragma unroll
-      for (int g = 0; g < C::SG; ++g) {
-        float acc[MT][NT][4], ones[NT][4];
+        for (int g = 0; g < C::SG; ++g) {
+          float acc[MT][NT][4], ones[NT][4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+          for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ones[j][i] = 0.f;
+            for (int i = 0; i < 4; ++i) {
+              ones[j][i] = 0.f;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) acc[m][j][i] = 0.f;
+              for (int m = 0; m < MT; ++m) acc[m][j][i] = 0.f;
+            }
+          // 32-column halves of this group: GS 128 has 4, 64 has 2, 32 has 1
+#pragma unroll
+          for (int hh = 0; hh < GS / 32; ++hh) {
+            const int half = g * (GS / 32) + hh;
+            uint4 xv[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+              xv[j] = *reinterpret_cast<const uint4*>(xp[j] + col + 32 * half);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              const uint2 w = *reinterpret_cast<const uint2*>(
+                  s + (m * C::TILES + (half >> 1)) * 512 + lane * 16 + (half & 1) * 8);
+              uint32_t a[4], b[4];
+              operand<T>(w.x, sh, a);
+              operand<T>(w.y, sh, b);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                mma<T>(acc[m][j], a[0], a[1], a[2], a[3], xv[j].x, xv[j].y);
+                mma<T>(acc[m][j], b[0], b[1], b[2], b[3], xv[j].z, xv[j].w);
+              }
+            }
+            if constexpr (SUMS) {
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                mma<T>(ones[j], ONES, ONES, ONES, ONES, xv[j].x, xv[j].y);
+                mma<T>(ones[j], ONES, ONES, ONES, ONES, xv[j].z, xv[j].w);
+              }
+            }
           }
-        // 32-column halves of this group: GS 128 has 4, 64 has 2, 32 has 1
-#pragma unroll
-        for (int hh = 0; hh < GS / 32; ++hh) {
-          const int half = g * (GS / 32) + hh;
-          uint4 xv[NT];
+          float* px = xs + (c * C::SG + g) * (NT * 8) + 2 * t;
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
-            xv[j] = make_uint4(0u, 0u, 0u, 0u);
-            if (has[j]) xv[j] = *reinterpret_cast<const uint4*>(xp[j] + col + 32 * half);
+            if constexpr (SUMS) {
+              if (keep_sums && r == 0)
+                *reinterpret_cast<float2*>(px + 8 * j) = make_float2(ones[j][0], ones[j][1]);
+            } else {
+              const float2 v = *reinterpret_cast<const float2*>(px + 8 * j);
+              ones[j][0] = v.x;
+              ones[j][1] = v.y;
+            }
           }
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             const uint2 w = *reinterpret_cast<const uint2*>(
-                s + (m * C::TILES + (half >> 1)) * 512 + lane * 16 + (half & 1) * 8);
-            uint32_t a[4], b[4];
-            operand<T>(w.x, a);
-            operand<T>(w.y, b);
+                s + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8);
+            const float2 lo = pair_f<T>(w.x), hi = pair_f<T>(w.y);
+            float s0, m0, s1, m1;
+            if constexpr (std::is_same<T, __half>::value) {
+              s0 = lo.x * 16777216.f;
+              m0 = lo.y;
+              s1 = hi.x * 1048576.f;
+              m1 = hi.y;
+            } else {
+              s0 = lo.x;
+              m0 = fmaf(-128.f, lo.x, lo.y);
+              s1 = hi.x;
+              m1 = fmaf(-128.f, hi.x, hi.y);
+            }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              mma<T>(acc[m][j], a[0], a[1], a[2], a[3], xv[j].x, xv[j].y);
-              mma<T>(acc[m][j], b[0], b[1], b[2], b[3], xv[j].z, xv[j].w);
+              sum[m][j][0] = fmaf(s0, acc[m][j][0], fmaf(m0, ones[j][0], sum[m][j][0]));
+              sum[m][j][1] = fmaf(s0, acc[m][j][1], fmaf(m0, ones[j][1], sum[m][j][1]));
+              sum[m][j][2] = fmaf(s1, acc[m][j][2], fmaf(m1, ones[j][0], sum[m][j][2]));
+              sum[m][j][3] = fmaf(s1, acc[m][j][3], fmaf(m1, ones[j][1], sum[m][j][3]));
             }
           }
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            mma<T>(ones[j], ONES, ONES, ONES, ONES, xv[j].x, xv[j].y);
-            mma<T>(ones[j], ONES, ONES, ONES, ONES, xv[j].z, xv[j].w);
-          }
         }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const uint2 w = *reinterpret_cast<const uint2*>(
-              s + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8);
-          const float2 lo = pair_f<T>(w.x), hi = pair_f<T>(w.y);
-          float s0, m0, s1, m1;
-          if constexpr (std::is_same<T, __half>::value) {
-            s0 = lo.x * 16777216.f;
-            m0 = lo.y;
-            s1 = hi.x * 1048576.f;
-            m1 = hi.y;
-          } else {
-            s0 = lo.x;
-            m0 = fmaf(-128.f, lo.x, lo.y);
-            s1 = hi.x;
-            m1 = fmaf(-128.f, hi.x, hi.y);
-          }
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            sum[m][j][0] = fmaf(s0, acc[m][j][0], fmaf(m0, ones[j][0], sum[m][j][0]));
-            sum[m][j][1] = fmaf(s0, acc[m][j][1], fmaf(m0, ones[j][1], sum[m][j][1]));
-            sum[m][j][2] = fmaf(s1, acc[m][j][2], fmaf(m1, ones[j][0], sum[m][j][2]));
-            sum[m][j][3] = fmaf(s1, acc[m][j][3], fmaf(m1, ones[j][1], sum[m][j][3]));
-          }
-        }
+        s += C::STAGE;
+        if (s == ring + C::RING) s = ring;
       }
+    };
+    if (fresh) {
+      chunks(std::true_type{});
+      fresh = !keep_sums;
+      __syncwarp();
+    } else {
+      chunks(std::false_type{});
     }
-    // partial sums of the 8 warps, [token][row] of the item, added in warp order
-    float* mine = red + (buf * WARPS + warp) * C::RED;
+    // partial sums of the warps, [token][row] of the item, added in warp order
+    float* mine = red + (buf * NW + warp) * C::RED;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -263,16 +307,16 @@ __global__ void __launch_bounds__(THREADS)
         p[MT * 16 + 8] = sum[m][j][3];
       }
     __syncthreads();
-    const float* all = red + buf * WARPS * C::RED;
+    const float* all = red + buf * NW * C::RED;
     auto total = [&](int at) {
       float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) v += all[w * C::RED + at];
+      for (int w = 0; w < NW; ++w) v += all[w * C::RED + at];
       return v;
     };
     if (epi == EPI_SWIGLU) {
       if constexpr (MT == 2)
-        for (int i = threadIdx.x; i < ntok * 16; i += THREADS) {
+        for (int i = threadIdx.x; i < ntok * 16; i += NW * 32) {
           const int tk = i >> 4, row = i & 15;
           const int64_t n = (int64_t)item * 16 + row;
           if (n >= n_out) continue;
@@ -281,12 +325,248 @@ __global__ void __launch_bounds__(THREADS)
               Num<T>::from_f(__fdividef(gate, 1.f + __expf(-gate)) * upv);
         }
     } else {
-      for (int i = threadIdx.x; i < ntok * (MT * 16); i += THREADS) {
+      for (int i = threadIdx.x; i < ntok * (MT * 16); i += NW * 32) {
         const int tk = i / (MT * 16), row = i % (MT * 16);
         const int64_t n = (int64_t)item * (MT * 16) + row;
         if (n >= n_out) continue;
         float v = total(i);
         const int64_t o = (int64_t)(tok0 + tk) * n_out + n;
+        if (epi == EPI_RESIDUAL) v += Num<T>::to_f(resid[o]);
+        out[o] = Num<T>::from_f(v);
+      }
+    }
+    buf ^= 1;
+  }
+  cp_wait<0>();
+}
+
+// ---------------------------------------------------------------------------
+// Up to 8 tokens whose x fits shared memory.  One CTA of 16 warps an SM; each
+// warp keeps its column range of x there as fp16 operands, scaled per token by
+// a power of two (largest value about 2^14), so bf16 takes the 5-instruction
+// unpacking too: what the scaling loses lies 2^-38 below the largest value.
+// The sums of x over the groups are taken once, in fp32.
+// ---------------------------------------------------------------------------
+template <int GS, int MT>
+struct FewCfg {
+  static constexpr int NW = 16;
+  static constexpr int CK = GS > 64 ? GS : 64;
+  static constexpr int TILES = CK / 64;
+  static constexpr int SG = CK / GS;
+  static constexpr int CODES = MT * TILES * 512;
+  static constexpr int STAGE = CODES + MT * SG * 64;
+  static constexpr int NST = CODES >= 2048 ? 3 : CODES >= 1024 ? 5 : 9;
+  static constexpr int RING = NST * STAGE;
+  static constexpr int RED = MT * 16 * 8;
+  static constexpr int SMEM = NW * (RING + 2 * RED * 4);
+  static constexpr int MAX_X = 232448 - SMEM;
+  // bytes of x operands and sums of a warp, for `chunks` chunks and `tokens` tokens
+  __host__ __device__ static constexpr int x_row(int chunks) { return chunks * CK * 2 + 64; }
+  __host__ __device__ static constexpr int64_t x_bytes(int64_t chunks, int tokens) {
+    return tokens * (chunks * CK * 2 + 64) + chunks * SG * 32;
+  }
+};
+
+template <typename T, int GS, int MT>
+__global__ void __launch_bounds__(512)
+    int4_few_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ numbers,
+                    const T* __restrict__ x, const T* resid, T* out, int tokens, int64_t n_out,
+                    int k, int items, int epi) {
+  using C = FewCfg<GS, MT>;
+  constexpr int NW = C::NW;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, t = lane & 3;
+  const int nchunks = k / C::CK;
+  const int64_t tile_codes = (int64_t)(k / 64) * 512, tile_numbers = (int64_t)(k / GS) * 64;
+  const int c0 = warp * nchunks / NW, nc = (warp + 1) * nchunks / NW - c0;
+  uint8_t* ring = smem + warp * C::RING;
+  const uint32_t ring_u = lpc::smem_u32(ring);
+  float* red = reinterpret_cast<float*>(smem + NW * C::RING);
+  const int most = (nchunks + NW - 1) / NW;
+  const int xrow = C::x_row(most);
+  uint8_t* xw = smem + C::SMEM + warp * (int)C::x_bytes(most, tokens);
+  float* xs = reinterpret_cast<float*>(xw + tokens * xrow);  // [group][8 tokens]
+
+  // the weight stream: this warp's chunks of item blockIdx.x, then of the next
+  const uint8_t* fcode = codes + (int64_t)blockIdx.x * MT * tile_codes + c0 * (C::TILES * 512) + lane * 16;
+  const uint8_t* fnum = numbers + (int64_t)blockIdx.x * MT * tile_numbers + c0 * (C::SG * 64) + r * 8;
+  const int64_t jump_code = gridDim.x * MT * tile_codes - nc * (C::TILES * 512);
+  const int64_t jump_num = gridDim.x * MT * tile_numbers - nc * (C::SG * 64);
+  int fleft = nc > 0 ? nc * ((items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) : 0;
+  int fc = nc;
+  int fto = 0;
+  auto advance = [&]() {
+    if (fleft > 0) {
+      --fleft;
+      const uint32_t dst = ring_u + fto;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int i = 0; i < C::TILES; ++i)
+          cp16(dst + (m * C::TILES + i) * 512 + lane * 16, fcode + m * tile_codes + i * 512);
+        if (t == 0)
+#pragma unroll
+          for (int g = 0; g < C::SG; ++g)
+            cp8(dst + C::CODES + (m * C::SG + g) * 64 + r * 8, fnum + m * tile_numbers + g * 64);
+      }
+      fcode += C::TILES * 512;
+      fnum += C::SG * 64;
+      if (--fc == 0) {
+        fc = nc;
+        fcode += jump_code;
+        fnum += jump_num;
+      }
+    }
+    cp_commit();
+    fto = fto == (C::NST - 1) * C::STAGE ? 0 : fto + C::STAGE;
+  };
+
+  lpc::pdl_trigger();
+  // the weights belong to no earlier kernel of the stream: their first stages
+  // are requested before the kernel that writes x is waited for
+#pragma unroll
+  for (int i = 0; i < C::NST - 1; ++i) advance();
+  lpc::pdl_wait();
+
+  // x of this warp's columns
+  float down0 = 1.f, down1 = 1.f;  // 2^-e of tokens 2t and 2t + 1
+  {
+    const int width = nc * C::CK;
+    for (int tk = 0; tk < tokens; ++tk) {
+      const T* src = x + (int64_t)tk * k + c0 * C::CK;
+      int e = 0;
+      if constexpr (!std::is_same<T, __half>::value) {
+        float a = 0.f;
+        for (int c = lane * 8; c < width; c += 256) {
+          const uint4 u = *reinterpret_cast<const uint4*>(src + c);
+          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = pair_f<T>(w[i]);
+            a = fmaxf(a, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        if (a > 0.f && a < INFINITY) e = min(126, 14 - ((int)(__float_as_uint(a) >> 23) - 127));
+        const float d = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (tk == 2 * t) down0 = d;
+        if (tk == 2 * t + 1) down1 = d;
+      }
+      const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+      for (int c = lane * 8; c - lane * 8 < width; c += 256) {
+        float sum = 0.f;
+        if (c < width) {
+          uint4 u = *reinterpret_cast<const uint4*>(src + c);
+          uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = pair_f<T>(w[i]);
+            sum += f.x * up + f.y * up;
+            if constexpr (!std::is_same<T, __half>::value) {
+              const __half2 h = __floats2half2_rn(f.x * up, f.y * up);
+              w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+          }
+          *reinterpret_cast<uint4*>(xw + tk * xrow + c * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+#pragma unroll
+        for (int o = 1; o < GS / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (c < width && c % GS == 0) xs[(c / GS) * 8 + tk] = sum;
+      }
+    }
+  }
+  __syncwarp();
+  const uint8_t* px = xw + (r < tokens ? r : 0) * xrow + t * 16;
+
+  int at = 0, buf = 0;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    float sum[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[m][i] = 0.f;
+    const uint8_t* pc = px;
+    const float* ps = xs + 2 * t;
+    for (int c = 0; c < nc; ++c) {
+      cp_wait<C::NST - 2>();
+      __syncwarp();  // the stage has arrived, and the one before it is free
+      advance();
+      const uint8_t* s = ring + at;
+      at = at == (C::NST - 1) * C::STAGE ? 0 : at + C::STAGE;
+#pragma unroll
+      for (int g = 0; g < C::SG; ++g) {
+        float acc[MT][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
+#pragma unroll
+        for (int hh = 0; hh < GS / 32; ++hh) {
+          const int half = g * (GS / 32) + hh;
+          const uint4 xv = *reinterpret_cast<const uint4*>(pc + half * 64);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const uint2 w = *reinterpret_cast<const uint2*>(
+                s + (m * C::TILES + (half >> 1)) * 512 + lane * 16 + (half & 1) * 8);
+            uint32_t a[4], b[4];
+            operand<__half>(w.x, 0u, a);
+            operand<__half>(w.y, 0u, b);
+            mma<__half>(acc[m], a[0], a[1], a[2], a[3], xv.x, xv.y);
+            mma<__half>(acc[m], b[0], b[1], b[2], b[3], xv.z, xv.w);
+          }
+        }
+        const float2 x2 = *reinterpret_cast<const float2*>(ps + g * 8);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint2 w = *reinterpret_cast<const uint2*>(s + C::CODES + (m * C::SG + g) * 64 + r * 8);
+          const float2 lo = pair_f<T>(w.x), hi = pair_f<T>(w.y);
+          // codes enter as c * 2^-24, those of rows r + 8 as c * 2^-20
+          const float s0 = lo.x * 16777216.f, s1 = hi.x * 1048576.f;
+          sum[m][0] = fmaf(s0, acc[m][0], fmaf(lo.y, x2.x, sum[m][0]));
+          sum[m][1] = fmaf(s0, acc[m][1], fmaf(lo.y, x2.y, sum[m][1]));
+          sum[m][2] = fmaf(s1, acc[m][2], fmaf(hi.y, x2.x, sum[m][2]));
+          sum[m][3] = fmaf(s1, acc[m][3], fmaf(hi.y, x2.y, sum[m][3]));
+        }
+      }
+      pc += C::CK * 2;
+      ps += C::SG * 8;
+    }
+    // partial sums of the warps, [token][row] of the item, added in warp order
+    float* mine = red + (buf * NW + warp) * C::RED;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float* p = mine + 2 * t * (MT * 16) + m * 16 + r;
+      p[0] = sum[m][0] * down0;
+      p[MT * 16] = sum[m][1] * down1;
+      p[8] = sum[m][2] * down0;
+      p[MT * 16 + 8] = sum[m][3] * down1;
+    }
+    __syncthreads();
+    const float* all = red + buf * NW * C::RED;
+    auto total = [&](int i) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) v += all[w * C::RED + i];
+      return v;
+    };
+    if (epi == EPI_SWIGLU) {
+      if constexpr (MT == 2)
+        for (int i = threadIdx.x; i < tokens * 16; i += NW * 32) {
+          const int tk = i >> 4, row = i & 15;
+          const int64_t n = (int64_t)item * 16 + row;
+          if (n >= n_out) continue;
+          const float gate = total(tk * 32 + row), upv = total(tk * 32 + 16 + row);
+          out[(int64_t)tk * n_out + n] = Num<T>::from_f(__fdividef(gate, 1.f + __expf(-gate)) * upv);
+        }
+    } else {
+      for (int i = threadIdx.x; i < tokens * (MT * 16); i += NW * 32) {
+        const int tk = i / (MT * 16), row = i % (MT * 16);
+        const int64_t n = (int64_t)item * (MT * 16) + row;
+        if (n >= n_out) continue;
+        float v = total(i);
+        const int64_t o = (int64_t)tk * n_out + n;
         if (epi == EPI_RESIDUAL) v += Num<T>::to_f(resid[o]);
         out[o] = Num<T>::from_f(v);
       }
@@ -395,44 +675,97 @@ bool use_pdl() {
   return on;
 }
 
-template <typename T, int GS, int MT, int NT>
+template <typename T, int GS, int MT, int NT, int NW>
 int launch(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
            cudaStream_t s) {
-  using C = Cfg<GS, MT, NT>;
+  using C = Cfg<GS, MT, NT, NW>;
   static std::atomic<uint64_t> mask{0};
-  int rc = lpc::once_per_device_smem((const void*)int4_linear_kernel<T, GS, MT, NT>, C::SMEM, mask);
+  int rc = lpc::once_per_device_smem((const void*)int4_linear_kernel<T, GS, MT, NT, NW>,
+                                     C::SMEM + C::XS_MAX, mask);
   if (rc) return rc;
   const int64_t tr = tile_rows(w->n_out, w->layout);
   const int items = (int)(w->layout == 1 ? tr / 2 : (w->n_out + 16 * MT - 1) / (16 * MT));
-  const int slots = lpc::current_device_sms() * std::max(1, (int)(227 * 1024 / (C::SMEM + 1024)));
-  const int rounds = (items + slots - 1) / slots;
+  // the sums of x are computed with the first item and kept for the next ones
+  const int64_t sums = (int64_t)NW * ((w->k / C::CK + NW - 1) / NW) * C::SG * NT * 8 * 4;
+  const int slots = lpc::current_device_sms() * (16 / NW);
+  const int keep = items > slots && sums <= C::XS_MAX;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((items + rounds - 1) / rounds),
-                     (unsigned)((tokens + NT * 8 - 1) / (NT * 8)));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.gridDim = dim3((unsigned)std::min(items, slots), (unsigned)((tokens + NT * 8 - 1) / (NT * 8)));
+  cfg.blockDim = dim3(NW * 32);
+  cfg.dynamicSmemBytes = C::SMEM + (keep ? (int)sums : 0);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const uint8_t* codes = (const uint8_t*)w->packed;
-  cudaLaunchKernelEx(&cfg, int4_linear_kernel<T, GS, MT, NT>, codes,
+  cudaLaunchKernelEx(&cfg, int4_linear_kernel<T, GS, MT, NT, NW>, codes,
+                     codes + tr * 16 * (int64_t)(w->k / 2), (const T*)x, (const T*)resid, (T*)out,
+                     (int)tokens, w->n_out, w->k, items, epi, keep, 1u << 28);
+  return lpc::check_launch("int4_linear");
+}
+
+// Two tile rows share the loads of x; with too few rows to give each SM an
+// item, one tile row an item and 16 warps to share its columns.
+template <typename T, int GS, int NT>
+int launch_mt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
+              cudaStream_t s) {
+  const int64_t tr = (w->n_out + 15) / 16, sms = lpc::current_device_sms();
+  if constexpr (NT < 4) {  // 32 tokens' accumulators do not fit 128 registers
+    if (tr <= sms)
+      return w->layout == 1 ? launch<T, GS, 2, NT, 16>(w, x, out, resid, tokens, epi, s)
+                            : launch<T, GS, 1, NT, 16>(w, x, out, resid, tokens, epi, s);
+  }
+  if (w->layout == 1) return launch<T, GS, 2, NT, 8>(w, x, out, resid, tokens, epi, s);
+  if (NT == 1 || tr <= 2 * sms) return launch<T, GS, 1, NT, 8>(w, x, out, resid, tokens, epi, s);
+  return launch<T, GS, 2, NT, 8>(w, x, out, resid, tokens, epi, s);
+}
+
+template <typename T, int GS, int MT>
+int launch_few(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens,
+               int epi, cudaStream_t s) {
+  using C = FewCfg<GS, MT>;
+  static std::atomic<uint64_t> mask{0};
+  int rc = lpc::once_per_device_smem((const void*)int4_few_kernel<T, GS, MT>, 232448, mask);
+  if (rc) return rc;
+  const int64_t tr = tile_rows(w->n_out, w->layout);
+  const int items = (int)(w->layout == 1 ? tr / 2 : (w->n_out + 16 * MT - 1) / (16 * MT));
+  const int64_t most = (w->k / C::CK + C::NW - 1) / C::NW;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min(items, lpc::current_device_sms()));
+  cfg.blockDim = dim3(512);
+  cfg.dynamicSmemBytes = (size_t)(C::SMEM + C::NW * C::x_bytes(most, (int)tokens));
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const uint8_t* codes = (const uint8_t*)w->packed;
+  cudaLaunchKernelEx(&cfg, int4_few_kernel<T, GS, MT>, codes,
                      codes + tr * 16 * (int64_t)(w->k / 2), (const T*)x, (const T*)resid, (T*)out,
                      (int)tokens, w->n_out, w->k, items, epi);
   return lpc::check_launch("int4_linear");
 }
 
+template <int GS, int MT>
+bool few_fits(const lpc_w4* w, int64_t tokens) {
+  using C = FewCfg<GS, MT>;
+  const int64_t most = (w->k / C::CK + C::NW - 1) / C::NW;
+  return tokens <= 8 && C::NW * C::x_bytes(most, (int)tokens) <= C::MAX_X;
+}
+
 template <typename T, int GS>
 int launch_nt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
               cudaStream_t s) {
-  if (tokens <= 8) {
-    if (w->layout == 1) return launch<T, GS, 2, 1>(w, x, out, resid, tokens, epi, s);
-    return launch<T, GS, 1, 1>(w, x, out, resid, tokens, epi, s);
-  }
-  if (tokens <= 16) return launch<T, GS, 2, 2>(w, x, out, resid, tokens, epi, s);
-  return launch<T, GS, 2, 4>(w, x, out, resid, tokens, epi, s);
+  if (few_fits<GS, 2>(w, tokens))
+    return w->layout == 0 && (w->n_out + 15) / 16 <= lpc::current_device_sms()
+               ? launch_few<T, GS, 1>(w, x, out, resid, tokens, epi, s)
+               : launch_few<T, GS, 2>(w, x, out, resid, tokens, epi, s);
+  if (tokens <= 8) return launch_mt<T, GS, 1>(w, x, out, resid, tokens, epi, s);
+  if (tokens <= 16) return launch_mt<T, GS, 2>(w, x, out, resid, tokens, epi, s);
+  return launch_mt<T, GS, 4>(w, x, out, resid, tokens, epi, s);
 }
 
 template <typename T>

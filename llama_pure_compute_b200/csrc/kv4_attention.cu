@@ -66,14 +66,19 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+// The same, zeros instead of the source's bytes when not `ok`.
+__device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
                : "memory");
 }
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 8 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(n)
+__device__ __forceinline__ void cp8z(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0)
                : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -100,6 +105,15 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// w >> 8 as the upper word of a product with 2^24 that the compiler does not
+// see: the masks' LOP3 and a shift share the half-rate ALU pipe, which bounds
+// this loop; the product runs on the FMA pipe.
+__device__ __forceinline__ uint32_t shift8(uint32_t w, uint32_t p24) {
+  uint64_t p;
+  asm("mul.wide.u32 %0, %1, %2;" : "=l"(p) : "r"(w), "r"(p24));
+  return (uint32_t)(p >> 32);
 }
 
 template <typename T>
@@ -151,7 +165,7 @@ __global__ void __launch_bounds__(W * 32)
                      const uint8_t* __restrict__ vscales, const int32_t* __restrict__ seq_lens,
                      T* __restrict__ out, float* __restrict__ part_o, float* __restrict__ part_ml,
                      int H, int G, int head_blocks, int max_splits, int chunk, float scale_log2,
-                     lpc::Kv4Rows rows) {
+                     uint32_t p24, lpc::Kv4Rows rows) {
   using L = Layout<D>;
   constexpr int CB = L::CB;
   constexpr int KW = D / 32;              // K words of a lane and key
@@ -182,7 +196,6 @@ __global__ void __launch_bounds__(W * 32)
   }
   const int start = split * chunk;
   const int end = min(start + chunk, len);
-  const int ntiles = (end - start + TK - 1) / TK;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
 
@@ -192,33 +205,43 @@ __global__ void __launch_bounds__(W * 32)
   const uint8_t* ks = kscales + head_row * 8;
   const uint8_t* vs = vscales + head_row * 8;
   uint8_t* ring = smem + warp * (NST * L::STAGE);
-  const uint32_t ring_u = lpc::smem_u32(ring);
 
-  // stage `st` <- tile `tile` of this CTA; rows past `end` become zeros
-  auto fetch = [&](int tile, int st) {
-    const int k0 = start + tile * TK;
-    const uint32_t dst = ring_u + st * L::STAGE;
+  // stage at ring offset `to` <- this warp's next tile; rows past `end` become zeros
+  const uint8_t* fk = kc + (int64_t)(start + warp * TK) * CB + lane * 16;
+  const uint8_t* fv = vc + (int64_t)(start + warp * TK) * CB + lane * 16;
+  const uint8_t* fks = ks + (int64_t)(start + warp * TK + lane) * 8;
+  const uint8_t* fvs = vs + (int64_t)(start + warp * TK + lane) * 8;
+  int fleft = end - (start + warp * TK);  // keys from the next tile's first on
+  const uint32_t fdst = lpc::smem_u32(ring) + lane * 16, fdst_s = fdst - lane * 8;
+  auto fetch = [&](int to) {
+    if (fleft >= TK) {
 #pragma unroll
-    for (int c = 0; c < L::CODES / 512; ++c) {
-      const int off = (c * 32 + lane) * 16;
-      const int key = k0 + off / CB;
-      const bool ok = key < end;
-      const int64_t src = (int64_t)(ok ? key : start) * CB + off % CB;
-      cp16(dst + off, kc + src, ok);
-      cp16(dst + L::CODES + off, vc + src, ok);
+      for (int c = 0; c < L::CODES / 512; ++c) {
+        cp16(fdst + to + c * 512, fk + c * 512);
+        cp16(fdst + to + L::CODES + c * 512, fv + c * 512);
+      }
+      cp8(fdst_s + to + 2 * L::CODES, fks);
+      cp8(fdst_s + to + 2 * L::CODES + L::SCALES, fvs);
+    } else if (fleft > 0) {
+#pragma unroll
+      for (int c = 0; c < L::CODES / 512; ++c) {
+        const bool ok = (c * 512 + lane * 16) / CB < fleft;
+        cp16z(fdst + to + c * 512, ok ? fk + c * 512 : kc, ok);
+        cp16z(fdst + to + L::CODES + c * 512, ok ? fv + c * 512 : vc, ok);
+      }
+      const bool ok = lane < fleft;
+      cp8z(fdst_s + to + 2 * L::CODES, ok ? fks : ks, ok);
+      cp8z(fdst_s + to + 2 * L::CODES + L::SCALES, ok ? fvs : vs, ok);
     }
-    const int key = k0 + lane;
-    const bool ok = key < end;
-    const int64_t src = (int64_t)(ok ? key : start) * 8;
-    cp8(dst + 2 * L::CODES + lane * 8, ks + src, ok);
-    cp8(dst + 2 * L::CODES + L::SCALES + lane * 8, vs + src, ok);
+    cp_commit();
+    fleft -= W * TK;
+    fk += W * TK * CB;
+    fv += W * TK * CB;
+    fks += W * TK * 8;
+    fvs += W * TK * 8;
   };
 #pragma unroll
-  for (int i = 0; i < NST - 1; ++i) {
-    const int tile = warp + i * W;
-    if (tile < ntiles) fetch(tile, i);
-    cp_commit();
-  }
+  for (int i = 0; i < NST - 1; ++i) fetch(i * L::STAGE);
 
   // q as the products' column operand.  Lane (r, t) holds head r's dims of
   // words t*KW .. t*KW + KW - 1: word w covers dims 4w..4w+3 of each group.
@@ -279,23 +302,18 @@ __global__ void __launch_bounds__(W * 32)
       for (int j = 0; j < 4; ++j) acc[g][i][j] = 0.f;
 
   constexpr uint32_t LOW = 0x000F000Fu, HIGH = 0x00F000F0u;
-  int st = 0;
-  for (int tile = warp; tile < ntiles; tile += W) {
-    {
-      const int next = tile + (NST - 1) * W;
-      int to = st + NST - 1;
-      if (to >= NST) to -= NST;
-      __syncwarp();  // every lane has read that stage's last tile
-      if (next < ntiles) fetch(next, to);
-      cp_commit();
-    }
+  int at = 0, to = (NST - 1) * L::STAGE;  // ring offsets of this tile and of the next fetch
+  for (int left = end - (start + warp * TK); left > 0; left -= W * TK) {
+    __syncwarp();  // every lane has read the stage that is filled next
+    fetch(to);
     cp_wait<NST - 1>();
     __syncwarp();
-    const uint8_t* sk = ring + st * L::STAGE;
+    const uint8_t* sk = ring + at;
     const uint8_t* sv = sk + L::CODES;
     const uint8_t* sks = sk + 2 * L::CODES;
     const uint8_t* svs = sks + L::SCALES;
-    if (++st == NST) st = 0;
+    at = at == (NST - 1) * L::STAGE ? 0 : at + L::STAGE;
+    to = to == (NST - 1) * L::STAGE ? 0 : to + L::STAGE;
 
     // scores of keys 16u + r and 16u + r + 8
     float x[2][2][NH];
@@ -319,7 +337,7 @@ __global__ void __launch_bounds__(W * 32)
       float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const uint32_t a8 = wa[w] >> 8, b8 = wb[w] >> 8;
+        const uint32_t a8 = shift8(wa[w], p24), b8 = shift8(wb[w], p24);
         mma_f16(c0, wa[w] & LOW, wb[w] & LOW, a8 & LOW, b8 & LOW, qb[w][0][0], qb[w][0][1]);
         mma_f16(c1, wa[w] & HIGH, wb[w] & HIGH, a8 & HIGH, b8 & HIGH, qb[w][1][0], qb[w][1][1]);
       }
@@ -336,7 +354,6 @@ __global__ void __launch_bounds__(W * 32)
         }
       }
     }
-    const int left = end - (start + tile * TK);
     if (left < TK) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -431,7 +448,7 @@ __global__ void __launch_bounds__(W * 32)
             const uint32_t sel = hf ? 0x7632 : 0x5410;
             const uint32_t lo = __byte_perm(kw[0][w], kw[1][w], sel);
             const uint32_t hi = __byte_perm(kw[2][w], kw[3][w], sel);
-            const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+            const uint32_t lo8 = shift8(lo, p24), hi8 = shift8(hi, p24);
             mma_f16(acc[0][2 * w + hf], lo & LOW, lo8 & LOW, hi & LOW, hi8 & LOW, pb[0][0], pb[0][1]);
             mma_f16(acc[1][2 * w + hf], lo & HIGH, lo8 & HIGH, hi & HIGH, hi8 & HIGH, pb[1][0],
                     pb[1][1]);
@@ -499,19 +516,20 @@ __global__ void __launch_bounds__(W * 32)
   }
 }
 
-// One warp per (sequence, head): the splits' partials, in split order.
-constexpr int CWARPS = 4;
+// One CTA per (sequence, head).  Warp w adds the splits w, w + CWARPS, ..., the
+// warps' sums meet in shared memory: the order is fixed.
+constexpr int CWARPS = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(CWARPS * 32)
     kv4_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                        const int32_t* __restrict__ seq_lens, T* __restrict__ out, int H,
-                       int max_splits, int chunk, lpc::Kv4Rows rows, int64_t bh_total) {
+                       int max_splits, int chunk, lpc::Kv4Rows rows) {
   lpc::pdl_trigger();
   lpc::pdl_wait();
   constexpr int DPL = D / 32;
-  const int64_t bh = (int64_t)blockIdx.x * CWARPS + (threadIdx.x >> 5);
-  if (bh >= bh_total) return;
-  const int lane = threadIdx.x & 31;
+  __shared__ float so[CWARPS][D + 2];
+  const int64_t bh = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t b = bh / H;
   int64_t row0, head_rows, cap;
   const bool inside = rows.locate(b, &row0, &head_rows, &cap);
@@ -519,26 +537,37 @@ __global__ void __launch_bounds__(CWARPS * 32)
   if (len > cap) len = (int)cap;
   const int ns = inside && len > 0 ? (len + chunk - 1) / chunk : 0;
   if (ns <= 1) return;  // written by the split kernel
-  const float* ml = part_ml + bh * max_splits * 2;
+  const float2* ml = reinterpret_cast<const float2*>(part_ml) + bh * max_splits;
   const float* po = part_o + bh * max_splits * D + lane * DPL;
   float mx = -INFINITY;
-  for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml[2 * s]);
+  for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml[s].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const float Mu = mx == -INFINITY ? 0.f : mx;
   float O[DPL], Ls = 0.f;
 #pragma unroll
   for (int i = 0; i < DPL; ++i) O[i] = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < ns; ++s) {
-    const float f = fast_exp2(ml[2 * s] - Mu);
+#pragma unroll 4
+  for (int s = warp; s < ns; s += CWARPS) {
+    const float2 v = ml[s];
+    const float f = fast_exp2(v.x - Mu);
 #pragma unroll
     for (int i = 0; i < DPL; ++i) O[i] = fmaf(f, po[(int64_t)s * D + i], O[i]);
-    Ls = fmaf(f, ml[2 * s + 1], Ls);
+    Ls = fmaf(f, v.y, Ls);
   }
-  T* o = out + bh * D + lane * DPL;
 #pragma unroll
-  for (int i = 0; i < DPL; ++i) o[i] = Num<T>::from_f(Ls == 0.f ? 0.f : O[i] / Ls);
+  for (int i = 0; i < DPL; ++i) so[warp][lane * DPL + i] = O[i];
+  if (lane == 0) so[warp][D] = Ls;
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += CWARPS * 32) {
+    float o = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < CWARPS; ++w) {
+      o += so[w][d];
+      l += so[w][D];
+    }
+    out[bh * D + d] = Num<T>::from_f(l == 0.f ? 0.f : o / l);
+  }
 }
 
 bool use_pdl() {
@@ -574,16 +603,15 @@ int launch(const lpc_kv4* kv, const void* q, const int32_t* lens, void* out, flo
                          (const uint8_t*)kv->key_codes, (const uint8_t*)kv->key_scales,
                          (const uint8_t*)kv->value_codes, (const uint8_t*)kv->value_scales, lens,
                          (T*)out, po, pml, heads, G, blocks, max_splits, chunk, scale_log2,
-                         rows) != cudaSuccess)
+                         1u << 24, rows) != cudaSuccess)
     return lpc::check_launch("decode_attention_int4 (split)");
   if ((rc = lpc::check_launch("decode_attention_int4 (split)"))) return rc;
   if (grid_splits == 1) return LPC_OK;
-  const int64_t bh_total = batch * heads;
-  cfg.gridDim = dim3((unsigned)((bh_total + CWARPS - 1) / CWARPS));
+  cfg.gridDim = dim3((unsigned)(batch * heads));
   cfg.blockDim = dim3(CWARPS * 32);
   cfg.dynamicSmemBytes = 0;
   if (cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D>, (const float*)po, (const float*)pml, lens,
-                         (T*)out, heads, max_splits, chunk, rows, bh_total) != cudaSuccess)
+                         (T*)out, heads, max_splits, chunk, rows) != cudaSuccess)
     return lpc::check_launch("decode_attention_int4 (combine)");
   return lpc::check_launch("decode_attention_int4 (combine)");
 }
@@ -595,6 +623,12 @@ constexpr int MAX_HEADS = 65535;
 // Split length: the longest of the candidates that still gives the launch
 // enough CTAs to fill the GPU several times over (592 run at once).
 int split_keys(const lpc_kv4* kv, int64_t batch, int heads) {
+  static const int forced = [] {
+    const char* e = getenv("LPC_DECODE_CHUNK");
+    const int v = e ? atoi(e) : 0;
+    return (v >= UNIT && v <= 65536 && v % UNIT == 0) ? v : 0;
+  }();
+  if (forced) return forced;
   const int64_t G = heads / kv->kv_heads, blocks = (G + HB - 1) / HB;
   const int64_t pairs = batch * kv->kv_heads * blocks;
   for (int c : {1024, 512, 256})
@@ -604,7 +638,7 @@ int split_keys(const lpc_kv4* kv, int64_t batch, int heads) {
 
 bool sizes_ok(const lpc_kv4* kv, int64_t batch, int heads) {
   return batch >= 0 && batch <= MAX_BATCH && heads > 0 && heads <= MAX_HEADS &&
-         heads % kv->kv_heads == 0 && kv->max_seq_len <= MAX_SEQ;
+         heads % kv->kv_heads == 0 && kv->max_seq_len <= MAX_SEQ && batch * heads <= 0x7fffffffLL;
 }
 
 }  // namespace
