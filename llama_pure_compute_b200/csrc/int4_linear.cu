@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(NW * 32)
             uint4 xv[NT];
 #pragma unroll
             for (int j = 0; j < NT; ++j)
-              xv[j] = *reinterpret_cast<const uint4*>(xp[j] + col + 32 * half);
+              xv[j] = lpc::ld_dep16(xp[j] + col + 32 * half);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
               const uint2 w = *reinterpret_cast<const uint2*>(
@@ -341,13 +341,17 @@ __global__ void __launch_bounds__(NW * 32)
 }
 
 // ---------------------------------------------------------------------------
-// Up to 8 tokens whose x fits shared memory.  One CTA of 16 warps an SM; each
-// warp keeps its column range of x there as fp16 operands, scaled per token by
-// a power of two (largest value about 2^14), so bf16 takes the 5-instruction
-// unpacking too: what the scaling loses lies 2^-38 below the largest value.
-// The sums of x over the groups are taken once, in fp32.
+// Up to 8 tokens whose x fits shared memory.  CTAs of 16 warps; each warp keeps
+// its column range of x there as fp16 operands, scaled per token by a power of
+// two (largest value about 2^14), so bf16 takes the 5-instruction unpacking
+// too: what the scaling loses lies 2^-38 below the largest value.  The sums of
+// x over the groups are taken once, in fp32.  TC is 1 or 8: one token alone has
+// half the accumulators and leaves room for two CTAs an SM.
 // ---------------------------------------------------------------------------
-template <int GS, int MT>
+constexpr int64_t MAX_SMEM = 232448;   // of a CTA
+constexpr int64_t HALF_SMEM = 115712;  // of each of two CTAs on an SM
+
+template <int GS, int MT, int TC>
 struct FewCfg {
   static constexpr int NW = 16;
   static constexpr int CK = GS > 64 ? GS : 64;
@@ -355,25 +359,38 @@ struct FewCfg {
   static constexpr int SG = CK / GS;
   static constexpr int CODES = MT * TILES * 512;
   static constexpr int STAGE = CODES + MT * SG * 64;
-  static constexpr int NST = CODES >= 2048 ? 3 : CODES >= 1024 ? 5 : 9;
+  static constexpr int NST = (TC == 1 ? 75 : 107) * 1024 / (NW * STAGE);
   static constexpr int RING = NST * STAGE;
-  static constexpr int RED = MT * 16 * 8;
-  static constexpr int SMEM = NW * (RING + 2 * RED * 4);
-  static constexpr int MAX_X = 232448 - SMEM;
+  static_assert(NST >= 2, "no stage ahead");
   // bytes of x operands and sums of a warp, for `chunks` chunks and `tokens` tokens
   __host__ __device__ static constexpr int x_row(int chunks) { return chunks * CK * 2 + 64; }
   __host__ __device__ static constexpr int64_t x_bytes(int64_t chunks, int tokens) {
     return tokens * (chunks * CK * 2 + 64) + chunks * SG * 32;
   }
+  // items whose partial sums meet at one barrier, so that it has about 128
+  // values to add whatever the number of tokens
+  __host__ __device__ static constexpr int batch(int tokens) {
+    return tokens >= 8 / MT ? 1 : 8 / (MT * tokens);
+  }
+  // words of a warp's partial sums; 8 apart from a multiple of 16, so that 8
+  // neighbouring values of 4 warps lie in 32 banks
+  __host__ __device__ static constexpr int red(int tokens) {
+    return batch(tokens) * tokens * MT * 16 + 8;
+  }
+  static constexpr int64_t smem(int64_t k, int tokens) {
+    return NW * (RING + x_bytes((k / CK + NW - 1) / NW, tokens) + 2 * red(tokens) * 4);
+  }
 };
 
-template <typename T, int GS, int MT>
-__global__ void __launch_bounds__(512)
+template <typename T, int GS, int MT, int TC>
+__global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
     int4_few_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ numbers,
-                    const T* __restrict__ x, const T* resid, T* out, int tokens, int64_t n_out,
-                    int k, int items, int epi) {
-  using C = FewCfg<GS, MT>;
+                    const T* x, const T* resid, T* out, int tokens_, int64_t n_out, int k,
+                    int items, int epi) {
+  using C = FewCfg<GS, MT, TC>;
   constexpr int NW = C::NW;
+  constexpr int NC = TC == 1 ? 1 : 2;  // columns of the products that a lane keeps
+  const int tokens = TC == 1 ? 1 : tokens_;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
@@ -382,10 +399,11 @@ __global__ void __launch_bounds__(512)
   const int c0 = warp * nchunks / NW, nc = (warp + 1) * nchunks / NW - c0;
   uint8_t* ring = smem + warp * C::RING;
   const uint32_t ring_u = lpc::smem_u32(ring);
-  float* red = reinterpret_cast<float*>(smem + NW * C::RING);
   const int most = (nchunks + NW - 1) / NW;
   const int xrow = C::x_row(most);
-  uint8_t* xw = smem + C::SMEM + warp * (int)C::x_bytes(most, tokens);
+  uint8_t* xw = smem + NW * C::RING + warp * (int)C::x_bytes(most, tokens);
+  const int rs = C::red(tokens);
+  float* red = reinterpret_cast<float*>(smem + NW * (C::RING + (int)C::x_bytes(most, tokens)));
   float* xs = reinterpret_cast<float*>(xw + tokens * xrow);  // [group][8 tokens]
 
   // the weight stream: this warp's chunks of item blockIdx.x, then of the next
@@ -401,15 +419,16 @@ __global__ void __launch_bounds__(512)
       --fleft;
       const uint32_t dst = ring_u + fto;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int i = 0; i < C::TILES; ++i)
           cp16(dst + (m * C::TILES + i) * 512 + lane * 16, fcode + m * tile_codes + i * 512);
-        if (t == 0)
+      if (t == 0)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int g = 0; g < C::SG; ++g)
             cp8(dst + C::CODES + (m * C::SG + g) * 64 + r * 8, fnum + m * tile_numbers + g * 64);
-      }
       fcode += C::TILES * 512;
       fnum += C::SG * 64;
       if (--fc == 0) {
@@ -429,66 +448,100 @@ __global__ void __launch_bounds__(512)
   for (int i = 0; i < C::NST - 1; ++i) advance();
   lpc::pdl_wait();
 
-  // x of this warp's columns
-  float down0 = 1.f, down1 = 1.f;  // 2^-e of tokens 2t and 2t + 1
+  // x of this warp's columns.  All tokens' loads of a stretch of 256 columns
+  // are in flight at once; a range of one stretch is read once.
+  constexpr bool SCALE = !std::is_same<T, __half>::value;
+  float down[NC];  // 2^-e of tokens 2t (and 2t + 1)
+#pragma unroll
+  for (int i = 0; i < NC; ++i) down[i] = 1.f;
   {
     const int width = nc * C::CK;
-    for (int tk = 0; tk < tokens; ++tk) {
-      const T* src = x + (int64_t)tk * k + c0 * C::CK;
-      int e = 0;
-      if constexpr (!std::is_same<T, __half>::value) {
-        float a = 0.f;
-        for (int c = lane * 8; c < width; c += 256) {
-          const uint4 u = *reinterpret_cast<const uint4*>(src + c);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    const T* src = x + c0 * C::CK + lane * 8;
+    uint4 u[TC];
+    auto load = [&](int c) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = pair_f<T>(w[i]);
-            a = fmaxf(a, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
+      for (int tk = 0; tk < TC; ++tk)
+        if (tk < tokens) {
+          u[tk] = make_uint4(0u, 0u, 0u, 0u);
+          if (c + lane * 8 < width) u[tk] = lpc::ld_dep16(src + (int64_t)tk * k + c);
         }
+    };
+    load(0);
+    float up[TC];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        if (a > 0.f && a < INFINITY) e = min(126, 14 - ((int)(__float_as_uint(a) >> 23) - 127));
-        const float d = __uint_as_float((uint32_t)(127 - e) << 23);
-        if (tk == 2 * t) down0 = d;
-        if (tk == 2 * t + 1) down1 = d;
-      }
-      const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-      for (int c = lane * 8; c - lane * 8 < width; c += 256) {
-        float sum = 0.f;
-        if (c < width) {
-          uint4 u = *reinterpret_cast<const uint4*>(src + c);
-          uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int tk = 0; tk < TC; ++tk) up[tk] = SCALE ? 0.f : 1.f;
+    if constexpr (SCALE) {
+      for (int c = 0;;) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = pair_f<T>(w[i]);
-            sum += f.x * up + f.y * up;
-            if constexpr (!std::is_same<T, __half>::value) {
-              const __half2 h = __floats2half2_rn(f.x * up, f.y * up);
-              w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int tk = 0; tk < TC; ++tk)
+          if (tk < tokens) {
+            const uint32_t w[4] = {u[tk].x, u[tk].y, u[tk].z, u[tk].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = pair_f<T>(w[i]);
+              up[tk] = fmaxf(up[tk], fmaxf(fabsf(f.x), fabsf(f.y)));
             }
           }
-          *reinterpret_cast<uint4*>(xw + tk * xrow + c * 2) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-#pragma unroll
-        for (int o = 1; o < GS / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (c < width && c % GS == 0) xs[(c / GS) * 8 + tk] = sum;
+        c += 256;
+        if (c >= width) break;
+        load(c);
       }
+      if (width > 256) load(0);
+#pragma unroll
+      for (int tk = 0; tk < TC; ++tk)
+        if (tk < tokens) {
+          // the bits of a non-negative float order as integers do
+          const float a = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(up[tk])));
+          int e = 0;
+          if (a > 0.f && a < INFINITY) e = min(126, 14 - ((int)(__float_as_uint(a) >> 23) - 127));
+          up[tk] = __uint_as_float((uint32_t)(127 + e) << 23);
+          const float d = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+          for (int i = 0; i < NC; ++i)
+            if (tk == NC * t + i) down[i] = d;
+        }
+    }
+    for (int c = 0; c < width;) {
+#pragma unroll
+      for (int tk = 0; tk < TC; ++tk)
+        if (tk < tokens) {
+          uint32_t w[4] = {u[tk].x, u[tk].y, u[tk].z, u[tk].w};
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = pair_f<T>(w[i]);
+            if constexpr (SCALE) {
+              const __half2 h = __floats2half2_rn(f.x * up[tk], f.y * up[tk]);
+              w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            sum += f.x * up[tk] + f.y * up[tk];
+          }
+          const int col = c + lane * 8;
+          if (col < width)
+            *reinterpret_cast<uint4*>(xw + tk * xrow + col * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+          for (int o = 1; o < GS / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          // in the units of the accumulators, which hold c * 2^-24
+          if (col < width && col % GS == 0) xs[(col / GS) * 8 + tk] = sum * 0x1p-24f;
+        }
+      c += 256;
+      if (c < width) load(c);
     }
   }
   __syncwarp();
   const uint8_t* px = xw + (r < tokens ? r : 0) * xrow + t * 16;
 
-  int at = 0, buf = 0;
+  int at = 0, buf = 0, held = 0;
+  const int batch = C::batch(tokens), values = tokens * MT * 16;
+  const int prs = (epi == EPI_SWIGLU ? 3 : 4) + (MT == 2);  // log2 of an item's output rows
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    float sum[MT][4];
+    float sum[MT][2 * NC];  // rows r, then r + 8
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[m][i] = 0.f;
+      for (int i = 0; i < 2 * NC; ++i) sum[m][i] = 0.f;
     const uint8_t* pc = px;
-    const float* ps = xs + 2 * t;
+    const float* ps = xs + (NC == 1 ? 0 : 2 * t);
     for (int c = 0; c < nc; ++c) {
       cp_wait<C::NST - 2>();
       __syncwarp();  // the stage has arrived, and the one before it is free
@@ -517,60 +570,76 @@ __global__ void __launch_bounds__(512)
             mma<__half>(acc[m], b[0], b[1], b[2], b[3], xv.z, xv.w);
           }
         }
-        const float2 x2 = *reinterpret_cast<const float2*>(ps + g * 8);
+        float x2[NC];
+        x2[0] = ps[g * 8];
+        if constexpr (NC == 2) {
+          const float2 v = *reinterpret_cast<const float2*>(ps + g * 8);
+          x2[0] = v.x;
+          x2[1] = v.y;
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const uint2 w = *reinterpret_cast<const uint2*>(s + C::CODES + (m * C::SG + g) * 64 + r * 8);
           const float2 lo = pair_f<T>(w.x), hi = pair_f<T>(w.y);
-          // codes enter as c * 2^-24, those of rows r + 8 as c * 2^-20
-          const float s0 = lo.x * 16777216.f, s1 = hi.x * 1048576.f;
-          sum[m][0] = fmaf(s0, acc[m][0], fmaf(lo.y, x2.x, sum[m][0]));
-          sum[m][1] = fmaf(s0, acc[m][1], fmaf(lo.y, x2.y, sum[m][1]));
-          sum[m][2] = fmaf(s1, acc[m][2], fmaf(hi.y, x2.x, sum[m][2]));
-          sum[m][3] = fmaf(s1, acc[m][3], fmaf(hi.y, x2.y, sum[m][3]));
+          // the codes of rows r + 8 count 16-fold: so does their minimum, and
+          // the sum is divided at the end
+#pragma unroll
+          for (int i = 0; i < NC; ++i) {
+            sum[m][i] = fmaf(lo.x, acc[m][i], fmaf(lo.y, x2[i], sum[m][i]));
+            sum[m][NC + i] = fmaf(hi.x, acc[m][2 + i], fmaf(hi.y, x2[i] * 16.f, sum[m][NC + i]));
+          }
         }
       }
       pc += C::CK * 2;
       ps += C::SG * 8;
     }
     // partial sums of the warps, [token][row] of the item, added in warp order
-    float* mine = red + (buf * NW + warp) * C::RED;
+    float* mine = red + (buf * NW + warp) * rs + held * values;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      float* p = mine + 2 * t * (MT * 16) + m * 16 + r;
-      p[0] = sum[m][0] * down0;
-      p[MT * 16] = sum[m][1] * down1;
-      p[8] = sum[m][2] * down0;
-      p[MT * 16 + 8] = sum[m][3] * down1;
-    }
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (NC * t + i < tokens) {
+          float* p = mine + (NC * t + i) * (MT * 16) + m * 16 + r;
+          p[0] = sum[m][i] * down[i] * 0x1p24f;
+          p[8] = sum[m][NC + i] * down[i] * 0x1p20f;
+        }
+    if (++held < batch && item + (int)gridDim.x < items) continue;
     __syncthreads();
-    const float* all = red + buf * NW * C::RED;
+    // 4 lanes to a value, each adding 4 warps' parts
+    const float* part = red + buf * NW * rs + (lane & 3) * rs;
     auto total = [&](int i) {
       float v = 0.f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) v += all[w * C::RED + i];
-      return v;
+      for (int w = 0; w < NW / 4; ++w) v += part[w * 4 * rs + i];
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      return v + __shfl_xor_sync(0xffffffffu, v, 2);
     };
-    if (epi == EPI_SWIGLU) {
-      if constexpr (MT == 2)
-        for (int i = threadIdx.x; i < tokens * 16; i += NW * 32) {
-          const int tk = i >> 4, row = i & 15;
-          const int64_t n = (int64_t)item * 16 + row;
-          if (n >= n_out) continue;
-          const float gate = total(tk * 32 + row), upv = total(tk * 32 + 16 + row);
-          out[(int64_t)tk * n_out + n] = Num<T>::from_f(__fdividef(gate, 1.f + __expf(-gate)) * upv);
-        }
-    } else {
-      for (int i = threadIdx.x; i < tokens * (MT * 16); i += NW * 32) {
-        const int tk = i / (MT * 16), row = i % (MT * 16);
-        const int64_t n = (int64_t)item * (MT * 16) + row;
-        if (n >= n_out) continue;
-        float v = total(i);
-        const int64_t o = (int64_t)tk * n_out + n;
+    const int per_item = tokens << prs, count = held * per_item;
+    for (int i0 = warp * 8; i0 < count; i0 += NW * 8) {  // whole warps leave together
+      const int at_i = i0 + (lane >> 2), i = min(at_i, count - 1);
+      const int row = i & ((1 << prs) - 1);
+      int tk = i >> prs, sub = 0;  // row of the batch's [item][token]
+      while (tk >= tokens) {
+        tk -= tokens;
+        ++sub;
+      }
+      const int64_t n = ((int64_t)(item - (held - 1 - sub) * (int)gridDim.x) << prs) + row;
+      const int64_t o = (int64_t)tk * n_out + n;
+      float v;
+      if (epi == EPI_SWIGLU) {
+        const int p = sub * values + tk * (MT * 16) + row;
+        const float gate = total(p), upv = total(p + 16);
+        v = __fdividef(gate, 1.f + __expf(-gate)) * upv;
+      } else {
+        v = total(i);
+      }
+      if ((lane & 3) == 0 && at_i < count && n < n_out) {
         if (epi == EPI_RESIDUAL) v += Num<T>::to_f(resid[o]);
         out[o] = Num<T>::from_f(v);
       }
     }
+    held = 0;
     buf ^= 1;
   }
   cp_wait<0>();
@@ -580,10 +649,11 @@ __global__ void __launch_bounds__(512)
 // layout
 // ---------------------------------------------------------------------------
 // Tile rows of 16: of the weight (layout 0), or gate tile i, up tile i, ...
-// (layout 1, gate rows first in the source).  An even number of them.
+// (layout 1, gate rows first in the source).  A multiple of 4 of them, so that
+// no item reaches past the last.
 __host__ __device__ inline int64_t tile_rows(int64_t n_out, int layout) {
-  const int64_t t = (n_out + 15) / 16;
-  return layout == 1 ? 2 * t : (t + 1) / 2 * 2;
+  const int64_t t = (n_out + 15) / 16 * (layout == 1 ? 2 : 1);
+  return (t + 3) / 4 * 4;
 }
 // Source row of row `i` of tile row `p`, or -1 for padding.
 __device__ __forceinline__ int64_t source_row(int64_t p, int i, int64_t n_out, int layout) {
@@ -643,8 +713,6 @@ template <typename T>
 __global__ void int4_unpack_kernel(const uint32_t* __restrict__ codes, const T* __restrict__ numbers,
                                    T* __restrict__ out, int64_t words, int64_t n_out, int k,
                                    int group, int layout) {
-  lpc::pdl_trigger();
-  lpc::pdl_wait();
   const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (at >= words) return;
   const int j = (int)(at & 3), lane = (int)((at >> 2) & 31);
@@ -722,47 +790,57 @@ int launch_mt(const lpc_w4* w, const void* x, void* out, const void* resid, int6
   return launch<T, GS, 2, NT, 8>(w, x, out, resid, tokens, epi, s);
 }
 
-template <typename T, int GS, int MT>
+// Items of MT tile rows each.
+int few_items(const lpc_w4* w, int mt) {
+  const int64_t tr = (w->n_out + 15) / 16 * (w->layout == 1 ? 2 : 1);
+  return (int)((tr + mt - 1) / mt);
+}
+
+template <typename T, int GS, int MT, int TC>
 int launch_few(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens,
                int epi, cudaStream_t s) {
-  using C = FewCfg<GS, MT>;
+  using C = FewCfg<GS, MT, TC>;
   static std::atomic<uint64_t> mask{0};
-  int rc = lpc::once_per_device_smem((const void*)int4_few_kernel<T, GS, MT>, 232448, mask);
+  int rc = lpc::once_per_device_smem((const void*)int4_few_kernel<T, GS, MT, TC>, (int)MAX_SMEM, mask);
   if (rc) return rc;
-  const int64_t tr = tile_rows(w->n_out, w->layout);
-  const int items = (int)(w->layout == 1 ? tr / 2 : (w->n_out + 16 * MT - 1) / (16 * MT));
-  const int64_t most = (w->k / C::CK + C::NW - 1) / C::NW;
+  const int items = few_items(w, MT);
+  const int64_t smem = C::smem(w->k, (int)tokens);
+  const int slots = lpc::current_device_sms() * (TC == 1 && smem <= HALF_SMEM ? 2 : 1);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min(items, lpc::current_device_sms()));
+  cfg.gridDim = dim3((unsigned)std::min(items, slots));
   cfg.blockDim = dim3(512);
-  cfg.dynamicSmemBytes = (size_t)(C::SMEM + C::NW * C::x_bytes(most, (int)tokens));
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const uint8_t* codes = (const uint8_t*)w->packed;
-  cudaLaunchKernelEx(&cfg, int4_few_kernel<T, GS, MT>, codes,
-                     codes + tr * 16 * (int64_t)(w->k / 2), (const T*)x, (const T*)resid, (T*)out,
-                     (int)tokens, w->n_out, w->k, items, epi);
+  cudaLaunchKernelEx(&cfg, int4_few_kernel<T, GS, MT, TC>, codes,
+                     codes + tile_rows(w->n_out, w->layout) * 16 * (int64_t)(w->k / 2), (const T*)x,
+                     (const T*)resid, (T*)out, (int)tokens, w->n_out, w->k, items, epi);
   return lpc::check_launch("int4_linear");
 }
 
-template <int GS, int MT>
-bool few_fits(const lpc_w4* w, int64_t tokens) {
-  using C = FewCfg<GS, MT>;
-  const int64_t most = (w->k / C::CK + C::NW - 1) / C::NW;
-  return tokens <= 8 && C::NW * C::x_bytes(most, (int)tokens) <= C::MAX_X;
+// Two tile rows an item share x's operands and the barrier; one where that
+// leaves an SM without work.
+template <typename T, int GS, int TC>
+int launch_few_mt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens,
+                  int epi, cudaStream_t s) {
+  static const int force = [] { const char* e = getenv("LPC_MT"); return e ? atoi(e) : 0; }();
+  const bool one = force ? force == 1 : few_items(w, 1) <= lpc::current_device_sms() * (TC == 1 ? 2 : 1);
+  if (w->layout == 0 && one) return launch_few<T, GS, 1, TC>(w, x, out, resid, tokens, epi, s);
+  return launch_few<T, GS, 2, TC>(w, x, out, resid, tokens, epi, s);
 }
 
 template <typename T, int GS>
 int launch_nt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
               cudaStream_t s) {
-  if (few_fits<GS, 2>(w, tokens))
-    return w->layout == 0 && (w->n_out + 15) / 16 <= lpc::current_device_sms()
-               ? launch_few<T, GS, 1>(w, x, out, resid, tokens, epi, s)
-               : launch_few<T, GS, 2>(w, x, out, resid, tokens, epi, s);
+  if (tokens == 1 && FewCfg<GS, 2, 1>::smem(w->k, 1) <= MAX_SMEM)
+    return launch_few_mt<T, GS, 1>(w, x, out, resid, tokens, epi, s);
+  if (tokens <= 8 && FewCfg<GS, 2, 8>::smem(w->k, (int)tokens) <= MAX_SMEM)
+    return launch_few_mt<T, GS, 8>(w, x, out, resid, tokens, epi, s);
   if (tokens <= 8) return launch_mt<T, GS, 1>(w, x, out, resid, tokens, epi, s);
   if (tokens <= 16) return launch_mt<T, GS, 2>(w, x, out, resid, tokens, epi, s);
   return launch_mt<T, GS, 4>(w, x, out, resid, tokens, epi, s);

@@ -38,8 +38,8 @@ struct Kv4Rows {
       *capacity = max_seq;
       return true;
     }
-    const int64_t sb = __ldg(base + b);
-    const int64_t c = __ldg(cap + b);
+    const int64_t sb = ld_dep(base + b);
+    const int64_t c = ld_dep(cap + b);
     *row0 = sb;
     *head_rows = total_rows;
     *capacity = c;

@@ -97,12 +97,12 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 template <typename TT>
 __device__ __forceinline__ void load8(const TT* p, float (&f)[8]) {
   if constexpr (sizeof(TT) == 4) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    const uint4 a = lpc::ld_dep16(p), b = lpc::ld_dep16(p + 4);
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
   } else {
-    unpack8<TT>(__ldg(reinterpret_cast<const uint4*>(p)), f);
+    unpack8<TT>(lpc::ld_dep16(p), f);
   }
 }
 
@@ -154,11 +154,11 @@ __global__ void __launch_bounds__(THREADS) kv4_append_kernel(
     x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
     if (hh < all) {
       const T* p = src + (int64_t)hh * D;
-      x0[k] = __ldg(reinterpret_cast<const uint4*>(p));
-      x1[k] = __ldg(reinterpret_cast<const uint4*>(p + D / 2));
+      x0[k] = lpc::ld_dep16(p);
+      x1[k] = lpc::ld_dep16(p + D / 2);
     }
   }
-  const int64_t pos = __ldg(positions + tok);
+  const int64_t pos = lpc::ld_dep(positions + tok);
   const int64_t b = tok / seq;
   const int64_t q_row = b * H * seq + (tok - b * seq);  // q_out row of (b, head 0, s)
   int64_t row0 = 0, head_rows = 0, cap = 0;
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(THREADS) kv4_read_kernel(
   const int c = threadIdx.x % C;
   const int h = blockIdx.y;
   const int64_t b = blockIdx.z;
-  const int64_t pos = __ldg(positions + b * seq + s);
+  const int64_t pos = lpc::ld_dep(positions + b * seq + s);
   int64_t row0, head_rows, cap;
   const bool inside = rows.locate(b, &row0, &head_rows, &cap);
   const int64_t o = ((b * rows.kv_heads + h) * seq + s) * D + c * 8;
@@ -278,9 +278,9 @@ __global__ void __launch_bounds__(THREADS) kv4_read_kernel(
     return;
   }
   const int64_t row = row0 + (int64_t)h * head_rows + pos;
-  const uint2 cw[2] = {*reinterpret_cast<const uint2*>(kcodes + row * (D / 2) + c * 8),
-                       *reinterpret_cast<const uint2*>(vcodes + row * (D / 2) + c * 8)};
-  const uint2 sw[2] = {*reinterpret_cast<const uint2*>(kscales + row * 8),
+  const uint2 cw[2] = {lpc::ld_dep8(kcodes + row * (D / 2) + c * 8),
+                       lpc::ld_dep8(vcodes + row * (D / 2) + c * 8)};
+  const uint2 sw[2] = {lpc::ld_dep8(kscales + row * 8),
                        *reinterpret_cast<const uint2*>(vscales + row * 8)};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {

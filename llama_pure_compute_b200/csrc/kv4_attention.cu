@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(W * 32)
   const int64_t h0 = (int64_t)kvh * G + hb * HB;      // the first of them
   int64_t row0, head_rows, cap;
   const bool inside = rows.locate(b, &row0, &head_rows, &cap);
-  int len = __ldg(seq_lens + b);
+  int len = lpc::ld_dep(seq_lens + b);
   if (!inside || len > cap) {
     if (split == 0 && threadIdx.x == 0) atomicOr(&g_kv4_attn_status, LPC_DEV_ERR_BOUNDS);
     len = inside ? (int)cap : 0;
@@ -249,19 +249,35 @@ __global__ void __launch_bounds__(W * 32)
   float qs0 = 0.f, qs1 = 0.f, amax = 0.f;
   float qv[KW][8];
   {
-    const T* qp = q + (b * H + h0 + (r < heads ? r : 0)) * D;
+    const T* qp = q + (b * H + h0 + (r < heads ? r : 0)) * D + 4 * KW * t;
 #pragma unroll
-    for (int w = 0; w < KW; ++w)
+    for (int g = 0; g < 2; ++g) {
+      uint32_t w[2 * KW];  // 4 KW dims
+      if constexpr (KW == 1) {
+        const uint2 v = lpc::ld_dep8(qp + g * (D / 2));
+        w[0] = v.x;
+        w[1] = v.y;
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int d = 4 * (t * KW + w) + i + g * (D / 2);
-          const float f = r < heads ? Num<T>::to_f(qp[d]) : 0.f;
-          qv[w][g * 4 + i] = f;
-          amax = fmaxf(amax, fabsf(f));
-          if (g == 0) qs0 += f; else qs1 += f;
+        for (int i = 0; i < KW / 2; ++i) {
+          const uint4 v = lpc::ld_dep16(qp + g * (D / 2) + 8 * i);
+          w[4 * i] = v.x;
+          w[4 * i + 1] = v.y;
+          w[4 * i + 2] = v.z;
+          w[4 * i + 3] = v.w;
         }
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * KW; ++i) {
+        float lo, hi;
+        unpack_sm<T>(w[i], lo, hi);
+        if (r >= heads) lo = hi = 0.f;
+        qv[i / 2][g * 4 + 2 * (i & 1)] = lo;
+        qv[i / 2][g * 4 + 2 * (i & 1) + 1] = hi;
+        amax = fmaxf(amax, fmaxf(fabsf(lo), fabsf(hi)));
+        if (g == 0) qs0 += lo + hi; else qs1 += lo + hi;
+      }
+    }
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
@@ -521,8 +537,8 @@ __global__ void __launch_bounds__(W * 32)
 constexpr int CWARPS = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(CWARPS * 32)
-    kv4_combine_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                       const int32_t* __restrict__ seq_lens, T* __restrict__ out, int H,
+    kv4_combine_kernel(const float* part_o, const float* part_ml,
+                       const int32_t* __restrict__ seq_lens, T* out, int H,
                        int max_splits, int chunk, lpc::Kv4Rows rows) {
   lpc::pdl_trigger();
   lpc::pdl_wait();
@@ -533,7 +549,7 @@ __global__ void __launch_bounds__(CWARPS * 32)
   const int64_t b = bh / H;
   int64_t row0, head_rows, cap;
   const bool inside = rows.locate(b, &row0, &head_rows, &cap);
-  int len = __ldg(seq_lens + b);
+  int len = lpc::ld_dep(seq_lens + b);
   if (len > cap) len = (int)cap;
   const int ns = inside && len > 0 ? (len + chunk - 1) / chunk : 0;
   if (ns <= 1) return;  // written by the split kernel

@@ -119,8 +119,8 @@ def test_linear_refusals():
     bad = weight(dtype=0)
     assert lib.lpc_int4_linear(ctypes.addressof(bad), 16, 16, None, 1, 0, None) == UNSUPPORTED
     assert lib.lpc_int4_weight_bytes(100, 100, 128, 0) == 0
-    # 17 rows make two tiles of 16; a pair of 17 makes four
-    assert lib.lpc_int4_weight_bytes(17, 256, 128, 0) == 2 * 16 * 128 + 2 * 64 * 2
+    # tile rows of 16, a multiple of 4 of them: 17 rows need two, a pair of 17 four
+    assert lib.lpc_int4_weight_bytes(17, 256, 128, 0) == 4 * 16 * 128 + 4 * 64 * 2
     assert lib.lpc_int4_weight_bytes(17, 256, 128, 1) == 4 * 16 * 128 + 4 * 64 * 2
     del w0, w1
 
