@@ -51,7 +51,7 @@ using lpc::Num;
 
 constexpr int W = 4;          // warps
 constexpr int TK = 32;        // keys per warp tile
-constexpr int NST = 4;        // stages per warp
+constexpr int NST = 3;          // stages per warp
 constexpr int HB = 8;         // query heads per CTA (columns of the products)
 constexpr int UNIT = 128;     // shortest split: one tile per warp; workspace granularity
 constexpr float LOG2E = 1.4426950408889634f;
@@ -95,6 +95,30 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same with a zero accumulator going in.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Four (two) 8x8 matrices of 16-bit units, transposed: rows are keys, and the
+// lane (r, t) gets unit r of keys 2t and 2t + 1.
+__device__ __forceinline__ void ldm4(uint32_t (&v)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldm2(uint32_t (&v)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+               : "=r"(v[0]), "=r"(v[1])
+               : "r"(addr)
+               : "memory");
+}
+
 // Transpose of an 8x8 matrix of 16-bit values spread over the warp.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t d;
@@ -105,15 +129,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
-}
-
-// w >> 8 as the upper word of a product with 2^24 that the compiler does not
-// see: the masks' LOP3 and a shift share the half-rate ALU pipe, which bounds
-// this loop; the product runs on the FMA pipe.
-__device__ __forceinline__ uint32_t shift8(uint32_t w, uint32_t p24) {
-  uint64_t p;
-  asm("mul.wide.u32 %0, %1, %2;" : "=l"(p) : "r"(w), "r"(p24));
-  return (uint32_t)(p >> 32);
 }
 
 template <typename T>
@@ -155,17 +170,21 @@ struct Layout {
   static constexpr int SCALES = TK * 8;
   static constexpr int STAGE = 2 * CODES + 2 * SCALES;
   static constexpr int RED = HB * (D + 2) * 4;     // merge buffer of a warp
+  // where piece p of key's V row is stored
+  __device__ static __forceinline__ int place(int key, int p) {
+    return D == 128 ? p ^ ((key >> 1) & 3) : D == 64 ? p ^ ((key >> 2) & 1) : p;
+  }
   static constexpr int SMEM = W * (NST * STAGE > RED ? NST * STAGE : RED);
 };
 
 template <typename T, int D, int NH>
-__global__ void __launch_bounds__(W * 32)
+__global__ void __launch_bounds__(W * 32, 4)
     kv4_split_kernel(const T* __restrict__ q, const uint8_t* __restrict__ kcodes,
                      const uint8_t* __restrict__ kscales, const uint8_t* __restrict__ vcodes,
                      const uint8_t* __restrict__ vscales, const int32_t* __restrict__ seq_lens,
                      T* __restrict__ out, float* __restrict__ part_o, float* __restrict__ part_ml,
                      int H, int G, int head_blocks, int max_splits, int chunk, float scale_log2,
-                     uint32_t p24, lpc::Kv4Rows rows) {
+                     lpc::Kv4Rows rows) {
   using L = Layout<D>;
   constexpr int CB = L::CB;
   constexpr int KW = D / 32;              // K words of a lane and key
@@ -212,13 +231,17 @@ __global__ void __launch_bounds__(W * 32)
   const uint8_t* fks = ks + (int64_t)(start + warp * TK + lane) * 8;
   const uint8_t* fvs = vs + (int64_t)(start + warp * TK + lane) * 8;
   int fleft = end - (start + warp * TK);  // keys from the next tile's first on
-  const uint32_t fdst = lpc::smem_u32(ring) + lane * 16, fdst_s = fdst - lane * 8;
+  const uint32_t ring_u = lpc::smem_u32(ring);
+  const uint32_t fdst = ring_u + lane * 16, fdst_s = fdst - lane * 8;
+  // V's 16-byte pieces are stored with their place in the row mixed with the
+  // key, so that one piece of 8 keys -- what ldmatrix reads -- lies in 32 banks
+  const uint32_t fdst_v = ring_u + L::CODES + (lane * 16 / CB) * CB + L::place(lane * 16 / CB, lane * 16 % CB / 16) * 16;
   auto fetch = [&](int to) {
     if (fleft >= TK) {
 #pragma unroll
       for (int c = 0; c < L::CODES / 512; ++c) {
         cp16(fdst + to + c * 512, fk + c * 512);
-        cp16(fdst + to + L::CODES + c * 512, fv + c * 512);
+        cp16(fdst_v + to + c * 512, fv + c * 512);
       }
       cp8(fdst_s + to + 2 * L::CODES, fks);
       cp8(fdst_s + to + 2 * L::CODES + L::SCALES, fvs);
@@ -227,7 +250,7 @@ __global__ void __launch_bounds__(W * 32)
       for (int c = 0; c < L::CODES / 512; ++c) {
         const bool ok = (c * 512 + lane * 16) / CB < fleft;
         cp16z(fdst + to + c * 512, ok ? fk + c * 512 : kc, ok);
-        cp16z(fdst + to + L::CODES + c * 512, ok ? fv + c * 512 : vc, ok);
+        cp16z(fdst_v + to + c * 512, ok ? fv + c * 512 : vc, ok);
       }
       const bool ok = lane < fleft;
       cp8z(fdst_s + to + 2 * L::CODES, ok ? fks : ks, ok);
@@ -243,13 +266,17 @@ __global__ void __launch_bounds__(W * 32)
 #pragma unroll
   for (int i = 0; i < NST - 1; ++i) fetch(i * L::STAGE);
 
-  // q as the products' column operand.  Lane (r, t) holds head r's dims of
-  // words t*KW .. t*KW + KW - 1: word w covers dims 4w..4w+3 of each group.
+  // q as the products' column operand: column c is head c, or, where at most 4
+  // heads share the KV head (NH = 1), head c / 2 of the even columns, so that
+  // each lane has one head's scores.  Lane (r, t) holds column r's dims of words
+  // t*KW .. t*KW + KW - 1: word w covers dims 4w..4w+3 of each group.
+  const int qh = NH == 1 ? r >> 1 : r;
+  const bool has_q = qh < heads && (NH == 2 || !(r & 1));
   uint32_t qb[KW][2][2];
   float qs0 = 0.f, qs1 = 0.f, amax = 0.f;
   float qv[KW][8];
   {
-    const T* qp = q + (b * H + h0 + (r < heads ? r : 0)) * D + 4 * KW * t;
+    const T* qp = q + (b * H + h0 + (has_q ? qh : 0)) * D + 4 * KW * t;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       uint32_t w[2 * KW];  // 4 KW dims
@@ -271,7 +298,7 @@ __global__ void __launch_bounds__(W * 32)
       for (int i = 0; i < 2 * KW; ++i) {
         float lo, hi;
         unpack_sm<T>(w[i], lo, hi);
-        if (r >= heads) lo = hi = 0.f;
+        if (!has_q) lo = hi = 0.f;
         qv[i / 2][g * 4 + 2 * (i & 1)] = lo;
         qv[i / 2][g * 4 + 2 * (i & 1) + 1] = hi;
         amax = fmaxf(amax, fmaxf(fabsf(lo), fabsf(hi)));
@@ -297,7 +324,7 @@ __global__ void __launch_bounds__(W * 32)
       qb[w][g][0] = pack_half2(qv[w][g * 4 + 0] * f, qv[w][g * 4 + 2] * f);
       qb[w][g][1] = pack_half2(qv[w][g * 4 + 1] * f, qv[w][g * 4 + 3] * f);
     }
-  // what this lane needs of its two score columns, heads 2t and 2t + 1
+  // what this lane needs of its score columns: head t, or heads 2t and 2t + 1
   float cs[NH], z0[NH], z1[NH], M[NH], l[NH], a0s[NH], a1s[NH];
 #pragma unroll
   for (int n = 0; n < NH; ++n) {
@@ -318,6 +345,9 @@ __global__ void __launch_bounds__(W * 32)
       for (int j = 0; j < 4; ++j) acc[g][i][j] = 0.f;
 
   constexpr uint32_t LOW = 0x000F000Fu, HIGH = 0x00F000F0u;
+  // this lane's row of the V matrices: lanes 0-7 keys 0-7 and 8-15 keys 8-15 of
+  // the first piece, 16-31 the same of the second
+  const uint32_t vsrc = (lane & 15) * CB + (D == 32 ? 0 : L::place(lane & 7, lane >> 4) * 16);
   int at = 0, to = (NST - 1) * L::STAGE;  // ring offsets of this tile and of the next fetch
   for (int left = end - (start + warp * TK); left > 0; left -= W * TK) {
     __syncwarp();  // every lane has read the stage that is filled next
@@ -325,7 +355,7 @@ __global__ void __launch_bounds__(W * 32)
     cp_wait<NST - 1>();
     __syncwarp();
     const uint8_t* sk = ring + at;
-    const uint8_t* sv = sk + L::CODES;
+    const uint32_t sv = ring_u + at + L::CODES;
     const uint8_t* sks = sk + 2 * L::CODES;
     const uint8_t* svs = sks + L::SCALES;
     at = at == (NST - 1) * L::STAGE ? 0 : at + L::STAGE;
@@ -350,12 +380,17 @@ __global__ void __launch_bounds__(W * 32)
         wa[0] = *reinterpret_cast<const uint32_t*>(pa);
         wb[0] = *reinterpret_cast<const uint32_t*>(pb);
       }
-      float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+      float c0[4], c1[4];
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const uint32_t a8 = shift8(wa[w], p24), b8 = shift8(wb[w], p24);
-        mma_f16(c0, wa[w] & LOW, wb[w] & LOW, a8 & LOW, b8 & LOW, qb[w][0][0], qb[w][0][1]);
-        mma_f16(c1, wa[w] & HIGH, wb[w] & HIGH, a8 & HIGH, b8 & HIGH, qb[w][1][0], qb[w][1][1]);
+        const uint32_t a8 = wa[w] >> 8, b8 = wb[w] >> 8;
+        if (w == 0) {
+          mma_f16_first(c0, wa[w] & LOW, wb[w] & LOW, a8 & LOW, b8 & LOW, qb[w][0][0], qb[w][0][1]);
+          mma_f16_first(c1, wa[w] & HIGH, wb[w] & HIGH, a8 & HIGH, b8 & HIGH, qb[w][1][0], qb[w][1][1]);
+        } else {
+          mma_f16(c0, wa[w] & LOW, wb[w] & LOW, a8 & LOW, b8 & LOW, qb[w][0][0], qb[w][0][1]);
+          mma_f16(c1, wa[w] & HIGH, wb[w] & HIGH, a8 & HIGH, b8 & HIGH, qb[w][1][0], qb[w][1][1]);
+        }
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -406,8 +441,9 @@ __global__ void __launch_bounds__(W * 32)
         for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int i = 0; i < VM; ++i) {
-            acc[g][i][n] *= f;
-            acc[g][i][2 + n] *= f;
+            const int c = NH == 1 ? g : n;
+            acc[g][i][c] *= f;
+            acc[g][i][2 + c] *= f;
           }
       }
     }
@@ -429,46 +465,28 @@ __global__ void __launch_bounds__(W * 32)
           a0s[n] = fmaf(p[n], m0, a0s[n]);
           a1s[n] = fmaf(p[n], m1, a1s[n]);
         }
-        pb[0][i] = transpose8(pack_half2(p[0] * s0, NH > 1 ? p[1] * s0 : 0.f));
-        pb[1][i] = transpose8(pack_half2(p[0] * s1, NH > 1 ? p[1] * s1 : 0.f));
-      }
-      // lane (r, t): keys 2t, 2t+1, 2t+8, 2t+9; for D = 128 words 2r, 2r+1
-      const uint8_t* pv = sv + (16 * u + 2 * t) * CB;
-      if constexpr (D == 32) {  // bytes 2r, 2r+1
-        const uint32_t k0 = *reinterpret_cast<const uint16_t*>(pv + 2 * r);
-        const uint32_t k1 = *reinterpret_cast<const uint16_t*>(pv + CB + 2 * r);
-        const uint32_t k2 = *reinterpret_cast<const uint16_t*>(pv + 8 * CB + 2 * r);
-        const uint32_t k3 = *reinterpret_cast<const uint16_t*>(pv + 9 * CB + 2 * r);
-        const uint32_t lo = __byte_perm(k0, k1, 0x5410), hi = __byte_perm(k2, k3, 0x5410);
-        mma_f16(acc[0][0], lo & LOW, (lo >> 8) & LOW, hi & LOW, (hi >> 8) & LOW, pb[0][0], pb[0][1]);
-        mma_f16(acc[1][0], lo & HIGH, (lo >> 8) & HIGH, hi & HIGH, (hi >> 8) & HIGH, pb[1][0],
-                pb[1][1]);
-      } else {
-        constexpr int VW = D / 64;
-        uint32_t kw[4][VW];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint8_t* p = pv + ((k & 1) + (k >> 1) * 8) * CB + r * (VW * 4);
-          if constexpr (VW == 2) {
-            const uint2 v = *reinterpret_cast<const uint2*>(p);
-            kw[k][0] = v.x;
-            kw[k][1] = v.y;
-          } else {
-            kw[k][0] = *reinterpret_cast<const uint32_t*>(p);
-          }
+        if constexpr (NH == 1) {
+          // the odd columns are free: 2t and 2t + 1 carry head t's P s0 and P s1
+          pb[0][i] = pb[1][i] = transpose8(pack_half2(p[0] * s0, p[0] * s1));
+        } else {
+          pb[0][i] = transpose8(pack_half2(p[0] * s0, p[1] * s0));
+          pb[1][i] = transpose8(pack_half2(p[0] * s1, p[1] * s1));
         }
+      }
+      // codes of keys 16u .. 16u + 15, 16 dims (8 units) of each group at a time
 #pragma unroll
-        for (int w = 0; w < VW; ++w)
+      for (int j = 0; j < VM; j += 2) {
+        uint32_t v[4];
+        const uint32_t src = sv + 16 * u * CB + (j == 0 ? vsrc : vsrc ^ 32u);
+        if constexpr (VM == 1) ldm2(v, src);
+        else ldm4(v, src);
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {  // bytes 0, 1 or 2, 3 of the word
-            const uint32_t sel = hf ? 0x7632 : 0x5410;
-            const uint32_t lo = __byte_perm(kw[0][w], kw[1][w], sel);
-            const uint32_t hi = __byte_perm(kw[2][w], kw[3][w], sel);
-            const uint32_t lo8 = shift8(lo, p24), hi8 = shift8(hi, p24);
-            mma_f16(acc[0][2 * w + hf], lo & LOW, lo8 & LOW, hi & LOW, hi8 & LOW, pb[0][0], pb[0][1]);
-            mma_f16(acc[1][2 * w + hf], lo & HIGH, lo8 & HIGH, hi & HIGH, hi8 & HIGH, pb[1][0],
-                    pb[1][1]);
-          }
+        for (int i = 0; i < (VM == 1 ? 1 : 2); ++i) {
+          const uint32_t lo = v[2 * i], hi = v[2 * i + 1];
+          const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+          mma_f16(acc[0][j + i], lo & LOW, lo8 & LOW, hi & LOW, hi8 & LOW, pb[0][0], pb[0][1]);
+          mma_f16(acc[1][j + i], lo & HIGH, lo8 & HIGH, hi & HIGH, hi8 & HIGH, pb[1][0], pb[1][1]);
+        }
       }
     }
   }
@@ -486,17 +504,18 @@ __global__ void __launch_bounds__(W * 32)
   float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
   for (int n = 0; n < NH; ++n) {
-    const int h = 2 * t + n;
+    const int h = NH == 1 ? t : 2 * t + n;
     if (h >= heads) continue;
     float* p = red + (warp * HB + h) * (D + 2);
 #pragma unroll
     for (int i = 0; i < VM; ++i) {
-      // row r of product i is dim 4 * word + 2 * half of its group, row r + 8 the next one
-      const int d = D == 32 ? 2 * r : 4 * (r * (D / 64) + (i >> 1)) + 2 * (i & 1);
+      // rows r and r + 8 of product i are the two dims of unit 8i + r
+      const int d = 2 * (8 * i + r);
+      const int n1 = NH == 1 ? 1 : n;
       p[d] = fmaf(acc[0][i][n], 16777216.f, a0s[n]);
       p[d + 1] = fmaf(acc[0][i][2 + n], 16777216.f, a0s[n]);
-      p[d + D / 2] = fmaf(acc[1][i][n], 1048576.f, a1s[n]);
-      p[d + D / 2 + 1] = fmaf(acc[1][i][2 + n], 1048576.f, a1s[n]);
+      p[d + D / 2] = fmaf(acc[1][i][n1], 1048576.f, a1s[n]);
+      p[d + D / 2 + 1] = fmaf(acc[1][i][2 + n1], 1048576.f, a1s[n]);
     }
     if (r == 0) {
       p[D] = M[n];
@@ -619,7 +638,7 @@ int launch(const lpc_kv4* kv, const void* q, const int32_t* lens, void* out, flo
                          (const uint8_t*)kv->key_codes, (const uint8_t*)kv->key_scales,
                          (const uint8_t*)kv->value_codes, (const uint8_t*)kv->value_scales, lens,
                          (T*)out, po, pml, heads, G, blocks, max_splits, chunk, scale_log2,
-                         1u << 24, rows) != cudaSuccess)
+                         rows) != cudaSuccess)
     return lpc::check_launch("decode_attention_int4 (split)");
   if ((rc = lpc::check_launch("decode_attention_int4 (split)"))) return rc;
   if (grid_splits == 1) return LPC_OK;
@@ -636,8 +655,11 @@ constexpr int64_t MAX_BATCH = 65535;
 constexpr int64_t MAX_SEQ = 65535LL * UNIT;
 constexpr int MAX_HEADS = 65535;
 
-// Split length: the longest of the candidates that still gives the launch
-// enough CTAs to fill the GPU several times over (592 run at once).
+// Split length, a multiple of UNIT: the one with the least estimated time for
+// sequences of the cache's full length.  A CTA costs its keys and about OVERHEAD
+// more (q, the pipeline's start, the merge); SLOTS run at once.  Up to four
+// rounds of CTAs count as whole rounds, beyond that the last one overlaps.
+constexpr int64_t OVERHEAD = 256, SLOTS_PER_SM = 4;
 int split_keys(const lpc_kv4* kv, int64_t batch, int heads) {
   static const int forced = [] {
     const char* e = getenv("LPC_DECODE_CHUNK");
@@ -646,10 +668,22 @@ int split_keys(const lpc_kv4* kv, int64_t batch, int heads) {
   }();
   if (forced) return forced;
   const int64_t G = heads / kv->kv_heads, blocks = (G + HB - 1) / HB;
-  const int64_t pairs = batch * kv->kv_heads * blocks;
-  for (int c : {1024, 512, 256})
-    if (pairs * (kv->max_seq_len / c) >= 2048) return c;
-  return UNIT;
+  const int64_t pairs = batch * kv->kv_heads * blocks, cap = kv->max_seq_len;
+  const int64_t slots = SLOTS_PER_SM * lpc::current_device_sms();
+  int64_t best = UNIT, cost = INT64_MAX;
+  for (int64_t n = 1; n <= 1024 && n * pairs <= 8 * slots + pairs; ++n) {
+    const int64_t chunk = ((cap + n - 1) / n + UNIT - 1) / UNIT * UNIT;
+    const int64_t ctas = pairs * ((cap + chunk - 1) / chunk);
+    const int64_t each = chunk + OVERHEAD;
+    const int64_t c = ctas <= 4 * slots ? (ctas + slots - 1) / slots * each * slots
+                                        : ctas * each + each * slots / 2;
+    if (c < cost) {
+      cost = c;
+      best = chunk;
+    }
+    if (chunk == UNIT) break;
+  }
+  return (int)best;
 }
 
 bool sizes_ok(const lpc_kv4* kv, int64_t batch, int heads) {
@@ -699,7 +733,7 @@ extern "C" int lpc_decode_attention_int4(const lpc_kv4* kv, const void* q, const
   float* pml = po ? po + batch * heads * splits * kv->head_dim : nullptr;
   const float sl2 = sm_scale * LOG2E;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool one = heads == kv->kv_heads;
+  const bool one = heads / kv->kv_heads <= 4;
 #define LPC_KV4(T, DD)                                                                            \
   return one ? launch<T, DD, 1>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits, chunk,  \
                                 sl2, s)                                                           \
