@@ -417,12 +417,14 @@ LPC_API int lpc_kv_read_int4(const lpc_kv4* kv, const int64_t* positions, void* 
  * heads, head_dim], keys [0, seq_lens[b]) of sequence b; an empty sequence
  * gives zeros, a length beyond the sequence's rows is cut to them and flagged.
  * Any number of query heads per KV head.  workspace: the split partials,
- * lpc_decode_attention_int4_workspace_bytes() bytes always suffice (NULL when
- * one split covers the cache).  One kernel then, else two.  The partials of
- * calls that overlap need workspaces of their own.
+ * lpc_decode_attention_int4_workspace_bytes() bytes (0 where one split covers
+ * the cache or a cluster merges the splits: NULL then).  Calls that overlap
+ * need workspaces of their own.
  */
 LPC_API int64_t lpc_decode_attention_int4_workspace_bytes(const lpc_kv4* kv, int64_t batch,
                                                           int heads);
+/* Kernels that a call of these sizes enqueues: 1 or 2 (0 for invalid sizes). */
+LPC_API int lpc_decode_attention_int4_kernels(const lpc_kv4* kv, int64_t batch, int heads);
 LPC_API int lpc_decode_attention_int4(const lpc_kv4* kv, const void* q, const int32_t* seq_lens,
                                       void* out, void* workspace, int64_t workspace_bytes,
                                       int64_t batch, int heads, float sm_scale, void* stream);

@@ -78,6 +78,7 @@ SIGNATURES = {
     "lpc_rope_kv_append_int4": (_I, [_P, _P, _P, _P, _P, _I64, _P, _I64, _I64, _I, _I, _P]),
     "lpc_kv_read_int4": (_I, [_P, _P, _P, _P, _I64, _I64, _P]),
     "lpc_decode_attention_int4_workspace_bytes": (_I64, [_P, _I64, _I]),
+    "lpc_decode_attention_int4_kernels": (_I, [_P, _I64, _I]),
     "lpc_decode_attention_int4": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I, _F, _P]),
     "lpc_int4_weight_bytes": (_I64, [_I64, _I, _I, _I]),
     "lpc_int4_pack": (_I, [_P, _P, _P, _P, _P]),
@@ -178,6 +179,21 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+# A Stream object costs 2 us to make; the handle alone does not.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def call_on(index: int, fn, *args) -> int:
+    """``fn(*args, stream)``: a C entry point with CUDA device ``index`` current
+    and that device's current stream as its last argument."""
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return call_on(index, fn, *args)
+    if _raw_stream is not None:
+        return fn(*args, _raw_stream(index))
+    return fn(*args, torch.cuda.current_stream(index).cuda_stream)
 
 
 def dtype_code(dt: torch.dtype, what: str) -> int:

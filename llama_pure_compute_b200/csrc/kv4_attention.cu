@@ -28,6 +28,7 @@
 // filled by cp.async, with no barrier between warps until the end; the warps
 // merge through shared memory, the splits through the workspace and a second
 // kernel (none when one split covers the cache).
+#include <algorithm>
 #include <atomic>
 #include <cstdlib>
 
@@ -49,11 +50,11 @@ namespace {
 
 using lpc::Num;
 
-constexpr int W = 4;          // warps
 constexpr int TK = 32;        // keys per warp tile
 constexpr int NST = 3;          // stages per warp
 constexpr int HB = 8;         // query heads per CTA (columns of the products)
 constexpr int UNIT = 128;     // shortest split: one tile per warp; workspace granularity
+constexpr int CLUSTER = 4;    // splits that a cluster merges
 constexpr float LOG2E = 1.4426950408889634f;
 // The reference M is set RISE below the heaviest key and moved when a key
 // exceeds it by LIFT: fp16 holds 2^(LIFT + 1), and a tile that stays below
@@ -85,6 +86,12 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -163,29 +170,29 @@ __device__ __forceinline__ float scale_exponent(uint32_t bits) {
   return fmaxf((float)((int)(bits >> 7) - 127), -60.f);
 }
 
-template <int D>
+template <int D, int W>
 struct Layout {
   static constexpr int CB = D / 2;                 // code bytes of a row
   static constexpr int CODES = TK * CB;            // of a tile, K or V
   static constexpr int SCALES = TK * 8;
   static constexpr int STAGE = 2 * CODES + 2 * SCALES;
-  static constexpr int RED = HB * (D + 2) * 4;     // merge buffer of a warp
+  static constexpr int RED = HB * (D + 2) * 4;     // merge buffer of a warp, or of the CTA
   // where piece p of key's V row is stored
   __device__ static __forceinline__ int place(int key, int p) {
     return D == 128 ? p ^ ((key >> 1) & 3) : D == 64 ? p ^ ((key >> 2) & 1) : p;
   }
-  static constexpr int SMEM = W * (NST * STAGE > RED ? NST * STAGE : RED);
+  static constexpr int SMEM = W * NST * STAGE > (W + 1) * RED ? W * NST * STAGE : (W + 1) * RED;
 };
 
-template <typename T, int D, int NH>
-__global__ void __launch_bounds__(W * 32, 4)
+template <typename T, int D, int NH, int W>
+__global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
     kv4_split_kernel(const T* __restrict__ q, const uint8_t* __restrict__ kcodes,
                      const uint8_t* __restrict__ kscales, const uint8_t* __restrict__ vcodes,
                      const uint8_t* __restrict__ vscales, const int32_t* __restrict__ seq_lens,
                      T* __restrict__ out, float* __restrict__ part_o, float* __restrict__ part_ml,
-                     int H, int G, int head_blocks, int max_splits, int chunk, float scale_log2,
-                     lpc::Kv4Rows rows) {
-  using L = Layout<D>;
+                     int H, int G, int head_blocks, int max_splits, int chunk, int cluster,
+                     float scale_log2, lpc::Kv4Rows rows) {
+  using L = Layout<D, W>;
   constexpr int CB = L::CB;
   constexpr int KW = D / 32;              // K words of a lane and key
   constexpr int VM = D / 32;              // V products per group: 16 dims each
@@ -208,6 +215,10 @@ __global__ void __launch_bounds__(W * 32, 4)
   }
   const int nsplits = len > 0 ? (len + chunk - 1) / chunk : 0;
   if (split >= nsplits) {
+    if (W == 16 && len > 0 && cluster && nsplits > 1) {  // the others read no sums of this CTA, but wait for it
+      lpc::cluster_sync();
+      lpc::cluster_sync();
+    }
     if (len <= 0 && split == 0)  // an empty context attends to nothing
       for (int i = threadIdx.x; i < heads * D; i += blockDim.x)
         out[(b * H + h0) * D + i] = Num<T>::from_f(0.f);
@@ -540,6 +551,13 @@ __global__ void __launch_bounds__(W * 32, 4)
     const int64_t bh = b * H + h0 + h;
     if (nsplits == 1) {
       out[bh * D + d] = Num<T>::from_f(Ls == 0.f ? 0.f : O / Ls);
+    } else if (W == 16 && cluster) {
+      float* p = red + (W * HB + h) * (D + 2);
+      p[d] = O;
+      if (d == 0) {
+        p[D] = Mx;
+        p[D + 1] = Ls;
+      }
     } else {
       const int64_t pi = bh * max_splits + split;
       part_o[pi * D + d] = O;
@@ -549,6 +567,40 @@ __global__ void __launch_bounds__(W * 32, 4)
       }
     }
   }
+  if (W == 4 || !cluster || nsplits == 1) return;
+  // the splits of this cluster: each CTA adds its share of the outputs over all
+  // of them through distributed shared memory, in split order
+  lpc::cluster_sync();
+  const int share = (heads * D + nsplits - 1) / nsplits;
+  for (int i = threadIdx.x; i < share; i += W * 32) {
+    const int idx = split * share + i;
+    if (idx >= heads * D) break;
+    const int h = idx / D, d = idx - h * D;
+    const uint32_t at_h = lpc::smem_u32(red + (W * HB + h) * (D + 2));
+    float Mx = -INFINITY, mv[CLUSTER], lv[CLUSTER], ov[CLUSTER];
+#pragma unroll
+    for (int s = 0; s < CLUSTER; ++s)
+      if (s < nsplits) {
+        const uint32_t p = lpc::mapa_shared(at_h, s);
+        mv[s] = ld_cluster(p + D * 4);
+        lv[s] = ld_cluster(p + D * 4 + 4);
+        ov[s] = ld_cluster(p + d * 4);
+      }
+#pragma unroll
+    for (int s = 0; s < CLUSTER; ++s)
+      if (s < nsplits) Mx = fmaxf(Mx, mv[s]);
+    const float Mu = Mx == -INFINITY ? 0.f : Mx;
+    float O = 0.f, Ls = 0.f;
+#pragma unroll
+    for (int s = 0; s < CLUSTER; ++s)
+      if (s < nsplits) {
+        const float f = fast_exp2(mv[s] - Mu);
+        O = fmaf(f, ov[s], O);
+        Ls = fmaf(f, lv[s], Ls);
+      }
+    out[(b * H + h0 + h) * D + d] = Num<T>::from_f(Ls == 0.f ? 0.f : O / Ls);
+  }
+  lpc::cluster_sync();  // no CTA leaves while its sums are read
 }
 
 // One CTA per (sequence, head).  Warp w adds the splits w, w + CWARPS, ..., the
@@ -613,35 +665,50 @@ bool use_pdl() {
   return on;
 }
 
-template <typename T, int D, int NH>
+// A cluster of up to 4 CTAs of 16 warps merges its splits in distributed shared
+// memory: 1000 keys of 32 KV heads 5.9 us against 6.7 with the second kernel, 8
+// sequences of 8,000 keys 19.4 against 21.3.  128 CTAs in such clusters fit 16
+// SMs of each of the GPU's 8 parts at once; 144 in clusters of 6 did not (74 us
+// against 41 for three sequences of 60,000).
+bool merges_in_cluster(int64_t pairs, int64_t splits) {
+  return splits > 1 && splits <= CLUSTER && pairs * splits <= 128;
+}
+
+template <typename T, int D, int NH, int W>
 int launch(const lpc_kv4* kv, const void* q, const int32_t* lens, void* out, float* po, float* pml,
            int64_t batch, int heads, int max_splits, int chunk, float scale_log2, cudaStream_t s) {
-  using L = Layout<D>;
+  using L = Layout<D, W>;
   static std::atomic<uint64_t> mask{0};
-  int rc = lpc::once_per_device_smem((const void*)kv4_split_kernel<T, D, NH>, L::SMEM, mask);
+  int rc = lpc::once_per_device_smem((const void*)kv4_split_kernel<T, D, NH, W>, L::SMEM, mask);
   if (rc) return rc;
   const int G = heads / kv->kv_heads;
   const int blocks = (G + HB - 1) / HB;
   const int grid_splits = (int)((kv->max_seq_len + chunk - 1) / chunk);
   const lpc::Kv4Rows rows = lpc::kv4_rows(kv);
-  cudaLaunchAttribute attr[1];
+  const int cluster = W == 16 && merges_in_cluster(batch * kv->kv_heads * blocks, grid_splits);
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)grid_splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid_splits, (unsigned)(kv->kv_heads * blocks), (unsigned)batch);
   cfg.blockDim = dim3(W * 32);
   cfg.dynamicSmemBytes = L::SMEM;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kv4_split_kernel<T, D, NH>, (const T*)q,
+  cfg.numAttrs = cluster ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kv4_split_kernel<T, D, NH, W>, (const T*)q,
                          (const uint8_t*)kv->key_codes, (const uint8_t*)kv->key_scales,
                          (const uint8_t*)kv->value_codes, (const uint8_t*)kv->value_scales, lens,
-                         (T*)out, po, pml, heads, G, blocks, max_splits, chunk, scale_log2,
+                         (T*)out, po, pml, heads, G, blocks, max_splits, chunk, cluster, scale_log2,
                          rows) != cudaSuccess)
     return lpc::check_launch("decode_attention_int4 (split)");
   if ((rc = lpc::check_launch("decode_attention_int4 (split)"))) return rc;
-  if (grid_splits == 1) return LPC_OK;
+  if (grid_splits == 1 || cluster) return LPC_OK;
+  cfg.numAttrs = 1;
   cfg.gridDim = dim3((unsigned)(batch * heads));
   cfg.blockDim = dim3(CWARPS * 32);
   cfg.dynamicSmemBytes = 0;
@@ -655,33 +722,58 @@ constexpr int64_t MAX_BATCH = 65535;
 constexpr int64_t MAX_SEQ = 65535LL * UNIT;
 constexpr int MAX_HEADS = 65535;
 
-// Split length, a multiple of UNIT: the one with the least estimated time for
-// sequences of the cache's full length.  A CTA costs its keys and about OVERHEAD
-// more (q, the pipeline's start, the merge); SLOTS run at once.  Up to four
-// rounds of CTAs count as whole rounds, beyond that the last one overlaps.
-constexpr int64_t OVERHEAD = 256, SLOTS_PER_SM = 4;
-int split_keys(const lpc_kv4* kv, int64_t batch, int heads) {
-  static const int forced = [] {
-    const char* e = getenv("LPC_DECODE_CHUNK");
-    const int v = e ? atoi(e) : 0;
-    return (v >= UNIT && v <= 65536 && v % UNIT == 0) ? v : 0;
-  }();
-  if (forced) return forced;
+// Split length (a multiple of UNIT) and CTA width of a launch, by the least
+// estimated time, in keys of one of the 592 four-warp CTAs that run at once (about 67
+// keys a microsecond at D = 128).  A CTA costs its keys and an overhead (q, the
+// pipeline's start, the merge); splits that no cluster merges cost the second
+// kernel, and each a little there.
+//   * 4 warps, four CTAs an SM: any number of rounds of CTAs, which overlap.  Up
+//     to four rounds count as whole rounds.  Among lengths within an eighth of the
+//     least the shortest is taken: sequences are rarely all of the full length,
+//     and short splits even them out (32 sequences of 1 to 4096 keys: 59 us with
+//     splits of 1024, 63 with 4096).
+//   * 16 warps, one CTA an SM, one round: a quarter of the splits for the same
+//     keys a warp.  Measured 16 / 4 warps, us: 1000 keys of 32 heads 5.9 / 7.6,
+//     300 keys of 4 x 32 heads 4.5 / 7.1, three sequences of 60,000 (64 heads on
+//     8) 41 / 46, one of 131,000 (32 on 8) 33 / 37.
+constexpr int64_t SLOTS_PER_SM = 4;
+int split_keys(const lpc_kv4* kv, int64_t batch, int heads, bool* wide) {
   const int64_t G = heads / kv->kv_heads, blocks = (G + HB - 1) / HB;
   const int64_t pairs = batch * kv->kv_heads * blocks, cap = kv->max_seq_len;
-  const int64_t slots = SLOTS_PER_SM * lpc::current_device_sms();
-  int64_t best = UNIT, cost = INT64_MAX;
-  for (int64_t n = 1; n <= 1024 && n * pairs <= 8 * slots + pairs; ++n) {
-    const int64_t chunk = ((cap + n - 1) / n + UNIT - 1) / UNIT * UNIT;
-    const int64_t ctas = pairs * ((cap + chunk - 1) / chunk);
-    const int64_t each = chunk + OVERHEAD;
-    const int64_t c = ctas <= 4 * slots ? (ctas + slots - 1) / slots * each * slots
-                                        : ctas * each + each * slots / 2;
-    if (c < cost) {
-      cost = c;
-      best = chunk;
+  const int64_t sms = lpc::current_device_sms(), slots = SLOTS_PER_SM * sms;
+  const int64_t overhead = G <= 4 ? 200 : 400;
+  auto joined = [](int64_t splits) { return splits > 1 ? 200 + 4 * splits : 0; };
+  auto units = [](int64_t keys) { return (keys + UNIT - 1) / UNIT * UNIT; };
+  auto estimate = [&](int64_t chunk) {
+    const int64_t splits = (cap + chunk - 1) / chunk, ctas = pairs * splits, each = chunk + overhead;
+    const int64_t t = ctas <= 4 * slots ? (ctas + slots - 1) / slots * each
+                                        : (ctas * each + each * slots / 2) / slots;
+    return t + joined(splits);
+  };
+  // 1 to 12 splits, and what fills 1 to 8 rounds
+  constexpr int CAND = 20;
+  int64_t chunks[CAND], costs[CAND], least = INT64_MAX;
+  int count = 0;
+  for (int i = 0; i < CAND; ++i) {
+    const int64_t n = i < 12 ? i + 1 : (i - 11) * slots / pairs;
+    if (n < 1 || (n > 1 && n * pairs > 8 * slots)) continue;
+    const int64_t chunk = units((cap + n - 1) / n);
+    chunks[count] = chunk;
+    costs[count] = estimate(chunk);
+    least = std::min(least, costs[count++]);
+  }
+  int64_t best = INT64_MAX;
+  for (int i = 0; i < count; ++i)
+    if (costs[i] <= least + least / 8) best = std::min(best, chunks[i]);
+  *wide = false;
+  if (pairs <= sms) {
+    const int64_t n = sms / pairs, chunk = units((cap + n - 1) / n);
+    const int64_t splits = (cap + chunk - 1) / chunk;
+    const int64_t t = chunk / 4 + 250 + (merges_in_cluster(pairs, splits) ? 80 : joined(splits));
+    if (t < least) {
+      *wide = true;
+      return (int)chunk;
     }
-    if (chunk == UNIT) break;
   }
   return (int)best;
 }
@@ -693,11 +785,37 @@ bool sizes_ok(const lpc_kv4* kv, int64_t batch, int heads) {
 
 }  // namespace
 
+namespace {
+
+struct Plan {
+  int chunk, splits;
+  bool wide, joined;  // 16-warp CTAs; splits merged by the second kernel
+};
+Plan make_plan(const lpc_kv4* kv, int64_t batch, int heads) {
+  Plan p;
+  p.chunk = split_keys(kv, batch, heads, &p.wide);
+  p.splits = (int)((kv->max_seq_len + p.chunk - 1) / p.chunk);
+  const int64_t pairs = batch * kv->kv_heads * ((heads / kv->kv_heads + HB - 1) / HB);
+  p.joined = p.splits > 1 && !(p.wide && merges_in_cluster(pairs, p.splits));
+  return p;
+}
+int64_t plan_bytes(const Plan& p, const lpc_kv4* kv, int64_t batch, int heads) {
+  return p.joined ? batch * heads * p.splits * (int64_t)(kv->head_dim + 2) * 4 : 0;
+}
+
+}  // namespace
+
 extern "C" int64_t lpc_decode_attention_int4_workspace_bytes(const lpc_kv4* kv, int64_t batch,
                                                              int heads) {
-  if (lpc::kv4_check(kv, "decode_attention_int4") || !sizes_ok(kv, batch, heads)) return 0;
-  const int64_t splits = (kv->max_seq_len + UNIT - 1) / UNIT;
-  return batch * heads * splits * (int64_t)(kv->head_dim + 2) * 4;
+  if (lpc::kv4_check(kv, "decode_attention_int4") || !sizes_ok(kv, batch, heads) || batch == 0)
+    return 0;
+  return plan_bytes(make_plan(kv, batch, heads), kv, batch, heads);
+}
+
+extern "C" int lpc_decode_attention_int4_kernels(const lpc_kv4* kv, int64_t batch, int heads) {
+  if (lpc::kv4_check(kv, "decode_attention_int4") || !sizes_ok(kv, batch, heads) || batch == 0)
+    return 0;
+  return make_plan(kv, batch, heads).joined ? 2 : 1;
 }
 
 extern "C" int lpc_decode_attention_int4(const lpc_kv4* kv, const void* q, const int32_t* seq_lens,
@@ -717,9 +835,10 @@ extern "C" int lpc_decode_attention_int4(const lpc_kv4* kv, const void* q, const
     set_error("decode_attention_int4: q, seq_lens and out must be given, q and out 16-byte aligned");
     return LPC_ERR_INVALID;
   }
-  const int chunk = split_keys(kv, batch, heads);
-  const int64_t splits = (kv->max_seq_len + chunk - 1) / chunk;
-  const int64_t need = splits > 1 ? batch * heads * splits * (int64_t)(kv->head_dim + 2) * 4 : 0;
+  const Plan plan = make_plan(kv, batch, heads);
+  const int chunk = plan.chunk;
+  const int64_t splits = plan.splits, need = plan_bytes(plan, kv, batch, heads);
+  const bool wide = plan.wide;
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
     set_error("decode_attention_int4: workspace of %lld bytes required, got %lld", (long long)need,
               (long long)workspace_bytes);
@@ -735,10 +854,14 @@ extern "C" int lpc_decode_attention_int4(const lpc_kv4* kv, const void* q, const
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool one = heads / kv->kv_heads <= 4;
 #define LPC_KV4(T, DD)                                                                            \
-  return one ? launch<T, DD, 1>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits, chunk,  \
-                                sl2, s)                                                           \
-             : launch<T, DD, 2>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits, chunk,  \
-                                sl2, s)
+  return one ? wide ? launch<T, DD, 1, 16>(kv, q, seq_lens, out, po, pml, batch, heads,           \
+                                           (int)splits, chunk, sl2, s)                            \
+                    : launch<T, DD, 1, 4>(kv, q, seq_lens, out, po, pml, batch, heads,            \
+                                          (int)splits, chunk, sl2, s)                             \
+         : wide ? launch<T, DD, 2, 16>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits,  \
+                                       chunk, sl2, s)                                             \
+                : launch<T, DD, 2, 4>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits,   \
+                                      chunk, sl2, s)
   if (kv->dtype == LPC_DTYPE_BF16) {
     if (kv->head_dim == 128) LPC_KV4(__nv_bfloat16, 128);
     if (kv->head_dim == 64) LPC_KV4(__nv_bfloat16, 64);

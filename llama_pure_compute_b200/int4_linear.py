@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _on_device, _require_cuda
+from .ops import _require_cuda
 
 __all__ = ["Int4Weight", "int4_linear", "MAX_TOKENS"]
 
@@ -134,8 +134,9 @@ class Int4Weight:
                           _lib.DTYPE_CODE[self.dtype])
         self.ref = ctypes.addressof(self._c)
         codes, scales, mins = codes.contiguous(), scales.contiguous(), mins.contiguous()
-        rc = _on_device(self.device, "lpc_int4_pack", self.ref, codes.data_ptr(), scales.data_ptr(),
-                        mins.data_ptr())
+        self.index = codes.get_device()
+        rc = _lib.call_on(self.index, lib.lpc_int4_pack, self.ref, codes.data_ptr(),
+                          scales.data_ptr(), mins.data_ptr())
         _lib.check(rc, "int4_pack")
         _lib.count_launch("lpc_int4_pack")
 
@@ -153,7 +154,7 @@ class Int4Weight:
         ``MAX_TOKENS``, whose products are library GEMMs."""
         rows = self.n_out * (2 if self.layout == "swiglu" else 1)
         out = torch.empty(rows, self.k, dtype=self.dtype, device=self.device)
-        rc = _on_device(self.device, "lpc_int4_unpack", self.ref, out.data_ptr())
+        rc = _lib.call_on(self.index, _lib.load().lpc_int4_unpack, self.ref, out.data_ptr())
         _lib.check(rc, "int4_unpack")
         _lib.count_launch("lpc_int4_unpack")
         return out
@@ -168,36 +169,40 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
     "swiglu": silu(x Wg^T) * (x Wu^T) on a weight of layout "swiglu".
     fp32 accumulation, one rounding to x's dtype.
     """
-    if epilogue not in EPILOGUES:
+    epi = EPILOGUES.get(epilogue)
+    if epi is None:
         raise ValueError(f"LlamaPureComputeError: unknown epilogue {epilogue!r}")
-    if (epilogue == "swiglu") != (w.layout == "swiglu"):
+    if (epi == 2) != (w.layout == "swiglu"):
         raise ValueError("LlamaPureComputeError: the swiglu epilogue needs a swiglu-packed weight.")
     _require_cuda(x, "x")
-    k, n = w.k, w.n_out
-    if x.dim() == 0 or x.shape[-1] != k or x.dtype != w.dtype or x.device != w.device:
+    k, n, index = w.k, w.n_out, w.index
+    shape = x.shape
+    if not shape or shape[-1] != k or x.dtype != w.dtype or x.get_device() != index:
         raise ValueError("LlamaPureComputeError: x must be [..., k] in the weight's dtype and device.")
-    x2 = x.contiguous()
-    tokens = x2.numel() // k
+    if not x.is_contiguous():
+        x = x.contiguous()
+    tokens = x.numel() // k
     if tokens > MAX_TOKENS:
         raise ValueError(f"LlamaPureComputeError: int4_linear takes at most {MAX_TOKENS} rows.")
     rp = None
-    if epilogue == "residual":
+    if epi == 1:
         if resid is None or resid.numel() != tokens * n or not resid.is_contiguous() \
-                or resid.dtype != x.dtype or resid.device != x.device:
+                or resid.dtype != x.dtype or resid.get_device() != index:
             raise ValueError("LlamaPureComputeError: residual must be a contiguous [..., n_out] tensor.")
         rp = resid.data_ptr()
     elif resid is not None:
         raise ValueError("LlamaPureComputeError: resid is for the residual epilogue.")
+    xp = x.data_ptr()
     if out is None:
-        out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+        out = x.new_empty((*shape[:-1], n))
     elif out.numel() != tokens * n or not out.is_contiguous() or out.dtype != x.dtype \
-            or out.device != x.device:
+            or out.get_device() != index:
         raise ValueError("LlamaPureComputeError: out must be a contiguous [..., n_out] tensor.")
-    elif out.data_ptr() == x2.data_ptr() and tokens:
+    elif out.data_ptr() == xp and tokens:
         raise ValueError("LlamaPureComputeError: out must not be x.")
-    rc = _on_device(w.device, "lpc_int4_linear", w.ref, x2.data_ptr(), out.data_ptr(), rp, tokens,
-                    EPILOGUES[epilogue])
-    _lib.check(rc, "int4_linear")
+    rc = _lib.call_on(index, _lib.load().lpc_int4_linear, w.ref, xp, out.data_ptr(), rp, tokens, epi)
+    if rc:
+        _lib.check(rc, "int4_linear")
     if tokens:
         _lib.count_launch("lpc_int4_linear")
     return out

@@ -587,7 +587,8 @@ class Int4KV:
     """
 
     __slots__ = ("key_codes", "key_scales", "value_codes", "value_scales", "seq_base", "seq_cap",
-                 "max_seq_len", "kv_heads", "head_dim", "dtype", "device", "max_batch", "_c", "ref")
+                 "max_seq_len", "kv_heads", "head_dim", "dtype", "device", "index", "max_batch",
+                 "_c", "ref", "_kernels")
 
     def __init__(self, key_codes: torch.Tensor, key_scales: torch.Tensor,
                  value_codes: torch.Tensor, value_scales: torch.Tensor,
@@ -640,11 +641,13 @@ class Int4KV:
         self.value_codes, self.value_scales = value_codes, value_scales
         self.seq_base, self.seq_cap = seq_base, seq_cap
         self.device = key_codes.device
+        self.index = key_codes.get_device()
         self._c = _lib.Kv4(key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(),
                            value_scales.data_ptr(), _lib.ptr(seq_base), _lib.ptr(seq_cap),
                            self.max_batch, self.max_seq_len, total_rows, self.kv_heads,
                            self.head_dim, _lib.DTYPE_CODE[self.dtype], 0)
         self.ref = ctypes.addressof(self._c)
+        self._kernels = {}  # (batch, heads) -> kernels of an attention call
 
     @classmethod
     def empty(cls, max_batch: int, kv_heads: int, max_seq_len: int, head_dim: int,
@@ -692,36 +695,25 @@ class Int4KV:
                       seq_base, seq_cap, self.max_seq_len)
 
 
-def _on_device(device: torch.device, name: str, *args) -> int:
-    """Calls a C entry point, its stream argument appended, with the tensors'
-    device current."""
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == device.index:
-        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    with torch.cuda.device(device):
-        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
-
-
-def _int4_out(out: Optional[torch.Tensor], name: str, shape, kv: Int4KV) -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=kv.dtype, device=kv.device)
-    if out.shape != torch.Size(shape) or out.dtype != kv.dtype or out.device != kv.device \
+def _int4_out(out: torch.Tensor, name: str, shape, kv: Int4KV) -> None:
+    if out.shape != torch.Size(shape) or out.dtype != kv.dtype or out.get_device() != kv.index \
             or not out.is_contiguous():
         raise ValueError(f"LlamaPureComputeError: {name} must be a contiguous {tuple(shape)} tensor "
                          "of the cache's dtype and device.")
-    return out
 
 
 def _int4_positions(positions: torch.Tensor, B: int, S: int, kv: Int4KV) -> torch.Tensor:
-    if tuple(positions.shape) != (B, S):
+    if positions.dim() != 2 or positions.shape[0] != B or positions.shape[1] != S:
         raise ValueError("LlamaPureComputeError: positions must be [batch, seq].")
-    if positions.device != kv.device:
+    if positions.get_device() != kv.index:
         raise ValueError("LlamaPureComputeError: positions must be on the cache's device.")
-    if positions.dtype.is_floating_point or positions.dtype == torch.bool:
-        raise TypeError("LlamaPureComputeError: positions must be integers.")
     if B > kv.max_batch:
         raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
-    return positions.to(torch.int64).contiguous()
+    if positions.dtype is not torch.int64:
+        if positions.dtype.is_floating_point or positions.dtype == torch.bool:
+            raise TypeError("LlamaPureComputeError: positions must be integers.")
+        positions = positions.to(torch.int64)
+    return positions.contiguous()
 
 
 def rope_kv_append_int4(
@@ -752,7 +744,8 @@ def rope_kv_append_int4(
     B, S, _ = qkv.shape
     if qkv.dtype != kv.dtype:
         raise TypeError("LlamaPureComputeError: qkv and cache dtypes differ.")
-    if qkv.device != kv.device or cos_table.device != kv.device or sin_table.device != kv.device:
+    if qkv.get_device() != kv.index or cos_table.get_device() != kv.index \
+            or sin_table.get_device() != kv.index:
         raise ValueError("LlamaPureComputeError: qkv and the rope tables must be on the cache's device.")
     if cos_table.dim() != 2 or cos_table.shape[-1] != D or sin_table.shape != cos_table.shape \
             or sin_table.dtype != cos_table.dtype:
@@ -760,12 +753,16 @@ def rope_kv_append_int4(
     pos = _int4_positions(positions, B, S, kv)
     qkv = qkv.contiguous()
     cos_table, sin_table = cos_table.contiguous(), sin_table.contiguous()
-    q_out = _int4_out(q_out, "q_out", (B, num_heads, S, D), kv)
-    rc = _on_device(kv.device, "lpc_rope_kv_append_int4", kv.ref, qkv.data_ptr(), pos.data_ptr(),
-                    cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0],
-                    q_out.data_ptr(), B, S, num_heads,
-                    _lib.dtype_code(cos_table.dtype, "rope_kv_append_int4"))
-    _lib.check(rc, "rope_kv_append_int4")
+    if q_out is None:
+        q_out = qkv.new_empty((B, num_heads, S, D))
+    else:
+        _int4_out(q_out, "q_out", (B, num_heads, S, D), kv)
+    rc = _lib.call_on(kv.index, _lib.load().lpc_rope_kv_append_int4, kv.ref, qkv.data_ptr(),
+                      pos.data_ptr(), cos_table.data_ptr(), sin_table.data_ptr(),
+                      cos_table.shape[0], q_out.data_ptr(), B, S, num_heads,
+                      _lib.dtype_code(cos_table.dtype, "rope_kv_append_int4"))
+    if rc:
+        _lib.check(rc, "rope_kv_append_int4")
     if B and S:
         _lib.count_launch("lpc_rope_kv_append_int4")
     return q_out
@@ -788,11 +785,18 @@ def kv_read_int4(
     B, S = positions.shape
     pos = _int4_positions(positions, B, S, kv)
     shape = (B, kv.kv_heads, S, kv.head_dim)
-    k_out = _int4_out(k_out, "k_out", shape, kv)
-    v_out = _int4_out(v_out, "v_out", shape, kv)
-    rc = _on_device(kv.device, "lpc_kv_read_int4", kv.ref, pos.data_ptr(), k_out.data_ptr(),
-                    v_out.data_ptr(), B, S)
-    _lib.check(rc, "kv_read_int4")
+    if k_out is None:
+        k_out = kv.key_scales.new_empty(shape)
+    else:
+        _int4_out(k_out, "k_out", shape, kv)
+    if v_out is None:
+        v_out = kv.key_scales.new_empty(shape)
+    else:
+        _int4_out(v_out, "v_out", shape, kv)
+    rc = _lib.call_on(kv.index, _lib.load().lpc_kv_read_int4, kv.ref, pos.data_ptr(),
+                      k_out.data_ptr(), v_out.data_ptr(), B, S)
+    if rc:
+        _lib.check(rc, "kv_read_int4")
     if B and S:
         _lib.count_launch("lpc_kv_read_int4")
     return k_out, v_out
@@ -835,19 +839,26 @@ def decode_attention_int4(
         raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
     if seq_lens.numel() < B or not seq_lens.is_contiguous():
         raise ValueError("LlamaPureComputeError: seq_lens must have a contiguous entry per sequence.")
-    if q.device != kv.device or seq_lens.device != kv.device:
+    if q.get_device() != kv.index or seq_lens.get_device() != kv.index:
         raise ValueError("LlamaPureComputeError: q and seq_lens must be on the cache's device.")
     qc = q.contiguous()
-    out = _int4_out(out, "out", q.shape, kv)
+    if out is None:
+        out = torch.empty_like(qc)
+    else:
+        _int4_out(out, "out", q.shape, kv)
+    lib = _lib.load()
     if workspace is None:
         workspace = decode_attention_int4_workspace(kv, B, H)
-    elif workspace.device != kv.device or not workspace.is_contiguous():
+    elif workspace.get_device() != kv.index or not workspace.is_contiguous():
         raise ValueError("LlamaPureComputeError: workspace must be contiguous on the cache's device.")
-    rc = _on_device(kv.device, "lpc_decode_attention_int4", kv.ref, qc.data_ptr(),
-                    seq_lens.data_ptr(), out.data_ptr(), workspace.data_ptr(),
-                    workspace.numel() * workspace.element_size(), B, H,
-                    D ** -0.5 if sm_scale is None else float(sm_scale))
-    _lib.check(rc, "decode_attention_int4")
+    rc = _lib.call_on(kv.index, lib.lpc_decode_attention_int4, kv.ref, qc.data_ptr(),
+                      seq_lens.data_ptr(), out.data_ptr(), workspace.data_ptr(), workspace.nbytes,
+                      B, H, D ** -0.5 if sm_scale is None else sm_scale)
+    if rc:
+        _lib.check(rc, "decode_attention_int4")
     if B:
-        _lib.count_launch("lpc_decode_attention_int4")
+        n = kv._kernels.get((B, H))
+        if n is None:
+            n = kv._kernels[B, H] = lib.lpc_decode_attention_int4_kernels(kv.ref, B, H)
+        _lib.count_launch("lpc_decode_attention_int4", n)
     return out
