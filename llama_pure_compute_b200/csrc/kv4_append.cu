@@ -4,7 +4,7 @@
 // rotated and rounded to the data type as the 16-bit append does, v as given,
 // both held as
 //   m = min of the group,  s = T(fl(fl(max - min) / 15)),
-//   c = clamp(rint(fl(fl(x - m) * fl(1 / s))), 0, 15),
+//   c = rint(clamp(fl(fl(x - m) * fl(1 / s)), 0, 15)),
 // every operation one fp32 rounding, so that the same bytes come out of any
 // correct evaluation.  m is exact in T.  A scale below 2^-126 (whose inverse
 // fp32 does not hold) becomes 0 and its codes 0; a group with a non-finite
@@ -69,62 +69,114 @@ namespace {
 
 using lpc::Num;
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-  float d;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-
+// Pairs of T as they lie in a 32-bit word; a NaN wins.
 template <typename T>
-__device__ __forceinline__ void unpack8(uint4 u, float (&f)[8]) {
-  const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = Num<T>::to_f(e[i]);
-}
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t min(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ float lo(uint32_t w) { return lpc::bf16lo(w); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return lpc::bf16hi(w); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ uint32_t min(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ float lo(uint32_t w) {
+    return __half2float(__ushort_as_half((unsigned short)w));
+  }
+  static __device__ __forceinline__ float hi(uint32_t w) {
+    return __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint4 u;
-  T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = Num<T>::from_f(f[i]);
-  return u;
-}
-template <typename TT>
-__device__ __forceinline__ void load8(const TT* p, float (&f)[8]) {
-  if constexpr (sizeof(TT) == 4) {
-    const uint4 a = lpc::ld_dep16(p), b = lpc::ld_dep16(p + 4);
-    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
-  } else {
-    unpack8<TT>(lpc::ld_dep16(p), f);
-  }
+  return make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]),
+                    Pair<T>::pack(f[6], f[7]));
 }
 
-// Scale, minimum (as T) and the factor that turns x - m into a code.
+// 8 table entries: as they lie (16 bits), or fp32.
+template <typename TT>
+struct Entries {
+  uint32_t w[sizeof(TT) * 2];
+  __device__ __forceinline__ void load(const TT* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(TT) / 2; ++i) {
+      const uint4 v = lpc::ld_dep16(p + 4 * i);
+      w[4 * i] = v.x;
+      w[4 * i + 1] = v.y;
+      w[4 * i + 2] = v.z;
+      w[4 * i + 3] = v.w;
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(TT) == 4) return __uint_as_float(w[i]);
+    else return i & 1 ? Pair<TT>::hi(w[i / 2]) : Pair<TT>::lo(w[i / 2]);
+  }
+};
+
+// a * b + c * d (c * d subtracted where MINUS), each operation rounded once.
+// Products of two 16-bit numbers are exact in fp32, so that the sum may be an FMA.
+template <bool EXACT, bool MINUS>
+__device__ __forceinline__ float rot(float a, float b, float c, float d) {
+  const float p = __fmul_rn(c, d);
+  if constexpr (EXACT) return __fmaf_rn(a, b, MINUS ? -p : p);
+  else return MINUS ? __fsub_rn(__fmul_rn(a, b), p) : __fadd_rn(__fmul_rn(a, b), p);
+}
+
+// d / 15, correctly rounded: one step on the product with the rounded inverse.
+// Checked against the division for every significand; d below 2^-100, where the
+// remainder loses bits, takes the division.
+__device__ __forceinline__ float over15(float d) {
+  if (d < 0x1p-100f) return __fdiv_rn(d, 15.f);
+  const float inv = 1.f / 15.f;
+  const float q = __fmul_rn(d, inv);
+  return __fmaf_rn(__fmaf_rn(-15.f, q, d), inv, q);
+}
+
+// Scale (as T) of a group and the factor that turns x - min into a code; NaN
+// and 0 where the group has no finite scale.
 template <typename T>
-__device__ __forceinline__ void group_numbers(float lo, float hi, T& s, T& m, float& inv) {
-  s = Num<T>::from_f(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
-  m = Num<T>::from_f(lo);
+__device__ __forceinline__ void group_numbers(float lo, float hi, T& s, float& inv) {
+  s = Num<T>::from_f(over15(__fsub_rn(hi, lo)));
   const float sf = Num<T>::to_f(s);
   inv = 0.f;
-  if (!(sf < INFINITY)) {
-    s = m = Num<T>::from_f(__int_as_float(0x7fffffff));
-  } else if (sf < 1.17549435e-38f) {
-    s = Num<T>::from_f(0.f);
-  } else {
-    inv = __frcp_rn(sf);
-  }
+  if (!(sf < INFINITY)) s = Num<T>::from_f(__int_as_float(0x7fffffff));
+  else if (sf < 1.17549435e-38f) s = Num<T>::from_f(0.f);
+  else inv = __frcp_rn(sf);
 }
 
-__device__ __forceinline__ uint32_t code_of(float x, float m, float inv) {
-  const float t = __fmul_rn(__fsub_rn(x, m), inv);
-  return (uint32_t)__float2int_rn(fminf(fmaxf(t, 0.f), 15.f));
+// rint(clamp((x - lo) * inv)) in the low bits of an fp32 number: adding 1.5 * 2^23
+// rounds to an integer, halves to even.  x >= lo, so that only the upper end clamps.
+__device__ __forceinline__ uint32_t code_bits(float x, float lo, float inv) {
+  const float t = __fmul_rn(__fsub_rn(x, lo), inv);
+  return __float_as_uint(__fadd_rn(fminf(t, 15.f), 12582912.f));
 }
 
 constexpr int THREADS = 256;
@@ -132,11 +184,13 @@ constexpr int THREADS = 256;
 // One CTA: one token, K * (threads / chunks) of its heads; thread t owns chunk
 // t % chunks of head t / chunks + k * hpb, as in the 16-bit append.
 template <typename T, typename TT, int D, int K>
-__global__ void __launch_bounds__(THREADS) kv4_append_kernel(
-    const T* __restrict__ qkv, const int64_t* __restrict__ positions, const TT* __restrict__ cosb,
-    const TT* __restrict__ sinb, int64_t table_rows, T* __restrict__ q_out, uint8_t* kcodes,
-    uint8_t* kscales, uint8_t* vcodes, uint8_t* vscales, int64_t seq, int H, lpc::Kv4Rows rows) {
+__global__ void __launch_bounds__(THREADS, sizeof(TT) == 2 ? 4 : 3) kv4_append_kernel(
+    const T* qkv, const int64_t* positions, const TT* cosb, const TT* sinb, int64_t table_rows,
+    T* q_out, uint8_t* kcodes, uint8_t* kscales, uint8_t* vcodes, uint8_t* vscales, int64_t seq,
+    int H, lpc::Kv4Rows rows) {
   constexpr int C = D / 16;  // threads of a row
+  constexpr bool EXACT = sizeof(TT) == 2;
+  using P = Pair<T>;
   lpc::pdl_trigger();
   lpc::pdl_wait();
   const int Hkv = rows.kv_heads;
@@ -146,104 +200,112 @@ __global__ void __launch_bounds__(THREADS) kv4_append_kernel(
   const int c = (int)threadIdx.x % C;
   const int hh0 = (int)threadIdx.x / C + (int)blockIdx.y * K * hpb;
   const int d = c * 8;
-  const T* src = qkv + tok * (int64_t)all * D + d;
+  const T* src = qkv + (tok * all + hh0) * D + d;
   uint4 x0[K], x1[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int hh = hh0 + k * hpb;
     x0[k] = x1[k] = make_uint4(0u, 0u, 0u, 0u);
-    if (hh < all) {
-      const T* p = src + (int64_t)hh * D;
-      x0[k] = lpc::ld_dep16(p);
-      x1[k] = lpc::ld_dep16(p + D / 2);
+    if (hh0 + k * hpb < all) {
+      x0[k] = lpc::ld_dep16(src + k * hpb * D);
+      x1[k] = lpc::ld_dep16(src + k * hpb * D + D / 2);
     }
   }
   const int64_t pos = lpc::ld_dep(positions + tok);
   const int64_t b = tok / seq;
-  const int64_t q_row = b * H * seq + (tok - b * seq);  // q_out row of (b, head 0, s)
+  T* qdst = q_out + ((b * H + hh0) * seq + (tok - b * seq)) * D + d;
   int64_t row0 = 0, head_rows = 0, cap = 0;
   const bool inside = rows.locate(b, &row0, &head_rows, &cap);
   if (pos < 0 || !inside || pos >= cap || pos >= table_rows) {  // the same for the whole CTA
     if (pos >= 0 && threadIdx.x == 0) atomicOr(&g_kv4_append_status, LPC_DEV_ERR_BOUNDS);
     // a skipped token leaves the cache as it is; its q rows become zero
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int hh = hh0 + k * hpb;
-      if (hh < H) {
-        T* dst = q_out + (q_row + (int64_t)hh * seq) * D + d;
+    for (int k = 0; k < K; ++k)
+      if (hh0 + k * hpb < H) {
+        T* dst = qdst + (int64_t)k * hpb * seq * D;
         *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
         *reinterpret_cast<uint4*>(dst + D / 2) = make_uint4(0u, 0u, 0u, 0u);
       }
-    }
     return;
   }
-  float c0[8], s0[8], c1[8], s1[8];
+  Entries<TT> c0, s0, c1, s1;
   if (hh0 < H + Hkv) {  // the thread's first head is its lowest; v heads are not rotated
     const TT* cr = cosb + pos * D + d;
     const TT* sr = sinb + pos * D + d;
-    load8<TT>(cr, c0);
-    load8<TT>(sr, s0);
-    load8<TT>(cr + D / 2, c1);
-    load8<TT>(sr + D / 2, s1);
+    c0.load(cr);
+    s0.load(sr);
+    c1.load(cr + D / 2);
+    s1.load(sr + D / 2);
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int hh = hh0 + k * hpb;
-    uint4 u0 = x0[k], u1 = x1[k];
-    float a0[8], a1[8];
-    unpack8<T>(u0, a0);
-    unpack8<T>(u1, a1);
+    uint32_t a0[4] = {x0[k].x, x0[k].y, x0[k].z, x0[k].w};
+    uint32_t a1[4] = {x1[k].x, x1[k].y, x1[k].z, x1[k].w};
     if (hh < H + Hkv) {
-      float o0[8], o1[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        o0[i] = __fsub_rn(__fmul_rn(a0[i], c0[i]), __fmul_rn(a1[i], s0[i]));
-        o1[i] = __fadd_rn(__fmul_rn(a1[i], c1[i]), __fmul_rn(a0[i], s1[i]));
+      for (int i = 0; i < 4; ++i) {
+        float o0[2], o1[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float f0 = j ? P::hi(a0[i]) : P::lo(a0[i]), f1 = j ? P::hi(a1[i]) : P::lo(a1[i]);
+          const int e = 2 * i + j;
+          o0[j] = rot<EXACT, true>(f0, c0.at(e), f1, s0.at(e));
+          o1[j] = rot<EXACT, false>(f1, c1.at(e), f0, s1.at(e));
+        }
+        a0[i] = P::pack(o0[0], o0[1]);  // the values that the 16-bit cache would hold
+        a1[i] = P::pack(o1[0], o1[1]);
       }
-      u0 = pack8<T>(o0);
-      u1 = pack8<T>(o1);
       if (hh < H) {
-        T* dst = q_out + (q_row + (int64_t)hh * seq) * D + d;
-        *reinterpret_cast<uint4*>(dst) = u0;
-        *reinterpret_cast<uint4*>(dst + D / 2) = u1;
+        T* dst = qdst + (int64_t)k * hpb * seq * D;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(a0[0], a0[1], a0[2], a0[3]);
+        *reinterpret_cast<uint4*>(dst + D / 2) = make_uint4(a1[0], a1[1], a1[2], a1[3]);
       }
-      unpack8<T>(u0, a0);  // the values that the 16-bit cache would hold
-      unpack8<T>(u1, a1);
     }
     if (!__any_sync(0xffffffffu, hh >= H && hh < all)) continue;
-    float lo0 = a0[0], hi0 = a0[0], lo1 = a1[0], hi1 = a1[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-      lo0 = min_nan(lo0, a0[i]);
-      hi0 = max_nan(hi0, a0[i]);
-      lo1 = min_nan(lo1, a1[i]);
-      hi1 = max_nan(hi1, a1[i]);
-    }
+    // min and max of both groups, group 0 in the low half of the words
+    const uint32_t m0 = P::min(P::min(a0[0], a0[1]), P::min(a0[2], a0[3]));
+    const uint32_t m1 = P::min(P::min(a1[0], a1[1]), P::min(a1[2], a1[3]));
+    const uint32_t M0 = P::max(P::max(a0[0], a0[1]), P::max(a0[2], a0[3]));
+    const uint32_t M1 = P::max(P::max(a1[0], a1[1]), P::max(a1[2], a1[3]));
+    uint32_t mn = P::min(__byte_perm(m0, m1, 0x5410), __byte_perm(m0, m1, 0x7632));
+    uint32_t mx = P::max(__byte_perm(M0, M1, 0x5410), __byte_perm(M0, M1, 0x7632));
 #pragma unroll
     for (int o = 1; o < C; o <<= 1) {
-      lo0 = min_nan(lo0, __shfl_xor_sync(0xffffffffu, lo0, o));
-      hi0 = max_nan(hi0, __shfl_xor_sync(0xffffffffu, hi0, o));
-      lo1 = min_nan(lo1, __shfl_xor_sync(0xffffffffu, lo1, o));
-      hi1 = max_nan(hi1, __shfl_xor_sync(0xffffffffu, hi1, o));
+      mn = P::min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = P::max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     }
     if (hh < H || hh >= all) continue;
+    const float lo0 = P::lo(mn), lo1 = P::hi(mn);
     __align__(8) T sc[4];
     float i0, i1;
-    group_numbers<T>(lo0, hi0, sc[0], sc[1], i0);
-    group_numbers<T>(lo1, hi1, sc[2], sc[3], i1);
-    uint32_t w[2] = {0u, 0u};
+    group_numbers<T>(lo0, P::lo(mx), sc[0], i0);
+    group_numbers<T>(lo1, P::hi(mx), sc[2], i1);
+    const bool bad0 = sc[0] != sc[0], bad1 = sc[2] != sc[2];
+    sc[1] = bad0 ? sc[0] : Num<T>::from_f(lo0);
+    sc[3] = bad1 ? sc[2] : Num<T>::from_f(lo1);
+    uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t byte = code_of(a0[i], lo0, i0) | code_of(a1[i], lo1, i1) << 4;
-      w[i >> 2] |= byte << (8 * (i & 3));
+    for (int i = 0; i < 2; ++i) {
+      uint32_t byte[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t f0 = a0[2 * i + j / 2], f1 = a1[2 * i + j / 2];
+        // the low bits of b1 * 16 + b0: the constant's share of them is 0
+        byte[j] = code_bits(j & 1 ? P::hi(f1) : P::lo(f1), lo1, i1) * 16u +
+                  code_bits(j & 1 ? P::hi(f0) : P::lo(f0), lo0, i0);
+      }
+      w[i] = __byte_perm(__byte_perm(byte[0], byte[1], 0x0040), __byte_perm(byte[2], byte[3], 0x0040),
+                         0x5410);
+      // fminf took a NaN for 15: a group without a scale has codes 0
+      if (bad0) w[i] &= 0xF0F0F0F0u;
+      if (bad1) w[i] &= 0x0F0F0F0Fu;
     }
     const bool key = hh < H + Hkv;
     const int64_t row = row0 + pos + (int64_t)(hh - H - (key ? 0 : Hkv)) * head_rows;
-    uint8_t* codes = key ? kcodes : vcodes;
-    uint8_t* scales = key ? kscales : vscales;
-    *reinterpret_cast<uint2*>(codes + row * (D / 2) + d) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>((key ? kcodes : vcodes) + row * (D / 2) + d) = make_uint2(w[0], w[1]);
     if (c == 0)
-      *reinterpret_cast<uint2*>(scales + row * 8) = *reinterpret_cast<const uint2*>(sc);
+      *reinterpret_cast<uint2*>((key ? kscales : vscales) + row * 8) =
+          *reinterpret_cast<const uint2*>(sc);
   }
 }
 

@@ -476,6 +476,16 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
           a0s[n] = fmaf(p[n], m0, a0s[n]);
           a1s[n] = fmaf(p[n], m1, a1s[n]);
         }
+        if constexpr (std::is_same<T, __half>::value) {
+          // an fp16 output shows the rounding of P s to fp16, which the products
+          // take times a code; with 8 times it taken out, times a code - 8
+#pragma unroll
+          for (int n = 0; n < NH; ++n) {
+            const float e0 = p[n] * s0, e1 = p[n] * s1;
+            a0s[n] = fmaf(8.f, e0 - __half2float(__float2half_rn(e0)), a0s[n]);
+            a1s[n] = fmaf(8.f, e1 - __half2float(__float2half_rn(e1)), a1s[n]);
+          }
+        }
         if constexpr (NH == 1) {
           // the odd columns are free: 2t and 2t + 1 carry head t's P s0 and P s1
           pb[0][i] = pb[1][i] = transpose8(pack_half2(p[0] * s0, p[0] * s1));
