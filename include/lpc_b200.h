@@ -458,10 +458,15 @@ LPC_API int lpc_int4_unpack(const lpc_w4* w, void* out, void* stream);
 /*
  * out[t, n] = epilogue(sum_k x[t, k] * W[n, k]) for x [tokens, k], tokens <= 64:
  * epilogue 0 store, 1 resid + (resid may equal out), 2 silu(gate) * up (layout 1
- * and only it).  fp32 accumulation, one rounding.  No workspace.
+ * and only it).  fp32 accumulation, one rounding.  workspace:
+ * lpc_int4_linear_workspace_bytes() bytes (0 for fp16 and wherever up to 8 tokens
+ * of x fit shared memory: NULL then); calls that overlap need one each.  One
+ * kernel, two where the workspace is used.
  */
+LPC_API int64_t lpc_int4_linear_workspace_bytes(const lpc_w4* w, int64_t tokens);
 LPC_API int lpc_int4_linear(const lpc_w4* w, const void* x, void* out, const void* resid,
-                            int64_t tokens, int epilogue, void* stream);
+                            int64_t tokens, int epilogue, void* workspace, int64_t workspace_bytes,
+                            void* stream);
 
 /*
  * HBM read-rate probe (a measurement utility; no reference counterpart).

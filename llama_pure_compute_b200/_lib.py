@@ -83,7 +83,8 @@ SIGNATURES = {
     "lpc_int4_weight_bytes": (_I64, [_I64, _I, _I, _I]),
     "lpc_int4_pack": (_I, [_P, _P, _P, _P, _P]),
     "lpc_int4_unpack": (_I, [_P, _P, _P]),
-    "lpc_int4_linear": (_I, [_P, _P, _P, _P, _I64, _I, _P]),
+    "lpc_int4_linear_workspace_bytes": (_I64, [_P, _I64]),
+    "lpc_int4_linear": (_I, [_P, _P, _P, _P, _I64, _I, _P, _I64, _P]),
     "lpc_hbm_read_probe": (_I, [_P, _I64, _P]),
 }
 
@@ -98,7 +99,7 @@ KERNELS_PER_CALL = {
     "lpc_pack_weights": 1, "lpc_wsgemm": 1, "lpc_qkv_rope_append": 1, "lpc_rope_kv_append_ragged": 1,
     "lpc_decode_attention_ragged": 2, "lpc_rmsswiglu_folded_forward": 1, "lpc_hbm_read_probe": 1,
     "lpc_rope_kv_append_int4": 1, "lpc_kv_read_int4": 1, "lpc_decode_attention_int4": 2,
-    "lpc_int4_pack": 2, "lpc_int4_unpack": 1, "lpc_int4_linear": 1,
+    "lpc_int4_pack": 3, "lpc_int4_unpack": 1, "lpc_int4_linear": 1,
 }
 launch_count = 0
 

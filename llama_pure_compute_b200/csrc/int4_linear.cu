@@ -30,7 +30,7 @@
 #include <atomic>
 #include <cstdlib>
 
-#include "lpc_common.cuh"
+#include "int4.cuh"
 
 namespace {
 
@@ -50,46 +50,22 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                    uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __half>::value)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                    uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The 8 codes of a word as the A operand: rows r, r + 8 of columns 2t.., then
-// the same rows of columns 2t + 8...  The bf16 shifts are products by a power
-// of two that the compiler does not see (`sh` = 2^28): LOP3 and SHF share the
-// half-rate ALU pipe, which 7 of them a word would fill, the products run on
-// the FMA pipe beside it.
-__device__ __forceinline__ uint32_t shift4(uint32_t w, uint32_t sh) {
-  uint64_t p;
-  asm("mul.wide.u32 %0, %1, %2;" : "=l"(p) : "r"(w), "r"(sh));
-  return (uint32_t)(p >> 32);
-}
-template <typename T>
-__device__ __forceinline__ void operand(uint32_t w, uint32_t sh, uint32_t (&a)[4]) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const uint32_t v = w >> 8;
-    a[0] = w & 0x000F000Fu;
-    a[1] = w & 0x00F000F0u;
-    a[2] = v & 0x000F000Fu;
-    a[3] = v & 0x00F000F0u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = (w & 0x000F000Fu) | 0x43004300u;
-      if (i < 3) w = shift4(w, sh);
-    }
-  }
+// The 8 codes of a word as the A operand: rows r, r + 8 (16-fold) of columns
+// 2t.., then the same rows of columns 2t + 8...  Code c of row r is the subnormal c * 2^-24.
+__device__ __forceinline__ void operand(uint32_t w, uint32_t (&a)[4]) {
+  const uint32_t v = w >> 8;
+  a[0] = w & 0x000F000Fu;
+  a[1] = w & 0x00F000F0u;
+  a[2] = v & 0x000F000Fu;
+  a[3] = v & 0x00F000F0u;
 }
 
 template <typename T>
@@ -100,245 +76,7 @@ __device__ __forceinline__ float2 pair_f(uint32_t w) {
     return make_float2(lpc::bf16lo(w), lpc::bf16hi(w));
 }
 
-template <int GS, int MT, int NT, int NW>
-struct Cfg {
-  static constexpr int CK = GS > 64 ? GS : 64;  // columns of a pipeline stage
-  static constexpr int TILES = CK / 64;
-  static constexpr int SG = CK / GS;            // groups of a stage
-  static constexpr int STAGE = MT * (TILES * 512 + SG * 256);
-  static constexpr int NST = (MT * TILES == 4 ? 4 : MT * TILES == 2 ? 8 : 12) * 8 / NW + (NW > 8);
-  static constexpr int RING = NST * STAGE;
-  static constexpr int RED = MT * 16 * NT * 8;  // fp32 partial sums of a warp
-  static constexpr int SMEM = NW * (RING + 2 * RED * 4);
-  // bytes for the sums of x, beside the above
-  static constexpr int XS_MAX = 232448 - SMEM < 24576 ? 232448 - SMEM : 24576;
-  static_assert(XS_MAX >= 0, "shared memory");
-};
-
 enum { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_SWIGLU = 2 };
-
-template <typename T, int GS, int MT, int NT, int NW>
-__global__ void __launch_bounds__(NW * 32)
-    int4_linear_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ numbers,
-                       const T* __restrict__ x, const T* resid, T* out, int tokens, int64_t n_out,
-                       int k, int items, int epi, int keep_sums, uint32_t sh) {
-  using C = Cfg<GS, MT, NT, NW>;
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = lane >> 2, t = lane & 3;
-  const int nchunks = k / C::CK;
-  const int64_t tile_codes = (int64_t)(k / 64) * 512, tile_numbers = (int64_t)(k / GS) * 64;
-  const int c0 = warp * nchunks / NW, nc = (warp + 1) * nchunks / NW - c0;
-  const int tok0 = blockIdx.y * (NT * 8);
-  const int ntok = min(NT * 8, tokens - tok0);
-  uint8_t* ring = smem + warp * C::RING;
-  const uint32_t ring_u = lpc::smem_u32(ring);
-  float* red = reinterpret_cast<float*>(smem + NW * C::RING);
-  // sums of x of this warp's groups, [group][token]
-  float* xs = reinterpret_cast<float*>(smem + C::SMEM) +
-              warp * ((nchunks + NW - 1) / NW) * C::SG * NT * 8;
-
-  // the weight stream: this warp's chunks of item blockIdx.x, then of the next
-  const uint8_t* fcode = codes + (int64_t)blockIdx.x * MT * tile_codes + c0 * (C::TILES * 512) + lane * 16;
-  const uint8_t* fnum = numbers + (int64_t)blockIdx.x * MT * tile_numbers + c0 * (C::SG * 64) + r * 8;
-  const int64_t jump_code = gridDim.x * MT * tile_codes - nc * (C::TILES * 512);
-  const int64_t jump_num = gridDim.x * MT * tile_numbers - nc * (C::SG * 64);
-  int fleft = nc > 0 ? nc * ((items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) : 0;
-  int fc = nc;
-  uint32_t fdst = ring_u;
-  auto advance = [&]() {
-    if (fleft > 0) {
-      --fleft;
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-#pragma unroll
-        for (int i = 0; i < C::TILES; ++i)
-          cp16(fdst + (m * C::TILES + i) * 512 + lane * 16, fcode + m * tile_codes + i * 512);
-#pragma unroll
-        for (int g = 0; g < C::SG; ++g)
-          cp8(fdst + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8,
-              fnum + m * tile_numbers + g * 64);
-      }
-      fcode += C::TILES * 512;
-      fnum += C::SG * 64;
-      if (--fc == 0) {
-        fc = nc;
-        fcode += jump_code;
-        fnum += jump_num;
-      }
-    }
-    cp_commit();
-    fdst += C::STAGE;
-    if (fdst == ring_u + C::RING) fdst = ring_u;
-  };
-
-  lpc::pdl_trigger();
-  // the weights belong to no earlier kernel of the stream: their first stages
-  // are requested before the kernel that writes x is waited for
-#pragma unroll
-  for (int i = 0; i < C::NST - 1; ++i) advance();
-  lpc::pdl_wait();
-
-  // x of token tok0 + 8 j + r: 8 columns at 32 h + 8 t of every 64.  A column
-  // without a token repeats the first one; its sums are not stored.
-  const T* xp[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-    xp[j] = x + (int64_t)(tok0 + (8 * j + r < ntok ? 8 * j + r : 0)) * k + c0 * C::CK + 8 * t;
-  constexpr uint32_t ONES = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
-
-  const uint8_t* s = ring;
-  int buf = 0;
-  bool fresh = true;  // the sums of x are not in xs
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    float sum[MT][NT][4];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[m][j][i] = 0.f;
-
-    auto chunks = [&](auto with_sums) {
-      constexpr bool SUMS = decltype(with_sums)::value;
-      for (int c = 0; c < nc; ++c) {
-        advance();
-        cp_wait<C::NST - 1>();
-        const int col = c * C::CK;
-#pragma unroll
-        for (int g = 0; g < C::SG; ++g) {
-          float acc[MT][NT][4], ones[NT][4];
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              ones[j][i] = 0.f;
-#pragma unroll
-              for (int m = 0; m < MT; ++m) acc[m][j][i] = 0.f;
-            }
-          // 32-column halves of this group: GS 128 has 4, 64 has 2, 32 has 1
-#pragma unroll
-          for (int hh = 0; hh < GS / 32; ++hh) {
-            const int half = g * (GS / 32) + hh;
-            uint4 xv[NT];
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-              xv[j] = lpc::ld_dep16(xp[j] + col + 32 * half);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const uint2 w = *reinterpret_cast<const uint2*>(
-                  s + (m * C::TILES + (half >> 1)) * 512 + lane * 16 + (half & 1) * 8);
-              uint32_t a[4], b[4];
-              operand<T>(w.x, sh, a);
-              operand<T>(w.y, sh, b);
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                mma<T>(acc[m][j], a[0], a[1], a[2], a[3], xv[j].x, xv[j].y);
-                mma<T>(acc[m][j], b[0], b[1], b[2], b[3], xv[j].z, xv[j].w);
-              }
-            }
-            if constexpr (SUMS) {
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                mma<T>(ones[j], ONES, ONES, ONES, ONES, xv[j].x, xv[j].y);
-                mma<T>(ones[j], ONES, ONES, ONES, ONES, xv[j].z, xv[j].w);
-              }
-            }
-          }
-          float* px = xs + (c * C::SG + g) * (NT * 8) + 2 * t;
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if constexpr (SUMS) {
-              if (keep_sums && r == 0)
-                *reinterpret_cast<float2*>(px + 8 * j) = make_float2(ones[j][0], ones[j][1]);
-            } else {
-              const float2 v = *reinterpret_cast<const float2*>(px + 8 * j);
-              ones[j][0] = v.x;
-              ones[j][1] = v.y;
-            }
-          }
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            const uint2 w = *reinterpret_cast<const uint2*>(
-                s + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8);
-            const float2 lo = pair_f<T>(w.x), hi = pair_f<T>(w.y);
-            float s0, m0, s1, m1;
-            if constexpr (std::is_same<T, __half>::value) {
-              s0 = lo.x * 16777216.f;
-              m0 = lo.y;
-              s1 = hi.x * 1048576.f;
-              m1 = hi.y;
-            } else {
-              s0 = lo.x;
-              m0 = fmaf(-128.f, lo.x, lo.y);
-              s1 = hi.x;
-              m1 = fmaf(-128.f, hi.x, hi.y);
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              sum[m][j][0] = fmaf(s0, acc[m][j][0], fmaf(m0, ones[j][0], sum[m][j][0]));
-              sum[m][j][1] = fmaf(s0, acc[m][j][1], fmaf(m0, ones[j][1], sum[m][j][1]));
-              sum[m][j][2] = fmaf(s1, acc[m][j][2], fmaf(m1, ones[j][0], sum[m][j][2]));
-              sum[m][j][3] = fmaf(s1, acc[m][j][3], fmaf(m1, ones[j][1], sum[m][j][3]));
-            }
-          }
-        }
-        s += C::STAGE;
-        if (s == ring + C::RING) s = ring;
-      }
-    };
-    if (fresh) {
-      chunks(std::true_type{});
-      fresh = !keep_sums;
-      __syncwarp();
-    } else {
-      chunks(std::false_type{});
-    }
-    // partial sums of the warps, [token][row] of the item, added in warp order
-    float* mine = red + (buf * NW + warp) * C::RED;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float* p = mine + (8 * j + 2 * t) * (MT * 16) + m * 16 + r;
-        p[0] = sum[m][j][0];
-        p[MT * 16] = sum[m][j][1];
-        p[8] = sum[m][j][2];
-        p[MT * 16 + 8] = sum[m][j][3];
-      }
-    __syncthreads();
-    const float* all = red + buf * NW * C::RED;
-    auto total = [&](int at) {
-      float v = 0.f;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) v += all[w * C::RED + at];
-      return v;
-    };
-    if (epi == EPI_SWIGLU) {
-      if constexpr (MT == 2)
-        for (int i = threadIdx.x; i < ntok * 16; i += NW * 32) {
-          const int tk = i >> 4, row = i & 15;
-          const int64_t n = (int64_t)item * 16 + row;
-          if (n >= n_out) continue;
-          const float gate = total(tk * 32 + row), upv = total(tk * 32 + 16 + row);
-          out[(int64_t)(tok0 + tk) * n_out + n] =
-              Num<T>::from_f(__fdividef(gate, 1.f + __expf(-gate)) * upv);
-        }
-    } else {
-      for (int i = threadIdx.x; i < ntok * (MT * 16); i += NW * 32) {
-        const int tk = i / (MT * 16), row = i % (MT * 16);
-        const int64_t n = (int64_t)item * (MT * 16) + row;
-        if (n >= n_out) continue;
-        float v = total(i);
-        const int64_t o = (int64_t)(tok0 + tk) * n_out + n;
-        if (epi == EPI_RESIDUAL) v += Num<T>::to_f(resid[o]);
-        out[o] = Num<T>::from_f(v);
-      }
-    }
-    buf ^= 1;
-  }
-  cp_wait<0>();
-}
 
 // ---------------------------------------------------------------------------
 // Up to 8 tokens whose x fits shared memory.  CTAs of 16 warps; each warp keeps
@@ -564,10 +302,10 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
             const uint2 w = *reinterpret_cast<const uint2*>(
                 s + (m * C::TILES + (half >> 1)) * 512 + lane * 16 + (half & 1) * 8);
             uint32_t a[4], b[4];
-            operand<__half>(w.x, 0u, a);
-            operand<__half>(w.y, 0u, b);
-            mma<__half>(acc[m], a[0], a[1], a[2], a[3], xv.x, xv.y);
-            mma<__half>(acc[m], b[0], b[1], b[2], b[3], xv.z, xv.w);
+            operand(w.x, a);
+            operand(w.y, b);
+            mma(acc[m], a, xv.x, xv.y);
+            mma(acc[m], b, xv.z, xv.w);
           }
         }
         float x2[NC];
@@ -646,15 +384,278 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
 }
 
 // ---------------------------------------------------------------------------
+// Up to 16 tokens where x does not fit shared memory or its preparation does not
+// pay, on weights of up to MID_MOST elements: x straight from global memory (the
+// L1 and L2 caches), as it is.  fp16 takes the operands above; bf16 the pairs
+// 128 + c, (w & 0x000F000F) | 0x43004300, exactly (a bf16 subnormal times x would
+// underflow the fp32 sum), 7 instructions a word.  The 128 is taken out again with the
+// group's sum of x, which costs the fp32 accumulator about 5 of its 24 bits and
+// leaves an error some hundred times below the output's rounding.  The sum of x is
+// one more product, of a row of ones, kept in shared memory for the next items.
+// ---------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void operand_of(uint32_t w, uint32_t (&a)[4]) {
+  if constexpr (std::is_same<T, __half>::value) {
+    operand(w, a);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void mma_of(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                       uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    mma(c, a, b0, b1);
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int GS, int MT, int NT, int NW>
+struct Cfg {
+  static constexpr int CK = GS > 64 ? GS : 64;  // columns of a pipeline stage
+  static constexpr int TILES = CK / 64;
+  static constexpr int SG = CK / GS;            // groups of a stage
+  static constexpr int STAGE = MT * (TILES * 512 + SG * 256);
+  static constexpr int NST = (MT * TILES == 4 ? 4 : MT * TILES == 2 ? 8 : 12) * 8 / NW + (NW > 8);
+  static constexpr int RING = NST * STAGE;
+  static constexpr int RED = MT * 16 * NT * 8;  // fp32 partial sums of a warp
+  static constexpr int SMEM = NW * (RING + 2 * RED * 4);
+  // bytes for the sums of x, beside the above
+  static constexpr int XS_MAX = 232448 - SMEM < 24576 ? 232448 - SMEM : 24576;
+  static_assert(XS_MAX >= 0, "shared memory");
+};
+
+template <typename T, int GS, int MT, int NT, int NW>
+__global__ void __launch_bounds__(NW * 32)
+    int4_mid_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ numbers,
+                       const T* x, const T* resid, T* out, int tokens, int64_t n_out,
+                       int k, int items, int epi, int keep_sums) {
+  using C = Cfg<GS, MT, NT, NW>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = lane >> 2, t = lane & 3;
+  const int nchunks = k / C::CK;
+  const int64_t tile_codes = (int64_t)(k / 64) * 512, tile_numbers = (int64_t)(k / GS) * 64;
+  const int c0 = warp * nchunks / NW, nc = (warp + 1) * nchunks / NW - c0;
+  const int tok0 = blockIdx.y * (NT * 8);
+  const int ntok = min(NT * 8, tokens - tok0);
+  uint8_t* ring = smem + warp * C::RING;
+  const uint32_t ring_u = lpc::smem_u32(ring);
+  float* red = reinterpret_cast<float*>(smem + NW * C::RING);
+  // sums of x of this warp's groups, [group][token]
+  float* xs = reinterpret_cast<float*>(smem + C::SMEM) +
+              warp * ((nchunks + NW - 1) / NW) * C::SG * NT * 8;
+
+  // the weight stream: this warp's chunks of item blockIdx.x, then of the next
+  const uint8_t* fcode = codes + (int64_t)blockIdx.x * MT * tile_codes + c0 * (C::TILES * 512) + lane * 16;
+  const uint8_t* fnum = numbers + (int64_t)blockIdx.x * MT * tile_numbers + c0 * (C::SG * 64) + r * 8;
+  const int64_t jump_code = gridDim.x * MT * tile_codes - nc * (C::TILES * 512);
+  const int64_t jump_num = gridDim.x * MT * tile_numbers - nc * (C::SG * 64);
+  int fleft = nc > 0 ? nc * ((items - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) : 0;
+  int fc = nc;
+  uint32_t fdst = ring_u;
+  auto advance = [&]() {
+    if (fleft > 0) {
+      --fleft;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int i = 0; i < C::TILES; ++i)
+          cp16(fdst + (m * C::TILES + i) * 512 + lane * 16, fcode + m * tile_codes + i * 512);
+#pragma unroll
+        for (int g = 0; g < C::SG; ++g)
+          cp8(fdst + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8,
+              fnum + m * tile_numbers + g * 64);
+      }
+      fcode += C::TILES * 512;
+      fnum += C::SG * 64;
+      if (--fc == 0) {
+        fc = nc;
+        fcode += jump_code;
+        fnum += jump_num;
+      }
+    }
+    cp_commit();
+    fdst += C::STAGE;
+    if (fdst == ring_u + C::RING) fdst = ring_u;
+  };
+
+  lpc::pdl_trigger();
+  // the weights belong to no earlier kernel of the stream: their first stages
+  // are requested before the kernel that writes x is waited for
+#pragma unroll
+  for (int i = 0; i < C::NST - 1; ++i) advance();
+  lpc::pdl_wait();
+
+  // x of token tok0 + 8 j + r: 8 columns at 32 h + 8 t of every 64.  A column
+  // without a token repeats the first one; its sums are not stored.
+  const T* xp[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+    xp[j] = x + (int64_t)(tok0 + (8 * j + r < ntok ? 8 * j + r : 0)) * k + c0 * C::CK + 8 * t;
+  constexpr uint32_t ONE = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
+  const uint32_t one[4] = {ONE, ONE, ONE, ONE};
+
+  const uint8_t* s = ring;
+  int buf = 0;
+  bool fresh = true;  // the sums of x are not in xs
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    float sum[MT][NT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[m][j][i] = 0.f;
+
+    auto chunks = [&](auto with_sums) {
+      constexpr bool SUMS = decltype(with_sums)::value;
+      for (int c = 0; c < nc; ++c) {
+        advance();
+        cp_wait<C::NST - 1>();
+        const int col = c * C::CK;
+#pragma unroll
+        for (int g = 0; g < C::SG; ++g) {
+          float acc[MT][NT][4], ones[NT][4];
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              ones[j][i] = 0.f;
+#pragma unroll
+              for (int m = 0; m < MT; ++m) acc[m][j][i] = 0.f;
+            }
+          // 32-column halves of this group: GS 128 has 4, 64 has 2, 32 has 1
+#pragma unroll
+          for (int hh = 0; hh < GS / 32; ++hh) {
+            const int half = g * (GS / 32) + hh;
+            uint4 xv[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+              xv[j] = lpc::ld_dep16(xp[j] + col + 32 * half);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              const uint2 w = *reinterpret_cast<const uint2*>(
+                  s + (m * C::TILES + (half >> 1)) * 512 + lane * 16 + (half & 1) * 8);
+              uint32_t a[4], b[4];
+              operand_of<T>(w.x, a);
+              operand_of<T>(w.y, b);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                mma_of<T>(acc[m][j], a, xv[j].x, xv[j].y);
+                mma_of<T>(acc[m][j], b, xv[j].z, xv[j].w);
+              }
+            }
+            if constexpr (SUMS) {
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                mma_of<T>(ones[j], one, xv[j].x, xv[j].y);
+                mma_of<T>(ones[j], one, xv[j].z, xv[j].w);
+              }
+            }
+          }
+          float* px = xs + (c * C::SG + g) * (NT * 8) + 2 * t;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            if constexpr (SUMS) {
+              if (keep_sums && r == 0)
+                *reinterpret_cast<float2*>(px + 8 * j) = make_float2(ones[j][0], ones[j][1]);
+            } else {
+              const float2 v = *reinterpret_cast<const float2*>(px + 8 * j);
+              ones[j][0] = v.x;
+              ones[j][1] = v.y;
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const uint2 w = *reinterpret_cast<const uint2*>(
+                s + MT * C::TILES * 512 + (m * C::SG + g) * 256 + lane * 8);
+            const float2 lo = pair_f<T>(w.x), hi = pair_f<T>(w.y);
+            float s0, m0, s1, m1;
+            if constexpr (std::is_same<T, __half>::value) {
+              s0 = lo.x * 16777216.f;
+              m0 = lo.y;
+              s1 = hi.x * 1048576.f;
+              m1 = hi.y;
+            } else {
+              s0 = lo.x;
+              m0 = fmaf(-128.f, lo.x, lo.y);
+              s1 = hi.x;
+              m1 = fmaf(-128.f, hi.x, hi.y);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              sum[m][j][0] = fmaf(s0, acc[m][j][0], fmaf(m0, ones[j][0], sum[m][j][0]));
+              sum[m][j][1] = fmaf(s0, acc[m][j][1], fmaf(m0, ones[j][1], sum[m][j][1]));
+              sum[m][j][2] = fmaf(s1, acc[m][j][2], fmaf(m1, ones[j][0], sum[m][j][2]));
+              sum[m][j][3] = fmaf(s1, acc[m][j][3], fmaf(m1, ones[j][1], sum[m][j][3]));
+            }
+          }
+        }
+        s += C::STAGE;
+        if (s == ring + C::RING) s = ring;
+      }
+    };
+    if (fresh) {
+      chunks(std::true_type{});
+      fresh = !keep_sums;
+      __syncwarp();
+    } else {
+      chunks(std::false_type{});
+    }
+    // partial sums of the warps, [token][row] of the item, added in warp order
+    float* mine = red + (buf * NW + warp) * C::RED;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float* p = mine + (8 * j + 2 * t) * (MT * 16) + m * 16 + r;
+        p[0] = sum[m][j][0];
+        p[MT * 16] = sum[m][j][1];
+        p[8] = sum[m][j][2];
+        p[MT * 16 + 8] = sum[m][j][3];
+      }
+    __syncthreads();
+    const float* all = red + buf * NW * C::RED;
+    auto total = [&](int at) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) v += all[w * C::RED + at];
+      return v;
+    };
+    if (epi == EPI_SWIGLU) {
+      if constexpr (MT == 2)
+        for (int i = threadIdx.x; i < ntok * 16; i += NW * 32) {
+          const int tk = i >> 4, row = i & 15;
+          const int64_t n = (int64_t)item * 16 + row;
+          if (n >= n_out) continue;
+          const float gate = total(tk * 32 + row), upv = total(tk * 32 + 16 + row);
+          out[(int64_t)(tok0 + tk) * n_out + n] =
+              Num<T>::from_f(__fdividef(gate, 1.f + __expf(-gate)) * upv);
+        }
+    } else {
+      for (int i = threadIdx.x; i < ntok * (MT * 16); i += NW * 32) {
+        const int tk = i / (MT * 16), row = i % (MT * 16);
+        const int64_t n = (int64_t)item * (MT * 16) + row;
+        if (n >= n_out) continue;
+        float v = total(i);
+        const int64_t o = (int64_t)(tok0 + tk) * n_out + n;
+        if (epi == EPI_RESIDUAL) v += Num<T>::to_f(resid[o]);
+        out[o] = Num<T>::from_f(v);
+      }
+    }
+    buf ^= 1;
+  }
+  cp_wait<0>();
+}
+
+// ---------------------------------------------------------------------------
 // layout
 // ---------------------------------------------------------------------------
-// Tile rows of 16: of the weight (layout 0), or gate tile i, up tile i, ...
-// (layout 1, gate rows first in the source).  A multiple of 4 of them, so that
-// no item reaches past the last.
-__host__ __device__ inline int64_t tile_rows(int64_t n_out, int layout) {
-  const int64_t t = (n_out + 15) / 16 * (layout == 1 ? 2 : 1);
-  return (t + 3) / 4 * 4;
-}
 // Source row of row `i` of tile row `p`, or -1 for padding.
 __device__ __forceinline__ int64_t source_row(int64_t p, int i, int64_t n_out, int layout) {
   const int64_t n = (layout == 1 ? p >> 1 : p) * 16 + i;
@@ -708,6 +709,39 @@ __global__ void int4_pack_numbers_kernel(const T* __restrict__ s, const T* __res
   }
 }
 
+// One thread: one row of a tile row, the power that brings its numbers into
+// fp16's range and the numbers in it.
+template <typename T>
+__global__ void int4_pack_scaled_kernel(const T* __restrict__ s, const T* __restrict__ m,
+                                        __half2* __restrict__ scaled, float* __restrict__ factors,
+                                        int64_t count, int64_t n_out, int ng, int layout) {
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;  // (tile row, row)
+  if (at >= count) return;
+  const int64_t p = at >> 4;
+  const int i = (int)(at & 15);
+  const int64_t row = source_row(p, i, n_out, layout);
+  float top = 0.f;
+  for (int g = 0; row >= 0 && g < ng; ++g) {
+    const float a = fabsf(Num<T>::to_f(s[row * ng + g])) * 16777216.f;
+    const float b = fabsf(Num<T>::to_f(m[row * ng + g]));
+    if (a < INFINITY) top = fmaxf(top, a);
+    if (b < INFINITY) top = fmaxf(top, b);
+  }
+  int e = 0;
+  if (top > 0.f) e = max(-126, min(126, 14 - ((int)(__float_as_uint(top) >> 23) - 127)));
+  const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+  factors[at] = __uint_as_float((uint32_t)(127 - e) << 23);
+  for (int g = 0; g < ng; ++g) {
+    float a = 0.f, b = 0.f;
+    if (row >= 0) {
+      a = Num<T>::to_f(s[row * ng + g]) * 16777216.f * up;
+      b = Num<T>::to_f(m[row * ng + g]) * up;
+    }
+    // the codes of rows 8..15 lie 4 bits higher in their words
+    scaled[(p * ng + g) * 16 + i] = __floats2half2_rn(i < 8 ? a : a * 0.0625f, b);
+  }
+}
+
 // One thread: one packed word, 8 values written as 4 pairs.
 template <typename T>
 __global__ void int4_unpack_kernel(const uint32_t* __restrict__ codes, const T* __restrict__ numbers,
@@ -743,53 +777,6 @@ bool use_pdl() {
   return on;
 }
 
-template <typename T, int GS, int MT, int NT, int NW>
-int launch(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
-           cudaStream_t s) {
-  using C = Cfg<GS, MT, NT, NW>;
-  static std::atomic<uint64_t> mask{0};
-  int rc = lpc::once_per_device_smem((const void*)int4_linear_kernel<T, GS, MT, NT, NW>,
-                                     C::SMEM + C::XS_MAX, mask);
-  if (rc) return rc;
-  const int64_t tr = tile_rows(w->n_out, w->layout);
-  const int items = (int)(w->layout == 1 ? tr / 2 : (w->n_out + 16 * MT - 1) / (16 * MT));
-  // the sums of x are computed with the first item and kept for the next ones
-  const int64_t sums = (int64_t)NW * ((w->k / C::CK + NW - 1) / NW) * C::SG * NT * 8 * 4;
-  const int slots = lpc::current_device_sms() * (16 / NW);
-  const int keep = items > slots && sums <= C::XS_MAX;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min(items, slots), (unsigned)((tokens + NT * 8 - 1) / (NT * 8)));
-  cfg.blockDim = dim3(NW * 32);
-  cfg.dynamicSmemBytes = C::SMEM + (keep ? (int)sums : 0);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const uint8_t* codes = (const uint8_t*)w->packed;
-  cudaLaunchKernelEx(&cfg, int4_linear_kernel<T, GS, MT, NT, NW>, codes,
-                     codes + tr * 16 * (int64_t)(w->k / 2), (const T*)x, (const T*)resid, (T*)out,
-                     (int)tokens, w->n_out, w->k, items, epi, keep, 1u << 28);
-  return lpc::check_launch("int4_linear");
-}
-
-// Two tile rows share the loads of x; with too few rows to give each SM an
-// item, one tile row an item and 16 warps to share its columns.
-template <typename T, int GS, int NT>
-int launch_mt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
-              cudaStream_t s) {
-  const int64_t tr = (w->n_out + 15) / 16, sms = lpc::current_device_sms();
-  if constexpr (NT < 4) {  // 32 tokens' accumulators do not fit 128 registers
-    if (tr <= sms)
-      return w->layout == 1 ? launch<T, GS, 2, NT, 16>(w, x, out, resid, tokens, epi, s)
-                            : launch<T, GS, 1, NT, 16>(w, x, out, resid, tokens, epi, s);
-  }
-  if (w->layout == 1) return launch<T, GS, 2, NT, 8>(w, x, out, resid, tokens, epi, s);
-  if (NT == 1 || tr <= 2 * sms) return launch<T, GS, 1, NT, 8>(w, x, out, resid, tokens, epi, s);
-  return launch<T, GS, 2, NT, 8>(w, x, out, resid, tokens, epi, s);
-}
-
 // Items of MT tile rows each.
 int few_items(const lpc_w4* w, int mt) {
   const int64_t tr = (w->n_out + 15) / 16 * (w->layout == 1 ? 2 : 1);
@@ -816,9 +803,9 @@ int launch_few(const lpc_w4* w, const void* x, void* out, const void* resid, int
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const uint8_t* codes = (const uint8_t*)w->packed;
-  cudaLaunchKernelEx(&cfg, int4_few_kernel<T, GS, MT, TC>, codes,
-                     codes + tile_rows(w->n_out, w->layout) * 16 * (int64_t)(w->k / 2), (const T*)x,
+  const lpc::Int4Parts p = lpc::int4_parts(w->packed, w->n_out, w->k, w->group, w->layout);
+  cudaLaunchKernelEx(&cfg, int4_few_kernel<T, GS, MT, TC>, (const uint8_t*)p.codes,
+                     (const uint8_t*)p.numbers, (const T*)x,
                      (const T*)resid, (T*)out, (int)tokens, w->n_out, w->k, items, epi);
   return lpc::check_launch("int4_linear");
 }
@@ -828,22 +815,80 @@ int launch_few(const lpc_w4* w, const void* x, void* out, const void* resid, int
 template <typename T, int GS, int TC>
 int launch_few_mt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens,
                   int epi, cudaStream_t s) {
-  static const int force = [] { const char* e = getenv("LPC_MT"); return e ? atoi(e) : 0; }();
-  const bool one = force ? force == 1 : few_items(w, 1) <= lpc::current_device_sms() * (TC == 1 ? 2 : 1);
+  const bool one = few_items(w, 1) <= lpc::current_device_sms() * (TC == 1 ? 2 : 1);
   if (w->layout == 0 && one) return launch_few<T, GS, 1, TC>(w, x, out, resid, tokens, epi, s);
   return launch_few<T, GS, 2, TC>(w, x, out, resid, tokens, epi, s);
+}
+
+template <typename T, int GS, int MT, int NT, int NW>
+int launch_mid(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
+           cudaStream_t s) {
+  using C = Cfg<GS, MT, NT, NW>;
+  static std::atomic<uint64_t> mask{0};
+  int rc = lpc::once_per_device_smem((const void*)int4_mid_kernel<T, GS, MT, NT, NW>,
+                                     C::SMEM + C::XS_MAX, mask);
+  if (rc) return rc;
+  const int items = few_items(w, MT);
+  // the sums of x are computed with the first item and kept for the next ones
+  const int64_t sums = (int64_t)NW * ((w->k / C::CK + NW - 1) / NW) * C::SG * NT * 8 * 4;
+  const int slots = lpc::current_device_sms() * (16 / NW);
+  const int keep = items > slots && sums <= C::XS_MAX;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min(items, slots), (unsigned)((tokens + NT * 8 - 1) / (NT * 8)));
+  cfg.blockDim = dim3(NW * 32);
+  cfg.dynamicSmemBytes = C::SMEM + (keep ? (int)sums : 0);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const lpc::Int4Parts p = lpc::int4_parts(w->packed, w->n_out, w->k, w->group, w->layout);
+  cudaLaunchKernelEx(&cfg, int4_mid_kernel<T, GS, MT, NT, NW>, (const uint8_t*)p.codes,
+                     (const uint8_t*)p.numbers, (const T*)x, (const T*)resid, (T*)out, (int)tokens,
+                     w->n_out, w->k, items, epi, keep);
+  return lpc::check_launch("int4_linear");
+}
+
+// Which kernel takes the products (int4_many.cu has MANY).
+enum Kernel { FEW, MID, MANY };
+// Measured, us, mid / many: 4096 x 4096 at 16 tokens 6.3 / 10.4, 4096 x 11,008 at 8
+// tokens 10.2 / 19, 22,016 x 4096 at 16 tokens 30 / 23.
+constexpr int64_t MID_MOST = 64 << 20;
+template <int GS>
+Kernel pick(const lpc_w4* w, int64_t tokens) {
+  if ((tokens == 1 && FewCfg<GS, 2, 1>::smem(w->k, 1) <= MAX_SMEM) ||
+      (tokens <= 8 && FewCfg<GS, 2, 8>::smem(w->k, (int)tokens) <= MAX_SMEM))
+    return FEW;
+  return tokens <= 16 && (w->n_out << w->layout) * w->k <= MID_MOST ? MID : MANY;
+}
+Kernel pick(const lpc_w4* w, int64_t tokens) {
+  return w->group == 128 ? pick<128>(w, tokens) : w->group == 64 ? pick<64>(w, tokens) : pick<32>(w, tokens);
+}
+
+// Two tile rows share the loads of x; with too few rows to give each SM an
+// item, one tile row an item and 16 warps to share its columns.
+template <typename T, int GS, int NT>
+int launch_mid_mt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens,
+                  int epi, cudaStream_t s) {
+  const int64_t tr = (w->n_out + 15) / 16, sms = lpc::current_device_sms();
+  if (w->layout == 1)
+    return tr <= sms ? launch_mid<T, GS, 2, NT, 16>(w, x, out, resid, tokens, epi, s)
+                     : launch_mid<T, GS, 2, NT, 8>(w, x, out, resid, tokens, epi, s);
+  if (tr <= sms) return launch_mid<T, GS, 1, NT, 16>(w, x, out, resid, tokens, epi, s);
+  if (NT == 1 || tr <= 2 * sms) return launch_mid<T, GS, 1, NT, 8>(w, x, out, resid, tokens, epi, s);
+  return launch_mid<T, GS, 2, NT, 8>(w, x, out, resid, tokens, epi, s);
 }
 
 template <typename T, int GS>
 int launch_nt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
               cudaStream_t s) {
+  if (pick<GS>(w, tokens) == MID)
+    return tokens <= 8 ? launch_mid_mt<T, GS, 1>(w, x, out, resid, tokens, epi, s)
+                       : launch_mid_mt<T, GS, 2>(w, x, out, resid, tokens, epi, s);
   if (tokens == 1 && FewCfg<GS, 2, 1>::smem(w->k, 1) <= MAX_SMEM)
     return launch_few_mt<T, GS, 1>(w, x, out, resid, tokens, epi, s);
-  if (tokens <= 8 && FewCfg<GS, 2, 8>::smem(w->k, (int)tokens) <= MAX_SMEM)
-    return launch_few_mt<T, GS, 8>(w, x, out, resid, tokens, epi, s);
-  if (tokens <= 8) return launch_mt<T, GS, 1>(w, x, out, resid, tokens, epi, s);
-  if (tokens <= 16) return launch_mt<T, GS, 2>(w, x, out, resid, tokens, epi, s);
-  return launch_mt<T, GS, 4>(w, x, out, resid, tokens, epi, s);
+  return launch_few_mt<T, GS, 8>(w, x, out, resid, tokens, epi, s);
 }
 
 template <typename T>
@@ -877,8 +922,14 @@ int weight_check(const lpc_w4* w, const char* what) {
 
 extern "C" int64_t lpc_int4_weight_bytes(int64_t n_out, int k, int group, int layout) {
   if (!shape_ok(n_out, k, group, layout)) return 0;
-  const int64_t tr = tile_rows(n_out, layout);
-  return tr * 16 * (int64_t)(k / 2) + tr * 64 * (int64_t)(k / group);
+  return lpc::int4_parts(nullptr, n_out, k, group, layout).bytes;
+}
+
+extern "C" int64_t lpc_int4_linear_workspace_bytes(const lpc_w4* w, int64_t tokens) {
+  if (weight_check(w, "int4_linear") || tokens <= 0 || tokens > MAX_TOKENS || pick(w, tokens) != MANY ||
+      w->dtype == LPC_DTYPE_F16)
+    return 0;
+  return tokens * (int64_t)w->k * 2 + MAX_TOKENS * 4;
 }
 
 extern "C" int lpc_int4_pack(const lpc_w4* w, const void* codes, const void* scales,
@@ -891,17 +942,26 @@ extern "C" int lpc_int4_pack(const lpc_w4* w, const void* codes, const void* sca
     return LPC_ERR_INVALID;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int64_t tr = tile_rows(w->n_out, w->layout);
+  const int64_t tr = lpc::int4_tile_rows(w->n_out, w->layout);
   const int64_t words = tr * (w->k / 64) * 128;
   const int ng = w->k / w->group;
   const int64_t count = tr * ng * 8;
-  uint8_t* base = (uint8_t*)w->packed;
+  const Int4Parts p = int4_parts(w->packed, w->n_out, w->k, w->group, w->layout);
   int4_pack_kernel<<<(unsigned)((words + 255) / 256), 256, 0, s>>>(
-      (const uint8_t*)codes, (uint32_t*)base, words, w->n_out, w->k, w->layout);
+      (const uint8_t*)codes, (uint32_t*)p.codes, words, w->n_out, w->k, w->layout);
   // 16-bit numbers are moved, not computed with: one type serves both
   int4_pack_numbers_kernel<__half><<<(unsigned)((count + 255) / 256), 256, 0, s>>>(
-      (const __half*)scales, (const __half*)mins, (__half*)(base + tr * 16 * (int64_t)(w->k / 2)),
-      count, w->n_out, ng, w->layout);
+      (const __half*)scales, (const __half*)mins, (__half*)p.numbers, count, w->n_out, ng,
+      w->layout);
+  const unsigned rows = (unsigned)((tr * 16 + 127) / 128);
+  if (w->dtype == LPC_DTYPE_BF16)
+    int4_pack_scaled_kernel<__nv_bfloat16><<<rows, 128, 0, s>>>(
+        (const __nv_bfloat16*)scales, (const __nv_bfloat16*)mins, (__half2*)p.scaled, p.factors,
+        tr * 16, w->n_out, ng, w->layout);
+  else
+    int4_pack_scaled_kernel<__half><<<rows, 128, 0, s>>>(
+        (const __half*)scales, (const __half*)mins, (__half2*)p.scaled, p.factors, tr * 16,
+        w->n_out, ng, w->layout);
   if ((rc = check_launch("int4_pack"))) return rc;
   // the products read the weight before they wait on the kernel before them
   if (cudaStreamSynchronize(s) != cudaSuccess) {
@@ -919,10 +979,10 @@ extern "C" int lpc_int4_unpack(const lpc_w4* w, void* out, void* stream) {
     set_error("int4_unpack: out must be given and 16-byte aligned");
     return LPC_ERR_INVALID;
   }
-  const int64_t tr = tile_rows(w->n_out, w->layout);
+  const int64_t tr = lpc::int4_tile_rows(w->n_out, w->layout);
   const int64_t words = tr * (w->k / 64) * 128;
-  const uint8_t* base = (const uint8_t*)w->packed;
-  const uint8_t* nb = base + tr * 16 * (int64_t)(w->k / 2);
+  const Int4Parts parts = int4_parts(w->packed, w->n_out, w->k, w->group, w->layout);
+  const uint8_t *base = parts.codes, *nb = parts.numbers;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned grid = (unsigned)((words + 255) / 256);
   if (w->dtype == LPC_DTYPE_BF16)
@@ -938,7 +998,8 @@ extern "C" int lpc_int4_unpack(const lpc_w4* w, void* out, void* stream) {
 }
 
 extern "C" int lpc_int4_linear(const lpc_w4* w, const void* x, void* out, const void* resid,
-                               int64_t tokens, int epilogue, void* stream) {
+                               int64_t tokens, int epilogue, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
   using namespace lpc;
   int rc = weight_check(w, "int4_linear");
   if (rc) return rc;
@@ -957,7 +1018,15 @@ extern "C" int lpc_int4_linear(const lpc_w4* w, const void* x, void* out, const 
     return LPC_ERR_INVALID;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return w->dtype == LPC_DTYPE_BF16
-             ? launch_gs<__nv_bfloat16>(w, x, out, resid, tokens, epilogue, s)
-             : launch_gs<__half>(w, x, out, resid, tokens, epilogue, s);
+  if (pick(w, tokens) != MANY)
+    return w->dtype == LPC_DTYPE_BF16
+               ? launch_gs<__nv_bfloat16>(w, x, out, resid, tokens, epilogue, s)
+               : launch_gs<__half>(w, x, out, resid, tokens, epilogue, s);
+  const int64_t need = lpc_int4_linear_workspace_bytes(w, tokens);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
+    set_error("int4_linear: workspace of %lld bytes required, got %lld", (long long)need,
+              (long long)workspace_bytes);
+    return LPC_ERR_INVALID;
+  }
+  return int4_many(w, x, out, resid, tokens, epilogue, workspace, s);
 }

@@ -133,6 +133,7 @@ class Int4Weight:
         self._c = _lib.W4(self.data.data_ptr(), self.n_out, self.k, group_size, lay,
                           _lib.DTYPE_CODE[self.dtype])
         self.ref = ctypes.addressof(self._c)
+        self._workspace = {}
         codes, scales, mins = codes.contiguous(), scales.contiguous(), mins.contiguous()
         self.index = codes.get_device()
         rc = _lib.call_on(self.index, lib.lpc_int4_pack, self.ref, codes.data_ptr(),
@@ -147,6 +148,14 @@ class Int4Weight:
 
     def memory_footprint_bytes(self) -> int:
         return self.data.numel()
+
+    def workspace_bytes(self, tokens: int) -> int:
+        """Scratch that a product of this many tokens takes from torch's allocator."""
+        n = self._workspace.get(tokens)
+        if n is None:
+            n = _lib.load().lpc_int4_linear_workspace_bytes(self.ref, tokens)
+            self._workspace[tokens] = n
+        return n
 
     def dequantize(self) -> torch.Tensor:
         """The 16-bit weight that the codes stand for, ``[n_out, k]`` (layout
@@ -200,9 +209,12 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
         raise ValueError("LlamaPureComputeError: out must be a contiguous [..., n_out] tensor.")
     elif out.data_ptr() == xp and tokens:
         raise ValueError("LlamaPureComputeError: out must not be x.")
-    rc = _lib.call_on(index, _lib.load().lpc_int4_linear, w.ref, xp, out.data_ptr(), rp, tokens, epi)
+    need = w.workspace_bytes(tokens)
+    ws = x.new_empty((need + 1) // 2) if need else None
+    rc = _lib.call_on(index, _lib.load().lpc_int4_linear, w.ref, xp, out.data_ptr(), rp, tokens, epi,
+                      ws.data_ptr() if need else None, need)
     if rc:
         _lib.check(rc, "int4_linear")
     if tokens:
-        _lib.count_launch("lpc_int4_linear")
+        _lib.count_launch("lpc_int4_linear", 2 if need else 1)
     return out

@@ -100,29 +100,42 @@ def test_append_and_read_refusals():
 def test_bad_weights_are_refused(kw):
     lib, w = _lib.load(), weight(**kw)
     ref = ctypes.addressof(w)
-    assert lib.lpc_int4_linear(ref, 16, 16, None, 1, 0, None) == INVALID
+    assert lib.lpc_int4_linear(ref, 16, 16, None, 1, 0, None, 0, None) == INVALID
     assert lib.lpc_int4_pack(ref, 16, 16, 16, None) == INVALID
     assert lib.lpc_int4_unpack(ref, 16, None) == INVALID
 
 
 def test_linear_refusals():
     lib = _lib.load()
-    ref = ctypes.addressof(w0 := weight())
-    pair = ctypes.addressof(w1 := weight(layout=1))
-    assert lib.lpc_int4_linear(ref, 16, 16, None, 65, 0, None) == INVALID
+    w0, w1, bad, wide = weight(), weight(layout=1), weight(dtype=0), weight(n_out=128, k=16384)
+    huge = weight(n_out=8192, k=16384)
+    ref, pair = ctypes.addressof(w0), ctypes.addressof(w1)
+
+    def call(r, *a, ws=None, nbytes=0):
+        return lib.lpc_int4_linear(r, *a, ws, nbytes, None)
+    assert call(ref, 16, 16, None, 65, 0) == INVALID
     assert b"at most 64" in lib.lpc_last_error()
-    assert lib.lpc_int4_linear(ref, 16, 16, None, 1, 2, None) == INVALID   # swiglu on a plain weight
-    assert lib.lpc_int4_linear(pair, 16, 16, None, 1, 0, None) == INVALID
-    assert lib.lpc_int4_linear(ref, 16, 16, None, 1, 1, None) == INVALID   # no resid
-    assert lib.lpc_int4_linear(ref, 24, 16, None, 1, 0, None) == INVALID
-    assert lib.lpc_int4_linear(ref, 16, 16, None, 0, 0, None) == _lib.LPC_OK
-    bad = weight(dtype=0)
-    assert lib.lpc_int4_linear(ctypes.addressof(bad), 16, 16, None, 1, 0, None) == UNSUPPORTED
-    assert lib.lpc_int4_weight_bytes(100, 100, 128, 0) == 0
-    # tile rows of 16, a multiple of 4 of them: 17 rows need two, a pair of 17 four
-    assert lib.lpc_int4_weight_bytes(17, 256, 128, 0) == 4 * 16 * 128 + 4 * 64 * 2
-    assert lib.lpc_int4_weight_bytes(17, 256, 128, 1) == 4 * 16 * 128 + 4 * 64 * 2
-    del w0, w1
+    assert call(ref, 16, 16, None, 1, 2) == INVALID   # swiglu on a plain weight
+    assert call(pair, 16, 16, None, 1, 0) == INVALID
+    assert call(ref, 16, 16, None, 1, 1) == INVALID   # no resid
+    assert call(ref, 24, 16, None, 1, 0) == INVALID
+    assert call(ref, 16, 16, None, 0, 0) == _lib.LPC_OK
+    assert call(ctypes.addressof(bad), 16, 16, None, 1, 0) == UNSUPPORTED
+    # the workspace: bf16, more than 16 tokens, or more than 8 on a large weight
+    need = lib.lpc_int4_linear_workspace_bytes
+    assert need(ref, 16) == 0 and need(ref, 0) == 0 and need(ref, 65) == 0
+    assert need(ref, 17) == 17 * 256 * 2 + 256
+    assert need(ctypes.addressof(wide), 8) == 0 and need(ctypes.addressof(huge), 8) == 8 * 16384 * 2 + 256
+    half = weight(dtype=1)
+    assert need(ctypes.addressof(half), 64) == 0
+    assert call(ref, 16, 16, None, 17, 0) == INVALID and b"workspace" in lib.lpc_last_error()
+    assert call(ref, 16, 16, None, 17, 0, ws=16, nbytes=100) == INVALID
+    assert call(ref, 16, 16, None, 17, 0, ws=24, nbytes=1 << 20) == INVALID
+    size = lib.lpc_int4_weight_bytes
+    assert size(100, 100, 128, 0) == 0
+    # tile rows of 16, a multiple of 8 of them: codes, two sets of numbers, a factor a row
+    assert size(17, 256, 128, 0) == size(17, 256, 128, 1) == 8 * (16 * 128 + 2 * 128 + 64)
+    assert size(129, 256, 128, 0) == 2 * size(128, 256, 128, 0)
 
 
 def test_python_layer_refuses_cpu_tensors():
