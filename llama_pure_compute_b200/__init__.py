@@ -7,8 +7,11 @@ and the model / generator call sites, all running hand-written CUDA kernels
 for sm_100a through the C-ABI library ``lib/liblpc_b200.so``.
 """
 from .config import PRESETS, LlamaModelConfig, Precision
-from .ops import (decode_attention, is_cuda_backend_available, rmsnorm_forward, rmsswiglu_forward,
-                  rope_forward, rope_kv_append, update_kv_cache)
+from .int4_cache import Int4KVCache, Int4RaggedKVCache
+from .int4_linear import Int4Weight
+from .ops import (Int4KV, decode_attention, decode_attention_int4, is_cuda_backend_available,
+                  kv_read_int4, rmsnorm_forward, rmsswiglu_forward, rope_forward, rope_kv_append,
+                  rope_kv_append_int4, update_kv_cache)
 
 __version__ = "0.1.0"
 
@@ -23,4 +26,11 @@ __all__ = [
     "rmsnorm_forward",
     "rope_kv_append",
     "decode_attention",
+    "Int4KV",
+    "rope_kv_append_int4",
+    "kv_read_int4",
+    "decode_attention_int4",
+    "Int4Weight",
+    "Int4KVCache",
+    "Int4RaggedKVCache",
 ]

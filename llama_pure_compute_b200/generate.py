@@ -19,6 +19,7 @@ import torch
 import torch.nn.functional as F
 
 from .config import LlamaModelConfig
+from .int4_cache import Int4KVCache
 from .kv_manager import KVCacheManager
 from .ragged_cache import RaggedKVCache
 
@@ -110,11 +111,19 @@ class _RowView:
 class LlamaGenerator:
     """Batch-1 streaming generator (generate.py:156-333)."""
 
-    def __init__(self, model: torch.nn.Module, config: LlamaModelConfig) -> None:
+    def __init__(self, model: torch.nn.Module, config: LlamaModelConfig,
+                 kv_cache: Union[KVCacheManager, Int4KVCache, None] = None) -> None:
+        """``kv_cache``: a cache to use instead of a 16-bit one of the
+        configuration's ``max_seq_len``, e.g. an ``Int4KVCache``."""
         self.model = model
         self.config = config
         p = next(model.parameters())
         self.device = p.device
+        if kv_cache is not None:
+            if kv_cache.max_seq_len < config.max_seq_len:
+                raise ValueError("kv_cache is shorter than the configuration's max_seq_len")
+            self.kv_cache = kv_cache
+            return
         self.kv_cache = KVCacheManager(num_layers=config.num_layers, max_batch_size=1,
                                        max_seq_len=config.max_seq_len, n_kv_heads=config.num_kv_heads,
                                        head_dim=config.head_dim, dtype=p.dtype, device=self.device)
@@ -169,7 +178,7 @@ class BatchedGreedyDecoder:
     generated tokens; ``step`` advances every sequence by one token.
     """
 
-    def __init__(self, model: torch.nn.Module, kv_cache: Union[KVCacheManager, RaggedKVCache],
+    def __init__(self, model: torch.nn.Module, kv_cache: Union[KVCacheManager, Int4KVCache, RaggedKVCache],
                  batch_size: int, use_cuda_graph: bool = True, prefill_chunk: int = 16) -> None:
         self.ragged = isinstance(kv_cache, RaggedKVCache)
         cap = kv_cache.num_sequences if self.ragged else kv_cache.max_batch_size
@@ -214,6 +223,8 @@ class BatchedGreedyDecoder:
             if self.ragged:
                 self.kv.select(range(i, j))
                 view = self.kv
+            elif isinstance(self.kv, Int4KVCache):
+                view = self.kv.row_view(i, j - i)
             else:
                 view = _RowView(self.kv, i, j - i)
             logits = self.model(ids, positions=pos, kv_cache=view, last_token_only=True)

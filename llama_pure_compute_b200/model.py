@@ -31,6 +31,11 @@ checkpoints and call sites carry over.  What runs underneath:
                        (default) one lpc_wsgemm, norm weight folded
   down + residual   -> one addmm; decode steps of <= PACKED_RESIDUAL_MAX_TOKENS
                        tokens: lpc_wsgemm (residual epilogue), packed down_proj
+
+``LlamaForCausalLM.quantize_weights_int4`` holds the projections in 4 bits
+instead: up to 64 tokens a step run on them (lpc_int4_linear, with the residual
+and SiLU*up epilogues), larger steps on a 16-bit copy made for the call.
+
   lm_head           -> all positions by default (model.py:475), or only the
                        last one with ``last_token_only=True``
 
@@ -123,6 +128,28 @@ class _StepContext:
         self.workspace = None
 
 
+def _int4_project(x: torch.Tensor, w, resid: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """(resid +) x w^T for an ``Int4Weight``: the 4-bit kernel for decode-sized
+    steps, a GEMM on the 16-bit values above (what a prefill costs anyway)."""
+    from .int4_linear import MAX_TOKENS, int4_linear
+    x2 = x.reshape(-1, x.shape[-1])
+    if resid is not None:
+        r2 = resid.reshape(-1, resid.shape[-1])
+        if x2.shape[0] <= MAX_TOKENS:
+            return int4_linear(x2, w, "residual", resid=r2.contiguous()).view(resid.shape)
+        return torch.addmm(r2, x2, w.dequantize().t()).view(resid.shape)
+    if x2.shape[0] <= MAX_TOKENS:
+        return int4_linear(x, w)
+    return F.linear(x, w.dequantize())
+
+
+def _drop(*linears: nn.Linear) -> None:
+    for lin in linears:
+        w = lin.weight
+        lin.weight = nn.Parameter(torch.empty(0, w.shape[1], dtype=w.dtype, device=w.device),
+                                  requires_grad=False)
+
+
 def _packable(x: torch.Tensor, w: torch.Tensor) -> bool:
     return (x.dtype in (torch.bfloat16, torch.float16) and w.dtype == x.dtype
             and x.shape[-1] % 64 == 0 and w.is_cuda)
@@ -148,6 +175,16 @@ class LlamaAttention(nn.Module):
         self._packed_qkv_key = None
         self._packed_o = None
         self._packed_o_key = None
+        self.int4_qkv = None  # Int4Weight of the stacked q/k/v projections
+        self.int4_o = None
+
+    @torch.no_grad()
+    def quantize_weights_int4(self, group_size: int) -> None:
+        from .int4_linear import Int4Weight
+        self.int4_qkv = Int4Weight(self.qkv_weight(), group_size=group_size)
+        self.int4_o = Int4Weight(self.o_proj.weight, group_size=group_size)
+        self._qkv = self._qkv_key = self._packed_qkv = self._packed_o = None
+        _drop(self.q_proj, self.k_proj, self.v_proj, self.o_proj)
 
     def qkv_weight(self) -> torch.Tensor:
         """[(H+2Hkv)*D, dim] weight; q/k/v parameters are re-pointed into it once."""
@@ -190,7 +227,8 @@ class LlamaAttention(nn.Module):
         return self._packed_o
 
     def _fused_qkv(self, x: torch.Tensor, ctx: Optional[_StepContext]) -> bool:
-        return (ctx is not None and ctx.decode and 0 < x.numel() // x.shape[-1] <= ctx.fused_qkv_max
+        return (ctx is not None and ctx.decode and self.int4_qkv is None
+                and 0 < x.numel() // x.shape[-1] <= ctx.fused_qkv_max
                 and self.head_dim == 128 and x.dtype in (torch.bfloat16, torch.float16)
                 and ctx.cos_table is not None and ctx.cos_table.dtype == x.dtype
                 and self.q_proj.weight.dtype == x.dtype and x.shape[-1] % 64 == 0)
@@ -231,7 +269,10 @@ class LlamaAttention(nn.Module):
                                    positions=positions, ctx=ctx, num_heads=H, scale=self.scale)
         if input_norm is not None:
             raise ValueError("input_norm is only applied inside the fused decode kernel")
-        qkv = F.linear(x, self.qkv_weight())
+        if self.int4_qkv is not None:
+            qkv = _int4_project(x, self.int4_qkv)
+        else:
+            qkv = F.linear(x, self.qkv_weight())
         if kv_cache is not None:
             if ctx is None or ctx.cos_table is None:
                 raise ValueError("cached attention needs the model's RoPE tables (call via LlamaModel)")
@@ -259,6 +300,8 @@ class LlamaAttention(nn.Module):
         """residual + attn @ o_proj^T in one GEMM (the residual added in the
         epilogue): the packed weight-streaming kernel for decode steps of at
         most ``ctx.resid_max`` tokens, else cuBLAS (beta=1 epilogue)."""
+        if self.int4_o is not None:
+            return _int4_project(attn, self.int4_o, residual)
         shp = residual.shape
         r2 = residual.reshape(-1, shp[-1])
         a2 = attn.reshape(-1, attn.shape[-1])
@@ -285,6 +328,18 @@ class LlamaDecodeLayer(nn.Module):
         self._packed_down_key = None
         self._folded = None
         self._folded_key = None
+        self.int4_gate_up = None  # Int4Weight, layout "swiglu"
+        self.int4_down = None
+
+    @torch.no_grad()
+    def quantize_weights_int4(self, group_size: int) -> None:
+        from .int4_linear import Int4Weight
+        self.self_attn.quantize_weights_int4(group_size)
+        self.int4_gate_up = Int4Weight(self.gate_proj.weight, self.up_proj.weight, layout="swiglu",
+                                       group_size=group_size)
+        self.int4_down = Int4Weight(self.down_proj.weight, group_size=group_size)
+        self._packed_gate_up = self._packed_down = self._folded = None
+        _drop(self.gate_proj, self.up_proj, self.down_proj)
 
     def packed_gate_up(self, fold_norm: bool = False):
         """gate/up weights in the packed SwiGLU tile layout (lpc_pack_weights),
@@ -335,6 +390,14 @@ class LlamaDecodeLayer(nn.Module):
                    norm_in_gemm: bool = False) -> torch.Tensor:
         norm = self.post_attention_layernorm
         tokens = h.numel() // h.shape[-1]
+        if self.int4_gate_up is not None:
+            from .int4_linear import MAX_TOKENS, int4_linear
+            from .ops import rmsnorm_forward
+            if tokens <= MAX_TOKENS:
+                return int4_linear(rmsnorm_forward(h, norm.weight, norm.eps), self.int4_gate_up,
+                                   "swiglu")
+            return rmsswiglu_forward(h, rms_weight=norm.weight, gate_w=self.int4_gate_up.dequantize(),
+                                     up_w=h.new_empty(0), eps=norm.eps)
         if tokens <= packed_max and _packable(h, self.gate_proj.weight):
             # decode-sized: the weight-streaming GEMM on the packed gate/up with
             # the SiLU*up epilogue; the norm either in its own kernel (faster on
@@ -358,6 +421,8 @@ class LlamaDecodeLayer(nn.Module):
 
     def _down(self, inter: torch.Tensor, h: torch.Tensor, ctx: Optional[_StepContext]) -> torch.Tensor:
         """h + inter @ down_proj^T (residual in the GEMM epilogue)."""
+        if self.int4_down is not None:
+            return _int4_project(inter, self.int4_down, h)
         shp = h.shape
         h2 = h.reshape(-1, shp[-1])
         i2 = inter.reshape(-1, inter.shape[-1])
@@ -475,6 +540,28 @@ class LlamaForCausalLM(nn.Module):
         self.config = config
         self.model = LlamaModel(config)
         self.lm_head = nn.Linear(config.dim, config.vocab_size, bias=False)
+        self.int4_lm_head = None
+
+    def quantize_weights_int4(self, group_size: int = 128, lm_head: bool = True) -> None:
+        """Holds every projection (and with ``lm_head`` the vocabulary
+        projection) in 4 bits with group scales (``int4_linear.Int4Weight``) and
+        frees its 16-bit weight: the module's state dict then lacks them, and a
+        CUDA graph captured before must be captured again.  ``group_size``: 32, 64
+        or 128 columns; it and 64 must divide every projection's width.  Takes
+        the layers one by one, so that it needs little memory on top."""
+        if self.int4_lm_head is not None or self.model.layers[0].int4_down is not None:
+            raise RuntimeError("the weights are in 4 bits already")
+        widths = {self.config.dim, self.config.inter_dim,
+                  self.config.num_heads * self.config.head_dim}
+        if group_size not in (32, 64, 128) or any(w % max(64, group_size) for w in widths):
+            raise ValueError(f"group_size {group_size} (32, 64 or 128) and 64 must divide the "
+                             f"projections' widths {sorted(widths)}")
+        for layer in self.model.layers:
+            layer.quantize_weights_int4(group_size)
+        if lm_head:
+            from .int4_linear import Int4Weight
+            self.int4_lm_head = Int4Weight(self.lm_head.weight, group_size=group_size)
+            _drop(self.lm_head)
 
     def forward(
         self,
@@ -494,6 +581,8 @@ class LlamaForCausalLM(nn.Module):
         hidden = self.model(input_ids, positions=positions, kv_cache=kv_cache, mask=mask)
         if last_token_only:
             hidden = hidden[:, -1:, :]
+        if self.int4_lm_head is not None:
+            return _int4_project(hidden, self.int4_lm_head)
         return self.lm_head(hidden)
 
     # -- construction helpers ----------------------------------------------

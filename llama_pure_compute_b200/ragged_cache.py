@@ -57,14 +57,17 @@ class RaggedKVCache:
         self.bases: List[int] = bases
         self.total_rows = acc
         self.max_seq_len = max(caps)
-        shape = (n_kv_heads, self.total_rows, head_dim)
-        self.k_cache = [torch.empty(shape, dtype=dtype, device=self.device) for _ in range(num_layers)]
-        self.v_cache = [torch.empty(shape, dtype=dtype, device=self.device) for _ in range(num_layers)]
         self.seq_base = torch.tensor(bases, dtype=torch.int64, device=self.device)
         self.seq_cap = torch.tensor(caps, dtype=torch.int32, device=self.device)
         self.seq_lens = torch.zeros(len(caps), dtype=torch.int32, device=self.device)
         self._ws = None
+        self._allocate()
         self.select(range(len(caps)))
+
+    def _allocate(self) -> None:
+        shape = (self.n_kv_heads, self.total_rows, self.head_dim)
+        self.k_cache, self.v_cache = ([torch.empty(shape, dtype=self.dtype, device=self.device)
+                                       for _ in range(self.num_layers)] for _ in range(2))
 
     @property
     def num_sequences(self) -> int:
