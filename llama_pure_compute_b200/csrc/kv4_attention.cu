@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
   // each lane has one head's scores.  Lane (r, t) holds column r's dims of words
   // t*KW .. t*KW + KW - 1: word w covers dims 4w..4w+3 of each group.
   const int qh = NH == 1 ? r >> 1 : r;
-  const bool has_q = qh < heads && (NH == 2 || !(r & 1));
+  const bool has_q = qh < heads;
   uint32_t qb[KW][2][2];
   float qs0 = 0.f, qs1 = 0.f, amax = 0.f;
   float qv[KW][8];
@@ -327,13 +327,21 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
   if (amax > 0.f && amax < INFINITY) e = 14 - ((int)(__float_as_uint(amax) >> 23) - 127);
   e = max(-100, min(100, e));
   const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+  // NH = 1: operands of the bytes (q0 | 0) and of their upper nibbles (-q0 | q1 / 16),
+  // for the even | odd columns; NH = 2: of the lower nibbles (q0) and the upper (q1 / 16)
 #pragma unroll
   for (int w = 0; w < KW; ++w)
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float f = g ? up * 0.0625f : up;
-      qb[w][g][0] = pack_half2(qv[w][g * 4 + 0] * f, qv[w][g * 4 + 2] * f);
-      qb[w][g][1] = pack_half2(qv[w][g * 4 + 1] * f, qv[w][g * 4 + 3] * f);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t q0 = pack_half2(qv[w][i] * up, qv[w][i + 2] * up);
+      const uint32_t q1 = pack_half2(qv[w][4 + i] * (up * 0.0625f), qv[w][6 + i] * (up * 0.0625f));
+      if constexpr (NH == 1) {
+        qb[w][0][i] = r & 1 ? 0u : q0;
+        qb[w][1][i] = r & 1 ? q1 : q0 ^ 0x80008000u;
+      } else {
+        qb[w][0][i] = q0;
+        qb[w][1][i] = q1;
+      }
     }
   // what this lane needs of its score columns: head t, or heads 2t and 2t + 1
   float cs[NH], z0[NH], z1[NH], M[NH], l[NH], a0s[NH], a1s[NH];
@@ -347,15 +355,17 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
     M[n] = -INFINITY;
     l[n] = a0s[n] = a1s[n] = 0.f;
   }
-  float acc[2][VM][4];
+  constexpr int AG = NH;  // NH = 1: columns 2t and 2t + 1 are the groups of head t
+  float acc[AG][VM][4];
 #pragma unroll
-  for (int g = 0; g < 2; ++g)
+  for (int g = 0; g < AG; ++g)
 #pragma unroll
     for (int i = 0; i < VM; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[g][i][j] = 0.f;
 
-  constexpr uint32_t LOW = 0x000F000Fu, HIGH = 0x00F000F0u;
+  constexpr uint32_t LOW = 0x000F000Fu, HIGH = 0x00F000F0u, BYTES = 0x00FF00FFu;
+  const uint32_t even = r & 1 ? 0u : 0xFFFFFFFFu;
   // this lane's row of the V matrices: lanes 0-7 keys 0-7 and 8-15 keys 8-15 of
   // the first piece, 16-31 the same of the second
   const uint32_t vsrc = (lane & 15) * CB + (D == 32 ? 0 : L::place(lane & 7, lane >> 4) * 16);
@@ -394,13 +404,22 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
       float c0[4], c1[4];
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const uint32_t a8 = wa[w] >> 8, b8 = wb[w] >> 8;
-        if (w == 0) {
-          mma_f16_first(c0, wa[w] & LOW, wb[w] & LOW, a8 & LOW, b8 & LOW, qb[w][0][0], qb[w][0][1]);
-          mma_f16_first(c1, wa[w] & HIGH, wb[w] & HIGH, a8 & HIGH, b8 & HIGH, qb[w][1][0], qb[w][1][1]);
+        if constexpr (NH == 1) {
+          const uint32_t a0 = wa[w] & BYTES, b0 = wb[w] & BYTES;
+          const uint32_t a1 = __byte_perm(wa[w], 0u, 0x4341), b1 = __byte_perm(wb[w], 0u, 0x4341);
+          if (w == 0) mma_f16_first(c0, a0, b0, a1, b1, qb[w][0][0], qb[w][0][1]);
+          else mma_f16(c0, a0, b0, a1, b1, qb[w][0][0], qb[w][0][1]);
+          mma_f16(c0, a0 & HIGH, b0 & HIGH, a1 & HIGH, b1 & HIGH, qb[w][1][0], qb[w][1][1]);
         } else {
-          mma_f16(c0, wa[w] & LOW, wb[w] & LOW, a8 & LOW, b8 & LOW, qb[w][0][0], qb[w][0][1]);
-          mma_f16(c1, wa[w] & HIGH, wb[w] & HIGH, a8 & HIGH, b8 & HIGH, qb[w][1][0], qb[w][1][1]);
+          const uint32_t a8 = wa[w] >> 8, b8 = wb[w] >> 8;
+          if (w == 0) {
+            mma_f16_first(c0, wa[w] & LOW, wb[w] & LOW, a8 & LOW, b8 & LOW, qb[w][0][0], qb[w][0][1]);
+            mma_f16_first(c1, wa[w] & HIGH, wb[w] & HIGH, a8 & HIGH, b8 & HIGH, qb[w][1][0],
+                          qb[w][1][1]);
+          } else {
+            mma_f16(c0, wa[w] & LOW, wb[w] & LOW, a8 & LOW, b8 & LOW, qb[w][0][0], qb[w][0][1]);
+            mma_f16(c1, wa[w] & HIGH, wb[w] & HIGH, a8 & HIGH, b8 & HIGH, qb[w][1][0], qb[w][1][1]);
+          }
         }
       }
 #pragma unroll
@@ -411,7 +430,8 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
         unpack_sm<T>(w.y, s1, m1);
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
-          const float sc = fmaf(s1, c1[2 * i + n], s0 * c0[2 * i + n]);
+          const float sc = NH == 1 ? fmaf(s1, c0[2 * i + 1], s0 * c0[2 * i])
+                                   : fmaf(s1, c1[2 * i + n], s0 * c0[2 * i + n]);
           x[u][i][n] = fmaf(sc, cs[n], fmaf(m1, z1[n], m0 * z0[n]));
         }
       }
@@ -449,12 +469,15 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
         a0s[n] *= f;
         a1s[n] *= f;
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < AG; ++g)
 #pragma unroll
           for (int i = 0; i < VM; ++i) {
-            const int c = NH == 1 ? g : n;
-            acc[g][i][c] *= f;
-            acc[g][i][2 + c] *= f;
+            acc[g][i][n] *= f;
+            acc[g][i][2 + n] *= f;
+            if constexpr (NH == 1) {
+              acc[g][i][1] *= f;
+              acc[g][i][3] *= f;
+            }
           }
       }
     }
@@ -487,8 +510,10 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
           }
         }
         if constexpr (NH == 1) {
-          // the odd columns are free: 2t and 2t + 1 carry head t's P s0 and P s1
-          pb[0][i] = pb[1][i] = transpose8(pack_half2(p[0] * s0, p[0] * s1));
+          // columns 2t and 2t + 1 carry head t's groups: the bytes times (P s0 | 0) and
+          // their upper nibbles times (-P s0 | P s1) leave the lower nibbles in one
+          pb[1][i] = transpose8(pack_half2(-p[0] * s0, p[0] * s1));
+          pb[0][i] = (pb[1][i] ^ 0x80008000u) & even;
         } else {
           pb[0][i] = transpose8(pack_half2(p[0] * s0, p[1] * s0));
           pb[1][i] = transpose8(pack_half2(p[0] * s1, p[1] * s1));
@@ -504,9 +529,17 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
 #pragma unroll
         for (int i = 0; i < (VM == 1 ? 1 : 2); ++i) {
           const uint32_t lo = v[2 * i], hi = v[2 * i + 1];
-          const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
-          mma_f16(acc[0][j + i], lo & LOW, lo8 & LOW, hi & LOW, hi8 & LOW, pb[0][0], pb[0][1]);
-          mma_f16(acc[1][j + i], lo & HIGH, lo8 & HIGH, hi & HIGH, hi8 & HIGH, pb[1][0], pb[1][1]);
+          if constexpr (NH == 1) {
+            const uint32_t l0 = lo & BYTES, h0 = hi & BYTES;
+            const uint32_t l1 = __byte_perm(lo, 0u, 0x4341), h1 = __byte_perm(hi, 0u, 0x4341);
+            mma_f16(acc[0][j + i], l0, l1, h0, h1, pb[0][0], pb[0][1]);
+            mma_f16(acc[0][j + i], l0 & HIGH, l1 & HIGH, h0 & HIGH, h1 & HIGH, pb[1][0], pb[1][1]);
+          } else {
+            const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+            mma_f16(acc[0][j + i], lo & LOW, lo8 & LOW, hi & LOW, hi8 & LOW, pb[0][0], pb[0][1]);
+            mma_f16(acc[AG - 1][j + i], lo & HIGH, lo8 & HIGH, hi & HIGH, hi8 & HIGH, pb[1][0],
+                    pb[1][1]);
+          }
         }
       }
     }
@@ -532,11 +565,12 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
     for (int i = 0; i < VM; ++i) {
       // rows r and r + 8 of product i are the two dims of unit 8i + r
       const int d = 2 * (8 * i + r);
+      constexpr int g1 = AG - 1;
       const int n1 = NH == 1 ? 1 : n;
       p[d] = fmaf(acc[0][i][n], 16777216.f, a0s[n]);
       p[d + 1] = fmaf(acc[0][i][2 + n], 16777216.f, a0s[n]);
-      p[d + D / 2] = fmaf(acc[1][i][n1], 1048576.f, a1s[n]);
-      p[d + D / 2 + 1] = fmaf(acc[1][i][2 + n1], 1048576.f, a1s[n]);
+      p[d + D / 2] = fmaf(acc[g1][i][n1], 1048576.f, a1s[n]);
+      p[d + D / 2 + 1] = fmaf(acc[g1][i][2 + n1], 1048576.f, a1s[n]);
     }
     if (r == 0) {
       p[D] = M[n];
