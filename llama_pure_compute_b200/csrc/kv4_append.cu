@@ -390,12 +390,15 @@ int append(const lpc_kv4* kv, const void* qkv, const int64_t* pos, const void* c
            cudaStream_t s) {
   constexpr int C = D / 16;
   const int all = H + 2 * kv->kv_heads;
-  // whole warps, no more threads than the token has chunks
-  const int threads = std::min(THREADS, (all * C + 31) / 32 * 32);
-  const int hpb = threads / C;
-  const int steps = (all + hpb - 1) / hpb;
-  const int K = steps < 2 ? 1 : 2;
-  Launch l(dim3((unsigned)(batch * seq), (unsigned)((all + K * hpb - 1) / (K * hpb))), threads, s);
+  // two heads a thread, one where that would leave SMs without a CTA; CTAs of equal
+  // size (whole warps), no thread without a head but in the last one
+  const int chunks = all * C;
+  const int K = chunks > THREADS && batch * seq * ((chunks + 2 * THREADS - 1) / (2 * THREADS)) >=
+                                        2 * lpc::current_device_sms() ? 2 : 1;
+  const int ctas = (chunks + K * THREADS - 1) / (K * THREADS);
+  const int threads = std::min(THREADS, ((chunks + K * ctas - 1) / (K * ctas) + 31) / 32 * 32);
+  Launch l(dim3((unsigned)(batch * seq), (unsigned)((chunks + K * threads - 1) / (K * threads))),
+           threads, s);
   const lpc::Kv4Rows rows = lpc::kv4_rows(kv);
 #define LPC_APPEND(KK)                                                                          \
   cudaLaunchKernelEx(&l.cfg, kv4_append_kernel<T, TT, D, KK>, (const T*)qkv, pos,               \
