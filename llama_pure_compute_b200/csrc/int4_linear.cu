@@ -10,16 +10,9 @@
 // instructions a code costs.  mma.sync m16n8k16 takes 16 weight rows (A) by 8
 // tokens (B); a packed 32-bit word holds exactly the lane's 8 codes of one
 // product, in the order in which masks pick them:
-//   fp16: (w & 0x000F000F) is a pair of subnormal halves c * 2^-24, exactly;
-//         0x00F000F0 picks rows r + 8, 16-fold.  5 instructions a word.
-//   bf16: (w & 0x000F000F) | 0x43004300 is the pair 128 + c, exactly (a bf16
-//         subnormal times x would underflow the fp32 sum).  7 instructions;
-//         the 128 is taken out again with the group's sum of x, which
-//         costs the fp32 accumulator about 5 of its 24 bits and leaves an error
-//         some hundred times below the output's rounding.
-// The sum of x over a group is one more product, of a row of ones.
-// tcgen05 would want the weights converted into shared memory for 128-row
-// tiles: at these token counts more work than the products themselves.
+// (w & 0x000F000F) is a pair of subnormal halves c * 2^-24, exactly, and x enters
+// as fp16 too.  tcgen05 would want whole 128-row tiles of converted weights
+// (int4_many.cu): at these token counts more work than the products themselves.
 //
 // Packed weight: tiles of 16 rows x 64 columns, 512 contiguous bytes, 16 a
 // lane, read with cp.async into the lane's own slots (no barrier), followed by
@@ -58,14 +51,16 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The 8 codes of a word as the A operand: rows r, r + 8 (16-fold) of columns
-// 2t.., then the same rows of columns 2t + 8...  Code c of row r is the subnormal c * 2^-24.
+// The 8 codes of a word as the A operand, columns 2t.. and 2t + 8..: rows r + 8
+// are the upper nibbles (16-fold), rows r whole bytes, c_r + 16 c_{r+8}, so that the
+// lower nibbles need no mask of their own: the accumulator of row r + 8, which the
+// same lane holds, is taken off that of row r once a group.  Four instructions a
+// word; the accumulator loses 4 of its 24 bits.  Code c is the subnormal c * 2^-24.
 __device__ __forceinline__ void operand(uint32_t w, uint32_t (&a)[4]) {
-  const uint32_t v = w >> 8;
-  a[0] = w & 0x000F000Fu;
+  a[0] = w & 0x00FF00FFu;
   a[1] = w & 0x00F000F0u;
-  a[2] = v & 0x000F000Fu;
-  a[3] = v & 0x00F000F0u;
+  a[2] = __byte_perm(w, 0u, 0x4341);
+  a[3] = a[2] & 0x00F000F0u;
 }
 
 template <typename T>
@@ -286,6 +281,7 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
       advance();
       const uint8_t* s = ring + at;
       at = at == (C::NST - 1) * C::STAGE ? 0 : at + C::STAGE;
+      uint4 wv[MT];
 #pragma unroll
       for (int g = 0; g < C::SG; ++g) {
         float acc[MT][4];
@@ -299,11 +295,11 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
           const uint4 xv = *reinterpret_cast<const uint4*>(pc + half * 64);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            const uint2 w = *reinterpret_cast<const uint2*>(
-                s + (m * C::TILES + (half >> 1)) * 512 + lane * 16 + (half & 1) * 8);
+            const uint8_t* at_w = s + (m * C::TILES + (half >> 1)) * 512 + lane * 16;
+            if (!(half & 1)) wv[m] = *reinterpret_cast<const uint4*>(at_w);  // and the next half's
             uint32_t a[4], b[4];
-            operand(w.x, a);
-            operand(w.y, b);
+            operand(half & 1 ? wv[m].z : wv[m].x, a);
+            operand(half & 1 ? wv[m].w : wv[m].y, b);
             mma(acc[m], a, xv.x, xv.y);
             mma(acc[m], b, xv.z, xv.w);
           }
@@ -323,7 +319,7 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
           // the sum is divided at the end
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
-            sum[m][i] = fmaf(lo.x, acc[m][i], fmaf(lo.y, x2[i], sum[m][i]));
+            sum[m][i] = fmaf(lo.x, acc[m][i] - acc[m][2 + i], fmaf(lo.y, x2[i], sum[m][i]));
             sum[m][NC + i] = fmaf(hi.x, acc[m][2 + i], fmaf(hi.y, x2[i] * 16.f, sum[m][NC + i]));
           }
         }
@@ -589,6 +585,10 @@ __global__ void __launch_bounds__(NW * 32)
             }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
+              if constexpr (std::is_same<T, __half>::value) {
+                acc[m][j][0] -= acc[m][j][2];
+                acc[m][j][1] -= acc[m][j][3];
+              }
               sum[m][j][0] = fmaf(s0, acc[m][j][0], fmaf(m0, ones[j][0], sum[m][j][0]));
               sum[m][j][1] = fmaf(s0, acc[m][j][1], fmaf(m0, ones[j][1], sum[m][j][1]));
               sum[m][j][2] = fmaf(s1, acc[m][j][2], fmaf(m1, ones[j][0], sum[m][j][2]));
