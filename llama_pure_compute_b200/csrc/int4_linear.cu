@@ -181,8 +181,7 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
   for (int i = 0; i < C::NST - 1; ++i) advance();
   lpc::pdl_wait();
 
-  // x of this warp's columns.  All tokens' loads of a stretch of 256 columns
-  // are in flight at once; a range of one stretch is read once.
+  // x of this warp's columns, in stretches of 256 (8 a lane)
   constexpr bool SCALE = !std::is_same<T, __half>::value;
   float down[NC];  // 2^-e of tokens 2t (and 2t + 1)
 #pragma unroll
@@ -190,75 +189,91 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
   {
     const int width = nc * C::CK;
     const T* src = x + c0 * C::CK + lane * 8;
-    uint4 u[TC];
-    auto load = [&](int c) {
+    auto load = [&](int tk, int st) {
+      return tk < tokens && st * 256 + lane * 8 < width
+                 ? lpc::ld_dep16(src + (int64_t)tk * k + st * 256) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    auto largest = [&](float a, const uint4& u) {
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int tk = 0; tk < TC; ++tk)
-        if (tk < tokens) {
-          u[tk] = make_uint4(0u, 0u, 0u, 0u);
-          if (c + lane * 8 < width) u[tk] = lpc::ld_dep16(src + (int64_t)tk * k + c);
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = pair_f<T>(w[i]);
+        a = fmaxf(a, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
+      return a;
+    };
+    auto factor = [&](int tk, float most) {  // 2^e of a token; keeps 2^-e where it is this lane's
+      // the bits of a non-negative float order as integers do
+      const float a = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+      int e = 0;
+      if (a > 0.f && a < INFINITY) e = min(126, 14 - ((int)(__float_as_uint(a) >> 23) - 127));
+      const float d = __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (tk == NC * t + i) down[i] = d;
+      return __uint_as_float((uint32_t)(127 + e) << 23);
+    };
+    auto keep = [&](int tk, int st, const uint4& u, float up) {
+      uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = pair_f<T>(w[i]);
+        if constexpr (SCALE) {
+          const __half2 h = __floats2half2_rn(f.x * up, f.y * up);
+          w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        sum += f.x * up + f.y * up;
+      }
+      const int col = st * 256 + lane * 8;
+      if (col < width)
+        *reinterpret_cast<uint4*>(xw + tk * xrow + col * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+      for (int o = 1; o < GS / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      // in the units of the accumulators, which hold c * 2^-24
+      if (col < width && col % GS == 0) xs[(col / GS) * 8 + tk] = sum * 0x1p-24f;
+    };
+    // TK tokens by ST stretches at once: every load in flight, each value read once
+    auto block = [&](auto tks, auto sts, int tk0) {
+      constexpr int TK = decltype(tks)::value, ST = decltype(sts)::value;
+      uint4 u[TK][ST];
+#pragma unroll
+      for (int i = 0; i < TK; ++i)
+        if (tk0 + i < tokens)
+#pragma unroll
+          for (int j = 0; j < ST; ++j) u[i][j] = load(tk0 + i, j);
+#pragma unroll
+      for (int i = 0; i < TK; ++i)
+        if (tk0 + i < tokens) {
+          float up = 1.f;
+          if constexpr (SCALE) {
+            float a = 0.f;
+#pragma unroll
+            for (int j = 0; j < ST; ++j) a = largest(a, u[i][j]);
+            up = factor(tk0 + i, a);
+          }
+#pragma unroll
+          for (int j = 0; j < ST; ++j)
+            if (j * 256 < width) keep(tk0 + i, j, u[i][j], up);
         }
     };
-    load(0);
-    float up[TC];
-#pragma unroll
-    for (int tk = 0; tk < TC; ++tk) up[tk] = SCALE ? 0.f : 1.f;
-    if constexpr (SCALE) {
-      for (int c = 0;;) {
-#pragma unroll
-        for (int tk = 0; tk < TC; ++tk)
-          if (tk < tokens) {
-            const uint32_t w[4] = {u[tk].x, u[tk].y, u[tk].z, u[tk].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 f = pair_f<T>(w[i]);
-              up[tk] = fmaxf(up[tk], fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-          }
-        c += 256;
-        if (c >= width) break;
-        load(c);
+    using one = std::integral_constant<int, 1>;
+    using four = std::integral_constant<int, 4>;
+    if (width <= 256) {
+      block(std::integral_constant<int, TC>{}, one{}, 0);
+    } else if (width <= 1024) {
+      constexpr int TK = TC == 1 ? 1 : 2;
+      for (int tk = 0; tk < tokens; tk += TK) block(std::integral_constant<int, TK>{}, four{}, tk);
+    } else {
+      for (int tk = 0; tk < tokens; ++tk) {
+        float up = 1.f;
+        if constexpr (SCALE) {
+          float a = 0.f;
+          for (int st = 0; st * 256 < width; ++st) a = largest(a, load(tk, st));
+          up = factor(tk, a);
+        }
+        for (int st = 0; st * 256 < width; ++st) keep(tk, st, load(tk, st), up);
       }
-      if (width > 256) load(0);
-#pragma unroll
-      for (int tk = 0; tk < TC; ++tk)
-        if (tk < tokens) {
-          // the bits of a non-negative float order as integers do
-          const float a = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(up[tk])));
-          int e = 0;
-          if (a > 0.f && a < INFINITY) e = min(126, 14 - ((int)(__float_as_uint(a) >> 23) - 127));
-          up[tk] = __uint_as_float((uint32_t)(127 + e) << 23);
-          const float d = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-          for (int i = 0; i < NC; ++i)
-            if (tk == NC * t + i) down[i] = d;
-        }
-    }
-    for (int c = 0; c < width;) {
-#pragma unroll
-      for (int tk = 0; tk < TC; ++tk)
-        if (tk < tokens) {
-          uint32_t w[4] = {u[tk].x, u[tk].y, u[tk].z, u[tk].w};
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = pair_f<T>(w[i]);
-            if constexpr (SCALE) {
-              const __half2 h = __floats2half2_rn(f.x * up[tk], f.y * up[tk]);
-              w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            sum += f.x * up[tk] + f.y * up[tk];
-          }
-          const int col = c + lane * 8;
-          if (col < width)
-            *reinterpret_cast<uint4*>(xw + tk * xrow + col * 2) = make_uint4(w[0], w[1], w[2], w[3]);
-#pragma unroll
-          for (int o = 1; o < GS / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          // in the units of the accumulators, which hold c * 2^-24
-          if (col < width && col % GS == 0) xs[(col / GS) * 8 + tk] = sum * 0x1p-24f;
-        }
-      c += 256;
-      if (c < width) load(c);
     }
   }
   __syncwarp();
