@@ -4,21 +4,30 @@
 //
 // epilogues: store, residual (+ resid), SwiGLU (silu(gate) * up).
 //
-// Bound: HBM, by the weight stream of k/2 + 4 k/group bytes a row; a byte of
-// codes has 4 FLOPs a token, so up to about 30 tokens the tensor cores are not
-// the limit even on mma.sync, and what has to be kept small is the number of
-// instructions a code costs.  mma.sync m16n8k16 takes 16 weight rows (A) by 8
-// tokens (B); a packed 32-bit word holds exactly the lane's 8 codes of one
-// product, in the order in which masks pick them:
-// (w & 0x000F000F) is a pair of subnormal halves c * 2^-24, exactly, and x enters
-// as fp16 too.  tcgen05 would want whole 128-row tiles of converted weights
-// (int4_many.cu): at these token counts more work than the products themselves.
+// Bound: HBM, by the weight stream of k/2 + 4 k/group bytes a row, and behind it
+// the instructions a code costs: HBM's rate leaves an SM's four schedulers about
+// 1.3 instructions a 32-bit word of 8 codes and lane.  So codes are never
+// converted.  mma.sync m16n8k16 takes 16 weight rows (A) by 8 tokens (B); a
+// packed word holds exactly the lane's 8 codes of one product, in the order in
+// which masks pick them, and a code in the low bits of a half is the subnormal
+// c * 2^-24, exactly.  x enters as fp16 too.
+//
+// Three kernels; pick() chooses by the token count and what of x fits:
+//   FEW   up to 8 tokens, x in shared memory (int4_few_kernel, below);
+//   MID   up to 16 tokens on smaller weights, x from the caches (int4_mid_kernel);
+//   MANY  the rest up to 64 tokens: tcgen05 (int4_many.cu), which wants whole
+//         128-row tiles of converted weights, at few tokens more work than the
+//         products themselves.
+// Measured at groups of 128, bf16 (us; in brackets the stream at 6397 GB/s): one
+// token, 128,256 x 4096 44 (43.7) and 4096 x 4096 3.7 (1.4: the launch, x and one
+// round of loads); SwiGLU 2 x 11,008 x 4096 at 1 / 4 / 8 tokens 10.8 / 12.2 / 15.3
+// (7.5); 4096 x 11,008 at 4 tokens 8.5 (3.8).
 //
 // Packed weight: tiles of 16 rows x 64 columns, 512 contiguous bytes, 16 a
 // lane, read with cp.async into the lane's own slots (no barrier), followed by
-// the group numbers, 64 bytes per tile row and group.  The 8 warps of a CTA
-// share a tile row's k range and add their partial sums through shared memory;
-// CTAs walk over the tile rows, and the weight stream runs on across them.
+// the group numbers, 64 bytes per tile row and group.  The warps of a CTA share
+// a tile row's k range and add their partial sums through shared memory; CTAs
+// walk over the tile rows, and the weight stream runs on across them.
 #include <algorithm>
 #include <atomic>
 #include <cstdlib>
@@ -76,10 +85,16 @@ enum { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_SWIGLU = 2 };
 // ---------------------------------------------------------------------------
 // Up to 8 tokens whose x fits shared memory.  CTAs of 16 warps; each warp keeps
 // its column range of x there as fp16 operands, scaled per token by a power of
-// two (largest value about 2^14), so bf16 takes the 5-instruction unpacking
+// two (largest value about 2^14), so that bf16 has the four-instruction operands
 // too: what the scaling loses lies 2^-38 below the largest value.  The sums of
 // x over the groups are taken once, in fp32.  TC is 1 or 8: one token alone has
 // half the accumulators and leaves room for two CTAs an SM.
+// What took it there (128,256 x 4096, one token): 58 us with 8 warps and a barrier
+// an item, 50.6 with the sums of several items at one barrier and 16 warps, 45.1
+// with x's sums and numbers read once a group, 43.5 with the operands of operand().
+// With several tokens the instructions bound it: a code word has 4 of unpacking
+// and its product, whatever the token count, but the accumulators and x's operands
+// of 8 tokens leave room for one CTA an SM.
 // ---------------------------------------------------------------------------
 constexpr int64_t MAX_SMEM = 232448;   // of a CTA
 constexpr int64_t HALF_SMEM = 115712;  // of each of two CTAs on an SM
@@ -403,6 +418,8 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
 // group's sum of x, which costs the fp32 accumulator about 5 of its 24 bits and
 // leaves an error some hundred times below the output's rounding.  The sum of x is
 // one more product, of a row of ones, kept in shared memory for the next items.
+// 4096 x 4096 at 16 tokens: 6.2 us (stream 1.4); the loads of x, one of each 8
+// columns and token for every tile row, bound it.
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void operand_of(uint32_t w, uint32_t (&a)[4]) {
@@ -443,8 +460,8 @@ struct Cfg {
 template <typename T, int GS, int MT, int NT, int NW>
 __global__ void __launch_bounds__(NW * 32)
     int4_mid_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ numbers,
-                       const T* x, const T* resid, T* out, int tokens, int64_t n_out,
-                       int k, int items, int epi, int keep_sums) {
+                   const T* x, const T* resid, T* out, int tokens, int64_t n_out, int k, int items,
+                   int epi, int keep_sums) {
   using C = Cfg<GS, MT, NT, NW>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -870,11 +887,16 @@ enum Kernel { FEW, MID, MANY };
 // Measured, us, mid / many: 4096 x 4096 at 16 tokens 6.3 / 10.4, 4096 x 11,008 at 8
 // tokens 10.2 / 19, 22,016 x 4096 at 16 tokens 30 / 23.
 constexpr int64_t MID_MOST = 64 << 20;
+// x fits the few-token kernel's shared memory, with one tile row an item or two
+// (the rings round differently).
+template <int GS, int TC>
+bool few_fits(int k, int64_t tokens) {
+  return tokens <= TC && std::max(FewCfg<GS, 1, TC>::smem(k, (int)tokens),
+                                  FewCfg<GS, 2, TC>::smem(k, (int)tokens)) <= MAX_SMEM;
+}
 template <int GS>
 Kernel pick(const lpc_w4* w, int64_t tokens) {
-  if ((tokens == 1 && FewCfg<GS, 2, 1>::smem(w->k, 1) <= MAX_SMEM) ||
-      (tokens <= 8 && FewCfg<GS, 2, 8>::smem(w->k, (int)tokens) <= MAX_SMEM))
-    return FEW;
+  if (few_fits<GS, 1>(w->k, tokens) || few_fits<GS, 8>(w->k, tokens)) return FEW;
   return tokens <= 16 && (w->n_out << w->layout) * w->k <= MID_MOST ? MID : MANY;
 }
 Kernel pick(const lpc_w4* w, int64_t tokens) {
@@ -901,7 +923,7 @@ int launch_nt(const lpc_w4* w, const void* x, void* out, const void* resid, int6
   if (pick<GS>(w, tokens) == MID)
     return tokens <= 8 ? launch_mid_mt<T, GS, 1>(w, x, out, resid, tokens, epi, s)
                        : launch_mid_mt<T, GS, 2>(w, x, out, resid, tokens, epi, s);
-  if (tokens == 1 && FewCfg<GS, 2, 1>::smem(w->k, 1) <= MAX_SMEM)
+  if (few_fits<GS, 1>(w->k, tokens))
     return launch_few_mt<T, GS, 1>(w, x, out, resid, tokens, epi, s);
   return launch_few_mt<T, GS, 8>(w, x, out, resid, tokens, epi, s);
 }
@@ -915,7 +937,8 @@ int launch_gs(const lpc_w4* w, const void* x, void* out, const void* resid, int6
 }
 
 bool shape_ok(int64_t n_out, int k, int group, int layout) {
-  return n_out > 0 && n_out <= (1 << 24) && k > 0 && k <= (1 << 20) && k % 64 == 0 &&
+  return n_out > 0 && n_out <= (1 << 24) && k > 0 && k <= (1 << 20) && n_out * k <= (1LL << 38) &&
+         k % 64 == 0 &&
          (group == 32 || group == 64 || group == 128) && k % group == 0 &&
          (layout == 0 || layout == 1);
 }

@@ -1,4 +1,4 @@
-// Products with 4-bit weights for more tokens than int4_linear.cu's kernel takes
+// Products with 4-bit weights for more tokens than int4_linear.cu's kernels take
 // (up to 64): tcgen05, weights as the M operand.
 //
 // mma.sync needs one instruction for 16 rows x 8 tokens x 16 columns: from 16
@@ -16,8 +16,13 @@
 // A step is a chain of waits and dependent instructions of about 1000 cycles, far
 // more than its share of HBM's time (175), so the CTAs are small, four an SM, and
 // their chains overlap.
-// The rounding of a weight to fp16 (2^-12 of it on average) lies well below the
-// output's.  e is a power per weight row (int4.cuh), undone with x's in the epilogue.
+// Measured, bf16, groups of 128: 22,016 x 4096 at 16 / 32 / 64 tokens 23 / 24 / 26
+// us (stream 7.5), 4096 x 4096 at 32 / 64 12 / 14.  The chain bounds it; two
+// warpgroups a CTA (its one issuing thread then the limit) and clusters of 16 were
+// slower.
+// A weight is rounded to fp16: off by at most 2^-11 of itself, or 2^-15 of its row's
+// largest scale where that is more.  Over k these average to far below the output's
+// rounding.  e is a power per weight row (int4.cuh), undone with x's in the epilogue.
 // Few row tiles: clusters of up to 8 CTAs split the columns and add their sums
 // through distributed shared memory, in rank order.
 #include <algorithm>
@@ -259,12 +264,17 @@ __global__ void __launch_bounds__(THREADS, 4)
       xf[i] = p.x_factors && i < p.tokens
                   ? __int_as_float(lpc::ld_dep(reinterpret_cast<const int32_t*>(p.x_factors) + i)) : 1.f;
     if (lane == 0) {
-      for (int step = 0; step < nk; ++step) {
+      int step = 0;
+      for (; step < nk; ++step) {
         const int xs = step % XST;
         if (!wait(x_empty(xs), ((uint32_t)(step / XST) & 1u) ^ 1u)) break;
         lpc::mbar_arrive_expect_tx(x_full(xs), XSTAGE);
         lpc::tma_load_2d(xring + xs * XSTAGE, &tm_x, (kb0 + step) * 64, 0, x_full(xs));
       }
+      // the last loads have landed before this CTA's shared memory is let go, even
+      // where the products gave up on them
+      for (int i = max(0, step - XST); i < step; ++i)
+        if (!wait(x_full(i % XST), (uint32_t)(i / XST) & 1u)) break;
     }
     __syncwarp();
   }

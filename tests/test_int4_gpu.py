@@ -10,7 +10,13 @@ Bars, from arithmetic:
                  once (2^-23), of magnitude 143 s sum|x| for bf16 (codes enter as
                  128 + c) and as much again for the sum of x that takes the 128
                  out: 2 * 8 * 2^-23 * 143 < 2^-11 of s sum|x|; and 2^-19 of
-                 |m| sum|x|."""
+                 |m| sum|x|.  Fewer than that for the operands without the 128.
+                 From 17 tokens on (16 on weights above 2^26 values) a weight
+                 enters as fp16, off by 2^-11 |w| and 2^-15 of its row's largest
+                 s at most: `rounded` adds that in full.  Without it (normal x and
+                 w, |w| about 4.6 s): the roundings are independent, 2.7 s |x|
+                 2^-11 sqrt(k) in the mean square, and 5 of those are below the
+                 above from k = 384 on."""
 import pytest
 import torch
 
@@ -460,9 +466,13 @@ def linear_bar(x, codes, s, m, y):
     return ax @ s.double().mT * 2.0 ** -11 + ax @ m.double().abs().mT * 2.0 ** -19
 
 
-def check_linear(y, x, codes, s, m, epilogue="store", resid=None):
+def check_linear(y, x, codes, s, m, epilogue="store", resid=None, rounded=False):
     z = x.double() @ weight_ref(codes, s, m).mT
     e = linear_bar(x, codes, s, m, z)
+    if rounded:
+        ax = x.double().abs()
+        e = e + ax @ weight_ref(codes, s, m).abs().mT * 2.0 ** -11 \
+            + ax.sum(-1, keepdim=True) * s.double().abs().amax(-1) * 2.0 ** -15
     if epilogue == "residual":
         z = z + resid.double()
     if epilogue == "swiglu":
@@ -566,6 +576,173 @@ def test_linear_values(dtype):
     keep = [0, 2, 3, 5]
     assert torch.equal(z[keep], y[keep])
     assert not z[1].isfinite().any() and not z[4].isfinite().any()
+
+
+@pytest.mark.parametrize("tokens", [2, 3, 5, 7, 8])
+def test_linear_items_that_share_a_barrier(tokens):
+    """Few tokens add up several items' sums at once: full and broken batches, the
+    last item past the rows; twice the same."""
+    g = gen(tokens)
+    for n, epilogue in ((20011, "store"), (9999, "swiglu"), (2369, "residual")):
+        codes, s, m = random_weight(g, 2 * n if epilogue == "swiglu" else n, 256, 128, BF)
+        w = Int4Weight.from_codes(codes, s, m, group_size=128,
+                                  layout="swiglu" if epilogue == "swiglu" else "linear")
+        x = torch.randn(tokens, 256, device=DEV, generator=g).to(BF)
+        r = torch.randn(tokens, n, device=DEV, generator=g).to(BF) if epilogue == "residual" else None
+        y = int4_linear(x, w, epilogue, resid=r)
+        check_linear(y, x, codes, s, m, epilogue, r)
+        assert torch.equal(int4_linear(x, w, epilogue, resid=r), y)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("tokens,k,group", [
+    (1, 4160, 64), (8, 4096, 128), (3, 5504, 128), (4, 11008, 128), (1, 17408, 128), (2, 18432, 128),
+    # as much of x as fits beside the weight ring, and the next width
+    (2, 26624, 64), (2, 24576, 64), (1, 49152, 32), (1, 47104, 32), (8, 5120, 128), (7, 5120, 128)])
+def test_linear_widths_of_x(dtype, tokens, k, group):
+    """x of 256, 1024 and more columns a warp, up to where it fits no longer."""
+    g = gen(k + tokens)
+    codes, s, m = random_weight(g, 72, k, group, dtype)
+    w = Int4Weight.from_codes(codes, s, m, group_size=group)
+    x = torch.randn(tokens, k, device=DEV, generator=g).to(dtype)
+    check_linear(int4_linear(x, w), x, codes, s, m)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("tokens,n,k,group,epilogue", [
+    (8, 200, 16384, 128, "store"), (5, 40, 32768, 64, "residual"), (8, 2400, 11008, 128, "store"),
+    (9, 5000, 640, 32, "store"), (16, 5000, 640, 64, "residual"), (13, 2500, 512, 128, "swiglu"),
+    (16, 100, 16384, 32, "swiglu"), (16, 4800, 8192, 32, "store")])
+def test_linear_x_from_the_caches(dtype, tokens, n, k, group, epilogue):
+    """Up to 16 tokens whose x is not kept in shared memory: with and without kept
+    sums of x, 8 and 16 warps, one and two tile rows."""
+    g = gen(tokens + n)
+    codes, s, m = random_weight(g, 2 * n if epilogue == "swiglu" else n, k, group, dtype)
+    w = Int4Weight.from_codes(codes, s, m, group_size=group,
+                              layout="swiglu" if epilogue == "swiglu" else "linear")
+    assert w.workspace_bytes(tokens) == 0
+    x = torch.randn(tokens, k, device=DEV, generator=g).to(dtype)
+    r = torch.randn(tokens, n, device=DEV, generator=g).to(dtype) if epilogue == "residual" else None
+    y = int4_linear(x, w, epilogue, resid=r)
+    check_linear(y, x, codes, s, m, epilogue, r)
+    if r is not None:
+        assert torch.equal(int4_linear(x, w, epilogue, resid=r, out=r), y) and torch.equal(r, y)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("tokens,n,k,group,epilogue", [
+    (17, 1, 64, 32, "store"), (32, 129, 192, 64, "residual"), (33, 63, 256, 128, "swiglu"),
+    (64, 65, 4096, 128, "swiglu"), (48, 3000, 128, 32, "residual"), (64, 40000, 128, 128, "store"),
+    (20, 12000, 320, 32, "swiglu")])
+def test_linear_many_tokens(dtype, tokens, n, k, group, epilogue):
+    """17 to 64 tokens: columns split over clusters or not, ragged last tiles."""
+    g = gen(tokens + n)
+    codes, s, m = random_weight(g, 2 * n if epilogue == "swiglu" else n, k, group, dtype)
+    w = Int4Weight.from_codes(codes, s, m, group_size=group,
+                              layout="swiglu" if epilogue == "swiglu" else "linear")
+    assert (w.workspace_bytes(tokens) > 0) == (dtype == BF)
+    x = torch.randn(tokens, k, device=DEV, generator=g).to(dtype)
+    r = torch.randn(tokens, n, device=DEV, generator=g).to(dtype) if epilogue == "residual" else None
+    y = int4_linear(x, w, epilogue, resid=r)
+    check_linear(y, x, codes, s, m, epilogue, r, rounded=True)
+    if r is not None:
+        assert torch.equal(int4_linear(x, w, epilogue, resid=r, out=r), y) and torch.equal(r, y)
+
+
+@pytest.mark.parametrize("tokens", [9, 16])
+def test_linear_of_a_large_weight(tokens):
+    """The same from 9 tokens on where the weight has more than 2^26 values."""
+    g = gen(tokens)
+    codes, s, m = random_weight(g, 17000, 4096, 128, BF)
+    w = Int4Weight.from_codes(codes, s, m, group_size=128)
+    assert w.workspace_bytes(tokens) > 0
+    x = torch.randn(tokens, 4096, device=DEV, generator=g).to(BF)
+    check_linear(int4_linear(x, w), x, codes, s, m, rounded=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_linear_many_tokens_values(dtype):
+    """Groups of very different scale in a row, negative scales, rows of zeros, x of
+    very different sizes; a non-finite token stays in its row."""
+    g = gen(21)
+    n, k = 130, 512
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device=DEV, generator=g)
+    s = (torch.rand(n, 4, device=DEV, generator=g) + 0.5) * torch.tensor([1e-2, 1e-4, -3e-3, 1.0], device=DEV)
+    m = torch.randn(n, 4, device=DEV, generator=g) * torch.tensor([0.1, 1e-3, 1e-2, 8.0], device=DEV)
+    s[5], m[5] = 0, 0
+    s[6] = 0
+    s, m = s.to(dtype), m.to(dtype)
+    w = Int4Weight.from_codes(codes, s, m, group_size=128)
+    x = torch.randn(40, k, device=DEV, generator=g)
+    x[1] *= 30
+    x[2] *= 1e-4
+    x[3] = 0
+    x[4, 7] = 900.0
+    x = x.to(dtype)
+    y = int4_linear(x, w)
+    z = x.double() @ weight_ref(codes, s, m).mT
+    ax = x.double().abs()
+    e = linear_bar(x, codes, s.abs(), m, z) + ax @ weight_ref(codes, s, m).abs().mT * 2.0 ** -11 \
+        + ax.sum(-1, keepdim=True) * s.double().abs().amax(-1) * 2.0 ** -15
+    far = (y.double() - z).abs()
+    bar = z.abs() * (torch.finfo(dtype).eps / 2) + e + torch.finfo(dtype).tiny
+    assert (far <= bar).all(), (far / bar).max().item()
+    assert (y[3] == 0).all() and (y[:, 5] == 0).all()
+    x[1, 3], x[39, 500] = float("nan"), float("inf")
+    z = int4_linear(x, w)
+    keep = [i for i in range(40) if i not in (1, 39)]
+    assert torch.equal(z[keep], y[keep])
+    assert not z[1].isfinite().any() and not z[39].isfinite().any()
+
+
+def test_linear_many_tokens_in_graphs_and_streams():
+    """Two graphs and two streams at once, each call with scratch of its own."""
+    g = gen(22)
+    codes, s, m = random_weight(g, 2048, 2048, 128, BF)
+    w = Int4Weight.from_codes(codes, s, m, group_size=128)
+    xs = [torch.randn(t, 2048, device=DEV, generator=g).to(BF) for t in (24, 64)]
+    nw = torch.ones(2048, dtype=BF, device=DEV)
+    want = [int4_linear(int4_linear(ops.rmsnorm_forward(x, nw), w), w) for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(int4_linear(int4_linear(ops.rmsnorm_forward(x, nw), w), w))
+        graphs.append(gr)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    eager = []
+    for _ in range(10):
+        for x, st in zip(xs, streams):
+            with torch.cuda.stream(st):
+                eager.append(int4_linear(int4_linear(ops.rmsnorm_forward(x, nw), w), w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(eager))
+
+
+def test_views_off_the_16_byte_grid():
+    """Inputs that start in the middle of 16 bytes give what their copies give."""
+    g = gen(23)
+    codes, s, m = random_weight(g, 128, 128, 64, BF)
+    w = Int4Weight.from_codes(codes, s, m, group_size=64)
+    for tokens in (1, 12, 30):
+        x = torch.randn(tokens * 128 + 1, device=DEV, generator=g).to(BF)[1:].view(tokens, 128)
+        assert torch.equal(int4_linear(x, w), int4_linear(x.clone(), w))
+    kv = make_cache(g, 2, 2, 40, 32, BF)
+    q = torch.randn(2 * 4 * 32 + 3, device=DEV, generator=g).to(BF)[3:].view(2, 4, 32)
+    ln = torch.tensor([40, 7], dtype=torch.int32, device=DEV)
+    assert torch.equal(ops.decode_attention_int4(q, kv, ln), ops.decode_attention_int4(q.clone(), kv, ln))
+    qkv = torch.randn(2 * 8 * 32 + 1, device=DEV, generator=g).to(BF)[1:].view(2, 1, 256)
+    pos = torch.zeros(2, 1, dtype=torch.int64, device=DEV)
+    cos, sin = tables(32, 8, BF)
+    assert torch.equal(ops.rope_kv_append_int4(qkv, pos, cos, sin, kv, 4),
+                       ops.rope_kv_append_int4(qkv.clone(), pos, cos, sin, kv, 4))
 
 
 def test_weight_from_16_bits_and_back():
