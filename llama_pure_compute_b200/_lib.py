@@ -183,18 +183,18 @@ def stream_of(t: torch.Tensor) -> int:
 
 
 # A Stream object costs 2 us to make; the handle alone does not.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def call_on(index: int, fn, *args) -> int:
     """``fn(*args, stream)``: a C entry point with CUDA device ``index`` current
     and that device's current stream as its last argument."""
-    if torch.cuda.current_device() != index:
+    if _current_device() != index:
         with torch.cuda.device(index):
-            return call_on(index, fn, *args)
-    if _raw_stream is not None:
-        return fn(*args, _raw_stream(index))
-    return fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            return fn(*args, _raw_stream(index))
+    return fn(*args, _raw_stream(index))
 
 
 def dtype_code(dt: torch.dtype, what: str) -> int:

@@ -133,7 +133,8 @@ class Int4Weight:
         self._c = _lib.W4(self.data.data_ptr(), self.n_out, self.k, group_size, lay,
                           _lib.DTYPE_CODE[self.dtype])
         self.ref = ctypes.addressof(self._c)
-        self._workspace = {}
+        self._workspace = {}  # tokens -> bytes
+        self._linear = lib.lpc_int4_linear
         codes, scales, mins = codes.contiguous(), scales.contiguous(), mins.contiguous()
         self.index = codes.get_device()
         rc = _lib.call_on(self.index, lib.lpc_int4_pack, self.ref, codes.data_ptr(),
@@ -183,16 +184,17 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
         raise ValueError(f"LlamaPureComputeError: unknown epilogue {epilogue!r}")
     if (epi == 2) != (w.layout == "swiglu"):
         raise ValueError("LlamaPureComputeError: the swiglu epilogue needs a swiglu-packed weight.")
-    _require_cuda(x, "x")
-    k, n, index = w.k, w.n_out, w.index
-    shape = x.shape
-    if not shape or shape[-1] != k or x.dtype != w.dtype or x.get_device() != index:
+    index, n, k, shape = w.index, w.n_out, w.k, x.shape
+    if x.get_device() != index or not shape or shape[-1] != k or x.dtype != w.dtype:
+        _require_cuda(x, "x")
         raise ValueError("LlamaPureComputeError: x must be [..., k] in the weight's dtype and device.")
-    given = x
-    x = _dense16(x)
-    tokens = x.numel() // k
+    tokens = shape[0] if len(shape) == 2 else x.numel() // k
     if tokens > MAX_TOKENS:
         raise ValueError(f"LlamaPureComputeError: int4_linear takes at most {MAX_TOKENS} rows.")
+    xp = given = x.data_ptr()
+    if xp % 16 or not x.is_contiguous():
+        x = _dense16(x)
+        xp = x.data_ptr()
     rp = None
     if epi == 1:
         if resid is None or resid.numel() != tokens * n or not resid.is_contiguous() \
@@ -201,20 +203,22 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
         rp = resid.data_ptr()
     elif resid is not None:
         raise ValueError("LlamaPureComputeError: resid is for the residual epilogue.")
-    xp = x.data_ptr()
     if out is None:
-        out = x.new_empty((*shape[:-1], n))
+        out = x.new_empty(tokens, n) if len(shape) == 2 else x.new_empty(*shape[:-1], n)
     elif out.numel() != tokens * n or not out.is_contiguous() or out.dtype != x.dtype \
             or out.get_device() != index:
         raise ValueError("LlamaPureComputeError: out must be a contiguous [..., n_out] tensor.")
-    elif out.data_ptr() == given.data_ptr() and tokens:
+    elif out.data_ptr() == given and tokens:
         raise ValueError("LlamaPureComputeError: out must not be x.")
-    need = w.workspace_bytes(tokens)
+    if not tokens:
+        return out
+    need = w._workspace.get(tokens)
+    if need is None:
+        need = w.workspace_bytes(tokens)
     ws = x.new_empty((need + 1) // 2) if need else None
-    rc = _lib.call_on(index, _lib.load().lpc_int4_linear, w.ref, xp, out.data_ptr(), rp, tokens, epi,
+    rc = _lib.call_on(index, w._linear, w.ref, xp, out.data_ptr(), rp, tokens, epi,
                       ws.data_ptr() if need else None, need)
     if rc:
         _lib.check(rc, "int4_linear")
-    if tokens:
-        _lib.count_launch("lpc_int4_linear", 2 if need else 1)
+    _lib.launch_count += 2 if need else 1
     return out

@@ -709,18 +709,19 @@ def _int4_out(out: torch.Tensor, name: str, shape, kv: Int4KV) -> None:
                          "of the cache's dtype and device.")
 
 
-def _int4_positions(positions: torch.Tensor, B: int, S: int, kv: Int4KV) -> torch.Tensor:
-    if positions.dim() != 2 or positions.shape[0] != B or positions.shape[1] != S:
+def _int4_positions(positions: torch.Tensor, shape, kv: Int4KV) -> torch.Tensor:
+    """positions as contiguous int64 [batch, seq]; ``shape`` starts with the batch
+    and the sequence that they must have."""
+    have = positions.shape
+    if len(have) != 2 or have[0] != shape[0] or have[1] != shape[1]:
         raise ValueError("LlamaPureComputeError: positions must be [batch, seq].")
-    if positions.get_device() != kv.index:
-        raise ValueError("LlamaPureComputeError: positions must be on the cache's device.")
-    if B > kv.max_batch:
+    if have[0] > kv.max_batch:
         raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
     if positions.dtype is not torch.int64:
         if positions.dtype.is_floating_point or positions.dtype == torch.bool:
             raise TypeError("LlamaPureComputeError: positions must be integers.")
         positions = positions.to(torch.int64)
-    return positions.contiguous()
+    return positions if positions.is_contiguous() else positions.contiguous()
 
 
 def rope_kv_append_int4(
@@ -743,34 +744,37 @@ def rope_kv_append_int4(
     NaN.  A negative position skips its token (its q is zero); a position
     outside the sequence's rows or the tables skips it and sets the device
     status.  The positions of one sequence must differ."""
-    for t, n in ((qkv, "qkv"), (positions, "positions"), (cos_table, "cos"), (sin_table, "sin")):
-        _require_cuda(t, n)
+    index = kv.index
+    if qkv.get_device() != index or positions.get_device() != index \
+            or cos_table.get_device() != index or sin_table.get_device() != index:
+        for t, n in ((qkv, "qkv"), (positions, "positions"), (cos_table, "cos"), (sin_table, "sin")):
+            _require_cuda(t, n)
+        raise ValueError("LlamaPureComputeError: qkv, positions and the rope tables must be on the "
+                         "cache's device.")
     D = kv.head_dim
-    if qkv.dim() != 3 or qkv.shape[-1] != (num_heads + 2 * kv.kv_heads) * D or num_heads <= 0:
+    shape, rows = qkv.shape, cos_table.shape
+    if len(shape) != 3 or shape[2] != (num_heads + 2 * kv.kv_heads) * D or num_heads <= 0:
         raise ValueError("LlamaPureComputeError: qkv width does not match heads * head_dim.")
-    B, S, _ = qkv.shape
     if qkv.dtype != kv.dtype:
         raise TypeError("LlamaPureComputeError: qkv and cache dtypes differ.")
-    if qkv.get_device() != kv.index or cos_table.get_device() != kv.index \
-            or sin_table.get_device() != kv.index:
-        raise ValueError("LlamaPureComputeError: qkv and the rope tables must be on the cache's device.")
-    if cos_table.dim() != 2 or cos_table.shape[-1] != D or sin_table.shape != cos_table.shape \
-            or sin_table.dtype != cos_table.dtype:
+    table_dtype = cos_table.dtype
+    if len(rows) != 2 or rows[1] != D or sin_table.shape != rows or sin_table.dtype != table_dtype:
         raise ValueError("LlamaPureComputeError: rope tables must be matching [max_pos, head_dim].")
-    pos = _int4_positions(positions, B, S, kv)
+    B, S, _ = shape
+    pos = _int4_positions(positions, shape, kv)
     qkv, cos_table, sin_table = _dense16(qkv), _dense16(cos_table), _dense16(sin_table)
     if q_out is None:
-        q_out = qkv.new_empty((B, num_heads, S, D))
+        q_out = qkv.new_empty(B, num_heads, S, D)
     else:
         _int4_out(q_out, "q_out", (B, num_heads, S, D), kv)
-    rc = _lib.call_on(kv.index, _lib.load().lpc_rope_kv_append_int4, kv.ref, qkv.data_ptr(),
-                      pos.data_ptr(), cos_table.data_ptr(), sin_table.data_ptr(),
-                      cos_table.shape[0], q_out.data_ptr(), B, S, num_heads,
-                      _lib.dtype_code(cos_table.dtype, "rope_kv_append_int4"))
+    rc = _lib.call_on(index, _lib.load().lpc_rope_kv_append_int4, kv.ref, qkv.data_ptr(),
+                      pos.data_ptr(), cos_table.data_ptr(), sin_table.data_ptr(), rows[0],
+                      q_out.data_ptr(), B, S, num_heads,
+                      _lib.dtype_code(table_dtype, "rope_kv_append_int4"))
     if rc:
         _lib.check(rc, "rope_kv_append_int4")
     if B and S:
-        _lib.count_launch("lpc_rope_kv_append_int4")
+        _lib.launch_count += 1
     return q_out
 
 
@@ -785,18 +789,20 @@ def kv_read_int4(
     what ``flash_attention_v2`` needs of the context before a prompt chunk.
     Rows of negative positions are zero; so are those of positions outside the
     sequence's rows, which set the device status as well."""
-    _require_cuda(positions, "positions")
+    if positions.get_device() != kv.index:
+        _require_cuda(positions, "positions")
+        raise ValueError("LlamaPureComputeError: positions must be on the cache's device.")
     if positions.dim() != 2:
         raise ValueError("LlamaPureComputeError: positions must be [batch, seq].")
     B, S = positions.shape
-    pos = _int4_positions(positions, B, S, kv)
+    pos = _int4_positions(positions, (B, S), kv)
     shape = (B, kv.kv_heads, S, kv.head_dim)
     if k_out is None:
-        k_out = kv.key_scales.new_empty(shape)
+        k_out = kv.key_scales.new_empty(*shape)
     else:
         _int4_out(k_out, "k_out", shape, kv)
     if v_out is None:
-        v_out = kv.key_scales.new_empty(shape)
+        v_out = kv.key_scales.new_empty(*shape)
     else:
         _int4_out(v_out, "v_out", shape, kv)
     rc = _lib.call_on(kv.index, _lib.load().lpc_kv_read_int4, kv.ref, pos.data_ptr(),
@@ -804,7 +810,7 @@ def kv_read_int4(
     if rc:
         _lib.check(rc, "kv_read_int4")
     if B and S:
-        _lib.count_launch("lpc_kv_read_int4")
+        _lib.launch_count += 1
     return k_out, v_out
 
 
@@ -830,35 +836,36 @@ def decode_attention_int4(
     heads per KV head.  An empty sequence gives zeros; a length beyond the
     sequence's rows is cut to them and sets the device status.  fp32 softmax
     and accumulation; returns q's shape."""
-    _require_cuda(q, "q")
-    _require_cuda(seq_lens, "seq_lens")
+    index = kv.index
+    if q.get_device() != index or seq_lens.get_device() != index:
+        _require_cuda(q, "q")
+        _require_cuda(seq_lens, "seq_lens")
+        raise ValueError("LlamaPureComputeError: q and seq_lens must be on the cache's device.")
     if seq_lens.dtype != torch.int32:
         raise TypeError("LlamaPureComputeError: seq_lens must be int32.")
     if q.dtype != kv.dtype:
         raise TypeError("LlamaPureComputeError: q and cache dtypes differ.")
-    D = kv.head_dim
-    if q.dim() not in (3, 4) or q.shape[-1] != D or (q.dim() == 4 and q.shape[2] != 1):
+    D, shape = kv.head_dim, q.shape
+    if len(shape) not in (3, 4) or shape[-1] != D or (len(shape) == 4 and shape[2] != 1):
         raise ValueError("LlamaPureComputeError: q must be [B, H, D] with the cache's head_dim.")
-    B, H = q.shape[0], q.shape[1]
+    B, H = shape[0], shape[1]
     if H == 0 or H % kv.kv_heads:
         raise ValueError("LlamaPureComputeError: heads must be a multiple of the cache's KV heads.")
     if B > kv.max_batch:
         raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
     if seq_lens.numel() < B or not seq_lens.is_contiguous():
         raise ValueError("LlamaPureComputeError: seq_lens must have a contiguous entry per sequence.")
-    if q.get_device() != kv.index or seq_lens.get_device() != kv.index:
-        raise ValueError("LlamaPureComputeError: q and seq_lens must be on the cache's device.")
-    qc = _dense16(q)
+    q = _dense16(q)
     if out is None:
-        out = torch.empty_like(qc)
+        out = torch.empty_like(q)
     else:
-        _int4_out(out, "out", q.shape, kv)
+        _int4_out(out, "out", shape, kv)
     lib = _lib.load()
     if workspace is None:
         workspace = decode_attention_int4_workspace(kv, B, H)
-    elif workspace.get_device() != kv.index or not workspace.is_contiguous():
+    elif workspace.get_device() != index or not workspace.is_contiguous():
         raise ValueError("LlamaPureComputeError: workspace must be contiguous on the cache's device.")
-    rc = _lib.call_on(kv.index, lib.lpc_decode_attention_int4, kv.ref, qc.data_ptr(),
+    rc = _lib.call_on(index, lib.lpc_decode_attention_int4, kv.ref, q.data_ptr(),
                       seq_lens.data_ptr(), out.data_ptr(), workspace.data_ptr(), workspace.nbytes,
                       B, H, D ** -0.5 if sm_scale is None else sm_scale)
     if rc:
@@ -867,5 +874,5 @@ def decode_attention_int4(
         n = kv._kernels.get((B, H))
         if n is None:
             n = kv._kernels[B, H] = lib.lpc_decode_attention_int4_kernels(kv.ref, B, H)
-        _lib.count_launch("lpc_decode_attention_int4", n)
+        _lib.launch_count += n
     return out
