@@ -34,6 +34,18 @@
 
 #include "int4.cuh"
 
+LPC_DECLARE_STATUS(g_int4_few_status)
+
+unsigned int lpc_status_int4_few(bool clear) {
+  unsigned int v = 0;
+  cudaMemcpyFromSymbol(&v, g_int4_few_status, sizeof(v));
+  if (clear && v) {
+    unsigned int z = 0;
+    cudaMemcpyToSymbol(g_int4_few_status, &z, sizeof(z));
+  }
+  return v;
+}
+
 namespace {
 
 using lpc::Num;
@@ -115,18 +127,17 @@ struct FewCfg {
   __host__ __device__ static constexpr int64_t x_bytes(int64_t chunks, int tokens) {
     return tokens * (chunks * CK * 2 + 64) + chunks * SG * 32;
   }
-  // items whose partial sums meet at one barrier, so that it has about 128
-  // values to add whatever the number of tokens
+  // items whose partial sums are added at once: about 128 values, one a lane of four
+  // warps, whatever the number of tokens
   __host__ __device__ static constexpr int batch(int tokens) {
     return tokens >= 8 / MT ? 1 : 8 / (MT * tokens);
   }
-  // words of a warp's partial sums; 8 apart from a multiple of 16, so that 8
-  // neighbouring values of 4 warps lie in 32 banks
-  __host__ __device__ static constexpr int red(int tokens) {
-    return batch(tokens) * tokens * MT * 16 + 8;
-  }
+  // words between two tokens' partial sums: lanes 2t tokens and r rows apart write
+  // to 32 banks
+  static constexpr int TS = MT * 16 + 4;
+  __host__ __device__ static constexpr int red(int tokens) { return batch(tokens) * tokens * TS; }
   static constexpr int64_t smem(int64_t k, int tokens) {
-    return NW * (RING + x_bytes((k / CK + NW - 1) / NW, tokens) + 2 * red(tokens) * 4);
+    return NW * (RING + x_bytes((k / CK + NW - 1) / NW, tokens) + 2 * red(tokens) * 4) + 32;
   }
 };
 
@@ -153,6 +164,10 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
   const int rs = C::red(tokens);
   float* red = reinterpret_cast<float*>(smem + NW * (C::RING + (int)C::x_bytes(most, tokens)));
   float* xs = reinterpret_cast<float*>(xw + tokens * xrow);  // [group][8 tokens]
+  // two buffers of partial sums: written by all warps (full), added by four (empty)
+  const uint32_t bars = lpc::smem_u32(red + 2 * NW * rs);
+  auto full = [&](int i) { return bars + 8u * i; };
+  auto empty = [&](int i) { return bars + 16u + 8u * i; };
 
   // the weight stream: this warp's chunks of item blockIdx.x, then of the next
   const uint8_t* fcode = codes + (int64_t)blockIdx.x * MT * tile_codes + c0 * (C::TILES * 512) + lane * 16;
@@ -194,6 +209,14 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
   // are requested before the kernel that writes x is waited for
 #pragma unroll
   for (int i = 0; i < C::NST - 1; ++i) advance();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      lpc::mbar_init(full(i), NW);
+      lpc::mbar_init(empty(i), 4);
+    }
+    lpc::fence_mbar_init();
+  }
+  __syncthreads();
   lpc::pdl_wait();
 
   // x of this warp's columns, in stretches of 256 (8 a lane)
@@ -294,8 +317,10 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
   __syncwarp();
   const uint8_t* px = xw + (r < tokens ? r : 0) * xrow + t * 16;
 
-  int at = 0, buf = 0, held = 0;
-  const int batch = C::batch(tokens), values = tokens * MT * 16;
+  int at = 0, held = 0;
+  uint32_t turn = 0;  // batches so far
+  bool ok = true;
+  const int batch = C::batch(tokens), values = tokens * C::TS;
   const int prs = (epi == EPI_SWIGLU ? 3 : 4) + (MT == 2);  // log2 of an item's output rows
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
     float sum[MT][2 * NC];  // rows r, then r + 8
@@ -357,54 +382,73 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
       pc += C::CK * 2;
       ps += C::SG * 8;
     }
-    // partial sums of the warps, [token][row] of the item, added in warp order
+    // partial sums of the warps, [token][row] of the item; a buffer's last ones must
+    // have been added
+    const int buf = (int)(turn & 1u);
+    if (held == 0 && turn >= 2 && ok)
+      ok = __all_sync(0xffffffffu, lpc::mbar_wait(empty(buf), ((turn >> 1) & 1u) ^ 1u, &g_int4_few_status));
     float* mine = red + (buf * NW + warp) * rs + held * values;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int i = 0; i < NC; ++i)
         if (NC * t + i < tokens) {
-          float* p = mine + (NC * t + i) * (MT * 16) + m * 16 + r;
+          float* p = mine + (NC * t + i) * C::TS + m * 16 + r;
           p[0] = sum[m][i] * down[i] * 0x1p24f;
           p[8] = sum[m][NC + i] * down[i] * 0x1p20f;
         }
     if (++held < batch && item + (int)gridDim.x < items) continue;
-    __syncthreads();
-    // 4 lanes to a value, each adding 4 warps' parts
-    const float* part = red + buf * NW * rs + (lane & 3) * rs;
-    auto total = [&](int i) {
-      float v = 0.f;
+    __syncwarp();
+    if (lane == 0) lpc::mbar_arrive(full(buf));
+    // four warps, in turns, add the parts up, a value a lane, in a fixed order; the
+    // others go on
+    if ((uint32_t)(warp >> 2) == (turn & 3u)) {
+      const float* part = red + buf * NW * rs;
+      auto total = [&](int i) {
+        float v[4];
 #pragma unroll
-      for (int w = 0; w < NW / 4; ++w) v += part[w * 4 * rs + i];
-      v += __shfl_xor_sync(0xffffffffu, v, 1);
-      return v + __shfl_xor_sync(0xffffffffu, v, 2);
-    };
-    const int per_item = tokens << prs, count = held * per_item;
-    for (int i0 = warp * 8; i0 < count; i0 += NW * 8) {  // whole warps leave together
-      const int at_i = i0 + (lane >> 2), i = min(at_i, count - 1);
-      const int row = i & ((1 << prs) - 1);
-      int tk = i >> prs, sub = 0;  // row of the batch's [item][token]
-      while (tk >= tokens) {
-        tk -= tokens;
-        ++sub;
+        for (int w = 0; w < 4; ++w) v[w] = part[w * rs + i];
+#pragma unroll
+        for (int w = 4; w < NW; ++w) v[w & 3] += part[w * rs + i];
+        return (v[0] + v[1]) + (v[2] + v[3]);
+      };
+      const int count = (held * tokens) << prs;
+      for (int i0 = (warp & 3) * 32; i0 < count; i0 += 128) {  // whole warps
+        const int i = min(i0 + lane, count - 1), row = i & ((1 << prs) - 1);
+        int tk = i >> prs, sub = 0;  // row of the batch's [item][token]
+        if (tokens == 1) {
+          sub = tk;
+          tk = 0;
+        } else {
+          while (tk >= tokens) {
+            tk -= tokens;
+            ++sub;
+          }
+        }
+        const int64_t n = ((int64_t)(item - (held - 1 - sub) * (int)gridDim.x) << prs) + row;
+        const int64_t o = (int64_t)tk * n_out + n;
+        const bool writes = n < n_out && i0 + lane < count;
+        const float plus = epi == EPI_RESIDUAL && writes ? Num<T>::to_f(resid[o]) : 0.f;
+        if (i0 < 128 && ok)
+          ok = __all_sync(0xffffffffu, lpc::mbar_wait(full(buf), (turn >> 1) & 1u, &g_int4_few_status));
+        const int at_p = sub * values + tk * C::TS + row;
+        float v;
+        if (epi == EPI_SWIGLU) {
+          // half the lanes take up before gate: 32 banks
+          const int first = lane & 16;
+          const float a = total(at_p + first), b = total(at_p + 16 - first);
+          const float gate = first ? b : a, upv = first ? a : b;
+          v = __fdividef(gate, 1.f + __expf(-gate)) * upv;
+        } else {
+          v = total(at_p) + plus;
+        }
+        if (writes) out[o] = Num<T>::from_f(v);
       }
-      const int64_t n = ((int64_t)(item - (held - 1 - sub) * (int)gridDim.x) << prs) + row;
-      const int64_t o = (int64_t)tk * n_out + n;
-      float v;
-      if (epi == EPI_SWIGLU) {
-        const int p = sub * values + tk * (MT * 16) + row;
-        const float gate = total(p), upv = total(p + 16);
-        v = __fdividef(gate, 1.f + __expf(-gate)) * upv;
-      } else {
-        v = total(i);
-      }
-      if ((lane & 3) == 0 && at_i < count && n < n_out) {
-        if (epi == EPI_RESIDUAL) v += Num<T>::to_f(resid[o]);
-        out[o] = Num<T>::from_f(v);
-      }
+      __syncwarp();
+      if (lane == 0) lpc::mbar_arrive(empty(buf));
     }
     held = 0;
-    buf ^= 1;
+    ++turn;
   }
   cp_wait<0>();
 }

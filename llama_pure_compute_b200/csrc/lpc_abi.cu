@@ -158,6 +158,7 @@ unsigned int lpc_status_probe(bool clear);
 unsigned int lpc_status_kv4_append(bool clear);
 unsigned int lpc_status_kv4_attention(bool clear);
 unsigned int lpc_status_int4(bool clear);
+unsigned int lpc_status_int4_few(bool clear);
 
 extern "C" int lpc_version(void) { return 100; }
 
@@ -171,6 +172,7 @@ extern "C" int lpc_device_status(void) {
   unsigned int s = lpc_status_kv(true) | lpc_status_rope(true) | lpc_status_decode(true) |
                    lpc_status_swiglu(true) | lpc_status_prefill(true) | lpc_status_wsgemm(true) |
                    lpc_status_probe(true) | lpc_status_kv4_append(true) |
-                   lpc_status_kv4_attention(true) | lpc_status_int4(true);
+                   lpc_status_kv4_attention(true) | lpc_status_int4(true) |
+                   lpc_status_int4_few(true);
   return static_cast<int>(s);
 }
