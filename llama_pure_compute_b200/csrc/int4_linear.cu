@@ -231,20 +231,15 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
       return tk < tokens && st * 256 + lane * 8 < width
                  ? lpc::ld_dep16(src + (int64_t)tk * k + st * 256) : make_uint4(0u, 0u, 0u, 0u);
     };
-    auto largest = [&](float a, const uint4& u) {
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = pair_f<T>(w[i]);
-        a = fmaxf(a, fmaxf(fabsf(f.x), fabsf(f.y)));
-      }
-      return a;
+    // magnitudes of bf16 order as their bits do, two at a time; a NaN is the largest
+    auto largest = [&](uint32_t a, const uint4& u) {
+      constexpr uint32_t M = 0x7FFF7FFFu;
+      return __vimax3_u16x2(__vimax3_u16x2(a, u.x & M, u.y & M), u.z & M, u.w & M);
     };
-    auto factor = [&](int tk, float most) {  // 2^e of a token; keeps 2^-e where it is this lane's
-      // the bits of a non-negative float order as integers do
-      const float a = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+    auto factor = [&](int tk, uint32_t most) {  // 2^e of a token; keeps 2^-e where it is this lane's
+      const uint32_t a = __reduce_max_sync(0xffffffffu, max(most & 0xFFFFu, most >> 16));
       int e = 0;
-      if (a > 0.f && a < INFINITY) e = min(126, 14 - ((int)(__float_as_uint(a) >> 23) - 127));
+      if (a > 0u && a < 0x7F80u) e = min(126, 14 - ((int)(a >> 7) - 127));
       const float d = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
       for (int i = 0; i < NC; ++i)
@@ -285,7 +280,7 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
         if (tk0 + i < tokens) {
           float up = 1.f;
           if constexpr (SCALE) {
-            float a = 0.f;
+            uint32_t a = 0u;
 #pragma unroll
             for (int j = 0; j < ST; ++j) a = largest(a, u[i][j]);
             up = factor(tk0 + i, a);
@@ -306,7 +301,7 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
       for (int tk = 0; tk < tokens; ++tk) {
         float up = 1.f;
         if constexpr (SCALE) {
-          float a = 0.f;
+          uint32_t a = 0u;
           for (int st = 0; st * 256 < width; ++st) a = largest(a, load(tk, st));
           up = factor(tk, a);
         }
