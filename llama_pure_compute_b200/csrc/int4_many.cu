@@ -49,7 +49,8 @@ using lpc::Num;
 
 constexpr int THREADS = 192;   // 4 converter warps, MMA issuer, x loader
 constexpr int CST = 4;         // code stages
-constexpr int XST = 4;         // x stages
+constexpr int XST = 4;         // x stages; loops over steps are unrolled by 4, so that
+                               // slots and the phases of A's two tiles are constants
 constexpr int CODES = 4096;    // code bytes of a 128 x 64 tile
 constexpr int MAX_TOKENS = 64;
 constexpr uint32_t TMEM_COLS = 128;  // 64 sums + 2 tiles of 32; four CTAs share an SM's 512
@@ -68,7 +69,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void converters_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ void ld_cluster4(uint32_t addr, float (&v)[4]) {
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
                : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
@@ -82,23 +82,29 @@ __device__ __forceinline__ uint32_t fma_h2(uint32_t a, __half2 s, __half2 m) {
 
 // lpc::mbar_wait with a hint to sleep on the barrier: four CTAs' waits would
 // otherwise poll away a third of the SM's issue slots.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0u;
+}
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity) {
   const uint64_t t0 = lpc::global_timer_ns();
   for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
+    if (try_wait(bar, parity)) return true;
     if (lpc::global_timer_ns() - t0 > LPC_WAIT_LIMIT_NS) {
       atomicOr(&g_int4_status, LPC_DEV_ERR_TIMEOUT);
       return false;
     }
   }
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+  return try_wait(bar, parity) || wait_on(bar, parity);
 }
 
 struct Args {
@@ -139,22 +145,20 @@ __global__ void __launch_bounds__(THREADS, 4)
   const int nk = (int)((int64_t)(rank + 1) * p.kb / p.splits) - kb0;
 
   const int row = threadIdx.x & 127;  // converters: row of the tile
-  // the code stream: a thread copies two 16-byte pieces of each step (places mixed
-  // so that a thread's row reads without bank conflicts) and its own row's numbers
+  // the code stream: a warp copies the two tile rows of its own 32 weight rows, 16
+  // bytes of each a lane (places mixed so that a thread's row reads without bank
+  // conflicts), and a thread its own row's numbers
   const int64_t ng = ((int64_t)p.kb * 64) >> group_shift;
-  const uint8_t* csrc[2];
-  uint32_t cdst[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int piece = row + 128 * u, i = piece >> 5, r = (piece >> 2) & 7, t = piece & 3;
-    csrc[u] = p.codes + ((int64_t)(tile * 8 + i) * p.kb + kb0) * 512 + (piece & 31) * 16;
-    cdst[u] = cring + i * 512 + r * 64 + ((t ^ (r >> 1)) & 3) * 16;
-  }
+  const int cr = lane >> 2, ct = lane & 3;
+  const uint8_t* csrc = p.codes + ((int64_t)(tile * 8 + (row >> 5) * 2) * p.kb + kb0) * 512 + lane * 16;
+  const int64_t cnext = (int64_t)p.kb * 512;  // the next tile row
+  const uint32_t cdst = cring + (row >> 5) * 1024 + cr * 64 + ((ct ^ (cr >> 1)) & 3) * 16;
   const uint8_t* nsrc = p.scaled + (int64_t)(tile * 8 + (row >> 4)) * ng * 64 + (row & 15) * 4;
   auto fetch = [&](int step, int slot) {
     if (step < nk) {
-      cp16(cdst[0] + slot * CSTAGE, csrc[0] + (uint32_t)step * 512u);
-      cp16(cdst[1] + slot * CSTAGE, csrc[1] + (uint32_t)step * 512u);
+      const uint8_t* src = csrc + (uint32_t)step * 512u;
+      cp16(cdst + slot * CSTAGE, src);
+      cp16(cdst + slot * CSTAGE + 512, src + cnext);
       const uint32_t g = (uint32_t)(kb0 + step) * 64u >> group_shift;
 #pragma unroll
       for (int i = 0; i < SG; ++i)
@@ -197,64 +201,72 @@ __global__ void __launch_bounds__(THREADS, 4)
     const int r = row & 7;
     const uint8_t* src = smem_raw + (cring - raw) + (row >> 4) * 512 + r * 64;
     const uint8_t* num = smem_raw + (cring - raw) + CODES + row * 4;
+    uint32_t places[4];  // of the row's four pieces
+#pragma unroll
+    for (int t = 0; t < 4; ++t) places[t] = ((t ^ (r >> 1)) & 3) * 16;
     bool ok = true;
-    int slot = 0, to = CST - 1;
-    for (int step = 0; step < nk; ++step) {
-      cp_wait<CST - 2>();
-      converters_sync();  // everyone's copies have arrived, and the slot before is free
-      fetch(step + CST - 1, to);
-      to = to == CST - 1 ? 0 : to + 1;
-      __half2 sc[SG], mn[SG];
+    for (int first = 0; first < nk; first += CST) {
 #pragma unroll
-      for (int i = 0; i < SG; ++i) {
-        const __half2 v = *reinterpret_cast<const __half2*>(num + slot * CSTAGE + i * 512);
-        sc[i] = __low2half2(v);
-        mn[i] = __high2half2(v);
-      }
-      uint32_t v[2][16];  // 32 columns each, as pairs
+      for (int u = 0; u < CST; ++u) {  // step first + u is in slot u
+        if (first + u >= nk) break;
+        cp_wait<CST - 2>();
+        __syncwarp();  // the warp's copies have arrived, and the slot before is free
+        fetch(first + u + CST - 1, (u + CST - 1) % CST);
+        __half2 sc[SG], mn[SG];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint4 c = *reinterpret_cast<const uint4*>(src + slot * CSTAGE + ((t ^ (r >> 1)) & 3) * 16);
-        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {  // columns 32 (j / 2) + 8 t + 4 (j % 2) + 0..3
-          const int h = j >> 1, at = 4 * t + 2 * (j & 1), g = SG == 2 ? h : 0;
-          v[h][at] = fma_h2(w[j] & mask, sc[g], mn[g]);
-          v[h][at + 1] = fma_h2((w[j] >> 8) & mask, sc[g], mn[g]);
+        for (int i = 0; i < SG; ++i) {
+          const __half2 v = *reinterpret_cast<const __half2*>(num + u * CSTAGE + i * 512);
+          sc[i] = __low2half2(v);
+          mn[i] = __high2half2(v);
         }
+        uint32_t v[2][16];  // 32 columns each, as pairs
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint4 c = *reinterpret_cast<const uint4*>(src + places[t] + u * CSTAGE);
+          const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {  // columns 32 (j / 2) + 8 t + 4 (j % 2) + 0..3
+            const int h = j >> 1, at = 4 * t + 2 * (j & 1), g = SG == 2 ? h : 0;
+            v[h][at] = fma_h2(w[j] & mask, sc[g], mn[g]);
+            v[h][at + 1] = fma_h2((w[j] >> 8) & mask, sc[g], mn[g]);
+          }
+        }
+        // the tile's last products must be done (a warp goes on as one)
+        constexpr int PAIR = 2;  // tiles of A
+        const int a = u % PAIR;
+        if (ok) ok = __all_sync(0xffffffffu, wait(a_empty(a), (u / PAIR % 2) ^ 1u));
+        if (ok) {
+          lpc::tc_fence_after();
+          lpc::tmem_st16(a_tmem + 32u * a, v[0]);
+          lpc::tmem_st16(a_tmem + 32u * a + 16u, v[1]);
+          lpc::tmem_wait_st();
+          lpc::tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) lpc::mbar_arrive(a_full(a));
       }
-      slot = slot == CST - 1 ? 0 : slot + 1;
-      // the tile's last products must be done (a warp goes on as one)
-      const int a = step & 1;
-      if (ok)
-        ok = __all_sync(0xffffffffu,
-                        wait(a_empty(a), ((uint32_t)(step >> 1) & 1u) ^ 1u));
-      if (ok) {
-        lpc::tc_fence_after();
-        lpc::tmem_st16(a_tmem + 32u * a, v[0]);
-        lpc::tmem_st16(a_tmem + 32u * a + 16u, v[1]);
-        lpc::tmem_wait_st();
-        lpc::tc_fence_before();
-      }
-      __syncwarp();
-      if (lane == 0) lpc::mbar_arrive(a_full(a));
     }
     cp_wait<0>();
   } else if (warp == 4) {
     if (lane == 0) {
       const uint64_t bd0 = lpc::smem_desc_sw128(xring, 16, 1024);
-      for (int step = 0; step < nk; ++step) {
-        const int a = step & 1, xs = step % XST;
-        const uint32_t at = tmem + A_COL + 32u * a;
-        const uint64_t bd = bd0 + (uint32_t)(xs * (XSTAGE >> 4));
-        if (!wait(x_full(xs), (uint32_t)(step / XST) & 1u)) break;
-        if (!wait(a_full(a), (uint32_t)(step >> 1) & 1u)) break;
-        lpc::tc_fence_after();
+      bool ok = true;
+      for (int first = 0; first < nk && ok; first += XST) {
+        const uint32_t turn = (uint32_t)(first / XST) & 1u;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)  // 16 columns: 8 TMEM columns of A, 32 bytes of B
-          lpc::umma_ts(tmem, at + 8u * kk, bd + 2u * kk, p.idesc, (step | kk) != 0);
-        lpc::umma_commit(a_empty(a));
-        lpc::umma_commit(x_empty(xs));
+        for (int u = 0; u < XST; ++u) {
+          if (first + u >= nk) break;
+          const int a = u & 1;
+          ok = wait(x_full(u), turn) && wait(a_full(a), (u >> 1) & 1u);
+          if (!ok) break;
+          lpc::tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)  // 16 columns: 8 TMEM columns of A, 32 bytes of B
+            lpc::umma_ts(tmem, tmem + A_COL + 32u * a + 8u * kk, bd0 + (uint32_t)(u * (XSTAGE >> 4)) + 2u * kk,
+                         p.idesc, (first | u | kk) != 0);
+          lpc::umma_commit(a_empty(a));
+          lpc::umma_commit(x_empty(u));
+        }
       }
       lpc::umma_commit(done);
     }
