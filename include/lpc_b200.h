@@ -459,9 +459,8 @@ LPC_API int lpc_int4_unpack(const lpc_w4* w, void* out, void* stream);
  * out[t, n] = epilogue(sum_k x[t, k] * W[n, k]) for x [tokens, k], tokens <= 64:
  * epilogue 0 store, 1 resid + (resid may equal out), 2 silu(gate) * up (layout 1
  * and only it).  fp32 accumulation, one rounding.  workspace:
- * lpc_int4_linear_workspace_bytes() bytes (0 for fp16, for up to 8 tokens whose x
- * fits shared memory and for up to 16 on weights of at most 2^26 values: NULL
- * then); calls that overlap need one each.  One kernel, two where the workspace is
+ * lpc_int4_linear_workspace_bytes() bytes (0 for fp16, few tokens and small weights:
+ * NULL then); calls that overlap need one each.  One kernel, two where the workspace is
  * used.  A row of x with a value that is not finite gives an output row of values
  * that are not finite; the other rows do not see it.
  */

@@ -14,7 +14,7 @@
 //
 // Three kernels; pick() chooses by the token count and what of x fits:
 //   FEW   up to 8 tokens, x in shared memory (int4_few_kernel, below);
-//   MID   up to 16 tokens on smaller weights, x from the caches (int4_mid_kernel);
+//   MID   smaller weights, x from the caches (int4_mid_kernel);
 //   MANY  the rest up to 64 tokens: tcgen05 (int4_many.cu), which wants whole
 //         128-row tiles of converted weights, at few tokens more work than the
 //         products themselves.
@@ -449,9 +449,9 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
 }
 
 // ---------------------------------------------------------------------------
-// Up to 16 tokens where x does not fit shared memory or its preparation does not
-// pay, on weights of up to MID_MOST elements: x straight from global memory (the
-// L1 and L2 caches), as it is.  fp16 takes the operands above; bf16 the pairs
+// Where x does not fit shared memory, on weights small enough (MID_MOST,
+// MID_BLOCKS): blocks of up to 16 tokens, x straight from global memory (the L1 and
+// L2 caches), as it is.  fp16 takes the operands above; bf16 the pairs
 // 128 + c, (w & 0x000F000F) | 0x43004300, exactly (a bf16 subnormal times x would
 // underflow the fp32 sum), 7 instructions a word.  The 128 is taken out again with the
 // group's sum of x, which costs the fp32 accumulator about 5 of its 24 bits and
@@ -923,9 +923,13 @@ int launch_mid(const lpc_w4* w, const void* x, void* out, const void* resid, int
 
 // Which kernel takes the products (int4_many.cu has MANY).
 enum Kernel { FEW, MID, MANY };
-// Measured, us, mid / many: 4096 x 4096 at 16 tokens 6.3 / 10.4, 4096 x 11,008 at 8
-// tokens 10.2 / 19, 22,016 x 4096 at 16 tokens 30 / 23.
-constexpr int64_t MID_MOST = 64 << 20;
+// Up to 16 tokens MID on weights of up to MID_MOST values; more tokens, in blocks of
+// 16 that each read the weight, where blocks times values are at most MID_BLOCKS.
+// Measured, us, mid / many: 12,288 x 4096 at 16 tokens 16.5 / 19.8, 22,016 x 4096
+// 29.7 / 21.3; at 32 tokens 1024 x 4096 4.0 / 9.3, 4096 x 1024 5.7 / 7.9, 4096 x 4096
+// 11.6 / 11.4; at 64 tokens 1024 x 1024 5.2 / 8.1, 4096 x 1024 10.8 / 10.8, 4096 x
+// 4096 20.4 / 14.7.
+constexpr int64_t MID_MOST = 64 << 20, MID_BLOCKS = 16 << 20;
 // x fits the few-token kernel's shared memory, with one tile row an item or two
 // (the rings round differently).
 template <int GS, int TC>
@@ -936,7 +940,8 @@ bool few_fits(int k, int64_t tokens) {
 template <int GS>
 Kernel pick(const lpc_w4* w, int64_t tokens) {
   if (few_fits<GS, 1>(w->k, tokens) || few_fits<GS, 8>(w->k, tokens)) return FEW;
-  return tokens <= 16 && (w->n_out << w->layout) * w->k <= MID_MOST ? MID : MANY;
+  const int64_t values = (w->n_out << w->layout) * w->k, blocks = (tokens + 15) / 16;
+  return blocks * values <= (blocks == 1 ? MID_MOST : MID_BLOCKS) ? MID : MANY;
 }
 Kernel pick(const lpc_w4* w, int64_t tokens) {
   return w->group == 128 ? pick<128>(w, tokens) : w->group == 64 ? pick<64>(w, tokens) : pick<32>(w, tokens);

@@ -11,12 +11,12 @@ Bars, from arithmetic:
                  128 + c) and as much again for the sum of x that takes the 128
                  out: 2 * 8 * 2^-23 * 143 < 2^-11 of s sum|x|; and 2^-19 of
                  |m| sum|x|.  Fewer than that for the operands without the 128.
-                 From 17 tokens on (16 on weights above 2^26 values) a weight
-                 enters as fp16, off by 2^-11 |w| and 2^-15 of its row's largest
-                 s at most: `rounded` adds that in full.  Without it (normal x and
-                 w, |w| about 4.6 s): the roundings are independent, 2.7 s |x|
-                 2^-11 sqrt(k) in the mean square, and 5 of those are below the
-                 above from k = 384 on."""
+                 Where the kernel for more tokens takes over (9 on weights above 2^26
+                 values, 17 where blocks of 16 cost more), a weight enters as fp16,
+                 off by 2^-11 |w| and 2^-15 of its row's largest s at most: `rounded`
+                 adds that in full.  Without it (normal x and w, |w| about 4.6 s):
+                 the roundings are independent, 2.7 s |x| 2^-11 sqrt(k) in the mean
+                 square, and 5 of those are below the above from k = 384 on."""
 import pytest
 import torch
 
@@ -612,10 +612,14 @@ def test_linear_widths_of_x(dtype, tokens, k, group):
 @pytest.mark.parametrize("tokens,n,k,group,epilogue", [
     (8, 200, 16384, 128, "store"), (5, 40, 32768, 64, "residual"), (8, 2400, 11008, 128, "store"),
     (9, 5000, 640, 32, "store"), (16, 5000, 640, 64, "residual"), (13, 2500, 512, 128, "swiglu"),
-    (16, 100, 16384, 32, "swiglu"), (16, 4800, 8192, 32, "store")])
+    (16, 100, 16384, 32, "swiglu"), (16, 4800, 8192, 32, "store"),
+    # blocks of 16 tokens
+    (17, 1, 64, 32, "store"), (32, 129, 192, 64, "residual"), (33, 63, 256, 128, "swiglu"),
+    (64, 65, 4096, 128, "swiglu"), (48, 3000, 128, 32, "residual"), (20, 5000, 320, 32, "swiglu"),
+    (64, 4096, 1024, 128, "store")])
 def test_linear_x_from_the_caches(dtype, tokens, n, k, group, epilogue):
-    """Up to 16 tokens whose x is not kept in shared memory: with and without kept
-    sums of x, 8 and 16 warps, one and two tile rows."""
+    """x not kept in shared memory: with and without kept sums of x, 8 and 16 warps,
+    one and two tile rows, one to four blocks of tokens."""
     g = gen(tokens + n)
     codes, s, m = random_weight(g, 2 * n if epilogue == "swiglu" else n, k, group, dtype)
     w = Int4Weight.from_codes(codes, s, m, group_size=group,
@@ -631,11 +635,12 @@ def test_linear_x_from_the_caches(dtype, tokens, n, k, group, epilogue):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("tokens,n,k,group,epilogue", [
-    (17, 1, 64, 32, "store"), (32, 129, 192, 64, "residual"), (33, 63, 256, 128, "swiglu"),
-    (64, 65, 4096, 128, "swiglu"), (48, 3000, 128, 32, "residual"), (64, 40000, 128, 128, "store"),
-    (20, 12000, 320, 32, "swiglu")])
+    (17, 1025, 16384, 128, "store"), (32, 129, 65536, 64, "residual"), (33, 601, 8192, 128, "swiglu"),
+    (64, 65, 65536, 128, "swiglu"), (48, 3000, 4096, 32, "residual"), (64, 40000, 128, 128, "store"),
+    (20, 12000, 1088, 32, "swiglu")])
 def test_linear_many_tokens(dtype, tokens, n, k, group, epilogue):
-    """17 to 64 tokens: columns split over clusters or not, ragged last tiles."""
+    """17 to 64 tokens, larger weights: columns split over clusters or not, ragged
+    last tiles."""
     g = gen(tokens + n)
     codes, s, m = random_weight(g, 2 * n if epilogue == "swiglu" else n, k, group, dtype)
     w = Int4Weight.from_codes(codes, s, m, group_size=group,
@@ -665,7 +670,7 @@ def test_linear_many_tokens_values(dtype):
     """Groups of very different scale in a row, negative scales, rows of zeros, x of
     very different sizes; a non-finite token stays in its row."""
     g = gen(21)
-    n, k = 130, 512
+    n, k = 16403, 512
     codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device=DEV, generator=g)
     s = (torch.rand(n, 4, device=DEV, generator=g) + 0.5) * torch.tensor([1e-2, 1e-4, -3e-3, 1.0], device=DEV)
     m = torch.randn(n, 4, device=DEV, generator=g) * torch.tensor([0.1, 1e-3, 1e-2, 8.0], device=DEV)
@@ -698,10 +703,11 @@ def test_linear_many_tokens_values(dtype):
 def test_linear_many_tokens_in_graphs_and_streams():
     """Two graphs and two streams at once, each call with scratch of its own."""
     g = gen(22)
-    codes, s, m = random_weight(g, 2048, 2048, 128, BF)
+    codes, s, m = random_weight(g, 4096, 4096, 128, BF)
     w = Int4Weight.from_codes(codes, s, m, group_size=128)
-    xs = [torch.randn(t, 2048, device=DEV, generator=g).to(BF) for t in (24, 64)]
-    nw = torch.ones(2048, dtype=BF, device=DEV)
+    assert w.workspace_bytes(24) > 0
+    xs = [torch.randn(t, 4096, device=DEV, generator=g).to(BF) for t in (24, 64)]
+    nw = torch.ones(4096, dtype=BF, device=DEV)
     want = [int4_linear(int4_linear(ops.rmsnorm_forward(x, nw), w), w) for x in xs]
     graphs, outs = [], []
     for x in xs:
