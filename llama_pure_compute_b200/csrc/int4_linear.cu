@@ -13,7 +13,7 @@
 // c * 2^-24, exactly.  x enters as fp16 too.
 //
 // Three kernels; pick() chooses by the token count and what of x fits:
-//   FEW   up to 8 tokens, x in shared memory (int4_few_kernel, below);
+//   FEW   up to 8 tokens on larger weights, x in shared memory (int4_few_kernel, below);
 //   MID   smaller weights, x from the caches (int4_mid_kernel);
 //   MANY  the rest up to 64 tokens: tcgen05 (int4_many.cu), which wants whole
 //         128-row tiles of converted weights, at few tokens more work than the
@@ -449,8 +449,7 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
 }
 
 // ---------------------------------------------------------------------------
-// Where x does not fit shared memory, on weights small enough (MID_MOST,
-// MID_BLOCKS): blocks of up to 16 tokens, x straight from global memory (the L1 and
+// Weights small enough (pick()): blocks of up to 16 tokens, x straight from global memory (the L1 and
 // L2 caches), as it is.  fp16 takes the operands above; bf16 the pairs
 // 128 + c, (w & 0x000F000F) | 0x43004300, exactly (a bf16 subnormal times x would
 // underflow the fp32 sum), 7 instructions a word.  The 128 is taken out again with the
@@ -923,6 +922,10 @@ int launch_mid(const lpc_w4* w, const void* x, void* out, const void* resid, int
 
 // Which kernel takes the products (int4_many.cu has MANY).
 enum Kernel { FEW, MID, MANY };
+// MID has no preparation of x, FEW a faster weight stream: MID up to (8 + 2 tokens) 2^20
+// values.  Measured, us, few / mid at 1 / 4 / 8 tokens: 1024 x 4096 3.0 / 2.8, 3.7 / 2.9,
+// 4.8 / 3.0; 4096 x 4096 3.8 / 4.3, 4.5 / 4.4, 5.8 / 4.6; 12,288 x 4096 7.1 / 10.2,
+// 7.6 / 10.5, 9.2 / 11.1.
 // Up to 16 tokens MID on weights of up to MID_MOST values; more tokens, in blocks of
 // 16 that each read the weight, where blocks times values are at most MID_BLOCKS.
 // Measured, us, mid / many: 12,288 x 4096 at 16 tokens 16.5 / 19.8, 22,016 x 4096
@@ -939,8 +942,10 @@ bool few_fits(int k, int64_t tokens) {
 }
 template <int GS>
 Kernel pick(const lpc_w4* w, int64_t tokens) {
-  if (few_fits<GS, 1>(w->k, tokens) || few_fits<GS, 8>(w->k, tokens)) return FEW;
   const int64_t values = (w->n_out << w->layout) * w->k, blocks = (tokens + 15) / 16;
+  if (values > (8 + 2 * tokens) << 20 &&
+      (few_fits<GS, 1>(w->k, tokens) || few_fits<GS, 8>(w->k, tokens)))
+    return FEW;
   return blocks * values <= (blocks == 1 ? MID_MOST : MID_BLOCKS) ? MID : MANY;
 }
 Kernel pick(const lpc_w4* w, int64_t tokens) {

@@ -539,10 +539,11 @@ def test_linear_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-def test_linear_code_by_code(dtype):
+@pytest.mark.parametrize("n", [48, 33008])
+def test_linear_code_by_code(dtype, n):
     """One-hot x reads single weights: every code of every column in its place."""
     g = gen(4)
-    n, k = 48, 128
+    k = 128
     codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device=DEV, generator=g)
     s = torch.ones(n, 1, dtype=dtype, device=DEV)
     m = torch.zeros(n, 1, dtype=dtype, device=DEV)
@@ -554,12 +555,13 @@ def test_linear_code_by_code(dtype):
         assert torch.equal(int4_linear(eye[at:at + 64], w), want.t()[at:at + 64])
 
 
+@pytest.mark.parametrize("n", [65, 20500])
 @pytest.mark.parametrize("dtype", [BF, HF])
-def test_linear_values(dtype):
+def test_linear_values(dtype, n):
     """Offset activations (large sums of x), large and small ones; a non-finite
     token stays in its row."""
     g = gen(7)
-    codes, s, m = random_weight(g, 65, 1024, 128, dtype)
+    codes, s, m = random_weight(g, n, 1024, 128, dtype)
     w = Int4Weight.from_codes(codes, s, m, group_size=128)
     x = torch.randn(6, 1024, device=DEV, generator=g)
     x[1] += 4.0
@@ -578,20 +580,24 @@ def test_linear_values(dtype):
     assert not z[1].isfinite().any() and not z[4].isfinite().any()
 
 
-@pytest.mark.parametrize("tokens", [2, 3, 5, 7, 8])
-def test_linear_items_that_share_a_barrier(tokens):
-    """Few tokens add up several items' sums at once: full and broken batches, the
-    last item past the rows; twice the same."""
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("tokens", [1, 2, 3, 5, 8])
+def test_linear_items_that_share_their_sums(dtype, group, tokens):
+    """Few tokens on larger weights add up several items' sums at once: full and
+    broken batches, the last item past the rows; twice the same."""
     g = gen(tokens)
-    for n, epilogue in ((20011, "store"), (9999, "swiglu"), (2369, "residual")):
-        codes, s, m = random_weight(g, 2 * n if epilogue == "swiglu" else n, 256, 128, BF)
-        w = Int4Weight.from_codes(codes, s, m, group_size=128,
+    for n, k, epilogue in ((20011, 1280, "store"), (9999, 1280, "swiglu"), (6401, 4096, "residual")):
+        codes, s, m = random_weight(g, 2 * n if epilogue == "swiglu" else n, k, group, dtype)
+        w = Int4Weight.from_codes(codes, s, m, group_size=group,
                                   layout="swiglu" if epilogue == "swiglu" else "linear")
-        x = torch.randn(tokens, 256, device=DEV, generator=g).to(BF)
-        r = torch.randn(tokens, n, device=DEV, generator=g).to(BF) if epilogue == "residual" else None
+        x = torch.randn(tokens, k, device=DEV, generator=g).to(dtype)
+        r = torch.randn(tokens, n, device=DEV, generator=g).to(dtype) if epilogue == "residual" else None
         y = int4_linear(x, w, epilogue, resid=r)
         check_linear(y, x, codes, s, m, epilogue, r)
         assert torch.equal(int4_linear(x, w, epilogue, resid=r), y)
+        if r is not None:
+            assert torch.equal(int4_linear(x, w, epilogue, resid=r, out=r), y)
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
@@ -602,7 +608,8 @@ def test_linear_items_that_share_a_barrier(tokens):
 def test_linear_widths_of_x(dtype, tokens, k, group):
     """x of 256, 1024 and more columns a warp, up to where it fits no longer."""
     g = gen(k + tokens)
-    codes, s, m = random_weight(g, 72, k, group, dtype)
+    n = ((8 + 2 * tokens) << 20) // k + 17  # the least weight whose x is kept
+    codes, s, m = random_weight(g, n, k, group, dtype)
     w = Int4Weight.from_codes(codes, s, m, group_size=group)
     x = torch.randn(tokens, k, device=DEV, generator=g).to(dtype)
     check_linear(int4_linear(x, w), x, codes, s, m)
@@ -773,11 +780,12 @@ def test_weight_from_16_bits_and_back():
         assert torch.equal(Int4Weight(odd, layout="swiglu", group_size=group).data, pair.data)
 
 
-def test_linear_after_a_kernel_that_writes_x_in_graphs_and_streams():
+@pytest.mark.parametrize("n", [512, 8192])
+def test_linear_after_a_kernel_that_writes_x_in_graphs_and_streams(n):
     """Launched programmatically under the kernel before it: x, written by that
     kernel, is not read early; the same in a graph and on another stream."""
     g = gen(18)
-    codes, s, m = random_weight(g, 512, 4096, 128, BF)
+    codes, s, m = random_weight(g, n, 4096, 128, BF)
     w = Int4Weight.from_codes(codes, s, m, group_size=128)
     src = torch.randn(4, 4096, device=DEV, generator=g).to(BF)
     nw = torch.ones(4096, dtype=BF, device=DEV)
