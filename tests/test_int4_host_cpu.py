@@ -121,16 +121,18 @@ def test_linear_refusals():
     assert call(ref, 24, 16, None, 1, 0) == INVALID
     assert call(ref, 16, 16, None, 0, 0) == _lib.LPC_OK
     assert call(ctypes.addressof(bad), 16, 16, None, 1, 0) == UNSUPPORTED
-    # the workspace: bf16, more than 16 tokens, or more than 8 on a large weight
+    # the workspace: bf16, more tokens and values than the kernels without one take
     need = lib.lpc_int4_linear_workspace_bytes
-    assert need(ref, 16) == 0 and need(ref, 0) == 0 and need(ref, 65) == 0
-    assert need(ref, 17) == 17 * 256 * 2 + 256
+    assert need(ref, 64) == 0 and need(ref, 0) == 0 and need(ref, 65) == 0
+    large = weight(n_out=8192, k=4096)
+    big = ctypes.addressof(large)
+    assert need(big, 16) == 0 and need(big, 17) == 17 * 4096 * 2 + 256
     assert need(ctypes.addressof(wide), 8) == 0 and need(ctypes.addressof(huge), 8) == 8 * 16384 * 2 + 256
-    half = weight(dtype=1)
+    half = weight(dtype=1, n_out=8192, k=4096)
     assert need(ctypes.addressof(half), 64) == 0
-    assert call(ref, 16, 16, None, 17, 0) == INVALID and b"workspace" in lib.lpc_last_error()
-    assert call(ref, 16, 16, None, 17, 0, ws=16, nbytes=100) == INVALID
-    assert call(ref, 16, 16, None, 17, 0, ws=24, nbytes=1 << 20) == INVALID
+    assert call(big, 16, 16, None, 17, 0) == INVALID and b"workspace" in lib.lpc_last_error()
+    assert call(big, 16, 16, None, 17, 0, ws=16, nbytes=100) == INVALID
+    assert call(big, 16, 16, None, 17, 0, ws=24, nbytes=1 << 20) == INVALID
     size = lib.lpc_int4_weight_bytes
     assert size(100, 100, 128, 0) == 0
     # tile rows of 16, a multiple of 8 of them: codes, two sets of numbers, a factor a row
