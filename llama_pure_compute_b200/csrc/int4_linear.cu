@@ -449,14 +449,14 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
 }
 
 // ---------------------------------------------------------------------------
-// Weights small enough (pick()): blocks of up to 16 tokens, x straight from global memory (the L1 and
-// L2 caches), as it is.  fp16 takes the operands above; bf16 the pairs
+// Smaller weights (pick()): blocks of up to 16 tokens, x straight from global
+// memory (the L1 and L2 caches), as it is.  fp16 takes the operands above; bf16 the pairs
 // 128 + c, (w & 0x000F000F) | 0x43004300, exactly (a bf16 subnormal times x would
 // underflow the fp32 sum), 7 instructions a word.  The 128 is taken out again with the
 // group's sum of x, which costs the fp32 accumulator about 5 of its 24 bits and
 // leaves an error some hundred times below the output's rounding.  The sum of x is
 // one more product, of a row of ones, kept in shared memory for the next items.
-// 4096 x 4096 at 16 tokens: 6.2 us (stream 1.4); the loads of x, one of each 8
+// 4096 x 4096 at 8 / 16 tokens: 4.2 / 5.6 us (stream 1.4); the loads of x, one of each 8
 // columns and token for every tile row, bound it.
 // ---------------------------------------------------------------------------
 template <typename T>
@@ -480,13 +480,14 @@ __device__ __forceinline__ void mma_of(float (&c)[4], const uint32_t (&a)[4], ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int GS, int MT, int NT, int NW>
+template <int GS, int MT, int NT>
 struct Cfg {
+  static constexpr int NW = 16;
   static constexpr int CK = GS > 64 ? GS : 64;  // columns of a pipeline stage
   static constexpr int TILES = CK / 64;
   static constexpr int SG = CK / GS;            // groups of a stage
   static constexpr int STAGE = MT * (TILES * 512 + SG * 256);
-  static constexpr int NST = (MT * TILES == 4 ? 4 : MT * TILES == 2 ? 8 : 12) * 8 / NW + (NW > 8);
+  static constexpr int NST = MT * TILES == 4 ? 3 : MT * TILES == 2 ? 5 : 7;
   static constexpr int RING = NST * STAGE;
   static constexpr int RED = MT * 16 * NT * 8;  // fp32 partial sums of a warp
   static constexpr int SMEM = NW * (RING + 2 * RED * 4);
@@ -495,12 +496,13 @@ struct Cfg {
   static_assert(XS_MAX >= 0, "shared memory");
 };
 
-template <typename T, int GS, int MT, int NT, int NW>
-__global__ void __launch_bounds__(NW * 32)
+template <typename T, int GS, int MT, int NT>
+__global__ void __launch_bounds__(512, 1)
     int4_mid_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ numbers,
                    const T* x, const T* resid, T* out, int tokens, int64_t n_out, int k, int items,
                    int epi, int keep_sums) {
-  using C = Cfg<GS, MT, NT, NW>;
+  using C = Cfg<GS, MT, NT>;
+  constexpr int NW = C::NW;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
@@ -890,18 +892,19 @@ int launch_few_mt(const lpc_w4* w, const void* x, void* out, const void* resid, 
   return launch_few<T, GS, 2, TC>(w, x, out, resid, tokens, epi, s);
 }
 
-template <typename T, int GS, int MT, int NT, int NW>
+template <typename T, int GS, int MT, int NT>
 int launch_mid(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens, int epi,
            cudaStream_t s) {
-  using C = Cfg<GS, MT, NT, NW>;
+  using C = Cfg<GS, MT, NT>;
+  constexpr int NW = C::NW;
   static std::atomic<uint64_t> mask{0};
-  int rc = lpc::once_per_device_smem((const void*)int4_mid_kernel<T, GS, MT, NT, NW>,
+  int rc = lpc::once_per_device_smem((const void*)int4_mid_kernel<T, GS, MT, NT>,
                                      C::SMEM + C::XS_MAX, mask);
   if (rc) return rc;
   const int items = few_items(w, MT);
   // the sums of x are computed with the first item and kept for the next ones
   const int64_t sums = (int64_t)NW * ((w->k / C::CK + NW - 1) / NW) * C::SG * NT * 8 * 4;
-  const int slots = lpc::current_device_sms() * (16 / NW);
+  const int slots = lpc::current_device_sms();
   const int keep = items > slots && sums <= C::XS_MAX;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -914,7 +917,7 @@ int launch_mid(const lpc_w4* w, const void* x, void* out, const void* resid, int
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const lpc::Int4Parts p = lpc::int4_parts(w->packed, w->n_out, w->k, w->group, w->layout);
-  cudaLaunchKernelEx(&cfg, int4_mid_kernel<T, GS, MT, NT, NW>, (const uint8_t*)p.codes,
+  cudaLaunchKernelEx(&cfg, int4_mid_kernel<T, GS, MT, NT>, (const uint8_t*)p.codes,
                      (const uint8_t*)p.numbers, (const T*)x, (const T*)resid, (T*)out, (int)tokens,
                      w->n_out, w->k, items, epi, keep);
   return lpc::check_launch("int4_linear");
@@ -922,17 +925,16 @@ int launch_mid(const lpc_w4* w, const void* x, void* out, const void* resid, int
 
 // Which kernel takes the products (int4_many.cu has MANY).
 enum Kernel { FEW, MID, MANY };
-// MID has no preparation of x, FEW a faster weight stream: MID up to (8 + 2 tokens) 2^20
-// values.  Measured, us, few / mid at 1 / 4 / 8 tokens: 1024 x 4096 3.0 / 2.8, 3.7 / 2.9,
-// 4.8 / 3.0; 4096 x 4096 3.8 / 4.3, 4.5 / 4.4, 5.8 / 4.6; 12,288 x 4096 7.1 / 10.2,
-// 7.6 / 10.5, 9.2 / 11.1.
-// Up to 16 tokens MID on weights of up to MID_MOST values; more tokens, in blocks of
-// 16 that each read the weight, where blocks times values are at most MID_BLOCKS.
-// Measured, us, mid / many: 12,288 x 4096 at 16 tokens 16.5 / 19.8, 22,016 x 4096
-// 29.7 / 21.3; at 32 tokens 1024 x 4096 4.0 / 9.3, 4096 x 1024 5.7 / 7.9, 4096 x 4096
-// 11.6 / 11.4; at 64 tokens 1024 x 1024 5.2 / 8.1, 4096 x 1024 10.8 / 10.8, 4096 x
-// 4096 20.4 / 14.7.
-constexpr int64_t MID_MOST = 64 << 20, MID_BLOCKS = 16 << 20;
+// MID has no preparation of x, FEW a faster weight stream: MID up to (8 + 3 tokens) 2^20
+// values.  Measured, us, few / mid at 1 / 4 / 8 tokens: 2048 x 4096 3.0 / 2.9, 4.1 / 3.0
+// at 4; 4096 x 4096 3.8 / 4.0, 4.5 / 4.1, 5.8 / 4.2; 6144 x 4096 4.8 / 6.6, 5.8 / 6.8,
+// 7.2 / 6.8; 12,288 x 4096 7.7 / 9.9, 7.6 / 9.9, 9.4 / 10.1.
+// More than 16 tokens cost MID a pass over the weight per 16, and MANY hardly more than
+// few do: MID where blocks^2 times values are at most MID_MOST.  Measured, us, mid /
+// many: 14,336 x 4096 at 16 tokens 18.5 / 19.4, 22,016 x 4096 25.0 / 21.2; at 32 tokens
+// 4096 x 4096 10.2 / 11.3, 6144 x 4096 14.6 / 12.8; at 64 4096 x 1024 11.0 / 10.7,
+// 2048 x 4096 15.4 / 11.3.
+constexpr int64_t MID_MOST = 72 << 20;
 // x fits the few-token kernel's shared memory, with one tile row an item or two
 // (the rings round differently).
 template <int GS, int TC>
@@ -943,27 +945,24 @@ bool few_fits(int k, int64_t tokens) {
 template <int GS>
 Kernel pick(const lpc_w4* w, int64_t tokens) {
   const int64_t values = (w->n_out << w->layout) * w->k, blocks = (tokens + 15) / 16;
-  if (values > (8 + 2 * tokens) << 20 &&
+  if (values > (8 + 3 * tokens) << 20 &&
       (few_fits<GS, 1>(w->k, tokens) || few_fits<GS, 8>(w->k, tokens)))
     return FEW;
-  return blocks * values <= (blocks == 1 ? MID_MOST : MID_BLOCKS) ? MID : MANY;
+  return blocks * blocks * values <= MID_MOST ? MID : MANY;
 }
 Kernel pick(const lpc_w4* w, int64_t tokens) {
   return w->group == 128 ? pick<128>(w, tokens) : w->group == 64 ? pick<64>(w, tokens) : pick<32>(w, tokens);
 }
 
-// Two tile rows share the loads of x; with too few rows to give each SM an
-// item, one tile row an item and 16 warps to share its columns.
+// Two tile rows an item share the loads of x; one where two would leave SMs without
+// an item.  Measured, us, one / two: 2048 x 4096 at 16 tokens 4.3 / 5.0, 4096 x 4096
+// 6.5 / 5.6, 4096 x 11,008 14.7 / 11.1.
 template <typename T, int GS, int NT>
 int launch_mid_mt(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens,
                   int epi, cudaStream_t s) {
-  const int64_t tr = (w->n_out + 15) / 16, sms = lpc::current_device_sms();
-  if (w->layout == 1)
-    return tr <= sms ? launch_mid<T, GS, 2, NT, 16>(w, x, out, resid, tokens, epi, s)
-                     : launch_mid<T, GS, 2, NT, 8>(w, x, out, resid, tokens, epi, s);
-  if (tr <= sms) return launch_mid<T, GS, 1, NT, 16>(w, x, out, resid, tokens, epi, s);
-  if (NT == 1 || tr <= 2 * sms) return launch_mid<T, GS, 1, NT, 8>(w, x, out, resid, tokens, epi, s);
-  return launch_mid<T, GS, 2, NT, 8>(w, x, out, resid, tokens, epi, s);
+  if (w->layout == 0 && few_items(w, 1) <= lpc::current_device_sms())
+    return launch_mid<T, GS, 1, NT>(w, x, out, resid, tokens, epi, s);
+  return launch_mid<T, GS, 2, NT>(w, x, out, resid, tokens, epi, s);
 }
 
 template <typename T, int GS>

@@ -11,8 +11,8 @@ Bars, from arithmetic:
                  128 + c) and as much again for the sum of x that takes the 128
                  out: 2 * 8 * 2^-23 * 143 < 2^-11 of s sum|x|; and 2^-19 of
                  |m| sum|x|.  Fewer than that for the operands without the 128.
-                 Where the kernel for more tokens takes over (9 on weights above 2^26
-                 values, 17 where blocks of 16 cost more), a weight enters as fp16,
+                 Where the kernel for more tokens takes over (9 on weights above 72 *
+                 2^20 values, 17 where blocks of 16 cost more), a weight enters as fp16,
                  off by 2^-11 |w| and 2^-15 of its row's largest s at most: `rounded`
                  adds that in full.  Without it (normal x and w, |w| about 4.6 s):
                  the roundings are independent, 2.7 s |x| 2^-11 sqrt(k) in the mean
@@ -539,7 +539,7 @@ def test_linear_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-@pytest.mark.parametrize("n", [48, 33008])
+@pytest.mark.parametrize("n", [48, 37008])
 def test_linear_code_by_code(dtype, n):
     """One-hot x reads single weights: every code of every column in its place."""
     g = gen(4)
@@ -555,7 +555,7 @@ def test_linear_code_by_code(dtype, n):
         assert torch.equal(int4_linear(eye[at:at + 64], w), want.t()[at:at + 64])
 
 
-@pytest.mark.parametrize("n", [65, 20500])
+@pytest.mark.parametrize("n", [65, 27000])
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_linear_values(dtype, n):
     """Offset activations (large sums of x), large and small ones; a non-finite
@@ -587,7 +587,7 @@ def test_linear_items_that_share_their_sums(dtype, group, tokens):
     """Few tokens on larger weights add up several items' sums at once: full and
     broken batches, the last item past the rows; twice the same."""
     g = gen(tokens)
-    for n, k, epilogue in ((20011, 1280, "store"), (9999, 1280, "swiglu"), (6401, 4096, "residual")):
+    for n, k, epilogue in ((20011, 1792, "store"), (9999, 1792, "swiglu"), (8209, 4096, "residual")):
         codes, s, m = random_weight(g, 2 * n if epilogue == "swiglu" else n, k, group, dtype)
         w = Int4Weight.from_codes(codes, s, m, group_size=group,
                                   layout="swiglu" if epilogue == "swiglu" else "linear")
@@ -608,7 +608,7 @@ def test_linear_items_that_share_their_sums(dtype, group, tokens):
 def test_linear_widths_of_x(dtype, tokens, k, group):
     """x of 256, 1024 and more columns a warp, up to where it fits no longer."""
     g = gen(k + tokens)
-    n = ((8 + 2 * tokens) << 20) // k + 17  # the least weight whose x is kept
+    n = ((8 + 3 * tokens) << 20) // k + 17  # the least weight whose x is kept
     codes, s, m = random_weight(g, n, k, group, dtype)
     w = Int4Weight.from_codes(codes, s, m, group_size=group)
     x = torch.randn(tokens, k, device=DEV, generator=g).to(dtype)
@@ -642,7 +642,7 @@ def test_linear_x_from_the_caches(dtype, tokens, n, k, group, epilogue):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("tokens,n,k,group,epilogue", [
-    (17, 1025, 16384, 128, "store"), (32, 129, 65536, 64, "residual"), (33, 601, 8192, 128, "swiglu"),
+    (17, 1225, 16384, 128, "store"), (32, 301, 65536, 64, "residual"), (33, 601, 8192, 128, "swiglu"),
     (64, 65, 65536, 128, "swiglu"), (48, 3000, 4096, 32, "residual"), (64, 40000, 128, 128, "store"),
     (20, 12000, 1088, 32, "swiglu")])
 def test_linear_many_tokens(dtype, tokens, n, k, group, epilogue):
@@ -663,9 +663,9 @@ def test_linear_many_tokens(dtype, tokens, n, k, group, epilogue):
 
 @pytest.mark.parametrize("tokens", [9, 16])
 def test_linear_of_a_large_weight(tokens):
-    """The same from 9 tokens on where the weight has more than 2^26 values."""
+    """The same from 9 tokens on where the weight has more than 72 * 2^20 values."""
     g = gen(tokens)
-    codes, s, m = random_weight(g, 17000, 4096, 128, BF)
+    codes, s, m = random_weight(g, 19000, 4096, 128, BF)
     w = Int4Weight.from_codes(codes, s, m, group_size=128)
     assert w.workspace_bytes(tokens) > 0
     x = torch.randn(tokens, 4096, device=DEV, generator=g).to(BF)
@@ -710,11 +710,11 @@ def test_linear_many_tokens_values(dtype):
 def test_linear_many_tokens_in_graphs_and_streams():
     """Two graphs and two streams at once, each call with scratch of its own."""
     g = gen(22)
-    codes, s, m = random_weight(g, 4096, 4096, 128, BF)
+    codes, s, m = random_weight(g, 5120, 5120, 128, BF)
     w = Int4Weight.from_codes(codes, s, m, group_size=128)
     assert w.workspace_bytes(24) > 0
-    xs = [torch.randn(t, 4096, device=DEV, generator=g).to(BF) for t in (24, 64)]
-    nw = torch.ones(4096, dtype=BF, device=DEV)
+    xs = [torch.randn(t, 5120, device=DEV, generator=g).to(BF) for t in (24, 64)]
+    nw = torch.ones(5120, dtype=BF, device=DEV)
     want = [int4_linear(int4_linear(ops.rmsnorm_forward(x, nw), w), w) for x in xs]
     graphs, outs = [], []
     for x in xs:
