@@ -709,13 +709,11 @@ def _int4_out(out: torch.Tensor, name: str, shape, kv: Int4KV) -> None:
                          "of the cache's dtype and device.")
 
 
-def _int4_positions(positions: torch.Tensor, shape, kv: Int4KV) -> torch.Tensor:
-    """positions as contiguous int64 [batch, seq]; ``shape`` starts with the batch
-    and the sequence that they must have."""
-    have = positions.shape
-    if len(have) != 2 or have[0] != shape[0] or have[1] != shape[1]:
+def _int4_positions(positions: torch.Tensor, B: int, S: int, kv: Int4KV) -> torch.Tensor:
+    """positions as contiguous int64 [B, S]."""
+    if positions.shape != (B, S):
         raise ValueError("LlamaPureComputeError: positions must be [batch, seq].")
-    if have[0] > kv.max_batch:
+    if B > kv.max_batch:
         raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
     if positions.dtype is not torch.int64:
         if positions.dtype.is_floating_point or positions.dtype == torch.bool:
@@ -761,16 +759,21 @@ def rope_kv_append_int4(
     if len(rows) != 2 or rows[1] != D or sin_table.shape != rows or sin_table.dtype != table_dtype:
         raise ValueError("LlamaPureComputeError: rope tables must be matching [max_pos, head_dim].")
     B, S, _ = shape
-    pos = _int4_positions(positions, shape, kv)
-    qkv, cos_table, sin_table = _dense16(qkv), _dense16(cos_table), _dense16(sin_table)
+    pos = _int4_positions(positions, B, S, kv)
+    qp, cp, sp = qkv.data_ptr(), cos_table.data_ptr(), sin_table.data_ptr()
+    if (qp | cp | sp) & 15 or not (qkv.is_contiguous() and cos_table.is_contiguous()
+                                   and sin_table.is_contiguous()):
+        qkv, cos_table, sin_table = _dense16(qkv), _dense16(cos_table), _dense16(sin_table)
+        qp, cp, sp = qkv.data_ptr(), cos_table.data_ptr(), sin_table.data_ptr()
+    code = _lib.DTYPE_CODE.get(table_dtype)
+    if code is None:
+        raise TypeError(f"LlamaPureComputeError: rope_kv_append_int4: unsupported dtype {table_dtype}")
     if q_out is None:
         q_out = qkv.new_empty(B, num_heads, S, D)
     else:
         _int4_out(q_out, "q_out", (B, num_heads, S, D), kv)
-    rc = _lib.call_on(index, _lib.load().lpc_rope_kv_append_int4, kv.ref, qkv.data_ptr(),
-                      pos.data_ptr(), cos_table.data_ptr(), sin_table.data_ptr(), rows[0],
-                      q_out.data_ptr(), B, S, num_heads,
-                      _lib.dtype_code(table_dtype, "rope_kv_append_int4"))
+    rc = _lib.call_on(index, _lib.load().lpc_rope_kv_append_int4, kv.ref, qp, pos.data_ptr(), cp, sp,
+                      rows[0], q_out.data_ptr(), B, S, num_heads, code)
     if rc:
         _lib.check(rc, "rope_kv_append_int4")
     if B and S:
@@ -795,7 +798,7 @@ def kv_read_int4(
     if positions.dim() != 2:
         raise ValueError("LlamaPureComputeError: positions must be [batch, seq].")
     B, S = positions.shape
-    pos = _int4_positions(positions, (B, S), kv)
+    pos = _int4_positions(positions, B, S, kv)
     shape = (B, kv.kv_heads, S, kv.head_dim)
     if k_out is None:
         k_out = kv.key_scales.new_empty(*shape)
@@ -855,7 +858,10 @@ def decode_attention_int4(
         raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
     if seq_lens.numel() < B or not seq_lens.is_contiguous():
         raise ValueError("LlamaPureComputeError: seq_lens must have a contiguous entry per sequence.")
-    q = _dense16(q)
+    qp = q.data_ptr()
+    if qp & 15 or not q.is_contiguous():
+        q = _dense16(q)
+        qp = q.data_ptr()
     if out is None:
         out = torch.empty_like(q)
     else:
@@ -865,8 +871,8 @@ def decode_attention_int4(
         workspace = decode_attention_int4_workspace(kv, B, H)
     elif workspace.get_device() != index or not workspace.is_contiguous():
         raise ValueError("LlamaPureComputeError: workspace must be contiguous on the cache's device.")
-    rc = _lib.call_on(index, lib.lpc_decode_attention_int4, kv.ref, q.data_ptr(),
-                      seq_lens.data_ptr(), out.data_ptr(), workspace.data_ptr(), workspace.nbytes,
+    rc = _lib.call_on(index, lib.lpc_decode_attention_int4, kv.ref, qp, seq_lens.data_ptr(),
+                      out.data_ptr(), workspace.data_ptr(), workspace.nbytes,
                       B, H, D ** -0.5 if sm_scale is None else sm_scale)
     if rc:
         _lib.check(rc, "decode_attention_int4")
