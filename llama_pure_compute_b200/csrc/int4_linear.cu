@@ -19,9 +19,9 @@
 //         128-row tiles of converted weights, at few tokens more work than the
 //         products themselves.
 // Measured at groups of 128, bf16 (us; in brackets the stream at 6397 GB/s): one
-// token, 128,256 x 4096 44 (43.7) and 4096 x 4096 3.7 (1.4: the launch, x and one
-// round of loads); SwiGLU 2 x 11,008 x 4096 at 1 / 4 / 8 tokens 10.8 / 12.2 / 15.3
-// (7.5); 4096 x 11,008 at 4 tokens 8.5 (3.8).
+// token, 128,256 x 4096 42.9 (43.7) and 4096 x 4096 3.8 (1.4: the launch, x and one
+// round of loads); 22,016 x 4096 at 1 / 4 / 8 tokens 10.8 / 11.3 / 13.7 (7.5), 4096 x
+// 11,008 at 4 8.6 (3.8).
 //
 // Packed weight: tiles of 16 rows x 64 columns, 512 contiguous bytes, 16 a
 // lane, read with cp.async into the lane's own slots (no barrier), followed by
@@ -103,7 +103,9 @@ enum { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_SWIGLU = 2 };
 // half the accumulators and leaves room for two CTAs an SM.
 // What took it there (128,256 x 4096, one token): 58 us with 8 warps and a barrier
 // an item, 50.6 with the sums of several items at one barrier and 16 warps, 45.1
-// with x's sums and numbers read once a group, 43.5 with the operands of operand().
+// with x's sums and numbers read once a group, 43.5 with the operands of operand(),
+// 42.9 with four warps at a time for the sums, which the others do not wait for (at 8
+// tokens 54 instead of 64).
 // With several tokens the instructions bound it: a code word has 4 of unpacking
 // and its product, whatever the token count, but the accumulators and x's operands
 // of 8 tokens leave room for one CTA an SM.

@@ -13,13 +13,13 @@
 //   * x, fp16 (bf16 rows are converted first, scaled by a power of two each, by a
 //     small kernel), comes by TMA as the B operand;
 //   * one thread issues tcgen05.mma with the fp32 sums in tensor memory.
-// A step is a chain of waits and dependent instructions of about 1000 cycles, far
-// more than its share of HBM's time (175), so the CTAs are small, four an SM, and
-// their chains overlap.
-// Measured, bf16, groups of 128: 22,016 x 4096 at 16 / 32 / 64 tokens 23 / 24 / 26
-// us (stream 7.5), 4096 x 4096 at 32 / 64 12 / 14.  The chain bounds it; two
-// warpgroups a CTA (its one issuing thread then the limit) and clusters of 16 were
-// slower.
+// A step is a chain of waits and dependent instructions of 810 cycles (unpacking 310,
+// the wait for the tile 175, the store 110), far more than its share of HBM's time
+// (175), so the CTAs are small, four an SM, and their chains overlap: 330 a step. The
+// tensor pipe takes 256 of them, 64 a product whatever the tokens.
+// Measured, bf16, groups of 128: 22,016 x 4096 at 16 / 32 / 64 tokens 21 / 22 / 25
+// us (stream 7.5), 4096 x 4096 at 64 14.5, 128,256 x 4096 at 32 82 (44).  Two
+// warpgroups a CTA and clusters of 16 were slower.
 // A weight is rounded to fp16: off by at most 2^-11 of itself, or 2^-15 of its row's
 // largest scale where that is more.  Over k these average to far below the output's
 // rounding.  e is a power per weight row (int4.cuh), undone with x's in the epilogue.
