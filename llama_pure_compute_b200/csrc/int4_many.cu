@@ -433,13 +433,58 @@ bool use_pdl() {
   return on;
 }
 
+constexpr int SPLITS = 8;  // a portable cluster
+
+// CTAs per row tile: the least time of the busiest SM, a CTA costing its 64-column
+// steps and about 6 more.  `clusters[s]` clusters of s CTAs run at once, which is
+// fewer than the SMs' room divided by s: 12,288 x 4096 at 32 tokens (96 tiles) 16.3 us
+// in clusters of 5, 21.3 in clusters of 6.
+int pick_splits(int tiles, int kb, const std::atomic<int>* clusters) {
+  int best = 1;
+  int64_t cost = INT64_MAX;
+  for (int s = 1; s <= SPLITS && s <= kb; ++s) {
+    const int64_t room = clusters[s].load(std::memory_order_relaxed);
+    const int64_t c = (tiles + room - 1) / room * ((kb + s - 1) / s + 6);
+    if (c < cost) {
+      cost = c;
+      best = s;
+    }
+  }
+  return best;
+}
+
 template <typename T, int N, int SG>
-int launch(const lpc::TmaDesc& tm, const Args& a, int tiles, int group_shift, cudaStream_t s) {
+int launch(const lpc::TmaDesc& tm, Args a, int tiles, int group_shift, cudaStream_t s) {
   constexpr int SMEM = 1024 + XST * N * 128 + CST * (CODES + SG * 512) + 512;
   static std::atomic<uint64_t> mask{0};
   int rc = lpc::once_per_device_smem((const void*)int4_many_kernel<T, N, SG>, SMEM, mask);
   if (rc) return rc;
   cudaLaunchAttribute attr[2];
+  static std::atomic<int> clusters[SPLITS + 1];  // that run at once, by their size; 0: not asked yet
+  if (clusters[SPLITS].load(std::memory_order_acquire) == 0) {
+    const int sms = lpc::current_device_sms();
+    int each = 1;  // CTAs an SM that the answers count with: 4 run
+    for (int n = 1; n <= SPLITS; ++n) {
+      cudaLaunchConfig_t q = {};
+      q.gridDim = dim3((unsigned)n);
+      q.blockDim = dim3(THREADS);
+      q.dynamicSmemBytes = SMEM;
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = (unsigned)n;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      q.attrs = attr;
+      q.numAttrs = 1;
+      int count = 0;
+      if (cudaOccupancyMaxActiveClusters(&count, int4_many_kernel<T, N, SG>, &q) != cudaSuccess || count <= 0) {
+        cudaGetLastError();
+        count = each * sms / n;
+      }
+      if (n == 1) each = std::max(1, std::min(4, count / sms));
+      clusters[n].store(std::max(1, count * 4 / each), std::memory_order_release);
+    }
+  }
+  a.splits = pick_splits(tiles, a.kb, clusters);
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -464,22 +509,6 @@ int launch_n(const lpc::TmaDesc& tm, const Args& a, int n, int tiles, int group_
   if (n == 16) return two ? launch<T, 16, 2>(tm, a, tiles, group_shift, s) : launch<T, 16, 1>(tm, a, tiles, group_shift, s);
   if (n == 32) return two ? launch<T, 32, 2>(tm, a, tiles, group_shift, s) : launch<T, 32, 1>(tm, a, tiles, group_shift, s);
   return two ? launch<T, 64, 2>(tm, a, tiles, group_shift, s) : launch<T, 64, 1>(tm, a, tiles, group_shift, s);
-}
-
-// CTAs per row tile, up to 8: the least time of the busiest SM, a CTA costing its
-// 64-column steps and about 6 more; four run at once.
-int pick_splits(int tiles, int kb) {
-  const int64_t slots = 4 * lpc::current_device_sms();
-  int best = 1;
-  int64_t cost = INT64_MAX;
-  for (int s = 1; s <= 8 && s <= kb; ++s) {
-    const int64_t c = (tiles * (int64_t)s + slots - 1) / slots * ((kb + s - 1) / s + 6);
-    if (c < cost) {
-      cost = c;
-      best = s;
-    }
-  }
-  return best;
 }
 
 }  // namespace
@@ -525,7 +554,6 @@ int int4_many(const lpc_w4* w, const void* x, void* out, const void* resid, int6
   if (rc) return rc;
   const int64_t rows = (w->n_out + 15) / 16 * 16 * (w->layout == 1 ? 2 : 1);
   const int tiles = (int)((rows + 127) / 128);
-  a.splits = pick_splits(tiles, a.kb);
   a.idesc = idesc_f16(0u, 128u, (uint32_t)n, 0u, 0u);
   const int shift = w->group == 128 ? 7 : w->group == 64 ? 6 : 5;
   return w->dtype == LPC_DTYPE_BF16 ? launch_n<__nv_bfloat16>(tm, a, n, tiles, shift, s)
