@@ -17,6 +17,11 @@ Bars, from arithmetic:
                  adds that in full.  Without it (normal x and w, |w| about 4.6 s):
                  the roundings are independent, 2.7 s |x| 2^-11 sqrt(k) in the mean
                  square, and 5 of those are below the above from k = 384 on."""
+import subprocess
+import sys
+import threading
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -737,6 +742,82 @@ def test_linear_many_tokens_in_graphs_and_streams():
                 eager.append(int4_linear(int4_linear(ops.rmsnorm_forward(x, nw), w), w))
     torch.cuda.synchronize()
     assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(eager))
+
+
+FIRST_CALLS_IN_A_GRAPH = """
+import torch
+from llama_pure_compute_b200 import _lib, ops
+from llama_pure_compute_b200.int4_linear import Int4Weight, int4_linear
+g = torch.Generator(device="cuda").manual_seed(1)
+def rnd(*s):
+    return torch.randn(*s, device="cuda", generator=g).bfloat16()
+ws = [Int4Weight(rnd(n, 4096)) for n in (8192, 1024)]
+xs = [rnd(t, 4096) for t in (1, 2, 8, 16, 33, 64)]
+kv = ops.Int4KV.empty(4, 8, 700, 128)
+for t in (kv.key_codes, kv.value_codes):
+    t.random_(0, 255)
+for t in (kv.key_scales, kv.value_scales):
+    t.normal_()
+q, qkv = rnd(4, 32, 128), rnd(4, 1, 48 * 128)
+lens = torch.tensor([700, 1, 0, 350], dtype=torch.int32, device="cuda")
+pos = torch.tensor([[699], [0], [5], [349]], device="cuda")
+cos, sin = torch.ones(700, 128, device="cuda").bfloat16(), torch.zeros(700, 128, device="cuda").bfloat16()
+def all_of_them():
+    y = [int4_linear(x, w) for w in ws for x in xs]
+    y.append(ops.rope_kv_append_int4(qkv, pos, cos, sin, kv, 32))
+    y.append(ops.decode_attention_int4(q, kv, lens))
+    return y + list(ops.kv_read_int4(kv, pos))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = all_of_them()
+for _ in range(3):
+    graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, all_of_them())) and _lib.device_status() == 0
+"""
+
+
+def test_first_calls_of_a_process_are_captured():
+    """No entry point needs a call outside a graph before one inside."""
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS_IN_A_GRAPH], cwd=Path(__file__).parents[1],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_calls_from_several_threads():
+    """Each thread on a stream of its own, sizes in another order."""
+    g = gen(24)
+    weights = []
+    for n in (8192, 1024):
+        codes, s, m = random_weight(g, n, 4096, 128, BF)
+        weights.append(Int4Weight.from_codes(codes, s, m, group_size=128))
+    xs = [torch.randn(t, 4096, device=DEV, generator=g).to(BF) for t in (1, 2, 8, 16, 33, 64)]
+    kv = make_cache(g, 4, 8, 700, 128, BF)
+    q = torch.randn(4, 32, 128, device=DEV, generator=g).to(BF)
+    lens = torch.tensor([700, 1, 0, 350], dtype=torch.int32, device=DEV)
+    want = [[int4_linear(x, w) for x in xs] for w in weights]
+    att = ops.decode_attention_int4(q, kv, lens)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(start):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(start, start + 30):
+                    got = [int4_linear(xs[i % 6], w) for w in weights]
+                    out = ops.decode_attention_int4(q, kv, lens)
+                    torch.cuda.current_stream().synchronize()
+                    if not (torch.equal(out, att) and all(torch.equal(y, r[i % 6]) for y, r in zip(got, want))):
+                        wrong.append(i)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
 
 
 def test_views_off_the_16_byte_grid():
