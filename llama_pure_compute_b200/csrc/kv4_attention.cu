@@ -36,9 +36,9 @@
 // the workspace and a second kernel, or not at all where one split covers the cache.
 //
 // Measured, D = 128, bf16 (us; of the cache's bytes at 6397 GB/s): 64 sequences of
-// 1000 keys, 32 heads, 47 (99%); 32 of 1 to 4096 keys 57.5 (86%: the short ones leave
-// SMs idle at the end); 3 of 60,000 keys, 64 heads on 8, 41.6 (77%: 24 instructions
-// a key and lane, issue slots); one of 1000 keys 5.5.  What took 32 sequences of 4096
+// 1000 keys, 32 heads, 47 (99%); 32 of 1 to 4096 keys 57.1 (87%: the short ones leave
+// SMs idle at the end); 3 of 60,000 keys, 64 heads on 8, 40.4 (80%: 500 instructions
+// a warp's tile of 32 keys, 60% of the issue slots); one of 1000 keys 5.5.  What took 32 sequences of 4096
 // there from 83: ldmatrix and movmatrix in place of shuffles, the mask-free operands,
 // splits of equal length by the rule at split_keys.
 #include <algorithm>
@@ -661,7 +661,10 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
 }
 
 // One CTA per (sequence, head).  Warp w adds the splits w, w + CWARPS, ..., the
-// warps' sums meet in shared memory: the order is fixed.
+// warps' sums meet in shared memory: the order is fixed.  The kernel is a chain of
+// latencies, so the length and the first AHEAD splits a warp are asked for at once,
+// before it is known how many the sequence has (the others' numbers are not used):
+// one of 131,000 keys 31.6 us against 33.4, 8 of 8,000 19.2 against 20.3.
 constexpr int CWARPS = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(CWARPS * 32)
@@ -670,29 +673,48 @@ __global__ void __launch_bounds__(CWARPS * 32)
                        int max_splits, int chunk, lpc::Kv4Rows rows) {
   lpc::pdl_trigger();
   lpc::pdl_wait();
-  constexpr int DPL = D / 32;
+  constexpr int DPL = D / 32, AHEAD = 4;
   __shared__ float so[CWARPS][D + 2];
   const int64_t bh = blockIdx.x;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t b = bh / H;
+  const float2* ml = reinterpret_cast<const float2*>(part_ml) + bh * max_splits;
+  const float* po = part_o + bh * max_splits * D + lane * DPL;
+  const float first_m = lane < max_splits ? ml[lane].x : 0.f;
+  float pre[AHEAD][DPL];
+  float2 pre_ml[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int s = warp + k * CWARPS;
+    pre_ml[k] = make_float2(0.f, 0.f);
+    if (s < max_splits) pre_ml[k] = ml[s];
+#pragma unroll
+    for (int i = 0; i < DPL; ++i) pre[k][i] = s < max_splits ? po[(int64_t)s * D + i] : 0.f;
+  }
   int64_t row0, head_rows, cap;
   const bool inside = rows.locate(b, &row0, &head_rows, &cap);
   int len = lpc::ld_dep(seq_lens + b);
   if (len > cap) len = (int)cap;
   const int ns = inside && len > 0 ? (len + chunk - 1) / chunk : 0;
   if (ns <= 1) return;  // written by the split kernel
-  const float2* ml = reinterpret_cast<const float2*>(part_ml) + bh * max_splits;
-  const float* po = part_o + bh * max_splits * D + lane * DPL;
-  float mx = -INFINITY;
-  for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml[s].x);
+  float mx = lane < ns ? first_m : -INFINITY;
+  for (int s = lane + 32; s < ns; s += 32) mx = fmaxf(mx, ml[s].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const float Mu = mx == -INFINITY ? 0.f : mx;
   float O[DPL], Ls = 0.f;
 #pragma unroll
   for (int i = 0; i < DPL; ++i) O[i] = 0.f;
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (warp + k * CWARPS < ns) {
+      const float f = fast_exp2(pre_ml[k].x - Mu);
+#pragma unroll
+      for (int i = 0; i < DPL; ++i) O[i] = fmaf(f, pre[k][i], O[i]);
+      Ls = fmaf(f, pre_ml[k].y, Ls);
+    }
 #pragma unroll 4
-  for (int s = warp; s < ns; s += CWARPS) {
+  for (int s = warp + AHEAD * CWARPS; s < ns; s += CWARPS) {
     const float2 v = ml[s];
     const float f = fast_exp2(v.x - Mu);
 #pragma unroll
@@ -792,7 +814,7 @@ constexpr int MAX_HEADS = 65535;
 //   * 16 warps, one CTA an SM, one round: a quarter of the splits for the same
 //     keys a warp.  Measured 16 / 4 warps, us: 1000 keys of 32 heads 5.9 / 7.6,
 //     300 keys of 4 x 32 heads 4.5 / 7.1, three sequences of 60,000 (64 heads on
-//     8) 41 / 46, one of 131,000 (32 on 8) 33 / 37.
+//     8) 41 / 46, one of 131,000 (32 on 8) 33 / 37 (then with a slower second kernel).
 constexpr int64_t SLOTS_PER_SM = 4;
 int split_keys(const lpc_kv4* kv, int64_t batch, int heads, bool* wide) {
   const int64_t G = heads / kv->kv_heads, blocks = (G + HB - 1) / HB;
