@@ -38,9 +38,9 @@
 // Measured, D = 128, bf16 (us; of the cache's bytes at 6397 GB/s): 64 sequences of
 // 1000 keys, 32 heads, 47 (99%); 32 of 1 to 4096 keys 57.1 (87%: the short ones leave
 // SMs idle at the end); 3 of 60,000 keys, 64 heads on 8, 40.4 (80%: 500 instructions
-// a warp's tile of 32 keys, 60% of the issue slots); one of 1000 keys 5.5.  What took 32 sequences of 4096
-// there from 83: ldmatrix and movmatrix in place of shuffles, the mask-free operands,
-// splits of equal length by the rule at split_keys.
+// a warp's tile of 32 keys, 60% of the issue slots); one of 1000 keys 5.5.  What took
+// 32 sequences of 4096 there from 83: ldmatrix and movmatrix in place of shuffles, the
+// mask-free operands, splits of equal length by the rule at split_keys.
 #include <algorithm>
 #include <atomic>
 #include <cstdlib>
@@ -815,7 +815,11 @@ constexpr int MAX_HEADS = 65535;
 //     keys a warp.  Measured 16 / 4 warps, us: 1000 keys of 32 heads 5.9 / 7.6,
 //     300 keys of 4 x 32 heads 4.5 / 7.1, three sequences of 60,000 (64 heads on
 //     8) 41 / 46, one of 131,000 (32 on 8) 33 / 37 (then with a slower second kernel).
+//     They fill their SMs: where it costs at most an eighth more keys a CTA, SMs are
+//     left free for the second kernel's CTAs to wait on (one of 32,000 keys, 32 on 8:
+//     13.6 us in 16 splits, 14.8 in 18).
 constexpr int64_t SLOTS_PER_SM = 4;
+constexpr int64_t JOIN_PER_SM = 6;  // CTAs of the second kernel that an SM holds
 int split_keys(const lpc_kv4* kv, int64_t batch, int heads, bool* wide) {
   const int64_t G = heads / kv->kv_heads, blocks = (G + HB - 1) / HB;
   const int64_t pairs = batch * kv->kv_heads * blocks, cap = kv->max_seq_len;
@@ -846,9 +850,14 @@ int split_keys(const lpc_kv4* kv, int64_t batch, int heads, bool* wide) {
     if (costs[i] <= least + least / 8) best = std::min(best, chunks[i]);
   *wide = false;
   if (pairs <= sms) {
-    const int64_t n = sms / pairs, chunk = units((cap + n - 1) / n);
+    auto even = [&](int64_t n) { return units((cap + n - 1) / n); };
+    int64_t chunk = even(sms / pairs);
+    if (!merges_in_cluster(pairs, (cap + chunk - 1) / chunk)) {
+      const int64_t n = (sms - (batch * heads + JOIN_PER_SM - 1) / JOIN_PER_SM) / pairs;
+      if (n >= 1 && even(n) <= chunk + chunk / 8) chunk = even(n);
+    }
     const int64_t splits = (cap + chunk - 1) / chunk;
-    const int64_t t = chunk / 4 + 250 + (merges_in_cluster(pairs, splits) ? 80 : joined(splits));
+    const int64_t t = chunk / 4 + 220 + (merges_in_cluster(pairs, splits) ? 80 : joined(splits));
     if (t < least) {
       *wide = true;
       return (int)chunk;
