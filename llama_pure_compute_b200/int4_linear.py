@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ops import _dense16, _require_cuda
+from .ops import _dense16, _overlap, _require_cuda
 
 __all__ = ["Int4Weight", "int4_linear", "MAX_TOKENS"]
 
@@ -142,11 +142,6 @@ class Int4Weight:
         _lib.check(rc, "int4_pack")
         _lib.count_launch("lpc_int4_pack")
 
-    @staticmethod
-    def supported(w: torch.Tensor, group_size: int = 128) -> bool:
-        return (w.is_cuda and w.dim() == 2 and w.dtype in (torch.bfloat16, torch.float16)
-                and w.shape[1] % max(64, group_size) == 0)
-
     def memory_footprint_bytes(self) -> int:
         return self.data.numel()
 
@@ -191,7 +186,7 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
     tokens = shape[0] if len(shape) == 2 else x.numel() // k
     if tokens > MAX_TOKENS:
         raise ValueError(f"LlamaPureComputeError: int4_linear takes at most {MAX_TOKENS} rows.")
-    xp = given = x.data_ptr()
+    xp = x.data_ptr()
     if xp % 16 or not x.is_contiguous():
         x = _dense16(x)
         xp = x.data_ptr()
@@ -208,8 +203,10 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
     elif out.numel() != tokens * n or not out.is_contiguous() or out.dtype != x.dtype \
             or out.get_device() != index:
         raise ValueError("LlamaPureComputeError: out must be a contiguous [..., n_out] tensor.")
-    elif out.data_ptr() == given and tokens:
-        raise ValueError("LlamaPureComputeError: out must not be x.")
+    elif _overlap(out, x):
+        raise ValueError("LlamaPureComputeError: out must not be x or overlap it.")
+    elif rp is not None and out.data_ptr() != rp and _overlap(out, resid):
+        raise ValueError("LlamaPureComputeError: out may be resid, but not overlap it otherwise.")
     if not tokens:
         return out
     need = w._workspace.get(tokens)

@@ -702,6 +702,12 @@ def _dense16(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share bytes."""
+    x, y = a.data_ptr(), b.data_ptr()
+    return x < y + b.nbytes and y < x + a.nbytes
+
+
 def _int4_out(out: torch.Tensor, name: str, shape, kv: Int4KV) -> None:
     if out.shape != torch.Size(shape) or out.dtype != kv.dtype or out.get_device() != kv.index \
             or not out.is_contiguous():
@@ -772,6 +778,8 @@ def rope_kv_append_int4(
         q_out = qkv.new_empty(B, num_heads, S, D)
     else:
         _int4_out(q_out, "q_out", (B, num_heads, S, D), kv)
+        if _overlap(q_out, qkv):
+            raise ValueError("LlamaPureComputeError: q_out must not overlap qkv.")
     rc = _lib.call_on(index, _lib.load().lpc_rope_kv_append_int4, kv.ref, qp, pos.data_ptr(), cp, sp,
                       rows[0], q_out.data_ptr(), B, S, num_heads, code)
     if rc:
@@ -808,6 +816,8 @@ def kv_read_int4(
         v_out = kv.key_scales.new_empty(*shape)
     else:
         _int4_out(v_out, "v_out", shape, kv)
+        if _overlap(k_out, v_out):
+            raise ValueError("LlamaPureComputeError: k_out and v_out must not overlap.")
     rc = _lib.call_on(kv.index, _lib.load().lpc_kv_read_int4, kv.ref, pos.data_ptr(),
                       k_out.data_ptr(), v_out.data_ptr(), B, S)
     if rc:
@@ -866,6 +876,8 @@ def decode_attention_int4(
         out = torch.empty_like(q)
     else:
         _int4_out(out, "out", shape, kv)
+        if out.data_ptr() != qp and _overlap(out, q):
+            raise ValueError("LlamaPureComputeError: out may be q, but not overlap it otherwise.")
     lib = _lib.load()
     if workspace is None:
         workspace = decode_attention_int4_workspace(kv, B, H)

@@ -400,6 +400,20 @@ def test_attention_layouts_streams_and_repeats():
     assert torch.equal(other, out)
 
 
+@pytest.mark.parametrize("B,Hkv,G,cap,lens", [
+    (1, 8, 4, 20000, [19999]), (1, 32, 1, 1064, [1000]), (3, 2, 8, 5000, [5000, 1, 0]),
+    (64, 8, 1, 300, [5 * i for i in range(60)] + [300] * 4)])
+def test_attention_into_its_query(B, Hkv, G, cap, lens):
+    """out may be q: every split has read its queries when the first output is written."""
+    g = gen(cap + 1)
+    kv = make_cache(g, B, Hkv, cap, 128, BF)
+    q = torch.randn(B, Hkv * G, 128, device=DEV, generator=g).to(BF)
+    ln = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    want = ops.decode_attention_int4(q, kv, ln)
+    ops.decode_attention_int4(q, kv, ln, out=q)
+    assert torch.equal(q, want)
+
+
 def test_two_graphs_with_workspaces_of_their_own():
     g = gen(16)
     kv = make_cache(g, 2, 4, 1500, 128, BF)
@@ -959,6 +973,19 @@ def test_refusals():
     sq = Int4Weight(torch.zeros(128, 128, dtype=BF, device=DEV))
     with pytest.raises(ValueError, match="out must not be x"):
         int4_linear(x, sq, out=x)
+    flat = torch.zeros(5 * 128, dtype=BF, device=DEV)
+    with pytest.raises(ValueError, match="out must not be x"):
+        int4_linear(flat[:256].view(2, 128), sq, out=flat[128:384].view(2, 128))
+    with pytest.raises(ValueError, match="out may be resid"):
+        int4_linear(x, sq, "residual", resid=flat[:256].view(2, 128), out=flat[128:384].view(2, 128))
+    with pytest.raises(ValueError, match="out may be q"):
+        flat4 = torch.zeros(2 * 4 * 64 + 64, dtype=BF, device=DEV)
+        ops.decode_attention_int4(flat4[:512].view(2, 4, 64), kv, ln, out=flat4[64:].view(2, 4, 64))
+    with pytest.raises(ValueError, match="overlap qkv"):
+        ops.rope_kv_append_int4(qkv, pos, cos, sin, kv, 4, q_out=qkv.view(-1)[:512].view(2, 4, 1, 64))
+    with pytest.raises(ValueError, match="k_out and v_out"):
+        both = torch.zeros(2, 2, 1, 64, dtype=BF, device=DEV)
+        ops.kv_read_int4(kv, pos, k_out=both, v_out=both)
     # nothing to do is no error
     assert ops.decode_attention_int4(q[:0], kv, ln).shape == (0, 4, 64)
     assert ops.kv_read_int4(kv, pos[:, :0])[0].shape == (2, 2, 0, 64)
