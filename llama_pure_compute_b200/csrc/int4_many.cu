@@ -17,8 +17,8 @@
 // the wait for the tile 175, the store 110), far more than its share of HBM's time
 // (175), so the CTAs are small, four an SM, and their chains overlap: 330 a step. The
 // tensor pipe takes 256 of them, 64 a product whatever the tokens.
-// Measured, bf16, groups of 128: 22,016 x 4096 at 16 / 32 / 64 tokens 21 / 22 / 25
-// us (stream 7.5), 4096 x 4096 at 64 14.5, 128,256 x 4096 at 32 82 (44).  Two
+// Measured, bf16, groups of 128: 22,016 x 4096 at 16 / 32 / 64 tokens 21 / 22 / 24
+// us (stream 7.5), 4096 x 4096 at 64 14.3, 128,256 x 4096 at 32 82 (44).  Two
 // warpgroups a CTA and clusters of 16 were slower.
 // A weight is rounded to fp16: off by at most 2^-11 of itself, or 2^-15 of its row's
 // largest scale where that is more.  Over k these average to far below the output's
@@ -388,41 +388,57 @@ __global__ void __launch_bounds__(THREADS, 4)
 }
 
 // x [tokens, k] in bf16 as fp16, each token scaled by a power of two that brings
-// its largest value to about 2^14 (what that loses lies 2^-38 below that value).
-__global__ void __launch_bounds__(256)
+// its largest value to about 2^14 (what that loses lies 2^-38 below that value).  A
+// CTA has a token; a thread holds its first KEEP pieces of 8 values between the search
+// and the conversion, so that all loads are in flight at once.
+constexpr int XT = 512, KEEP = 4;
+__global__ void __launch_bounds__(XT)
     int4_x_kernel(const __nv_bfloat16* x, uint4* xh, float* factors, int k) {
   lpc::pdl_trigger();
   lpc::pdl_wait();
-  const uint4* src = reinterpret_cast<const uint4*>(x) + (int64_t)blockIdx.x * (k / 8);
-  uint4* dst = xh + (int64_t)blockIdx.x * (k / 8);
-  __shared__ float most[8];
-  float a = 0.f;
-  for (int i = threadIdx.x; i < k / 8; i += 256) {
-    const uint4 u = lpc::ld_dep16(src + i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  const int pieces = k / 8;
+  const uint4* src = reinterpret_cast<const uint4*>(x) + (int64_t)blockIdx.x * pieces;
+  uint4* dst = xh + (int64_t)blockIdx.x * pieces;
+  __shared__ uint32_t most[XT / 32];
+  uint4 held[KEEP];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a = fmaxf(a, fmaxf(fabsf(lpc::bf16lo(w[j])), fabsf(lpc::bf16hi(w[j]))));
+  for (int j = 0; j < KEEP; ++j) {
+    const int i = threadIdx.x + j * XT;
+    held[j] = i < pieces ? lpc::ld_dep16(src + i) : make_uint4(0u, 0u, 0u, 0u);
   }
-  // the bits of a non-negative float order as integers do
-  a = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(a)));
+  // magnitudes of bf16 order as their bits do, two at a time; a NaN is the largest
+  auto largest = [](uint32_t a, const uint4& u) {
+    constexpr uint32_t M = 0x7FFF7FFFu;
+    return __vimax3_u16x2(__vimax3_u16x2(a, u.x & M, u.y & M), u.z & M, u.w & M);
+  };
+  uint32_t a = 0u;
+#pragma unroll
+  for (int j = 0; j < KEEP; ++j) a = largest(a, held[j]);
+  for (int i = threadIdx.x + KEEP * XT; i < pieces; i += XT) a = largest(a, lpc::ld_dep16(src + i));
+  a = __reduce_max_sync(0xffffffffu, max(a & 0xFFFFu, a >> 16));
   if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = a;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a = fmaxf(a, most[i]);
+  for (int i = 0; i < XT / 32; ++i) a = max(a, most[i]);
   int e = 0;
-  if (a > 0.f && a < INFINITY) e = min(126, 14 - ((int)(__float_as_uint(a) >> 23) - 127));
+  if (a > 0u && a < 0x7F80u) e = min(126, 14 - ((int)(a >> 7) - 127));
   const float up = __uint_as_float((uint32_t)(127 + e) << 23);
   if (threadIdx.x == 0) factors[blockIdx.x] = __uint_as_float((uint32_t)(127 - e) << 23);
-  for (int i = threadIdx.x; i < k / 8; i += 256) {
-    const uint4 u = lpc::ld_dep16(src + i);
+  auto scaled = [&](const uint4& u) {
     uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const __half2 h = __floats2half2_rn(lpc::bf16lo(w[j]) * up, lpc::bf16hi(w[j]) * up);
       w[j] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+#pragma unroll
+  for (int j = 0; j < KEEP; ++j) {
+    const int i = threadIdx.x + j * XT;
+    if (i < pieces) dst[i] = scaled(held[j]);
   }
+  for (int i = threadIdx.x + KEEP * XT; i < pieces; i += XT) dst[i] = scaled(lpc::ld_dep16(src + i));
 }
 
 bool use_pdl() {
@@ -538,7 +554,7 @@ int int4_many(const lpc_w4* w, const void* x, void* out, const void* resid, int6
     attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)tokens);
-    cfg.blockDim = dim3(256);
+    cfg.blockDim = dim3(XT);
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
