@@ -78,10 +78,13 @@ class RaggedKVCache:
         return 2 * self.num_layers * per
 
     def select(self, ids: Sequence[int]) -> None:
-        """Batch row b of the next forwards is sequence ids[b]."""
+        """Batch row b of the next forwards is sequence ids[b], each sequence at
+        most once: two rows of a batch would write the same cache rows."""
         ids = [int(i) for i in ids]
         if not ids or min(ids) < 0 or max(ids) >= self.num_sequences:
             raise ValueError("sequence ids outside the cache")
+        if len(set(ids)) < len(ids):
+            raise ValueError("a sequence is selected twice")
         self.active_ids = ids
         idx = torch.tensor(ids, dtype=torch.int64, device=self.device)
         self.active_base = self.seq_base[idx].contiguous()
