@@ -238,6 +238,8 @@ class BatchedGreedyDecoder:
 
     # -- decode --------------------------------------------------------------
     def _step_body(self) -> None:
+        if self.ragged and self.kv.active_ids != list(range(self.B)):
+            self.kv.select(range(self.B))  # another user of the cache selected since
         logits = self.model(self.tokens, positions=self.positions, kv_cache=self.kv,
                             last_token_only=True)
         nxt = torch.argmax(logits[:, -1, :], dim=-1)

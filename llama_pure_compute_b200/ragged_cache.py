@@ -61,6 +61,7 @@ class RaggedKVCache:
         self.seq_cap = torch.tensor(caps, dtype=torch.int32, device=self.device)
         self.seq_lens = torch.zeros(len(caps), dtype=torch.int32, device=self.device)
         self._ws = None
+        self._captured: list = []
         self._allocate()
         self.select(range(len(caps)))
 
@@ -79,7 +80,8 @@ class RaggedKVCache:
 
     def select(self, ids: Sequence[int]) -> None:
         """Batch row b of the next forwards is sequence ids[b], each sequence at
-        most once: two rows of a batch would write the same cache rows."""
+        most once: two rows of a batch would write the same cache rows.  A step
+        captured in a CUDA graph stays with the sequences of its capture."""
         ids = [int(i) for i in ids]
         if not ids or min(ids) < 0 or max(ids) >= self.num_sequences:
             raise ValueError("sequence ids outside the cache")
@@ -105,6 +107,9 @@ class RaggedKVCache:
         B, S = positions.shape
         if B != len(self.active_ids):
             raise ValueError(f"batch of {B} rows but {len(self.active_ids)} selected sequences")
+        if torch.cuda.is_current_stream_capturing():
+            # the graph reads and writes these wherever the selection goes later
+            self._captured.append((self._idx, self.active_base, self.active_cap, self.active_lens))
         if S == 1:
             ctx.decode = True
             self.active_lens.copy_(positions[:, -1] + 1)
