@@ -21,6 +21,7 @@ import torch.nn.functional as F
 from .config import LlamaModelConfig
 from .int4_cache import Int4KVCache
 from .kv_manager import KVCacheManager
+from .ops import StepWorkspaces
 from .ragged_cache import RaggedKVCache
 
 __all__ = ["GenerationConfig", "apply_repetition_penalty", "sample_next_token", "LlamaGenerator",
@@ -87,6 +88,7 @@ class _RowView:
         self.n_kv_heads = base.n_kv_heads
         self.head_dim = base.head_dim
         self.num_layers = base.num_layers
+        self._workspaces = StepWorkspaces()
 
     def append_qkv(self, **kw):
         return KVCacheManager.append_qkv(self, **kw)  # type: ignore[arg-type]

@@ -21,8 +21,8 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from .flash_attention import flash_attention_v2
-from .ops import (Int4KV, decode_attention_int4, decode_attention_int4_workspace, kv_read_int4,
-                  rope_kv_append_int4)
+from .ops import (Int4KV, StepWorkspaces, decode_attention_int4, decode_attention_int4_workspace,
+                  kv_read_int4, rope_kv_append_int4)
 from .ragged_cache import RaggedKVCache
 
 __all__ = ["Int4KVCache", "Int4RaggedKVCache"]
@@ -76,7 +76,7 @@ class Int4KVCache:
         self.max_seq_len, self.n_kv_heads = first.max_seq_len, first.kv_heads
         self.head_dim, self.dtype, self.device = first.head_dim, first.dtype, first.device
         self.active_batch_size = 0
-        self._ws = None
+        self._workspaces = StepWorkspaces()
         self._context: Optional[torch.Tensor] = None
 
     def row_view(self, start: int, count: int) -> "Int4KVCache":
@@ -123,10 +123,8 @@ class Int4KVCache:
     # -- step interface used by the model -----------------------------------
     def decode_workspace(self, batch: int, num_heads: int) -> torch.Tensor:
         """Split partials of the decode kernel, kept across steps."""
-        if self._ws is None or self._ws[0] != (batch, num_heads):
-            self._ws = ((batch, num_heads),
-                        decode_attention_int4_workspace(self.layers[0], batch, num_heads))
-        return self._ws[1]
+        return self._workspaces.get((batch, num_heads), lambda: decode_attention_int4_workspace(
+            self.layers[0], batch, num_heads))
 
     @torch.no_grad()
     def prepare_forward(self, positions: torch.Tensor, ctx, num_heads: int) -> None:
@@ -175,10 +173,8 @@ class Int4RaggedKVCache(RaggedKVCache):
         self.active = [kv.select(self.active_base, self.active_cap) for kv in self.layers]
 
     def decode_workspace(self, batch: int, num_heads: int) -> torch.Tensor:
-        key = (batch, num_heads)
-        if self._ws is None or self._ws[0] != key:
-            self._ws = (key, decode_attention_int4_workspace(self.layers[0], batch, num_heads))
-        return self._ws[1]
+        return self._workspaces.get((batch, num_heads), lambda: decode_attention_int4_workspace(
+            self.layers[0], batch, num_heads))
 
     @torch.no_grad()
     def prepare_forward(self, positions: torch.Tensor, ctx, num_heads: int) -> None:

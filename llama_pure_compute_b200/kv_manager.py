@@ -24,8 +24,8 @@ from typing import Optional, Tuple, Union
 import torch
 
 from .flash_attention import flash_attention_v2
-from .ops import (decode_attention, decode_attention_workspace, qkv_rope_append, rope_kv_append,
-                  update_kv_cache)
+from .ops import (StepWorkspaces, decode_attention, decode_attention_workspace, qkv_rope_append,
+                  rope_kv_append, update_kv_cache)
 
 logger = logging.getLogger("llama_pure_compute_b200.kv_manager")
 
@@ -77,6 +77,7 @@ class KVCacheManager:
                                             for _ in range(num_layers)]
         self.seq_lens = torch.zeros(max_batch_size, dtype=torch.int32, device=self.device)
         self.active_batch_size = 0
+        self._workspaces = StepWorkspaces()
         logger.info("Allocated KV cache: layers=%d batch=%d seq=%d kv_heads=%d head_dim=%d "
                     "memory=%.2f GiB", num_layers, max_batch_size, max_seq_len, n_kv_heads,
                     head_dim, self.memory_footprint_bytes() / 2**30)
@@ -216,14 +217,8 @@ class KVCacheManager:
     # -- model-facing step interface (KVCacheManager and RaggedKVCache) -------
     def decode_workspace(self, batch: int, num_heads: int) -> torch.Tensor:
         """Split-KV partials buffer of the decode kernel, kept across steps."""
-        key = (batch, num_heads)
-        ws = getattr(self, "_decode_ws", None)
-        if ws is None or ws[0] != key:
-            t = decode_attention_workspace(batch, num_heads, self.max_seq_len, self.head_dim,
-                                           self.seq_lens.device)
-            ws = (key, t)
-            self._decode_ws = ws
-        return ws[1]
+        return self._workspaces.get((batch, num_heads), lambda: decode_attention_workspace(
+            batch, num_heads, self.max_seq_len, self.head_dim, self.seq_lens.device))
 
     @torch.no_grad()
     def prepare_forward(self, positions: torch.Tensor, ctx, num_heads: int) -> None:

@@ -335,6 +335,28 @@ def decode_attention_workspace(batch: int, heads: int, max_seq_len: int, head_di
     return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
+class StepWorkspaces:
+    """The decode workspaces of a cache's steps, by (batch, heads): the last one
+    asked for and, for good, each that a step was captured with, since its graph
+    keeps writing there.  The steps of one cache run one after another, as they
+    share its lengths too."""
+
+    def __init__(self) -> None:
+        self._last = (None, None)
+        self._captured = {}
+
+    def get(self, key, make) -> torch.Tensor:
+        ws = self._captured.get(key)
+        if ws is None and self._last[0] == key:
+            ws = self._last[1]
+        if ws is None:
+            ws = make()
+            self._last = (key, ws)
+        if torch.cuda.is_current_stream_capturing():
+            self._captured[key] = ws
+        return ws
+
+
 def decode_attention(
     q: torch.Tensor,
     key_cache: torch.Tensor,

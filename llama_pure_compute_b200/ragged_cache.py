@@ -29,8 +29,8 @@ from typing import List, Optional, Sequence
 import torch
 
 from .flash_attention import flash_attention_v2
-from .ops import (decode_attention_ragged, decode_attention_workspace, qkv_rope_append,
-                  rope_kv_append_ragged)
+from .ops import (StepWorkspaces, decode_attention_ragged, decode_attention_workspace,
+                  qkv_rope_append, rope_kv_append_ragged)
 
 __all__ = ["RaggedKVCache"]
 
@@ -60,7 +60,7 @@ class RaggedKVCache:
         self.seq_base = torch.tensor(bases, dtype=torch.int64, device=self.device)
         self.seq_cap = torch.tensor(caps, dtype=torch.int32, device=self.device)
         self.seq_lens = torch.zeros(len(caps), dtype=torch.int32, device=self.device)
-        self._ws = None
+        self._workspaces = StepWorkspaces()
         self._captured: list = []
         self._allocate()
         self.select(range(len(caps)))
@@ -96,11 +96,9 @@ class RaggedKVCache:
 
     # -- step interface used by the model ----------------------------------
     def decode_workspace(self, batch: int, num_heads: int) -> torch.Tensor:
-        key = (batch, num_heads)
-        if self._ws is None or self._ws[0] != key:
-            self._ws = (key, decode_attention_workspace(batch, num_heads, self.max_seq_len,
-                                                        self.head_dim, self.device))
-        return self._ws[1]
+        """Split partials of the decode kernel, kept across steps."""
+        return self._workspaces.get((batch, num_heads), lambda: decode_attention_workspace(
+            batch, num_heads, self.max_seq_len, self.head_dim, self.device))
 
     @torch.no_grad()
     def prepare_forward(self, positions: torch.Tensor, ctx, num_heads: int) -> None:
