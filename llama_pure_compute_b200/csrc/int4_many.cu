@@ -56,6 +56,18 @@ constexpr int MAX_TOKENS = 64;
 constexpr uint32_t TMEM_COLS = 128;  // 64 sums + 2 tiles of 32; four CTAs share an SM's 512
 constexpr uint32_t A_COL = 64;
 
+// A CTA that waits for tensor memory while its cluster waits for it, beside one of
+// another stream's clusters that waits the other way round, would wait for ever.  So
+// shared memory is asked for such that whatever shares an SM also shares its 512
+// columns: four of these CTAs and not five, two beside a wsgemm CTA of 256 columns
+// (which asks for 90 KB), none beside a CTA pair of the SwiGLU kernel (182 KB, 512
+// columns) or two such wsgemm CTAs.
+constexpr int SM_SMEM = 228 * 1024;  // of an SM; a CTA takes 1 KB more than it asks for
+constexpr int MIN_SMEM = 52 * 1024;
+static_assert(5 * (MIN_SMEM + 1024) > SM_SMEM && 91 * 1024 + 3 * (MIN_SMEM + 1024) > SM_SMEM &&
+                  2 * 91 * 1024 + MIN_SMEM + 1024 > SM_SMEM &&
+                  182 * 1024 + MIN_SMEM + 1024 > SM_SMEM, "tensor memory");
+
 enum { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_SWIGLU = 2 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
@@ -471,7 +483,9 @@ int pick_splits(int tiles, int kb, const std::atomic<int>* clusters) {
 
 template <typename T, int N, int SG>
 int launch(const lpc::TmaDesc& tm, Args a, int tiles, int group_shift, cudaStream_t s) {
-  constexpr int SMEM = 1024 + XST * N * 128 + CST * (CODES + SG * 512) + 512;
+  constexpr int USED = 1024 + XST * N * 128 + CST * (CODES + SG * 512) + 512;
+  constexpr int SMEM = USED > MIN_SMEM ? USED : MIN_SMEM;
+  static_assert(4 * (SMEM + 1024) <= SM_SMEM, "four CTAs an SM");
   static std::atomic<uint64_t> mask{0};
   int rc = lpc::once_per_device_smem((const void*)int4_many_kernel<T, N, SG>, SMEM, mask);
   if (rc) return rc;

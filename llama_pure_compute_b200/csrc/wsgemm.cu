@@ -722,6 +722,12 @@ Plan make_plan(int64_t M, int64_t n_out, int K, int epilogue, bool norm) {
   p.smem = p.stages * stage_bytes + 1024 + 8 * (2 * p.stages + 4) + extra;
   p.tmem_cols = 32;
   while ((int)p.tmem_cols < p.NT) p.tmem_cols <<= 1;
+  // What shares an SM has to share its 512 columns of tensor memory: a CTA that
+  // waits for them while its cluster waits for it, beside one of another stream that
+  // waits the other way round, would wait for ever.  At 256 columns: two of these
+  // CTAs, not three (which two stages of 144 to 176 tokens would leave room for), and
+  // none of the 4-bit products' CTAs (128 columns, 53 KB) beside two.
+  if (p.tmem_cols == 256) p.smem = std::max(p.smem, 90 * 1024);
   p.splits = choose_splits(p, K);
   return p;
 }
