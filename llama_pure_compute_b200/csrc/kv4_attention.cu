@@ -25,10 +25,12 @@
 // q enters as fp16 scaled per head by a power of two so that its largest value
 // is about 2^14: a bf16 or fp16 q (below 2^114) then loses nothing but what lies
 // 2^-38 below that value.  P s_g enters as fp16 (rounded to 2^-11, finer than the
-// bf16 that P is usually held in); the running reference M of the softmax includes
-// the exponent of the tile's largest V scale, so that P s_g stays near 2^5 for
-// the heaviest key whatever the scales are (and a key counts down to 2^-29 of its
-// tile's largest scale).  Sums, maxima and statistics are fp32.
+// bf16 that P is usually held in); the running reference M of the softmax is that of
+// P s, each key's score with the exponent of its own V scale, so that the largest P s
+// stays near 2^5 whatever the scales are.  What is 2^-19 of it loses a bit a halving:
+// another key's share, which then does not show beside the largest, or the other half
+// of the dims where its scales are that much smaller.  Sums, maxima and statistics are
+// fp32.
 //
 // Each warp walks its own 32-key tiles through a ring of shared-memory stages
 // filled by cp.async, with no barrier between warps until the end; the warps
@@ -69,7 +71,7 @@ constexpr int HB = 8;         // query heads per CTA (columns of the products)
 constexpr int UNIT = 128;     // shortest split: one tile per warp; workspace granularity
 constexpr int CLUSTER = 4;    // splits that a cluster merges
 constexpr float LOG2E = 1.4426950408889634f;
-// The reference M is set RISE below the heaviest key and moved when a key
+// The reference M is set RISE below the largest P s and moved when a key
 // exceeds it by LIFT: fp16 holds 2^(LIFT + 1), and a tile that stays below
 // costs one vote instead of a rescaling of the accumulators.
 constexpr float RISE = 5.f, LIFT = 13.f;
@@ -165,22 +167,20 @@ __device__ __forceinline__ void unpack_sm<__half>(uint32_t w, float& s, float& m
   m = f.y;
 }
 
-// Exponent of the larger of a row's two V scales as an integer key (its bits,
-// 0 for a non-finite scale, which must not move the other keys' reference).
+// What a key adds to its score for the reference M: the exponent of the larger of its two
+// V scales, as an integer that orders as it (non-finite numbers, which must not move the
+// other keys' reference, turn negative).
 template <typename T>
 __device__ __forceinline__ uint32_t scale_bits(uint2 row) {
-  constexpr uint32_t INF = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-  uint32_t a = row.x & 0x7FFFu, b = row.y & 0x7FFFu;
-  a = a >= INF ? 0u : a;
-  b = b >= INF ? 0u : b;
-  return a > b ? a : b;
+  constexpr uint32_t UP = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+  return __vimax3_s16x2((row.x & 0x7FFF7FFFu) + UP, (row.y & 0x7FFF7FFFu) + UP, 0u) & 0xFFFFu;
 }
 template <typename T>
 __device__ __forceinline__ float scale_exponent(uint32_t bits) {
-  if constexpr (std::is_same<T, __half>::value) return (float)((int)(bits >> 10) - 15);
+  if constexpr (std::is_same<T, __half>::value) return (float)((int)(bits >> 10) - 16);
   // below 2^-60 the scales no longer move the reference: the sum of the P
   // themselves, up to 2^60 times larger than P s, has to stay in fp32
-  return fmaxf((float)((int)(bits >> 7) - 127), -60.f);
+  return fmaxf((float)((int)(bits >> 7) - 128), -60.f);
 }
 
 template <int D, int W>
@@ -459,23 +459,30 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
             for (int n = 0; n < NH; ++n) x[u][i][n] = -INFINITY;
     }
     // the reference M, moved only when a key rises far above it
-    const float ev = scale_exponent<T>(__reduce_max_sync(
-        0xffffffffu, scale_bits<T>(*reinterpret_cast<const uint2*>(svs + lane * 8))));
-    float top[NH];
-    bool rise = false;
+    const uint32_t bits = scale_bits<T>(*reinterpret_cast<const uint2*>(svs + lane * 8));
+    const float most = scale_exponent<T>(__reduce_max_sync(0xffffffffu, bits));
+    bool rise = false;  // for all that the highest score and the largest scale say
 #pragma unroll
-    for (int n = 0; n < NH; ++n) {
-      top[n] = fmaxf(fmaxf(x[0][0][n], x[0][1][n]), fmaxf(x[1][0][n], x[1][1][n])) + ev;
-      rise |= top[n] > M[n] + LIFT;
-    }
+    for (int n = 0; n < NH; ++n)
+      rise |= fmaxf(fmaxf(x[0][0][n], x[0][1][n]), fmaxf(x[1][0][n], x[1][1][n])) + most > M[n] + LIFT;
     if (__any_sync(0xffffffffu, rise)) {
+      const float mine = scale_exponent<T>(bits);
+      float v[NH];
+#pragma unroll
+      for (int n = 0; n < NH; ++n) v[n] = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float e = __shfl_sync(0xffffffffu, mine, 16 * u + 8 * i + r);
+#pragma unroll
+          for (int n = 0; n < NH; ++n) v[n] = fmaxf(v[n], x[u][i][n] + e);
+        }
 #pragma unroll
       for (int n = 0; n < NH; ++n) {
-        float v = top[n];
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-        const float next = fmaxf(fmaxf(M[n], v - RISE), -1e30f);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) v[n] = fmaxf(v[n], __shfl_xor_sync(0xffffffffu, v[n], o));
+        const float next = fmaxf(fmaxf(M[n], v[n] - RISE), -1e30f);
         const float f = fast_exp2(M[n] - next);
         M[n] = next;
         l[n] *= f;
