@@ -170,10 +170,15 @@ __device__ __forceinline__ void unpack_sm<__half>(uint32_t w, float& s, float& m
 // What a key adds to its score for the reference M: the exponent of the larger of its two
 // V scales, as an integer that orders as it (non-finite numbers, which must not move the
 // other keys' reference, turn negative).
+// In bf16 at least 40 below the exponent of its minima, so that P m stays in fp32 too;
+// the codes of a key that this decides count less than 2^-40 of its minimum.
 template <typename T>
 __device__ __forceinline__ uint32_t scale_bits(uint2 row) {
-  constexpr uint32_t UP = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
-  return __vimax3_s16x2((row.x & 0x7FFF7FFFu) + UP, (row.y & 0x7FFF7FFFu) + UP, 0u) & 0xFFFFu;
+  constexpr bool HALF = std::is_same<T, __half>::value;
+  constexpr uint32_t UP = HALF ? 0x04000400u : 0x00800080u;
+  const uint32_t v = __vimax3_s16x2((row.x & 0x7FFF7FFFu) + UP, (row.y & 0x7FFF7FFFu) + UP, 0u);
+  if constexpr (HALF) return v & 0xFFFFu;
+  return (uint32_t)max((int)(v & 0xFFFFu), (int)(v >> 16) - (40 << 7));
 }
 template <typename T>
 __device__ __forceinline__ float scale_exponent(uint32_t bits) {

@@ -86,3 +86,18 @@ def test_values_of_all_sizes_in_any_order(dtype, spread):
     size = 2.0 ** (torch.rand(1, Hkv, n, 1, device=DEV, generator=g) * (hi - lo) + lo)
     q = (torch.randn(1, Hkv * G, D, device=DEV, generator=g) * spread).to(dtype)
     check(q, ops.Int4KV(kc, ks, vc, (vs * size).to(dtype)), n)
+
+
+@pytest.mark.parametrize("value", [1e-30, 1.0, 1e18, -3e25, 2e38])
+@pytest.mark.parametrize("n", [1, 33, 700])
+def test_constant_values(value, n):
+    """Rows whose halves are constants (scale 0): the output is the constant, however
+    large."""
+    g = gen(4)
+    D = 64
+    kc, ks = held_rows(g, (1, 1, n), D, BF)
+    vc = torch.zeros(1, 1, n, D // 2, dtype=torch.uint8, device=DEV)
+    vs = torch.zeros(1, 1, n, 4, dtype=BF, device=DEV)
+    vs[..., 1::2] = value
+    q = torch.randn(1, 4, D, device=DEV, generator=g).to(BF)
+    check(q, ops.Int4KV(kc, ks, vc, vs), n)
