@@ -2,11 +2,10 @@
 // description of the codes' order).
 //   codes    [tile row][k / 64][512 bytes]        tile rows of 16 weight rows
 //   numbers  [tile row][k / group][8][4] of T     (s, m) of rows r and r + 8
-//   scaled   [tile row][k / group][16][2] fp16    (s 2^(24 + e), m 2^e) of each row,
-//                                                 s 2^(20 + e) for rows 8..15
+//   scaled   [tile row][k / group][16][2] fp16    (s 2^e, m 2^e) of each row
 //   factors  [tile row][16] fp32                  2^-e of each row
-// e is a power per row that brings the larger of |s| 2^24 and |m| to about 2^14:
-// fp16 holds both exactly unless a group's are 2^-28 of the row's largest.
+// e is a power per row that brings the largest 15 |s| + |m| to 2^14..2^15: fp16 holds
+// its groups' numbers exactly unless they are below 2^-28 of that.
 #pragma once
 
 #include "lpc_common.cuh"
@@ -37,7 +36,7 @@ inline Int4Parts int4_parts(void* base, int64_t n_out, int k, int group, int lay
   return p;
 }
 
-// Token counts and widths whose x does not fit the kernel for few tokens.
+// Token counts and weights that the kernels of int4_linear.cu are not for.
 int int4_many(const lpc_w4* w, const void* x, void* out, const void* resid, int64_t tokens,
               int epilogue, void* workspace, cudaStream_t s);
 

@@ -796,10 +796,8 @@ __global__ void int4_pack_scaled_kernel(const T* __restrict__ s, const T* __rest
   const int64_t row = source_row(p, i, n_out, layout);
   float top = 0.f;
   for (int g = 0; row >= 0 && g < ng; ++g) {
-    const float a = fabsf(Num<T>::to_f(s[row * ng + g])) * 16777216.f;
-    const float b = fabsf(Num<T>::to_f(m[row * ng + g]));
+    const float a = fmaf(15.f, fabsf(Num<T>::to_f(s[row * ng + g])), fabsf(Num<T>::to_f(m[row * ng + g])));
     if (a < INFINITY) top = fmaxf(top, a);
-    if (b < INFINITY) top = fmaxf(top, b);
   }
   int e = 0;
   if (top > 0.f) e = max(-126, min(126, 14 - ((int)(__float_as_uint(top) >> 23) - 127)));
@@ -808,11 +806,10 @@ __global__ void int4_pack_scaled_kernel(const T* __restrict__ s, const T* __rest
   for (int g = 0; g < ng; ++g) {
     float a = 0.f, b = 0.f;
     if (row >= 0) {
-      a = Num<T>::to_f(s[row * ng + g]) * 16777216.f * up;
+      a = Num<T>::to_f(s[row * ng + g]) * up;
       b = Num<T>::to_f(m[row * ng + g]) * up;
     }
-    // the codes of rows 8..15 lie 4 bits higher in their words
-    scaled[(p * ng + g) * 16 + i] = __floats2half2_rn(i < 8 ? a : a * 0.0625f, b);
+    scaled[(p * ng + g) * 16 + i] = __floats2half2_rn(a, b);
   }
 }
 

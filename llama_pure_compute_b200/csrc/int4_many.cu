@@ -1,28 +1,33 @@
-// Products with 4-bit weights for more tokens than int4_linear.cu's kernels take
-// (up to 64): tcgen05, weights as the M operand.
+// Products with 4-bit weights, up to 64 tokens, where int4_linear.cu's pick() finds
+// neither of its own kernels cheaper: tcgen05, weights as the M operand.
 //
 // mma.sync needs one instruction for 16 rows x 8 tokens x 16 columns: from 16
 // tokens on its issue rate, not HBM, is the limit (32 tokens, 22,016 x 4096: 41
 // us).  Here a CTA takes 128 weight rows and all tokens; 64 columns at a time
 //   * a warpgroup turns codes into fp16 weights in registers, a thread its own
-//     row (one AND and half a packed FMA a code: code c is the subnormal half
-//     c * 2^-24, and the packed FMA with (s 2^(24 + e), m 2^e) gives (s c + m) 2^e
-//     with one rounding), and stores them to tensor memory: the A operand never
-//     touches shared memory, whose bandwidth a 16 KB tile per 4 KB of codes
-//     would exceed;
+//     row (one logic instruction makes two codes the halves 1024 + c, or 64 + c from
+//     the upper nibbles; a packed subtraction leaves c, and the packed FMA with
+//     (s 2^e, m 2^e) gives (s c + m) 2^e with one rounding), and stores them to tensor
+//     memory: the A operand never touches shared memory, whose bandwidth a 16 KB tile
+//     per 4 KB of codes would exceed.  Without the subtraction, codes as the subnormals
+//     c * 2^-24, it was 2 to 6% faster, but s had to carry the 2^24, which left the
+//     weights the lowest of fp16's exponents: groups 2^-8 of their row's largest lost bits;
 //   * x, fp16 (bf16 rows are converted first, scaled by a power of two each, by a
 //     small kernel), comes by TMA as the B operand;
 //   * one thread issues tcgen05.mma with the fp32 sums in tensor memory.
-// A step is a chain of waits and dependent instructions of 810 cycles (unpacking 310,
-// the wait for the tile 175, the store 110), far more than its share of HBM's time
-// (175), so the CTAs are small, four an SM, and their chains overlap: 330 a step. The
-// tensor pipe takes 256 of them, 64 a product whatever the tokens.
-// Measured, bf16, groups of 128: 22,016 x 4096 at 16 / 32 / 64 tokens 21 / 22 / 24
-// us (stream 7.5), 4096 x 4096 at 64 14.3, 128,256 x 4096 at 32 82 (44).  Two
+// A step is a chain of waits and dependent instructions of over 800 cycles (without the
+// subtraction 810: unpacking 310, the wait for the tile 175, the store 110), far more than
+// its share of HBM's time (175), so the CTAs are small, four an SM, and their chains
+// overlap: about 350 a step. The tensor pipe takes 256 of them, 64 a product whatever the
+// tokens.
+// Measured, bf16, groups of 128: 22,016 x 4096 at 16 / 32 / 64 tokens 21.3 / 22.9 / 24.7
+// us (stream 7.5), 4096 x 4096 at 64 14.6, 128,256 x 4096 at 32 86.8 (44).  Two
 // warpgroups a CTA and clusters of 16 were slower.
-// A weight is rounded to fp16: off by at most 2^-11 of itself, or 2^-15 of its row's
-// largest scale where that is more.  Over k these average to far below the output's
-// rounding.  e is a power per weight row (int4.cuh), undone with x's in the epilogue.
+// A weight is rounded to fp16: off by at most 2^-11 of itself, or 2^-39 of its row's
+// largest |m| + 15 |s| where that is more.  The roundings are independent.  Measured,
+// normal x and w, k = 4096, relative: with bf16 numbers 2.2e-5, which the outputs (1.7e-3)
+// do not show; with fp16 numbers 2.0e-4, beside the outputs' own 2.1e-4 2.9e-4 in all.  e
+// is a power per weight row (int4.cuh), undone with x's in the epilogue.
 // Few row tiles: clusters of up to 8 CTAs split the columns and add their sums
 // through distributed shared memory, in rank order.
 #include <algorithm>
@@ -87,8 +92,11 @@ __device__ __forceinline__ void ld_cluster4(uint32_t addr, float (&v)[4]) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ uint32_t fma_h2(uint32_t a, __half2 s, __half2 m) {
-  const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&a), s, m);
+// s c + m of two codes: with `one` in its upper bits a code is the half base + c, exactly.
+__device__ __forceinline__ uint32_t weights(uint32_t w, uint32_t mask, uint32_t one, __half2 base,
+                                            __half2 s, __half2 m) {
+  const uint32_t a = (w & mask) | one;
+  const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&a), base), s, m);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
@@ -208,8 +216,10 @@ __global__ void __launch_bounds__(THREADS, 4)
 
   if (warp < 4) {
     const uint32_t a_tmem = tmem + ((uint32_t)(warp * 32) << 16) + A_COL;
-    // rows 8..15 of a tile row are the nibbles beside: 16-fold, which their scale undoes
+    // rows 8..15 of a tile row are the nibbles beside: as low bits of 64 + c, not of 1024 + c
     const uint32_t mask = (row & 8) ? 0x00F000F0u : 0x000F000Fu;
+    const uint32_t one = (row & 8) ? 0x54005400u : 0x64006400u;
+    const __half2 base = *reinterpret_cast<const __half2*>(&one);
     const int r = row & 7;
     const uint8_t* src = smem_raw + (cring - raw) + (row >> 4) * 512 + r * 64;
     const uint8_t* num = smem_raw + (cring - raw) + CODES + row * 4;
@@ -239,8 +249,8 @@ __global__ void __launch_bounds__(THREADS, 4)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {  // columns 32 (j / 2) + 8 t + 4 (j % 2) + 0..3
             const int h = j >> 1, at = 4 * t + 2 * (j & 1), g = SG == 2 ? h : 0;
-            v[h][at] = fma_h2(w[j] & mask, sc[g], mn[g]);
-            v[h][at + 1] = fma_h2((w[j] >> 8) & mask, sc[g], mn[g]);
+            v[h][at] = weights(w[j], mask, one, base, sc[g], mn[g]);
+            v[h][at + 1] = weights(w[j] >> 8, mask, one, base, sc[g], mn[g]);
           }
         }
         // the tile's last products must be done (a warp goes on as one)
