@@ -43,13 +43,11 @@ class Int4Weight:
         if layout not in LAYOUTS:
             raise ValueError(f"LlamaPureComputeError: unknown packed layout {layout!r}")
         for t in (w0,) if w1 is None else (w0, w1):
-            _require_cuda(t, "weight")
-            if t.dim() != 2 or t.shape[1] != w0.shape[1]:
+            self._check_source(t)
+            if t.shape[1] != w0.shape[1]:
                 raise ValueError("LlamaPureComputeError: weights must be 2-D, of the same width.")
             if t.dtype != w0.dtype or t.device != w0.device:
                 raise ValueError("LlamaPureComputeError: up weight must match the gate weight.")
-        if w0.dtype not in (torch.bfloat16, torch.float16):
-            raise TypeError("LlamaPureComputeError: int4 weights are made of bf16 or fp16 weights.")
         if w1 is not None and (layout != "swiglu" or w1.shape != w0.shape):
             raise ValueError("LlamaPureComputeError: up weight must match the gate weight (layout "
                              "'swiglu').")
@@ -84,6 +82,23 @@ class Int4Weight:
         self._pack(codes, scales, mins, layout, group_size)
         return self
 
+    @classmethod
+    def check(cls, w: torch.Tensor, group_size: int = 128) -> None:
+        """Raises what ``Int4Weight(w, group_size=)`` would of its arguments and
+        values, and makes nothing."""
+        cls._check_source(w)
+        cls._check_sizes(w.shape[1], group_size)
+        for _ in cls._stretches(w.detach(), group_size):
+            pass
+
+    @staticmethod
+    def _check_source(w: torch.Tensor) -> None:
+        _require_cuda(w, "weight")
+        if w.dim() != 2:
+            raise ValueError("LlamaPureComputeError: weights must be 2-D, of the same width.")
+        if w.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError("LlamaPureComputeError: int4 weights are made of bf16 or fp16 weights.")
+
     @staticmethod
     def _check_sizes(k: int, group_size: int) -> None:
         if group_size not in (32, 64, 128):
@@ -98,24 +113,33 @@ class Int4Weight:
         takes them; runs where the weight is, a stretch of rows at a time."""
         rows, k = w.shape
         Int4Weight._check_sizes(k, group_size)
-        if not bool(torch.isfinite(w).all()):
-            raise ValueError("LlamaPureComputeError: a weight with non-finite values has no 4-bit form.")
         codes = torch.empty(rows, k // 2, dtype=torch.uint8, device=w.device)
         scales = torch.empty(rows, k // group_size, dtype=w.dtype, device=w.device)
         mins = torch.empty_like(scales)
-        step = max(1, (1 << 25) // k)
-        for at in range(0, rows, step):
-            g = w[at:at + step].float().view(-1, k // group_size, group_size)
-            lo = g.amin(-1)
-            s = ((g.amax(-1) - lo) / 15).to(w.dtype)
-            if not bool(torch.isfinite(s).all()):
-                raise ValueError("LlamaPureComputeError: a group's range overflows the scale's dtype.")
+        for at, g, lo, s in Int4Weight._stretches(w, group_size):
             sf = s.float()[..., None]
             c = ((g - lo[..., None]) / torch.where(sf == 0, torch.ones_like(sf), sf)).round_()
             c = c.clamp_(0, 15).to(torch.uint8).view(-1, k // 2, 2)
-            codes[at:at + step] = c[..., 0] | (c[..., 1] << 4)
-            scales[at:at + step], mins[at:at + step] = s, lo.to(w.dtype)
+            to = slice(at, at + c.shape[0])
+            codes[to] = c[..., 0] | (c[..., 1] << 4)
+            scales[to], mins[to] = s, lo.to(w.dtype)
         return codes, scales, mins
+
+    @staticmethod
+    def _stretches(w: torch.Tensor, group_size: int):
+        """(first row, groups in fp32, their minima in fp32, their scales in w's
+        dtype) of some rows at a time."""
+        k = w.shape[1]
+        step = max(1, (1 << 25) // k)
+        for at in range(0, w.shape[0], step):
+            g = w[at:at + step].float().view(-1, k // group_size, group_size)
+            lo, hi = g.amin(-1), g.amax(-1)
+            if not bool((lo.isfinite() & hi.isfinite()).all()):
+                raise ValueError("LlamaPureComputeError: a weight with non-finite values has no 4-bit form.")
+            s = ((hi - lo) / 15).to(w.dtype)
+            if not bool(s.isfinite().all()):
+                raise ValueError("LlamaPureComputeError: a group's range overflows the scale's dtype.")
+            yield at, g, lo, s
 
     def _pack(self, codes, scales, mins, layout, group_size) -> None:
         rows = codes.shape[0]

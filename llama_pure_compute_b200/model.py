@@ -181,8 +181,11 @@ class LlamaAttention(nn.Module):
     @torch.no_grad()
     def quantize_weights_int4(self, group_size: int) -> None:
         from .int4_linear import Int4Weight
-        self.int4_qkv = Int4Weight(self.qkv_weight(), group_size=group_size)
+        if self.int4_qkv is not None:
+            return
+        qkv = Int4Weight(self.qkv_weight(), group_size=group_size)
         self.int4_o = Int4Weight(self.o_proj.weight, group_size=group_size)
+        self.int4_qkv = qkv
         self._qkv = self._qkv_key = self._packed_qkv = self._packed_o = None
         _drop(self.q_proj, self.k_proj, self.v_proj, self.o_proj)
 
@@ -335,9 +338,10 @@ class LlamaDecodeLayer(nn.Module):
     def quantize_weights_int4(self, group_size: int) -> None:
         from .int4_linear import Int4Weight
         self.self_attn.quantize_weights_int4(group_size)
-        self.int4_gate_up = Int4Weight(self.gate_proj.weight, self.up_proj.weight, layout="swiglu",
-                                       group_size=group_size)
+        gate_up = Int4Weight(self.gate_proj.weight, self.up_proj.weight, layout="swiglu",
+                             group_size=group_size)
         self.int4_down = Int4Weight(self.down_proj.weight, group_size=group_size)
+        self.int4_gate_up = gate_up
         self._packed_gate_up = self._packed_down = self._folded = None
         _drop(self.gate_proj, self.up_proj, self.down_proj)
 
@@ -548,18 +552,30 @@ class LlamaForCausalLM(nn.Module):
         frees its 16-bit weight: the module's state dict then lacks them, and a
         CUDA graph captured before must be captured again.  ``group_size``: 32, 64
         or 128 columns; it and 64 must divide every projection's width.  Takes
-        the layers one by one, so that it needs little memory on top."""
-        if self.int4_lm_head is not None or self.model.layers[0].int4_down is not None:
+        the layers one by one, so that it needs little memory on top.  Refuses
+        before it has changed anything; where memory runs out on the way, another
+        call goes on with what is left."""
+        from .int4_linear import Int4Weight
+        todo = [layer for layer in self.model.layers if layer.int4_down is None]
+        lm_head = lm_head and self.int4_lm_head is None
+        if not todo and not lm_head:
             raise RuntimeError("the weights are in 4 bits already")
         widths = {self.config.dim, self.config.inter_dim,
                   self.config.num_heads * self.config.head_dim}
         if group_size not in (32, 64, 128) or any(w % max(64, group_size) for w in widths):
             raise ValueError(f"group_size {group_size} (32, 64 or 128) and 64 must divide the "
                              f"projections' widths {sorted(widths)}")
-        for layer in self.model.layers:
+        linears = [self.lm_head] if lm_head else []
+        for layer in todo:
+            attn = layer.self_attn
+            linears += [layer.gate_proj, layer.up_proj, layer.down_proj]
+            if attn.int4_qkv is None:
+                linears += [attn.q_proj, attn.k_proj, attn.v_proj, attn.o_proj]
+        for lin in linears:
+            Int4Weight.check(lin.weight, group_size)
+        for layer in todo:
             layer.quantize_weights_int4(group_size)
         if lm_head:
-            from .int4_linear import Int4Weight
             self.int4_lm_head = Int4Weight(self.lm_head.weight, group_size=group_size)
             _drop(self.lm_head)
 
