@@ -124,6 +124,14 @@ class LlamaGenerator:
         if kv_cache is not None:
             if kv_cache.max_seq_len < config.max_seq_len:
                 raise ValueError("kv_cache is shorter than the configuration's max_seq_len")
+            for what, has, needs in (("layers", kv_cache.num_layers, config.num_layers),
+                                     ("KV heads", kv_cache.n_kv_heads, config.num_kv_heads),
+                                     ("head_dim", kv_cache.head_dim, config.head_dim),
+                                     ("dtype", kv_cache.dtype, p.dtype)):
+                if has != needs:
+                    raise ValueError(f"kv_cache has {what} {has}, the model {needs}")
+            if kv_cache.seq_lens.device != p.device:
+                raise ValueError(f"kv_cache is on {kv_cache.seq_lens.device}, the model on {p.device}")
             self.kv_cache = kv_cache
             return
         self.kv_cache = KVCacheManager(num_layers=config.num_layers, max_batch_size=1,
