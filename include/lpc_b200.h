@@ -377,7 +377,8 @@ typedef struct lpc_kv4 {
   void* value_scales;
   const int64_t* seq_base; /* device, ragged only */
   const int32_t* seq_cap;  /* device, ragged only */
-  int64_t max_batch;       /* dense only */
+  int64_t max_batch;       /* sequences: of the cache (dense), or entries of seq_base and
+                              seq_cap (ragged; 0: not checked) */
   int64_t max_seq_len;
   int64_t total_rows;      /* ragged only */
   int32_t kv_heads;

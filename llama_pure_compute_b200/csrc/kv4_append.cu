@@ -438,7 +438,7 @@ extern "C" int lpc_rope_kv_append_int4(const lpc_kv4* kv, const void* qkv,
   if (rc) return rc;
   if (batch < 0 || seq < 0 || num_heads <= 0 || num_heads > 65535 || table_rows <= 0 ||
       batch > 0x7fffffffLL || seq > 0x7fffffffLL || batch * seq > 0x7fffffffLL ||
-      (!kv->seq_base && batch > kv->max_batch)) {
+      (kv->max_batch > 0 && batch > kv->max_batch)) {
     set_error("rope_kv_append_int4: invalid sizes (batch=%lld seq=%lld heads=%d max_batch=%lld)",
               (long long)batch, (long long)seq, num_heads, (long long)kv->max_batch);
     return LPC_ERR_INVALID;
@@ -477,7 +477,7 @@ extern "C" int lpc_kv_read_int4(const lpc_kv4* kv, const int64_t* positions, voi
   int rc = kv4_check(kv, "kv_read_int4");
   if (rc) return rc;
   if (batch < 0 || batch > 65535 || seq < 0 || seq > 0x7fffffffLL ||
-      (!kv->seq_base && batch > kv->max_batch)) {
+      (kv->max_batch > 0 && batch > kv->max_batch)) {
     set_error("kv_read_int4: invalid sizes (batch=%lld seq=%lld max_batch=%lld)", (long long)batch,
               (long long)seq, (long long)kv->max_batch);
     return LPC_ERR_INVALID;

@@ -924,7 +924,7 @@ extern "C" int lpc_decode_attention_int4(const lpc_kv4* kv, const void* q, const
   using namespace lpc;
   int rc = kv4_check(kv, "decode_attention_int4");
   if (rc) return rc;
-  if (!sizes_ok(kv, batch, heads) || (!kv->seq_base && batch > kv->max_batch)) {
+  if (!sizes_ok(kv, batch, heads) || (kv->max_batch > 0 && batch > kv->max_batch)) {
     set_error("decode_attention_int4: invalid sizes (batch=%lld heads=%d kv_heads=%d "
               "max_batch=%lld max_seq_len=%lld)", (long long)batch, heads, kv->kv_heads,
               (long long)kv->max_batch, (long long)kv->max_seq_len);
