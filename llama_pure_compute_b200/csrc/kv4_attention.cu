@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
       for (int n = 0; n < NH; ++n) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) v[n] = fmaxf(v[n], __shfl_xor_sync(0xffffffffu, v[n], o));
-        const float next = fmaxf(fmaxf(M[n], v[n] - RISE), -1e30f);
+        const float next = fmaxf(fmaxf(M[n], v[n] - RISE), -3.4e38f);
         const float f = fast_exp2(M[n] - next);
         M[n] = next;
         l[n] *= f;

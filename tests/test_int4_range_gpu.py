@@ -101,3 +101,18 @@ def test_constant_values(value, n):
     vs[..., 1::2] = value
     q = torch.randn(1, 4, D, device=DEV, generator=g).to(BF)
     check(q, ops.Int4KV(kc, ks, vc, vs), n)
+
+
+@pytest.mark.parametrize("n", [1, 40, 900])
+@pytest.mark.parametrize("score", [-3e29, -3e31, -2e36])
+def test_scores_far_below_zero(score, n):
+    """However low the scores are, the highest keys have all the weight: equal ones the
+    mean of their values."""
+    g = gen(5)
+    D = 64
+    kc, ks = held_rows(g, (1, 1, n), D, BF)
+    vc, vs = held_rows(g, (1, 1, n), D, BF)
+    q = torch.full((1, 2, D), 2.0 ** 50, dtype=BF, device=DEV)
+    ks[..., 0::2] = 0
+    ks[..., 1::2] = score / (2.0 ** 50 * math.sqrt(D))
+    check(q, ops.Int4KV(kc, ks, vc, vs), n)
