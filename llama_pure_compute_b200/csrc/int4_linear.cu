@@ -30,7 +30,6 @@
 // walk over the tile rows, and the weight stream runs on across them.
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 
 #include "int4.cuh"
 
@@ -49,20 +48,13 @@ unsigned int lpc_status_int4_few(bool clear) {
 namespace {
 
 using lpc::Num;
+using lpc::cp16;
+using lpc::cp8;
+using lpc::cp_commit;
+using lpc::cp_wait;
 
 constexpr int MAX_TOKENS = 64;
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                     uint32_t b1) {
@@ -840,14 +832,6 @@ __global__ void int4_unpack_kernel(const uint32_t* __restrict__ codes, const T* 
   }
 }
 
-bool use_pdl() {
-  static const bool on = [] {
-    const char* e = getenv("LPC_PDL");
-    return !(e && e[0] == '0');
-  }();
-  return on;
-}
-
 // Items of MT tile rows each.
 int few_items(const lpc_w4* w, int mt) {
   const int64_t tr = (w->n_out + 15) / 16 * (w->layout == 1 ? 2 : 1);
@@ -866,7 +850,7 @@ int launch_few(const lpc_w4* w, const void* x, void* out, const void* resid, int
   const int slots = lpc::current_device_sms() * (TC == 1 && smem <= HALF_SMEM ? 2 : 1);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+  attr[0].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)std::min(items, slots));
   cfg.blockDim = dim3(512);
@@ -907,7 +891,7 @@ int launch_mid(const lpc_w4* w, const void* x, void* out, const void* resid, int
   const int keep = items > slots && sums <= C::XS_MAX;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+  attr[0].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)std::min(items, slots), (unsigned)((tokens + NT * 8 - 1) / (NT * 8)));
   cfg.blockDim = dim3(NW * 32);

@@ -32,7 +32,6 @@
 // through distributed shared memory, in rank order.
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 
 #include "int4.cuh"
 
@@ -51,6 +50,9 @@ unsigned int lpc_status_int4(bool clear) {
 namespace {
 
 using lpc::Num;
+using lpc::cp16;
+using lpc::cp_commit;
+using lpc::cp_wait;
 
 constexpr int THREADS = 192;   // 4 converter warps, MMA issuer, x loader
 constexpr int CST = 4;         // code stages
@@ -75,16 +77,8 @@ static_assert(5 * (MIN_SMEM + 1024) > SM_SMEM && 91 * 1024 + 3 * (MIN_SMEM + 102
 
 enum { EPI_STORE = 0, EPI_RESIDUAL = 1, EPI_SWIGLU = 2 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void ld_cluster4(uint32_t addr, float (&v)[4]) {
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
@@ -463,14 +457,6 @@ __global__ void __launch_bounds__(XT)
   for (int i = threadIdx.x + KEEP * XT; i < pieces; i += XT) dst[i] = scaled(lpc::ld_dep16(src + i));
 }
 
-bool use_pdl() {
-  static const bool on = [] {
-    const char* e = getenv("LPC_PDL");
-    return !(e && e[0] == '0');
-  }();
-  return on;
-}
-
 constexpr int SPLITS = 8;  // a portable cluster
 
 // CTAs per row tile: the least time of the busiest SM, a CTA costing its 64-column
@@ -526,7 +512,7 @@ int launch(const lpc::TmaDesc& tm, Args a, int tiles, int group_shift, cudaStrea
   }
   a.splits = pick_splits(tiles, a.kb, clusters);
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+  attr[0].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = (unsigned)a.splits;
   attr[1].val.clusterDim.y = 1;
@@ -575,7 +561,7 @@ int int4_many(const lpc_w4* w, const void* x, void* out, const void* resid, int6
     xh = f + MAX_TOKENS;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+    attr[0].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)tokens);
     cfg.blockDim = dim3(XT);

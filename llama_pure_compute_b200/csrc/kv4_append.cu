@@ -19,7 +19,6 @@
 // decode tokens of 32 heads 2.1 us (16-bit 2.5).  The read-back of 2 x 16,000 rows
 // of 32 heads: 109 us, 96% of the rate, mostly its 16-bit output.
 #include <algorithm>
-#include <cstdlib>
 
 #include "kv4.cuh"
 
@@ -154,8 +153,9 @@ __device__ __forceinline__ float rot(float a, float b, float c, float d) {
   else return MINUS ? __fsub_rn(__fmul_rn(a, b), p) : __fadd_rn(__fmul_rn(a, b), p);
 }
 
-// d / 15, correctly rounded: one step on the product with the rounded inverse.
-// Checked against the division for every significand; d below 2^-100, where the
+// d / 15, correctly rounded: division by a constant as the product with its rounded
+// inverse, corrected once by the remainder d - 15 q, which an FMA gives exactly (Markstein's
+// scheme).  Checked against the division for every significand; d below 2^-100, where the
 // remainder loses bits, takes the division.
 __device__ __forceinline__ float over15(float d) {
   if (d < 0x1p-100f) return __fdiv_rn(d, 15.f);
@@ -366,20 +366,12 @@ __global__ void __launch_bounds__(THREADS) kv4_read_kernel(
   }
 }
 
-bool use_pdl() {
-  static const bool on = [] {
-    const char* e = getenv("LPC_PDL");
-    return !(e && e[0] == '0');
-  }();
-  return on;
-}
-
 struct Launch {
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = {};
   Launch(dim3 grid, int threads, cudaStream_t s) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+    attr[0].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
     cfg.stream = s;

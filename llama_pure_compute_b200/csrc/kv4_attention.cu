@@ -45,7 +45,6 @@
 // mask-free operands, splits of equal length by the rule at split_keys.
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 
 #include "kv4.cuh"
 
@@ -64,6 +63,10 @@ unsigned int lpc_status_kv4_attention(bool clear) {
 namespace {
 
 using lpc::Num;
+using lpc::cp16;
+using lpc::cp8;
+using lpc::cp_commit;
+using lpc::cp_wait;
 
 constexpr int TK = 32;        // keys per warp tile
 constexpr int NST = 3;          // stages per warp
@@ -82,12 +85,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-}
 // The same, zeros instead of the source's bytes when not `ok`.
 __device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
@@ -96,11 +93,6 @@ __device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool ok) {
 __device__ __forceinline__ void cp8z(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(ok ? 8 : 0)
                : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
@@ -748,14 +740,6 @@ __global__ void __launch_bounds__(CWARPS * 32)
   }
 }
 
-bool use_pdl() {
-  static const bool on = [] {
-    const char* e = getenv("LPC_PDL");
-    return !(e && e[0] == '0');
-  }();
-  return on;
-}
-
 // A cluster of up to 4 CTAs of 16 warps merges its splits in distributed shared
 // memory: 1000 keys of 32 KV heads 5.9 us against 6.7 with the second kernel, 8
 // sequences of 8,000 keys 19.4 against 21.3.  128 CTAs in such clusters fit 16
@@ -779,7 +763,7 @@ int launch(const lpc_kv4* kv, const void* q, const int32_t* lens, void* out, flo
   const int cluster = W == 16 && merges_in_cluster(batch * kv->kv_heads * blocks, grid_splits);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = use_pdl() ? 1 : 0;
+  attr[0].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = (unsigned)grid_splits;
   attr[1].val.clusterDim.y = 1;

@@ -16,6 +16,7 @@
 
 #include <atomic>
 #include <cstdint>
+#include <cstdlib>
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -46,6 +47,15 @@ bool aligned16(const void* p);
 // is per device context).  `mask` holds one bit per device ordinal.
 int once_per_device_smem(const void* kernel, int bytes, std::atomic<uint64_t>& mask);
 int current_device_sms();
+// Whether kernels are launched programmatically under the one before them (LPC_PDL=0:
+// not).
+inline bool use_pdl() {
+  static const bool on = [] {
+    const char* e = getenv("LPC_PDL");
+    return !(e && e[0] == '0');
+  }();
+  return on;
+}
 // The calling thread's current CUDA driver context (a CUcontext), or null when
 // the driver entry point is unavailable.
 void* current_context();
@@ -262,6 +272,19 @@ __device__ __forceinline__ int64_t ld_dep(const int64_t* p) {
   int64_t v;
   asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
   return v;
+}
+
+// Asynchronous copies of a thread's 16 or 8 bytes to shared memory.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void cluster_sync() {
