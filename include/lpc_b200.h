@@ -417,7 +417,8 @@ LPC_API int lpc_kv_read_int4(const lpc_kv4* kv, const int64_t* positions, void* 
  * lpc_decode_attention (and _ragged) over a 4-bit cache: q and out [batch,
  * heads, head_dim], keys [0, seq_lens[b]) of sequence b; an empty sequence
  * gives zeros, a length beyond the sequence's rows is cut to them and flagged.
- * Any number of query heads per KV head.  workspace: the split partials,
+ * Softmax statistics and sums in fp32; weight times V scale enters the products in
+ * fp16 (11 bits).  Any number of query heads per KV head.  workspace: the split partials,
  * lpc_decode_attention_int4_workspace_bytes() bytes (0 where one split covers
  * the cache or a cluster merges the splits: NULL then).  Calls that overlap
  * need workspaces of their own.
@@ -459,7 +460,9 @@ LPC_API int lpc_int4_unpack(const lpc_w4* w, void* out, void* stream);
 /*
  * out[t, n] = epilogue(sum_k x[t, k] * W[n, k]) for x [tokens, k], tokens <= 64:
  * epilogue 0 store, 1 resid + (resid may equal out), 2 silu(gate) * up (layout 1
- * and only it).  fp32 accumulation, one rounding.  workspace:
+ * and only it).  Sums in fp32, one rounding of the result; where the tensor-memory
+ * kernel takes a product (that of the workspace below, and its fp16 counterpart) each
+ * weight is rounded to fp16's 11 bits before.  workspace:
  * lpc_int4_linear_workspace_bytes() bytes (0 for fp16, few tokens and small weights:
  * NULL then); calls that overlap need one each.  One kernel, two where the workspace is
  * used.  A row of x with a value that is not finite gives an output row of values

@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(512, TC == 1 ? 2 : 1)
 // 128 + c, (w & 0x000F000F) | 0x43004300, exactly (a bf16 subnormal times x would
 // underflow the fp32 sum), 7 instructions a word.  The 128 is taken out again with the
 // group's sum of x, which costs the fp32 accumulator about 5 of its 24 bits and
-// leaves an error some hundred times below the output's rounding.  The sum of x is
+// leaves an error some hundred times below the output's rounding, and x up to 2^113.  The sum of x is
 // one more product, of a row of ones, kept in shared memory for the next items.
 // 4096 x 4096 at 8 / 16 tokens: 4.2 / 5.6 us (stream 1.4); the loads of x, one of each 8
 // columns and token for every tile row, bound it.
@@ -916,7 +916,7 @@ enum Kernel { FEW, MID, MANY };
 // few do: MID where blocks^2 times values are at most MID_MOST.  Measured, us, mid /
 // many: 14,336 x 4096 at 16 tokens 18.5 / 19.4, 22,016 x 4096 25.0 / 21.2; at 32 tokens
 // 4096 x 4096 10.2 / 11.3, 6144 x 4096 14.6 / 12.8; at 64 4096 x 1024 11.0 / 10.7,
-// 2048 x 4096 15.4 / 11.3.
+// 2048 x 4096 15.4 / 11.3 (MANY before its weights' subtraction, 2 to 6% less than now).
 constexpr int64_t MID_MOST = 72 << 20;
 // x fits the few-token kernel's shared memory, with one tile row an item or two
 // (the rings round differently).

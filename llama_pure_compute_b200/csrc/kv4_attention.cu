@@ -38,8 +38,8 @@
 // the workspace and a second kernel, or not at all where one split covers the cache.
 //
 // Measured, D = 128, bf16 (us; of the cache's bytes at 6397 GB/s): 64 sequences of
-// 1000 keys, 32 heads, 47 (99%); 32 of 1 to 4096 keys 57.1 (87%: the short ones leave
-// SMs idle at the end); 3 of 60,000 keys, 64 heads on 8, 40.4 (80%: 500 instructions
+// 1000 keys, 32 heads, 47 (99%); 32 of 1 to 4096 keys 57.7 (86%: the short ones leave
+// SMs idle at the end); 3 of 60,000 keys, 64 heads on 8, 40.9 (79%: 500 instructions
 // a warp's tile of 32 keys, 60% of the issue slots); one of 1000 keys 5.5.  What took
 // 32 sequences of 4096 there from 83: ldmatrix and movmatrix in place of shuffles, the
 // mask-free operands, splits of equal length by the rule at split_keys.

@@ -12,7 +12,8 @@ reads 3.5 times fewer cache bytes.
     same keys and values whether it comes in one piece or several.
 
 The q/k/v projection with the append in its epilogue (``qkv_rope_append``)
-writes 16-bit rows, so these caches turn it off for their steps.
+writes 16-bit rows, so these caches turn it off for their steps: on 16-bit weights a
+step of one short sequence takes 2% longer than with a 16-bit cache.
 """
 from __future__ import annotations
 

@@ -549,8 +549,12 @@ class LlamaForCausalLM(nn.Module):
     def quantize_weights_int4(self, group_size: int = 128, lm_head: bool = True) -> None:
         """Holds every projection (and with ``lm_head`` the vocabulary
         projection) in 4 bits with group scales (``int4_linear.Int4Weight``) and
-        frees its 16-bit weight: the module's state dict then lacks them, and a
-        CUDA graph captured before must be captured again.  ``group_size``: 32, 64
+        frees its 16-bit weight: the module's state dict then holds empty tensors
+        in their place (save it before), ``.to()`` and ``copy.deepcopy`` do not take
+        the 4-bit weights along, and a CUDA graph captured before must be captured
+        again.  Steps of more than 64 tokens write a 16-bit copy of each weight for
+        the library's GEMM every time and are slower than on 16-bit weights: for
+        decoding up to 64 sequences.  ``group_size``: 32, 64
         or 128 columns; it and 64 must divide every projection's width.  Takes
         the layers one by one, so that it needs little memory on top.  Refuses
         before it has changed anything; where memory runs out on the way, another

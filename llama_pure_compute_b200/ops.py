@@ -869,8 +869,12 @@ def decode_attention_int4(
     one query per sequence, q [B, H, D] (or [B, H, 1, D]), keys
     ``[0, seq_lens[b])`` of sequence b (int32, device).  Any number of query
     heads per KV head.  An empty sequence gives zeros; a length beyond the
-    sequence's rows is cut to them and sets the device status.  fp32 softmax
-    and accumulation; returns q's shape."""
+    sequence's rows is cut to them and sets the device status.  Softmax
+    statistics and sums in fp32; a key's weight times its V scale enters the
+    products in fp16 (11 bits).  Returns q's shape.
+
+    Sequences are cut by the cache's capacity: one that fills little of a large
+    cache runs on few SMs."""
     index = kv.index
     if q.get_device() != index or seq_lens.get_device() != index:
         _require_cuda(q, "q")
