@@ -114,6 +114,8 @@ class Int4KVCache:
         dtype, ``[B, Hkv, S, D]`` each."""
         if not 0 <= layer_idx < self.num_layers:
             raise IndexError("invalid layer index")
+        if batch_size < 0 or seq_len < 0:
+            raise ValueError("batch_size and seq_len must not be negative")
         if batch_size > self.max_batch_size:
             raise ValueError("batch size exceeds cache capacity")
         if seq_len > self.max_seq_len:

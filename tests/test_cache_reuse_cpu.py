@@ -1,4 +1,4 @@
-"""Ragged caches and decode workspaces that are used again, host side: the caches'
+"""Caches, host side: selections and decode workspaces that are used again, arguments; the
 bookkeeping on CPU tensors (no kernel runs)."""
 import ctypes
 import types
@@ -87,3 +87,12 @@ def test_a_captured_workspace_outlives_other_batch_sizes(monkeypatch, kind):
     kv.decode_workspace(3, 4)
     assert eager() is None  # no more than the last one is kept for eager steps
     assert graph() is not None and kv.decode_workspace(4, 4) is graph()
+
+
+def test_int4_cache_read_of_negative_sizes():
+    """-1 is no batch: expand() would take it for one row."""
+    kv = Int4KVCache.__new__(Int4KVCache)
+    kv.num_layers, kv.max_batch_size, kv.max_seq_len, kv.device = 1, 4, 10, torch.device("cpu")
+    for batch, seq in ((-1, 3), (2, -3)):
+        with pytest.raises(ValueError, match="negative"):
+            kv.read(layer_idx=0, batch_size=batch, seq_len=seq)
