@@ -21,7 +21,7 @@
 // groups instead of 8 heads: a lane has one head's scores, half the exponentials,
 // and the lower nibbles need no mask, since whole bytes times q0 less the upper
 // nibbles times q0 are the lower nibbles times q0.  With 5 to 8 (NH = 2) a lane has
-// two heads; more take several CTAs.
+// two heads; more take several CTAs.  Long caches take V's sums more finely (sums_finely).
 // q enters as fp16 scaled per head by a power of two so that its largest value
 // is about 2^14: a bf16 or fp16 q (below 2^114) then loses nothing but what lies
 // 2^-38 below that value.  P s_g enters as fp16 (rounded to 2^-11, finer than the
@@ -194,7 +194,7 @@ struct Layout {
   static constexpr int SMEM = W * NST * STAGE > (W + 1) * RED ? W * NST * STAGE : (W + 1) * RED;
 };
 
-template <typename T, int D, int NH, int W>
+template <typename T, int D, int NH, int W, bool FINE>
 __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
     kv4_split_kernel(const T* __restrict__ q, const uint8_t* __restrict__ kcodes,
                      const uint8_t* __restrict__ kscales, const uint8_t* __restrict__ vcodes,
@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
   constexpr int CB = L::CB;
   constexpr int KW = D / 32;              // K words of a lane and key
   constexpr int VM = D / 32;              // V products per group: 16 dims each
+  constexpr int NI = VM == 1 ? 1 : 2;     // of them from one ldmatrix
   extern __shared__ __align__(16) uint8_t smem[];
 
   lpc::pdl_trigger();
@@ -499,9 +500,9 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
       }
     }
     // weights, then the output products
+    uint32_t pb[2][2][2];  // [u][group][keys 0-7 / 8-15]
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      uint32_t pb[2][2];  // [group][keys 0-7 / 8-15]
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint2 w = *reinterpret_cast<const uint2*>(svs + (16 * u + r + 8 * i) * 8);
@@ -526,40 +527,78 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
             a1s[n] = fmaf(8.f, e1 - __half2float(__float2half_rn(e1)), a1s[n]);
           }
         }
-        if constexpr (NH == 1) {
-          // columns 2t and 2t + 1 carry head t's groups: the bytes times (P s0 | 0) and
-          // their upper nibbles times (-P s0 | P s1) leave the lower nibbles in one
-          pb[1][i] = transpose8(pack_half2(-p[0] * s0, p[0] * s1));
-          pb[0][i] = (pb[1][i] ^ 0x80008000u) & even;
+        if constexpr (NH == 1 && FINE) {
+          // columns 2t and 2t + 1 carry head t's groups: the lower nibbles times (P s0 | 0)
+          // and the upper ones times (0 | P s1)
+          const uint32_t both = transpose8(pack_half2(p[0] * s0, p[0] * s1));
+          pb[u][0][i] = both & even;
+          pb[u][1][i] = both & ~even;
+        } else if constexpr (NH == 1) {
+          // the same, the bytes times (P s0 | 0) and their upper nibbles times
+          // (-P s0 | P s1), which leave the lower nibbles in one
+          pb[u][1][i] = transpose8(pack_half2(-p[0] * s0, p[0] * s1));
+          pb[u][0][i] = (pb[u][1][i] ^ 0x80008000u) & even;
         } else {
-          pb[0][i] = transpose8(pack_half2(p[0] * s0, p[1] * s0));
-          pb[1][i] = transpose8(pack_half2(p[0] * s1, p[1] * s1));
+          pb[u][0][i] = transpose8(pack_half2(p[0] * s0, p[1] * s0));
+          pb[u][1][i] = transpose8(pack_half2(p[0] * s1, p[1] * s1));
         }
       }
       // codes of keys 16u .. 16u + 15, 16 dims (8 units) of each group at a time
+      if constexpr (!FINE)
 #pragma unroll
-      for (int j = 0; j < VM; j += 2) {
-        uint32_t v[4];
-        const uint32_t src = sv + 16 * u * CB + (j == 0 ? vsrc : vsrc ^ 32u);
-        if constexpr (VM == 1) ldm2(v, src);
-        else ldm4(v, src);
+        for (int j = 0; j < VM; j += NI) {
+          uint32_t v[4];
+          const uint32_t src = sv + 16 * u * CB + (j == 0 ? vsrc : vsrc ^ 32u);
+          if constexpr (VM == 1) ldm2(v, src);
+          else ldm4(v, src);
 #pragma unroll
-        for (int i = 0; i < (VM == 1 ? 1 : 2); ++i) {
-          const uint32_t lo = v[2 * i], hi = v[2 * i + 1];
-          if constexpr (NH == 1) {
-            const uint32_t l0 = lo & BYTES, h0 = hi & BYTES;
-            const uint32_t l1 = __byte_perm(lo, 0u, 0x4341), h1 = __byte_perm(hi, 0u, 0x4341);
-            mma_f16(acc[0][j + i], l0, l1, h0, h1, pb[0][0], pb[0][1]);
-            mma_f16(acc[0][j + i], l0 & HIGH, l1 & HIGH, h0 & HIGH, h1 & HIGH, pb[1][0], pb[1][1]);
-          } else {
-            const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
-            mma_f16(acc[0][j + i], lo & LOW, lo8 & LOW, hi & LOW, hi8 & LOW, pb[0][0], pb[0][1]);
-            mma_f16(acc[AG - 1][j + i], lo & HIGH, lo8 & HIGH, hi & HIGH, hi8 & HIGH, pb[1][0],
-                    pb[1][1]);
+          for (int i = 0; i < NI; ++i) {
+            const uint32_t lo = v[2 * i], hi = v[2 * i + 1];
+            if constexpr (NH == 1) {
+              const uint32_t l0 = lo & BYTES, h0 = hi & BYTES;
+              const uint32_t l1 = __byte_perm(lo, 0u, 0x4341), h1 = __byte_perm(hi, 0u, 0x4341);
+              mma_f16(acc[0][j + i], l0, l1, h0, h1, pb[u][0][0], pb[u][0][1]);
+              mma_f16(acc[0][j + i], l0 & HIGH, l1 & HIGH, h0 & HIGH, h1 & HIGH, pb[u][1][0], pb[u][1][1]);
+            } else {
+              const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+              mma_f16(acc[0][j + i], lo & LOW, lo8 & LOW, hi & LOW, hi8 & LOW, pb[u][0][0], pb[u][0][1]);
+              mma_f16(acc[AG - 1][j + i], lo & HIGH, lo8 & HIGH, hi & HIGH, hi8 & HIGH, pb[u][1][0],
+                      pb[u][1][1]);
+            }
           }
         }
-      }
     }
+    if constexpr (FINE)
+#pragma unroll
+      for (int j = 0; j < VM; j += NI) {
+        float part[AG][NI][4];  // of this tile
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t v[4];
+          const uint32_t src = sv + 16 * u * CB + (j == 0 ? vsrc : vsrc ^ 32u);
+          if constexpr (VM == 1) ldm2(v, src);
+          else ldm4(v, src);
+#pragma unroll
+          for (int i = 0; i < NI; ++i) {
+            const uint32_t lo = v[2 * i], hi = v[2 * i + 1];
+            const uint32_t l0 = (lo << 4) & HIGH, l1 = (lo >> 4) & HIGH, h0 = (hi << 4) & HIGH,
+                           h1 = (hi >> 4) & HIGH;
+            if (u == 0) mma_f16_first(part[0][i], l0, l1, h0, h1, pb[0][0][0], pb[0][0][1]);
+            else mma_f16(part[0][i], l0, l1, h0, h1, pb[1][0][0], pb[1][0][1]);
+            const uint32_t l8 = (lo >> 8) & HIGH, h8 = (hi >> 8) & HIGH;
+            if (u == 0 && AG == 2)
+              mma_f16_first(part[1 % AG][i], lo & HIGH, l8, hi & HIGH, h8, pb[0][1][0], pb[0][1][1]);
+            else
+              mma_f16(part[AG - 1][i], lo & HIGH, l8, hi & HIGH, h8, pb[u][1][0], pb[u][1][1]);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < AG; ++g)
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) acc[g][j + i][n] += part[g][i][n];
+      }
   }
   cp_wait<0>();
   // a head's sums over the 8 lanes that hold its keys
@@ -584,8 +623,9 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 4 : 1)
       const int d = 2 * (8 * i + r);
       constexpr int g1 = AG - 1;
       const int n1 = NH == 1 ? 1 : n;
-      p[d] = fmaf(acc[0][i][n], 16777216.f, a0s[n]);
-      p[d + 1] = fmaf(acc[0][i][2 + n], 16777216.f, a0s[n]);
+      constexpr float ONE = FINE ? 1048576.f : 16777216.f;
+      p[d] = fmaf(acc[0][i][n], ONE, a0s[n]);
+      p[d + 1] = fmaf(acc[0][i][2 + n], ONE, a0s[n]);
       p[d + D / 2] = fmaf(acc[g1][i][n1], 1048576.f, a1s[n]);
       p[d + D / 2 + 1] = fmaf(acc[g1][i][2 + n1], 1048576.f, a1s[n]);
     }
@@ -749,12 +789,12 @@ bool merges_in_cluster(int64_t pairs, int64_t splits) {
   return splits > 1 && splits <= CLUSTER && pairs * splits <= 128;
 }
 
-template <typename T, int D, int NH, int W>
+template <typename T, int D, int NH, int W, bool FINE>
 int launch(const lpc_kv4* kv, const void* q, const int32_t* lens, void* out, float* po, float* pml,
            int64_t batch, int heads, int max_splits, int chunk, float scale_log2, cudaStream_t s) {
   using L = Layout<D, W>;
   static std::atomic<uint64_t> mask{0};
-  int rc = lpc::once_per_device_smem((const void*)kv4_split_kernel<T, D, NH, W>, L::SMEM, mask);
+  int rc = lpc::once_per_device_smem((const void*)kv4_split_kernel<T, D, NH, W, FINE>, L::SMEM, mask);
   if (rc) return rc;
   const int G = heads / kv->kv_heads;
   const int blocks = (G + HB - 1) / HB;
@@ -775,7 +815,7 @@ int launch(const lpc_kv4* kv, const void* q, const int32_t* lens, void* out, flo
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = cluster ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, kv4_split_kernel<T, D, NH, W>, (const T*)q,
+  if (cudaLaunchKernelEx(&cfg, kv4_split_kernel<T, D, NH, W, FINE>, (const T*)q,
                          (const uint8_t*)kv->key_codes, (const uint8_t*)kv->key_scales,
                          (const uint8_t*)kv->value_codes, (const uint8_t*)kv->value_scales, lens,
                          (T*)out, po, pml, heads, G, blocks, max_splits, chunk, cluster, scale_log2,
@@ -791,6 +831,38 @@ int launch(const lpc_kv4* kv, const void* q, const int32_t* lens, void* out, flo
                          (T*)out, heads, max_splits, chunk, rows) != cudaSuccess)
     return lpc::check_launch("decode_attention_int4 (combine)");
   return lpc::check_launch("decode_attention_int4 (combine)");
+}
+
+// Whether V's sums are taken finely (FINE of the split kernel).  The tensor core does not
+// normalise subnormal operands and cuts what it adds: a code in the lowest four bits of its
+// half keeps 10 bits less of its product than fp32, and the accumulator cuts again as it
+// grows, always towards zero.  The sums come out 3 to 6e-6 of their codes' part too
+// small, which an output, the difference of the codes' and the minima's parts, shows once
+// many keys average to little.  FINE: codes in bits 4 to 7, and sums that start at zero
+// with each tile of 32 keys and are added in fp32.  Relative error plain / FINE (fp32 with
+// outputs rounded once): fp16 of 4096 keys 2.6 / 2.5e-4 (2.0e-4), 32,768 3.4 / 2.8,
+// 131,072 5.1 / 2.6; bf16 of 131,072 1.84 / 1.83e-3 (1.73), 4,000,000 3.4 / 1.8.  It costs
+// 8%: fp16, 32 sequences of 1 to 4096 keys 59.7 / 64.6 us, 3 of 60,000 42.1 / 45.4.
+bool sums_finely(const lpc_kv4* kv) {
+  return kv->max_seq_len > (kv->dtype == LPC_DTYPE_F16 ? 1 << 13 : 1 << 18);
+}
+
+template <typename T, int D>
+int launch_nw(const lpc_kv4* kv, const void* q, const int32_t* lens, void* out, float* po,
+              float* pml, int64_t batch, int heads, int max_splits, int chunk, float scale_log2,
+              bool wide, cudaStream_t s) {
+#define LPC_KV4_NW(NH, W)                                                                         \
+  return sums_finely(kv) ? launch<T, D, NH, W, true>(kv, q, lens, out, po, pml, batch, heads,     \
+                                                     max_splits, chunk, scale_log2, s)            \
+                         : launch<T, D, NH, W, false>(kv, q, lens, out, po, pml, batch, heads,    \
+                                                      max_splits, chunk, scale_log2, s)
+  if (heads / kv->kv_heads <= 4) {
+    if (wide) LPC_KV4_NW(1, 16);
+    LPC_KV4_NW(1, 4);
+  }
+  if (wide) LPC_KV4_NW(2, 16);
+  LPC_KV4_NW(2, 4);
+#undef LPC_KV4_NW
 }
 
 constexpr int64_t MAX_BATCH = 65535;
@@ -936,16 +1008,8 @@ extern "C" int lpc_decode_attention_int4(const lpc_kv4* kv, const void* q, const
   float* pml = po ? po + batch * heads * splits * kv->head_dim : nullptr;
   const float sl2 = sm_scale * LOG2E;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool one = heads / kv->kv_heads <= 4;
-#define LPC_KV4(T, DD)                                                                            \
-  return one ? wide ? launch<T, DD, 1, 16>(kv, q, seq_lens, out, po, pml, batch, heads,           \
-                                           (int)splits, chunk, sl2, s)                            \
-                    : launch<T, DD, 1, 4>(kv, q, seq_lens, out, po, pml, batch, heads,            \
-                                          (int)splits, chunk, sl2, s)                             \
-         : wide ? launch<T, DD, 2, 16>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits,  \
-                                       chunk, sl2, s)                                             \
-                : launch<T, DD, 2, 4>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits,   \
-                                      chunk, sl2, s)
+#define LPC_KV4(T, DD) \
+  return launch_nw<T, DD>(kv, q, seq_lens, out, po, pml, batch, heads, (int)splits, chunk, sl2, wide, s)
   if (kv->dtype == LPC_DTYPE_BF16) {
     if (kv->head_dim == 128) LPC_KV4(__nv_bfloat16, 128);
     if (kv->head_dim == 64) LPC_KV4(__nv_bfloat16, 64);

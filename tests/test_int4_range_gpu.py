@@ -116,3 +116,32 @@ def test_scores_far_below_zero(score, n):
     ks[..., 0::2] = 0
     ks[..., 1::2] = score / (2.0 ** 50 * math.sqrt(D))
     check(q, ops.Int4KV(kc, ks, vc, vs), n)
+
+
+@pytest.mark.parametrize("dtype,n,Hkv,G,D", [(HF, 131072, 4, 2, 128), (HF, 60000, 2, 8, 64), (HF, 9000, 8, 1, 128),
+                                             (BF, 3000000, 1, 2, 64), (BF, 600000, 1, 8, 32)])
+def test_sums_over_long_sequences(dtype, n, Hkv, G, D):
+    """Many keys average to little: errors of the sums that all lean one way would show.
+    In the mean square, over all heads and dims: a rounding to e bits is off by
+    2^-e / sqrt(3) of the value at the lower end of a binade, 0.736 of that over
+    significands of equal weight in the logarithm (E 1/m^2 = 0.75 / (2 ln 2)); the output
+    has one, and P s (11 bits) one that counts times c (bf16) or c - 8 (fp16, whose
+    products take 8 of them out again).  A tenth more for the number of outputs."""
+    g = gen(6)
+    kc, ks = held_rows(g, (1, Hkv, n), D, dtype)
+    vc, vs = held_rows(g, (1, Hkv, n), D, dtype)
+    q = torch.randn(1, Hkv * G, D, device=DEV, generator=g).to(dtype)
+    out = ops.decode_attention_int4(q, ops.Int4KV(kc, ks, vc, vs),
+                                    torch.tensor([n], dtype=torch.int32, device=DEV)).double()
+    half = torch.finfo(dtype).eps / 2 / math.sqrt(3)
+    off, bar = 0.0, 0.0
+    for h in range(Hkv):
+        p = torch.softmax(q[0, h * G:(h + 1) * G].double() @ rows_ref(kc[0, h], ks[0, h]).T / math.sqrt(D), -1)
+        v = rows_ref(vc[0, h], vs[0, h])
+        want = p @ v
+        taken = vs[0, h].clone()  # s (c - 8), or s c
+        taken[:, 1::2] = -8 * taken[:, 0::2] if dtype == HF else 0
+        rounded = p.square() @ rows_ref(vc[0, h], taken).square()
+        off += (out[0, h * G:(h + 1) * G] - want).square().sum().item()
+        bar += (want.square() * half ** 2 + rounded * (2.0 ** -11 / math.sqrt(3)) ** 2).sum().item()
+    assert off <= (1.1 * 0.736) ** 2 * bar, math.sqrt(off / bar)
