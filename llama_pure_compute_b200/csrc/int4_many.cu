@@ -26,8 +26,9 @@
 // A weight is rounded to fp16: off by at most 2^-11 of itself, or 2^-39 of its row's
 // largest |m| + 15 |s| where that is more.  The roundings are independent.  Measured,
 // normal x and w, k = 4096, relative: with bf16 numbers 2.2e-5, which the outputs (1.7e-3)
-// do not show; with fp16 numbers 2.0e-4, beside the outputs' own 2.1e-4 2.9e-4 in all.  e
-// is a power per weight row (int4.cuh), undone with x's in the epilogue.
+// do not show; with fp16 numbers 2.0e-4, beside the outputs' own 2.1e-4 2.9e-4 in all
+// (SwiGLU, two products, 3.5e-4), as a 16-bit copy of the weight would give.  e is a power
+// per weight row (int4.cuh), undone with x's in the epilogue.
 // Few row tiles: clusters of up to 8 CTAs split the columns and add their sums
 // through distributed shared memory, in rank order.
 #include <algorithm>
