@@ -222,7 +222,7 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
         xp = x.data_ptr()
     rp = None
     if epi == 1:
-        if resid is None or resid.numel() != tokens * n or resid.shape[-1:] != (n,) \
+        if resid is None or resid.numel() != tokens * n or not resid.dim() or resid.shape[-1] != n \
                 or not resid.is_contiguous() or resid.dtype != x.dtype or resid.get_device() != index:
             raise ValueError("LlamaPureComputeError: residual must be a contiguous [..., n_out] tensor.")
         rp = resid.data_ptr()
@@ -230,7 +230,7 @@ def int4_linear(x: torch.Tensor, w: Int4Weight, epilogue: str = "store",
         raise ValueError("LlamaPureComputeError: resid is for the residual epilogue.")
     if out is None:
         out = x.new_empty(tokens, n) if len(shape) == 2 else x.new_empty(*shape[:-1], n)
-    elif out.numel() != tokens * n or out.shape[-1:] != (n,) or not out.is_contiguous() \
+    elif out.numel() != tokens * n or not out.dim() or out.shape[-1] != n or not out.is_contiguous() \
             or out.dtype != x.dtype or out.get_device() != index:
         raise ValueError("LlamaPureComputeError: out must be a contiguous [..., n_out] tensor.")
     elif _overlap(out, x):
