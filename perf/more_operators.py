@@ -38,15 +38,15 @@ def listed():
     return [
         # -- sampling --------------------------------------------------------
         # one chat, vocabulary of the 7B shape, the generator's own top-k and top-p: latency
-        {"name": "sample 1 x 32000, top-k 50, top-p 0.9", "op": "sample", "rows": 1, "vocab": 32000,
+        {"name": "sample 1 x 32000 top-k 50 top-p 0.9", "op": "sample", "rows": 1, "vocab": 32000,
          "temperature": 0.8, "top_k": 50, "top_p": 0.9, "min_p": 0.0, "per_row": False,
          "type": "bf16"},
         # a small odd vocabulary, every row with its own settings, greedy rows among them
-        {"name": "sample 37 x 1003, fp32", "op": "sample", "rows": 37, "vocab": 1003,
+        {"name": "sample 37 x 1003 fp32", "op": "sample", "rows": 37, "vocab": 1003,
          "temperature": 0.9, "top_k": 40, "top_p": 0.8, "min_p": 0.05, "per_row": True,
          "type": "fp32"},
         # the nodes of 32 trees of 16, by nucleus, without top-k
-        {"name": "sample 512 x 32000, top-p 0.95", "op": "sample", "rows": 512, "vocab": 32000,
+        {"name": "sample 512 x 32000 top-p 0.95", "op": "sample", "rows": 512, "vocab": 32000,
          "temperature": 0.7, "top_k": 0, "top_p": 0.95, "min_p": 0.0, "per_row": False,
          "type": "bf16"},
         # the largest: 256 sequences, the 128,256-row vocabulary, temperature alone
@@ -55,19 +55,19 @@ def listed():
          "type": "bf16"},
         # -- attention of drafted trees --------------------------------------
         # one chat of about a thousand tokens, 7B heads, a tree of 16: latency
-        {"name": "tree of 16, 1 sequence, 1000 keys", "op": "attend", "batch": 1, "nodes": 16,
+        {"name": "tree of 16 1 sequence 1000 keys", "op": "attend", "batch": 1, "nodes": 16,
          "heads": 32, "kv_heads": 32, "dim": 128, "cap": 1064, "shortest": 1000, "longest": 1000,
          "layout": "dense", "type": "bf16"},
         # a serving batch of mixed lengths, 32 heads on 8
-        {"name": "tree of 24, 32 sequences up to 4096, 32:8", "op": "attend", "batch": 32,
+        {"name": "tree of 24 32 sequences up to 4096 32:8", "op": "attend", "batch": 32,
          "nodes": 24, "heads": 32, "kv_heads": 8, "dim": 128, "cap": 4120, "shortest": 1,
          "longest": 4096, "layout": "dense", "type": "bf16"},
         # few long documents, 64 heads on 8 as in 70B, the widest tree: 512 rows a KV head
-        {"name": "tree of 64, 3 sequences of 60000, 64:8", "op": "attend", "batch": 3, "nodes": 64,
+        {"name": "tree of 64 3 sequences of 60000 64:8", "op": "attend", "batch": 3, "nodes": 64,
          "heads": 64, "kv_heads": 8, "dim": 128, "cap": 60081, "shortest": 59000, "longest": 60017,
          "layout": "dense", "type": "bf16"},
         # packed cache of odd capacities, small heads, an empty sequence among them
-        {"name": "tree of 13, ragged, 17 sequences, D=64", "op": "attend", "batch": 17, "nodes": 13,
+        {"name": "tree of 13 ragged 17 sequences D=64", "op": "attend", "batch": 17, "nodes": 13,
          "heads": 12, "kv_heads": 6, "dim": 64, "cap": 1514, "shortest": 0, "longest": 1501,
          "layout": "ragged", "type": "fp16"},
         # -- append of drafted trees -----------------------------------------
@@ -75,14 +75,14 @@ def listed():
         {"name": "append a tree of 16", "op": "append", "batch": 1, "nodes": 16, "heads": 32,
          "kv_heads": 32, "dim": 128, "cap": 1064, "layout": "dense", "type": "bf16"},
         # 64 wide trees, 32 heads on 8, packed cache
-        {"name": "append 64 trees of 64, ragged", "op": "append", "batch": 64, "nodes": 64,
+        {"name": "append 64 trees of 64 ragged", "op": "append", "batch": 64, "nodes": 64,
          "heads": 32, "kv_heads": 8, "dim": 128, "cap": 400, "layout": "ragged", "type": "bf16"},
         # -- acceptance ------------------------------------------------------
         # one tree, the 32 layers of the 7B shape: latency
-        {"name": "accept 1 of 16, 32 layers", "op": "accept", "batch": 1, "nodes": 16, "layers": 32,
+        {"name": "accept 1 of 16 32 layers", "op": "accept", "batch": 1, "nodes": 16, "layers": 32,
          "kv_heads": 32, "dim": 128, "cap": 300, "layout": "dense", "type": "bf16"},
         # 64 wide trees with long agreed branches, 32 layers of 8 KV heads, packed cache
-        {"name": "accept 64 of 64, 32 layers, ragged", "op": "accept", "batch": 64, "nodes": 64,
+        {"name": "accept 64 of 64 32 layers ragged", "op": "accept", "batch": 64, "nodes": 64,
          "layers": 32, "kv_heads": 8, "dim": 128, "cap": 200, "layout": "ragged", "type": "bf16"},
     ]
 
@@ -264,7 +264,9 @@ def prepare(case, seed):
         st["sampled"] = torch.where(agreed, st["drafted"].gather(1, child),
                                     torch.randint(50, 32000, (batch, nodes), device=DEV,
                                                   generator=gen))
-        st["k_layers"], st["v_layers"] = list(st["k"].unbind(0)), list(st["v"].unbind(0))
+        if own:
+            from llama_pure_compute_b200 import ops
+            st["kv"] = ops.LayerCaches(st["k"].unbind(0), st["v"].unbind(0), st["base"], st["caps"])
     return {"case": case, **st}
 
 
@@ -291,8 +293,7 @@ def _own(st):
                                     seq_base=st["base"], seq_cap=st["caps"])
         return {"q": q, "k": st["k"], "v": st["v"]}
     accepted, tokens, path = ops.tree_accept(st["drafted"], st["parents"], st["sampled"], st["lens"],
-                                             st["k_layers"], st["v_layers"], seq_base=st["base"],
-                                             seq_cap=st["caps"])
+                                             st["kv"])
     return {"accepted": accepted, "tokens": tokens, "path": path, "k": st["k"], "v": st["v"]}
 
 
