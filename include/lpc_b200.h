@@ -474,6 +474,73 @@ LPC_API int lpc_int4_linear(const lpc_w4* w, const void* x, void* out, const voi
                             void* stream);
 
 /*
+ * A step of speculative decoding over a drafted tree.  No counterpart in the reference,
+ * which decodes one token at a time.  A tree has 1 to 64 nodes, node 0 the root (the token
+ * sampled last, not in the cache yet), every parent before its children.  Of a sequence with
+ * seq_lens[b] keys in its cache, node t stands at cache row seq_lens[b] + t and at rotary
+ * position seq_lens[b] + depth(t).  Caches are dense [max_batch, num_kv_heads, max_seq_len,
+ * head_dim] (seq_base NULL) or ragged [num_kv_heads, total_rows, head_dim] with seq_base
+ * (int64) and seq_cap (int32).
+ */
+
+/*
+ * lpc_rope_kv_append / lpc_rope_kv_append_ragged for the nodes of a tree: qkv [batch, nodes,
+ * (num_heads + 2*num_kv_heads) * head_dim]; seq_lens int32 [batch]; depths int32 [batch,
+ * nodes], depths_stride elements between sequences (0: [nodes], one tree for all).  A node
+ * of negative depth is skipped; one outside the sequence's rows or the tables is skipped and
+ * flagged in lpc_device_status(); the q of either is zero.
+ */
+LPC_API int lpc_rope_kv_append_tree(const void* qkv, const int32_t* seq_lens,
+                                    const int32_t* depths, int64_t depths_stride, const void* cos,
+                                    const void* sin, int64_t table_rows, void* q_out,
+                                    void* key_cache, void* value_cache, const int64_t* seq_base,
+                                    const int32_t* seq_cap, int64_t batch, int64_t nodes,
+                                    int num_heads, int num_kv_heads, int head_dim,
+                                    int64_t max_batch, int64_t max_seq_len, int64_t total_rows,
+                                    int dtype, int table_dtype, void* stream);
+
+/*
+ * The branch of each tree that the samples agree with.  drafted, sampled: int64 [batch,
+ * nodes], the token of a node and the one sampled after it; parents: int32, as depths above
+ * (parents[t] < t; the root's is not read; a node whose parent is not before it is nobody's
+ * child and flagged in lpc_device_status()).  From the root the branch goes on to the lowest
+ * child whose drafted token is the node's sampled one.  accepted: int32 [batch], nodes of the
+ * branch, the root among them; path: int32 [batch, nodes], those nodes, then -1; tokens:
+ * int64 [batch, nodes], what was sampled after them, then -1.  The K and V rows seq_lens[b] +
+ * path[i] of every layer's caches (host arrays of `layers` device pointers; layers 0: none)
+ * move to seq_lens[b] + i.  A branch that leaves the sequence's rows is flagged and not moved.
+ * seq_lens is not changed.  elem_bytes: 2 or 4; head_dim * elem_bytes a multiple of 16.
+ */
+LPC_API int lpc_tree_accept(const int64_t* drafted, const int32_t* parents, int64_t parents_stride,
+                            const int64_t* sampled, const int32_t* seq_lens,
+                            void* const* key_caches, void* const* value_caches, int layers,
+                            const int64_t* seq_base, const int32_t* seq_cap, int32_t* accepted,
+                            int64_t* tokens, int32_t* path, int64_t batch, int nodes,
+                            int num_kv_heads, int head_dim, int64_t max_batch, int64_t max_seq_len,
+                            int64_t total_rows, int elem_bytes, void* stream);
+
+/*
+ * One token a row from logits [rows, vocab] (row_stride elements between rows) and uniforms
+ * (fp32 [rows], in [0, 1)).  Replaces `sample_next_token`
+ * (src/llama_pure_compute/generate.py:58-153) for batches, with min-p and given random
+ * numbers.  Logits are ordered from the largest down, equal ones by index; w_i = exp((l_i -
+ * largest) / temperature).  top_k (<= 0 or >= vocab: off) keeps the first of the order; top_p
+ * of these the ones that have at most top_p * (their sum) before them; min_p of these the ones
+ * with w_i >= min_p.  out[r] (int64): the lowest index at which the running sum of the kept
+ * weights, in the order of the indices, exceeds uniforms[r] * (their sum); temperature 0: the
+ * first of the order.  -inf and NaN are never drawn; a row of nothing else gives -1.  Weights
+ * are held in 64 bits, rounded to 2^-44 of the largest.  temperature, top_p, min_p (fp32
+ * [rows]) and top_k (int32 [rows]) may be NULL: the numbers ..._all hold for every row then.
+ * A row with a setting or a random number out of range gives -1 and is flagged in
+ * lpc_device_status().  Up to 385,024 fp32 or 770,048 16-bit logits a row.
+ */
+LPC_API int lpc_sample_tokens(const void* logits, int64_t row_stride, const float* uniforms,
+                              const float* temperature, const int32_t* top_k, const float* top_p,
+                              const float* min_p, float temperature_all, int32_t top_k_all,
+                              float top_p_all, float min_p_all, int64_t* out, int64_t rows,
+                              int64_t vocab, int dtype, void* stream);
+
+/*
  * HBM read-rate probe (a measurement utility; no reference counterpart).
  * Reads `bytes` (a positive multiple of 131072) of `buf` the way the decode
  * attention reads its cache rows: one CTA per 128 KB, 16 KB 1-D bulk copies

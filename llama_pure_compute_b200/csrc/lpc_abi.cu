@@ -159,6 +159,8 @@ unsigned int lpc_status_kv4_append(bool clear);
 unsigned int lpc_status_kv4_attention(bool clear);
 unsigned int lpc_status_int4(bool clear);
 unsigned int lpc_status_int4_few(bool clear);
+unsigned int lpc_status_sample(bool clear);
+unsigned int lpc_status_tree_accept(bool clear);
 
 extern "C" int lpc_version(void) { return 100; }
 
@@ -173,6 +175,7 @@ extern "C" int lpc_device_status(void) {
                    lpc_status_swiglu(true) | lpc_status_prefill(true) | lpc_status_wsgemm(true) |
                    lpc_status_probe(true) | lpc_status_kv4_append(true) |
                    lpc_status_kv4_attention(true) | lpc_status_int4(true) |
-                   lpc_status_int4_few(true);
+                   lpc_status_int4_few(true) | lpc_status_sample(true) |
+                   lpc_status_tree_accept(true);
   return static_cast<int>(s);
 }

@@ -166,13 +166,23 @@ __global__ void __launch_bounds__(256) rope_kernel(T* q, T* k, const TT* __restr
 // all K items: no per-item index division, no shared memory, no barrier.
 constexpr int RA_THREADS = 256;  // block size at most (chunks * hpb)
 
-template <typename T, typename TT, int VEC, int K>
+// TREE: the seq tokens of sequence b are the nodes of a drafted tree.  Node s goes to cache row
+// seq_lens[b] + s and is rotated at position seq_lens[b] + depths[s]; a node of negative depth,
+// and one outside the rows or the tables, gives a zero q.
+struct TreeRows {
+  const int32_t* seq_lens;
+  const int32_t* depths;
+  int64_t depths_stride;  // of a sequence; 0: one tree for all
+};
+
+template <typename T, typename TT, int VEC, int K, bool TREE>
 __global__ void __launch_bounds__(RA_THREADS, 3) rope_kv_append_kernel(
     const T* __restrict__ qkv, const int64_t* __restrict__ positions, const TT* __restrict__ cosb,
     const TT* __restrict__ sinb, int64_t table_rows, T* __restrict__ q_out,
     T* __restrict__ kcache, T* __restrict__ vcache, int64_t seq, int num_heads, int num_kv_heads,
     int head_dim, int chunks, int hpb, int64_t max_batch, int64_t max_seq_len,
-    const int64_t* __restrict__ seq_base, const int32_t* __restrict__ seq_cap, int64_t total_rows) {
+    const int64_t* __restrict__ seq_base, const int32_t* __restrict__ seq_cap, int64_t total_rows,
+    const TreeRows tree) {
   // launched with programmatic stream serialisation: the decode attention
   // after it may be scheduled now (it waits for this grid before reading the
   // cache), and this grid waits for the projection that wrote qkv
@@ -195,27 +205,49 @@ __global__ void __launch_bounds__(RA_THREADS, 3) rope_kv_append_kernel(
       x1[k] = __ldg(reinterpret_cast<const uint4*>(p + half));
     }
   }
-  const int64_t pos = __ldg(positions + tok);
-  if (pos < 0) return;
   const int64_t b = tok / seq;
-  // cache row of (b, kv head 0, pos) and the distance between kv heads:
-  //   dense  [max_batch, Hkv, max_seq_len, D]: (b * Hkv) * max_seq_len + pos, max_seq_len
-  //   ragged [Hkv, total_rows, D] (seq_base != nullptr): seq_base[b] + pos, total_rows
+  int64_t pos, slot;  // rotary position, place in the sequence's rows
+  bool ok = true;
+  if constexpr (TREE) {
+    const int64_t s = tok - b * seq;
+    const int64_t n = lpc::ld_dep(tree.seq_lens + b);
+    const int32_t depth = lpc::ld_dep(tree.depths + b * tree.depths_stride + s);
+    ok = n >= 0;
+    slot = n + s;
+    pos = depth < 0 ? -1 : n < 0 ? 0 : n + depth;
+  } else {
+    slot = pos = __ldg(positions + tok);
+    if (pos < 0) return;
+  }
+  // cache row of (b, kv head 0, slot) and the distance between kv heads:
+  //   dense  [max_batch, Hkv, max_seq_len, D]: (b * Hkv) * max_seq_len + slot, max_seq_len
+  //   ragged [Hkv, total_rows, D] (seq_base != nullptr): seq_base[b] + slot, total_rows
   int64_t row, head_rows;
-  bool ok;
   if (seq_base == nullptr) {
-    ok = pos < max_seq_len && b < max_batch;
-    row = b * num_kv_heads * max_seq_len + pos;
+    ok = ok && slot < max_seq_len && b < max_batch;
+    row = b * num_kv_heads * max_seq_len + slot;
     head_rows = max_seq_len;
   } else {
     const int64_t sb = __ldg(seq_base + b);
     const int64_t cap = __ldg(seq_cap + b);
-    ok = sb >= 0 && pos < cap && sb + cap <= total_rows;
-    row = sb + pos;
+    ok = ok && sb >= 0 && slot < cap && sb + cap <= total_rows;
+    row = sb + slot;
     head_rows = total_rows;
   }
-  if (!ok || pos >= table_rows) {
-    if (threadIdx.x == 0) atomicOr(&g_rope_status, LPC_DEV_ERR_BOUNDS);
+  const int64_t q_row = (b * num_heads) * seq + (tok - b * seq);  // q_out row of (b, head 0, s)
+  if (!ok || pos >= table_rows || (TREE && pos < 0)) {
+    const bool skipped = TREE && pos < 0;
+    if (threadIdx.x == 0 && !skipped) atomicOr(&g_rope_status, LPC_DEV_ERR_BOUNDS);
+    if constexpr (TREE) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int hh = hh0 + k * hpb;
+        if (hh >= num_heads) continue;
+        T* dst = q_out + (q_row + (int64_t)hh * seq) * head_dim;
+        reinterpret_cast<uint4*>(dst + d)[0] = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(dst + d + half)[0] = make_uint4(0, 0, 0, 0);
+      }
+    }
     return;
   }
   const int rot_heads = num_heads + num_kv_heads;  // q and k heads come before v
@@ -228,7 +260,6 @@ __global__ void __launch_bounds__(RA_THREADS, 3) rope_kv_append_kernel(
     load_f<TT, VEC>(cr + d + half, c1);
     load_f<TT, VEC>(sr + d + half, s1);
   }
-  const int64_t q_row = (b * num_heads) * seq + (tok - b * seq);  // q_out row of (b, head 0, s)
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int hh = hh0 + k * hpb;
@@ -292,12 +323,12 @@ int launch_rope_t(int table_dtype, void* q, void* k, const void* c, const void* 
   return LPC_ERR_UNSUPPORTED;
 }
 
-template <typename T, typename TT, int K>
+template <typename T, typename TT, int K, bool TREE>
 cudaError_t launch_fused_k(dim3 grid, int threads, const void* qkv, const int64_t* positions,
                     const void* c, const void* sn, int64_t rows, void* q_out, void* kc, void* vc,
                     int64_t seq, int h, int hkv, int d, int chunks, int hpb, int64_t max_batch,
                     int64_t max_seq, const int64_t* seq_base, const int32_t* seq_cap,
-                    int64_t total_rows, cudaStream_t s) {
+                    int64_t total_rows, const TreeRows& tree, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   static const bool pdl = [] {
     const char* e = getenv("LPC_PDL");
@@ -313,16 +344,17 @@ cudaError_t launch_fused_k(dim3 grid, int threads, const void* qkv, const int64_
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, rope_kv_append_kernel<T, TT, VEC, K>, (const T*)qkv, positions,
+  return cudaLaunchKernelEx(&cfg, rope_kv_append_kernel<T, TT, VEC, K, TREE>, (const T*)qkv, positions,
                      (const TT*)c, (const TT*)sn, rows, (T*)q_out, (T*)kc, (T*)vc, seq, h, hkv, d,
-                     chunks, hpb, max_batch, max_seq, seq_base, seq_cap, total_rows);
+                     chunks, hpb, max_batch, max_seq, seq_base, seq_cap, total_rows,
+                     tree);
 }
 
-template <typename T, typename TT>
+template <typename T, typename TT, bool TREE>
 int launch_fused(const void* qkv, const int64_t* positions, const void* c, const void* sn,
                  int64_t rows, void* q_out, void* kc, void* vc, int64_t batch, int64_t seq, int h,
                  int hkv, int d, int64_t max_batch, int64_t max_seq, const int64_t* seq_base,
-                 const int32_t* seq_cap, int64_t total_rows, cudaStream_t s) {
+                 const int32_t* seq_cap, int64_t total_rows, const TreeRows& tree, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const int64_t tokens = batch * seq;
   if (tokens == 0) return LPC_OK;
@@ -338,8 +370,9 @@ int launch_fused(const void* qkv, const int64_t* positions, const void* c, const
   const dim3 grid((unsigned)tokens, (unsigned)((heads_all + K * hpb - 1) / (K * hpb)));
   const int threads = chunks * hpb;
 #define LPC_RA(KK)                                                                                 \
-  launch_fused_k<T, TT, KK>(grid, threads, qkv, positions, c, sn, rows, q_out, kc, vc, seq, h, hkv, \
-                            d, chunks, hpb, max_batch, max_seq, seq_base, seq_cap, total_rows, s)
+  launch_fused_k<T, TT, KK, TREE>(grid, threads, qkv, positions, c, sn, rows, q_out, kc, vc, seq, h, \
+                                  hkv, d, chunks, hpb, max_batch, max_seq, seq_base, seq_cap,       \
+                                  total_rows, tree, s)
   const cudaError_t e = K == 1 ? LPC_RA(1) : K == 2 ? LPC_RA(2) : K == 3 ? LPC_RA(3) : LPC_RA(4);
   if (e != cudaSuccess) {
     lpc::set_error("rope_kv_append: launch failed: %s", cudaGetErrorString(e));
@@ -393,14 +426,15 @@ extern "C" int lpc_rope_forward(void* q, void* k, const void* cos, const void* s
 
 namespace {
 
+template <bool TREE>
 int rope_kv_append_common(const void* qkv, const int64_t* positions, const void* cos,
                           const void* sin, int64_t table_rows, void* q_out, void* key_cache,
                           void* value_cache, int64_t batch, int64_t seq, int num_heads,
                           int num_kv_heads, int head_dim, int64_t max_batch, int64_t max_seq_len,
                           const int64_t* seq_base, const int32_t* seq_cap, int64_t total_rows,
-                          int dtype, int table_dtype, void* stream) {
+                          const TreeRows& tree, int dtype, int table_dtype, void* stream) {
   using namespace lpc;
-  if (!qkv || !positions || !cos || !sin || !q_out || !key_cache || !value_cache) {
+  if (!qkv || (TREE ? !tree.seq_lens || !tree.depths : !positions) || !cos || !sin || !q_out || !key_cache || !value_cache) {
     set_error("rope_kv_append: null pointer");
     return LPC_ERR_INVALID;
   }
@@ -419,9 +453,9 @@ int rope_kv_append_common(const void* qkv, const int64_t* positions, const void*
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define LPC_FUSED(T, TT)                                                                        \
-  return launch_fused<T, TT>(qkv, positions, cos, sin, table_rows, q_out, key_cache, value_cache, \
-                             batch, seq, num_heads, num_kv_heads, head_dim, max_batch,           \
-                             max_seq_len, seq_base, seq_cap, total_rows, s)
+  return launch_fused<T, TT, TREE>(qkv, positions, cos, sin, table_rows, q_out, key_cache,      \
+                                   value_cache, batch, seq, num_heads, num_kv_heads, head_dim,  \
+                                   max_batch, max_seq_len, seq_base, seq_cap, total_rows, tree, s)
   if (dtype == LPC_DTYPE_BF16) {
     if (table_dtype == LPC_DTYPE_BF16) LPC_FUSED(__nv_bfloat16, __nv_bfloat16);
     if (table_dtype == LPC_DTYPE_F32) LPC_FUSED(__nv_bfloat16, float);
@@ -454,9 +488,10 @@ extern "C" int lpc_rope_kv_append(const void* qkv, const int64_t* positions, con
               (long long)max_batch);
     return LPC_ERR_INVALID;
   }
-  return rope_kv_append_common(qkv, positions, cos, sin, table_rows, q_out, key_cache, value_cache,
-                               batch, seq, num_heads, num_kv_heads, head_dim, max_batch,
-                               max_seq_len, nullptr, nullptr, 0, dtype, table_dtype, stream);
+  return rope_kv_append_common<false>(qkv, positions, cos, sin, table_rows, q_out, key_cache,
+                                      value_cache, batch, seq, num_heads, num_kv_heads, head_dim,
+                                      max_batch, max_seq_len, nullptr, nullptr, 0, TreeRows{}, dtype,
+                                      table_dtype, stream);
 }
 
 extern "C" int lpc_rope_kv_append_ragged(const void* qkv, const int64_t* positions,
@@ -477,7 +512,37 @@ extern "C" int lpc_rope_kv_append_ragged(const void* qkv, const int64_t* positio
     set_error("rope_kv_append_ragged: seq_base and seq_cap are required");
     return LPC_ERR_INVALID;
   }
-  return rope_kv_append_common(qkv, positions, cos, sin, table_rows, q_out, key_cache, value_cache,
-                               batch, seq, num_heads, num_kv_heads, head_dim, batch, 1, seq_base,
-                               seq_cap, total_rows, dtype, table_dtype, stream);
+  return rope_kv_append_common<false>(qkv, positions, cos, sin, table_rows, q_out, key_cache,
+                                      value_cache, batch, seq, num_heads, num_kv_heads, head_dim,
+                                      batch, 1, seq_base, seq_cap, total_rows, TreeRows{}, dtype,
+                                      table_dtype, stream);
+}
+
+extern "C" int lpc_rope_kv_append_tree(const void* qkv, const int32_t* seq_lens,
+                                       const int32_t* depths, int64_t depths_stride,
+                                       const void* cos, const void* sin, int64_t table_rows,
+                                       void* q_out, void* key_cache, void* value_cache,
+                                       const int64_t* seq_base, const int32_t* seq_cap,
+                                       int64_t batch, int64_t nodes, int num_heads,
+                                       int num_kv_heads, int head_dim, int64_t max_batch,
+                                       int64_t max_seq_len, int64_t total_rows, int dtype,
+                                       int table_dtype, void* stream) {
+  using namespace lpc;
+  if (batch < 0 || nodes < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      table_rows <= 0 || (depths_stride != 0 && depths_stride < nodes) ||
+      (seq_base ? total_rows <= 0 || !seq_cap : max_batch <= 0 || max_seq_len <= 0)) {
+    set_error("rope_kv_append_tree: invalid sizes");
+    return LPC_ERR_INVALID;
+  }
+  if (batch == 0 || nodes == 0) return LPC_OK;
+  if (!seq_base && batch > max_batch) {
+    set_error("rope_kv_append_tree: batch %lld exceeds cache capacity %lld", (long long)batch,
+              (long long)max_batch);
+    return LPC_ERR_INVALID;
+  }
+  const TreeRows tree{seq_lens, depths, depths_stride};
+  return rope_kv_append_common<true>(qkv, nullptr, cos, sin, table_rows, q_out, key_cache,
+                                     value_cache, batch, nodes, num_heads, num_kv_heads, head_dim,
+                                     max_batch, max_seq_len, seq_base, seq_cap, total_rows, tree,
+                                     dtype, table_dtype, stream);
 }

@@ -16,11 +16,14 @@ ops module): ``rmsnorm_forward``, ``rope_kv_append`` and ``decode_attention``.
 
 4-bit KV cache: ``Int4KV`` (the cache's tensors), ``rope_kv_append_int4``,
 ``decode_attention_int4`` and ``kv_read_int4``.
+
+Speculative decoding over drafted trees: ``rope_kv_append_tree``, ``tree_attention``,
+``tree_accept`` (with ``LayerCaches``) and ``sample_tokens``, which draws from any logits.
 """
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -42,6 +45,10 @@ __all__ = [
     "decode_attention_int4",
     "decode_attention_int4_workspace",
     "kv_read_int4",
+    "sample_tokens",
+    "rope_kv_append_tree",
+    "LayerCaches",
+    "tree_accept",
 ]
 
 
@@ -920,3 +927,332 @@ def decode_attention_int4(
             n = kv._kernels[B, H] = lib.lpc_decode_attention_int4_kernels(kv.ref, B, H)
         _lib.launch_count += n
     return out
+
+
+# ---------------------------------------------------------------------------
+# Sampling
+# ---------------------------------------------------------------------------
+def _row_setting(value, name: str, rows: int, index: int, dtype: torch.dtype):
+    """(tensor or None, its address or None, number) of a setting given for all
+    rows or as a tensor with one entry a row."""
+    if not isinstance(value, torch.Tensor):
+        return None, None, value
+    if value.get_device() != index:
+        _require_cuda(value, name)
+        raise ValueError(f"LlamaPureComputeError: {name} must be on the logits' device.")
+    if value.numel() != rows:
+        raise ValueError(f"LlamaPureComputeError: {name} must have one entry per row.")
+    if value.dtype is not dtype:
+        if value.dtype.is_floating_point != dtype.is_floating_point or value.dtype == torch.bool:
+            raise TypeError(f"LlamaPureComputeError: {name} must be {dtype}.")
+        if dtype is torch.int32:
+            value = value.clamp(-2 ** 31, 2 ** 31 - 1)
+        value = value.to(dtype)
+    if not value.is_contiguous():
+        value = value.contiguous()
+    return value, value.data_ptr(), 0
+
+
+def sample_tokens(
+    logits: torch.Tensor,
+    uniforms: torch.Tensor,
+    temperature: Union[float, torch.Tensor] = 1.0,
+    top_k: Union[int, torch.Tensor] = 0,
+    top_p: Union[float, torch.Tensor] = 1.0,
+    min_p: Union[float, torch.Tensor] = 0.0,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """One token a row of ``logits`` [..., vocab] (fp32, bf16 or fp16), drawn with
+    the random numbers ``uniforms`` [...] (fp32, in [0, 1)); int64 [...].
+
+    Logits are ordered from the largest down, equal ones by index, and weigh
+    ``exp((logit - largest) / temperature)``.  ``top_k`` keeps the first of the
+    order (<= 0: all), ``top_p`` of these the ones that have at most ``top_p`` *
+    (their sum) before them, ``min_p`` of these the ones that weigh at least
+    ``min_p``.  The token is the lowest index at which the running sum of what is
+    kept, in the order of the indices, exceeds ``uniforms`` * (its sum); at
+    temperature 0 it is the first of the order, as ``torch.argmax`` of
+    ``sample_next_token`` (generate.py:58-153).  Weights are held in 64 bits.
+    -inf and NaN are never drawn; a row of nothing else gives -1.
+
+    Each setting is a number or a tensor with one entry a row (fp32; ``top_k``
+    int32).  Numbers are checked here; a row whose entry or random number is out
+    of range gives -1 and sets the device status."""
+    index, shape = logits.get_device(), logits.shape
+    if index < 0 or uniforms.get_device() != index:
+        _require_cuda(logits, "logits")
+        _require_cuda(uniforms, "uniforms")
+        raise ValueError("LlamaPureComputeError: logits and uniforms must be on one device.")
+    code = _lib.DTYPE_CODE.get(logits.dtype)
+    if code is None:
+        raise TypeError(f"LlamaPureComputeError: sample_tokens: unsupported dtype {logits.dtype}")
+    if not shape or shape[-1] == 0:
+        raise ValueError("LlamaPureComputeError: logits must be [..., vocab].")
+    lead, vocab = shape[:-1], shape[-1]
+    rows = lead.numel()
+    if len(shape) == 2 and (rows <= 1 or logits.stride(0) >= vocab) and logits.stride(1) == 1:
+        stride = logits.stride(0)
+    else:
+        if not logits.is_contiguous():
+            logits = logits.contiguous()
+        stride = vocab
+    if uniforms.dtype is not torch.float32:
+        raise TypeError("LlamaPureComputeError: uniforms must be float32.")
+    if uniforms.numel() != rows:
+        raise ValueError("LlamaPureComputeError: uniforms must have one entry per row.")
+    if not uniforms.is_contiguous():
+        uniforms = uniforms.contiguous()
+    t, tp, ta = _row_setting(temperature, "temperature", rows, index, torch.float32)
+    k, kp, ka = _row_setting(top_k, "top_k", rows, index, torch.int32)
+    p, pp, pa = _row_setting(top_p, "top_p", rows, index, torch.float32)
+    m, mp, ma = _row_setting(min_p, "min_p", rows, index, torch.float32)
+    if out is None:
+        out = torch.empty(lead, dtype=torch.int64, device=logits.device)
+    else:
+        if out.shape != lead or out.dtype != torch.int64 or out.get_device() != index \
+                or not out.is_contiguous():
+            raise ValueError(f"LlamaPureComputeError: out must be a contiguous int64 {tuple(lead)} "
+                             "tensor on the logits' device.")
+        at = out.untyped_storage().data_ptr()
+        if any(x is not None and x.untyped_storage().data_ptr() == at and out.numel()
+               for x in (logits, uniforms, t, k, p, m)):
+            raise ValueError("LlamaPureComputeError: out must not share memory with an input.")
+    rc = _lib.call_on(index, _lib.load().lpc_sample_tokens, logits.data_ptr(), stride,
+                      uniforms.data_ptr(), tp, kp, pp, mp, ta, max(-1, min(ka, 2 ** 31 - 1)), pa, ma,
+                      out.data_ptr(), rows, vocab, code)
+    if rc:
+        _lib.check(rc, "sample_tokens")
+    if rows:
+        _lib.launch_count += 1
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Speculative decoding over drafted trees.  A tree has T <= 64 nodes: node 0 is
+# the root (the token sampled last, not in the cache yet), parents stand before
+# their children.  Of a sequence with n keys in its cache, node t has cache row
+# n + t and rotary position n + depth(t).
+# ---------------------------------------------------------------------------
+MAX_TREE_NODES = 64
+
+
+def _tree_caches(key_cache, value_cache, seq_base, seq_cap, B: int, index: int):
+    """(kv heads, head_dim, max_batch, max_seq_len, total_rows) of one layer's caches."""
+    shape = key_cache.shape
+    ragged = seq_base is not None or seq_cap is not None
+    if value_cache.shape != shape or len(shape) != (3 if ragged else 4):
+        raise ValueError("LlamaPureComputeError: caches must be matching [B, H, S, D] (dense) or "
+                         "[H, rows, D] (ragged, with seq_base and seq_cap) tensors.")
+    if key_cache.get_device() != index or value_cache.get_device() != index:
+        _require_cuda(key_cache, "key_cache")
+        _require_cuda(value_cache, "value_cache")
+        raise ValueError("LlamaPureComputeError: the caches must be on the other tensors' device.")
+    if not key_cache.is_contiguous() or not value_cache.is_contiguous():
+        raise ValueError("LlamaPureComputeError: caches must be memory-contiguous.")
+    if value_cache.dtype != key_cache.dtype:
+        raise TypeError("LlamaPureComputeError: the caches' dtypes differ.")
+    if not ragged:
+        if B > shape[0]:
+            raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
+        return shape[1], shape[3], shape[0], shape[2], 0
+    if seq_base is None or seq_cap is None:
+        raise ValueError("LlamaPureComputeError: a ragged cache needs seq_base and seq_cap.")
+    _check_ragged_index(seq_base, seq_cap, B)
+    if seq_base.get_device() != index or seq_cap.get_device() != index:
+        raise ValueError("LlamaPureComputeError: seq_base and seq_cap must be on the caches' device.")
+    return shape[0], shape[2], B, 0, shape[1]
+
+
+def _tree_ints(t: torch.Tensor, name: str, B: int, T: int, index: int, dtype=torch.int32):
+    """A tensor [B, T], or [T] for all sequences, and its stride between sequences."""
+    if t.get_device() != index:
+        _require_cuda(t, name)
+        raise ValueError(f"LlamaPureComputeError: {name} must be on the other tensors' device.")
+    if t.dtype is not dtype:
+        raise TypeError(f"LlamaPureComputeError: {name} must be {dtype}.")
+    if t.shape != (B, T) and t.shape != (T,):
+        raise ValueError(f"LlamaPureComputeError: {name} must be [batch, nodes] or [nodes].")
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t, T if t.dim() == 2 else 0
+
+
+def _tree_lens(seq_lens: torch.Tensor, B: int, index: int) -> None:
+    if seq_lens.get_device() != index:
+        _require_cuda(seq_lens, "seq_lens")
+        raise ValueError("LlamaPureComputeError: seq_lens must be on the other tensors' device.")
+    if seq_lens.dtype != torch.int32:
+        raise TypeError("LlamaPureComputeError: seq_lens must be int32.")
+    if seq_lens.numel() < B or not seq_lens.is_contiguous():
+        raise ValueError("LlamaPureComputeError: seq_lens must have a contiguous entry per sequence.")
+
+
+def rope_kv_append_tree(
+    qkv: torch.Tensor,
+    seq_lens: torch.Tensor,
+    depths: torch.Tensor,
+    cos_table: torch.Tensor,
+    sin_table: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    num_heads: int,
+    num_kv_heads: int,
+    seq_base: Optional[torch.Tensor] = None,
+    seq_cap: Optional[torch.Tensor] = None,
+    q_out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``rope_kv_append`` (dense caches) / ``rope_kv_append_ragged`` (with
+    ``seq_base`` and ``seq_cap``) for a drafted tree a sequence: node t of ``qkv``
+    [B, T, (H+2Hkv)*D] goes to cache row ``seq_lens[b] + t`` and is rotated at
+    position ``seq_lens[b] + depths[b, t]``; returns q as [B, H, T, D].
+
+    ``seq_lens`` (int32 [B]): keys before the tree.  ``depths`` (int32 [B, T], or
+    [T] for one tree): a negative depth skips the node; a node outside the
+    sequence's rows or the tables is skipped and sets the device status.  The q
+    of a skipped node is zero."""
+    index = qkv.get_device()
+    if index < 0 or cos_table.get_device() != index or sin_table.get_device() != index:
+        for t, n in ((qkv, "qkv"), (cos_table, "cos"), (sin_table, "sin")):
+            _require_cuda(t, n)
+        raise ValueError("LlamaPureComputeError: qkv and the rope tables must be on one device.")
+    if qkv.dim() != 3:
+        raise ValueError("LlamaPureComputeError: qkv must be [batch, nodes, width].")
+    B, T, W = qkv.shape
+    kv_heads, D, max_batch, max_seq_len, total_rows = _tree_caches(key_cache, value_cache, seq_base,
+                                                                   seq_cap, B, index)
+    if kv_heads != num_kv_heads or num_heads <= 0 or W != (num_heads + 2 * num_kv_heads) * D:
+        raise ValueError("LlamaPureComputeError: qkv width does not match heads * head_dim.")
+    if qkv.dtype != key_cache.dtype:
+        raise TypeError("LlamaPureComputeError: qkv and cache dtypes differ.")
+    rows = cos_table.shape
+    if len(rows) != 2 or rows[1] != D or sin_table.shape != rows \
+            or sin_table.dtype != cos_table.dtype:
+        raise ValueError("LlamaPureComputeError: rope tables must be matching [max_pos, head_dim].")
+    _tree_lens(seq_lens, B, index)
+    depths, depths_stride = _tree_ints(depths, "depths", B, T, index)
+    qkv, cos_table, sin_table = _dense16(qkv), _dense16(cos_table), _dense16(sin_table)
+    if q_out is None:
+        q_out = qkv.new_empty(B, num_heads, T, D)
+    elif q_out.shape != (B, num_heads, T, D) or q_out.dtype != qkv.dtype \
+            or q_out.get_device() != index or not q_out.is_contiguous():
+        raise ValueError("LlamaPureComputeError: q_out must be a contiguous [B, H, T, D] tensor of "
+                         "qkv's dtype and device.")
+    elif _overlap(q_out, qkv):
+        raise ValueError("LlamaPureComputeError: q_out must not overlap qkv.")
+    code = _lib.dtype_code(qkv.dtype, "rope_kv_append_tree")
+    rc = _lib.call_on(index, _lib.load().lpc_rope_kv_append_tree, qkv.data_ptr(),
+                      seq_lens.data_ptr(), depths.data_ptr(), depths_stride, cos_table.data_ptr(),
+                      sin_table.data_ptr(), rows[0], q_out.data_ptr(), key_cache.data_ptr(),
+                      value_cache.data_ptr(), _lib.ptr(seq_base), _lib.ptr(seq_cap), B, T, num_heads,
+                      num_kv_heads, D, max_batch, max_seq_len, total_rows, code,
+                      _lib.dtype_code(cos_table.dtype, "rope_kv_append_tree"))
+    if rc:
+        _lib.check(rc, "rope_kv_append_tree")
+    if B and T:
+        _lib.launch_count += 1
+    return q_out
+
+
+class LayerCaches:
+    """The K and V caches of a model's layers, checked once and handed to
+    ``tree_accept``: dense [max_batch, kv_heads, max_seq_len, head_dim] each, or
+    ragged [kv_heads, total_rows, head_dim] with ``seq_base`` (int64) and
+    ``seq_cap`` (int32), one entry a sequence of the batch."""
+
+    __slots__ = ("key_caches", "value_caches", "seq_base", "seq_cap", "kv_heads", "head_dim",
+                 "max_batch", "max_seq_len", "total_rows", "elem_bytes", "index", "_k", "_v")
+
+    def __init__(self, key_caches: Sequence[torch.Tensor], value_caches: Sequence[torch.Tensor],
+                 seq_base: Optional[torch.Tensor] = None, seq_cap: Optional[torch.Tensor] = None):
+        keys, values = list(key_caches), list(value_caches)
+        if not keys or len(keys) != len(values):
+            raise ValueError("LlamaPureComputeError: every layer needs a key and a value cache.")
+        first = keys[0]
+        _require_cuda(first, "key_caches")
+        self.index = first.get_device()
+        batch = 0 if seq_base is None else seq_base.numel()
+        for k, v in zip(keys, values):
+            if k.shape != first.shape or k.dtype != first.dtype:
+                raise ValueError("LlamaPureComputeError: the layers' caches must be alike.")
+            if k.data_ptr() % 16 or v.data_ptr() % 16:
+                raise ValueError("LlamaPureComputeError: caches must be 16-byte aligned.")
+            (self.kv_heads, self.head_dim, self.max_batch, self.max_seq_len,
+             self.total_rows) = _tree_caches(k, v, seq_base, seq_cap, batch, self.index)
+        if seq_base is not None and seq_base.numel() != seq_cap.numel():
+            raise ValueError("LlamaPureComputeError: seq_base and seq_cap must have the same entries.")
+        self.elem_bytes = first.element_size()
+        if first.numel() == 0 or self.elem_bytes not in (2, 4) or self.head_dim * self.elem_bytes % 16:
+            raise TypeError("LlamaPureComputeError: cache rows must be whole 16-byte pieces of 16- or "
+                            "32-bit values.")
+        self.key_caches, self.value_caches = keys, values
+        self.seq_base, self.seq_cap = seq_base, seq_cap
+        pointers = ctypes.c_void_p * len(keys)
+        self._k = pointers(*[k.data_ptr() for k in keys])
+        self._v = pointers(*[v.data_ptr() for v in values])
+
+
+def tree_accept(
+    drafted: torch.Tensor,
+    parents: torch.Tensor,
+    sampled: torch.Tensor,
+    seq_lens: Optional[torch.Tensor] = None,
+    caches: Optional[LayerCaches] = None,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The branch of each drafted tree that the samples agree with, with its K/V
+    rows moved together in ``caches``.
+
+    ``drafted`` (int64 [B, T]): the tokens of the nodes; ``sampled`` (int64 [B, T]):
+    what the model draws after each; ``parents`` (int32 [B, T], or [T] for one
+    tree): ``parents[t] < t``, the root's is not read.  From the root the branch
+    goes on, while there is one, to the lowest child whose token is the node's
+    sampled one.  Returns
+
+      accepted  int32 [B]: nodes of the branch, the root among them (>= 1);
+      tokens    int64 [B, T]: what was sampled after them -- so many new tokens, of
+                which the last is the next root -- then -1;
+      path      int32 [B, T]: the nodes, then -1.
+
+    With ``caches`` (and ``seq_lens``, int32 [B]: keys before the tree) row
+    ``seq_lens[b] + path[b, i]`` of every layer moves to ``seq_lens[b] + i``; the
+    sequence then has ``seq_lens + accepted`` keys (``seq_lens`` itself stays).
+    A branch beyond the sequence's rows is not moved and sets the device status,
+    as does a parent that is not before its child (it is taken as having none)."""
+    index = drafted.get_device()
+    if index < 0:
+        _require_cuda(drafted, "drafted")
+    if drafted.dim() != 2:
+        raise ValueError("LlamaPureComputeError: drafted must be [batch, nodes].")
+    B, T = drafted.shape
+    if not 1 <= T <= MAX_TREE_NODES:
+        raise ValueError(f"LlamaPureComputeError: a tree has 1 to {MAX_TREE_NODES} nodes.")
+    if sampled.shape != (B, T):
+        raise ValueError("LlamaPureComputeError: sampled must be [batch, nodes].")
+    drafted, _ = _tree_ints(drafted, "drafted", B, T, index, torch.int64)
+    sampled, _ = _tree_ints(sampled, "sampled", B, T, index, torch.int64)
+    parents, parents_stride = _tree_ints(parents, "parents", B, T, index)
+    accepted = torch.empty(B, dtype=torch.int32, device=drafted.device)
+    tokens = torch.empty_like(drafted)
+    path = torch.empty(B, T, dtype=torch.int32, device=drafted.device)
+    lens = keys = values = base = cap = None
+    layers = kv_heads = head_dim = max_batch = max_seq_len = total_rows = elem = 0
+    if caches is not None:
+        if caches.index != index:
+            raise ValueError("LlamaPureComputeError: the caches must be on the other tensors' device.")
+        if seq_lens is None:
+            raise ValueError("LlamaPureComputeError: caches need seq_lens.")
+        _tree_lens(seq_lens, B, index)
+        if B > caches.max_batch:
+            raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
+        lens, keys, values, layers = seq_lens.data_ptr(), caches._k, caches._v, len(caches._k)
+        base, cap = _lib.ptr(caches.seq_base), _lib.ptr(caches.seq_cap)
+        kv_heads, head_dim, max_batch = caches.kv_heads, caches.head_dim, caches.max_batch
+        max_seq_len, total_rows, elem = caches.max_seq_len, caches.total_rows, caches.elem_bytes
+    rc = _lib.call_on(index, _lib.load().lpc_tree_accept, drafted.data_ptr(), parents.data_ptr(),
+                      parents_stride, sampled.data_ptr(), lens, keys, values, layers, base, cap,
+                      accepted.data_ptr(), tokens.data_ptr(), path.data_ptr(), B, T, kv_heads,
+                      head_dim, max_batch, max_seq_len, total_rows, elem)
+    if rc:
+        _lib.check(rc, "tree_accept")
+    if B:
+        _lib.launch_count += max(1, -(-layers // 128))
+    return accepted, tokens, path
