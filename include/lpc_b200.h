@@ -500,6 +500,31 @@ LPC_API int lpc_rope_kv_append_tree(const void* qkv, const int32_t* seq_lens,
                                     int dtype, int table_dtype, void* stream);
 
 /*
+ * Attention of the nodes over the context and the nodes: node t of sequence b sees the
+ * seq_lens[b] keys before the tree and the nodes whose bit is set in masks[b, t] (int64 [batch,
+ * nodes], masks_stride elements between sequences, 0: one tree for all; bits from `nodes` on are
+ * not read).  q: [batch, heads, nodes, head_dim], heads a multiple of kv_heads, head_dim 32, 64 or
+ * 128, bf16 or fp16; out: [batch, nodes, heads, head_dim].  fp32 scores, maxima and sums; weights
+ * rounded to the data type before they meet V.  Rows of K and V that a node does not see do not
+ * reach it, whatever they hold; a node that sees nothing gives zeros.  A length beyond the
+ * sequence's rows is cut to them; it and a visible node past them are flagged in
+ * lpc_device_status().  sm_scale > 0.  workspace: lpc_tree_attention_workspace_bytes() bytes for
+ * the current device (0: NULL); calls that overlap need one each.  One kernel, and one more where
+ * the workspace is not empty.  For ragged caches pass max_batch and max_seq_len 0, for dense ones
+ * total_rows 0.
+ */
+LPC_API int64_t lpc_tree_attention_workspace_bytes(int64_t batch, int nodes, int heads,
+                                                   int kv_heads, int head_dim, int64_t max_seq_len,
+                                                   int64_t total_rows);
+LPC_API int lpc_tree_attention(const void* q, const void* key_cache, const void* value_cache,
+                               const int32_t* seq_lens, const int64_t* masks, int64_t masks_stride,
+                               const int64_t* seq_base, const int32_t* seq_cap, void* out,
+                               void* workspace, int64_t workspace_bytes, int64_t batch, int nodes,
+                               int heads, int kv_heads, int head_dim, int64_t max_batch,
+                               int64_t max_seq_len, int64_t total_rows, float sm_scale, int dtype,
+                               void* stream);
+
+/*
  * The branch of each tree that the samples agree with.  drafted, sampled: int64 [batch,
  * nodes], the token of a node and the one sampled after it; parents: int32, as depths above
  * (parents[t] < t; the root's is not read; a node whose parent is not before it is nobody's

@@ -87,6 +87,9 @@ SIGNATURES = {
     "lpc_int4_linear": (_I, [_P, _P, _P, _P, _I64, _I, _P, _I64, _P]),
     "lpc_rope_kv_append_tree": (_I, [_P, _P, _P, _I64, _P, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64,
                                      _I, _I, _I, _I64, _I64, _I64, _I, _I, _P]),
+    "lpc_tree_attention_workspace_bytes": (_I64, [_I64, _I, _I, _I, _I, _I64, _I64]),
+    "lpc_tree_attention": (_I, [_P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I, _I, _I, _I,
+                                _I64, _I64, _I64, _F, _I, _P]),
     "lpc_tree_accept": (_I, [_P, _P, _I64, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I64, _I, _I, _I,
                              _I64, _I64, _I64, _I, _P]),
     "lpc_sample_tokens": (_I, [_P, _I64, _P, _P, _P, _P, _P, _F, _I, _F, _F, _P, _I64, _I64, _I,
@@ -106,7 +109,7 @@ KERNELS_PER_CALL = {
     "lpc_decode_attention_ragged": 2, "lpc_rmsswiglu_folded_forward": 1, "lpc_hbm_read_probe": 1,
     "lpc_rope_kv_append_int4": 1, "lpc_kv_read_int4": 1, "lpc_decode_attention_int4": 2,
     "lpc_int4_pack": 3, "lpc_int4_unpack": 1, "lpc_int4_linear": 1,
-    "lpc_rope_kv_append_tree": 1, "lpc_tree_accept": 1, "lpc_sample_tokens": 1,
+    "lpc_rope_kv_append_tree": 1, "lpc_tree_attention": 2, "lpc_tree_accept": 1, "lpc_sample_tokens": 1,
 }
 launch_count = 0
 

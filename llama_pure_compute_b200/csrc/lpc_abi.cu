@@ -161,6 +161,7 @@ unsigned int lpc_status_int4(bool clear);
 unsigned int lpc_status_int4_few(bool clear);
 unsigned int lpc_status_sample(bool clear);
 unsigned int lpc_status_tree_accept(bool clear);
+unsigned int lpc_status_tree_attention(bool clear);
 
 extern "C" int lpc_version(void) { return 100; }
 
@@ -176,6 +177,6 @@ extern "C" int lpc_device_status(void) {
                    lpc_status_probe(true) | lpc_status_kv4_append(true) |
                    lpc_status_kv4_attention(true) | lpc_status_int4(true) |
                    lpc_status_int4_few(true) | lpc_status_sample(true) |
-                   lpc_status_tree_accept(true);
+                   lpc_status_tree_accept(true) | lpc_status_tree_attention(true);
   return static_cast<int>(s);
 }

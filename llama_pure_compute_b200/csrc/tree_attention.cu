@@ -1,0 +1,1062 @@
+// Attention of a tree of drafted tokens over a KV cache (sm_100a, tcgen05).
+//
+// out[b, h, t] = sum_j p_j V_j, p = softmax over the visible keys j of
+// scale * q[b, h, t] . K_j, fp32 accumulation.  Visible to node t of sequence b:
+// the n = seq_lens[b] keys of the context and the nodes i whose bit i is set in
+// masks[b, t]; node i is cache row n + i.  A node that sees nothing gives zeros.
+//
+// The G * T query rows (G heads share a KV head, T <= 64 nodes) meet the same keys,
+// so K and V are read once for all of them: an item is one (sequence, KV head,
+// block of 128 or 256 rows).  Up to ~250 rows a key's bytes cost more than its
+// arithmetic (2 G T flops a byte of K and V), beyond it the tensor cores do.
+//
+// Schedule.  Every item is a row of 128-key tiles.  The tiles of all items, one
+// after another, are cut into equal stretches, one a CTA and one CTA an SM, from
+// the lengths as the device holds them: ragged batches are balanced and one long
+// sequence fills the GPU.  A CTA that holds a whole item writes its output; parts
+// of items go to a workspace (at most two a CTA, whatever the lengths) and a
+// second kernel joins them.
+//
+// CTA, 12 warps:
+//   warp 8      TMA: Q of the stretch's items, K and V tiles through one ring in
+//               the order K0 K1 V0 K2 V1 ...
+//   warp 9      TMEM, tcgen05.mma: S = Q K^T (M = 128 rows, N = 128 keys), O += P V
+//               (P from tensor memory).  Two streams, so that the tensor core works
+//               on one while the other's softmax runs:
+//                 up to 128 rows: even tiles and odd tiles of the item, each with its
+//                   own running maximum, sum and O, joined at the item's end;
+//                 more: rows 0-127 and 128-255, both on every tile.
+//   warps 0-3, 4-7  softmax of stream 0 and 1.  Thread r has row r: its 128 scores in
+//               one read, maximum, exp2 against a reference that moves only when the
+//               maximum has grown by more than 8 (factor 256: no overflow, same
+//               softmax), P rounded to the data type (half a step, 2^-9 or 2^-12 of p;
+//               the sum is of the unrounded), O rescaled in tensor memory when the
+//               reference moves.
+//   warps 10-11 the tiles that hold nodes or end the sequence: V rows that no node
+//               sees are cleared (0 * NaN would reach every row), and so are visible
+//               ones that are not finite; those are added in the epilogue, row by row,
+//               to the nodes that do see them.
+// Tensor memory: S0 S1 O0 O1, 128 columns each.
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "lpc_common.cuh"
+
+LPC_DECLARE_STATUS(g_tree_status)
+
+unsigned int lpc_status_tree_attention(bool clear) {
+  unsigned int v = 0;
+  cudaMemcpyFromSymbol(&v, g_tree_status, sizeof(v));
+  if (clear && v) {
+    unsigned int z = 0;
+    cudaMemcpyToSymbol(g_tree_status, &z, sizeof(z));
+  }
+  return v;
+}
+
+namespace {
+
+using lpc::Num;
+
+constexpr int MAX_NODES = 64;
+constexpr int ROWS = 128;                   // query rows a tile (UMMA M)
+constexpr int KEYS = 128;                   // keys a tile
+constexpr int BOX = 64;                     // columns a TMA box: one 128-byte swizzle row
+constexpr int HALF_BYTES = 128 * BOX * 2;   // 128 rows of a box
+constexpr int NTHREADS = 384;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float GROWTH = 8.0f;              // log2 units that a maximum may pass its reference
+constexpr int LAUNCH_REGS = 168, REGS_LOAD = 96, REGS_SOFTMAX = 200;
+static_assert(128 * REGS_LOAD + 256 * REGS_SOFTMAX <= NTHREADS * LAUNCH_REGS,
+              "register split exceeds the block's launch allocation");
+
+struct Shared {
+  float2 ml[2][ROWS];           // [stream][row]: maximum and sum, up to 128 rows
+  int64_t scan[NTHREADS / 32];
+  int64_t found[2];
+  unsigned long long bad[2];    // visible nodes of the segment whose V is not finite
+};
+constexpr int BAR_BYTES = 384;
+
+// HD: columns as the MMA sees them, 64 (head_dim 32 or 64) or 128.  WIDE: 256 rows an item.
+template <int HD, bool WIDE>
+struct Shape {
+  static constexpr int TILE = HD / BOX * HALF_BYTES;         // K, V or Q tile
+  static constexpr int QTILES = WIDE ? 2 : 1;
+  static constexpr int ITEM_ROWS = QTILES * ROWS;
+  static constexpr int SLOTS = (14 * HALF_BYTES - QTILES * TILE) / TILE;  // 224 KB with Q
+  static constexpr int TILES = (QTILES + SLOTS) * TILE;
+  static constexpr int SMEM = TILES + BAR_BYTES + (int)sizeof(Shared);
+  static constexpr int64_t PART = (int64_t)ITEM_ROWS * (HD + 2);  // floats of a part
+};
+
+struct TmaDesc4 { alignas(64) unsigned char bytes[128]; };
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int c0, int c1, int c2,
+                                            int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
+  return ((uint64_t)__float_as_uint(hi) << 32) | __float_as_uint(lo);
+}
+__device__ __forceinline__ float lo_f(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi_f(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+struct Params {
+  const void *q, *k, *v;
+  void* out;
+  const int32_t* seq_lens;
+  const int64_t* masks;
+  int64_t masks_stride;        // of a sequence; 0: one tree for all
+  const int64_t* seq_base;     // null: dense
+  const int32_t* seq_cap;
+  int64_t max_seq_len, total_rows;
+  float* parts;                // 2 a CTA
+  longlong2* split;            // the item that a CTA begins and does not finish (-1: none),
+                               // and the last CTA that has a part of it
+  int64_t batch;
+  int nodes, heads, kv_heads, group, head_dim, row_blocks;
+  float scale_log2;
+};
+
+// What a sequence holds: n keys of context, keys and nodes together up to `end`,
+// `tiles` of them; cache row of KV head 0 and the distance between KV heads.
+struct Sequence {
+  int64_t n, end, row0, head_rows;
+  int64_t tiles;
+};
+__device__ __forceinline__ Sequence sequence_of(const Params& p, int64_t b, bool report) {
+  Sequence s;
+  int64_t cap = p.max_seq_len;
+  s.row0 = b * p.kv_heads * p.max_seq_len;
+  s.head_rows = p.max_seq_len;
+  bool bad = false;
+  if (p.seq_base) {
+    const int64_t base = lpc::ld_dep(p.seq_base + b);
+    cap = lpc::ld_dep(p.seq_cap + b);
+    s.row0 = base;
+    s.head_rows = p.total_rows;
+    if (base < 0 || cap < 0 || base + cap > p.total_rows) {
+      bad = true;
+      s.row0 = 0;
+      cap = 0;
+    }
+  }
+  s.n = lpc::ld_dep(p.seq_lens + b);
+  bad |= s.n < 0 || s.n > cap;
+  s.n = max((int64_t)0, min(s.n, cap));
+  s.end = min(s.n + p.nodes, cap);
+  s.tiles = max((int64_t)1, (s.end + KEYS - 1) / KEYS);
+  if (bad && report) atomicOr(&g_tree_status, LPC_DEV_ERR_BOUNDS);
+  return s;
+}
+
+// A CTA's stretch of tiles, walked item by item.  Every role walks it on its own.
+struct Walk {
+  const Params& p;
+  int64_t pos, stop;      // tiles of the batch still to do: [pos, stop)
+  int64_t b, base;        // the sequence that pos lies in, and its first tile
+  Sequence s;
+  // the present segment
+  int kvh, rb;            // KV head, block of rows
+  int64_t item;           // (b * kv_heads + kvh) * row_blocks + rb
+  int64_t j0;             // first tile
+  int count;              // tiles
+  bool whole;
+
+  __device__ Walk(const Params& params, int64_t at, int64_t end, int64_t seq, int64_t seq_base)
+      : p(params), pos(at), stop(end), b(seq), base(seq_base) {
+    if (pos < stop) s = sequence_of(p, b, false);
+  }
+  __device__ __forceinline__ bool next() {
+    if (pos >= stop) return false;
+    const int64_t per = s.tiles * p.kv_heads * p.row_blocks;
+    if (pos - base >= per) {  // a sequence has at least one tile
+      base += per;
+      ++b;
+      s = sequence_of(p, b, false);
+    }
+    const int64_t within = pos - base;
+    const int64_t i = within / s.tiles;
+    j0 = within - i * s.tiles;
+    kvh = (int)(i / p.row_blocks);
+    rb = (int)(i - (int64_t)kvh * p.row_blocks);
+    item = (b * p.kv_heads + kvh) * p.row_blocks + rb;
+    count = (int)min(s.tiles - j0, stop - pos);
+    whole = count == s.tiles;
+    pos += count;
+    return true;
+  }
+  // whether tile j (of the item) needs masks: it holds nodes or ends the sequence
+  __device__ __forceinline__ bool tail(int64_t j) const { return (j + 1) * KEYS > s.n; }
+  __device__ __forceinline__ int tails() const {  // such tiles in the segment
+    int c = 0;
+    for (int64_t j = j0 + count - 1; j >= j0 && tail(j); --j) ++c;
+    return c;
+  }
+};
+
+// Bits of the nodes in the cache, of `nodes` and `end - n`.
+__device__ __forceinline__ uint64_t node_bits(int64_t count) {
+  return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1ull;
+}
+
+template <typename T, int HD, bool WIDE>
+__global__ void __launch_bounds__(NTHREADS, 1)
+    tree_attention_kernel(const __grid_constant__ TmaDesc4 tmQ, const __grid_constant__ TmaDesc4 tmK,
+                          const __grid_constant__ TmaDesc4 tmV, const Params p, uint32_t idesc_qk,
+                          uint32_t idesc_pv) {
+  using S = Shape<HD, WIDE>;
+  constexpr int TILE = S::TILE, SLOTS = S::SLOTS, NBOX = HD / BOX;
+  // tiles are swizzled by their addresses' bits below 1024
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw = lpc::smem_u32(smem_raw);
+  if (raw & 1023u) {
+    atomicOr(&g_tree_status, LPC_DEV_ERR_TIMEOUT);
+    return;
+  }
+  const uint32_t sQ = raw;
+  const uint32_t sRing = raw + S::QTILES * TILE;
+  const uint32_t bars = raw + S::TILES;
+  Shared& sh = *reinterpret_cast<Shared*>(smem_raw + S::TILES + BAR_BYTES);
+  auto full = [&](uint32_t c) { return bars + 8u * (c % SLOTS); };
+  auto empty = [&](uint32_t c) { return bars + 8u * (SLOTS + c % SLOTS); };
+  auto slot_parity = [&](uint32_t c) { return (c / SLOTS) & 1u; };
+  auto slot = [&](uint32_t c) { return sRing + (c % SLOTS) * (uint32_t)TILE; };
+  const uint32_t misc = bars + 16u * SLOTS;
+  const uint32_t q_full = misc, q_empty = misc + 8u, fixed = misc + 16u;
+  const uint32_t o_free = misc + 24u, ml_full = misc + 32u;
+  auto s_full = [&](int t) { return misc + 40u + 8u * t; };
+  auto p_half = [&](int t) { return misc + 56u + 8u * t; };
+  auto p_full = [&](int t) { return misc + 72u + 8u * t; };
+  auto o_done = [&](int t) { return misc + 88u + 8u * t; };
+  const uint32_t to_fix = misc + 104u;
+  const uint32_t tmem_slot = misc + 112u;
+  volatile uint32_t* tmem_slot_ptr =
+      reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - raw));
+  static_assert(16 * SLOTS + 116 <= BAR_BYTES, "barriers");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  unsigned int* st = &g_tree_status;
+  lpc::pdl_wait();
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SLOTS; ++i) {
+      lpc::mbar_init(full(i), 1);
+      lpc::mbar_init(empty(i), 1);
+    }
+    lpc::mbar_init(q_full, 1);
+    lpc::mbar_init(q_empty, 1);
+    lpc::mbar_init(to_fix, 1);
+    lpc::mbar_init(fixed, 2);
+    lpc::mbar_init(o_free, 8);
+    lpc::mbar_init(ml_full, 8);
+    for (int t = 0; t < 2; ++t) {
+      lpc::mbar_init(s_full(t), 1);
+      lpc::mbar_init(p_half(t), 4);
+      lpc::mbar_init(p_full(t), 4);
+      lpc::mbar_init(o_done(t), 1);
+    }
+    lpc::fence_mbar_init();
+  }
+  if (warp == 8 && lane == 0) {
+    lpc::tma_prefetch_desc(&tmQ);
+    lpc::tma_prefetch_desc(&tmK);
+    lpc::tma_prefetch_desc(&tmV);
+  }
+  if (warp == 9) {
+    lpc::tmem_alloc(tmem_slot, TMEM_COLS);
+    lpc::tmem_relinquish();
+  }
+
+  // ---- this CTA's stretch: total tiles, then the sequence that its first lies in ----
+  const int64_t copies = (int64_t)p.kv_heads * p.row_blocks;  // items of a sequence
+  auto block_scan = [&](int64_t v, int64_t& total) -> int64_t {  // exclusive
+    int64_t run = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t o = __shfl_up_sync(~0u, run, d);
+      if (lane >= d) run += o;
+    }
+    if (lane == 31) sh.scan[warp] = run;
+    __syncthreads();
+    int64_t others = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < NTHREADS / 32; ++i) {
+      if (i < warp) others += sh.scan[i];
+      total += sh.scan[i];
+    }
+    __syncthreads();
+    return others + run - v;
+  };
+  int64_t all = 0, first_chunk = 0, first_before = 0;
+  for (int64_t b0 = 0; b0 < p.batch; b0 += NTHREADS) {
+    const int64_t b = b0 + threadIdx.x;
+    const int64_t mine = b < p.batch ? sequence_of(p, b, blockIdx.x == 0).tiles * copies : 0;
+    int64_t total;
+    const int64_t before = block_scan(mine, total);
+    if (b0 == 0) first_chunk = mine, first_before = before;
+    all += total;
+  }
+  const int64_t grid = gridDim.x;
+  const int64_t used = min(grid, all);  // CTAs with work
+  const int64_t c = blockIdx.x;
+  const int64_t pos = c < used ? all * c / used : 0;
+  const int64_t stop = c < used ? all * (c + 1) / used : 0;
+  if (threadIdx.x == 0) sh.found[0] = 0, sh.found[1] = 0;
+  __syncthreads();
+  int64_t upto = 0;
+  for (int64_t b0 = 0; b0 < p.batch && pos < stop; b0 += NTHREADS) {
+    const int64_t b = b0 + threadIdx.x;
+    int64_t mine = first_chunk, before = first_before, total = 0;
+    if (p.batch > NTHREADS) {
+      mine = b < p.batch ? sequence_of(p, b, false).tiles * copies : 0;
+      before = block_scan(mine, total);
+    }
+    if (upto + before <= pos && pos < upto + before + mine) {
+      sh.found[0] = b;
+      sh.found[1] = upto + before;
+    }
+    upto += total;
+  }
+  lpc::tc_fence_before();
+  __syncthreads();
+  lpc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot_ptr;
+  lpc::pdl_trigger();  // only with the tensor memory in hand: the next grid may take what is left
+  const int64_t seq = sh.found[0], seq_first = sh.found[1];
+
+  // ring places of the K and V tiles of a segment's tile i: K0 K1 V0 K2 V1 ...
+  auto k_at = [](uint32_t ring, int i) { return ring + (uint32_t)(i == 0 ? 0 : 2 * i - 1); };
+  auto v_at = [](uint32_t ring, int i, int n) {
+    return ring + (uint32_t)(i == n - 1 ? 2 * n - 1 : 2 * i + 2);
+  };
+
+  if (warp >= 8) {
+    // hands registers to the softmax warps: 128 x 96 + 256 x 200 <= 384 x 168 (the
+    // host refuses to launch with any other count)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n" ::: "memory");
+    if (warp == 8) {
+      // ---------------- loads ----------------
+      if (lane == 0) {
+        bool ok = true;
+        uint32_t issued = 0;
+        int r = 0;
+        longlong2 begun = make_longlong2(-1, -1);
+        Walk w(p, pos, stop, seq, seq_first);
+        while (ok && w.next()) {
+          if (!(ok = lpc::mbar_wait(q_empty, ((uint32_t)r & 1u) ^ 1u, st))) break;
+          lpc::mbar_arrive_expect_tx(q_full, S::QTILES * TILE);
+          for (int t = 0; t < S::QTILES; ++t)
+#pragma unroll
+            for (int h = 0; h < NBOX; ++h)
+              tma_load_4d(sQ + t * TILE + h * HALF_BYTES, &tmQ, h * BOX, w.rb * S::ITEM_ROWS + t * ROWS,
+                          (int)(w.b * p.kv_heads + w.kvh), 0, q_full);
+          const int64_t row = p.seq_base ? w.s.row0 : 0;
+          const int b4 = p.seq_base ? 0 : (int)w.b;
+          auto load = [&](const void* map, int i) -> bool {
+            if (!lpc::mbar_wait(empty(issued), slot_parity(issued) ^ 1u, st)) return false;
+            lpc::mbar_arrive_expect_tx(full(issued), TILE);
+#pragma unroll
+            for (int h = 0; h < NBOX; ++h)
+              tma_load_4d(slot(issued) + h * HALF_BYTES, map, h * BOX,
+                          (int)(row + (w.j0 + i) * KEYS), w.kvh, b4, full(issued));
+            ++issued;
+            return true;
+          };
+          ok = load(&tmK, 0);
+          for (int i = 0; i < w.count && ok; ++i) {
+            if (i + 1 < w.count) ok = load(&tmK, i + 1);
+            ok = ok && load(&tmV, i);
+          }
+          ++r;
+          if (w.j0 == 0 && !w.whole) {  // the CTA c' of tile x: all c' / used <= x, the largest
+            const int64_t x = w.pos - w.count + w.s.tiles - 1;
+            begun = make_longlong2(w.item, ((x + 1) * used - 1) / all);
+          }
+        }
+        if (p.split) p.split[c] = begun;
+        if (!ok)  // copies in flight land before the CTA ends
+          for (uint32_t x = issued > SLOTS ? issued - SLOTS : 0; x < issued; ++x)
+            lpc::mbar_wait(full(x), slot_parity(x), st);
+      }
+    } else if (warp == 9) {
+      // ---------------- tensor core ----------------
+      if (lane == 0) {
+        bool ok = true;
+        uint32_t ring = 0, done[2] = {0, 0}, fixes = 0;  // P tiles of each stream; segments with tails
+        int r = 0;
+        const uint64_t dQ = lpc::smem_desc_sw128(sQ, 16, 1024);
+        const uint64_t dK = lpc::smem_desc_sw128(sRing, 16, 1024);
+        const uint64_t dV = lpc::smem_desc_sw128(sRing, HALF_BYTES, 1024);
+        auto issue_s = [&](int t, uint32_t at, bool release) -> bool {
+          if (!lpc::mbar_wait(full(at), slot_parity(at), st)) return false;
+          lpc::tc_fence_after();
+          const uint64_t aq = dQ + (uint64_t)(((WIDE ? t : 0) * TILE) >> 4);
+          const uint64_t bk = dK + (uint64_t)(((at % SLOTS) * (uint32_t)TILE) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = (uint32_t)(((kk >> 2) * HALF_BYTES) >> 4) + 2u * (kk & 3);
+            lpc::umma_ss(tmem + 128u * t, aq + off, bk + off, idesc_qk, kk != 0);
+          }
+          lpc::umma_commit(s_full(t));
+          if (release) lpc::umma_commit(empty(at));
+          return true;
+        };
+        auto issue_pv = [&](int t, uint32_t at, bool first, bool release) -> bool {
+          const uint32_t ph = done[t]++ & 1u;
+          if (!lpc::mbar_wait(p_half(t), ph, st)) return false;
+          if (!lpc::mbar_wait(full(at), slot_parity(at), st)) return false;
+          lpc::tc_fence_after();
+          const uint64_t bv = dV + (uint64_t)(((at % SLOTS) * (uint32_t)TILE) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < KEYS / 16; ++kk) {
+            if (kk == KEYS / 32) {
+              if (!lpc::mbar_wait(p_full(t), ph, st)) return false;
+              lpc::tc_fence_after();
+            }
+            lpc::umma_ts(tmem + 256u + 128u * t, tmem + 128u * t + 8u * kk,
+                         bv + (uint64_t)((kk * 16 * 128) >> 4), idesc_pv, !first || kk != 0);
+          }
+          if (release) lpc::umma_commit(empty(at));
+          return true;
+        };
+        Walk w(p, pos, stop, seq, seq_first);
+        while (ok && w.next()) {
+          const int n = w.count;
+          if (!(ok = lpc::mbar_wait(q_full, (uint32_t)r & 1u, st))) break;
+          lpc::tc_fence_after();
+          // S of tile i; the last one of the segment releases Q
+          auto scores = [&](int t, int i) -> bool {
+            const bool last = WIDE ? t == 1 : true;
+            if (!issue_s(t, k_at(ring, i), last)) return false;
+            if (last && i == n - 1) lpc::umma_commit(q_empty);
+            return true;
+          };
+          bool clean = false;  // the segment's tails are
+          auto values = [&](int t, int i) -> bool {
+            if (!clean && w.tail(w.j0 + i)) {
+              // the last V tile is here, so the ring is in the phase that the clearing warps
+              // wait for; it goes on under the softmax
+              const uint32_t last = v_at(ring, n - 1, n);
+              if (!lpc::mbar_wait(full(last), slot_parity(last), st)) return false;
+              lpc::mbar_arrive(to_fix);
+              if (!lpc::mbar_wait(fixed, fixes & 1u, st)) return false;
+              ++fixes;
+              clean = true;
+            }
+            const bool first = WIDE ? i == 0 : i < 2;
+            if (!issue_pv(t, v_at(ring, i, n), first, WIDE ? t == 1 : true)) return false;
+            // the stream's last: O is complete
+            if (WIDE ? i == n - 1 : i + 2 >= n) lpc::umma_commit(o_done(t));
+            return true;
+          };
+          // O of the segment before has been read
+          auto o_ready = [&]() -> bool {
+            return r == 0 || lpc::mbar_wait(o_free, (uint32_t)(r - 1) & 1u, st);
+          };
+          if constexpr (WIDE) {
+            ok = scores(0, 0) && scores(1, 0) && o_ready();
+            for (int i = 0; i < n && ok; ++i) {
+              ok = values(0, i) && (i + 1 >= n || scores(0, i + 1)) && values(1, i) &&
+                   (i + 1 >= n || scores(1, i + 1));
+            }
+          } else {
+            ok = scores(0, 0) && (n < 2 || scores(1, 1)) && o_ready();
+            for (int i = 0; i < n && ok; ++i)
+              ok = values(i & 1, i) && (i + 2 >= n || scores(i & 1, i + 2));
+          }
+          ring += 2u * (uint32_t)n;
+          ++r;
+        }
+      }
+    } else {
+      // ---------------- V rows of the tiles at the end of a sequence ----------------
+      bool ok = true;
+      uint32_t ring = 0, fixes = 0;
+      Walk w(p, pos, stop, seq, seq_first);
+      while (ok && w.next()) {
+        const int tails = w.tails();
+        if (tails) {
+          // asked for only once the epilogue before has read sh.bad
+          ok = __all_sync(~0u, lpc::mbar_wait(to_fix, fixes & 1u, st));
+          if (!ok) break;
+          ++fixes;
+          uint64_t seen = 0;  // by any node
+          for (int t = lane; t < p.nodes; t += 32)
+            seen |= (uint64_t)p.masks[w.b * p.masks_stride + t];
+#pragma unroll
+          for (int m = 16; m; m >>= 1) seen |= __shfl_xor_sync(~0u, seen, m);
+          if (seen & node_bits(p.nodes) & ~node_bits(w.s.end - w.s.n) && w.kvh == 0 && w.rb == 0 &&
+              lane == 0)
+            atomicOr(&g_tree_status, LPC_DEV_ERR_BOUNDS);  // a visible node past the rows
+          seen &= node_bits(w.s.end - w.s.n);
+          uint64_t bad = 0;
+          for (int i = w.count - tails; i < w.count && ok; ++i) {
+            // both tails at most: the ring holds them side by side
+            const uint32_t at = v_at(ring, i, w.count);
+            ok = __all_sync(~0u, lpc::mbar_wait(full(at), slot_parity(at), st));
+            if (!ok) break;
+            const int64_t k0 = (w.j0 + i) * KEYS;
+            uint8_t* tile = smem_raw + (slot(at) - raw);
+            // a row a turn, half a row of boxes a lane: 16 bytes a lane
+            constexpr int LANES = HD / 8;           // lanes that hold a row
+            constexpr int AT_ONCE = 32 / LANES;     // rows a warp looks at
+            const int sub = lane / LANES, part = lane % LANES;
+            const int from = (int)max((int64_t)0, min(w.s.n - k0, (int64_t)KEYS));
+            for (int q0 = from + (warp - 10) * AT_ONCE; q0 < KEYS; q0 += 2 * AT_ONCE) {
+              const int q = q0 + sub;
+              const int64_t node = k0 + q - w.s.n;
+              uint4* x = reinterpret_cast<uint4*>(tile + (part / 8) * HALF_BYTES + q * 128) + part % 8;
+              bool clear = q < KEYS, odd = false;
+              if (q < KEYS && node < 64 && (seen >> node & 1)) {
+                const uint4 v = *x;
+                constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+                auto inf = [&](uint32_t u) {
+                  const uint32_t m = u & e;
+                  return (m & 0xffffu) == (e & 0xffffu) || (m >> 16) == (e >> 16);
+                };
+                odd = inf(v.x) || inf(v.y) || inf(v.z) || inf(v.w);
+                clear = false;
+              }
+              // the whole row goes by any of its lanes
+              const unsigned group = (LANES == 32 ? ~0u : ((1u << LANES) - 1u)) << (sub * LANES);
+              const bool any = (__ballot_sync(~0u, odd) & group) != 0;
+              if (any) {
+                clear = true;
+                bad |= 1ull << node;
+              }
+              if (clear) *x = make_uint4(0, 0, 0, 0);
+            }
+          }
+          lpc::fence_proxy_async_smem();
+#pragma unroll
+          for (int m = 16; m; m >>= 1) bad |= __shfl_xor_sync(~0u, bad, m);
+          if (lane == 0) sh.bad[warp - 10] = bad;
+          __syncwarp();
+          if (lane == 0) lpc::mbar_arrive(fixed);
+        }
+        ring += 2u * (uint32_t)w.count;
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n" ::: "memory");
+    // ---------------- softmax and epilogue of stream t ----------------
+    const int t = warp >> 2;
+    const int rr = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + 128u * t + lane_off;
+    bool ok = true;
+    uint32_t tiles_done = 0, fixes = 0, twos = 0;  // tiles; segments with tails, of both streams
+    int r = 0;
+    auto wait_warp = [&](uint32_t bar, uint32_t parity) -> bool {  // the same for the warp
+      return __all_sync(~0u, lpc::mbar_wait(bar, parity, st));
+    };
+    const int all_rows = p.group * p.nodes;
+    Walk w(p, pos, stop, seq, seq_first);
+    while (ok && w.next()) {
+      const int n = w.count;
+      const int row = w.rb * S::ITEM_ROWS + (WIDE ? t * ROWS : 0) + rr;  // of the KV head's
+      const bool valid = row < all_rows;
+      const bool busy = __any_sync(~0u, valid);  // warps of padding only keep the barriers going
+      const int head = valid ? row / p.nodes : 0, node = valid ? row - head * p.nodes : 0;
+      const uint64_t visible =
+          valid ? (uint64_t)p.masks[w.b * p.masks_stride + node] & node_bits(w.s.end - w.s.n) : 0;
+      float m_used = -INFINITY, l = 0.f;
+      const int step = WIDE ? 1 : 2;
+      int mine = 0;  // tiles of this stream so far
+      for (int i = WIDE ? 0 : t; i < n; i += step, ++mine) {
+        const uint32_t ph = (tiles_done + (uint32_t)mine) & 1u;
+        if (!(ok = wait_warp(s_full(t), ph))) break;
+        if (!busy) {
+          if (lane == 0) {
+            lpc::mbar_arrive(p_half(t));
+            lpc::mbar_arrive(p_full(t));
+          }
+          continue;
+        }
+        lpc::tc_fence_after();
+        uint32_t sv[KEYS];
+#pragma unroll
+        for (int cc = 0; cc < KEYS; cc += 32)
+          lpc::tmem_ld32(tS + cc, *reinterpret_cast<uint32_t(*)[32]>(&sv[cc]));
+        lpc::tmem_wait_ld();
+        if (w.tail(w.j0 + i)) {
+          // bits of the tile's keys that this row sees: context below `rel`, nodes from it
+          const int64_t rel64 = w.s.n - (w.j0 + i) * KEYS;  // in (-64, 128)
+          const int rel = (int)max((int64_t)-64, rel64);
+          uint32_t see[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int sh = 32 * x - rel;  // bit 0 of the word is node sh
+            uint32_t bits = sh >= 64 ? 0u : sh >= 0 ? (uint32_t)(visible >> sh)
+                            : sh > -32 ? (uint32_t)visible << -sh : 0u;
+            const int ctx = rel - 32 * x;  // keys of the word that are context
+            bits |= ctx >= 32 ? ~0u : ctx > 0 ? (1u << ctx) - 1u : 0u;
+            see[x] = bits;
+          }
+#pragma unroll
+          for (int q = 0; q < KEYS; ++q)
+            if (!(see[q >> 5] >> (q & 31) & 1u)) sv[q] = 0xff800000u;  // -inf
+        }
+        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < KEYS; q += 8) {
+          m0 = max3(m0, __uint_as_float(sv[q]), __uint_as_float(sv[q + 1]));
+          m1 = max3(m1, __uint_as_float(sv[q + 2]), __uint_as_float(sv[q + 3]));
+          m2 = max3(m2, __uint_as_float(sv[q + 4]), __uint_as_float(sv[q + 5]));
+          m3 = max3(m3, __uint_as_float(sv[q + 6]), __uint_as_float(sv[q + 7]));
+        }
+        const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * p.scale_log2;  // scale > 0
+        // S of this tile was issued after PV of the stream's tile before: O is stable
+        const bool grow = top > m_used + GROWTH || (m_used == -INFINITY && top > -INFINITY);
+        if (__any_sync(~0u, grow)) {
+          float alpha = 1.f;
+          if (grow) {
+            alpha = m_used == -INFINITY ? 0.f : fast_exp2(m_used - top);
+            m_used = top;
+            l *= alpha;
+          }
+          if (mine > 0) {
+            const uint32_t tO = tmem + 256u + 128u * t + lane_off;
+#pragma unroll 1
+            for (int cc = 0; cc < HD; cc += 16) {
+              uint32_t v[16];
+              lpc::tmem_ld16(tO + cc, v);
+              lpc::tmem_wait_ld();
+#pragma unroll
+              for (int q = 0; q < 16; ++q) v[q] = __float_as_uint(__uint_as_float(v[q]) * alpha);
+              lpc::tmem_st16(tO + cc, v);
+            }
+          }
+        }
+        const float m_use = m_used == -INFINITY ? 0.f : m_used;
+        const uint64_t sc2 = pack_f2(p.scale_log2, p.scale_log2), nm2 = pack_f2(-m_use, -m_use);
+        uint64_t rsa = 0, rsb = 0;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[KEYS / 4];
+#pragma unroll
+          for (int q = 0; q < KEYS / 2; q += 2) {
+            const int at = half * (KEYS / 2) + q;
+            const uint64_t x = fma_f2(pack_f2(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])),
+                                      sc2, nm2);
+            const uint64_t e = pack_f2(fast_exp2(lo_f(x)), fast_exp2(hi_f(x)));
+            if ((q >> 1) & 1) rsb = add_f2(rsb, e);
+            else rsa = add_f2(rsa, e);
+            pk[q >> 1] = pack2<T>(lo_f(e), hi_f(e));
+          }
+#pragma unroll
+          for (int cc = 0; cc < KEYS / 4; cc += 16)
+            lpc::tmem_st16(tS + (uint32_t)(half * (KEYS / 4) + cc),
+                           *reinterpret_cast<uint32_t(*)[16]>(&pk[cc]));
+          lpc::tmem_wait_st();
+          lpc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) lpc::mbar_arrive(half ? p_full(t) : p_half(t));
+        }
+        const uint64_t rs2 = add_f2(rsa, rsb);
+        l += lo_f(rs2) + hi_f(rs2);
+      }
+      tiles_done += (uint32_t)mine;
+      if (!ok) break;
+
+      // ---- epilogue ----
+      const bool two = !WIDE && n > 1;  // both streams have part of these rows
+      float M = m_used, L = l, a0 = 1.f, a1 = 0.f;
+      if constexpr (!WIDE) {
+        // the segment before has been read
+        if (r > 0 && !(ok = wait_warp(o_free, (uint32_t)(r - 1) & 1u))) break;
+        sh.ml[t][rr] = make_float2(m_used, l);
+        __syncwarp();
+        if (lane == 0) lpc::mbar_arrive(ml_full);
+        if (!(ok = wait_warp(ml_full, (uint32_t)r & 1u))) break;
+        const float2 x0 = sh.ml[0][rr], x1 = sh.ml[1][rr];
+        M = fmaxf(x0.x, x1.x);
+        const float mu = M == -INFINITY ? 0.f : M;
+        a0 = fast_exp2(x0.x - mu);
+        a1 = two ? fast_exp2(x1.x - mu) : 0.f;
+        L = x0.y * a0 + (two ? x1.y * a1 : 0.f);
+      }
+      unsigned long long bad = 0;
+      if (w.tails()) {
+        if (!(ok = wait_warp(fixed, fixes & 1u))) break;
+        ++fixes;
+        bad = (*(volatile unsigned long long*)&sh.bad[0] | *(volatile unsigned long long*)&sh.bad[1]) &
+              visible;
+      }
+      // narrow: both streams' O, columns shared out to the two warpgroups
+      if (!(ok = wait_warp(o_done(WIDE ? t : 0), (uint32_t)r & 1u))) break;
+      if (two) {
+        if (!(ok = wait_warp(o_done(1), twos & 1u))) break;
+        ++twos;
+      }
+      lpc::tc_fence_after();
+      if (busy) {
+        const uint32_t tO0 = tmem + 256u + (WIDE ? 128u * t : 0u) + lane_off;
+        constexpr int COLS = WIDE ? HD : HD / 2;
+        const int col0 = WIDE ? 0 : t * COLS;
+        const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+        float* part = p.parts + (2 * c + (w.j0 == 0 ? 1 : 0)) * S::PART;
+        const int prow = (WIDE ? t * ROWS : 0) + rr;
+        T* orow = static_cast<T*>(p.out) +
+                  ((w.b * p.nodes + node) * p.heads + (int64_t)w.kvh * p.group + head) * p.head_dim;
+#pragma unroll 1
+        for (int cc = 0; cc < COLS; cc += 16) {
+          uint32_t v[16];
+          float o[16];
+          __syncwarp();  // rows part below; the reads are the whole warp's
+          lpc::tmem_ld16(tO0 + col0 + cc, v);
+          lpc::tmem_wait_ld();
+#pragma unroll
+          for (int q = 0; q < 16; ++q) o[q] = __uint_as_float(v[q]);
+          if (two) {
+            lpc::tmem_ld16(tO0 + 128u + col0 + cc, v);
+            lpc::tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 16; ++q) o[q] = o[q] * a0 + __uint_as_float(v[q]) * a1;
+          }
+          if (!valid) continue;
+          if (bad && col0 + cc < p.head_dim) {
+            // visible V rows that are not finite: cleared in the tile, added here
+            for (unsigned long long left = bad; left; left &= left - 1) {
+              const int j = __ffsll((long long)left) - 1;
+              const int64_t krow = (w.s.row0 + (int64_t)w.kvh * w.s.head_rows + w.s.n + j) * p.head_dim;
+              const int64_t at = (j + w.s.n) / KEYS;
+              if (at < w.j0 || at >= w.j0 + n) continue;  // in another part of the item
+              const T* kr = static_cast<const T*>(p.k) + krow;
+              const T* vr = static_cast<const T*>(p.v) + krow;
+              const T* qr = static_cast<const T*>(p.q) +
+                            ((w.b * p.kv_heads + w.kvh) * all_rows + row) * p.head_dim;
+              float dot = 0.f;
+              for (int d = 0; d < p.head_dim; ++d)
+                dot = fmaf(Num<T>::to_f(qr[d]), Num<T>::to_f(kr[d]), dot);
+              const float pj = fast_exp2(dot * p.scale_log2 - (M == -INFINITY ? 0.f : M));
+#pragma unroll
+              for (int q = 0; q < 16; ++q) o[q] = fmaf(pj, Num<T>::to_f(vr[col0 + cc + q]), o[q]);
+            }
+          }
+          if (w.whole) {
+            if (col0 + cc < p.head_dim) {
+              uint32_t pk[8];
+#pragma unroll
+              for (int q = 0; q < 16; q += 2) pk[q >> 1] = pack2<T>(o[q] * inv, o[q + 1] * inv);
+              uint4* dst = reinterpret_cast<uint4*>(orow + col0 + cc);
+              dst[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              dst[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+            }
+          } else {
+            // [four columns][row]: a warp's rows are 512 bytes side by side
+            float4* dst = reinterpret_cast<float4*>(part) + (int64_t)((col0 + cc) / 4) * S::ITEM_ROWS + prow;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              dst[q * S::ITEM_ROWS] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          }
+        }
+        if (valid && !w.whole && (WIDE || t == 0))
+          reinterpret_cast<float2*>(part + (int64_t)S::ITEM_ROWS * HD)[prow] = make_float2(M, L);
+      }
+      lpc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) lpc::mbar_arrive(o_free);
+      ++r;
+    }
+  }
+  lpc::tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    lpc::tc_fence_after();
+    lpc::tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Joins the parts of the item that CTA blockIdx.x began: its own second part and the
+// first part of each CTA after it up to the last.  A thread has four columns of a
+// row; a warp reads 8 rows side by side.
+template <typename T, int HD, bool WIDE>
+__global__ void __launch_bounds__(256) tree_join_kernel(const Params p) {
+  using S = Shape<HD, WIDE>;
+  constexpr int GROUPS = HD / 4, ROWS_HERE = 256 / GROUPS;
+  lpc::pdl_trigger();
+  lpc::pdl_wait();
+  const int64_t c0 = blockIdx.x;
+  const int64_t item = lpc::ld_dep(reinterpret_cast<const int64_t*>(&p.split[c0].x));
+  if (item < 0) return;
+  const int64_t last = lpc::ld_dep(reinterpret_cast<const int64_t*>(&p.split[c0].y));
+  const int rb = (int)(item % p.row_blocks);
+  const int64_t pair = item / p.row_blocks, b = pair / p.kv_heads;
+  const int kvh = (int)(pair - b * p.kv_heads);
+  const int prow = (int)blockIdx.y * ROWS_HERE + (int)threadIdx.x % ROWS_HERE;
+  const int group = (int)threadIdx.x / ROWS_HERE;
+  const int row = rb * S::ITEM_ROWS + prow;
+  if (prow >= S::ITEM_ROWS || row >= p.group * p.nodes || 4 * group >= p.head_dim) return;
+  auto part = [&](int64_t c) { return p.parts + (2 * c + (c == c0 ? 1 : 0)) * S::PART; };
+  auto stats = [&](int64_t c) {
+    return reinterpret_cast<const float2*>(part(c) + (int64_t)S::ITEM_ROWS * HD)[prow];
+  };
+  float M = -INFINITY;
+#pragma unroll 4
+  for (int64_t c = c0; c <= last; ++c) M = fmaxf(M, stats(c).x);
+  const float mu = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int64_t c = c0; c <= last; ++c) {
+    const float2 x = stats(c);
+    const float4 v = reinterpret_cast<const float4*>(part(c))[(int64_t)group * S::ITEM_ROWS + prow];
+    const float f = fast_exp2(x.x - mu);
+    L = fmaf(f, x.y, L);
+    o.x = fmaf(f, v.x, o.x);
+    o.y = fmaf(f, v.y, o.y);
+    o.z = fmaf(f, v.z, o.z);
+    o.w = fmaf(f, v.w, o.w);
+  }
+  const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+  const int head = row / p.nodes, node = row - head * p.nodes;
+  T* out = static_cast<T*>(p.out) +
+           ((b * p.nodes + node) * p.heads + (int64_t)kvh * p.group + head) * p.head_dim + 4 * group;
+  *reinterpret_cast<uint2*>(out) =
+      make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+}
+
+// CTAs of a call: one an SM, no more than there can be tiles.
+int64_t grid_of(int64_t batch, int64_t items_a_sequence, int64_t max_seq_len, int64_t total_rows,
+                int sms) {
+  const int64_t tiles = total_rows > 0 ? total_rows / KEYS + batch
+                                       : batch * ((max_seq_len + KEYS - 1) / KEYS);
+  return std::min<int64_t>(sms, tiles * items_a_sequence);
+}
+
+bool sizes_ok(int64_t batch, int64_t nodes, int heads, int kv_heads, int head_dim,
+              int64_t max_seq_len, int64_t total_rows) {
+  return batch >= 0 && batch <= 65535 && nodes >= 1 && nodes <= MAX_NODES && heads > 0 &&
+         heads <= 65535 && kv_heads > 0 && heads % kv_heads == 0 &&
+         (head_dim == 32 || head_dim == 64 || head_dim == 128) &&
+         (total_rows > 0 ? total_rows <= 0x7fffffffLL - KEYS
+                         : max_seq_len > 0 && max_seq_len <= 0x7fffffffLL - KEYS);
+}
+
+struct Plan {
+  bool wide;
+  int row_blocks;
+  int64_t grid, part_floats;
+  bool join;  // some item may have more than one tile
+};
+Plan plan_of(int64_t batch, int64_t nodes, int heads, int kv_heads, int head_dim,
+             int64_t max_seq_len, int64_t total_rows) {
+  Plan x;
+  const int64_t rows = (int64_t)(heads / kv_heads) * nodes;
+  x.wide = rows > ROWS;
+  const int item_rows = x.wide ? 2 * ROWS : ROWS;
+  x.row_blocks = (int)((rows + item_rows - 1) / item_rows);
+  x.grid = grid_of(batch, (int64_t)kv_heads * x.row_blocks, max_seq_len, total_rows,
+                   lpc::current_device_sms());
+  x.part_floats = (int64_t)item_rows * ((head_dim == 128 ? 128 : 64) + 2);
+  x.join = (total_rows > 0 ? total_rows : max_seq_len) > KEYS;
+  return x;
+}
+
+template <typename T, int HD, bool WIDE>
+int launch(const TmaDesc4& tq, const TmaDesc4& tk, const TmaDesc4& tv, const Params& p,
+           const Plan& plan, uint32_t id_qk, uint32_t id_pv, cudaStream_t s) {
+  using S = Shape<HD, WIDE>;
+  static std::atomic<int> regs{0};
+  int have = regs.load(std::memory_order_relaxed);
+  if (have == 0) {
+    cudaFuncAttributes fa;
+    have = cudaFuncGetAttributes(&fa, tree_attention_kernel<T, HD, WIDE>) == cudaSuccess ? fa.numRegs
+                                                                                         : -1;
+    regs.store(have, std::memory_order_relaxed);
+  }
+  if (have != LAUNCH_REGS) {
+    lpc::set_error("tree_attention: kernel built with %d registers per thread, its register split "
+                   "needs %d", have, LAUNCH_REGS);
+    return LPC_ERR_UNSUPPORTED;
+  }
+  static std::atomic<uint64_t> mask{0};
+  if (int rc = lpc::once_per_device_smem((const void*)tree_attention_kernel<T, HD, WIDE>, S::SMEM, mask))
+    return rc;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)plan.grid);
+  cfg.blockDim = dim3(NTHREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, tree_attention_kernel<T, HD, WIDE>, tq, tk, tv, p, id_qk,
+                                     id_pv);
+  if (e == cudaSuccess && plan.join) {
+    constexpr int rows_here = 256 / (HD / 4);
+    const int rows = std::min(p.group * p.nodes, S::ITEM_ROWS);
+    cfg.gridDim = dim3((unsigned)plan.grid, (unsigned)((rows + rows_here - 1) / rows_here));
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, tree_join_kernel<T, HD, WIDE>, p);
+  }
+  if (e != cudaSuccess) {
+    lpc::set_error("tree_attention: launch failed: %s", cudaGetErrorString(e));
+    return LPC_ERR_CUDA;
+  }
+  return lpc::check_launch("tree_attention");
+}
+
+template <typename T>
+int launch_t(const TmaDesc4& tq, const TmaDesc4& tk, const TmaDesc4& tv, const Params& p,
+             const Plan& plan, uint32_t fmt, cudaStream_t s) {
+  const int hd = p.head_dim == 128 ? 128 : 64;
+  const uint32_t qk = lpc::idesc_f16(fmt, ROWS, KEYS, 0u, 0u);
+  const uint32_t pv = lpc::idesc_f16(fmt, ROWS, (uint32_t)hd, 0u, 1u);
+  if (hd == 128)
+    return plan.wide ? launch<T, 128, true>(tq, tk, tv, p, plan, qk, pv, s)
+                     : launch<T, 128, false>(tq, tk, tv, p, plan, qk, pv, s);
+  return plan.wide ? launch<T, 64, true>(tq, tk, tv, p, plan, qk, pv, s)
+                   : launch<T, 64, false>(tq, tk, tv, p, plan, qk, pv, s);
+}
+
+}  // namespace
+
+extern "C" int64_t lpc_tree_attention_workspace_bytes(int64_t batch, int nodes, int heads,
+                                                      int kv_heads, int head_dim,
+                                                      int64_t max_seq_len, int64_t total_rows) {
+  if (!sizes_ok(batch, nodes, heads, kv_heads, head_dim, max_seq_len, total_rows) || batch == 0)
+    return 0;
+  const Plan x = plan_of(batch, nodes, heads, kv_heads, head_dim, max_seq_len, total_rows);
+  return x.join ? x.grid * (2 * x.part_floats * 4 + 16) : 0;
+}
+
+extern "C" int lpc_tree_attention(const void* q, const void* key_cache, const void* value_cache,
+                                  const int32_t* seq_lens, const int64_t* masks,
+                                  int64_t masks_stride, const int64_t* seq_base,
+                                  const int32_t* seq_cap, void* out, void* workspace,
+                                  int64_t workspace_bytes, int64_t batch, int nodes, int heads,
+                                  int kv_heads, int head_dim, int64_t max_batch,
+                                  int64_t max_seq_len, int64_t total_rows, float sm_scale,
+                                  int dtype, void* stream) {
+  using namespace lpc;
+  if (dtype != LPC_DTYPE_BF16 && dtype != LPC_DTYPE_F16) {
+    set_error("tree_attention: only bf16 and fp16 are supported");
+    return LPC_ERR_UNSUPPORTED;
+  }
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128) {
+    set_error("tree_attention: head_dim must be 32, 64 or 128, got %d", head_dim);
+    return LPC_ERR_UNSUPPORTED;
+  }
+  if ((seq_base != nullptr) != (seq_cap != nullptr) || (seq_base != nullptr) != (total_rows > 0)) {
+    set_error("tree_attention: a ragged cache has seq_base, seq_cap and total_rows");
+    return LPC_ERR_INVALID;
+  }
+  if (!sizes_ok(batch, nodes, heads, kv_heads, head_dim, max_seq_len, total_rows) ||
+      (masks_stride != 0 && masks_stride < nodes) || (!seq_base && batch > max_batch)) {
+    set_error("tree_attention: invalid sizes (batch=%lld of %lld, nodes=%d, heads=%d, kv_heads=%d, "
+              "max_seq_len=%lld, total_rows=%lld; 1 to %d nodes)", (long long)batch,
+              (long long)max_batch, nodes, heads, kv_heads, (long long)max_seq_len,
+              (long long)total_rows, MAX_NODES);
+    return LPC_ERR_INVALID;
+  }
+  if (!(sm_scale > 0.f && sm_scale < INFINITY)) {
+    set_error("tree_attention: sm_scale must be positive");
+    return LPC_ERR_INVALID;
+  }
+  if (batch == 0) return LPC_OK;
+  if (!q || !key_cache || !value_cache || !seq_lens || !masks || !out) {
+    set_error("tree_attention: null pointer");
+    return LPC_ERR_INVALID;
+  }
+  if (!aligned16(q) || !aligned16(key_cache) || !aligned16(value_cache) || !aligned16(out)) {
+    set_error("tree_attention: tensors must be 16-byte aligned");
+    return LPC_ERR_INVALID;
+  }
+  const Plan plan = plan_of(batch, nodes, heads, kv_heads, head_dim, max_seq_len, total_rows);
+  const int64_t need = plan.join ? plan.grid * (2 * plan.part_floats * 4 + 16) : 0;
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
+    set_error("tree_attention: workspace of %lld bytes required, got %lld", (long long)need,
+              (long long)workspace_bytes);
+    return LPC_ERR_INVALID;
+  }
+  Params p;
+  p.q = q;
+  p.k = key_cache;
+  p.v = value_cache;
+  p.out = out;
+  p.seq_lens = seq_lens;
+  p.masks = masks;
+  p.masks_stride = masks_stride;
+  p.seq_base = seq_base;
+  p.seq_cap = seq_cap;
+  p.max_seq_len = max_seq_len;
+  p.total_rows = total_rows;
+  p.split = plan.join ? static_cast<longlong2*>(workspace) : nullptr;
+  p.parts = plan.join ? reinterpret_cast<float*>(p.split + plan.grid) : nullptr;
+  p.batch = batch;
+  p.nodes = nodes;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.group = heads / kv_heads;
+  p.head_dim = head_dim;
+  p.row_blocks = plan.row_blocks;
+  p.scale_log2 = sm_scale * LOG2E;
+  TmaDesc4 tq, tk, tv;
+  const uint64_t rowb = (uint64_t)head_dim * 2;
+  const uint32_t box[4] = {BOX, 128, 1, 1};
+  {
+    const uint64_t rows = (uint64_t)p.group * nodes, pairs = (uint64_t)batch * kv_heads;
+    const uint64_t dims[4] = {(uint64_t)head_dim, rows, pairs, 1};
+    const uint64_t str[3] = {rowb, rowb * rows, rowb * rows * pairs};
+    if (int rc = make_tma_nd(reinterpret_cast<TmaDesc*>(&tq), q, dtype, 4, dims, str, box, true))
+      return rc;
+  }
+  {
+    const uint64_t rows = (uint64_t)(seq_base ? total_rows : max_seq_len);
+    const uint64_t dims[4] = {(uint64_t)head_dim, rows, (uint64_t)kv_heads,
+                              (uint64_t)(seq_base ? 1 : max_batch)};
+    const uint64_t str[3] = {rowb, rowb * rows, rowb * rows * kv_heads};
+    if (int rc = make_tma_nd(reinterpret_cast<TmaDesc*>(&tk), key_cache, dtype, 4, dims, str, box, true))
+      return rc;
+    if (int rc = make_tma_nd(reinterpret_cast<TmaDesc*>(&tv), value_cache, dtype, 4, dims, str, box, true))
+      return rc;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == LPC_DTYPE_BF16) return launch_t<__nv_bfloat16>(tq, tk, tv, p, plan, 1u, s);
+  return launch_t<__half>(tq, tk, tv, p, plan, 0u, s);
+}

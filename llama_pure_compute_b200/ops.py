@@ -47,6 +47,8 @@ __all__ = [
     "kv_read_int4",
     "sample_tokens",
     "rope_kv_append_tree",
+    "tree_attention",
+    "tree_attention_workspace",
     "LayerCaches",
     "tree_accept",
 ]
@@ -1151,6 +1153,92 @@ def rope_kv_append_tree(
     if B and T:
         _lib.launch_count += 1
     return q_out
+
+
+def _tree_attention_bytes(B: int, T: int, H: int, key_cache: torch.Tensor) -> int:
+    shape = key_cache.shape
+    if len(shape) == 4:
+        return _lib.load().lpc_tree_attention_workspace_bytes(B, T, H, shape[1], shape[3], shape[2], 0)
+    return _lib.load().lpc_tree_attention_workspace_bytes(B, T, H, shape[0], shape[2], 0, shape[1])
+
+
+def tree_attention_workspace(q: torch.Tensor, key_cache: torch.Tensor) -> torch.Tensor:
+    """Workspace for ``tree_attention`` calls with q [B, H, T, D] and caches of
+    these shapes.  Calls that may overlap (other streams, other graphs) need one
+    each."""
+    _require_cuda(q, "q")
+    if q.dim() != 4 or key_cache.dim() not in (3, 4):
+        raise ValueError("LlamaPureComputeError: q must be [B, H, T, D], caches [B, H, S, D] or "
+                         "[H, rows, D].")
+    with torch.cuda.device(q.device):
+        n = _tree_attention_bytes(q.shape[0], q.shape[2], q.shape[1], key_cache)
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
+
+
+def tree_attention(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    seq_lens: torch.Tensor,
+    masks: torch.Tensor,
+    sm_scale: Optional[float] = None,
+    seq_base: Optional[torch.Tensor] = None,
+    seq_cap: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of a drafted tree a sequence over its cache, whose rows
+    ``seq_lens[b] + t`` hold the nodes (``rope_kv_append_tree``): node t of q
+    [B, H, T, D] sees the ``seq_lens[b]`` keys before the tree and the nodes i
+    whose bit i is set in ``masks[b, t]`` (int64 [B, T], or [T] for one tree; its
+    own bit is not implied).  Caches dense [max_batch, Hkv, S, D] or, with
+    ``seq_base`` and ``seq_cap``, ragged [Hkv, rows, D]; bf16 or fp16, D 32, 64 or
+    128, any number of query heads a KV head.
+
+    Softmax statistics and sums in fp32, weights rounded to the data type before
+    they meet V.  What a node does not see does not reach it, whatever those rows
+    hold; a node that sees nothing gives zeros.  A length beyond the sequence's
+    rows is cut to them, which, as a visible node past them, sets the device
+    status.  ``sm_scale`` (positive) defaults to ``D ** -0.5``.
+
+    Returns [B, H, T, D], in the memory of a contiguous [B, T, H, D]: the output
+    projection reads it as it is."""
+    index, shape = q.get_device(), q.shape
+    if index < 0 or masks.get_device() != index:
+        _require_cuda(q, "q")
+        _require_cuda(masks, "masks")
+        raise ValueError("LlamaPureComputeError: q and masks must be on one device.")
+    if len(shape) != 4:
+        raise ValueError("LlamaPureComputeError: q must be [B, H, T, D].")
+    B, H, T, D = shape
+    if not 1 <= T <= MAX_TREE_NODES:
+        raise ValueError(f"LlamaPureComputeError: a tree has 1 to {MAX_TREE_NODES} nodes.")
+    kv_heads, dim, max_batch, max_seq_len, total_rows = _tree_caches(key_cache, value_cache, seq_base,
+                                                                     seq_cap, B, index)
+    if dim != D or D not in (32, 64, 128):
+        raise ValueError("LlamaPureComputeError: q must have the caches' head_dim; 32, 64 or 128.")
+    if H == 0 or kv_heads == 0 or H % kv_heads:
+        raise ValueError("LlamaPureComputeError: heads must be a multiple of the caches' KV heads.")
+    if q.dtype != key_cache.dtype:
+        raise TypeError("LlamaPureComputeError: q and cache dtypes differ.")
+    code = _lib.dtype_code(q.dtype, "tree_attention")
+    _tree_lens(seq_lens, B, index)
+    masks, masks_stride = _tree_ints(masks, "masks", B, T, index, torch.int64)
+    q = _dense16(q)
+    out = q.new_empty(B, T, H, D)
+    if workspace is None:
+        workspace = tree_attention_workspace(q, key_cache)
+    elif workspace.get_device() != index or not workspace.is_contiguous():
+        raise ValueError("LlamaPureComputeError: workspace must be contiguous on q's device.")
+    rc = _lib.call_on(index, _lib.load().lpc_tree_attention, q.data_ptr(), key_cache.data_ptr(),
+                      value_cache.data_ptr(), seq_lens.data_ptr(), masks.data_ptr(), masks_stride,
+                      _lib.ptr(seq_base), _lib.ptr(seq_cap), out.data_ptr(), workspace.data_ptr(),
+                      workspace.nbytes, B, T, H, kv_heads, D, max_batch, max_seq_len, total_rows,
+                      D ** -0.5 if sm_scale is None else sm_scale, code)
+    if rc:
+        _lib.check(rc, "tree_attention")
+    if B:
+        _lib.launch_count += 2 if (total_rows or max_seq_len) > 128 else 1
+    return out.transpose(1, 2)
 
 
 class LayerCaches:

@@ -41,21 +41,23 @@ def tree_masks_ref(parents: Sequence[int]) -> Tuple[List[int], List[int]]:
     return [m - (1 << 64) if m >> 63 else m for m in masks], depths
 
 
-def tree_attention_ref(q, k, v, n: int, masks, scale: float) -> torch.Tensor:
+def tree_attention_ref(q, k, v, n: int, masks, scale: float) -> Tuple[torch.Tensor, torch.Tensor]:
     """One sequence: q [H, T, D], k and v [Hkv, >= n + T, D] (rows of the cache), masks int64 [T].
-    Rows that nothing sees take no part, whatever they hold."""
+    Returns the output [H, T, D] and the same with |v| for v, which bounds what a relative error
+    of the weights does to it.  Rows that a node does not see take no part, whatever they hold."""
     heads, nodes, dim = q.shape
-    group = heads // k.shape[0]
-    out = torch.zeros(heads, nodes, dim, dtype=torch.float64)
-    q, k, v = (t.detach().cpu().double() for t in (q, k, v))
+    kv = k.shape[0]
+    out = torch.zeros(2, heads, nodes, dim, dtype=torch.float64, device=q.device)
+    q, k, v = q.double().view(kv, heads // kv, nodes, dim), k.double(), v.double()
+    masks = [int(m) for m in masks]
     for t in range(nodes):
-        rows = list(range(n)) + [n + i for i in range(nodes) if int(masks[t]) >> i & 1]
-        if not rows:
-            continue
-        for h in range(heads):
-            s = k[h // group, rows] @ q[h, t] * scale
-            out[h, t] = torch.softmax(s, 0) @ v[h // group, rows]
-    return out
+        rows = list(range(n)) + [n + i for i in range(nodes) if masks[t] >> i & 1]
+        if rows:
+            s = torch.einsum("hgd,hrd->hgr", q[:, :, t], k[:, rows]) * scale
+            p = torch.softmax(s, -1)
+            for o, x in zip(out, (v, v.abs())):
+                o[:, t] = torch.einsum("hgr,hrd->hgd", p, x[:, rows]).reshape(heads, dim)
+    return out[0], out[1]
 
 
 def accept_ref(drafted: Sequence[int], parents: Sequence[int], sampled: Sequence[int]):
