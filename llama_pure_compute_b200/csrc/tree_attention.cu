@@ -10,11 +10,11 @@
 // block of 128 or 256 rows).  Up to ~250 rows a key's bytes cost more than its
 // arithmetic (2 G T flops a byte of K and V), beyond it the tensor cores do.
 //
-// Schedule.  Every item is a row of 128-key tiles.  The tiles of all items, one
-// after another, are cut into equal stretches, one a CTA and one CTA an SM, from
-// the lengths as the device holds them: ragged batches are balanced and one long
-// sequence fills the GPU.  A CTA that holds a whole item writes its output; parts
-// of items go to a workspace (at most two a CTA, whatever the lengths) and a
+// Schedule.  Every item is a row of 128-key tiles behind START tiles' worth of set-up.
+// The items, one after another, are cut into equal stretches, one a CTA and one CTA
+// an SM, from the lengths as the device holds them: ragged batches are balanced and
+// one long sequence fills the GPU.  A CTA that holds a whole item writes its output;
+// parts of items go to a workspace (at most two a CTA, whatever the lengths) and a
 // second kernel joins them.
 //
 // CTA, 12 warps:
@@ -72,22 +72,33 @@ constexpr int LAUNCH_REGS = 168, REGS_LOAD = 96, REGS_SOFTMAX = 200;
 static_assert(128 * REGS_LOAD + 256 * REGS_SOFTMAX <= NTHREADS * LAUNCH_REGS,
               "register split exceeds the block's launch allocation");
 
+constexpr int START = 2;                    // tiles that an item's begin and end cost
+
+// What a sequence holds: n keys of context, keys and nodes together up to `end`,
+// `tiles` of them; its cache row 0 (of KV head 0).
+struct Sequence {
+  int64_t row0;
+  int n, end, tiles, pad;
+};
+constexpr int KNOWN = 16;       // sequences from a CTA's first on that it keeps
 struct Shared {
   float2 ml[2][ROWS];           // [stream][row]: maximum and sum, up to 128 rows
-  int64_t scan[NTHREADS / 32];
-  int64_t found[2];
+  Sequence known[KNOWN];
   unsigned long long bad[2];    // visible nodes of the segment whose V is not finite
+  uint32_t scan[NTHREADS / 32];
+  uint32_t found[2];
 };
-constexpr int BAR_BYTES = 384;
+constexpr int BAR_BYTES = 336;
 
 // HD: columns as the MMA sees them, 64 (head_dim 32 or 64) or 128.  WIDE: 256 rows an item.
 template <int HD, bool WIDE>
 struct Shape {
   static constexpr int TILE = HD / BOX * HALF_BYTES;         // K, V or Q tile
-  static constexpr int QTILES = WIDE ? 2 : 1;
+  static constexpr int QTILES = WIDE ? 2 : 1;                // of an item
+  static constexpr int QBUFS = WIDE ? 1 : 2;                 // items whose Q is held
   static constexpr int ITEM_ROWS = QTILES * ROWS;
-  static constexpr int SLOTS = (14 * HALF_BYTES - QTILES * TILE) / TILE;  // 224 KB with Q
-  static constexpr int TILES = (QTILES + SLOTS) * TILE;
+  static constexpr int SLOTS = (14 * HALF_BYTES - QTILES * QBUFS * TILE) / TILE;  // 224 KB with Q
+  static constexpr int TILES = (QTILES * QBUFS + SLOTS) * TILE;
   static constexpr int SMEM = TILES + BAR_BYTES + (int)sizeof(Shared);
   static constexpr int64_t PART = (int64_t)ITEM_ROWS * (HD + 2);  // floats of a part
 };
@@ -150,92 +161,99 @@ struct Params {
   const int32_t* seq_cap;
   int64_t max_seq_len, total_rows;
   float* parts;                // 2 a CTA
-  longlong2* split;            // the item that a CTA begins and does not finish (-1: none),
+  int2* split;                 // the item that a CTA begins and does not finish (-1: none),
                                // and the last CTA that has a part of it
-  int64_t batch;
-  int nodes, heads, kv_heads, group, head_dim, row_blocks;
+  int batch, nodes, heads, kv_heads, group, head_dim, row_blocks;
   float scale_log2;
 };
 
-// What a sequence holds: n keys of context, keys and nodes together up to `end`,
-// `tiles` of them; cache row of KV head 0 and the distance between KV heads.
-struct Sequence {
-  int64_t n, end, row0, head_rows;
-  int64_t tiles;
-};
-__device__ __forceinline__ Sequence sequence_of(const Params& p, int64_t b, bool report) {
+__device__ __forceinline__ Sequence sequence_of(const Params& p, int b, bool report) {
   Sequence s;
   int64_t cap = p.max_seq_len;
-  s.row0 = b * p.kv_heads * p.max_seq_len;
-  s.head_rows = p.max_seq_len;
+  s.row0 = (int64_t)b * p.kv_heads * p.max_seq_len;
   bool bad = false;
+  int n = lpc::ld_dep(p.seq_lens + b);
   if (p.seq_base) {
-    const int64_t base = lpc::ld_dep(p.seq_base + b);
+    s.row0 = lpc::ld_dep(p.seq_base + b);
     cap = lpc::ld_dep(p.seq_cap + b);
-    s.row0 = base;
-    s.head_rows = p.total_rows;
-    if (base < 0 || cap < 0 || base + cap > p.total_rows) {
+    if (s.row0 < 0 || cap < 0 || s.row0 + cap > p.total_rows) {
       bad = true;
       s.row0 = 0;
       cap = 0;
     }
   }
-  s.n = lpc::ld_dep(p.seq_lens + b);
-  bad |= s.n < 0 || s.n > cap;
-  s.n = max((int64_t)0, min(s.n, cap));
-  s.end = min(s.n + p.nodes, cap);
-  s.tiles = max((int64_t)1, (s.end + KEYS - 1) / KEYS);
+  bad |= n < 0 || n > cap;
+  s.n = max(0, min(n, (int)cap));
+  s.end = min(s.n + p.nodes, (int)cap);
+  s.tiles = max(1, (s.end + KEYS - 1) / KEYS);
   if (bad && report) atomicOr(&g_tree_status, LPC_DEV_ERR_BOUNDS);
   return s;
 }
 
-// A CTA's stretch of tiles, walked item by item.  Every role walks it on its own.
+// The stretches: all = q * used + rem units, the first rem CTAs have one more.
+struct Cut {
+  uint32_t used, q, rem;
+  __device__ Cut(uint32_t all, uint32_t grid) : used(min(all, grid)), q(all / used), rem(all - q * used) {}
+  __device__ __forceinline__ uint32_t begin(uint32_t c) const { return c * q + min(c, rem); }
+  __device__ __forceinline__ uint32_t owner(uint32_t x) const {
+    const uint32_t big = rem * (q + 1);
+    return x < big ? x / (q + 1) : rem + (x - big) / q;
+  }
+};
+
+// A CTA's stretch, walked item by item.  Every role walks it on its own.
 struct Walk {
   const Params& p;
-  int64_t pos, stop;      // tiles of the batch still to do: [pos, stop)
-  int64_t b, base;        // the sequence that pos lies in, and its first tile
+  const Sequence* known;  // of sequences b0 to b0 + KNOWN - 1
+  uint32_t pos, stop;     // units still to do: [pos, stop)
+  uint32_t base;          // the first unit of sequence b
+  int b, b0;
   Sequence s;
   // the present segment
   int kvh, rb;            // KV head, block of rows
-  int64_t item;           // (b * kv_heads + kvh) * row_blocks + rb
-  int64_t j0;             // first tile
-  int count;              // tiles
+  int item;               // (b * kv_heads + kvh) * row_blocks + rb
+  int j0, count;          // first tile, tiles
+  uint32_t last;          // the unit of the item's last tile
   bool whole;
 
-  __device__ Walk(const Params& params, int64_t at, int64_t end, int64_t seq, int64_t seq_base)
-      : p(params), pos(at), stop(end), b(seq), base(seq_base) {
-    if (pos < stop) s = sequence_of(p, b, false);
-  }
+  __device__ Walk(const Params& params, const Shared& sh, uint32_t at, uint32_t end)
+      : p(params), known(sh.known), pos(at), stop(end), base(sh.found[1]), b((int)sh.found[0]),
+        b0(b), s(sh.known[0]) {}
   __device__ __forceinline__ bool next() {
-    if (pos >= stop) return false;
-    const int64_t per = s.tiles * p.kv_heads * p.row_blocks;
-    if (pos - base >= per) {  // a sequence has at least one tile
-      base += per;
-      ++b;
-      s = sequence_of(p, b, false);
+    while (pos < stop) {
+      const uint32_t unit = (uint32_t)(s.tiles + START);
+      const uint32_t per = unit * (uint32_t)(p.kv_heads * p.row_blocks);
+      if (pos - base >= per) {
+        base += per;
+        ++b;
+        s = b - b0 < KNOWN ? known[b - b0] : sequence_of(p, b, false);
+        continue;
+      }
+      const uint32_t within = pos - base, i = within / unit;
+      const int y = (int)(within - i * unit);
+      const int y1 = (int)min((uint32_t)unit, (uint32_t)y + (stop - pos));
+      last = pos + (uint32_t)(s.tiles + START - 1 - y);
+      pos += (uint32_t)(y1 - y);
+      j0 = max(0, y - START);
+      count = max(0, y1 - START) - j0;
+      if (count == 0) continue;  // the set-up alone: whoever has the first tile does it
+      kvh = (int)i / p.row_blocks;
+      rb = (int)i - kvh * p.row_blocks;
+      item = (b * p.kv_heads + kvh) * p.row_blocks + rb;
+      whole = count == s.tiles;
+      return true;
     }
-    const int64_t within = pos - base;
-    const int64_t i = within / s.tiles;
-    j0 = within - i * s.tiles;
-    kvh = (int)(i / p.row_blocks);
-    rb = (int)(i - (int64_t)kvh * p.row_blocks);
-    item = (b * p.kv_heads + kvh) * p.row_blocks + rb;
-    count = (int)min(s.tiles - j0, stop - pos);
-    whole = count == s.tiles;
-    pos += count;
-    return true;
+    return false;
   }
   // whether tile j (of the item) needs masks: it holds nodes or ends the sequence
-  __device__ __forceinline__ bool tail(int64_t j) const { return (j + 1) * KEYS > s.n; }
+  __device__ __forceinline__ bool tail(int j) const { return (j + 1) * KEYS > s.n; }
   __device__ __forceinline__ int tails() const {  // such tiles in the segment
-    int c = 0;
-    for (int64_t j = j0 + count - 1; j >= j0 && tail(j); --j) ++c;
-    return c;
+    return min(count, max(0, j0 + count - s.n / KEYS));
   }
 };
 
 // Bits of the nodes in the cache, of `nodes` and `end - n`.
-__device__ __forceinline__ uint64_t node_bits(int64_t count) {
+__device__ __forceinline__ uint64_t node_bits(int count) {
   return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1ull;
 }
 
@@ -254,7 +272,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     return;
   }
   const uint32_t sQ = raw;
-  const uint32_t sRing = raw + S::QTILES * TILE;
+  const uint32_t sRing = raw + S::QTILES * S::QBUFS * TILE;
   const uint32_t bars = raw + S::TILES;
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw + S::TILES + BAR_BYTES);
   auto full = [&](uint32_t c) { return bars + 8u * (c % SLOTS); };
@@ -262,107 +280,112 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   auto slot_parity = [&](uint32_t c) { return (c / SLOTS) & 1u; };
   auto slot = [&](uint32_t c) { return sRing + (c % SLOTS) * (uint32_t)TILE; };
   const uint32_t misc = bars + 16u * SLOTS;
-  const uint32_t q_full = misc, q_empty = misc + 8u, fixed = misc + 16u;
-  const uint32_t o_free = misc + 24u, ml_full = misc + 32u;
-  auto s_full = [&](int t) { return misc + 40u + 8u * t; };
-  auto p_half = [&](int t) { return misc + 56u + 8u * t; };
-  auto p_full = [&](int t) { return misc + 72u + 8u * t; };
-  auto o_done = [&](int t) { return misc + 88u + 8u * t; };
-  const uint32_t to_fix = misc + 104u;
-  const uint32_t tmem_slot = misc + 112u;
+  auto q_full = [&](int r) { return misc + 8u * (r % S::QBUFS); };
+  auto q_empty = [&](int r) { return misc + 16u + 8u * (r % S::QBUFS); };
+  auto q_parity = [&](int r) { return (uint32_t)(r / S::QBUFS) & 1u; };
+  const uint32_t fixed = misc + 32u, o_free = misc + 40u, ml_full = misc + 48u, to_fix = misc + 56u;
+  auto s_full = [&](int t) { return misc + 64u + 8u * t; };
+  auto p_half = [&](int t) { return misc + 80u + 8u * t; };
+  auto p_full = [&](int t) { return misc + 96u + 8u * t; };
+  auto o_done = [&](int t) { return misc + 112u + 8u * t; };
+  const uint32_t tmem_slot = misc + 128u;
   volatile uint32_t* tmem_slot_ptr =
       reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - raw));
-  static_assert(16 * SLOTS + 116 <= BAR_BYTES, "barriers");
+  static_assert(16 * SLOTS + 132 <= BAR_BYTES, "barriers");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   unsigned int* st = &g_tree_status;
-  lpc::pdl_wait();
-
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < SLOTS; ++i) {
-      lpc::mbar_init(full(i), 1);
-      lpc::mbar_init(empty(i), 1);
-    }
-    lpc::mbar_init(q_full, 1);
-    lpc::mbar_init(q_empty, 1);
-    lpc::mbar_init(to_fix, 1);
-    lpc::mbar_init(fixed, 2);
-    lpc::mbar_init(o_free, 8);
-    lpc::mbar_init(ml_full, 8);
-    for (int t = 0; t < 2; ++t) {
-      lpc::mbar_init(s_full(t), 1);
-      lpc::mbar_init(p_half(t), 4);
-      lpc::mbar_init(p_full(t), 4);
-      lpc::mbar_init(o_done(t), 1);
-    }
-    lpc::fence_mbar_init();
-  }
   if (warp == 8 && lane == 0) {
     lpc::tma_prefetch_desc(&tmQ);
     lpc::tma_prefetch_desc(&tmK);
     lpc::tma_prefetch_desc(&tmV);
   }
+  if (threadIdx.x < 2 * SLOTS) lpc::mbar_init(bars + 8u * threadIdx.x, 1);
+  if (warp == 2) {  // in the order of their places
+    constexpr int counts[16] = {1, 1, 1, 1, 2, 8, 8, 1, 1, 1, 4, 4, 4, 4, 1, 1};
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (lane == i) n = counts[i];
+    if (lane < 16) lpc::mbar_init(misc + 8u * lane, n);
+  }
+  lpc::fence_mbar_init();
+  lpc::pdl_wait();
+
   if (warp == 9) {
     lpc::tmem_alloc(tmem_slot, TMEM_COLS);
     lpc::tmem_relinquish();
   }
 
-  // ---- this CTA's stretch: total tiles, then the sequence that its first lies in ----
-  const int64_t copies = (int64_t)p.kv_heads * p.row_blocks;  // items of a sequence
-  auto block_scan = [&](int64_t v, int64_t& total) -> int64_t {  // exclusive
-    int64_t run = v;
+  // ---- this CTA's stretch: all units, then the sequence that its first lies in ----
+  const uint32_t copies = (uint32_t)(p.kv_heads * p.row_blocks);  // items of a sequence
+  auto block_scan = [&](uint32_t v, uint32_t& total) -> uint32_t {  // exclusive
+    uint32_t run = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t o = __shfl_up_sync(~0u, run, d);
+      const uint32_t o = __shfl_up_sync(~0u, run, d);
       if (lane >= d) run += o;
     }
     if (lane == 31) sh.scan[warp] = run;
     __syncthreads();
-    int64_t others = 0;
+    uint32_t others = 0;
     total = 0;
 #pragma unroll
     for (int i = 0; i < NTHREADS / 32; ++i) {
-      if (i < warp) others += sh.scan[i];
-      total += sh.scan[i];
+      const uint32_t w = sh.scan[i];
+      if (i < warp) others += w;
+      total += w;
     }
     __syncthreads();
     return others + run - v;
   };
-  int64_t all = 0, first_chunk = 0, first_before = 0;
-  for (int64_t b0 = 0; b0 < p.batch; b0 += NTHREADS) {
-    const int64_t b = b0 + threadIdx.x;
-    const int64_t mine = b < p.batch ? sequence_of(p, b, blockIdx.x == 0).tiles * copies : 0;
-    int64_t total;
-    const int64_t before = block_scan(mine, total);
-    if (b0 == 0) first_chunk = mine, first_before = before;
+  if (threadIdx.x == 0) sh.found[0] = sh.found[1] = 0;
+  uint32_t all = 0, mine = 0, before = 0;
+  Sequence own;
+  for (int b0 = 0; b0 < p.batch; b0 += NTHREADS) {
+    const int b = b0 + (int)threadIdx.x;
+    mine = 0;
+    if (b < p.batch) {
+      own = sequence_of(p, b, blockIdx.x == 0);
+      mine = (uint32_t)(own.tiles + START) * copies;
+    }
+    uint32_t total;
+    before = block_scan(mine, total);
     all += total;
   }
-  const int64_t grid = gridDim.x;
-  const int64_t used = min(grid, all);  // CTAs with work
-  const int64_t c = blockIdx.x;
-  const int64_t pos = c < used ? all * c / used : 0;
-  const int64_t stop = c < used ? all * (c + 1) / used : 0;
-  if (threadIdx.x == 0) sh.found[0] = 0, sh.found[1] = 0;
-  __syncthreads();
-  int64_t upto = 0;
-  for (int64_t b0 = 0; b0 < p.batch && pos < stop; b0 += NTHREADS) {
-    const int64_t b = b0 + threadIdx.x;
-    int64_t mine = first_chunk, before = first_before, total = 0;
+  const Cut cut(all, gridDim.x);
+  const uint32_t c = blockIdx.x;
+  const uint32_t pos = c < cut.used ? cut.begin(c) : 0;
+  const uint32_t stop = c < cut.used ? cut.begin(c + 1) : 0;
+  uint32_t upto = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += NTHREADS) {
+    const int b = b0 + (int)threadIdx.x;
+    uint32_t total = 0;
     if (p.batch > NTHREADS) {
-      mine = b < p.batch ? sequence_of(p, b, false).tiles * copies : 0;
+      mine = 0;
+      if (b < p.batch) {
+        own = sequence_of(p, b, false);
+        mine = (uint32_t)(own.tiles + START) * copies;
+      }
       before = block_scan(mine, total);
     }
     if (upto + before <= pos && pos < upto + before + mine) {
-      sh.found[0] = b;
+      sh.found[0] = (uint32_t)b;
       sh.found[1] = upto + before;
     }
     upto += total;
+  }
+  __syncthreads();
+  if (p.batch <= NTHREADS) {
+    const int at = (int)threadIdx.x - (int)sh.found[0];
+    if ((int)threadIdx.x < p.batch && at >= 0 && at < KNOWN) sh.known[at] = own;
+  } else if (threadIdx.x < KNOWN && (int)(sh.found[0] + threadIdx.x) < p.batch) {
+    sh.known[threadIdx.x] = sequence_of(p, (int)(sh.found[0] + threadIdx.x), false);
   }
   lpc::tc_fence_before();
   __syncthreads();
   lpc::tc_fence_after();
   const uint32_t tmem = *tmem_slot_ptr;
   lpc::pdl_trigger();  // only with the tensor memory in hand: the next grid may take what is left
-  const int64_t seq = sh.found[0], seq_first = sh.found[1];
 
   // ring places of the K and V tiles of a segment's tile i: K0 K1 V0 K2 V1 ...
   auto k_at = [](uint32_t ring, int i) { return ring + (uint32_t)(i == 0 ? 0 : 2 * i - 1); };
@@ -380,25 +403,26 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         bool ok = true;
         uint32_t issued = 0;
         int r = 0;
-        longlong2 begun = make_longlong2(-1, -1);
-        Walk w(p, pos, stop, seq, seq_first);
+        int2 begun = make_int2(-1, -1);
+        Walk w(p, sh, pos, stop);
         while (ok && w.next()) {
-          if (!(ok = lpc::mbar_wait(q_empty, ((uint32_t)r & 1u) ^ 1u, st))) break;
-          lpc::mbar_arrive_expect_tx(q_full, S::QTILES * TILE);
+          if (!(ok = lpc::mbar_wait(q_empty(r), q_parity(r) ^ 1u, st))) break;
+          lpc::mbar_arrive_expect_tx(q_full(r), S::QTILES * TILE);
+          const uint32_t q_at = sQ + (uint32_t)(r % S::QBUFS) * TILE;
           for (int t = 0; t < S::QTILES; ++t)
 #pragma unroll
             for (int h = 0; h < NBOX; ++h)
-              tma_load_4d(sQ + t * TILE + h * HALF_BYTES, &tmQ, h * BOX, w.rb * S::ITEM_ROWS + t * ROWS,
-                          (int)(w.b * p.kv_heads + w.kvh), 0, q_full);
-          const int64_t row = p.seq_base ? w.s.row0 : 0;
-          const int b4 = p.seq_base ? 0 : (int)w.b;
+              tma_load_4d(q_at + t * TILE + h * HALF_BYTES, &tmQ, h * BOX, w.rb * S::ITEM_ROWS + t * ROWS,
+                          w.b * p.kv_heads + w.kvh, 0, q_full(r));
+          const int row = p.seq_base ? (int)w.s.row0 : 0;
+          const int b4 = p.seq_base ? 0 : w.b;
           auto load = [&](const void* map, int i) -> bool {
             if (!lpc::mbar_wait(empty(issued), slot_parity(issued) ^ 1u, st)) return false;
             lpc::mbar_arrive_expect_tx(full(issued), TILE);
 #pragma unroll
             for (int h = 0; h < NBOX; ++h)
               tma_load_4d(slot(issued) + h * HALF_BYTES, map, h * BOX,
-                          (int)(row + (w.j0 + i) * KEYS), w.kvh, b4, full(issued));
+                          row + (w.j0 + i) * KEYS, w.kvh, b4, full(issued));
             ++issued;
             return true;
           };
@@ -408,10 +432,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             ok = ok && load(&tmV, i);
           }
           ++r;
-          if (w.j0 == 0 && !w.whole) {  // the CTA c' of tile x: all c' / used <= x, the largest
-            const int64_t x = w.pos - w.count + w.s.tiles - 1;
-            begun = make_longlong2(w.item, ((x + 1) * used - 1) / all);
-          }
+          if (w.j0 == 0 && !w.whole) begun = make_int2(w.item, (int)cut.owner(w.last));
         }
         if (p.split) p.split[c] = begun;
         if (!ok)  // copies in flight land before the CTA ends
@@ -430,7 +451,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         auto issue_s = [&](int t, uint32_t at, bool release) -> bool {
           if (!lpc::mbar_wait(full(at), slot_parity(at), st)) return false;
           lpc::tc_fence_after();
-          const uint64_t aq = dQ + (uint64_t)(((WIDE ? t : 0) * TILE) >> 4);
+          const uint64_t aq = dQ + (uint64_t)(((WIDE ? t : r % S::QBUFS) * TILE) >> 4);
           const uint64_t bk = dK + (uint64_t)(((at % SLOTS) * (uint32_t)TILE) >> 4);
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
@@ -459,16 +480,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           if (release) lpc::umma_commit(empty(at));
           return true;
         };
-        Walk w(p, pos, stop, seq, seq_first);
+        Walk w(p, sh, pos, stop);
         while (ok && w.next()) {
           const int n = w.count;
-          if (!(ok = lpc::mbar_wait(q_full, (uint32_t)r & 1u, st))) break;
+          if (!(ok = lpc::mbar_wait(q_full(r), q_parity(r), st))) break;
           lpc::tc_fence_after();
           // S of tile i; the last one of the segment releases Q
           auto scores = [&](int t, int i) -> bool {
             const bool last = WIDE ? t == 1 : true;
             if (!issue_s(t, k_at(ring, i), last)) return false;
-            if (last && i == n - 1) lpc::umma_commit(q_empty);
+            if (last && i == n - 1) lpc::umma_commit(q_empty(r));
             return true;
           };
           bool clean = false;  // the segment's tails are
@@ -512,7 +533,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       // ---------------- V rows of the tiles at the end of a sequence ----------------
       bool ok = true;
       uint32_t ring = 0, fixes = 0;
-      Walk w(p, pos, stop, seq, seq_first);
+      Walk w(p, sh, pos, stop);
       while (ok && w.next()) {
         const int tails = w.tails();
         if (tails) {
@@ -535,16 +556,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             const uint32_t at = v_at(ring, i, w.count);
             ok = __all_sync(~0u, lpc::mbar_wait(full(at), slot_parity(at), st));
             if (!ok) break;
-            const int64_t k0 = (w.j0 + i) * KEYS;
+            const int k0 = (w.j0 + i) * KEYS;
             uint8_t* tile = smem_raw + (slot(at) - raw);
             // a row a turn, half a row of boxes a lane: 16 bytes a lane
             constexpr int LANES = HD / 8;           // lanes that hold a row
             constexpr int AT_ONCE = 32 / LANES;     // rows a warp looks at
             const int sub = lane / LANES, part = lane % LANES;
-            const int from = (int)max((int64_t)0, min(w.s.n - k0, (int64_t)KEYS));
+            const int from = max(0, min(w.s.n - k0, KEYS));
             for (int q0 = from + (warp - 10) * AT_ONCE; q0 < KEYS; q0 += 2 * AT_ONCE) {
               const int q = q0 + sub;
-              const int64_t node = k0 + q - w.s.n;
+              const int node = k0 + q - w.s.n;
               uint4* x = reinterpret_cast<uint4*>(tile + (part / 8) * HALF_BYTES + q * 128) + part % 8;
               bool clear = q < KEYS, odd = false;
               if (q < KEYS && node < 64 && (seen >> node & 1)) {
@@ -591,7 +612,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       return __all_sync(~0u, lpc::mbar_wait(bar, parity, st));
     };
     const int all_rows = p.group * p.nodes;
-    Walk w(p, pos, stop, seq, seq_first);
+    Walk w(p, sh, pos, stop);
     while (ok && w.next()) {
       const int n = w.count;
       const int row = w.rb * S::ITEM_ROWS + (WIDE ? t * ROWS : 0) + rr;  // of the KV head's
@@ -621,8 +642,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         lpc::tmem_wait_ld();
         if (w.tail(w.j0 + i)) {
           // bits of the tile's keys that this row sees: context below `rel`, nodes from it
-          const int64_t rel64 = w.s.n - (w.j0 + i) * KEYS;  // in (-64, 128)
-          const int rel = (int)max((int64_t)-64, rel64);
+          const int rel = w.s.n - (w.j0 + i) * KEYS;  // in (-64, 128)
           uint32_t see[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -730,73 +750,78 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         ++twos;
       }
       lpc::tc_fence_after();
-      if (busy) {
-        const uint32_t tO0 = tmem + 256u + (WIDE ? 128u * t : 0u) + lane_off;
-        constexpr int COLS = WIDE ? HD : HD / 2;
-        const int col0 = WIDE ? 0 : t * COLS;
+      constexpr int COLS = WIDE ? HD : HD / 2;
+      const int col0 = WIDE ? 0 : t * COLS;
+      if (!busy) {
+        if (lane == 0) lpc::mbar_arrive(o_free);
+      } else {
+        const uint32_t tO0 = tmem + 256u + (WIDE ? 128u * t : 0u) + lane_off + col0;
         const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-        float* part = p.parts + (2 * c + (w.j0 == 0 ? 1 : 0)) * S::PART;
+        T* orow = static_cast<T*>(p.out) + (((int64_t)w.b * p.nodes + node) * p.heads +
+                                            w.kvh * p.group + head) * p.head_dim + col0;
+        // parts: [four columns][row], a warp's rows are 512 bytes side by side
+        float* part = p.parts + (2 * (int64_t)c + (w.j0 == 0 ? 1 : 0)) * S::PART;
         const int prow = (WIDE ? t * ROWS : 0) + rr;
-        T* orow = static_cast<T*>(p.out) +
-                  ((w.b * p.nodes + node) * p.heads + (int64_t)w.kvh * p.group + head) * p.head_dim;
+        if (valid && !w.whole && (WIDE || t == 0))
+          reinterpret_cast<float2*>(part + (int64_t)S::ITEM_ROWS * HD)[prow] = make_float2(M, L);
 #pragma unroll 1
-        for (int cc = 0; cc < COLS; cc += 16) {
-          uint32_t v[16];
-          float o[16];
+        for (int cc = 0; cc < COLS; cc += 32) {
+          uint32_t o[32];
           __syncwarp();  // rows part below; the reads are the whole warp's
-          lpc::tmem_ld16(tO0 + col0 + cc, v);
-          lpc::tmem_wait_ld();
-#pragma unroll
-          for (int q = 0; q < 16; ++q) o[q] = __uint_as_float(v[q]);
+          lpc::tmem_ld32(tO0 + cc, o);
           if (two) {
-            lpc::tmem_ld16(tO0 + 128u + col0 + cc, v);
+            uint32_t v[32];
+            lpc::tmem_ld32(tO0 + 128u + cc, v);
             lpc::tmem_wait_ld();
 #pragma unroll
-            for (int q = 0; q < 16; ++q) o[q] = o[q] * a0 + __uint_as_float(v[q]) * a1;
+            for (int q = 0; q < 32; ++q)
+              o[q] = __float_as_uint(__uint_as_float(o[q]) * a0 + __uint_as_float(v[q]) * a1);
           }
-          if (!valid) continue;
-          if (bad && col0 + cc < p.head_dim) {
+          lpc::tmem_wait_ld();
+          if (cc + 32 == COLS) {  // the next segment's first PV may overwrite O
+            lpc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) lpc::mbar_arrive(o_free);
+          }
+          if (!valid || col0 + cc >= p.head_dim) continue;
+          if (bad) {
             // visible V rows that are not finite: cleared in the tile, added here
             for (unsigned long long left = bad; left; left &= left - 1) {
               const int j = __ffsll((long long)left) - 1;
-              const int64_t krow = (w.s.row0 + (int64_t)w.kvh * w.s.head_rows + w.s.n + j) * p.head_dim;
-              const int64_t at = (j + w.s.n) / KEYS;
+              const int at = (j + w.s.n) / KEYS;
               if (at < w.j0 || at >= w.j0 + n) continue;  // in another part of the item
+              const int64_t head_rows = p.seq_base ? p.total_rows : p.max_seq_len;
+              const int64_t krow = (w.s.row0 + w.kvh * head_rows + w.s.n + j) * p.head_dim;
               const T* kr = static_cast<const T*>(p.k) + krow;
-              const T* vr = static_cast<const T*>(p.v) + krow;
+              const T* vr = static_cast<const T*>(p.v) + krow + col0 + cc;
               const T* qr = static_cast<const T*>(p.q) +
-                            ((w.b * p.kv_heads + w.kvh) * all_rows + row) * p.head_dim;
+                            ((int64_t)(w.b * p.kv_heads + w.kvh) * all_rows + row) * p.head_dim;
               float dot = 0.f;
               for (int d = 0; d < p.head_dim; ++d)
                 dot = fmaf(Num<T>::to_f(qr[d]), Num<T>::to_f(kr[d]), dot);
               const float pj = fast_exp2(dot * p.scale_log2 - (M == -INFINITY ? 0.f : M));
 #pragma unroll
-              for (int q = 0; q < 16; ++q) o[q] = fmaf(pj, Num<T>::to_f(vr[col0 + cc + q]), o[q]);
+              for (int q = 0; q < 32; ++q)
+                o[q] = __float_as_uint(fmaf(pj, Num<T>::to_f(vr[q]), __uint_as_float(o[q])));
             }
           }
           if (w.whole) {
-            if (col0 + cc < p.head_dim) {
-              uint32_t pk[8];
 #pragma unroll
-              for (int q = 0; q < 16; q += 2) pk[q >> 1] = pack2<T>(o[q] * inv, o[q + 1] * inv);
-              uint4* dst = reinterpret_cast<uint4*>(orow + col0 + cc);
-              dst[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-              dst[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+            for (int q = 0; q < 32; q += 8) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                pk[x] = pack2<T>(__uint_as_float(o[q + 2 * x]) * inv, __uint_as_float(o[q + 2 * x + 1]) * inv);
+              *reinterpret_cast<uint4*>(orow + cc + q) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             }
           } else {
-            // [four columns][row]: a warp's rows are 512 bytes side by side
-            float4* dst = reinterpret_cast<float4*>(part) + (int64_t)((col0 + cc) / 4) * S::ITEM_ROWS + prow;
+            uint4* dst = reinterpret_cast<uint4*>(part) + (col0 + cc) / 4 * S::ITEM_ROWS + prow;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              dst[q * S::ITEM_ROWS] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+            for (int q = 0; q < 8; ++q)
+              dst[q * S::ITEM_ROWS] = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
           }
         }
-        if (valid && !w.whole && (WIDE || t == 0))
-          reinterpret_cast<float2*>(part + (int64_t)S::ITEM_ROWS * HD)[prow] = make_float2(M, L);
       }
-      lpc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) lpc::mbar_arrive(o_free);
       ++r;
     }
   }
@@ -817,42 +842,51 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const Params p) {
   constexpr int GROUPS = HD / 4, ROWS_HERE = 256 / GROUPS;
   lpc::pdl_trigger();
   lpc::pdl_wait();
-  const int64_t c0 = blockIdx.x;
-  const int64_t item = lpc::ld_dep(reinterpret_cast<const int64_t*>(&p.split[c0].x));
+  const int c0 = blockIdx.x;
+  const int item = lpc::ld_dep(&p.split[c0].x);
   if (item < 0) return;
-  const int64_t last = lpc::ld_dep(reinterpret_cast<const int64_t*>(&p.split[c0].y));
-  const int rb = (int)(item % p.row_blocks);
-  const int64_t pair = item / p.row_blocks, b = pair / p.kv_heads;
-  const int kvh = (int)(pair - b * p.kv_heads);
+  const int last = lpc::ld_dep(&p.split[c0].y);
+  const int rb = item % p.row_blocks, pair = item / p.row_blocks;
+  const int b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
   const int prow = (int)blockIdx.y * ROWS_HERE + (int)threadIdx.x % ROWS_HERE;
   const int group = (int)threadIdx.x / ROWS_HERE;
   const int row = rb * S::ITEM_ROWS + prow;
   if (prow >= S::ITEM_ROWS || row >= p.group * p.nodes || 4 * group >= p.head_dim) return;
-  auto part = [&](int64_t c) { return p.parts + (2 * c + (c == c0 ? 1 : 0)) * S::PART; };
-  auto stats = [&](int64_t c) {
-    return reinterpret_cast<const float2*>(part(c) + (int64_t)S::ITEM_ROWS * HD)[prow];
-  };
-  float M = -INFINITY;
-#pragma unroll 4
-  for (int64_t c = c0; c <= last; ++c) M = fmaxf(M, stats(c).x);
-  const float mu = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
+  // four parts at a time: one memory round trip each
+  float M = -INFINITY, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int64_t c = c0; c <= last; ++c) {
-    const float2 x = stats(c);
-    const float4 v = reinterpret_cast<const float4*>(part(c))[(int64_t)group * S::ITEM_ROWS + prow];
-    const float f = fast_exp2(x.x - mu);
-    L = fmaf(f, x.y, L);
-    o.x = fmaf(f, v.x, o.x);
-    o.y = fmaf(f, v.y, o.y);
-    o.z = fmaf(f, v.z, o.z);
-    o.w = fmaf(f, v.w, o.w);
+  for (int c = c0; c <= last; c += 4) {
+    float2 x[4];
+    float4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = min(c + i, last);
+      const float* part = p.parts + (2 * (int64_t)at + (at == c0 ? 1 : 0)) * S::PART;
+      x[i] = reinterpret_cast<const float2*>(part + (int64_t)S::ITEM_ROWS * HD)[prow];
+      v[i] = reinterpret_cast<const float4*>(part)[group * S::ITEM_ROWS + prow];
+      if (c + i > last) x[i] = make_float2(-INFINITY, 0.f);
+    }
+    const float top = fmaxf(M, fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x)));
+    const float mu = top == -INFINITY ? 0.f : top;
+    const float f = fast_exp2(M - mu);
+    M = top;
+    L *= f;
+    o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (c + i > last) break;
+      const float w = fast_exp2(x[i].x - mu);
+      L = fmaf(w, x[i].y, L);
+      o.x = fmaf(w, v[i].x, o.x);
+      o.y = fmaf(w, v[i].y, o.y);
+      o.z = fmaf(w, v[i].z, o.z);
+      o.w = fmaf(w, v[i].w, o.w);
+    }
   }
   const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
   const int head = row / p.nodes, node = row - head * p.nodes;
   T* out = static_cast<T*>(p.out) +
-           ((b * p.nodes + node) * p.heads + (int64_t)kvh * p.group + head) * p.head_dim + 4 * group;
+           (((int64_t)b * p.nodes + node) * p.heads + kvh * p.group + head) * p.head_dim + 4 * group;
   *reinterpret_cast<uint2*>(out) =
       make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
 }
@@ -878,7 +912,8 @@ struct Plan {
   bool wide;
   int row_blocks;
   int64_t grid, part_floats;
-  bool join;  // some item may have more than one tile
+  bool join;   // some item may have more than one tile
+  bool fits;   // units and items are 31-bit numbers
 };
 Plan plan_of(int64_t batch, int64_t nodes, int heads, int kv_heads, int head_dim,
              int64_t max_seq_len, int64_t total_rows) {
@@ -891,6 +926,10 @@ Plan plan_of(int64_t batch, int64_t nodes, int heads, int kv_heads, int head_dim
                    lpc::current_device_sms());
   x.part_floats = (int64_t)item_rows * ((head_dim == 128 ? 128 : 64) + 2);
   x.join = (total_rows > 0 ? total_rows : max_seq_len) > KEYS;
+  const int64_t per = (int64_t)kv_heads * x.row_blocks;
+  const int64_t tiles = total_rows > 0 ? batch * ((total_rows + KEYS - 1) / KEYS + START)
+                                       : batch * ((max_seq_len + KEYS - 1) / KEYS + START);
+  x.fits = tiles <= 0x7fffffffLL / per;
   return x;
 }
 
@@ -962,7 +1001,7 @@ extern "C" int64_t lpc_tree_attention_workspace_bytes(int64_t batch, int nodes, 
   if (!sizes_ok(batch, nodes, heads, kv_heads, head_dim, max_seq_len, total_rows) || batch == 0)
     return 0;
   const Plan x = plan_of(batch, nodes, heads, kv_heads, head_dim, max_seq_len, total_rows);
-  return x.join ? x.grid * (2 * x.part_floats * 4 + 16) : 0;
+  return x.join && x.fits ? x.grid * (2 * x.part_floats * 4 + 16) : 0;
 }
 
 extern "C" int lpc_tree_attention(const void* q, const void* key_cache, const void* value_cache,
@@ -1008,6 +1047,10 @@ extern "C" int lpc_tree_attention(const void* q, const void* key_cache, const vo
     return LPC_ERR_INVALID;
   }
   const Plan plan = plan_of(batch, nodes, heads, kv_heads, head_dim, max_seq_len, total_rows);
+  if (!plan.fits) {
+    set_error("tree_attention: %lld sequences of these caches are too many tiles", (long long)batch);
+    return LPC_ERR_UNSUPPORTED;
+  }
   const int64_t need = plan.join ? plan.grid * (2 * plan.part_floats * 4 + 16) : 0;
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
     set_error("tree_attention: workspace of %lld bytes required, got %lld", (long long)need,
@@ -1026,9 +1069,10 @@ extern "C" int lpc_tree_attention(const void* q, const void* key_cache, const vo
   p.seq_cap = seq_cap;
   p.max_seq_len = max_seq_len;
   p.total_rows = total_rows;
-  p.split = plan.join ? static_cast<longlong2*>(workspace) : nullptr;
-  p.parts = plan.join ? reinterpret_cast<float*>(p.split + plan.grid) : nullptr;
-  p.batch = batch;
+  // the parts lie behind 16 bytes a CTA: they are 16-byte vectors
+  p.split = plan.join ? static_cast<int2*>(workspace) : nullptr;
+  p.parts = plan.join ? reinterpret_cast<float*>(p.split + 2 * plan.grid) : nullptr;
+  p.batch = (int)batch;
   p.nodes = nodes;
   p.heads = heads;
   p.kv_heads = kv_heads;
