@@ -16,6 +16,10 @@
 // one long sequence fills the GPU.  A CTA that holds a whole item writes its output;
 // parts of items go to a workspace (at most two a CTA, whatever the lengths) and a
 // second kernel joins them.
+//   Where few items of short capacity would spend their time on that (one sequence of
+// 1000 keys: 15 us, of which the cutting took 1 and the second kernel 5), an item is a
+// cluster of 1 to 8 CTAs, which share its tiles and join their parts through
+// distributed shared memory.
 //
 // CTA, 12 warps:
 //   warp 8      TMA: Q of the stretch's items, K and V tiles through one ring in
@@ -164,6 +168,7 @@ struct Params {
   int2* split;                 // the item that a CTA begins and does not finish (-1: none),
                                // and the last CTA that has a part of it
   int batch, nodes, heads, kv_heads, group, head_dim, row_blocks;
+  int cluster;                 // CTAs an item; 0: stretches
   float scale_log2;
 };
 
@@ -216,9 +221,11 @@ struct Walk {
   uint32_t last;          // the unit of the item's last tile
   bool whole;
 
-  __device__ Walk(const Params& params, const Shared& sh, uint32_t at, uint32_t end)
-      : p(params), known(sh.known), pos(at), stop(end), base(sh.found[1]), b((int)sh.found[0]),
-        b0(b), s(sh.known[0]) {}
+  __device__ Walk(const Params& params, const Shared& sh, uint32_t at, uint32_t end, uint32_t begin,
+                  int seq)
+      : p(params), known(sh.known), pos(at), stop(end), base(begin), b(seq), b0(seq) {
+    s = sh.known[0];
+  }
   __device__ __forceinline__ bool next() {
     while (pos < stop) {
       const uint32_t unit = (uint32_t)(s.tiles + START);
@@ -255,6 +262,31 @@ struct Walk {
 // Bits of the nodes in the cache, of `nodes` and `end - n`.
 __device__ __forceinline__ uint64_t node_bits(int count) {
   return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1ull;
+}
+
+// Four joined columns of a KV head's query row to the output.
+template <typename T>
+__device__ __forceinline__ void store_row(const Params& p, int b, int kvh, int row, int col,
+                                          const float4& o, float L) {
+  const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+  const int head = row / p.nodes, node = row - head * p.nodes;
+  T* out = static_cast<T*>(p.out) +
+           (((int64_t)b * p.nodes + node) * p.heads + kvh * p.group + head) * p.head_dim + col;
+  *reinterpret_cast<uint2*>(out) =
+      make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+}
+__device__ __forceinline__ float4 ld_remote16(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_remote8(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
 }
 
 template <typename T, int HD, bool WIDE>
@@ -338,54 +370,76 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     __syncthreads();
     return others + run - v;
   };
-  if (threadIdx.x == 0) sh.found[0] = sh.found[1] = 0;
-  uint32_t all = 0, mine = 0, before = 0;
-  Sequence own;
-  for (int b0 = 0; b0 < p.batch; b0 += NTHREADS) {
-    const int b = b0 + (int)threadIdx.x;
-    mine = 0;
-    if (b < p.batch) {
-      own = sequence_of(p, b, blockIdx.x == 0);
-      mine = (uint32_t)(own.tiles + START) * copies;
-    }
-    uint32_t total;
-    before = block_scan(mine, total);
-    all += total;
-  }
-  const Cut cut(all, gridDim.x);
   const uint32_t c = blockIdx.x;
-  const uint32_t pos = c < cut.used ? cut.begin(c) : 0;
-  const uint32_t stop = c < cut.used ? cut.begin(c + 1) : 0;
-  uint32_t upto = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += NTHREADS) {
-    const int b = b0 + (int)threadIdx.x;
-    uint32_t total = 0;
-    if (p.batch > NTHREADS) {
+  Cut cut(1, 1);
+  uint32_t pos, stop;
+  if (p.cluster) {
+    // item c / cluster, and an equal share of its tiles
+    const uint32_t item = c / (uint32_t)p.cluster, rank = c - item * (uint32_t)p.cluster;
+    const int b = (int)(item / copies);
+    const Sequence own = sequence_of(p, b, item == b * copies && rank == 0 && threadIdx.x == 0);
+    const uint32_t first = (item - b * copies) * (uint32_t)(own.tiles + START) + START;
+    pos = first + (uint32_t)own.tiles * rank / (uint32_t)p.cluster;
+    stop = first + (uint32_t)own.tiles * (rank + 1) / (uint32_t)p.cluster;
+    if (threadIdx.x == 0) {
+      sh.known[0] = own;
+      sh.found[0] = (uint32_t)b;
+      sh.found[1] = 0;
+    }
+  } else {
+    if (threadIdx.x == 0) sh.found[0] = sh.found[1] = 0;
+    uint32_t all = 0, mine = 0, before = 0;
+    Sequence own;
+    for (int b0 = 0; b0 < p.batch; b0 += NTHREADS) {
+      const int b = b0 + (int)threadIdx.x;
       mine = 0;
       if (b < p.batch) {
-        own = sequence_of(p, b, false);
+        own = sequence_of(p, b, blockIdx.x == 0);
         mine = (uint32_t)(own.tiles + START) * copies;
       }
+      uint32_t total;
       before = block_scan(mine, total);
+      all += total;
     }
-    if (upto + before <= pos && pos < upto + before + mine) {
-      sh.found[0] = (uint32_t)b;
-      sh.found[1] = upto + before;
+    cut = Cut(all, gridDim.x);
+    pos = c < cut.used ? cut.begin(c) : 0;
+    stop = c < cut.used ? cut.begin(c + 1) : 0;
+    uint32_t upto = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += NTHREADS) {
+      const int b = b0 + (int)threadIdx.x;
+      uint32_t total = 0;
+      if (p.batch > NTHREADS) {
+        mine = 0;
+        if (b < p.batch) {
+          own = sequence_of(p, b, false);
+          mine = (uint32_t)(own.tiles + START) * copies;
+        }
+        before = block_scan(mine, total);
+      }
+      if (upto + before <= pos && pos < upto + before + mine) {
+        sh.found[0] = (uint32_t)b;
+        sh.found[1] = upto + before;
+      }
+      upto += total;
     }
-    upto += total;
-  }
-  __syncthreads();
-  if (p.batch <= NTHREADS) {
-    const int at = (int)threadIdx.x - (int)sh.found[0];
-    if ((int)threadIdx.x < p.batch && at >= 0 && at < KNOWN) sh.known[at] = own;
-  } else if (threadIdx.x < KNOWN && (int)(sh.found[0] + threadIdx.x) < p.batch) {
-    sh.known[threadIdx.x] = sequence_of(p, (int)(sh.found[0] + threadIdx.x), false);
+    __syncthreads();
+    if (p.batch <= NTHREADS) {
+      const int at = (int)threadIdx.x - (int)sh.found[0];
+      if ((int)threadIdx.x < p.batch && at >= 0 && at < KNOWN) sh.known[at] = own;
+    } else if (threadIdx.x < KNOWN && (int)(sh.found[0] + threadIdx.x) < p.batch) {
+      sh.known[threadIdx.x] = sequence_of(p, (int)(sh.found[0] + threadIdx.x), false);
+    }
   }
   lpc::tc_fence_before();
   __syncthreads();
   lpc::tc_fence_after();
   const uint32_t tmem = *tmem_slot_ptr;
   lpc::pdl_trigger();  // only with the tensor memory in hand: the next grid may take what is left
+
+  const int seq = (int)sh.found[0];
+  const uint32_t seq_first = sh.found[1];
+  // an item in several parts, joined here
+  const bool joined = p.cluster > 1 && sh.known[0].tiles > 1;
 
   // ring places of the K and V tiles of a segment's tile i: K0 K1 V0 K2 V1 ...
   auto k_at = [](uint32_t ring, int i) { return ring + (uint32_t)(i == 0 ? 0 : 2 * i - 1); };
@@ -404,7 +458,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         uint32_t issued = 0;
         int r = 0;
         int2 begun = make_int2(-1, -1);
-        Walk w(p, sh, pos, stop);
+        Walk w(p, sh, pos, stop, seq_first, seq);
         while (ok && w.next()) {
           if (!(ok = lpc::mbar_wait(q_empty(r), q_parity(r) ^ 1u, st))) break;
           lpc::mbar_arrive_expect_tx(q_full(r), S::QTILES * TILE);
@@ -480,7 +534,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           if (release) lpc::umma_commit(empty(at));
           return true;
         };
-        Walk w(p, sh, pos, stop);
+        Walk w(p, sh, pos, stop, seq_first, seq);
         while (ok && w.next()) {
           const int n = w.count;
           if (!(ok = lpc::mbar_wait(q_full(r), q_parity(r), st))) break;
@@ -533,7 +587,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       // ---------------- V rows of the tiles at the end of a sequence ----------------
       bool ok = true;
       uint32_t ring = 0, fixes = 0;
-      Walk w(p, sh, pos, stop);
+      Walk w(p, sh, pos, stop, seq_first, seq);
       while (ok && w.next()) {
         const int tails = w.tails();
         if (tails) {
@@ -612,7 +666,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       return __all_sync(~0u, lpc::mbar_wait(bar, parity, st));
     };
     const int all_rows = p.group * p.nodes;
-    Walk w(p, sh, pos, stop);
+    Walk w(p, sh, pos, stop, seq_first, seq);
     while (ok && w.next()) {
       const int n = w.count;
       const int row = w.rb * S::ITEM_ROWS + (WIDE ? t * ROWS : 0) + rr;  // of the KV head's
@@ -749,6 +803,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (!(ok = wait_warp(o_done(1), twos & 1u))) break;
         ++twos;
       }
+      // the part goes where the ring was: nothing may still read it
+      if (WIDE && joined && !(ok = wait_warp(o_done(1 - t), (uint32_t)r & 1u))) break;
       lpc::tc_fence_after();
       constexpr int COLS = WIDE ? HD : HD / 2;
       const int col0 = WIDE ? 0 : t * COLS;
@@ -760,7 +816,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         T* orow = static_cast<T*>(p.out) + (((int64_t)w.b * p.nodes + node) * p.heads +
                                             w.kvh * p.group + head) * p.head_dim + col0;
         // parts: [four columns][row], a warp's rows are 512 bytes side by side
-        float* part = p.parts + (2 * (int64_t)c + (w.j0 == 0 ? 1 : 0)) * S::PART;
+        float* part = joined ? reinterpret_cast<float*>(smem_raw + (sRing - raw))
+                             : p.parts + (2 * (int64_t)c + (w.j0 == 0 ? 1 : 0)) * S::PART;
         const int prow = (WIDE ? t * ROWS : 0) + rr;
         if (valid && !w.whole && (WIDE || t == 0))
           reinterpret_cast<float2*>(part + (int64_t)S::ITEM_ROWS * HD)[prow] = make_float2(M, L);
@@ -831,6 +888,50 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     lpc::tc_fence_after();
     lpc::tmem_dealloc(tmem, TMEM_COLS);
   }
+  if (joined) {
+    // every CTA joins its share of the rows
+    __syncwarp();
+    lpc::cluster_sync();
+    const uint32_t n = (uint32_t)p.cluster, tiles = (uint32_t)sh.known[0].tiles;
+    const uint32_t item = c / n, rank = c - item * n;
+    const int rb = (int)(item % (uint32_t)p.row_blocks);
+    const int kvh = (int)(item / (uint32_t)p.row_blocks) - seq * p.kv_heads;
+    const int rows = min(S::ITEM_ROWS, p.group * p.nodes - rb * S::ITEM_ROWS);
+    const int r0 = rows * (int)rank / (int)n, mine = rows * (int)(rank + 1) / (int)n - r0;
+    const uint32_t part = sRing;
+    for (int x = (int)threadIdx.x; x < mine * (p.head_dim / 4); x += NTHREADS) {
+      const int group = x / mine, prow = r0 + x - group * mine;
+      float2 ml[8];
+      float4 v[8];
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < n && tiles * i / n < tiles * (i + 1) / n) {  // it has tiles
+          const uint32_t from = lpc::mapa_shared(part, i);
+          v[i] = ld_remote16(from + 16u * (uint32_t)(group * S::ITEM_ROWS + prow));
+          ml[i] = ld_remote8(from + 4u * S::ITEM_ROWS * HD + 8u * (uint32_t)prow);
+        }
+      }
+      float M = ml[0].x;
+#pragma unroll
+      for (int i = 1; i < 8; ++i) M = fmaxf(M, ml[i].x);
+      const float mu = M == -INFINITY ? 0.f : M;
+      float L = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = fast_exp2(ml[i].x - mu);
+        L = fmaf(f, ml[i].y, L);
+        o.x = fmaf(f, v[i].x, o.x);
+        o.y = fmaf(f, v[i].y, o.y);
+        o.z = fmaf(f, v[i].z, o.z);
+        o.w = fmaf(f, v[i].w, o.w);
+      }
+      store_row<T>(p, seq, kvh, rb * S::ITEM_ROWS + prow, 4 * group, o, L);
+    }
+    lpc::cluster_sync();  // a CTA's memory stays until all have read it
+  }
 }
 
 // Joins the parts of the item that CTA blockIdx.x began: its own second part and the
@@ -883,12 +984,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const Params p) {
       o.w = fmaf(w, v[i].w, o.w);
     }
   }
-  const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-  const int head = row / p.nodes, node = row - head * p.nodes;
-  T* out = static_cast<T*>(p.out) +
-           (((int64_t)b * p.nodes + node) * p.heads + kvh * p.group + head) * p.head_dim + 4 * group;
-  *reinterpret_cast<uint2*>(out) =
-      make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+  store_row<T>(p, b, kvh, row, 4 * group, o, L);
 }
 
 // CTAs of a call: one an SM, no more than there can be tiles.
@@ -908,11 +1004,47 @@ bool sizes_ok(int64_t batch, int64_t nodes, int heads, int kv_heads, int head_di
                          : max_seq_len > 0 && max_seq_len <= 0x7fffffffLL - KEYS);
 }
 
+// Clusters of 1 << e CTAs that the device runs at once: one CTA an SM, clusters within
+// the groups of SMs that the hardware has.
+int clusters_at_once(int e, int sms) {
+  static std::atomic<int> cache[64][4];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return std::max(1, sms >> e);
+  }
+  int v = cache[dev][e].load(std::memory_order_relaxed);
+  if (v > 0) return v;
+  using S = Shape<128, false>;
+  static std::atomic<uint64_t> mask{0};
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1u << e;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(1u << e);
+  cfg.blockDim = dim3(NTHREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const auto kernel = tree_attention_kernel<__nv_bfloat16, 128, false>;
+  if (lpc::once_per_device_smem((const void*)kernel, S::SMEM, mask) != LPC_OK ||
+      cudaOccupancyMaxActiveClusters(&v, kernel, &cfg) != cudaSuccess || v <= 0) {
+    cudaGetLastError();
+    v = std::max(1, sms >> e);
+  }
+  cache[dev][e].store(v, std::memory_order_relaxed);
+  return v;
+}
+
+constexpr int SAVED = 5;
+
 struct Plan {
   bool wide;
   int row_blocks;
   int64_t grid, part_floats;
-  bool join;   // some item may have more than one tile
+  int cluster; // CTAs an item (0: stretches)
+  bool join;   // stretches, and some item may have more than one tile
   bool fits;   // units and items are 31-bit numbers
 };
 Plan plan_of(int64_t batch, int64_t nodes, int heads, int kv_heads, int head_dim,
@@ -922,14 +1054,23 @@ Plan plan_of(int64_t batch, int64_t nodes, int heads, int kv_heads, int head_dim
   x.wide = rows > ROWS;
   const int item_rows = x.wide ? 2 * ROWS : ROWS;
   x.row_blocks = (int)((rows + item_rows - 1) / item_rows);
-  x.grid = grid_of(batch, (int64_t)kv_heads * x.row_blocks, max_seq_len, total_rows,
-                   lpc::current_device_sms());
+  const int sms = lpc::current_device_sms();
+  const int64_t items = batch * kv_heads * x.row_blocks;
+  const int64_t tiles = ((total_rows > 0 ? total_rows : max_seq_len) + KEYS - 1) / KEYS;  // an item's, at most
+  // A cluster an item, as many CTAs as one wave has; against stretches, whose set-up and
+  // second kernel cost about as much as SAVED tiles.
+  int e = 0;
+  while (e < 3 && (1 << e) < tiles && items <= clusters_at_once(e + 1, sms)) ++e;
+  const int64_t at_once = clusters_at_once(e, sms), n = 1 << e;
+  const int64_t of_cluster = (items + at_once - 1) / at_once * ((tiles + n - 1) / n + START);
+  const int64_t of_stretch = (items * (tiles + START) + sms - 1) / sms + SAVED;
+  x.cluster = of_cluster <= of_stretch ? (int)n : 0;
+  x.grid = x.cluster ? items * x.cluster
+                     : grid_of(batch, (int64_t)kv_heads * x.row_blocks, max_seq_len, total_rows, sms);
   x.part_floats = (int64_t)item_rows * ((head_dim == 128 ? 128 : 64) + 2);
-  x.join = (total_rows > 0 ? total_rows : max_seq_len) > KEYS;
+  x.join = !x.cluster && tiles > 1;
   const int64_t per = (int64_t)kv_heads * x.row_blocks;
-  const int64_t tiles = total_rows > 0 ? batch * ((total_rows + KEYS - 1) / KEYS + START)
-                                       : batch * ((max_seq_len + KEYS - 1) / KEYS + START);
-  x.fits = tiles <= 0x7fffffffLL / per;
+  x.fits = batch * (tiles + START) <= 0x7fffffffLL / per;
   return x;
 }
 
@@ -953,16 +1094,19 @@ int launch(const TmaDesc4& tq, const TmaDesc4& tk, const TmaDesc4& tv, const Par
   static std::atomic<uint64_t> mask{0};
   if (int rc = lpc::once_per_device_smem((const void*)tree_attention_kernel<T, HD, WIDE>, S::SMEM, mask))
     return rc;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)plan.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)plan.grid);
   cfg.blockDim = dim3(NTHREADS);
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = plan.cluster > 1 ? 2 : 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, tree_attention_kernel<T, HD, WIDE>, tq, tk, tv, p, id_qk,
                                      id_pv);
   if (e == cudaSuccess && plan.join) {
@@ -1079,6 +1223,7 @@ extern "C" int lpc_tree_attention(const void* q, const void* key_cache, const vo
   p.group = heads / kv_heads;
   p.head_dim = head_dim;
   p.row_blocks = plan.row_blocks;
+  p.cluster = plan.cluster;
   p.scale_log2 = sm_scale * LOG2E;
   TmaDesc4 tq, tk, tv;
   const uint64_t rowb = (uint64_t)head_dim * 2;

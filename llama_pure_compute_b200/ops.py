@@ -1155,11 +1155,20 @@ def rope_kv_append_tree(
     return q_out
 
 
-def _tree_attention_bytes(B: int, T: int, H: int, key_cache: torch.Tensor) -> int:
-    shape = key_cache.shape
-    if len(shape) == 4:
-        return _lib.load().lpc_tree_attention_workspace_bytes(B, T, H, shape[1], shape[3], shape[2], 0)
-    return _lib.load().lpc_tree_attention_workspace_bytes(B, T, H, shape[0], shape[2], 0, shape[1])
+_tree_bytes = {}  # sizes -> bytes of workspace
+
+
+def _tree_attention_bytes(index: int, *sizes: int) -> int:
+    """Bytes that a call with these (batch, nodes, heads, kv_heads, head_dim,
+    max_seq_len, total_rows) needs: 0 for one kernel, more for two."""
+    n = _tree_bytes.get((index, sizes))
+    if n is None:
+        with torch.cuda.device(index):
+            n = _lib.load().lpc_tree_attention_workspace_bytes(*sizes)
+        if len(_tree_bytes) > 4096:
+            _tree_bytes.clear()
+        _tree_bytes[index, sizes] = n
+    return n
 
 
 def tree_attention_workspace(q: torch.Tensor, key_cache: torch.Tensor) -> torch.Tensor:
@@ -1170,8 +1179,12 @@ def tree_attention_workspace(q: torch.Tensor, key_cache: torch.Tensor) -> torch.
     if q.dim() != 4 or key_cache.dim() not in (3, 4):
         raise ValueError("LlamaPureComputeError: q must be [B, H, T, D], caches [B, H, S, D] or "
                          "[H, rows, D].")
-    with torch.cuda.device(q.device):
-        n = _tree_attention_bytes(q.shape[0], q.shape[2], q.shape[1], key_cache)
+    B, H, T, D = q.shape
+    if key_cache.dim() == 4:
+        rest = (key_cache.shape[1], D, key_cache.shape[2], 0)
+    else:
+        rest = (key_cache.shape[0], D, 0, key_cache.shape[1])
+    n = _tree_attention_bytes(q.get_device(), B, T, H, *rest)
     return torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
 
 
@@ -1225,8 +1238,9 @@ def tree_attention(
     masks, masks_stride = _tree_ints(masks, "masks", B, T, index, torch.int64)
     q = _dense16(q)
     out = q.new_empty(B, T, H, D)
+    need = _tree_attention_bytes(index, B, T, H, kv_heads, D, max_seq_len, total_rows)
     if workspace is None:
-        workspace = tree_attention_workspace(q, key_cache)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     elif workspace.get_device() != index or not workspace.is_contiguous():
         raise ValueError("LlamaPureComputeError: workspace must be contiguous on q's device.")
     rc = _lib.call_on(index, _lib.load().lpc_tree_attention, q.data_ptr(), key_cache.data_ptr(),
@@ -1237,7 +1251,7 @@ def tree_attention(
     if rc:
         _lib.check(rc, "tree_attention")
     if B:
-        _lib.launch_count += 2 if (total_rows or max_seq_len) > 128 else 1
+        _lib.launch_count += 2 if need else 1
     return out.transpose(1, 2)
 
 

@@ -328,8 +328,7 @@ def test_refusals():
                dict(workspace=torch.empty(16, dtype=torch.uint8, device=DEV)), dict(seq_base=base),
                dict(workspace=torch.empty(1 << 26, dtype=torch.uint8)), dict(seq_base=base, seq_cap=cap)):
         if "workspace" in kw:
-            kw["workspace"] = kw["workspace"]
-            big = Case([500], 4, 4, 2, 64, BF, False)
+            big = Case([40000], 4, 8, 8, 64, BF, False)  # cut into stretches
             with pytest.raises(ValueError):
                 big.run(**kw)
             continue
