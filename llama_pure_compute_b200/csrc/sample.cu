@@ -22,10 +22,12 @@
 //     by a table, Tang 1989; the series' next term is 1.2e-12): nine fp64
 //     operations, a third of exp2()'s.
 //   * Every filter keeps a prefix of the order, so a filter is one place in it: a
-//     value and, among equals, an index.  A histogram over 2048 bins of 1/64 octave
-//     of the weight, of counts or of fp32 weights, says in which bins the place lies;
-//     their few elements go to a list and are ranked exactly, by pairs.  With top-k
-//     the list has all that is kept, and the rest is done on it.
+//     value and, among equals, an index.  A pass then compares floats: bins, min-p
+//     and the like are turned into the smallest float that passes.
+//   * A histogram over 2048 bins of 1/64 octave of the weight, of counts or of fp32
+//     weights, says in which bins the place lies; their few elements go to a list and
+//     are ranked exactly, by pairs.  With top-k the list has all that is kept, and the
+//     rest is done on it.
 //   * Where the list would not hold them (many equal logits, thousands kept by top-k,
 //     places beyond the bins), the place is found by radix select: histograms over 11
 //     bits of the order-preserving integer of the value, of counts or of integer
@@ -52,14 +54,18 @@ namespace {
 
 using lpc::Num;
 
+// 512 threads and shares of 64 KB: two CTAs an SM, so that one reads while the other computes
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_CLUSTER = 8;
 constexpr int BINS = 2048;                       // 11 bits a round
+constexpr int MINE = BINS / THREADS;             // bins a thread, at most
 constexpr int HIST_BYTES = BINS * 8;             // low and high words of a bin's sum
+constexpr int LIST = 1024;                       // elements of a list
+constexpr int PAIRS = 512;                       // elements that are ranked by pairs
+constexpr int LIST_BYTES = LIST * 8;
 constexpr double FIXED = 17592186044416.0;       // 2^44
 constexpr double ROUND52 = 4503599627370496.0;   // 2^52: adding it rounds to an integer
-constexpr int LIST = 512;                        // elements that are ranked by pairs
 constexpr int OCTAVE = 64;                       // bins an octave of the weight
 // What the fp32 histogram may be off, relative to all weights: its elements by 2^-16 of
 // rounding and 4e-6 of fp32 arithmetic, twice, and what lies below its 32 octaves, at most
@@ -113,6 +119,34 @@ struct Chunk {
       }
     }
   }
+  static __device__ __forceinline__ uint4 nothing() {  // -inf
+    constexpr uint32_t w = sizeof(T) == 4 ? 0xff800000u : GRAIN<T> == 16 ? 0xff80ff80u : 0xfc00fc00u;
+    return make_uint4(w, w, w, w);
+  }
+  // The largest; NaN if there is one.
+  __device__ __forceinline__ float largest() const {
+    if constexpr (sizeof(T) == 4) {
+      return max_nan(max_nan(get(0), get(1)), max_nan(get(2), get(3)));
+    } else {
+      const uint32_t m = max2_nan(max2_nan(raw.x, raw.y), max2_nan(raw.z, raw.w));
+      Chunk<T> x;
+      x.raw.x = m;
+      return max_nan(x.get(0), x.get(1));
+    }
+  }
+  static __device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+  }
+  static __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if constexpr (GRAIN<T> == 16)
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
 };
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
@@ -154,13 +188,13 @@ __device__ __forceinline__ uint32_t ld_remote(uint32_t addr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint4 ld_remote16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
+__device__ __forceinline__ uint64_t warp_min(uint64_t v) {  // over the warp
+#pragma unroll
+  for (int m = 16; m; m >>= 1) v = min(v, shfl_xor64(v, m));
   return v;
+}
+__device__ __forceinline__ void atom_add(uint32_t addr, uint32_t v) {
+  asm volatile("red.shared.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ void st_remote64(uint32_t addr, uint64_t v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
@@ -169,244 +203,342 @@ __device__ __forceinline__ void st_remote64(uint32_t addr, uint64_t v) {
 struct Entry {  // an element in the order: by offset from the largest, then by index
   uint32_t index, off;
 };
-__device__ __forceinline__ uint64_t place_of(const Entry& e) { return (uint64_t)e.off << 32 | e.index; }
+struct Listed {
+  uint64_t place, weight;  // place: offset, index
+};
+static_assert(LIST * (int)sizeof(Listed) <= HIST_BYTES && LIST * (int)sizeof(Entry) <= LIST_BYTES, "");
 
 struct Shared {
   double table[32];                       // 2^44 * 2^(j/32)
-  uint32_t listed;                        // elements that this CTA put on its list
-  uint32_t window[2];                     // first and last bin that may hold the place
-  unsigned long long cut;                 // place of the last that stays
-  uint64_t list_sum;
   uint64_t sums[3][MAX_CLUSTER * WARPS];  // written by every CTA of the cluster
   uint64_t found[2];                      // a located index, written by its finder
-  uint64_t warp_best[WARPS];
   uint64_t scan[WARPS];
-  uint64_t cross_before, cross_in;        // sum before the crossing bin, and in it
-  int cross_bin;
+  uint64_t parts[2][MAX_CLUSTER];         // sums of each CTA's bins
+  uint64_t cross[3];                      // the crossing bin (~0: none), the sum before it and in it
+  uint64_t window[2];                     // first and last bin that may hold the place
+  uint32_t listed;                        // elements that this CTA put on its list
 };
 
 template <typename T>
 class Row {
  public:
   static constexpr int N = Chunk<T>::N;
-  const Args& a;
   Shared& sh;
   uint4* chunks;              // this CTA's share of the row, -inf outside it
-  uint32_t* hist[2];          // low words, then high words
+  uint32_t* hist;             // BINS low words, BINS high words; or the cluster's list
+  Entry* own_list;
   int rank, ctas, warp, lane;
   int nchunks, segment;       // chunks of this CTA; of a warp (a multiple of 32)
   int first;                  // row index of element 0 of chunk 0 (may lie before the share)
   int begin, end;             // row indexes of the share
   int32_t kmax;               // order_of(largest)
-  double top, scale;          // largest, log2(e) / temperature
-  int turn = 0;               // which histogram the next round takes
+  float topf, floorf;         // largest; a logit that weighs nothing (2^-60)
+  double top, scale;          // largest; 32 log2(e) / temperature
+  float octaves, lowest;      // -OCTAVE log2(e) / temperature; offset of the last bin
+  uint32_t tab_lo, tab_hi;    // table entry `lane`, its index taken off the exponent
   int slot = 0;               // which sums the next exchange takes
-  int found_slot = 0;
+  int found_slot = 0, part_slot = 0;
 
-  __device__ Row(const Args& args, Shared& s) : a(args), sh(s) {}
+  __device__ explicit Row(Shared& s) : sh(s) {}
 
-  __device__ __forceinline__ Chunk<T> chunk(int c) const {
-    Chunk<T> r;
-    r.raw = chunks[c];
-    return r;
+  // Every thread of the cluster.
+  __device__ __forceinline__ void sync() const {
+    if (ctas == 1) __syncthreads();
+    else lpc::cluster_sync();
   }
-  float topf, octaves, lowest;  // largest; -OCTAVE log2(e) / temperature; offset of the last bin
-  uint32_t tab_lo, tab_hi;      // table entry `lane`
+  __device__ __forceinline__ void store_all(uint64_t* where, uint64_t v) const {  // in every CTA
+    for (int r = 0; r < ctas; ++r) st_remote64(lpc::mapa_shared(lpc::smem_u32(where), r), v);
+  }
 
-  // round(2^44 w) of a finite logit; `exact`: 2^44 w itself.  ALL: every lane of the
-  // warp is here, and the table comes from the lanes' registers.
+  // 2^44 w of a logit, before (`exact`) and after rounding.  ALL: every lane of the warp
+  // is here, and the table comes from the lanes' registers.
   template <bool ALL>
-  __device__ __forceinline__ uint64_t weight(float f, double& exact) const {
-    constexpr double A1 = 0.02166084939249829, A2 = 0.00023459619820224677;  // (ln2/32)^k / k!
+  __device__ __forceinline__ uint64_t weight(float f, double* exact = nullptr) const {
+    // (ln2/32)^k / k!
+    constexpr double A1 = 0.02166084939249829, A2 = 0.00023459619820224677;
     constexpr double A3 = 1.6938509724371819e-06, A4 = 9.172562701824643e-09;
     constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
-    const double d = f == topf ? 0.0 : (double)f - top;
+    const double d = (double)fmaxf(f, floorf) - top;
     const double t = fma(d, scale, MAGIC);
     const double r = fma(d, scale, MAGIC - t);
-    const int n = __double2loint(t);
+    const int n = __double2loint(t);              // 32 e + j
     const double poly = fma(fma(fma(fma(A4, r, A3), r, A2), r, A1), r, 1.0);
     uint32_t lo, hi;
     if constexpr (ALL) {
-      lo = __shfl_sync(~0u, tab_lo, n & 31);
-      hi = __shfl_sync(~0u, tab_hi, n & 31);
+      lo = __shfl_sync(~0u, tab_lo, n);
+      hi = __shfl_sync(~0u, tab_hi, n) + (uint32_t)n * 32768u;  // + e << 20
     } else {
       lo = (uint32_t)__double2loint(sh.table[n & 31]);
-      hi = (uint32_t)__double2hiint(sh.table[n & 31]);
+      hi = (uint32_t)__double2hiint(sh.table[n & 31]) + (uint32_t)((n >> 5) << 20);
     }
-    const double power = __hiloint2double((int)hi + ((n >> 5) << 20), (int)lo);
-    const bool some = d * scale > -32.0 * 46;  // less rounds to nothing
-    exact = some ? poly * power : 0.0;
-    return some ? (uint64_t)__double_as_longlong(fma(poly, power, ROUND52)) & 0xfffffffffffffull : 0ull;
-  }
-  template <bool ALL>
-  __device__ __forceinline__ uint64_t weight(float f) const {
-    double e;
-    return weight<ALL>(f, e);
+    const double power = __hiloint2double((int)hi, (int)lo);
+    if (exact) *exact = poly * power;
+    return (uint64_t)__double_as_longlong(fma(poly, power, ROUND52)) - 0x4330000000000000ull;
   }
   __device__ __forceinline__ uint32_t off_of(float f) const {
     return (uint32_t)kmax - (uint32_t)order_of(f);
   }
-  // Bin of a logit, rising along the order; BINS and more: below all bins.  `rest`:
-  // the logit's distance from the middle of its bin.
-  __device__ __forceinline__ uint32_t bin_of(float f, float& rest) const {
-    const float d = f - topf;
-    const float t = fmaf(d, octaves, 8388608.f);  // 2^23: rounds to an integer
-    rest = fmaf(d, octaves, 8388608.f - t);
-    return d < lowest ? BINS : __float_as_uint(t) & 0x7fffffu;
+  __device__ __forceinline__ float at_off(uint32_t off) const {
+    return value_of((int32_t)((uint32_t)kmax - off));
   }
+  // Bin of a logit, rising along the order; BINS: below all bins.
   __device__ __forceinline__ uint32_t bin_of(float f) const {
-    float rest;
-    return bin_of(f, rest);
+    const float d = f - topf;
+    return d < lowest ? BINS : __float_as_uint(fmaf(d, octaves, 8388608.f)) & 0x7fffffu;
   }
 
-  // fn(chunk, index of its first element, whether it exists) for the warp's chunks,
-  // every lane of the warp at once.
+  // The smallest float for which pass() holds, which holds from some float up to the
+  // largest logit on.  The whole warp.
+  template <typename F>
+  __device__ float smallest(F pass) const {
+    int32_t lo = order_of(-3.402823466e38f), hi = kmax;
+    while (lo < hi) {
+      const uint32_t span = (uint32_t)hi - (uint32_t)lo;
+      const int32_t c = (int32_t)((uint32_t)lo + (uint32_t)(((uint64_t)span * (uint32_t)lane) >> 5));
+      const unsigned ok = __ballot_sync(~0u, pass(value_of(c)));
+      const int s = ok ? __ffs(ok) - 1 : 32;  // the first that passes
+      if (s < 32) hi = __shfl_sync(~0u, c, s);
+      if (s > 0) lo = __shfl_sync(~0u, c, s - 1) + 1;
+    }
+    return value_of(hi);
+  }
+
+  // fn(chunk, index of its first element) for the warp's chunks, every lane of the warp
+  // at once; -inf where there is none.
   template <typename F>
   __device__ __forceinline__ void each(F fn) const {
-    const int end = min(nchunks, (warp + 1) * segment);
-    for (int c0 = warp * segment; c0 < end; c0 += 32) {
+    each_of(warp * segment, min(nchunks, (warp + 1) * segment), fn);
+  }
+  template <typename F>
+  __device__ __forceinline__ void each_of(int start, int stop, F fn) const {
+    for (int c0 = start; c0 < stop; c0 += 32) {
       const int c = c0 + lane;
       Chunk<T> x;
-      x.raw = make_uint4(0, 0, 0, 0);
-      if (c < end) x = chunk(c);
-      fn(x, first + c * N, c < end);
+      if (c < stop) x.raw = chunks[c];
+      else x.raw = Chunk<T>::nothing();
+      fn(x, first + c * N);
     }
   }
 
-  // Sum of v over the cluster's warps, and of the warps before each; `mine` is
-  // this warp's.  Every thread gets the total.
-  __device__ uint64_t exchange(uint64_t mine) {
+  // fn(chunk) for the chunks that this thread wrote, to change them.
+  template <typename F>
+  __device__ void each_own(F fn) const {
+    const int stop = min(nchunks, (warp + 1) * segment);
+    for (int c = warp * segment + lane; c < stop; c += 32) {
+      Chunk<T> x;
+      x.raw = chunks[c];
+      fn(x);
+      chunks[c] = x.raw;
+    }
+  }
+
+  // Every warp's `mine`, in sh.sums[the slot before], in the order of the row.
+  __device__ const uint64_t* exchange(uint64_t mine) {
     const int s = slot;
     slot = slot == 2 ? 0 : slot + 1;
     if (lane < ctas)
       st_remote64(lpc::mapa_shared(lpc::smem_u32(&sh.sums[s][rank * WARPS + warp]), lane), mine);
-    lpc::cluster_sync();
+    sync();
+    return sh.sums[s];
+  }
+  __device__ uint64_t total_of(const uint64_t* sums) const {
     uint64_t v = 0;
-    for (int i = lane; i < ctas * WARPS; i += 32) v += sh.sums[s][i];
+    for (int i = lane; i < ctas * WARPS; i += 32) v += sums[i];
     return warp_sum(v);
   }
 
-  // This warp's sum of fn(value, index).
-  template <typename F>
-  __device__ uint64_t sum_of(F fn) const {
-    uint64_t mine = 0;
-    each([&](const Chunk<T>& x, int at, bool in) {
+  // Of n <= 128 sums the one (-1: none) in which the running sum exceeds target; `before`:
+  // the sum before it.  The whole warp.
+  __device__ int crossing_of(const uint64_t* sums, int n, uint64_t target, uint64_t& before) const {
+    uint64_t v[4], own = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint64_t v = fn(x.get(i), at + i);
-        mine += in ? v : 0ull;
+    for (int i = 0; i < 4; ++i) {
+      v[i] = 4 * lane + i < n ? sums[4 * lane + i] : 0ull;
+      own += v[i];
+    }
+    uint64_t run = before + warp_scan(own, lane) - own, at = 0;
+    int which = -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (run <= target && target < run + v[i]) {
+        which = 4 * lane + i;
+        at = run;
       }
-    });
-    return warp_sum(mine);
+      run += v[i];
+    }
+    const unsigned who = __ballot_sync(~0u, which >= 0);
+    if (!who) return -1;
+    const int l = __ffs(who) - 1;
+    before = (uint64_t)__shfl_sync(~0u, (uint32_t)at, l) |
+             (uint64_t)__shfl_sync(~0u, (uint32_t)(at >> 32), l) << 32;
+    return __shfl_sync(~0u, which, l);
   }
 
   // Lowest row index at which the running sum of fn(value, index) exceeds
   // target(total); `mine` is this warp's sum.  Every thread of the cluster gets it.
-  // total > target.
+  // total > target.  The CTA that has it shares the warp's stretch out to all its warps.
   template <typename F, typename G>
   __device__ int locate(uint64_t mine, F fn, G target_of) {
-    const int s = slot;
-    const uint64_t total = exchange(mine);
-    const uint64_t target = target_of(total);
-    uint64_t upto = 0;  // the warps before this one
-    for (int i = lane; i < rank * WARPS + warp; i += 32) upto += sh.sums[s][i];
-    upto = warp_sum(upto);
+    const uint64_t* sums = exchange(mine);
+    const uint64_t target = target_of(total_of(sums));
+    uint64_t before = 0;
+    const int owner = crossing_of(sums, ctas * WARPS, target, before);
     const int f = found_slot;
     found_slot ^= 1;
-    if (upto <= target && target < upto + mine) {
-      bool done = false;
-      each([&](const Chunk<T>& x, int at, bool in) {
-        if (done) return;
-        uint64_t part = 0;
+    if (owner >= 0 && owner / WARPS == rank) {
+      const int start = owner % WARPS * segment, stop = min(nchunks, start + segment);
+      const int share = (segment + WARPS - 1) / WARPS;
+      const int from = start + warp * share, to = min(stop, from + share);
+      uint64_t sum = 0;
+      each_of(from, to, [&](const Chunk<T>& x, int at) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint64_t v = fn(x.get(i), at + i);
-          part += in ? v : 0ull;
-        }
-        const uint64_t scan = warp_scan(part, lane);
-        const unsigned over = __ballot_sync(~0u, upto + scan > target);
-        if (over) {
-          done = true;
-          const int who = __ffs(over) - 1;
-          // its elements once more, by all lanes together
-          uint64_t run = upto + scan - part;
-          int found = -1;
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            run += fn(x.get(i), at + i);
-            if (found < 0 && run > target) found = at + i;
-          }
-          if (lane == who)
-            for (int r = 0; r < ctas; ++r)
-              st_remote64(lpc::mapa_shared(lpc::smem_u32(&sh.found[f]), r), (uint64_t)found);
-        } else {
-          upto += (uint64_t)__shfl_sync(~0u, (uint32_t)scan, 31) |
-                  ((uint64_t)__shfl_sync(~0u, (uint32_t)(scan >> 32), 31) << 32);
-        }
+        for (int i = 0; i < N; ++i) sum += fn(x.get(i), at + i);
       });
+      sum = warp_sum(sum);
+      if (lane == 0) sh.scan[warp] = sum;
+      __syncthreads();
+      if (crossing_of(sh.scan, WARPS, target, before) == warp) {
+        bool done = false;
+        each_of(from, to, [&](const Chunk<T>& x, int at) {
+          if (done) return;
+          uint64_t part = 0;
+#pragma unroll
+          for (int i = 0; i < N; ++i) part += fn(x.get(i), at + i);
+          const uint64_t scan = warp_scan(part, lane);
+          const unsigned over = __ballot_sync(~0u, before + scan > target);
+          if (over) {
+            done = true;
+            uint64_t run = before + scan - part;
+            int found = -1;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {  // once more, all lanes together
+              run += fn(x.get(i), at + i);
+              if (found < 0 && run > target) found = at + i;
+            }
+            if (lane == __ffs(over) - 1) store_all(&sh.found[f], (uint64_t)found);
+          } else {
+            before += (uint64_t)__shfl_sync(~0u, (uint32_t)scan, 31) |
+                      ((uint64_t)__shfl_sync(~0u, (uint32_t)(scan >> 32), 31) << 32);
+          }
+        });
+      }
     }
-    lpc::cluster_sync();
+    sync();
     return (int)sh.found[f];
+  }
+  // This warp's sum of fn(value, index).
+  template <typename F>
+  __device__ uint64_t sum_of(F fn) const {
+    uint64_t mine = 0;
+    each([&](const Chunk<T>& x, int at) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) mine += fn(x.get(i), at + i);
+    });
+    return warp_sum(mine);
   }
 
   // Histogram over the bins: of counts, or of fp32 weights in units of 2^-15 of a bin's
-  // middle.  Every thread gets the cluster's bins 4 tid to 4 tid + 3.
+  // middle.
   template <bool MASS>
-  __device__ void histogram(uint64_t (&v)[4]) {
-    uint32_t* h = hist[0];
-    for (int i = threadIdx.x; i < BINS; i += THREADS) h[i] = 0u;
+  __device__ void histogram() {
+    for (int i = threadIdx.x; i < BINS; i += THREADS) hist[i] = 0u;
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    each([&](const Chunk<T>& x, int, bool in) {
+    const uint32_t base = lpc::smem_u32(hist) - 4u * 0x4b000000u;  // the bits of 2^23
+    each([&](const Chunk<T>& x, int) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        float rest;
-        const uint32_t bin = bin_of(x.get(i), rest);
-        // 2^15 * 2^(-rest / OCTAVE), by two terms of the series (2e-7 off)
-        const float e = rest * (-0.69314718f / OCTAVE);
-        const float m = fmaf(fmaf(e, 0.5f, 1.f) * e, 32768.f, 32768.f + 8388608.f);
-        if (in && bin < BINS) atomicAdd(h + bin, MASS ? __float_as_uint(m) & 0x7fffffu : 1u);
+        const float d = x.get(i) - topf;
+        const float t = fmaf(d, octaves, 8388608.f);
+        uint32_t add = 1u;
+        if constexpr (MASS) {
+          // 2^15 * 2^(-rest / OCTAVE), by two terms of the series (2e-7 off)
+          const float e = fmaf(d, octaves, 8388608.f - t) * (-0.69314718f / OCTAVE);
+          add = __float_as_uint(fmaf(fmaf(e, 0.5f, 1.f) * e, 32768.f, 32768.f + 8388608.f)) - 0x4b000000u;
+        }
+        if (d >= lowest) atom_add(base + 4u * __float_as_uint(t), add);
       }
     });
-    lpc::cluster_sync();
+    sync();
+  }
+  // Each CTA has BINS / ctas bins of the cluster's, a thread up to MINE of them.
+  __device__ __forceinline__ int bins_a_thread() const { return max(1, MINE / ctas); }
+  __device__ __forceinline__ int first_bin() const {
+    return rank * (BINS / ctas) + (int)threadIdx.x * bins_a_thread();
+  }
+  template <bool WIDE>
+  __device__ void merge(uint64_t (&v)[MINE]) const {
+    const int m = bins_a_thread(), at = first_bin();
+    const bool has = (int)threadIdx.x * m < BINS / ctas;
+    const uint32_t from = lpc::smem_u32(hist + at);
+    uint32_t lo[MAX_CLUSTER], hi[MAX_CLUSTER];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = 0;
-    const uint32_t at = lpc::smem_u32(h + 4 * threadIdx.x);
-    for (int r = 0; r < ctas; ++r) {
-      const uint4 l = ld_remote16(lpc::mapa_shared(at, r));
-      v[0] += l.x, v[1] += l.y, v[2] += l.z, v[3] += l.w;
+    for (int i = 0; i < MINE; ++i) {
+      v[i] = 0;
+      if (!has || i >= m) continue;
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r) {  // all in flight
+        lo[r] = hi[r] = 0;
+        if (r < ctas) {
+          lo[r] = ld_remote(lpc::mapa_shared(from + 4 * i, r));
+          if constexpr (WIDE) hi[r] = ld_remote(lpc::mapa_shared(from + 4 * BINS + 4 * i, r));
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r) v[i] += (uint64_t)hi[r] << 32 | lo[r];
     }
   }
-
-  // The bin whose running count first exceeds `target` (-1: none), from each thread's four;
-  // sh.cross_before and sh.cross_in: the count before it and in it.
-  __device__ int crossing(const uint64_t (&v)[4], uint64_t target) {
-    const uint64_t own = v[0] + v[1] + v[2] + v[3];
+  // The bin whose running sum, begun at `above`, first exceeds target(above + total)
+  // (-1: none); sh.cross: it, the sum before it and in it.
+  template <bool WIDE, typename G>
+  __device__ int crossing(uint64_t above, G target_of) {
+    uint64_t v[MINE], own = 0;
+    merge<WIDE>(v);
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) own += v[i];
     uint64_t run = warp_scan(own, lane);
     if (lane == 31) sh.scan[warp] = run;
-    if (threadIdx.x == 0) sh.cross_bin = -1;
+    if (threadIdx.x == 0) sh.cross[0] = ~0ull;
     __syncthreads();
-    for (int i = 0; i < warp; ++i) run += sh.scan[i];
-    run -= own;
+    uint64_t total = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < WARPS; ++i) {
+      const uint64_t s = sh.scan[i];
+      total += s;
+      if (i < warp) run += s;
+    }
+    run += above - own;
+    const int s = part_slot;
+    part_slot ^= 1;
+    if (threadIdx.x == 0) store_all(&sh.parts[s][rank], total);
+    sync();
+    total = above;
+    for (int r = 0; r < ctas; ++r) {
+      total += sh.parts[s][r];
+      if (r < rank) run += sh.parts[s][r];
+    }
+    const uint64_t target = target_of(total);
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
       if (run <= target && target < run + v[i]) {
-        sh.cross_bin = 4 * (int)threadIdx.x + i;
-        sh.cross_before = run;
-        sh.cross_in = v[i];
+        store_all(&sh.cross[0], (uint64_t)(first_bin() + i));
+        store_all(&sh.cross[1], run);
+        store_all(&sh.cross[2], v[i]);
       }
       run += v[i];
     }
-    __syncthreads();
-    return sh.cross_bin;
+    sync();
+    return (int)sh.cross[0];
   }
   // The bins between which the running sum of the weights passes p * (their sum), with
   // SLACK on either side: sh.window.  False: it may pass below all bins.
-  __device__ bool window(const uint64_t (&v)[4], float p) {
-    double w[4], own = 0;
+  __device__ bool window(float p) {
+    uint64_t v[MINE];
+    merge<false>(v);
+    double w[MINE], own = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = (double)v[i] * (double)exp2f(-(float)(4 * (int)threadIdx.x + i) / OCTAVE);
+    for (int i = 0; i < MINE; ++i) {
+      w[i] = v[i] ? (double)v[i] * (double)exp2f(-(float)(first_bin() + i) / OCTAVE) : 0.0;
       own += w[i];
     }
     double run = own;
@@ -419,188 +551,238 @@ class Row {
     if (lane == 31) scan[warp] = run;
     if (threadIdx.x == 0) sh.window[0] = sh.window[1] = BINS;
     __syncthreads();
-    double total = 0, others = 0;
+    double total = 0;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) {
-      if (i < warp) others += scan[i];
+      if (i < warp) run += scan[i];
       total += scan[i];
     }
-    run += others - own;
+    run -= own;
+    const int s = part_slot;
+    part_slot ^= 1;
+    if (threadIdx.x == 0) store_all(&sh.parts[s][rank], (uint64_t)__double_as_longlong(total));
+    sync();
+    total = 0;
+    for (int r = 0; r < ctas; ++r) {
+      const double x = __longlong_as_double((long long)sh.parts[s][r]);
+      if (r < rank) run += x;
+      total += x;
+    }
     const double lo = ((double)p - SLACK) * total, hi = ((double)p + SLACK) * total;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool first = threadIdx.x == 0 && i == 0;
-      if ((first || run <= lo) && lo < run + w[i]) atomicMin(&sh.window[0], 4 * threadIdx.x + i);
-      if ((first || run <= hi) && hi < run + w[i]) atomicMin(&sh.window[1], 4 * threadIdx.x + i);
+    for (int i = 0; i < MINE; ++i) {
+      const int bin = first_bin() + i;
+      if ((bin == 0 || run <= lo) && lo < run + w[i]) store_all(&sh.window[0], (uint64_t)bin);
+      if ((bin == 0 || run <= hi) && hi < run + w[i]) store_all(&sh.window[1], (uint64_t)bin);
       run += w[i];
     }
-    __syncthreads();
+    sync();
     return sh.window[0] < BINS && sh.window[1] < BINS;
   }
 
-  // The elements for which want(value, index) puts them on this CTA's list (in hist[1]);
-  // LIST of them at most are kept, all are counted.
-  __device__ __forceinline__ void list(bool want, float f, int at) {
-    const unsigned who = __ballot_sync(~0u, want);
-    if (!who) return;
-    uint32_t base = 0;
-    if (lane == __ffs(who) - 1) base = atomicAdd(&sh.listed, (uint32_t)__popc(who));
-    base = __shfl_sync(~0u, base, __ffs(who) - 1) + (uint32_t)__popc(who & ((1u << lane) - 1u));
-    if (want && base < (uint32_t)LIST)
-      reinterpret_cast<Entry*>(hist[1])[base] = Entry{(uint32_t)at, off_of(f)};
-  }
-  // The cluster's lists, with their weights, in this CTA's hist[0]; their length, or -1
-  // where they are longer than LIST.  The lists are complete in every CTA.
-  struct Listed {
-    uint64_t place, weight;
-  };
-  __device__ int gather() {
-    lpc::cluster_sync();
-    int total = 0, start = 0;
-    const uint32_t counts = lpc::smem_u32(&sh.listed);
-    for (int r = 0; r < ctas; ++r) total += (int)ld_remote(lpc::mapa_shared(counts, r));
-    if (total > LIST) return -1;
-    Listed* all = reinterpret_cast<Listed*>(hist[0]);
-    const uint32_t from = lpc::smem_u32(hist[1]);
-    for (int r = 0; r < ctas; ++r) {
-      const int n = (int)ld_remote(lpc::mapa_shared(counts, r));
-      const uint32_t list = lpc::mapa_shared(from, r);
-      for (int i = threadIdx.x; i < n; i += THREADS) {
-        Entry e;
-        e.index = ld_remote(list + 8u * i);
-        e.off = ld_remote(list + 8u * i + 4u);
-        all[start + i] = Listed{place_of(e), weight<false>(value_of((int32_t)((uint32_t)kmax - e.off)))};
+  // Puts the elements of a chunk in [from, below) on this CTA's list; LIST of them at most
+  // are kept, all are counted.
+  __device__ __forceinline__ void list(const Chunk<T>& x, int at, float from, float below) {
+    unsigned mine = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine |= x.get(i) >= from && x.get(i) < below ? 1u << i : 0u;
+    if (!mine) return;
+    uint32_t to = atomicAdd(&sh.listed, (uint32_t)__popc(mine));
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (mine >> i & 1u) {
+        if (to < (uint32_t)LIST) own_list[to] = Entry{(uint32_t)(at + i), off_of(x.get(i))};
+        ++to;
       }
-      start += n;
+  }
+  // The cluster's lists, with their weights, where this CTA's histogram was; their
+  // length, or -1 where they are longer than `most`.
+  __device__ int gather(int most) {
+    sync();  // lists are complete, histograms have been read
+    int n = 0;
+    if (lane < ctas) n = (int)ld_remote(lpc::mapa_shared(lpc::smem_u32(&sh.listed), lane));
+    int upto = n;  // inclusive
+#pragma unroll
+    for (int d = 1; d < MAX_CLUSTER; d <<= 1) {
+      const int o = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += o;
+    }
+    const int total = __shfl_sync(~0u, upto, MAX_CLUSTER - 1);
+    if (total > most) return -1;
+    Listed* all = reinterpret_cast<Listed*>(hist);
+    for (int i0 = 0; i0 < total; i0 += THREADS) {
+      const int i = i0 + (int)threadIdx.x;
+      int r = 0, start = 0;  // the list that has element i
+#pragma unroll
+      for (int x = 0; x < MAX_CLUSTER; ++x) {
+        const int end_x = __shfl_sync(~0u, upto, x);
+        if (i >= end_x) {
+          r = x + 1;
+          start = end_x;
+        }
+      }
+      if (i < total) {
+        const uint32_t from = lpc::mapa_shared(lpc::smem_u32(own_list + (i - start)), r);
+        const uint32_t index = ld_remote(from), off = ld_remote(from + 4u);
+        all[i] = Listed{(uint64_t)off << 32 | index, weight<false>(at_off(off))};
+      }
     }
     __syncthreads();
     return total;
   }
 
-  // One round of the select: sums of `measure` in bins of 2^shift of the offset
-  // from the largest, over offsets [lo, hi]; finds the first bin whose running
-  // sum, begun at `above`, exceeds target(above + total).  False: none does.
+  // The smallest x in [lo, hi] up to which the listed elements (key(place) <= x, those with
+  // an offset of `only` where that is not ~0), on top of `before`, weigh more than target; hi
+  // if none.  A warp a pivot.
+  __device__ uint32_t search(int n, bool by_index, uint32_t only, uint32_t lo, uint32_t hi,
+                             uint64_t before, uint64_t target) {
+    const Listed* all = reinterpret_cast<const Listed*>(hist);
+    while (lo < hi) {
+      const uint32_t x = lo + (uint32_t)((uint64_t)(hi - lo) * (uint32_t)warp / WARPS);
+      uint64_t sum = 0;
+      for (int i = lane; i < n; i += 32) {
+        const uint64_t place = all[i].place;
+        const uint32_t off = (uint32_t)(place >> 32);
+        if (by_index ? off == only && (uint32_t)place <= x : off <= x) sum += all[i].weight;
+      }
+      sum = warp_sum(sum);
+      if (lane == 0) sh.scan[warp] = before + sum > target;
+      __syncthreads();
+      const unsigned over = __ballot_sync(~0u, lane < WARPS && sh.scan[lane & (WARPS - 1)] != 0);
+      const int s = over ? __ffs(over) - 1 : WARPS;  // the first pivot that is enough
+      const uint32_t range = hi - lo, old = lo;
+      if (s < WARPS) hi = old + (uint32_t)((uint64_t)range * (uint32_t)s / WARPS);
+      if (s > 0) lo = old + (uint32_t)((uint64_t)range * (uint32_t)(s - 1) / WARPS) + 1u;
+      __syncthreads();
+    }
+    return hi;
+  }
+  // The listed elements' weight up to an offset, without it.
+  __device__ uint64_t listed_before(int n, uint32_t off) const {
+    const Listed* all = reinterpret_cast<const Listed*>(hist);
+    uint64_t sum = 0;
+    for (int i = lane; i < n; i += 32)
+      if ((uint32_t)(all[i].place >> 32) < off) sum += all[i].weight;
+    return warp_sum(sum);
+  }
+
+  // One round of the radix select: sums of counts or weights in bins of 2^shift of the
+  // offset from the largest, over offsets [lo, hi].  Crossing as above.
   template <bool MASS, typename G>
-  __device__ bool round(uint32_t lo, uint32_t hi, int shift, uint64_t above, G target_of) {
-    uint32_t* h = hist[turn];
-    turn ^= 1;
-    for (int i = threadIdx.x; i < BINS * (MASS ? 2 : 1); i += THREADS) h[i] = 0u;
+  __device__ int round(uint32_t lo, uint32_t hi, int shift, uint64_t above, G target_of) {
+    sync();  // the histogram before has been read
+    for (int i = threadIdx.x; i < BINS * 2; i += THREADS) hist[i] = 0u;
     __syncthreads();
-    for (int c = warp * segment + lane; c < min(nchunks, (warp + 1) * segment); c += 32) {
-      const Chunk<T> x = chunk(c);
+    each([&](const Chunk<T>& x, int) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float f = x.get(i);
-        const uint32_t off = (uint32_t)kmax - (uint32_t)order_of(f);
+        const uint32_t off = off_of(f);
         if (off - lo <= hi - lo && f != -INFINITY) {
           const uint32_t bin = (off - lo) >> shift;
-          if constexpr (MASS) {
-            const uint64_t w = weight<false>(f);
-            if (w) {
-              const uint32_t was = atomicAdd(h + bin, (uint32_t)w);
-              const uint32_t up = (uint32_t)(w >> 32) + (was + (uint32_t)w < was ? 1u : 0u);
-              if (up) atomicAdd(h + BINS + bin, up);
-            }
-          } else {
-            atomicAdd(h + bin, 1u);
-          }
+          const uint64_t w = MASS ? weight<false>(f) : 1ull;
+          const uint32_t was = atomicAdd(hist + bin, (uint32_t)w);
+          const uint32_t up = (uint32_t)(w >> 32) + (was + (uint32_t)w < was ? 1u : 0u);
+          if (up) atomicAdd(hist + BINS + bin, up);
         }
       }
+    });
+    sync();
+    return crossing<true>(above, target_of);
+  }
+  // Offset, sum before it and sum at it of the first value, of offsets up to `last`, at
+  // which the running sum exceeds target(total); false: none does.
+  template <bool MASS, typename G>
+  __device__ bool select(uint32_t last, G target_of, uint32_t& off, uint64_t& before, uint64_t& in) {
+    constexpr int G0 = GRAIN<T>;
+    uint32_t lo = 0, hi = last;
+    uint64_t above = 0, target = 0;
+    bool known = false;
+    for (int shift = 21;;) {
+      auto goal = [&](uint64_t total) { return known ? target : (target = target_of(total)); };
+      const int bin = round<MASS>(lo, hi, shift, above, goal);
+      if (bin < 0) return false;
+      known = true;
+      lo += (uint32_t)bin << shift;
+      above = sh.cross[1];
+      if (shift == G0) break;
+      hi = min(hi, lo + ((1u << shift) - 1u));
+      shift = max(G0, shift - 11);
     }
-    if (threadIdx.x == 0) sh.cross_bin = -1;
-    lpc::cluster_sync();
-    // four bins a thread, summed over the cluster
-    uint64_t v[4] = {0, 0, 0, 0};
-    const uint32_t at = lpc::smem_u32(h + 4 * threadIdx.x);
-    for (int r = 0; r < ctas; ++r) {
-      const uint32_t from = lpc::mapa_shared(at, r);
-      const uint4 l = ld_remote16(from);
-      v[0] += l.x, v[1] += l.y, v[2] += l.z, v[3] += l.w;
-      if constexpr (MASS) {
-        const uint4 u = ld_remote16(from + BINS * 4);
-        v[0] += (uint64_t)u.x << 32, v[1] += (uint64_t)u.y << 32;
-        v[2] += (uint64_t)u.z << 32, v[3] += (uint64_t)u.w << 32;
-      }
-    }
-    const uint64_t own = v[0] + v[1] + v[2] + v[3];
-    uint64_t run = warp_scan(own, lane);
-    if (lane == 31) sh.scan[warp] = run;
-    __syncthreads();
-    uint64_t others = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
-      const uint64_t s = sh.scan[i];
-      total += s;
-      if (i < warp) others += s;
-    }
-    const uint64_t target = target_of(above + total);
-    run += above + others - own;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (run <= target && target < run + v[i]) {
-        sh.cross_bin = 4 * (int)threadIdx.x + i;
-        sh.cross_before = run;
-        sh.cross_in = v[i];
-      }
-      run += v[i];
-    }
-    __syncthreads();
-    return sh.cross_bin >= 0;
+    off = lo;
+    before = above;
+    in = sh.cross[2];
+    return true;
   }
 };
 
-struct Count { static constexpr bool value = false; };
-struct Mass { static constexpr bool value = true; };
-
-static_assert(BINS == 4 * THREADS, "four bins a thread");
-
-// The token of a row of which the list (n elements, in hist[0]) holds the first top_k of
-// the order.  One CTA, every thread.
+// The token of a row of which the list (n elements, where the histogram was) holds the
+// first top_k of the order.  One CTA, every thread.
 template <typename T>
-__device__ void draw_from_list(Row<T>& row, int n, int top_k, float top_p, double least, float u,
+__device__ void draw_from_list(Row<T>& row, int n, int top_k, float top_p, float least, float u,
                                int64_t* out) {
   Shared& sh = row.sh;
-  typename Row<T>::Listed* all = reinterpret_cast<typename Row<T>::Listed*>(row.hist[0]);
-  static_assert(LIST <= THREADS, "an element a thread");
-  const int i = threadIdx.x;
-  const bool in = i < n;
-  const uint64_t place = in ? all[i].place : ~0ull, w = in ? all[i].weight : 0ull;
-  uint64_t run = 0;
-  int rank = 0;
-  if (in)
-    for (int j = 0; j < n; ++j)
-      if (all[j].place < place) {
-        run += all[j].weight;
-        ++rank;
-      }
-  bool stays = in && rank < top_k;
-  auto total = [&](uint64_t v) {
+  Listed* all = reinterpret_cast<Listed*>(row.hist);
+  constexpr int EACH = PAIRS / THREADS;
+  uint64_t place[EACH], w[EACH];
+  bool stays[EACH];
+  uint64_t run[EACH];
+  auto total = [&]() {
+    uint64_t v = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) v += stays[e] ? w[e] : 0ull;
     v = warp_sum(v);
     __syncthreads();
     if (row.lane == 0) sh.scan[row.warp] = v;
     __syncthreads();
-    uint64_t s = 0;
+    v = 0;
 #pragma unroll
-    for (int x = 0; x < WARPS; ++x) s += sh.scan[x];
-    return s;
+    for (int x = 0; x < WARPS; ++x) v += sh.scan[x];
+    return v;
   };
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = (int)threadIdx.x + e * THREADS;
+    const bool in = i < n;
+    place[e] = in ? all[i].place : ~0ull;
+    w[e] = in ? all[i].weight : 0ull;
+    run[e] = 0;
+    int rank = 0;
+    if (in)
+#pragma unroll 4
+      for (int j = 0; j < n; ++j)
+        if (all[j].place < place[e]) {
+          run[e] += all[j].weight;
+          ++rank;
+        }
+    stays[e] = in && rank < top_k;
+  }
   if (top_p < 1.f) {
-    const uint64_t target = part_of(top_p, total(stays ? w : 0ull));
-    stays = stays && run <= target;
+    const uint64_t target = part_of(top_p, total());
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) stays[e] = stays[e] && run[e] <= target;
   }
-  double exact = 0;
-  if (in) row.template weight<false>(value_of((int32_t)((uint32_t)row.kmax - (uint32_t)(place >> 32))), exact);
-  stays = stays && exact >= least;
-  const uint64_t target = part_of(u, total(stays ? w : 0ull));
-  // by index from here on
-  if (in) all[i].place = (uint64_t)(uint32_t)place << 32 | (stays ? 1u : 0u);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    stays[e] = stays[e] && row.at_off((uint32_t)(place[e] >> 32)) >= least;
+  const uint64_t target = part_of(u, total());
+  // by index from here on; every thread has read the places
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int i = (int)threadIdx.x + e * THREADS;
+    if (i < n) all[i].place = stays[e] ? (uint64_t)(uint32_t)place[e] : ~0ull;
+  }
   __syncthreads();
-  if (stays) {
-    uint64_t before = 0;
-    for (int j = 0; j < n; ++j)
-      if ((uint32_t)(all[j].place >> 32) < (uint32_t)place && (all[j].place & 1u)) before += all[j].weight;
-    if (before <= target && target < before + w) *out = (int64_t)(uint32_t)place;
-  }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e)
+    if (stays[e]) {
+      const uint64_t at = (uint32_t)place[e];
+      uint64_t before = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j)
+        if (all[j].place < at) before += all[j].weight;
+      if (before <= target && target < before + w[e]) *out = (int64_t)at;
+    }
 }
 
 template <typename T>
@@ -608,28 +790,29 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
   constexpr int N = Chunk<T>::N;
-  Row<T> row(a, sh);
+  Row<T> row(sh);
   row.rank = (int)lpc::cluster_ctarank();
   uint32_t ctas;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
   row.ctas = (int)ctas;
   row.warp = threadIdx.x >> 5;
   row.lane = threadIdx.x & 31;
-  row.hist[0] = reinterpret_cast<uint32_t*>(smem);
-  row.hist[1] = reinterpret_cast<uint32_t*>(smem + HIST_BYTES);
-  row.chunks = reinterpret_cast<uint4*>(smem + 2 * HIST_BYTES);
+  row.hist = reinterpret_cast<uint32_t*>(smem);
+  row.own_list = reinterpret_cast<Entry*>(smem + HIST_BYTES);
+  row.chunks = reinterpret_cast<uint4*>(smem + HIST_BYTES + LIST_BYTES);
   const int64_t r = blockIdx.x / ctas;
 
-  // ---- the share of the row, and the first of the order ----
+  // ---- the share of the row, and its largest ----
   const int begin = min(row.rank * a.slice, a.vocab);
   const int count = min(a.slice, a.vocab - begin);
   const T* src = static_cast<const T*>(a.logits) + r * a.row_stride + begin;
   const int skew = (int)((reinterpret_cast<uintptr_t>(src) & 15u) / sizeof(T));
   row.first = begin - skew;
   row.begin = begin;
-  row.end = begin + max(count, 0);
+  row.end = begin + count;
   row.nchunks = count > 0 ? (skew + count + N - 1) / N : 0;
   row.segment = ((row.nchunks + WARPS - 1) / WARPS + 31) / 32 * 32;
+  if (threadIdx.x < 32) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 32.0) * FIXED;
   lpc::pdl_wait();
   const float u = a.uniforms[r];
   const float temperature = a.temperature ? a.temperature[r] : a.t;
@@ -637,7 +820,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   const float min_p = a.min_p ? a.min_p[r] : a.m;
   const int32_t top_k = a.top_k ? a.top_k[r] : a.k;
   float best = -INFINITY;
-  int best_at = 0;
   const uint4* vec = reinterpret_cast<const uint4*>(src - skew);
   const int seg_end = min(row.nchunks, (row.warp + 1) * row.segment);
   for (int c0 = row.warp * row.segment + row.lane; c0 < seg_end; c0 += 32 * BATCH) {
@@ -654,23 +836,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
       if (c >= seg_end) break;
       const int e0 = c * N - skew;
       Chunk<T> x = xs[j];
-      if (e0 < 0 || e0 + N > count) {
+      if (e0 < 0 || e0 + N > count) {  // the row's ends
         alignas(16) T part[N];
         for (int i = 0; i < N; ++i)
           part[i] = e0 + i >= 0 && e0 + i < count ? src[e0 + i] : Num<T>::from_f(-INFINITY);
         x.raw = *reinterpret_cast<const uint4*>(part);
       }
-      bool nan = false;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float f = x.get(i);
-        nan |= f != f;
-        if (f > best) {
-          best = f;
-          best_at = begin + e0 + i;
-        }
-      }
-      if (nan) {
+      float m = x.largest();
+      if (m != m) {  // NaN counts as -inf
         alignas(16) T part[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -678,205 +851,217 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
           part[i] = Num<T>::from_f(f != f ? -INFINITY : f);
         }
         x.raw = *reinterpret_cast<const uint4*>(part);
+        m = x.largest();
       }
+      best = fmaxf(best, m);
       row.chunks[c] = x.raw;
     }
   }
-  uint64_t mine = ((uint64_t)((uint32_t)order_of(best) ^ 0x80000000u) << 32) | (uint32_t)~best_at;
 #pragma unroll
-  for (int m = 16; m; m >>= 1) mine = max(mine, shfl_xor64(mine, m));
+  for (int m = 16; m; m >>= 1) best = fmaxf(best, __shfl_xor_sync(~0u, best, m));
   // every CTA of the cluster has to have started before its memory is written
-  lpc::cluster_sync();
-  if (row.lane < row.ctas)
-    st_remote64(lpc::mapa_shared(lpc::smem_u32(&sh.sums[0][row.rank * WARPS + row.warp]), row.lane),
-                mine);
-  row.slot = 1;
-  lpc::cluster_sync();
-  mine = 0;
-  for (int i = row.lane; i < row.ctas * WARPS; i += 32) mine = max(mine, sh.sums[0][i]);
+  row.sync();
+  {
+    const uint64_t* all = row.exchange(__float_as_uint(best));
+    best = -INFINITY;
+    for (int i = row.lane; i < row.ctas * WARPS; i += 32) best = fmaxf(best, __uint_as_float((uint32_t)all[i]));
 #pragma unroll
-  for (int m = 16; m; m >>= 1) mine = max(mine, shfl_xor64(mine, m));
-
-  row.kmax = (int32_t)((uint32_t)(mine >> 32) ^ 0x80000000u);
-  const int32_t kmax = row.kmax;
+    for (int m = 16; m; m >>= 1) best = fmaxf(best, __shfl_xor_sync(~0u, best, m));
+  }
   const bool bad = !(temperature >= 0.f && temperature < INFINITY) || !(u >= 0.f && u < 1.f) ||
                    !(top_p > 0.f && top_p <= 1.f) || !(min_p >= 0.f && min_p <= 1.f);
-  const bool none = kmax == order_of(-INFINITY);
-  if (bad || none || temperature == 0.f) {  // the same for the whole cluster
+  if (bad || best == -INFINITY) {  // the same for the whole cluster
     if (row.rank == 0 && threadIdx.x == 0) {
       if (bad) atomicOr(&g_sample_status, LPC_DEV_ERR_BOUNDS);
-      a.out[r] = bad || none ? -1 : (int64_t)(uint32_t)~(uint32_t)mine;
+      a.out[r] = -1;
     }
     return;
   }
-  row.topf = value_of(kmax);
+  if (temperature == 0.f) {
+    uint64_t at = ~0ull;
+    row.each([&](const Chunk<T>& x, int i0) {
+#pragma unroll
+      for (int i = N - 1; i >= 0; --i)
+        if (x.get(i) == best) at = min(at, (uint64_t)(i0 + i));
+    });
+    const uint64_t* all = row.exchange(warp_min(at));
+    if (row.rank == 0 && row.warp == 0) {
+      at = ~0ull;
+      for (int i = row.lane; i < row.ctas * WARPS; i += 32) at = min(at, all[i]);
+      at = warp_min(at);
+      if (row.lane == 0) a.out[r] = (int64_t)at;
+    }
+    return;
+  }
+  if (best == INFINITY) {  // infinities weigh alike, the others nothing
+    row.each_own([&](Chunk<T>& x) {
+      alignas(16) T part[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) part[i] = Num<T>::from_f(x.get(i) == INFINITY ? 0.f : -INFINITY);
+      x.raw = *reinterpret_cast<const uint4*>(part);
+    });
+    best = 0.f;
+  }
+  row.kmax = order_of(best);
+  row.topf = value_of(row.kmax);
   row.top = (double)row.topf;
-  const double per_unit = 1.4426950408889634074 / (double)temperature;
+  // no steeper than what leaves the float below the largest nothing, so that every float's
+  // exponent stays a small integer
+  const double step = row.top - (double)value_of(row.kmax - 1);
+  const double per_unit = fmin(1.4426950408889634074 / (double)temperature, 61.0 / step);
   row.scale = 32.0 * per_unit;
+  row.floorf = fmaxf(__double2float_rd(row.top - 60.0 / per_unit), -3.402823466e38f);
   row.octaves = (float)(-OCTAVE * per_unit);
   row.lowest = (float)(-(BINS - 1) / (OCTAVE * per_unit));
-  if (threadIdx.x < 32) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 32.0) * FIXED;
   __syncthreads();
   row.tab_lo = (uint32_t)__double2loint(sh.table[row.lane]);
-  row.tab_hi = (uint32_t)__double2hiint(sh.table[row.lane]);
-  // where fp32 has the bins: not for infinities, nor for temperatures that nobody uses
+  row.tab_hi = (uint32_t)__double2hiint(sh.table[row.lane]) - (uint32_t)row.lane * 32768u;
+  // where fp32 has the bins: not for temperatures that nobody uses
   const bool binned = fabsf(row.topf) < 1e30f && per_unit < 1e25 && per_unit > 1e-25;
-  const double least = (double)min_p * FIXED;
+  // min-p: the smallest logit that weighs enough
+  float least = -INFINITY;
+  if (min_p > 0.f)
+    least = row.smallest([&](float f) {
+      double exact;
+      row.template weight<false>(f, &exact);
+      return exact >= (double)min_p * FIXED;
+    });
 
-  // ---- the place in the order up to which logits stay: offsets from the
-  // largest below `cut`, and `ties` of the ones at it (-1: all) ----
-  constexpr int G = GRAIN<T>;
-  const uint32_t off_all = (uint32_t)kmax - (uint32_t)order_of(-INFINITY) - 1u;
-  uint32_t cut = off_all;
-  uint64_t ties = ~0ull, present = ~0ull;  // kept at `cut`, and all there are
-  // offset, sum before it and sum at it of the first value at which the
-  // running sum exceeds the target
-  auto select = [&](auto mass, uint32_t last, auto target_of, uint32_t& off, uint64_t& before,
-                    uint64_t& in) -> bool {
-    constexpr bool MASS = decltype(mass)::value;
-    uint32_t lo = 0, hi = last;
-    uint64_t above = 0, target = 0;
-    bool known = false;
-    for (int shift = 21;;) {
-      auto goal = [&](uint64_t total) { return known ? target : (target = target_of(total)); };
-      if (!row.template round<MASS>(lo, hi, shift, above, goal)) return false;
-      known = true;
-      lo += (uint32_t)sh.cross_bin << shift;
-      above = sh.cross_before;
-      if (shift == G) break;
-      hi = min(hi, lo + ((1u << shift) - 1u));
-      shift = max(G, shift - 11);
-    }
-    off = lo;
-    before = above;
-    in = sh.cross_in;
-    return true;
-  };
+  // ---- the place in the order up to which logits stay: values above `cut`, and of
+  // those at it the ones with an index up to `last` ----
+  float cut = -3.402823466e38f;
+  int last = a.vocab;
+  // the same as an offset from the largest, how many stay of those at it (~0: all), and
+  // how many there are
+  uint32_t cut_off = row.off_of(cut);
+  uint64_t ties = ~0ull, present = ~0ull;
   if (top_k > 0 && top_k < a.vocab) {
-    // at most LIST elements in the bins down to the one of the last: all on the list
-    uint64_t v[4];
-    if (top_k <= LIST && binned) {
-      row.template histogram<false>(v);
-      const int bin = row.crossing(v, (uint64_t)top_k - 1u);
-      if (bin >= 0 && sh.cross_before + sh.cross_in <= (uint64_t)LIST) {
-        row.each([&](const Chunk<T>& x, int at, bool in) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float f = x.get(i);
-            row.list(in && row.bin_of(f) <= (uint32_t)bin, f, at + i);
-          }
+    // few elements in the bins down to the one of the last: all on the list
+    if (top_k <= PAIRS && binned) {
+      row.template histogram<false>();
+      const int bin = row.template crossing<false>(0, [&](uint64_t) { return (uint64_t)top_k - 1u; });
+      if (bin >= 0 && sh.cross[1] + sh.cross[2] <= (uint64_t)PAIRS) {
+        const float from = row.smallest([&](float f) { return row.bin_of(f) <= (uint32_t)bin; });
+        row.each([&](const Chunk<T>& x, int at) {
+          if (x.largest() >= from) row.list(x, at, from, INFINITY);
         });
-        const int n = row.gather();
-        lpc::cluster_sync();  // the lists have been read: the others may go
+        const int n = row.gather(PAIRS);
+        row.sync();  // the lists have been read: the other CTAs may go
         if (row.rank == 0) draw_from_list(row, n, top_k, top_p, least, u, a.out + r);
         return;
       }
     }
-    lpc::cluster_sync();  // histograms have been read
     uint64_t before, in;
-    if (select(Count{}, cut, [&](uint64_t) { return (uint64_t)top_k - 1u; }, cut, before, in)) {
+    if (row.template select<false>(cut_off, [&](uint64_t) { return (uint64_t)top_k - 1u; }, cut_off,
+                                   before, in)) {
       ties = (uint64_t)top_k - before;
       present = in;
     }
-    lpc::cluster_sync();
   }
   uint64_t mine_kept = 0;  // this warp's sum of the weights that stay, where it is known
   bool known = false;
-  int last = a.vocab;      // highest index that stays of those at `cut`
   if (top_p < 1.f && ties == ~0ull && binned) {
-    uint64_t v[4];
-    row.template histogram<true>(v);
-    if (row.window(v, top_p)) {
-      const uint32_t w0 = sh.window[0], w1 = sh.window[1];
-      uint64_t all = 0, above = 0, kept = 0;
-      row.each([&](const Chunk<T>& x, int at, bool in) {
+    if (top_k > 0 && top_k < a.vocab) row.sync();  // a histogram before has been read
+    row.template histogram<true>();
+    if (row.window(top_p)) {
+      const uint32_t w0 = (uint32_t)sh.window[0], w1 = (uint32_t)sh.window[1];
+      const float above_from = w0 == 0 ? INFINITY : row.smallest([&](float f) { return row.bin_of(f) < w0; });
+      const float list_from = row.smallest([&](float f) { return row.bin_of(f) <= w1; });
+      uint64_t all = 0, above = 0;
+      row.each([&](const Chunk<T>& x, int at) {
+        uint64_t w[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = row.template weight<true>(x.get(i));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const float f = x.get(i);
-          double exact;
-          uint64_t w = row.template weight<true>(f, exact);
-          w = in ? w : 0ull;
-          const uint32_t bin = row.bin_of(f);
-          all += w;
-          above += bin < w0 ? w : 0ull;
-          kept += bin < w0 && exact >= least ? w : 0ull;
-          row.list(in && bin >= w0 && bin <= w1, f, at + i);
+          all += w[i];
+          above += f >= above_from ? w[i] : 0ull;
+          mine_kept += f >= above_from && f >= least ? w[i] : 0ull;
         }
+        row.list(x, at, list_from, above_from);
       });
-      mine_kept = warp_sum(kept);
-      const uint64_t total = row.exchange(warp_sum(all));
-      const uint64_t before = row.exchange(warp_sum(above));
-      const int n = row.gather();
-      if (n >= 0) {
+      mine_kept = warp_sum(mine_kept);
+      const uint64_t total = row.total_of(row.exchange(warp_sum(all)));
+      const uint64_t before = row.total_of(row.exchange(warp_sum(above)));
+      const int n = row.gather(LIST);
+      if (n > 0) {
         const uint64_t target = part_of(top_p, total);
-        if (threadIdx.x == 0) sh.cut = 0;
-        __syncthreads();
-        typename Row<T>::Listed* all_listed = reinterpret_cast<typename Row<T>::Listed*>(row.hist[0]);
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-          const uint64_t place = all_listed[i].place;
-          uint64_t run = before;
-          for (int j = 0; j < n; ++j)
-            if (all_listed[j].place < place) run += all_listed[j].weight;
-          if (run <= target) atomicMax(&sh.cut, (unsigned long long)place + 1ull);
-        }
-        __syncthreads();
-        const uint64_t place = sh.cut;  // 1 more than the last that stays
-        if (place) {
-          cut = (uint32_t)((place - 1) >> 32);
+        const Listed* listed = reinterpret_cast<const Listed*>(row.hist);
+        // the first value, and of those like it the first index, at which the sum passes:
+        // the last that stays
+        const uint32_t off0 = w0 == 0 ? 0u : row.off_of(above_from), off1 = row.off_of(list_from);
+        const uint32_t off = row.search(n, false, 0u, off0, off1, before, target);
+        const uint64_t upto = before + row.listed_before(n, off);
+        const uint32_t index = row.search(n, true, off, 0u, (uint32_t)a.vocab, upto, target);
+        const uint64_t place = index < (uint32_t)a.vocab ? ((uint64_t)off << 32 | index) + 1ull : 0ull;
+        if (place) {  // 1 more than the last that stays
+          cut = row.at_off((uint32_t)((place - 1) >> 32));
           last = (int)(uint32_t)(place - 1);
           // the list's elements that stay, to the warps that have them
           uint64_t more = 0;
           const int lo = max(row.begin, row.first + row.warp * row.segment * N);
           const int hi = min(row.end, row.first + (row.warp + 1) * row.segment * N);
           for (int i = row.lane; i < n; i += 32) {
-            const uint64_t e = all_listed[i].place;
+            const uint64_t e = listed[i].place;
             const int at = (int)(uint32_t)e;
-            double exact;
-            row.template weight<false>(value_of((int32_t)((uint32_t)kmax - (uint32_t)(e >> 32))), exact);
-            if (e < place && at >= lo && at < hi && exact >= least) more += all_listed[i].weight;
+            if (e < place && at >= lo && at < hi && row.at_off((uint32_t)(e >> 32)) >= least)
+              more += listed[i].weight;
           }
           mine_kept += warp_sum(more);
           known = true;
         }
       }
     }
-    lpc::cluster_sync();  // histograms and lists have been read
   }
-  if (top_p < 1.f && !known) {
-    // of the last value's weight only `ties` count
-    const uint64_t w_cut = ties == ~0ull ? 0 : row.template weight<false>(value_of((int32_t)((uint32_t)kmax - cut)));
-    const uint64_t extra = ties == ~0ull ? 0 : (present - ties) * w_cut;
-    uint32_t off;
-    uint64_t before, in;
-    uint64_t target = 0;
-    if (select(Mass{}, cut,
-               [&](uint64_t total) { return target = part_of(top_p, total - extra); }, off, before,
-               in)) {
-      const uint64_t w = row.template weight<false>(value_of((int32_t)((uint32_t)kmax - off)));
-      cut = off;
-      ties = (target - before) / w + 1u;
-      present = in / w;
+  if (!known) {
+    if (top_p < 1.f) {
+      // of the last value's weight only `ties` count
+      const uint64_t extra =
+          ties == ~0ull ? 0 : (present - ties) * row.template weight<false>(row.at_off(cut_off));
+      uint64_t before, in, target = 0;
+      uint32_t off;
+      if (row.template select<true>(cut_off,
+                                    [&](uint64_t total) { return target = part_of(top_p, total - extra); },
+                                    off, before, in)) {
+        const uint64_t w = row.template weight<false>(row.at_off(off));
+        cut_off = off;
+        ties = (target - before) / w + 1u;
+        present = in / w;
+      }
+    }
+    cut = row.at_off(cut_off);
+    if (ties < present) {
+      auto tied = [&](float f, int) -> uint64_t { return f == cut; };
+      last = row.locate(row.sum_of(tied), tied, [&](uint64_t) { return ties - 1u; });
     }
   }
-  if (!known && ties < present) {
-    auto tied = [&](float f, int) -> uint64_t { return row.off_of(f) == cut && f != -INFINITY; };
-    last = row.locate(row.sum_of(tied), tied, [&](uint64_t) { return ties - 1u; });
+  if (least > cut) {
+    cut = least;
+    last = a.vocab;
   }
-  auto stays = [&](float f, int at) -> uint64_t {
-    const uint32_t off = row.off_of(f);
-    double exact;
-    const uint64_t w = row.template weight<true>(f, exact);
-    return off > cut || (off == cut && at > last) || !(exact >= least) ? 0ull : w;
-  };
-  if (!known) mine_kept = row.sum_of(stays);
-  const int token = row.locate(mine_kept, stays, [&](uint64_t total) { return part_of(u, total); });
+  int token;
+  auto draw = [&](uint64_t total) { return part_of(u, total); };
+  if (last < a.vocab) {
+    auto stays = [&](float f, int at) -> uint64_t {
+      const uint64_t w = row.template weight<true>(f);
+      return f > cut || (f == cut && at <= last) ? w : 0ull;
+    };
+    token = row.locate(known ? mine_kept : row.sum_of(stays), stays, draw);
+  } else {
+    auto stays = [&](float f, int) -> uint64_t {
+      const uint64_t w = row.template weight<true>(f);
+      return f >= cut ? w : 0ull;
+    };
+    token = row.locate(known ? mine_kept : row.sum_of(stays), stays, draw);
+  }
   if (row.rank == 0 && threadIdx.x == 0) a.out[r] = token;
 }
 
 template <typename T>
 int launch(const Args& args, int64_t rows, int ctas, cudaStream_t s) {
   static std::atomic<uint64_t> mask{0};
-  const int most = 2 * HIST_BYTES + MAX_SLICE_BYTES + 32;
+  const int most = HIST_BYTES + LIST_BYTES + MAX_SLICE_BYTES + 32;
   if (int rc = lpc::once_per_device_smem((const void*)sample_kernel<T>, most, mask)) return rc;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -888,7 +1073,7 @@ int launch(const Args& args, int64_t rows, int ctas, cudaStream_t s) {
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.blockDim = dim3(THREADS);
   // a chunk more than the share: it may begin inside one
-  cfg.dynamicSmemBytes = 2 * HIST_BYTES + ((size_t)args.slice * sizeof(T) + 15) / 16 * 16 + 16;
+  cfg.dynamicSmemBytes = HIST_BYTES + LIST_BYTES + ((size_t)args.slice * sizeof(T) + 15) / 16 * 16 + 16;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
@@ -938,13 +1123,12 @@ extern "C" int lpc_sample_tokens(const void* logits, int64_t row_stride, const f
     set_error("sample_tokens: logits are not aligned to their type");
     return LPC_ERR_INVALID;
   }
-  // CTAs a row: what brings its share to 64 KB (two CTAs an SM then overlap
-  // reading and computing); more while the rows leave SMs idle and a warp still
-  // has a kilobyte
+  // CTAs a row: what brings its share to SLICE_BYTES; more while the rows leave SMs idle
+  // and a warp still has a kilobyte
   int ctas = 1;
   while (ctas < MAX_CLUSTER && vocab * es > (int64_t)ctas * SLICE_BYTES) ctas *= 2;
   while (ctas < MAX_CLUSTER && rows * ctas * 2 <= current_device_sms() &&
-         vocab * es > (int64_t)ctas * WARPS * 512)
+         vocab * es > (int64_t)ctas * WARPS * 1024)
     ctas *= 2;
   Args args;
   args.logits = logits;
