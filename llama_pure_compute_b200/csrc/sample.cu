@@ -35,6 +35,7 @@
 //   * The token: sums of each warp's stretch, a scan over the cluster's warps, and
 //     the warp whose stretch holds the border walks it.
 #include <atomic>
+#include <type_traits>
 
 #include "lpc_common.cuh"
 
@@ -62,15 +63,16 @@ constexpr int BINS = 2048;                       // 11 bits a round
 constexpr int MINE = BINS / THREADS;             // bins a thread, at most
 constexpr int HIST_BYTES = BINS * 8;             // low and high words of a bin's sum
 constexpr int LIST = 1024;                       // elements of a list
-constexpr int PAIRS = 512;                       // elements that are ranked by pairs
+constexpr int PAIRS = 512;                       // elements that are ranked by pairs: of top-k
+constexpr int SHORT = 128;                       // and of top-p (1.5 us; searching 2.5 us or more)
 constexpr int LIST_BYTES = LIST * 8;
 constexpr double FIXED = 17592186044416.0;       // 2^44
 constexpr double ROUND52 = 4503599627370496.0;   // 2^52: adding it rounds to an integer
 constexpr int OCTAVE = 64;                       // bins an octave of the weight
 // What the fp32 histogram may be off, relative to all weights: its elements by 2^-16 of
-// rounding and 4e-6 of fp32 arithmetic, twice, and what lies below its 32 octaves, at most
-// 770,048 * 2^-32 = 1.8e-4.
-constexpr double SLACK = 2.5e-4;
+// rounding and 4e-6 of fp32 arithmetic, twice, their sums by 2048 * 2^-24, twice, and what
+// lies below its 32 octaves, at most 770,048 * 2^-32 = 1.8e-4.
+constexpr float SLACK = 5e-4f;
 constexpr int SLICE_BYTES = 64 * 1024;           // preferred share of a CTA
 constexpr int MAX_SLICE_BYTES = 188 * 1024;
 constexpr int BATCH = 4;                         // 16-byte loads in flight a thread
@@ -215,14 +217,17 @@ struct Shared {
   uint64_t scan[WARPS];
   uint64_t parts[2][MAX_CLUSTER];         // sums of each CTA's bins
   uint64_t cross[3];                      // the crossing bin (~0: none), the sum before it and in it
+  uint64_t last;                          // 1 more than the place of the last that stays (0: none)
   uint64_t window[2];                     // first and last bin that may hold the place
   uint32_t listed;                        // elements that this CTA put on its list
 };
 
-template <typename T>
+// ONE: a CTA a row, else a cluster.
+template <typename T, bool ONE>
 class Row {
  public:
   static constexpr int N = Chunk<T>::N;
+  static constexpr int CTAS = ONE ? 1 : MAX_CLUSTER;  // at most
   Shared& sh;
   uint4* chunks;              // this CTA's share of the row, -inf outside it
   uint32_t* hist;             // BINS low words, BINS high words; or the cluster's list
@@ -243,11 +248,22 @@ class Row {
 
   // Every thread of the cluster.
   __device__ __forceinline__ void sync() const {
-    if (ctas == 1) __syncthreads();
+    if constexpr (ONE) __syncthreads();
     else lpc::cluster_sync();
   }
-  __device__ __forceinline__ void store_all(uint64_t* where, uint64_t v) const {  // in every CTA
-    for (int r = 0; r < ctas; ++r) st_remote64(lpc::mapa_shared(lpc::smem_u32(where), r), v);
+  // In CTA r's shared memory, at the place of `where` in this one's.  The way over the
+  // cluster costs several times a plain access.
+  __device__ __forceinline__ void store(uint64_t* where, int r, uint64_t v) const {
+    if (ONE || r == rank) *where = v;
+    else st_remote64(lpc::mapa_shared(lpc::smem_u32(where), r), v);
+  }
+  __device__ __forceinline__ uint32_t load(const uint32_t* where, int r) const {
+    return ONE || r == rank ? *where : ld_remote(lpc::mapa_shared(lpc::smem_u32(where), r));
+  }
+  __device__ __forceinline__ void store_all(uint64_t* where, uint64_t v) const {
+#pragma unroll
+    for (int r = 0; r < CTAS; ++r)
+      if (ONE || r < ctas) store(where, r, v);
   }
 
   // 2^44 w of a logit, before (`exact`) and after rounding.  ALL: every lane of the warp
@@ -288,10 +304,15 @@ class Row {
   }
 
   // The smallest float for which pass() holds, which holds from some float up to the
-  // largest logit on.  The whole warp.
+  // largest logit on: the 32 around a guess, else all there are.  The whole warp.
   template <typename F>
-  __device__ float smallest(F pass) const {
+  __device__ float smallest(double guess, F pass) const {
     int32_t lo = order_of(-3.402823466e38f), hi = kmax;
+    const int32_t near = order_of((float)fmax(guess, -3e38));
+    if (near > lo + 64 && near < hi - 64) {
+      const unsigned ok = __ballot_sync(~0u, pass(value_of(near - 16 + lane)));
+      if (ok && ok != ~0u) return value_of(near - 16 + __ffs(ok) - 1);
+    }
     while (lo < hi) {
       const uint32_t span = (uint32_t)hi - (uint32_t)lo;
       const int32_t c = (int32_t)((uint32_t)lo + (uint32_t)(((uint64_t)span * (uint32_t)lane) >> 5));
@@ -301,6 +322,12 @@ class Row {
       if (s > 0) lo = __shfl_sync(~0u, c, s - 1) + 1;
     }
     return value_of(hi);
+  }
+
+  // The smallest float of the bins up to `bin`.
+  __device__ float bin_start(int bin, double unit) const {
+    return smallest(top - ((double)bin + 0.5) / OCTAVE * unit,
+                    [&](float f) { return bin_of(f) <= (uint32_t)bin; });
   }
 
   // fn(chunk, index of its first element) for the warp's chunks, every lane of the warp
@@ -336,8 +363,7 @@ class Row {
   __device__ const uint64_t* exchange(uint64_t mine) {
     const int s = slot;
     slot = slot == 2 ? 0 : slot + 1;
-    if (lane < ctas)
-      st_remote64(lpc::mapa_shared(lpc::smem_u32(&sh.sums[s][rank * WARPS + warp]), lane), mine);
+    if (lane < ctas) store(&sh.sums[s][rank * WARPS + warp], lane, mine);
     sync();
     return sh.sums[s];
   }
@@ -387,35 +413,40 @@ class Row {
     found_slot ^= 1;
     if (owner >= 0 && owner / WARPS == rank) {
       const int start = owner % WARPS * segment, stop = min(nchunks, start + segment);
-      const int share = (segment + WARPS - 1) / WARPS;
-      const int from = start + warp * share, to = min(stop, from + share);
-      uint64_t sum = 0;
-      each_of(from, to, [&](const Chunk<T>& x, int at) {
+      int from = start, to = stop;
+      bool mine_it = warp == owner % WARPS;
+      if (segment > 32) {  // several steps of a warp
+        const int share = (segment + WARPS - 1) / WARPS;
+        from = start + warp * share;
+        to = min(stop, from + share);
+        uint64_t sum = 0;
+        each_of(from, to, [&](const Chunk<T>& x, int at) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum += fn(x.get(i), at + i);
-      });
-      sum = warp_sum(sum);
-      if (lane == 0) sh.scan[warp] = sum;
-      __syncthreads();
-      if (crossing_of(sh.scan, WARPS, target, before) == warp) {
+          for (int i = 0; i < N; ++i) sum += fn(x.get(i), at + i);
+        });
+        sum = warp_sum(sum);
+        if (lane == 0) sh.scan[warp] = sum;
+        __syncthreads();
+        mine_it = crossing_of(sh.scan, WARPS, target, before) == warp;
+      }
+      if (mine_it) {
         bool done = false;
         each_of(from, to, [&](const Chunk<T>& x, int at) {
           if (done) return;
-          uint64_t part = 0;
+          uint64_t run[N], part = 0;
 #pragma unroll
-          for (int i = 0; i < N; ++i) part += fn(x.get(i), at + i);
+          for (int i = 0; i < N; ++i) run[i] = part += fn(x.get(i), at + i);
           const uint64_t scan = warp_scan(part, lane);
           const unsigned over = __ballot_sync(~0u, before + scan > target);
           if (over) {
             done = true;
-            uint64_t run = before + scan - part;
-            int found = -1;
+            if (lane == __ffs(over) - 1) {
+              int found = N - 1;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {  // once more, all lanes together
-              run += fn(x.get(i), at + i);
-              if (found < 0 && run > target) found = at + i;
+              for (int i = N - 2; i >= 0; --i)
+                if (before + scan - part + run[i] > target) found = i;
+              store_all(&sh.found[f], (uint64_t)(at + found));
             }
-            if (lane == __ffs(over) - 1) store_all(&sh.found[f], (uint64_t)found);
           } else {
             before += (uint64_t)__shfl_sync(~0u, (uint32_t)scan, 31) |
                       ((uint64_t)__shfl_sync(~0u, (uint32_t)(scan >> 32), 31) << 32);
@@ -462,30 +493,29 @@ class Row {
     sync();
   }
   // Each CTA has BINS / ctas bins of the cluster's, a thread up to MINE of them.
-  __device__ __forceinline__ int bins_a_thread() const { return max(1, MINE / ctas); }
+  __device__ __forceinline__ int bins_a_thread() const { return ONE ? MINE : max(1, MINE / ctas); }
   __device__ __forceinline__ int first_bin() const {
-    return rank * (BINS / ctas) + (int)threadIdx.x * bins_a_thread();
+    return ONE ? MINE * (int)threadIdx.x : rank * (BINS / ctas) + (int)threadIdx.x * bins_a_thread();
   }
   template <bool WIDE>
-  __device__ void merge(uint64_t (&v)[MINE]) const {
+  __device__ __forceinline__ void merge(uint64_t (&v)[MINE]) const {
     const int m = bins_a_thread(), at = first_bin();
-    const bool has = (int)threadIdx.x * m < BINS / ctas;
-    const uint32_t from = lpc::smem_u32(hist + at);
-    uint32_t lo[MAX_CLUSTER], hi[MAX_CLUSTER];
+    const bool has = ONE || (int)threadIdx.x * m < BINS / ctas;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
       v[i] = 0;
       if (!has || i >= m) continue;
+      uint32_t lo[CTAS], hi[CTAS];
 #pragma unroll
-      for (int r = 0; r < MAX_CLUSTER; ++r) {  // all in flight
+      for (int r = 0; r < CTAS; ++r) {  // all in flight
         lo[r] = hi[r] = 0;
-        if (r < ctas) {
-          lo[r] = ld_remote(lpc::mapa_shared(from + 4 * i, r));
-          if constexpr (WIDE) hi[r] = ld_remote(lpc::mapa_shared(from + 4 * BINS + 4 * i, r));
+        if (ONE || r < ctas) {
+          lo[r] = load(hist + at + i, r);
+          if constexpr (WIDE) hi[r] = load(hist + BINS + at + i, r);
         }
       }
 #pragma unroll
-      for (int r = 0; r < MAX_CLUSTER; ++r) v[i] += (uint64_t)hi[r] << 32 | lo[r];
+      for (int r = 0; r < CTAS; ++r) v[i] += (uint64_t)hi[r] << 32 | lo[r];
     }
   }
   // The bin whose running sum, begun at `above`, first exceeds target(above + total)
@@ -510,12 +540,18 @@ class Row {
     run += above - own;
     const int s = part_slot;
     part_slot ^= 1;
-    if (threadIdx.x == 0) store_all(&sh.parts[s][rank], total);
-    sync();
-    total = above;
-    for (int r = 0; r < ctas; ++r) {
-      total += sh.parts[s][r];
-      if (r < rank) run += sh.parts[s][r];
+    if constexpr (ONE) {
+      total += above;
+    } else {
+      if (threadIdx.x == 0) store_all(&sh.parts[s][rank], total);
+      sync();
+      total = above;
+#pragma unroll
+      for (int r = 0; r < CTAS; ++r)
+        if (r < ctas) {
+          total += sh.parts[s][r];
+          if (r < rank) run += sh.parts[s][r];
+        }
     }
     const uint64_t target = target_of(total);
 #pragma unroll
@@ -535,23 +571,27 @@ class Row {
   __device__ bool window(float p) {
     uint64_t v[MINE];
     merge<false>(v);
-    double w[MINE], own = 0;
+    // fp32 from here on: 2^-24 * 2048, far inside SLACK
+    float w[MINE], own = 0;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
-      w[i] = v[i] ? (double)v[i] * (double)exp2f(-(float)(first_bin() + i) / OCTAVE) : 0.0;
+      w[i] = (float)v[i] * exp2f(-(float)(first_bin() + i) / OCTAVE);
       own += w[i];
     }
-    double run = own;
+    float run = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const double o = __shfl_up_sync(~0u, run, d);
+      const float o = __shfl_up_sync(~0u, run, d);
       if (lane >= d) run += o;
     }
-    double* scan = reinterpret_cast<double*>(sh.scan);
+    float* scan = reinterpret_cast<float*>(sh.scan);
     if (lane == 31) scan[warp] = run;
-    if (threadIdx.x == 0) sh.window[0] = sh.window[1] = BINS;
+    if (threadIdx.x == 0) {
+      sh.window[0] = sh.window[1] = BINS;
+      sh.last = 0;
+    }
     __syncthreads();
-    double total = 0;
+    float total = 0;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) {
       if (i < warp) run += scan[i];
@@ -560,15 +600,19 @@ class Row {
     run -= own;
     const int s = part_slot;
     part_slot ^= 1;
-    if (threadIdx.x == 0) store_all(&sh.parts[s][rank], (uint64_t)__double_as_longlong(total));
-    sync();
-    total = 0;
-    for (int r = 0; r < ctas; ++r) {
-      const double x = __longlong_as_double((long long)sh.parts[s][r]);
-      if (r < rank) run += x;
-      total += x;
+    if constexpr (!ONE) {
+      if (threadIdx.x == 0) store_all(&sh.parts[s][rank], __float_as_uint(total));
+      sync();
+      total = 0;
+#pragma unroll
+      for (int r = 0; r < CTAS; ++r)
+        if (r < ctas) {
+          const float x = __uint_as_float((uint32_t)sh.parts[s][r]);
+          if (r < rank) run += x;
+          total += x;
+        }
     }
-    const double lo = ((double)p - SLACK) * total, hi = ((double)p + SLACK) * total;
+    const float lo = (p - SLACK) * total, hi = (p + SLACK) * total;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
       const int bin = first_bin() + i;
@@ -600,7 +644,7 @@ class Row {
   __device__ int gather(int most) {
     sync();  // lists are complete, histograms have been read
     int n = 0;
-    if (lane < ctas) n = (int)ld_remote(lpc::mapa_shared(lpc::smem_u32(&sh.listed), lane));
+    if (lane < ctas) n = (int)load(&sh.listed, lane);
     int upto = n;  // inclusive
 #pragma unroll
     for (int d = 1; d < MAX_CLUSTER; d <<= 1) {
@@ -622,8 +666,8 @@ class Row {
         }
       }
       if (i < total) {
-        const uint32_t from = lpc::mapa_shared(lpc::smem_u32(own_list + (i - start)), r);
-        const uint32_t index = ld_remote(from), off = ld_remote(from + 4u);
+        const uint32_t* from = &own_list[i - start].index;
+        const uint32_t index = load(from, r), off = load(from + 1, r);
         all[i] = Listed{(uint64_t)off << 32 | index, weight<false>(at_off(off))};
       }
     }
@@ -718,8 +762,8 @@ class Row {
 
 // The token of a row of which the list (n elements, where the histogram was) holds the
 // first top_k of the order.  One CTA, every thread.
-template <typename T>
-__device__ void draw_from_list(Row<T>& row, int n, int top_k, float top_p, float least, float u,
+template <typename T, bool ONE>
+__device__ void draw_from_list(Row<T, ONE>& row, int n, int top_k, float top_p, float least, float u,
                                int64_t* out) {
   Shared& sh = row.sh;
   Listed* all = reinterpret_cast<Listed*>(row.hist);
@@ -785,15 +829,15 @@ __device__ void draw_from_list(Row<T>& row, int n, int top_k, float top_p, float
     }
 }
 
-template <typename T>
+template <typename T, bool ONE>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Shared sh;
   constexpr int N = Chunk<T>::N;
-  Row<T> row(sh);
-  row.rank = (int)lpc::cluster_ctarank();
-  uint32_t ctas;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+  Row<T, ONE> row(sh);
+  uint32_t ctas = 1;
+  if constexpr (!ONE) asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+  row.rank = ONE ? 0 : (int)lpc::cluster_ctarank();
   row.ctas = (int)ctas;
   row.warp = threadIdx.x >> 5;
   row.lane = threadIdx.x & 31;
@@ -860,7 +904,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
 #pragma unroll
   for (int m = 16; m; m >>= 1) best = fmaxf(best, __shfl_xor_sync(~0u, best, m));
   // every CTA of the cluster has to have started before its memory is written
-  row.sync();
+  if constexpr (!ONE) row.sync();
   {
     const uint64_t* all = row.exchange(__float_as_uint(best));
     best = -INFINITY;
@@ -908,11 +952,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   // no steeper than what leaves the float below the largest nothing, so that every float's
   // exponent stays a small integer
   const double step = row.top - (double)value_of(row.kmax - 1);
-  const double per_unit = fmin(1.4426950408889634074 / (double)temperature, 61.0 / step);
+  double per_unit = 1.4426950408889634074 / (double)temperature;
+  double unit = 0.69314718055994530942 * (double)temperature;  // 1 / per_unit
+  if (step * per_unit > 61.0) {
+    per_unit = 61.0 / step;
+    unit = step / 61.0;
+  }
   row.scale = 32.0 * per_unit;
-  row.floorf = fmaxf(__double2float_rd(row.top - 60.0 / per_unit), -3.402823466e38f);
+  row.floorf = fmaxf(__double2float_rd(row.top - 60.0 * unit), -3.402823466e38f);
   row.octaves = (float)(-OCTAVE * per_unit);
-  row.lowest = (float)(-(BINS - 1) / (OCTAVE * per_unit));
+  row.lowest = (float)(-(double)(BINS - 1) / OCTAVE * unit);
   __syncthreads();
   row.tab_lo = (uint32_t)__double2loint(sh.table[row.lane]);
   row.tab_hi = (uint32_t)__double2hiint(sh.table[row.lane]) - (uint32_t)row.lane * 32768u;
@@ -921,7 +970,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   // min-p: the smallest logit that weighs enough
   float least = -INFINITY;
   if (min_p > 0.f)
-    least = row.smallest([&](float f) {
+    least = row.smallest(row.top + log2((double)min_p) * unit, [&](float f) {
       double exact;
       row.template weight<false>(f, &exact);
       return exact >= (double)min_p * FIXED;
@@ -941,7 +990,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
       row.template histogram<false>();
       const int bin = row.template crossing<false>(0, [&](uint64_t) { return (uint64_t)top_k - 1u; });
       if (bin >= 0 && sh.cross[1] + sh.cross[2] <= (uint64_t)PAIRS) {
-        const float from = row.smallest([&](float f) { return row.bin_of(f) <= (uint32_t)bin; });
+        const float from = row.bin_start(bin, unit);
         row.each([&](const Chunk<T>& x, int at) {
           if (x.largest() >= from) row.list(x, at, from, INFINITY);
         });
@@ -965,22 +1014,29 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
     row.template histogram<true>();
     if (row.window(top_p)) {
       const uint32_t w0 = (uint32_t)sh.window[0], w1 = (uint32_t)sh.window[1];
-      const float above_from = w0 == 0 ? INFINITY : row.smallest([&](float f) { return row.bin_of(f) < w0; });
-      const float list_from = row.smallest([&](float f) { return row.bin_of(f) <= w1; });
+      const float above_from = w0 == 0 ? INFINITY : row.bin_start((int)w0 - 1, unit);
+      const float list_from = row.bin_start((int)w1, unit);
       uint64_t all = 0, above = 0;
-      row.each([&](const Chunk<T>& x, int at) {
-        uint64_t w[N];
+      const float kept_from = fmaxf(above_from, least);
+      auto pass = [&](auto two) {  // kept apart from above where min-p is higher
+        row.each([&](const Chunk<T>& x, int at) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = row.template weight<true>(x.get(i));
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float f = x.get(i);
-          all += w[i];
-          above += f >= above_from ? w[i] : 0ull;
-          mine_kept += f >= above_from && f >= least ? w[i] : 0ull;
-        }
-        row.list(x, at, list_from, above_from);
-      });
+          for (int i = 0; i < N; ++i) {
+            const float f = x.get(i);
+            const uint64_t w = row.template weight<true>(f);
+            all += w;
+            above += f >= above_from ? w : 0ull;
+            if constexpr (decltype(two)::value) mine_kept += f >= kept_from ? w : 0ull;
+          }
+          row.list(x, at, list_from, above_from);
+        });
+      };
+      if (kept_from > above_from) {
+        pass(std::true_type{});
+      } else {
+        pass(std::false_type{});
+        mine_kept = above;
+      }
       mine_kept = warp_sum(mine_kept);
       const uint64_t total = row.total_of(row.exchange(warp_sum(all)));
       const uint64_t before = row.total_of(row.exchange(warp_sum(above)));
@@ -991,10 +1047,24 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
         // the first value, and of those like it the first index, at which the sum passes:
         // the last that stays
         const uint32_t off0 = w0 == 0 ? 0u : row.off_of(above_from), off1 = row.off_of(list_from);
-        const uint32_t off = row.search(n, false, 0u, off0, off1, before, target);
-        const uint64_t upto = before + row.listed_before(n, off);
-        const uint32_t index = row.search(n, true, off, 0u, (uint32_t)a.vocab, upto, target);
-        const uint64_t place = index < (uint32_t)a.vocab ? ((uint64_t)off << 32 | index) + 1ull : 0ull;
+        uint64_t place = 0;
+        if (n <= SHORT) {
+          if (threadIdx.x < (unsigned)n) {
+            const uint64_t at = listed[threadIdx.x].place, w = listed[threadIdx.x].weight;
+            uint64_t run = before;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j)
+              if (listed[j].place < at) run += listed[j].weight;
+            if (run <= target && target < run + w) sh.last = at + 1u;
+          }
+          __syncthreads();
+          place = sh.last;
+        } else {
+          const uint32_t off = row.search(n, false, 0u, off0, off1, before, target);
+          const uint64_t upto = before + row.listed_before(n, off);
+          const uint32_t index = row.search(n, true, off, 0u, (uint32_t)a.vocab, upto, target);
+          if (index < (uint32_t)a.vocab) place = ((uint64_t)off << 32 | index) + 1u;
+        }
         if (place) {  // 1 more than the last that stays
           cut = row.at_off((uint32_t)((place - 1) >> 32));
           last = (int)(uint32_t)(place - 1);
@@ -1058,17 +1128,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   if (row.rank == 0 && threadIdx.x == 0) a.out[r] = token;
 }
 
-template <typename T>
-int launch(const Args& args, int64_t rows, int ctas, cudaStream_t s) {
+template <typename T, bool ONE>
+int launch_as(const Args& args, int64_t rows, int ctas, cudaStream_t s) {
   static std::atomic<uint64_t> mask{0};
   const int most = HIST_BYTES + LIST_BYTES + MAX_SLICE_BYTES + 32;
-  if (int rc = lpc::once_per_device_smem((const void*)sample_kernel<T>, most, mask)) return rc;
+  if (int rc = lpc::once_per_device_smem((const void*)sample_kernel<T, ONE>, most, mask)) return rc;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = lpc::use_pdl() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.blockDim = dim3(THREADS);
@@ -1076,13 +1146,17 @@ int launch(const Args& args, int64_t rows, int ctas, cudaStream_t s) {
   cfg.dynamicSmemBytes = HIST_BYTES + LIST_BYTES + ((size_t)args.slice * sizeof(T) + 15) / 16 * 16 + 16;
   cfg.stream = s;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, args);
+  cfg.numAttrs = ONE ? 1 : 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T, ONE>, args);
   if (e != cudaSuccess) {
     lpc::set_error("sample_tokens: launch failed: %s", cudaGetErrorString(e));
     return LPC_ERR_CUDA;
   }
   return lpc::check_launch("sample_tokens");
+}
+template <typename T>
+int launch(const Args& args, int64_t rows, int ctas, cudaStream_t s) {
+  return ctas == 1 ? launch_as<T, true>(args, rows, ctas, s) : launch_as<T, false>(args, rows, ctas, s);
 }
 
 }  // namespace
