@@ -55,7 +55,8 @@ namespace {
 
 using lpc::Num;
 
-// 512 threads and shares of 64 KB: two CTAs an SM, so that one reads while the other computes
+// 512 threads and shares of 84 KB at most: two CTAs an SM, so that one reads while the other
+// computes
 constexpr int THREADS = 512;
 constexpr int WARPS = THREADS / 32;
 constexpr int MAX_CLUSTER = 8;
@@ -73,7 +74,7 @@ constexpr int OCTAVE = 64;                       // bins an octave of the weight
 // rounding and 4e-6 of fp32 arithmetic, twice, their sums by 2048 * 2^-24, twice, and what
 // lies below its 32 octaves, at most 770,048 * 2^-32 = 1.8e-4.
 constexpr float SLACK = 5e-4f;
-constexpr int SLICE_BYTES = 64 * 1024;           // preferred share of a CTA
+constexpr int SLICE_BYTES = 84 * 1024;           // preferred share of a CTA
 constexpr int MAX_SLICE_BYTES = 188 * 1024;
 constexpr int BATCH = 4;                         // 16-byte loads in flight a thread
 
@@ -189,6 +190,13 @@ __device__ __forceinline__ uint32_t ld_remote(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
+}
+// The two halves of a barrier of all threads of the cluster.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint64_t warp_min(uint64_t v) {  // over the warp
 #pragma unroll
@@ -359,13 +367,18 @@ class Row {
     }
   }
 
-  // Every warp's `mine`, in sh.sums[the slot before], in the order of the row.
-  __device__ const uint64_t* exchange(uint64_t mine) {
+  // Every warp's `mine` for the whole cluster, in the order of the row: where they are
+  // after the next sync().
+  __device__ const uint64_t* offer(uint64_t mine) {
     const int s = slot;
     slot = slot == 2 ? 0 : slot + 1;
     if (lane < ctas) store(&sh.sums[s][rank * WARPS + warp], lane, mine);
-    sync();
     return sh.sums[s];
+  }
+  __device__ const uint64_t* exchange(uint64_t mine) {
+    const uint64_t* sums = offer(mine);
+    sync();
+    return sums;
   }
   __device__ uint64_t total_of(const uint64_t* sums) const {
     uint64_t v = 0;
@@ -401,10 +414,11 @@ class Row {
   }
 
   // Lowest row index at which the running sum of fn(value, index) exceeds
-  // target(total); `mine` is this warp's sum.  Every thread of the cluster gets it.
-  // total > target.  The CTA that has it shares the warp's stretch out to all its warps.
+  // target(total); `mine` is this warp's sum.  total > target.  It goes to *out, or, if
+  // that is null, to every thread of the cluster.  The CTA that has it shares the warp's
+  // stretch out to all its warps.
   template <typename F, typename G>
-  __device__ int locate(uint64_t mine, F fn, G target_of) {
+  __device__ int locate(uint64_t mine, F fn, G target_of, int64_t* out) {
     const uint64_t* sums = exchange(mine);
     const uint64_t target = target_of(total_of(sums));
     uint64_t before = 0;
@@ -445,7 +459,8 @@ class Row {
 #pragma unroll
               for (int i = N - 2; i >= 0; --i)
                 if (before + scan - part + run[i] > target) found = i;
-              store_all(&sh.found[f], (uint64_t)(at + found));
+              if (out) *out = at + found;
+              else store_all(&sh.found[f], (uint64_t)(at + found));
             }
           } else {
             before += (uint64_t)__shfl_sync(~0u, (uint32_t)scan, 31) |
@@ -454,6 +469,7 @@ class Row {
         });
       }
     }
+    if (out) return 0;
     sync();
     return (int)sh.found[f];
   }
@@ -641,8 +657,8 @@ class Row {
   }
   // The cluster's lists, with their weights, where this CTA's histogram was; their
   // length, or -1 where they are longer than `most`.
+  // After a sync() since they were written and the histograms read.
   __device__ int gather(int most) {
-    sync();  // lists are complete, histograms have been read
     int n = 0;
     if (lane < ctas) n = (int)load(&sh.listed, lane);
     int upto = n;  // inclusive
@@ -856,6 +872,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   row.end = begin + count;
   row.nchunks = count > 0 ? (skew + count + N - 1) / N : 0;
   row.segment = ((row.nchunks + WARPS - 1) / WARPS + 31) / 32 * 32;
+  // every CTA of the cluster has to have started before its memory is written
+  if constexpr (!ONE) cluster_arrive();
   if (threadIdx.x < 32) sh.table[threadIdx.x] = exp2((double)threadIdx.x / 32.0) * FIXED;
   lpc::pdl_wait();
   const float u = a.uniforms[r];
@@ -903,8 +921,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   }
 #pragma unroll
   for (int m = 16; m; m >>= 1) best = fmaxf(best, __shfl_xor_sync(~0u, best, m));
-  // every CTA of the cluster has to have started before its memory is written
-  if constexpr (!ONE) row.sync();
+  if constexpr (!ONE) cluster_wait();
   {
     const uint64_t* all = row.exchange(__float_as_uint(best));
     best = -INFINITY;
@@ -994,6 +1011,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
         row.each([&](const Chunk<T>& x, int at) {
           if (x.largest() >= from) row.list(x, at, from, INFINITY);
         });
+        row.sync();
         const int n = row.gather(PAIRS);
         row.sync();  // the lists have been read: the other CTAs may go
         if (row.rank == 0) draw_from_list(row, n, top_k, top_p, least, u, a.out + r);
@@ -1038,8 +1056,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
         mine_kept = above;
       }
       mine_kept = warp_sum(mine_kept);
-      const uint64_t total = row.total_of(row.exchange(warp_sum(all)));
-      const uint64_t before = row.total_of(row.exchange(warp_sum(above)));
+      const uint64_t* alls = row.offer(warp_sum(all));
+      const uint64_t* aboves = row.exchange(warp_sum(above));
+      const uint64_t total = row.total_of(alls), before = row.total_of(aboves);
       const int n = row.gather(LIST);
       if (n > 0) {
         const uint64_t target = part_of(top_p, total);
@@ -1103,29 +1122,27 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
     cut = row.at_off(cut_off);
     if (ties < present) {
       auto tied = [&](float f, int) -> uint64_t { return f == cut; };
-      last = row.locate(row.sum_of(tied), tied, [&](uint64_t) { return ties - 1u; });
+      last = row.locate(row.sum_of(tied), tied, [&](uint64_t) { return ties - 1u; }, nullptr);
     }
   }
   if (least > cut) {
     cut = least;
     last = a.vocab;
   }
-  int token;
   auto draw = [&](uint64_t total) { return part_of(u, total); };
   if (last < a.vocab) {
     auto stays = [&](float f, int at) -> uint64_t {
       const uint64_t w = row.template weight<true>(f);
       return f > cut || (f == cut && at <= last) ? w : 0ull;
     };
-    token = row.locate(known ? mine_kept : row.sum_of(stays), stays, draw);
+    row.locate(known ? mine_kept : row.sum_of(stays), stays, draw, a.out + r);
   } else {
     auto stays = [&](float f, int) -> uint64_t {
       const uint64_t w = row.template weight<true>(f);
       return f >= cut ? w : 0ull;
     };
-    token = row.locate(known ? mine_kept : row.sum_of(stays), stays, draw);
+    row.locate(known ? mine_kept : row.sum_of(stays), stays, draw, a.out + r);
   }
-  if (row.rank == 0 && threadIdx.x == 0) a.out[r] = token;
 }
 
 template <typename T, bool ONE>
@@ -1197,13 +1214,13 @@ extern "C" int lpc_sample_tokens(const void* logits, int64_t row_stride, const f
     set_error("sample_tokens: logits are not aligned to their type");
     return LPC_ERR_INVALID;
   }
-  // CTAs a row: what brings its share to SLICE_BYTES; more while the rows leave SMs idle
-  // and a warp still has a kilobyte
+  // CTAs a row: what brings its share to SLICE_BYTES.  One is best while it can hold the row,
+  // as a barrier of a cluster costs 0.7 us and a row takes six to nine (one row of 32,000
+  // with top-p: 25 us by 8 CTAs, 14 by one); where it takes several anyway, twice as many
+  // while SMs are idle.
   int ctas = 1;
   while (ctas < MAX_CLUSTER && vocab * es > (int64_t)ctas * SLICE_BYTES) ctas *= 2;
-  while (ctas < MAX_CLUSTER && rows * ctas * 2 <= current_device_sms() &&
-         vocab * es > (int64_t)ctas * WARPS * 1024)
-    ctas *= 2;
+  if (ctas > 1 && ctas < MAX_CLUSTER && rows * ctas * 2 <= current_device_sms()) ctas *= 2;
   Args args;
   args.logits = logits;
   args.row_stride = row_stride;
