@@ -934,11 +934,9 @@ def decode_attention_int4(
 # ---------------------------------------------------------------------------
 # Sampling
 # ---------------------------------------------------------------------------
-def _row_setting(value, name: str, rows: int, index: int, dtype: torch.dtype):
-    """(tensor or None, its address or None, number) of a setting given for all
-    rows or as a tensor with one entry a row."""
-    if not isinstance(value, torch.Tensor):
-        return None, None, value
+def _row_setting(value: torch.Tensor, name: str, rows: int, index: int, dtype: torch.dtype):
+    """A setting with one entry a row, its address, and what stands for the number
+    that holds for all rows."""
     if value.get_device() != index:
         _require_cuda(value, name)
         raise ValueError(f"LlamaPureComputeError: {name} must be on the logits' device.")
@@ -1004,12 +1002,18 @@ def sample_tokens(
         raise ValueError("LlamaPureComputeError: uniforms must have one entry per row.")
     if not uniforms.is_contiguous():
         uniforms = uniforms.contiguous()
-    t, tp, ta = _row_setting(temperature, "temperature", rows, index, torch.float32)
-    k, kp, ka = _row_setting(top_k, "top_k", rows, index, torch.int32)
-    p, pp, pa = _row_setting(top_p, "top_p", rows, index, torch.float32)
-    m, mp, ma = _row_setting(min_p, "min_p", rows, index, torch.float32)
+    t = k = p = m = tp = kp = pp = mp = None
+    ta, ka, pa, ma = temperature, top_k, top_p, min_p
+    if isinstance(ta, torch.Tensor):
+        t, tp, ta = _row_setting(ta, "temperature", rows, index, torch.float32)
+    if isinstance(ka, torch.Tensor):
+        k, kp, ka = _row_setting(ka, "top_k", rows, index, torch.int32)
+    if isinstance(pa, torch.Tensor):
+        p, pp, pa = _row_setting(pa, "top_p", rows, index, torch.float32)
+    if isinstance(ma, torch.Tensor):
+        m, mp, ma = _row_setting(ma, "min_p", rows, index, torch.float32)
     if out is None:
-        out = torch.empty(lead, dtype=torch.int64, device=logits.device)
+        out = uniforms.new_empty(lead, dtype=torch.int64)
     else:
         if out.shape != lead or out.dtype != torch.int64 or out.get_device() != index \
                 or not out.is_contiguous():
@@ -1237,7 +1241,8 @@ def tree_attention(
     _tree_lens(seq_lens, B, index)
     masks, masks_stride = _tree_ints(masks, "masks", B, T, index, torch.int64)
     q = _dense16(q)
-    out = q.new_empty(B, T, H, D)
+    # [B, H, T, D] in the memory of [B, T, H, D]
+    out = q.new_empty_strided(shape, (T * H * D, D, H * D, 1))
     need = _tree_attention_bytes(index, B, T, H, kv_heads, D, max_seq_len, total_rows)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
@@ -1252,7 +1257,7 @@ def tree_attention(
         _lib.check(rc, "tree_attention")
     if B:
         _lib.launch_count += 2 if need else 1
-    return out.transpose(1, 2)
+    return out
 
 
 class LayerCaches:
