@@ -934,57 +934,82 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   }
 }
 
-// Joins the parts of the item that CTA blockIdx.x began: its own second part and the
-// first part of each CTA after it up to the last.  A thread has four columns of a
-// row; a warp reads 8 rows side by side.
-template <typename T, int HD, bool WIDE>
-__global__ void __launch_bounds__(256) tree_join_kernel(const Params p) {
+// Joins the parts of an item: the second part of the CTA that began it and the first part of
+// each CTA after it up to the last.  blockIdx.x is the item, or, where there are more of them
+// than CTAs, the CTA that began it.  A thread has four columns of a row and every LANES-th
+// part, four of them in flight; a warp reads rows side by side.
+template <int HD, int LANES>
+struct Join {
+  static constexpr int THREADS = LANES == 1 ? 256 : 512;
+  static constexpr int ROWS_HERE = THREADS / (HD / 4 * LANES);
+};
+template <typename T, int HD, bool WIDE, int LANES>
+__global__ void __launch_bounds__(Join<HD, LANES>::THREADS) tree_join_kernel(const Params p, int ctas) {
   using S = Shape<HD, WIDE>;
-  constexpr int GROUPS = HD / 4, ROWS_HERE = 256 / GROUPS;
+  constexpr int GROUPS = HD / 4, ROWS_HERE = Join<HD, LANES>::ROWS_HERE;
+  __shared__ int4 s_split;  // the item, its first and last CTA
   lpc::pdl_trigger();
   lpc::pdl_wait();
-  const int c0 = blockIdx.x;
-  const int item = lpc::ld_dep(&p.split[c0].x);
+  const int items = p.batch * p.kv_heads * p.row_blocks;
+  const bool by_item = items <= ctas;
+  if (threadIdx.x == 0) s_split.x = -1;
+  __syncthreads();
+  for (int c = by_item ? (int)threadIdx.x : (int)blockIdx.x; c < ctas; c += by_item ? (int)blockDim.x : ctas) {
+    if (!by_item && threadIdx.x) break;
+    const int item = lpc::ld_dep(&p.split[c].x);
+    if (item >= 0 && (!by_item || item == (int)blockIdx.x))
+      s_split = make_int4(item, c, lpc::ld_dep(&p.split[c].y), 0);
+  }
+  __syncthreads();
+  const int item = s_split.x, c0 = s_split.y, last = s_split.z;
   if (item < 0) return;
-  const int last = lpc::ld_dep(&p.split[c0].y);
   const int rb = item % p.row_blocks, pair = item / p.row_blocks;
   const int b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
   const int prow = (int)blockIdx.y * ROWS_HERE + (int)threadIdx.x % ROWS_HERE;
-  const int group = (int)threadIdx.x / ROWS_HERE;
+  const int group = (int)threadIdx.x / ROWS_HERE % GROUPS;
+  const int which = (int)threadIdx.x / (ROWS_HERE * GROUPS);  // of the LANES
   const int row = rb * S::ITEM_ROWS + prow;
-  if (prow >= S::ITEM_ROWS || row >= p.group * p.nodes || 4 * group >= p.head_dim) return;
-  // four parts at a time: one memory round trip each
+  const bool in = prow < S::ITEM_ROWS && row < p.group * p.nodes && 4 * group < p.head_dim;
   float M = -INFINITY, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = c0; c <= last; c += 4) {
-    float2 x[4];
-    float4 v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = min(c + i, last);
-      const float* part = p.parts + (2 * (int64_t)at + (at == c0 ? 1 : 0)) * S::PART;
-      x[i] = reinterpret_cast<const float2*>(part + (int64_t)S::ITEM_ROWS * HD)[prow];
-      v[i] = reinterpret_cast<const float4*>(part)[group * S::ITEM_ROWS + prow];
-      if (c + i > last) x[i] = make_float2(-INFINITY, 0.f);
-    }
-    const float top = fmaxf(M, fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x)));
-    const float mu = top == -INFINITY ? 0.f : top;
-    const float f = fast_exp2(M - mu);
+  auto add = [&](float m, float l, const float4& v) {  // one more part
+    const float top = fmaxf(M, m), mu = top == -INFINITY ? 0.f : top;
+    const float f = fast_exp2(M - mu), w = fast_exp2(m - mu);
     M = top;
-    L *= f;
-    o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+    L = L * f + w * l;
+    o.x = o.x * f + w * v.x;
+    o.y = o.y * f + w * v.y;
+    o.z = o.z * f + w * v.z;
+    o.w = o.w * f + w * v.w;
+  };
+  if (in)
+    for (int c = c0 + which; c <= last; c += 4 * LANES) {
+      float2 x[4];
+      float4 v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (c + i > last) break;
-      const float w = fast_exp2(x[i].x - mu);
-      L = fmaf(w, x[i].y, L);
-      o.x = fmaf(w, v[i].x, o.x);
-      o.y = fmaf(w, v[i].y, o.y);
-      o.z = fmaf(w, v[i].z, o.z);
-      o.w = fmaf(w, v[i].w, o.w);
+      for (int i = 0; i < 4; ++i) {
+        const int at = min(c + i * LANES, last);
+        const float* part = p.parts + (2 * (int64_t)at + (at == c0 ? 1 : 0)) * S::PART;
+        x[i] = reinterpret_cast<const float2*>(part + (int64_t)S::ITEM_ROWS * HD)[prow];
+        v[i] = reinterpret_cast<const float4*>(part)[group * S::ITEM_ROWS + prow];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i * LANES <= last) add(x[i].x, x[i].y, v[i]);
     }
+  if constexpr (LANES > 1) {
+    constexpr int HERE = ROWS_HERE * GROUPS;
+    __shared__ float4 s_o[LANES][HERE];
+    __shared__ float2 s_ml[LANES][HERE];
+    const int at = (int)threadIdx.x % HERE;
+    s_o[which][at] = o;
+    s_ml[which][at] = make_float2(M, L);
+    __syncthreads();
+    if (which) return;
+#pragma unroll
+    for (int i = 1; i < LANES; ++i) add(s_ml[i][at].x, s_ml[i][at].y, s_o[i][at]);
   }
-  store_row<T>(p, b, kvh, row, 4 * group, o, L);
+  if (in) store_row<T>(p, b, kvh, row, 4 * group, o, L);
 }
 
 // CTAs of a call: one an SM, no more than there can be tiles.
@@ -1110,12 +1135,17 @@ int launch(const TmaDesc4& tq, const TmaDesc4& tk, const TmaDesc4& tv, const Par
   cudaError_t e = cudaLaunchKernelEx(&cfg, tree_attention_kernel<T, HD, WIDE>, tq, tk, tv, p, id_qk,
                                      id_pv);
   if (e == cudaSuccess && plan.join) {
-    constexpr int rows_here = 256 / (HD / 4);
+    // few items have many parts each: eight threads share them (one KV head of 32,000 keys,
+    // 148 parts: 63 us in all by one, see the table of times for eight)
+    const int64_t items = (int64_t)p.batch * p.kv_heads * p.row_blocks;
+    const bool many = plan.grid > 8 * items;
+    const int here = many ? Join<HD, 8>::ROWS_HERE : Join<HD, 1>::ROWS_HERE;
     const int rows = std::min(p.group * p.nodes, S::ITEM_ROWS);
-    cfg.gridDim = dim3((unsigned)plan.grid, (unsigned)((rows + rows_here - 1) / rows_here));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3((unsigned)std::min(items, plan.grid), (unsigned)((rows + here - 1) / here));
+    cfg.blockDim = dim3(many ? Join<HD, 8>::THREADS : Join<HD, 1>::THREADS);
     cfg.dynamicSmemBytes = 0;
-    e = cudaLaunchKernelEx(&cfg, tree_join_kernel<T, HD, WIDE>, p);
+    e = many ? cudaLaunchKernelEx(&cfg, tree_join_kernel<T, HD, WIDE, 8>, p, (int)plan.grid)
+             : cudaLaunchKernelEx(&cfg, tree_join_kernel<T, HD, WIDE, 1>, p, (int)plan.grid);
   }
   if (e != cudaSuccess) {
     lpc::set_error("tree_attention: launch failed: %s", cudaGetErrorString(e));
