@@ -9,9 +9,11 @@ for sm_100a through the C-ABI library ``lib/liblpc_b200.so``.
 from .config import PRESETS, LlamaModelConfig, Precision
 from .int4_cache import Int4KVCache, Int4RaggedKVCache
 from .int4_linear import Int4Weight
-from .ops import (Int4KV, decode_attention, decode_attention_int4, is_cuda_backend_available,
-                  kv_read_int4, rmsnorm_forward, rmsswiglu_forward, rope_forward, rope_kv_append,
-                  rope_kv_append_int4, update_kv_cache)
+from .ops import (Int4KV, LayerCaches, decode_attention, decode_attention_int4,
+                  is_cuda_backend_available, kv_read_int4, rmsnorm_forward, rmsswiglu_forward,
+                  rope_forward, rope_kv_append, rope_kv_append_int4, rope_kv_append_tree,
+                  sample_tokens, tree_accept, tree_attention, update_kv_cache)
+from .tree_decode import BatchedTreeDecoder, DraftTree, TreeCache
 
 __version__ = "0.1.0"
 
@@ -33,4 +35,12 @@ __all__ = [
     "Int4Weight",
     "Int4KVCache",
     "Int4RaggedKVCache",
+    "sample_tokens",
+    "rope_kv_append_tree",
+    "tree_attention",
+    "LayerCaches",
+    "tree_accept",
+    "DraftTree",
+    "TreeCache",
+    "BatchedTreeDecoder",
 ]

@@ -21,7 +21,7 @@ import torch.nn.functional as F
 from .config import LlamaModelConfig
 from .int4_cache import Int4KVCache
 from .kv_manager import KVCacheManager
-from .ops import StepWorkspaces
+from .ops import StepWorkspaces, sample_tokens
 from .ragged_cache import RaggedKVCache
 
 __all__ = ["GenerationConfig", "apply_repetition_penalty", "sample_next_token", "LlamaGenerator",
@@ -36,6 +36,7 @@ class GenerationConfig:
     top_p: float = 0.9
     repetition_penalty: float = 1.0
     eos_token_ids: tuple = ()
+    min_p: float = 0.0
 
 
 def apply_repetition_penalty(logits: torch.Tensor, history: torch.Tensor, penalty: float) -> torch.Tensor:
@@ -50,10 +51,19 @@ def apply_repetition_penalty(logits: torch.Tensor, history: torch.Tensor, penalt
     return logits
 
 
-def sample_next_token(logits: torch.Tensor, *, temperature: float, top_k: int, top_p: float) -> torch.Tensor:
-    """generate.py:58-153: argmax at temperature 0, else top-k / top-p sampling."""
+def sample_next_token(logits: torch.Tensor, *, temperature: float, top_k: int, top_p: float,
+                      min_p: float = 0.0, uniforms: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """generate.py:58-153: argmax at temperature 0, else top-k / top-p sampling.
+
+    With ``min_p`` (tokens of less than that share of the likeliest one's probability are
+    out) or given random numbers ``uniforms`` (fp32, one a row, in [0, 1)) it is
+    ``ops.sample_tokens``."""
     if temperature < 0:
         raise ValueError("temperature must be >= 0")
+    if uniforms is not None or min_p != 0:
+        if uniforms is None:
+            uniforms = torch.rand(logits.shape[:-1], device=logits.device)
+        return sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p).unsqueeze(-1)
     if temperature == 0:
         return torch.argmax(logits, dim=-1, keepdim=True)
     logits = logits / temperature
@@ -159,7 +169,7 @@ class LlamaGenerator:
         logits = self.model(prompt, positions=positions, kv_cache=self.kv_cache, last_token_only=True)
         nl = apply_repetition_penalty(logits[:, -1, :], history[:, :P], generation.repetition_penalty)
         tok = sample_next_token(nl, temperature=generation.temperature, top_k=generation.top_k,
-                                top_p=generation.top_p)
+                                top_p=generation.top_p, min_p=generation.min_p)
         history[:, P] = tok
         hl = P + 1
         tid = int(tok.item())
@@ -171,7 +181,7 @@ class LlamaGenerator:
             logits = self.model(tok, positions=pid, kv_cache=self.kv_cache, last_token_only=True)
             nl = apply_repetition_penalty(logits[:, -1, :], history[:, :hl], generation.repetition_penalty)
             tok = sample_next_token(nl, temperature=generation.temperature, top_k=generation.top_k,
-                                    top_p=generation.top_p)
+                                    top_p=generation.top_p, min_p=generation.min_p)
             history[:, hl] = tok
             hl += 1
             tid = int(tok.item())
@@ -238,13 +248,20 @@ class BatchedGreedyDecoder:
             else:
                 view = _RowView(self.kv, i, j - i)
             logits = self.model(ids, positions=pos, kv_cache=view, last_token_only=True)
-            first[i:j] = torch.argmax(logits[:, -1, :], dim=-1)
+            first[i:j] = self._pick(logits[:, -1, :], i, j, P)
             i = j
         if self.ragged:
             self.kv.select(range(self.B))  # decode steps run on every sequence
+        self._begin(first, lens)
+        return first
+
+    def _pick(self, logits: torch.Tensor, start: int, stop: int, length: int) -> torch.Tensor:
+        """The first tokens of sequences start to stop - 1 after prompts of ``length``."""
+        return torch.argmax(logits, dim=-1)
+
+    def _begin(self, first: torch.Tensor, lens: List[int]) -> None:
         self.positions[:, 0] = torch.tensor(lens, dtype=torch.long, device=self.device)
         self.tokens[:, 0] = first
-        return first
 
     # -- decode --------------------------------------------------------------
     def _step_body(self) -> None:

@@ -1,0 +1,251 @@
+"""Speculative decoding: a drafted tree of tokens a sequence is verified in one forward.
+
+The reference decodes one token a step (src/llama_pure_compute/generate.py:156-333).
+Here a step runs the model on a tree of up to 64 tokens: its root is the token
+sampled last, the others are a drafter's guesses of what follows.  The model draws
+a token after every node; the branch that the draws agree with is kept, so that a
+step yields one token more than it had right guesses.  What is generated has the
+distribution of plain sampling whatever is drafted (the draw at a position has the
+same random number in every tree), and is greedy decoding at temperature 0.
+
+  * ``DraftTree``: the shape of the trees;
+  * ``TreeCache``: the step interface of a ``KVCacheManager`` or ``RaggedKVCache``
+    for a forward over trees (``rope_kv_append_tree``, ``tree_attention``);
+  * ``BatchedTreeDecoder``: prefill, then steps replayed from one CUDA graph, with
+    ``sample_tokens`` and ``tree_accept``.
+"""
+from __future__ import annotations
+
+from typing import Callable, List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from .generate import BatchedGreedyDecoder
+from .kv_manager import KVCacheManager
+from .ops import (MAX_TREE_NODES, LayerCaches, StepWorkspaces, rope_kv_append_tree, sample_tokens,
+                  tree_accept, tree_attention, tree_attention_workspace)
+from .ragged_cache import RaggedKVCache
+
+__all__ = ["DraftTree", "TreeCache", "BatchedTreeDecoder"]
+
+
+class DraftTree:
+    """The shape of a drafted tree: ``parents[t]`` of node t, before it; -1 of the
+    root, node 0.  ``parents`` and ``depths`` (int32 [T]) and ``masks`` (int64 [T],
+    the bits of a node's ancestors and its own) are tensors on ``device``."""
+
+    def __init__(self, parents: Sequence[int], device: Union[str, torch.device] = "cuda"):
+        parents = [int(p) for p in parents]
+        if not 1 <= len(parents) <= MAX_TREE_NODES:
+            raise ValueError(f"a tree has 1 to {MAX_TREE_NODES} nodes")
+        if parents[0] != -1 or any(not 0 <= p < t for t, p in enumerate(parents) if t):
+            raise ValueError("parents must stand before their children, and only node 0 has none")
+        depths, masks = [0], [1]
+        for t in range(1, len(parents)):
+            depths.append(depths[parents[t]] + 1)
+            masks.append(masks[parents[t]] | 1 << t)
+        self.nodes = len(parents)
+        self.max_depth = max(depths)
+        self.device = torch.device(device)
+        self.parents = torch.tensor(parents, dtype=torch.int32, device=self.device)
+        self.depths = torch.tensor(depths, dtype=torch.int32, device=self.device)
+        self.masks = torch.tensor([m - (1 << 64) if m >> 63 else m for m in masks],
+                                  dtype=torch.int64, device=self.device)
+
+    @classmethod
+    def chain(cls, nodes: int, device: Union[str, torch.device] = "cuda") -> "DraftTree":
+        """One branch: the root and ``nodes - 1`` tokens after it."""
+        return cls(range(-1, nodes - 1), device)
+
+
+class TreeCache:
+    """A 16-bit cache for forwards over trees: ``LlamaForCausalLM`` takes it as its
+    ``kv_cache`` with ``input_ids`` [B, T], row b a tree over the sequence of row b
+    (a ragged cache's selection).  The nodes' K and V go to the rows behind the
+    sequence's ``seq_lens`` keys; ``accept`` keeps a branch of them."""
+
+    def __init__(self, kv_cache: Union[KVCacheManager, RaggedKVCache], batch: int, tree: DraftTree):
+        if type(kv_cache) not in (KVCacheManager, RaggedKVCache):
+            raise TypeError("trees need a KVCacheManager or a RaggedKVCache")
+        self.kv, self.batch, self.tree = kv_cache, batch, tree
+        if tree.device.type != kv_cache.device.type or \
+                (tree.parents.get_device() != kv_cache.seq_lens.get_device()):
+            raise ValueError("the tree must be on the cache's device")
+        if isinstance(kv_cache, RaggedKVCache):
+            if batch != len(kv_cache.active_ids):
+                raise ValueError(f"batch of {batch} rows but {len(kv_cache.active_ids)} selected "
+                                 "sequences")
+            # the selection of now: a captured step stays with it
+            self.lens, self._ids = kv_cache.active_lens, kv_cache._idx
+            self.base, self.cap = kv_cache.active_base, kv_cache.active_cap
+        else:
+            if not 0 < batch <= kv_cache.max_batch_size:
+                raise ValueError("batch size exceeds cache capacity")
+            self.lens, self._ids = kv_cache.seq_lens[:batch], None
+            self.base = self.cap = None
+        self.layers = LayerCaches(kv_cache.k_cache, kv_cache.v_cache, self.base, self.cap)
+        self._workspaces = StepWorkspaces()
+
+    # -- the model's step interface ---------------------------------------------
+    @torch.no_grad()
+    def prepare_forward(self, positions: torch.Tensor, ctx, num_heads: int) -> None:
+        B, T = positions.shape
+        if B != self.batch or T != self.tree.nodes:
+            raise ValueError(f"forward of {B} x {T} tokens over {self.batch} trees of "
+                             f"{self.tree.nodes} nodes")
+        ctx.decode = True
+        ctx.fused_qkv_max = 0  # that kernel's rows are its rotary positions
+        ctx.seq_lens = self.lens
+        ctx.workspace = None
+
+    def attend(self, *, layer_idx: int, positions: torch.Tensor, ctx, num_heads: int, scale: float,
+               qkv: Optional[torch.Tensor] = None, x: Optional[torch.Tensor] = None,
+               packed_qkv=None, norm_eps: float = 0.0) -> torch.Tensor:
+        kc, vc = self.kv.k_cache[layer_idx], self.kv.v_cache[layer_idx]
+        q = rope_kv_append_tree(qkv, self.lens, self.tree.depths, ctx.cos_table, ctx.sin_table, kc,
+                                vc, num_heads, self.kv.n_kv_heads, self.base, self.cap)
+        if ctx.workspace is None:
+            ctx.workspace = self._workspaces.get(q.shape, lambda: tree_attention_workspace(q, kc))
+        out = tree_attention(q, kc, vc, self.lens, self.tree.masks, scale, self.base, self.cap,
+                             ctx.workspace)
+        B, H, T, D = out.shape
+        return out.transpose(1, 2).reshape(B, T, H * D)  # a view: it is laid out so
+
+    # -- after the forward --------------------------------------------------------
+    @torch.no_grad()
+    def accept(self, drafted: torch.Tensor, sampled: torch.Tensor, active: Optional[torch.Tensor] = None
+               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """``tree_accept`` in every layer; the sequences' lengths grow by what was
+        accepted (times ``active``, int32 [B], if given: 0 leaves a sequence where it
+        is).  Returns (accepted, tokens, path)."""
+        got = tree_accept(drafted, self.tree.parents, sampled, self.lens, self.layers)
+        self.lens.add_(got[0] if active is None else got[0] * active)
+        if self._ids is not None:
+            self.kv.seq_lens.index_copy_(0, self._ids, self.lens)
+        return got
+
+
+class BatchedTreeDecoder(BatchedGreedyDecoder):
+    """Speculative decoding of a (possibly ragged) batch, one graph replay a step.
+
+    ``drafter(roots)`` gets the tokens sampled last (int64 [B], device) and returns
+    its guesses for nodes 1 to T - 1 (int64 [B, T - 1]); it runs between the steps.
+    ``temperature``, ``top_k``, ``top_p`` and ``min_p`` are those of
+    ``sample_tokens`` (temperature 0: greedy); ``generator`` makes the random
+    numbers, one a sequence and position."""
+
+    def __init__(self, model: torch.nn.Module, kv_cache: Union[KVCacheManager, RaggedKVCache],
+                 batch_size: int, tree: DraftTree,
+                 drafter: Optional[Callable[[torch.Tensor], torch.Tensor]] = None, *,
+                 temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                 generator: Optional[torch.Generator] = None, use_cuda_graph: bool = True,
+                 prefill_chunk: int = 16) -> None:
+        if type(kv_cache) not in (KVCacheManager, RaggedKVCache):
+            raise TypeError("trees need a KVCacheManager or a RaggedKVCache")
+        super().__init__(model, kv_cache, batch_size, use_cuda_graph, prefill_chunk)
+        if tree.nodes > 1 and drafter is None:
+            raise ValueError("a tree of more than its root needs a drafter")
+        self.tree, self.drafter = tree, drafter
+        self.settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        self.generator = generator
+        self.rows = model.config.max_seq_len  # of the rotary tables
+        self.tokens = torch.zeros(batch_size, tree.nodes, dtype=torch.long, device=self.device)
+        self.positions = torch.zeros(batch_size, tree.nodes, dtype=torch.long, device=self.device)
+        self.active = torch.ones(batch_size, dtype=torch.int32, device=self.device)
+        # a random number for the token at each position
+        self.uniforms = torch.zeros(batch_size, self.rows + 1, device=self.device)
+        self.accepted = torch.zeros(batch_size, dtype=torch.int32, device=self.device)
+        self.new_tokens = torch.zeros(batch_size, tree.nodes, dtype=torch.long, device=self.device)
+        self.cache: Optional[TreeCache] = None
+
+    def _pick(self, logits: torch.Tensor, start: int, stop: int, length: int) -> torch.Tensor:
+        return sample_tokens(logits, self.uniforms[start:stop, length], **self.settings)
+
+    @torch.inference_mode()
+    def prefill(self, prompts: Union[torch.Tensor, List[List[int]]]) -> torch.Tensor:
+        """Returns the first generated token of each sequence (device, [B])."""
+        self.uniforms.uniform_(generator=self.generator)
+        first = super().prefill(prompts)
+        self.active.fill_(1)
+        if self.cache is None or self.graph is None:
+            self.cache = TreeCache(self.kv, self.B, self.tree)
+        elif self.ragged:  # the captured step has the lengths of its own selection
+            self.cache.lens.copy_(self.kv.active_lens)
+        return first
+
+    def _begin(self, first: torch.Tensor, lens: List[int]) -> None:
+        self.tokens[:, 0] = first
+
+    def _step_body(self) -> None:
+        cache = self.cache
+        torch.add(cache.lens[:, None], self.tree.depths, out=self.positions)
+        logits = self.model(self.tokens, positions=self.positions, kv_cache=cache)
+        # the token after a node stands one further
+        u = self.uniforms.gather(1, (self.positions + 1).clamp_(max=self.rows))
+        sampled = sample_tokens(logits, u, **self.settings)
+        accepted, tokens, _ = cache.accept(self.tokens, sampled, self.active)
+        self.accepted.copy_(accepted)
+        self.new_tokens.copy_(tokens)
+        self.tokens[:, :1].copy_(tokens.gather(1, (accepted[:, None] - 1).long()))
+
+    @torch.inference_mode()
+    def capture(self) -> None:
+        lens0 = self.cache.lens.clone()
+        tok0 = self.tokens.clone()
+        s = torch.cuda.Stream(self.device)
+        s.wait_stream(torch.cuda.current_stream(self.device))
+        with torch.cuda.stream(s):
+            self._step_body()
+        torch.cuda.current_stream(self.device).wait_stream(s)
+        self.cache.lens.copy_(lens0)
+        self.tokens.copy_(tok0)
+        torch.cuda.synchronize(self.device)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            self._step_body()
+        self.graph = g
+        torch.cuda.synchronize(self.device)
+
+    @torch.inference_mode()
+    def step(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """One forward: (tokens [B, T], accepted [B]) on the device -- sequence b goes on
+        by ``tokens[b, :accepted[b]]``.  Its cache needs T free rows."""
+        if self.cache is None:
+            raise RuntimeError("prefill first")
+        if self.tree.nodes > 1:
+            self.tokens[:, 1:].copy_(self.drafter(self.tokens[:, 0].clone()))
+        if self.use_graph:
+            if self.graph is None:
+                self.capture()
+            self.graph.replay()
+        else:
+            self._step_body()
+        return self.new_tokens, self.accepted
+
+    @torch.inference_mode()
+    def generate(self, prompts, max_new_tokens: int) -> torch.Tensor:
+        """Prefill and steps until every sequence has ``max_new_tokens``; [B,
+        max_new_tokens] ids (device).  Reads the accepted counts after each step."""
+        rows = prompts if isinstance(prompts, torch.Tensor) else list(prompts)
+        caps = self.kv.capacities[:self.B] if self.ragged else [self.kv.max_seq_len] * self.B
+        for r, cap in zip(rows, caps):
+            # the last step may overshoot by a branch, and the sequence goes along, unchanged,
+            # until the others are done
+            most = len(r) + max_new_tokens - 1 + self.tree.max_depth
+            if most + self.tree.nodes > cap:
+                raise ValueError(f"a prompt of {len(r)} and {max_new_tokens} new tokens need "
+                                 f"{most + self.tree.nodes} rows with these trees; the cache has {cap}")
+            if most + self.tree.max_depth >= self.rows:
+                raise ValueError("Requested generation exceeds configured max_seq_len.")
+        out = torch.empty(self.B, max_new_tokens, dtype=torch.long, device=self.device)
+        out[:, 0] = self.prefill(rows)
+        have = [1] * self.B
+        while min(have) < max_new_tokens:
+            tokens, accepted = self.step()
+            for b, n in enumerate(accepted.tolist()):
+                if have[b] < max_new_tokens:
+                    n = min(n, max_new_tokens - have[b])
+                    out[b, have[b]:have[b] + n] = tokens[b, :n]
+                    have[b] += n
+            self.active.copy_(torch.tensor([int(h < max_new_tokens) for h in have], dtype=torch.int32))
+        return out
