@@ -12,8 +12,6 @@
 // Every CTA walks the tree again (a warp, two nodes a lane, one ballot a step):
 // cheaper than a second launch that waits for the first.  The bound is latency: the
 // rows of a branch are a few kilobytes a layer.
-#include <cstring>
-
 #include "lpc_common.cuh"
 
 LPC_DECLARE_STATUS(g_accept_status)
@@ -31,12 +29,13 @@ unsigned int lpc_status_tree_accept(bool clear) {
 namespace {
 
 constexpr int MAX_NODES = 64;
-constexpr int MAX_CACHES = 256;  // K and V of 128 layers a launch
+constexpr int MAX_LAYERS = 128;  // a launch
 constexpr int THREADS = 128;
 constexpr int BATCH = 8;         // rows in flight a thread
 
+template <int LAYERS>
 struct Caches {
-  uint8_t* at[MAX_CACHES];
+  uint8_t* at[2 * LAYERS];  // K and V of each
 };
 
 struct Args {
@@ -54,8 +53,9 @@ struct Args {
   bool report;                           // this launch writes the results
 };
 
-__global__ void __launch_bounds__(THREADS) tree_accept_kernel(const Args a,
-                                                              const __grid_constant__ Caches caches) {
+template <int LAYERS>
+__global__ void __launch_bounds__(THREADS)
+    tree_accept_kernel(const Args a, const __grid_constant__ Caches<LAYERS> caches) {
   __shared__ int32_t s_path[MAX_NODES];
   __shared__ int s_count;
   const int64_t b = blockIdx.y;
@@ -145,6 +145,16 @@ __global__ void __launch_bounds__(THREADS) tree_accept_kernel(const Args a,
   }
 }
 
+template <int LAYERS>
+void launch(dim3 grid, cudaStream_t s, const Args& a, void* const* keys, void* const* values) {
+  Caches<LAYERS> c;
+  for (int l = 0; l < a.caches / 2; ++l) {
+    c.at[2 * l] = static_cast<uint8_t*>(keys[l]);
+    c.at[2 * l + 1] = static_cast<uint8_t*>(values[l]);
+  }
+  tree_accept_kernel<LAYERS><<<grid, THREADS, 0, s>>>(a, c);
+}
+
 }  // namespace
 
 extern "C" int lpc_tree_accept(const int64_t* drafted, const int32_t* parents,
@@ -211,13 +221,7 @@ extern "C" int lpc_tree_accept(const int64_t* drafted, const int32_t* parents,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int done = 0;
   do {
-    const int now = layers - done < MAX_CACHES / 2 ? layers - done : MAX_CACHES / 2;
-    Caches c;
-    memset(&c, 0, sizeof(c));
-    for (int l = 0; l < now; ++l) {
-      c.at[2 * l] = static_cast<uint8_t*>(key_caches[done + l]);
-      c.at[2 * l + 1] = static_cast<uint8_t*>(value_caches[done + l]);
-    }
+    const int now = layers - done < MAX_LAYERS ? layers - done : MAX_LAYERS;
     a.caches = 2 * now;
     a.report = done == 0;
     // a column a thread, until the grid is 16 CTAs an SM deep
@@ -225,7 +229,10 @@ extern "C" int lpc_tree_accept(const int64_t* drafted, const int32_t* parents,
     const int64_t want = now ? (work + THREADS - 1) / THREADS : 1;
     const int64_t most = ((int64_t)current_device_sms() * 16 + batch - 1) / batch;
     const dim3 grid((unsigned)(want < most ? want : most), (unsigned)batch);
-    tree_accept_kernel<<<grid, THREADS, 0, s>>>(a, c);
+    // the addresses travel as kernel parameters: no more of them than there are
+    if (now <= 4) launch<4>(grid, s, a, key_caches + done, value_caches + done);
+    else if (now <= 32) launch<32>(grid, s, a, key_caches + done, value_caches + done);
+    else launch<MAX_LAYERS>(grid, s, a, key_caches + done, value_caches + done);
     if (int rc = check_launch("tree_accept")) return rc;
     done += now;
   } while (done < layers);

@@ -1071,16 +1071,19 @@ def _tree_caches(key_cache, value_cache, seq_base, seq_cap, B: int, index: int):
 
 def _tree_ints(t: torch.Tensor, name: str, B: int, T: int, index: int, dtype=torch.int32):
     """A tensor [B, T], or [T] for all sequences, and its stride between sequences."""
+    shape = t.shape
     if t.get_device() != index:
         _require_cuda(t, name)
         raise ValueError(f"LlamaPureComputeError: {name} must be on the other tensors' device.")
     if t.dtype is not dtype:
         raise TypeError(f"LlamaPureComputeError: {name} must be {dtype}.")
-    if t.shape != (B, T) and t.shape != (T,):
-        raise ValueError(f"LlamaPureComputeError: {name} must be [batch, nodes] or [nodes].")
     if not t.is_contiguous():
         t = t.contiguous()
-    return t, T if t.dim() == 2 else 0
+    if shape == (B, T):
+        return t, T
+    if shape != (T,):
+        raise ValueError(f"LlamaPureComputeError: {name} must be [batch, nodes] or [nodes].")
+    return t, 0
 
 
 def _tree_lens(seq_lens: torch.Tensor, B: int, index: int) -> None:
@@ -1267,7 +1270,7 @@ class LayerCaches:
     ``seq_cap`` (int32), one entry a sequence of the batch."""
 
     __slots__ = ("key_caches", "value_caches", "seq_base", "seq_cap", "kv_heads", "head_dim",
-                 "max_batch", "max_seq_len", "total_rows", "elem_bytes", "index", "_k", "_v")
+                 "max_batch", "max_seq_len", "total_rows", "elem_bytes", "index", "_k", "_v", "_c")
 
     def __init__(self, key_caches: Sequence[torch.Tensor], value_caches: Sequence[torch.Tensor],
                  seq_base: Optional[torch.Tensor] = None, seq_cap: Optional[torch.Tensor] = None):
@@ -1296,6 +1299,9 @@ class LayerCaches:
         pointers = ctypes.c_void_p * len(keys)
         self._k = pointers(*[k.data_ptr() for k in keys])
         self._v = pointers(*[v.data_ptr() for v in values])
+        self._c = (ctypes.addressof(self._k), ctypes.addressof(self._v), len(keys),
+                   _lib.ptr(seq_base), _lib.ptr(seq_cap), self.kv_heads, self.head_dim,
+                   self.max_batch, self.max_seq_len, self.total_rows, self.elem_bytes)
 
 
 def tree_accept(
@@ -1324,22 +1330,25 @@ def tree_accept(
     sequence then has ``seq_lens + accepted`` keys (``seq_lens`` itself stays).
     A branch beyond the sequence's rows is not moved and sets the device status,
     as does a parent that is not before its child (it is taken as having none)."""
-    index = drafted.get_device()
+    index, shape = drafted.get_device(), drafted.shape
     if index < 0:
         _require_cuda(drafted, "drafted")
-    if drafted.dim() != 2:
+    if len(shape) != 2:
         raise ValueError("LlamaPureComputeError: drafted must be [batch, nodes].")
-    B, T = drafted.shape
+    B, T = shape
     if not 1 <= T <= MAX_TREE_NODES:
         raise ValueError(f"LlamaPureComputeError: a tree has 1 to {MAX_TREE_NODES} nodes.")
-    if sampled.shape != (B, T):
+    if sampled.shape != shape:
         raise ValueError("LlamaPureComputeError: sampled must be [batch, nodes].")
-    drafted, _ = _tree_ints(drafted, "drafted", B, T, index, torch.int64)
-    sampled, _ = _tree_ints(sampled, "sampled", B, T, index, torch.int64)
+    if sampled.get_device() != index or sampled.dtype is not torch.int64 \
+            or drafted.dtype is not torch.int64 or not drafted.is_contiguous() \
+            or not sampled.is_contiguous():
+        drafted, _ = _tree_ints(drafted, "drafted", B, T, index, torch.int64)
+        sampled, _ = _tree_ints(sampled, "sampled", B, T, index, torch.int64)
     parents, parents_stride = _tree_ints(parents, "parents", B, T, index)
-    accepted = torch.empty(B, dtype=torch.int32, device=drafted.device)
-    tokens = torch.empty_like(drafted)
-    path = torch.empty(B, T, dtype=torch.int32, device=drafted.device)
+    tokens = drafted.new_empty(shape)
+    path = parents.new_empty(shape)
+    accepted = parents.new_empty(B)
     lens = keys = values = base = cap = None
     layers = kv_heads = head_dim = max_batch = max_seq_len = total_rows = elem = 0
     if caches is not None:
@@ -1350,10 +1359,9 @@ def tree_accept(
         _tree_lens(seq_lens, B, index)
         if B > caches.max_batch:
             raise ValueError("LlamaPureComputeError: batch size exceeds cache capacity.")
-        lens, keys, values, layers = seq_lens.data_ptr(), caches._k, caches._v, len(caches._k)
-        base, cap = _lib.ptr(caches.seq_base), _lib.ptr(caches.seq_cap)
-        kv_heads, head_dim, max_batch = caches.kv_heads, caches.head_dim, caches.max_batch
-        max_seq_len, total_rows, elem = caches.max_seq_len, caches.total_rows, caches.elem_bytes
+        lens = seq_lens.data_ptr()
+        (keys, values, layers, base, cap, kv_heads, head_dim, max_batch, max_seq_len, total_rows,
+         elem) = caches._c
     rc = _lib.call_on(index, _lib.load().lpc_tree_accept, drafted.data_ptr(), parents.data_ptr(),
                       parents_stride, sampled.data_ptr(), lens, keys, values, layers, base, cap,
                       accepted.data_ptr(), tokens.data_ptr(), path.data_ptr(), B, T, kv_heads,
