@@ -76,7 +76,10 @@ constexpr int LAUNCH_REGS = 168, REGS_LOAD = 96, REGS_SOFTMAX = 200;
 static_assert(128 * REGS_LOAD + 256 * REGS_SOFTMAX <= NTHREADS * LAUNCH_REGS,
               "register split exceeds the block's launch allocation");
 
-constexpr int START = 2;                    // tiles that an item's begin and end cost
+// Tiles that an item's begin and end cost: the pipeline fills and drains, O is written.
+// 32 sequences of up to 4096 keys, 8 KV heads of 96 rows: 80.6 us counted as two, 73 as
+// three or four, 67 as five or six; 16 rows, D = 64 and long sequences differ by 3 %.
+constexpr int START = 5;
 
 // What a sequence holds: n keys of context, keys and nodes together up to `end`,
 // `tiles` of them; its cache row 0 (of KV head 0).
@@ -937,14 +940,17 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 // Joins the parts of an item: the second part of the CTA that began it and the first part of
 // each CTA after it up to the last.  blockIdx.x is the item, or, where there are more of them
 // than CTAs, the CTA that began it.  A thread has four columns of a row and every LANES-th
-// part, four of them in flight; a warp reads rows side by side.
+// part, two or four of them in flight; a warp reads rows side by side.
 template <int HD, int LANES>
 struct Join {
   static constexpr int THREADS = LANES == 1 ? 256 : 512;
   static constexpr int ROWS_HERE = THREADS / (HD / 4 * LANES);
+  static constexpr int BATCH = LANES == 1 ? 2 : 4;   // parts in flight a thread
+  static constexpr int BLOCKS = LANES == 1 ? 8 : 2;  // an SM
 };
 template <typename T, int HD, bool WIDE, int LANES>
-__global__ void __launch_bounds__(Join<HD, LANES>::THREADS) tree_join_kernel(const Params p, int ctas) {
+__global__ void __launch_bounds__(Join<HD, LANES>::THREADS, Join<HD, LANES>::BLOCKS)
+    tree_join_kernel(const Params p, int ctas) {
   using S = Shape<HD, WIDE>;
   constexpr int GROUPS = HD / 4, ROWS_HERE = Join<HD, LANES>::ROWS_HERE;
   __shared__ int4 s_split;  // the item, its first and last CTA
@@ -982,19 +988,20 @@ __global__ void __launch_bounds__(Join<HD, LANES>::THREADS) tree_join_kernel(con
     o.z = o.z * f + w * v.z;
     o.w = o.w * f + w * v.w;
   };
+  constexpr int BATCH = Join<HD, LANES>::BATCH;
   if (in)
-    for (int c = c0 + which; c <= last; c += 4 * LANES) {
-      float2 x[4];
-      float4 v[4];
+    for (int c = c0 + which; c <= last; c += BATCH * LANES) {
+      float2 x[BATCH];
+      float4 v[BATCH];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < BATCH; ++i) {
         const int at = min(c + i * LANES, last);
         const float* part = p.parts + (2 * (int64_t)at + (at == c0 ? 1 : 0)) * S::PART;
         x[i] = reinterpret_cast<const float2*>(part + (int64_t)S::ITEM_ROWS * HD)[prow];
         v[i] = reinterpret_cast<const float4*>(part)[group * S::ITEM_ROWS + prow];
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < BATCH; ++i)
         if (c + i * LANES <= last) add(x[i].x, x[i].y, v[i]);
     }
   if constexpr (LANES > 1) {
