@@ -292,6 +292,20 @@ __device__ __forceinline__ float2 ld_remote8(uint32_t addr) {
   return v;
 }
 
+// One thread of the warp, chosen so that the compiler knows it to be one: operands of
+// tcgen05.mma and TMA then go to uniform registers directly.  By `lane == 0` an MMA of 64
+// cycles took 85 to 120 to issue: 3 sequences of 60,000 keys, 512 rows a KV head 369 us, so
+// 339; 32 of up to 4096 keys, 6 KV heads of 26 rows, D = 64 38.6 us, so 35.7.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 template <typename T, int HD, bool WIDE>
 __global__ void __launch_bounds__(NTHREADS, 1)
     tree_attention_kernel(const __grid_constant__ TmaDesc4 tmQ, const __grid_constant__ TmaDesc4 tmK,
@@ -456,7 +470,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n" ::: "memory");
     if (warp == 8) {
       // ---------------- loads ----------------
-      if (lane == 0) {
+      if (elect_one()) {
         bool ok = true;
         uint32_t issued = 0;
         int r = 0;
@@ -498,7 +512,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
     } else if (warp == 9) {
       // ---------------- tensor core ----------------
-      if (lane == 0) {
+      if (elect_one()) {
         bool ok = true;
         uint32_t ring = 0, done[2] = {0, 0}, fixes = 0;  // P tiles of each stream; segments with tails
         int r = 0;
