@@ -77,8 +77,8 @@ static_assert(128 * REGS_LOAD + 256 * REGS_SOFTMAX <= NTHREADS * LAUNCH_REGS,
               "register split exceeds the block's launch allocation");
 
 // Tiles that an item's begin and end cost: the pipeline fills and drains, O is written.
-// 32 sequences of up to 4096 keys, 8 KV heads of 96 rows: 80.6 us counted as two, 73 as
-// three or four, 67 as five or six; 16 rows, D = 64 and long sequences differ by 3 %.
+// 32 sequences of up to 4096 keys, 8 KV heads of 96 rows: 73 us counted as three, 71 as
+// four, 65 as five or six; 16 rows, D = 64 and long sequences differ by 3 %.
 constexpr int START = 5;
 
 // What a sequence holds: n keys of context, keys and nodes together up to `end`,
@@ -967,21 +967,27 @@ __global__ void __launch_bounds__(Join<HD, LANES>::THREADS, Join<HD, LANES>::BLO
     tree_join_kernel(const Params p, int ctas) {
   using S = Shape<HD, WIDE>;
   constexpr int GROUPS = HD / 4, ROWS_HERE = Join<HD, LANES>::ROWS_HERE;
-  __shared__ int4 s_split;  // the item, its first and last CTA
   lpc::pdl_trigger();
   lpc::pdl_wait();
-  const int items = p.batch * p.kv_heads * p.row_blocks;
-  const bool by_item = items <= ctas;
-  if (threadIdx.x == 0) s_split.x = -1;
-  __syncthreads();
-  for (int c = by_item ? (int)threadIdx.x : (int)blockIdx.x; c < ctas; c += by_item ? (int)blockDim.x : ctas) {
-    if (!by_item && threadIdx.x) break;
-    const int item = lpc::ld_dep(&p.split[c].x);
-    if (item >= 0 && (!by_item || item == (int)blockIdx.x))
-      s_split = make_int4(item, c, lpc::ld_dep(&p.split[c].y), 0);
+  int item, c0, last;  // its first and last CTA
+  if (p.batch * p.kv_heads * p.row_blocks > ctas) {
+    c0 = (int)blockIdx.x;
+    const uint2 begun = lpc::ld_dep8(&p.split[c0]);
+    item = (int)begun.x;
+    last = (int)begun.y;
+  } else {
+    __shared__ int2 s_split;  // first and last CTA
+    if (threadIdx.x == 0) s_split.x = -1;
+    __syncthreads();
+    for (int c = (int)threadIdx.x; c < ctas; c += (int)blockDim.x) {
+      const uint2 begun = lpc::ld_dep8(&p.split[c]);
+      if (begun.x == blockIdx.x) s_split = make_int2(c, (int)begun.y);
+    }
+    __syncthreads();
+    c0 = s_split.x;
+    last = s_split.y;
+    item = c0 < 0 ? -1 : (int)blockIdx.x;
   }
-  __syncthreads();
-  const int item = s_split.x, c0 = s_split.y, last = s_split.z;
   if (item < 0) return;
   const int rb = item % p.row_blocks, pair = item / p.row_blocks;
   const int b = pair / p.kv_heads, kvh = pair - b * p.kv_heads;
@@ -1103,13 +1109,17 @@ Plan plan_of(int64_t batch, int64_t nodes, int heads, int kv_heads, int head_dim
   const int sms = lpc::current_device_sms();
   const int64_t items = batch * kv_heads * x.row_blocks;
   const int64_t tiles = ((total_rows > 0 ? total_rows : max_seq_len) + KEYS - 1) / KEYS;  // an item's, at most
-  // A cluster an item, as many CTAs as one wave has; against stretches, whose set-up and
-  // second kernel cost about as much as SAVED tiles.
+  // A cluster an item, as many CTAs as one wave has; against stretches, of which the second
+  // kernel costs about as much as SAVED tiles.  A CTA's own begin costs a tile more than an
+  // item's: of 8 KV heads of 64 rows and up to 250 keys, 32 sequences take 18.8 us (stretches
+  // 21.9), 64 35.0 (35.9), 128 65.3 (61.6); of up to 120 keys, where nothing is joined, 32
+  // take 16.4 (14.6) and 128 56.2 (41.1).
   int e = 0;
   while (e < 3 && (1 << e) < tiles && items <= clusters_at_once(e + 1, sms)) ++e;
   const int64_t at_once = clusters_at_once(e, sms), n = 1 << e;
-  const int64_t of_cluster = (items + at_once - 1) / at_once * ((tiles + n - 1) / n + START);
-  const int64_t of_stretch = (items * (tiles + START) + sms - 1) / sms + SAVED;
+  const int64_t waves = (items + at_once - 1) / at_once;
+  const int64_t of_cluster = waves * ((tiles + n - 1) / n + START + 1) - 1;
+  const int64_t of_stretch = (items * (tiles + START) + sms - 1) / sms + (tiles > 1 ? SAVED : 0);
   x.cluster = of_cluster <= of_stretch ? (int)n : 0;
   x.grid = x.cluster ? items * x.cluster
                      : grid_of(batch, (int64_t)kv_heads * x.row_blocks, max_seq_len, total_rows, sms);
@@ -1157,7 +1167,7 @@ int launch(const TmaDesc4& tq, const TmaDesc4& tk, const TmaDesc4& tv, const Par
                                      id_pv);
   if (e == cudaSuccess && plan.join) {
     // few items have many parts each: eight threads share them (one KV head of 32,000 keys,
-    // 148 parts: 63 us in all by one, see the table of times for eight)
+    // 148 parts: 28 us in all, 63 by one thread)
     const int64_t items = (int64_t)p.batch * p.kv_heads * p.row_blocks;
     const bool many = plan.grid > 8 * items;
     const int here = many ? Join<HD, 8>::ROWS_HERE : Join<HD, 1>::ROWS_HERE;
