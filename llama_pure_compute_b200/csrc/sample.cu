@@ -75,6 +75,7 @@ constexpr int OCTAVE = 64;                       // bins an octave of the weight
 // lies below its 32 octaves, at most 770,048 * 2^-32 = 1.8e-4.
 constexpr float SLACK = 5e-4f;
 constexpr int SLICE_BYTES = 84 * 1024;           // preferred share of a CTA
+constexpr int LONG = 24000;                      // elements of a row worth several CTAs
 constexpr int MAX_SLICE_BYTES = 188 * 1024;
 constexpr int BATCH = 4;                         // 16-byte loads in flight a thread
 
@@ -1214,13 +1215,16 @@ extern "C" int lpc_sample_tokens(const void* logits, int64_t row_stride, const f
     set_error("sample_tokens: logits are not aligned to their type");
     return LPC_ERR_INVALID;
   }
-  // CTAs a row: what brings its share to SLICE_BYTES.  One is best while it can hold the row,
-  // as a barrier of a cluster costs 0.7 us and a row takes six to nine (one row of 32,000
-  // with top-p: 25 us by 8 CTAs, 14 by one); where it takes several anyway, twice as many
-  // while SMs are idle.
-  int ctas = 1;
+  // CTAs a row: what brings its share to SLICE_BYTES; one is best while it can hold the row,
+  // as a barrier of a cluster costs 0.7 us and a row takes six to nine (37 rows of 16,000 with
+  // top-p: 14 us by one CTA each, 18 by two or four).  Few long rows get four or eight, while
+  // that takes half the SMs at most (beyond it clusters wait for one another): one row of
+  // 32,000 11.1 us by one, 6.9 by eight, with top-p 19.5 and 15.5, with top-k 50 11.8 either
+  // way; 16 rows 11.6 by one, 9.3 by four, 8.5 by eight, with top-k 50 12.1, 12.1, 14.3.
+  int ctas = 1, most = MAX_CLUSTER;
   while (ctas < MAX_CLUSTER && vocab * es > (int64_t)ctas * SLICE_BYTES) ctas *= 2;
-  if (ctas > 1 && ctas < MAX_CLUSTER && rows * ctas * 2 <= current_device_sms()) ctas *= 2;
+  while (most > ctas && rows * most * 2 > current_device_sms()) most /= 2;
+  if (vocab > LONG && most >= 4) ctas = most;
   Args args;
   args.logits = logits;
   args.row_stride = row_stride;
