@@ -267,16 +267,22 @@ __device__ __forceinline__ uint64_t node_bits(int count) {
   return count >= 64 ? ~0ull : count <= 0 ? 0ull : (1ull << count) - 1ull;
 }
 
-// Four joined columns of a KV head's query row to the output.
-template <typename T>
+// Joined columns of a KV head's query row, four a time, to the output.
+template <typename T, int FOURS>
 __device__ __forceinline__ void store_row(const Params& p, int b, int kvh, int row, int col,
-                                          const float4& o, float L) {
+                                          const float4 (&o)[FOURS], float L) {
   const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
   const int head = row / p.nodes, node = row - head * p.nodes;
   T* out = static_cast<T*>(p.out) +
            (((int64_t)b * p.nodes + node) * p.heads + kvh * p.group + head) * p.head_dim + col;
-  *reinterpret_cast<uint2*>(out) =
-      make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+  uint32_t x[2 * FOURS];
+#pragma unroll
+  for (int f = 0; f < FOURS; ++f) {
+    x[2 * f] = pack2<T>(o[f].x * inv, o[f].y * inv);
+    x[2 * f + 1] = pack2<T>(o[f].z * inv, o[f].w * inv);
+  }
+  if constexpr (FOURS == 1) *reinterpret_cast<uint2*>(out) = make_uint2(x[0], x[1]);
+  else *reinterpret_cast<uint4*>(out) = make_uint4(x[0], x[1], x[2], x[3]);
 }
 __device__ __forceinline__ float4 ld_remote16(uint32_t addr) {
   float4 v;
@@ -935,7 +941,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       for (int i = 1; i < 8; ++i) M = fmaxf(M, ml[i].x);
       const float mu = M == -INFINITY ? 0.f : M;
       float L = 0.f;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 all[1] = {make_float4(0.f, 0.f, 0.f, 0.f)};
+      float4& o = all[0];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float f = fast_exp2(ml[i].x - mu);
@@ -945,7 +952,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         o.z = fmaf(f, v[i].z, o.z);
         o.w = fmaf(f, v[i].w, o.w);
       }
-      store_row<T>(p, seq, kvh, rb * S::ITEM_ROWS + prow, 4 * group, o, L);
+      store_row<T, 1>(p, seq, kvh, rb * S::ITEM_ROWS + prow, 4 * group, all, L);
     }
     lpc::cluster_sync();  // a CTA's memory stays until all have read it
   }
@@ -953,20 +960,25 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
 // Joins the parts of an item: the second part of the CTA that began it and the first part of
 // each CTA after it up to the last.  blockIdx.x is the item, or, where there are more of them
-// than CTAs, the CTA that began it.  A thread has four columns of a row and every LANES-th
-// part, two or four of them in flight; a warp reads rows side by side.
+// than CTAs, the CTA that began it.  A thread has eight or four columns of a row and every
+// LANES-th part, two or four of them in flight; a warp reads rows side by side.  It is bound
+// by instructions: with four columns a thread throughout, 256 items of 96 rows and two to three
+// parts took 6.3 us, so 4.6.
 template <int HD, int LANES>
 struct Join {
   static constexpr int THREADS = LANES == 1 ? 256 : 512;
-  static constexpr int ROWS_HERE = THREADS / (HD / 4 * LANES);
+  static constexpr int FOURS = LANES == 1 ? 2 : 1;   // four columns each, a thread
+  static constexpr int GROUPS = HD / (4 * FOURS);
+  static constexpr int ROWS_HERE = THREADS / (GROUPS * LANES);
   static constexpr int BATCH = LANES == 1 ? 2 : 4;   // parts in flight a thread
-  static constexpr int BLOCKS = LANES == 1 ? 8 : 2;  // an SM
+  static constexpr int BLOCKS = LANES == 1 ? 6 : 2;  // an SM
 };
 template <typename T, int HD, bool WIDE, int LANES>
 __global__ void __launch_bounds__(Join<HD, LANES>::THREADS, Join<HD, LANES>::BLOCKS)
     tree_join_kernel(const Params p, int ctas) {
   using S = Shape<HD, WIDE>;
-  constexpr int GROUPS = HD / 4, ROWS_HERE = Join<HD, LANES>::ROWS_HERE;
+  using J = Join<HD, LANES>;
+  constexpr int GROUPS = J::GROUPS, ROWS_HERE = J::ROWS_HERE, FOURS = J::FOURS, BATCH = J::BATCH;
   lpc::pdl_trigger();
   lpc::pdl_wait();
   int item, c0, last;  // its first and last CTA
@@ -995,30 +1007,36 @@ __global__ void __launch_bounds__(Join<HD, LANES>::THREADS, Join<HD, LANES>::BLO
   const int group = (int)threadIdx.x / ROWS_HERE % GROUPS;
   const int which = (int)threadIdx.x / (ROWS_HERE * GROUPS);  // of the LANES
   const int row = rb * S::ITEM_ROWS + prow;
-  const bool in = prow < S::ITEM_ROWS && row < p.group * p.nodes && 4 * group < p.head_dim;
+  const bool in = prow < S::ITEM_ROWS && row < p.group * p.nodes && 4 * FOURS * group < p.head_dim;
   float M = -INFINITY, L = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float m, float l, const float4& v) {  // one more part
+  float4 o[FOURS];
+#pragma unroll
+  for (int f = 0; f < FOURS; ++f) o[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float m, float l, const float4 (&v)[FOURS]) {  // one more part
     const float top = fmaxf(M, m), mu = top == -INFINITY ? 0.f : top;
-    const float f = fast_exp2(M - mu), w = fast_exp2(m - mu);
+    const float a = fast_exp2(M - mu), w = fast_exp2(m - mu);
     M = top;
-    L = L * f + w * l;
-    o.x = o.x * f + w * v.x;
-    o.y = o.y * f + w * v.y;
-    o.z = o.z * f + w * v.z;
-    o.w = o.w * f + w * v.w;
+    L = L * a + w * l;
+#pragma unroll
+    for (int f = 0; f < FOURS; ++f) {
+      o[f].x = o[f].x * a + w * v[f].x;
+      o[f].y = o[f].y * a + w * v[f].y;
+      o[f].z = o[f].z * a + w * v[f].z;
+      o[f].w = o[f].w * a + w * v[f].w;
+    }
   };
-  constexpr int BATCH = Join<HD, LANES>::BATCH;
   if (in)
     for (int c = c0 + which; c <= last; c += BATCH * LANES) {
       float2 x[BATCH];
-      float4 v[BATCH];
+      float4 v[BATCH][FOURS];
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
         const int at = min(c + i * LANES, last);
         const float* part = p.parts + (2 * (int64_t)at + (at == c0 ? 1 : 0)) * S::PART;
         x[i] = reinterpret_cast<const float2*>(part + (int64_t)S::ITEM_ROWS * HD)[prow];
-        v[i] = reinterpret_cast<const float4*>(part)[group * S::ITEM_ROWS + prow];
+#pragma unroll
+        for (int f = 0; f < FOURS; ++f)
+          v[i][f] = reinterpret_cast<const float4*>(part)[(FOURS * group + f) * S::ITEM_ROWS + prow];
       }
 #pragma unroll
       for (int i = 0; i < BATCH; ++i)
@@ -1026,17 +1044,18 @@ __global__ void __launch_bounds__(Join<HD, LANES>::THREADS, Join<HD, LANES>::BLO
     }
   if constexpr (LANES > 1) {
     constexpr int HERE = ROWS_HERE * GROUPS;
-    __shared__ float4 s_o[LANES][HERE];
+    __shared__ float4 s_o[LANES][HERE][FOURS];
     __shared__ float2 s_ml[LANES][HERE];
     const int at = (int)threadIdx.x % HERE;
-    s_o[which][at] = o;
+#pragma unroll
+    for (int f = 0; f < FOURS; ++f) s_o[which][at][f] = o[f];
     s_ml[which][at] = make_float2(M, L);
     __syncthreads();
     if (which) return;
 #pragma unroll
     for (int i = 1; i < LANES; ++i) add(s_ml[i][at].x, s_ml[i][at].y, s_o[i][at]);
   }
-  if (in) store_row<T>(p, b, kvh, row, 4 * group, o, L);
+  if (in) store_row<T, FOURS>(p, b, kvh, row, 4 * FOURS * group, o, L);
 }
 
 // CTAs of a call: one an SM, no more than there can be tiles.
