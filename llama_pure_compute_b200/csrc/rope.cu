@@ -168,7 +168,8 @@ constexpr int RA_THREADS = 256;  // block size at most (chunks * hpb)
 
 // TREE: the seq tokens of sequence b are the nodes of a drafted tree.  Node s goes to cache row
 // seq_lens[b] + s and is rotated at position seq_lens[b] + depths[s]; a node of negative depth,
-// and one outside the rows or the tables, gives a zero q.
+// and one outside the rows or the tables, gives a zero q.  64 trees of 64 nodes (103 MB) 25 us,
+// 4.1 TB/s; one of 16 nodes 2.4 us.
 struct TreeRows {
   const int32_t* seq_lens;
   const int32_t* depths;
