@@ -37,7 +37,7 @@
 // Bound: issue slots (65 % of them at 512 rows; fp64 17 %).  512 rows of 32,000 bf16 with
 // top-p 61 us: a row takes 42,000 cycles with a second one on its SM, 4,000 of them loads,
 // 11,000 the histogram, 14,500 the weights' pass, 5,000 the token.  Without filters 37, top-k
-// 50 39, greedy 16; 256 rows of 128,256 77, with top-p 250 where the place's list overflows.
+// 50 39, greedy 16; 256 rows of 128,256 77, with top-p 197, as some rows' lists overflow.
 // fp32 weights first and the integers only near a border gained 15 % there and lost 35 % on
 // flat rows (registers, rows that need both); 1024 threads a row were slower.
 #include <atomic>
@@ -76,10 +76,13 @@ constexpr int LIST_BYTES = LIST * 8;
 constexpr double FIXED = 17592186044416.0;       // 2^44
 constexpr double ROUND52 = 4503599627370496.0;   // 2^52: adding it rounds to an integer
 constexpr int OCTAVE = 64;                       // bins an octave of the weight
-// What the fp32 histogram may be off, relative to all weights: its elements by 2^-16 of
-// rounding and 4e-6 of fp32 arithmetic, twice, their sums by 2048 * 2^-24, twice, and what
-// lies below its 32 octaves, at most 770,048 * 2^-32 = 1.8e-4.
-constexpr float SLACK = 5e-4f;
+// What the histogram may be off, relative to all weights, in a running sum and once more in
+// p * (their sum): its elements by 2^-16 of rounding and 4e-6 of fp32 arithmetic (3.9e-5 in
+// all), their fp32 sums by 33 roundings on the way (a thread's 4 bins, 5 steps of a scan, 16
+// warps, 8 CTAs; 4e-6 in all) and exp2f's 2 ulp; 5e-5 covers them.  Then what lies below its
+// 32 octaves, at most 2^-32 of the largest an element.  (By 5e-4 for all rows 256 of 128,256
+// with top-p 0.95 took 250 us, so 197: more of them have a list that holds their window.)
+__device__ __forceinline__ float slack_of(int vocab) { return 5e-5f + (float)vocab * 2.33e-10f; }
 constexpr int SLICE_BYTES = 84 * 1024;           // preferred share of a CTA
 constexpr int LONG = 24000;                      // elements of a row worth several CTAs
 constexpr int MAX_SLICE_BYTES = 188 * 1024;
@@ -590,11 +593,10 @@ class Row {
     return (int)sh.cross[0];
   }
   // The bins between which the running sum of the weights passes p * (their sum), with
-  // SLACK on either side: sh.window.  False: it may pass below all bins.
-  __device__ bool window(float p) {
+  // `slack` of all on either side: sh.window.  False: it may pass below all bins.
+  __device__ bool window(float p, float slack) {
     uint64_t v[MINE];
     merge<false>(v);
-    // fp32 from here on: 2^-24 * 2048, far inside SLACK
     float w[MINE], own = 0;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
@@ -635,7 +637,7 @@ class Row {
           total += x;
         }
     }
-    const float lo = (p - SLACK) * total, hi = (p + SLACK) * total;
+    const float lo = (p - slack) * total, hi = (p + slack) * total;
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
       const int bin = first_bin() + i;
@@ -1037,7 +1039,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
   if (top_p < 1.f && ties == ~0ull && binned) {
     if (top_k > 0 && top_k < a.vocab) row.sync();  // a histogram before has been read
     row.template histogram<true>();
-    if (row.window(top_p)) {
+    if (row.window(top_p, slack_of(a.vocab))) {
       const uint32_t w0 = (uint32_t)sh.window[0], w1 = (uint32_t)sh.window[1];
       const float above_from = w0 == 0 ? INFINITY : row.bin_start((int)w0 - 1, unit);
       const float list_from = row.bin_start((int)w1, unit);
