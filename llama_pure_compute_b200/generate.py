@@ -57,13 +57,13 @@ def sample_next_token(logits: torch.Tensor, *, temperature: float, top_k: int, t
 
     With ``min_p`` (tokens of less than that share of the likeliest one's probability are
     out) or given random numbers ``uniforms`` (fp32, one a row, in [0, 1)) it is
-    ``ops.sample_tokens``."""
+    ``ops.sample_tokens``; a row of nothing to draw gives token 0, as argmax does."""
     if temperature < 0:
         raise ValueError("temperature must be >= 0")
     if uniforms is not None or min_p != 0:
         if uniforms is None:
             uniforms = torch.rand(logits.shape[:-1], device=logits.device)
-        return sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p).unsqueeze(-1)
+        return sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p).clamp_(min=0).unsqueeze(-1)
     if temperature == 0:
         return torch.argmax(logits, dim=-1, keepdim=True)
     logits = logits / temperature

@@ -129,10 +129,12 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
     """Speculative decoding of a (possibly ragged) batch, one graph replay a step.
 
     ``drafter(roots)`` gets the tokens sampled last (int64 [B], device) and returns
-    its guesses for nodes 1 to T - 1 (int64 [B, T - 1]); it runs between the steps.
+    its guesses for nodes 1 to T - 1 (int64 [B, T - 1]; one outside the vocabulary counts
+    as its nearest token); it runs between the steps.
     ``temperature``, ``top_k``, ``top_p`` and ``min_p`` are those of
     ``sample_tokens`` (temperature 0: greedy); ``generator`` makes the random
-    numbers, one a sequence and position."""
+    numbers, one a sequence and position.  A token of -1: the model's logits left
+    nothing to draw; the sequence goes on as after token 0."""
 
     def __init__(self, model: torch.nn.Module, kv_cache: Union[KVCacheManager, RaggedKVCache],
                  batch_size: int, tree: DraftTree,
@@ -157,6 +159,7 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
         self.accepted = torch.zeros(batch_size, dtype=torch.int32, device=self.device)
         self.new_tokens = torch.zeros(batch_size, tree.nodes, dtype=torch.long, device=self.device)
         self.cache: Optional[TreeCache] = None
+        self.started = False  # a prefill's sequences stand where step() takes them on
 
     def _pick(self, logits: torch.Tensor, start: int, stop: int, length: int) -> torch.Tensor:
         return sample_tokens(logits, self.uniforms[start:stop, length], **self.settings)
@@ -171,10 +174,11 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
             self.cache = TreeCache(self.kv, self.B, self.tree)
         elif self.ragged:  # the captured step has the lengths of its own selection
             self.cache.lens.copy_(self.kv.active_lens)
+        self.started = True
         return first
 
     def _begin(self, first: torch.Tensor, lens: List[int]) -> None:
-        self.tokens[:, 0] = first
+        self.tokens[:, 0] = first.clamp(min=0)
 
     def _step_body(self) -> None:
         cache = self.cache
@@ -186,7 +190,7 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
         accepted, tokens, _ = cache.accept(self.tokens, sampled, self.active)
         self.accepted.copy_(accepted)
         self.new_tokens.copy_(tokens)
-        self.tokens[:, :1].copy_(tokens.gather(1, (accepted[:, None] - 1).long()))
+        self.tokens[:, :1].copy_(tokens.gather(1, (accepted[:, None] - 1).long()).clamp_(min=0))
 
     @torch.inference_mode()
     def capture(self) -> None:
@@ -209,11 +213,16 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
     @torch.inference_mode()
     def step(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """One forward: (tokens [B, T], accepted [B]) on the device -- sequence b goes on
-        by ``tokens[b, :accepted[b]]``.  Its cache needs T free rows."""
-        if self.cache is None:
+        by ``tokens[b, :accepted[b]]``.  Its cache needs T free rows.  After ``generate``,
+        whose sequences end at different steps, a prefill comes first."""
+        if not self.started:
             raise RuntimeError("prefill first")
         if self.tree.nodes > 1:
-            self.tokens[:, 1:].copy_(self.drafter(self.tokens[:, 0].clone()))
+            guesses = self.drafter(self.tokens[:, 0].clone())
+            if guesses.shape != (self.B, self.tree.nodes - 1) or guesses.dtype != torch.int64:
+                raise ValueError(f"the drafter gave {tuple(guesses.shape)} {guesses.dtype}, not int64 "
+                                 f"{(self.B, self.tree.nodes - 1)}")
+            self.tokens[:, 1:].copy_(guesses.clamp(0, self.model.config.vocab_size - 1))
         if self.use_graph:
             if self.graph is None:
                 self.capture()
@@ -248,4 +257,5 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
                     out[b, have[b]:have[b] + n] = tokens[b, :n]
                     have[b] += n
             self.active.copy_(torch.tensor([int(h < max_new_tokens) for h in have], dtype=torch.int32))
+        self.started = False
         return out

@@ -202,3 +202,25 @@ def test_refusals():
     with pytest.raises(ValueError, match="share memory"):
         both = torch.zeros(8, device=DEV)
         ops.sample_tokens(x, both[:4], out=both.view(torch.int64))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n", [1, 9, 10, 18, 19, 37])
+def test_few_long_rows(n, kind):
+    """Rows of eight, four and one CTA, of lengths that those do not divide, flat and peaked."""
+    for vocab in (24000, 24001, 40007):
+        x, u = rows(n, vocab, kind, n + vocab, spread=0.5 if vocab == 24001 else 2.0)
+        check(x, u, temperature=0.9, top_p=0.95)
+        check(x, u, top_k=60, top_p=0.9)
+        check(x, u, min_p=0.02)
+        check(x, u, temperature=0.0)
+
+
+@pytest.mark.parametrize("top_p", [1e-6, 4e-5, 0.5, 0.99, 0.9999, 1 - 2.0 ** -24])
+def test_window_of_top_p(top_p):
+    """Shares that end at, and next to, the histogram's own error; weights that all lie in a few
+    bins, and ones that mostly lie below all of them."""
+    for spread in (0.01, 1.0, 30.0):
+        x, u = rows(4, 20011, "fp32", 3, spread)
+        check(x, u, top_p=top_p)
+        check(x, u, top_p=top_p, temperature=0.05)

@@ -298,6 +298,17 @@ def test_graphs_streams_and_workspaces():
         assert torch.equal(a.run(), outs[0])
 
 
+@pytest.mark.parametrize("ragged", [False, True], ids=["dense", "ragged"])
+@pytest.mark.parametrize("dim,heads,kv,nodes", [(32, 8, 8, 16), (64, 16, 4, 64), (128, 16, 8, 20), (128, 32, 4, 64)])
+@pytest.mark.parametrize("batch,most", [(70, 60), (40, 190), (300, 60)])
+def test_many_short_items(batch, most, dim, heads, kv, nodes, ragged):
+    """Many items of one or two tiles: stretches of whole items, with and without parts to join,
+    and more CTAs than SMs."""
+    r = random.Random(batch)
+    c = Case([r.randint(0, most) for _ in range(batch)], nodes, heads, kv, dim, BF, ragged)
+    c.check(sequences=[0, 1, batch - 1] + r.sample(range(batch), 12))
+
+
 def test_views_of_q_and_masks():
     c = Case([50, 7], 6, 4, 2, 64, BF, False)
     want = c.run().clone()

@@ -262,3 +262,53 @@ def test_refusals(model):
     with pytest.raises(RuntimeError, match="prefill"):
         dec.step()
     assert c.num_layers == 3
+
+
+def test_steps_go_on_from_a_prefill_only(model):
+    """generate leaves its sequences at different places: step() would take them on wrongly."""
+    prompts = prompts_of([6, 9])
+    dec = BatchedTreeDecoder(model, cache_of(model, False, 2), 2, DraftTree([-1]))
+    dec.generate(prompts, 5)
+    with pytest.raises(RuntimeError, match="prefill"):
+        dec.step()
+    dec.prefill(prompts)
+    dec.step()
+    dec.release()
+
+
+def test_guesses_that_are_no_tokens(model):
+    """A drafter without a guess: nothing outside the embedding is read, tokens stay the greedy ones."""
+    prompts = prompts_of([6, 9])
+    tree = DraftTree(TREE)
+    want = BatchedTreeDecoder(model, cache_of(model, False, 2), 2, DraftTree([-1])).generate(prompts, 8)
+    for guess in (-1, -2 ** 63, 2 ** 63 - 1, SHAPE["vocab_size"]):
+        dec = BatchedTreeDecoder(model, cache_of(model, False, 2), 2, tree,
+                                 lambda r: torch.full((2, tree.nodes - 1), guess, device=DEV), use_cuda_graph=False)
+        got = dec.generate(prompts, 8)
+        for p, tokens in zip(prompts, got.cpu()):
+            mine, gap, _ = model.oracle.greedy(torch.tensor([p]), 8, forced=tokens[None])
+            assert ((mine[0] == tokens) | (gap[0] <= TIE)).all()
+        assert (got[:, 0] == want[:, 0]).all()
+    for bad in (torch.zeros(2, 1, dtype=torch.long, device=DEV), torch.zeros(2, tree.nodes - 1, device=DEV),
+                torch.zeros(tree.nodes - 1, dtype=torch.long, device=DEV)):
+        dec = BatchedTreeDecoder(model, cache_of(model, False, 2), 2, tree, lambda r: bad)
+        dec.prefill(prompts)
+        with pytest.raises(ValueError, match="drafter"):
+            dec.step()
+
+
+def test_logits_that_leave_nothing(model):
+    """A model whose logits are NaN gives -1 and does not read embeddings out of range."""
+    weight = model.lm_head.weight
+    was = weight.detach().clone()
+    try:
+        with torch.no_grad():
+            weight.fill_(float("nan"))
+        dec = BatchedTreeDecoder(model, cache_of(model, False, 2), 2, DraftTree([-1]), use_cuda_graph=False,
+                                 temperature=1.0)
+        assert (dec.generate(prompts_of([6, 9]), 4) == -1).all()
+        x = torch.full((2, 9), float("nan"), device=DEV)
+        assert (sample_next_token(x, temperature=1.0, top_k=0, top_p=1.0, min_p=0.5) == 0).all()
+    finally:
+        with torch.no_grad():
+            weight.copy_(was)
