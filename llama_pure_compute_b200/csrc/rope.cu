@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(RA_THREADS, 3) rope_kv_append_kernel(
   } else {
     const int64_t sb = __ldg(seq_base + b);
     const int64_t cap = __ldg(seq_cap + b);
-    ok = ok && sb >= 0 && slot < cap && sb + cap <= total_rows;
+    ok = ok && sb >= 0 && slot < cap && sb <= total_rows - cap;  // no sum that may overflow
     row = sb + slot;
     head_rows = total_rows;
   }

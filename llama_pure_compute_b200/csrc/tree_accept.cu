@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(THREADS)
   if (a.seq_base) {
     const int64_t base = a.seq_base[b];
     cap = a.seq_cap[b];
-    ok = ok && base >= 0 && cap >= 0 && base + cap <= a.total_rows;
+    ok = ok && base >= 0 && cap >= 0 && base <= a.total_rows - cap;
     row = base + n;
     head_rows = a.total_rows;
   } else {

@@ -194,7 +194,7 @@ __device__ __forceinline__ Sequence sequence_of(const Params& p, int b, bool rep
   if (p.seq_base) {
     s.row0 = lpc::ld_dep(p.seq_base + b);
     cap = lpc::ld_dep(p.seq_cap + b);
-    if (s.row0 < 0 || cap < 0 || s.row0 + cap > p.total_rows) {
+    if (s.row0 < 0 || cap < 0 || s.row0 > p.total_rows - cap) {
       bad = true;
       s.row0 = 0;
       cap = 0;

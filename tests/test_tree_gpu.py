@@ -230,3 +230,32 @@ def test_refusals():
         ops.LayerCaches([kc[..., :4].contiguous()], [kc[..., :4].contiguous()])
     torch.cuda.synchronize()
     _lib.device_status()
+
+
+@pytest.mark.parametrize("base", [2 ** 63 - 1, 2 ** 63 - 3, -2 ** 63, 2 ** 32])
+def test_places_that_no_sum_can_hold(base):
+    """A ragged sequence whose rows would begin past every number: flagged, nothing is moved."""
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    kc, vc = (new_cache((None, 40), 2, 64, torch.bfloat16, gen) for _ in range(2))
+    bases = torch.tensor([0, base], device=DEV)
+    caps = torch.tensor([20, 20], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([3, 3], dtype=torch.int32, device=DEV)
+    depths = torch.arange(3, dtype=torch.int32, device=DEV)
+    qkv = torch.randn(2, 3, 6 * 64, device=DEV, generator=gen).to(torch.bfloat16)
+    table = torch.randn(20, 64, device=DEV, generator=gen).to(torch.bfloat16)
+    was = kc.clone(), vc.clone()
+    q = ops.rope_kv_append_tree(qkv, lens, depths, table, table, kc, vc, 2, 2, bases, caps)
+    assert _lib.device_status() == 2 and (q[1] == 0).all() and (q[0] != 0).any()
+    for c, w in zip((kc, vc), was):
+        assert torch.equal(c[:, :3], w[:, :3]) and torch.equal(c[:, 6:], w[:, 6:])
+    masks = torch.tensor([1, 3, 7], device=DEV)
+    out = ops.tree_attention(torch.ones_like(q), kc, vc, lens, masks, seq_base=bases, seq_cap=caps)
+    assert _lib.device_status() == 2 and (out[1] == 0).all() and (out[0] != 0).any()
+    was = kc.clone(), vc.clone()
+    drafted = torch.tensor([[0, 1, 2]] * 2, device=DEV)
+    parents = torch.tensor([-1, 0, 0], dtype=torch.int32, device=DEV)
+    sampled = torch.tensor([[2, 0, 0]] * 2, device=DEV)  # node 2 moves to row 1
+    got = ops.tree_accept(drafted, parents, sampled, lens, ops.LayerCaches([kc], [vc], bases, caps))
+    assert _lib.device_status() == 2 and got[0].tolist() == [2, 2]
+    for c, w in zip((kc, vc), was):
+        assert torch.equal(c[:, 4], w[:, 5]) and torch.equal(c[:, 5:], w[:, 5:]) and torch.equal(c[:, :4], w[:, :4])
