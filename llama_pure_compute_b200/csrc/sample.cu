@@ -35,9 +35,10 @@
 //   * The token: sums of each warp's stretch, a scan over the cluster's warps, and
 //     the warp whose stretch holds the border walks it.
 // Bound: issue slots (65 % of them at 512 rows; fp64 17 %).  512 rows of 32,000 bf16 with
-// top-p 61 us: a row takes 42,000 cycles with a second one on its SM, 4,000 of them loads,
-// 11,000 the histogram, 14,500 the weights' pass, 5,000 the token.  Without filters 37, top-k
-// 50 39, greedy 16; 256 rows of 128,256 77, with top-p 197, as some rows' lists overflow.
+// top-p 59 us, 75 instructions an element: a row takes 40,000 cycles with a second one on its
+// SM, 4,000 of them loads, 10,000 the histogram, 14,500 the weights' pass, 5,000 the token.
+// Without filters 37 (43 instructions), top-k 50 39 (33), greedy 16 (17); 256 rows of 128,256
+// 77, with top-p 191, as some rows' lists overflow.
 // fp32 weights first and the integers only near a border gained 15 % there and lost 35 % on
 // flat rows (registers, rows that need both); 1024 threads a row were slower.
 #include <atomic>
@@ -502,6 +503,9 @@ class Row {
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     const uint32_t base = lpc::smem_u32(hist) - 4u * 0x4b000000u;  // the bits of 2^23
+    // what lies below all bins goes to unused words: a branch an element cost 7 instructions
+    // of 82 (512 rows of 32,000 with top-p: 62.4 us, so 58.9)
+    const uint32_t nowhere = lpc::smem_u32(hist + BINS + lane);
     each([&](const Chunk<T>& x, int) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -510,10 +514,12 @@ class Row {
         uint32_t add = 1u;
         if constexpr (MASS) {
           // 2^15 * 2^(-rest / OCTAVE), by two terms of the series (2e-7 off)
-          const float e = fmaf(d, octaves, 8388608.f - t) * (-0.69314718f / OCTAVE);
-          add = __float_as_uint(fmaf(fmaf(e, 0.5f, 1.f) * e, 32768.f, 32768.f + 8388608.f)) - 0x4b000000u;
+          constexpr float STEP = -0.69314718f / OCTAVE;
+          const float rest = fmaf(d, octaves, 8388608.f - t);
+          add = __float_as_uint(fmaf(fmaf(rest, 16384.f * STEP * STEP, 32768.f * STEP), rest,
+                                     32768.f + 8388608.f)) - 0x4b000000u;
         }
-        if (d >= lowest) atom_add(base + 4u * __float_as_uint(t), add);
+        atom_add(d >= lowest ? base + 4u * __float_as_uint(t) : nowhere, add);
       }
     });
     sync();
@@ -654,7 +660,7 @@ class Row {
   __device__ __forceinline__ void list(const Chunk<T>& x, int at, float from, float below) {
     unsigned mine = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) mine |= x.get(i) >= from && x.get(i) < below ? 1u << i : 0u;
+    for (int i = 0; i < N; ++i) mine |= x.get(i) >= from && !(x.get(i) >= below) ? 1u << i : 0u;
     if (!mine) return;
     uint32_t to = atomicAdd(&sh.listed, (uint32_t)__popc(mine));
 #pragma unroll
@@ -1052,8 +1058,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const Args a) {
             const float f = x.get(i);
             const uint64_t w = row.template weight<true>(f);
             all += w;
-            above += f >= above_from ? w : 0ull;
-            if constexpr (decltype(two)::value) mine_kept += f >= kept_from ? w : 0ull;
+            if (f >= above_from) above += w;
+            if constexpr (decltype(two)::value)
+              if (f >= kept_from) mine_kept += w;
           }
           row.list(x, at, list_from, above_from);
         });
