@@ -624,10 +624,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       while (ok && w.next()) {
         const int tails = w.tails();
         if (tails) {
-          // asked for only once the epilogue before has read sh.bad
-          ok = __all_sync(~0u, lpc::mbar_wait(to_fix, fixes & 1u, st));
-          if (!ok) break;
-          ++fixes;
           uint64_t seen = 0;  // by any node
           for (int t = lane; t < p.nodes; t += 32)
             seen |= (uint64_t)p.masks[w.b * p.masks_stride + t];
@@ -637,42 +633,60 @@ __global__ void __launch_bounds__(NTHREADS, 1)
               lane == 0)
             atomicOr(&g_tree_status, LPC_DEV_ERR_BOUNDS);  // a visible node past the rows
           seen &= node_bits(w.s.end - w.s.n);
+          // asked for only once the epilogue before has read sh.bad
+          ok = __all_sync(~0u, lpc::mbar_wait(to_fix, fixes & 1u, st));
+          if (!ok) break;
+          ++fixes;
           uint64_t bad = 0;
           for (int i = w.count - tails; i < w.count && ok; ++i) {
             // both tails at most: the ring holds them side by side
             const uint32_t at = v_at(ring, i, w.count);
             ok = __all_sync(~0u, lpc::mbar_wait(full(at), slot_parity(at), st));
             if (!ok) break;
-            const int k0 = (w.j0 + i) * KEYS;
+            // A row is LANES 16-byte pieces, one a lane.  Rows behind the nodes are overwritten
+            // unread, nodes are looked at four rows at a time: the last product of an item
+            // and its epilogue wait for this (6000 cycles a row after a row, of the 8800
+            // from the last softmax to the next item's).
+            const int first = (w.j0 + i) * KEYS - w.s.n;  // row 0 as a node
             uint8_t* tile = smem_raw + (slot(at) - raw);
-            // a row a turn, half a row of boxes a lane: 16 bytes a lane
-            constexpr int LANES = HD / 8;           // lanes that hold a row
-            constexpr int AT_ONCE = 32 / LANES;     // rows a warp looks at
+            constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES, BATCH = 4;
             const int sub = lane / LANES, part = lane % LANES;
-            const int from = max(0, min(w.s.n - k0, KEYS));
-            for (int q0 = from + (warp - 10) * AT_ONCE; q0 < KEYS; q0 += 2 * AT_ONCE) {
-              const int q = q0 + sub;
-              const int node = k0 + q - w.s.n;
-              uint4* x = reinterpret_cast<uint4*>(tile + (part / 8) * HALF_BYTES + q * 128) + part % 8;
-              bool clear = q < KEYS, odd = false;
-              if (q < KEYS && node < 64 && (seen >> node & 1)) {
-                const uint4 v = *x;
+            const int mine = (warp - 10) * AT_ONCE + sub;
+            auto piece = [&](int q) {
+              return reinterpret_cast<uint4*>(tile + (part / 8) * HALF_BYTES + q * 128) + part % 8;
+            };
+            const int from = max(0, -first);                     // the first node's row
+            const int to = min(KEYS, w.s.end - w.s.n - first);   // behind the last one's
+#pragma unroll 8
+            for (int q = max(from, to) + mine; q < KEYS; q += 2 * AT_ONCE)
+              *piece(q) = make_uint4(0, 0, 0, 0);
+            for (int q0 = from; q0 < to; q0 += 2 * AT_ONCE * BATCH) {
+              uint4 v[BATCH];
+              bool clear[BATCH];
+#pragma unroll
+              for (int u = 0; u < BATCH; ++u) {
+                const int q = q0 + mine + 2 * AT_ONCE * u;
+                v[u] = make_uint4(0, 0, 0, 0);
+                clear[u] = q < to && !(seen >> (first + q) & 1);  // nobody sees it
+                if (q < to) v[u] = *piece(q);
+              }
+#pragma unroll
+              for (int u = 0; u < BATCH; ++u) {
+                const int q = q0 + mine + 2 * AT_ONCE * u;
                 constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
-                auto inf = [&](uint32_t u) {
-                  const uint32_t m = u & e;
+                auto inf = [&](uint32_t x) {
+                  const uint32_t m = x & e;
                   return (m & 0xffffu) == (e & 0xffffu) || (m >> 16) == (e >> 16);
                 };
-                odd = inf(v.x) || inf(v.y) || inf(v.z) || inf(v.w);
-                clear = false;
+                const bool odd = !clear[u] && (inf(v[u].x) || inf(v[u].y) || inf(v[u].z) || inf(v[u].w));
+                // the whole row goes by any of its pieces
+                const unsigned row = (LANES == 32 ? ~0u : ((1u << LANES) - 1u)) << (sub * LANES);
+                if (__ballot_sync(~0u, odd) & row) {
+                  clear[u] = true;
+                  bad |= 1ull << (first + q);
+                }
+                if (clear[u]) *piece(q) = make_uint4(0, 0, 0, 0);
               }
-              // the whole row goes by any of its lanes
-              const unsigned group = (LANES == 32 ? ~0u : ((1u << LANES) - 1u)) << (sub * LANES);
-              const bool any = (__ballot_sync(~0u, odd) & group) != 0;
-              if (any) {
-                clear = true;
-                bad |= 1ull << node;
-              }
-              if (clear) *x = make_uint4(0, 0, 0, 0);
             }
           }
           lpc::fence_proxy_async_smem();
