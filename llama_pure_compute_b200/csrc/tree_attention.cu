@@ -572,21 +572,25 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           const int n = w.count;
           if (!(ok = lpc::mbar_wait(q_full(r), q_parity(r), st))) break;
           lpc::tc_fence_after();
+          // Tails may be cleared from the scores of the first of them on: every use of the
+          // ring's slots before theirs has landed by then, so the clearing warps cannot take
+          // an older phase for theirs.
+          const int tails = w.tails();
+          bool ready = false;  // O of the segment before, and with it sh.bad, has been read
+          auto ask = [&](int i) {
+            if (tails && i == n - tails) lpc::mbar_arrive(to_fix);
+          };
           // S of tile i; the last one of the segment releases Q
           auto scores = [&](int t, int i) -> bool {
             const bool last = WIDE ? t == 1 : true;
             if (!issue_s(t, k_at(ring, i), last)) return false;
             if (last && i == n - 1) lpc::umma_commit(q_empty(r));
+            if (ready && (!WIDE || t == 0)) ask(i);
             return true;
           };
           bool clean = false;  // the segment's tails are
           auto values = [&](int t, int i) -> bool {
             if (!clean && w.tail(w.j0 + i)) {
-              // the last V tile is here, so the ring is in the phase that the clearing warps
-              // wait for; it goes on under the softmax
-              const uint32_t last = v_at(ring, n - 1, n);
-              if (!lpc::mbar_wait(full(last), slot_parity(last), st)) return false;
-              lpc::mbar_arrive(to_fix);
               if (!lpc::mbar_wait(fixed, fixes & 1u, st)) return false;
               ++fixes;
               clean = true;
@@ -597,9 +601,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             if (WIDE ? i == n - 1 : i + 2 >= n) lpc::umma_commit(o_done(t));
             return true;
           };
-          // O of the segment before has been read
           auto o_ready = [&]() -> bool {
-            return r == 0 || lpc::mbar_wait(o_free, (uint32_t)(r - 1) & 1u, st);
+            ready = r == 0 || lpc::mbar_wait(o_free, (uint32_t)(r - 1) & 1u, st);
+            if (ready) ask(0);
+            if (ready && !WIDE) ask(1);  // their scores are on the way
+            return ready;
           };
           if constexpr (WIDE) {
             ok = scores(0, 0) && scores(1, 0) && o_ready();
