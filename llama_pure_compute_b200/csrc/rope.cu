@@ -168,8 +168,11 @@ constexpr int RA_THREADS = 256;  // block size at most (chunks * hpb)
 
 // TREE: the seq tokens of sequence b are the nodes of a drafted tree.  Node s goes to cache row
 // seq_lens[b] + s and is rotated at position seq_lens[b] + depths[s]; a node of negative depth,
-// and one outside the rows or the tables, gives a zero q.  64 trees of 64 nodes (103 MB) 25 us,
-// 4.1 TB/s; one of 16 nodes 2.4 us.
+// and one outside the rows or the tables, gives a zero q.  64 trees of 64 nodes, 32 heads on 8
+// (103 MB) 22.6 us, 4.5 TB/s; one of 16 nodes 2.3 us.  A token is a chain of dependent reads, so
+// up to two items a thread leave registers for a fourth CTA an SM (24.9 us with three); with
+// three or four items it would spill (32 x 64 nodes, 32 heads: 19.7 us with three, 20.3 with
+// four CTAs of two items).
 struct TreeRows {
   const int32_t* seq_lens;
   const int32_t* depths;
@@ -177,7 +180,7 @@ struct TreeRows {
 };
 
 template <typename T, typename TT, int VEC, int K, bool TREE>
-__global__ void __launch_bounds__(RA_THREADS, 3) rope_kv_append_kernel(
+__global__ void __launch_bounds__(RA_THREADS, TREE && K <= 2 ? 4 : 3) rope_kv_append_kernel(
     const T* __restrict__ qkv, const int64_t* __restrict__ positions, const TT* __restrict__ cosb,
     const TT* __restrict__ sinb, int64_t table_rows, T* __restrict__ q_out,
     T* __restrict__ kcache, T* __restrict__ vcache, int64_t seq, int num_heads, int num_kv_heads,
