@@ -43,9 +43,9 @@
 // Tensor memory: S0 S1 O0 O1, 128 columns each.
 //
 // Times (us; bytes' or operations' floor): 32 sequences of up to 4096 keys, 8 KV heads of 96
-// rows 65 (45), of 16 rows 60 (42): 0.8 us a tile of 64 KB while all SMs load, 4 us a further
+// rows 63 (45), of 16 rows 58 (42): 0.8 us a tile of 64 KB while all SMs load, 2.5 us a further
 // item of a stretch (pipeline out and in, O), 5 to 6 around (cutting, join).  3 sequences of
-// 60,000 keys, 8 KV heads of 512 rows 338 (225 at the burst rate of dense products, 271 at the
+// 60,000 keys, 8 KV heads of 512 rows 322 to 336 (225 at the burst rate of dense products, 271 at the
 // sustained): 1.1 PFLOP/s at the 1.4 GHz that the power cap leaves.  A tile of 256 rows takes
 // 3150 cycles, 2048 of them MMA: a stream's softmax 1920 (scores 95, maximum 345, exponentials
 // 1380), 200 to hand P over, 1030 for its PV and next S.  Slower, all measured: S in two
@@ -87,8 +87,8 @@ static_assert(128 * REGS_LOAD + 256 * REGS_SOFTMAX <= NTHREADS * LAUNCH_REGS,
               "register split exceeds the block's launch allocation");
 
 // Tiles that an item's begin and end cost: the pipeline fills and drains, O is written.
-// 32 sequences of up to 4096 keys, 8 KV heads of 96 rows: 73 us counted as three, 71 as
-// four, 65 as five or six; 16 rows, D = 64 and long sequences differ by 3 %.
+// 32 sequences of up to 4096 keys, 8 KV heads of 96 rows: 65.5 us counted as three, 64.5 as
+// four, 63 as five; 16 rows, D = 64 and long sequences differ by 2 %.
 constexpr int START = 5;
 
 // What a sequence holds: n keys of context, keys and nodes together up to `end`,
