@@ -22,8 +22,9 @@ import torch
 
 from .generate import BatchedGreedyDecoder
 from .kv_manager import KVCacheManager
-from .ops import (MAX_TREE_NODES, LayerCaches, StepWorkspaces, rope_kv_append_tree, sample_tokens,
-                  tree_accept, tree_attention, tree_attention_workspace)
+from .ops import (MAX_TREE_NODES, LayerCaches, StepWorkspaces, decode_attention, decode_attention_ragged,
+                  qkv_rope_append, rope_kv_append, rope_kv_append_ragged, rope_kv_append_tree,
+                  sample_tokens, tree_accept, tree_attention, tree_attention_workspace)
 from .ragged_cache import RaggedKVCache
 
 __all__ = ["DraftTree", "TreeCache", "BatchedTreeDecoder"]
@@ -62,7 +63,8 @@ class TreeCache:
     """A 16-bit cache for forwards over trees: ``LlamaForCausalLM`` takes it as its
     ``kv_cache`` with ``input_ids`` [B, T], row b a tree over the sequence of row b
     (a ragged cache's selection).  The nodes' K and V go to the rows behind the
-    sequence's ``seq_lens`` keys; ``accept`` keeps a branch of them."""
+    sequence's ``seq_lens`` keys; ``accept`` keeps a branch of them.  A tree of one
+    node is a decode step, and takes that step's kernels."""
 
     def __init__(self, kv_cache: Union[KVCacheManager, RaggedKVCache], batch: int, tree: DraftTree):
         if type(kv_cache) not in (KVCacheManager, RaggedKVCache):
@@ -83,6 +85,9 @@ class TreeCache:
                 raise ValueError("batch size exceeds cache capacity")
             self.lens, self._ids = kv_cache.seq_lens[:batch], None
             self.base = self.cap = None
+        if tree.nodes == 1:
+            self.keys = torch.empty(batch, dtype=torch.int32, device=kv_cache.device)
+            self.place = torch.empty(batch, 1, dtype=torch.int64, device=kv_cache.device)
         self.layers = LayerCaches(kv_cache.k_cache, kv_cache.v_cache, self.base, self.cap)
         self._workspaces = StepWorkspaces()
 
@@ -94,6 +99,11 @@ class TreeCache:
             raise ValueError(f"forward of {B} x {T} tokens over {self.batch} trees of "
                              f"{self.tree.nodes} nodes")
         ctx.decode = True
+        if T == 1:
+            self.place.copy_(self.lens[:, None])
+            ctx.seq_lens = torch.add(self.lens, 1, out=self.keys)
+            ctx.workspace = self.kv.decode_workspace(B, num_heads)
+            return
         ctx.fused_qkv_max = 0  # that kernel's rows are its rotary positions
         ctx.seq_lens = self.lens
         ctx.workspace = None
@@ -102,6 +112,8 @@ class TreeCache:
                qkv: Optional[torch.Tensor] = None, x: Optional[torch.Tensor] = None,
                packed_qkv=None, norm_eps: float = 0.0) -> torch.Tensor:
         kc, vc = self.kv.k_cache[layer_idx], self.kv.v_cache[layer_idx]
+        if self.tree.nodes == 1:
+            return self._attend_one(kc, vc, ctx, num_heads, scale, qkv, x, packed_qkv, norm_eps)
         q = rope_kv_append_tree(qkv, self.lens, self.tree.depths, ctx.cos_table, ctx.sin_table, kc,
                                 vc, num_heads, self.kv.n_kv_heads, self.base, self.cap)
         if ctx.workspace is None:
@@ -110,6 +122,25 @@ class TreeCache:
                              ctx.workspace)
         B, H, T, D = out.shape
         return out.transpose(1, 2).reshape(B, T, H * D)  # a view: it is laid out so
+
+    def _attend_one(self, kc, vc, ctx, num_heads, scale, qkv, x, packed_qkv, norm_eps):
+        kv_heads, base, cap = self.kv.n_kv_heads, self.base, self.cap
+        if packed_qkv is not None:
+            q = qkv_rope_append(x, packed_qkv, self.place, ctx.cos_table, ctx.sin_table, kc, vc, num_heads,
+                                kv_heads, seq_base=base, seq_cap=cap, norm_eps=norm_eps)
+        elif base is None:
+            q = rope_kv_append(qkv, self.place, ctx.cos_table, ctx.sin_table, kc, vc, num_heads, kv_heads)
+        else:
+            q = rope_kv_append_ragged(qkv, self.place, ctx.cos_table, ctx.sin_table, kc, vc, base, cap,
+                                      num_heads, kv_heads)
+        B, D = self.batch, self.kv.head_dim
+        q = q.view(B, num_heads, D)
+        if base is None:
+            out = decode_attention(q, kc, vc, ctx.seq_lens, scale, workspace=ctx.workspace)
+        else:
+            out = decode_attention_ragged(q, kc, vc, ctx.seq_lens, base, cap, self.kv.max_seq_len, scale,
+                                          workspace=ctx.workspace)
+        return out.view(B, 1, num_heads * D)
 
     # -- after the forward --------------------------------------------------------
     @torch.no_grad()

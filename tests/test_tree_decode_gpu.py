@@ -312,3 +312,23 @@ def test_logits_that_leave_nothing(model):
     finally:
         with torch.no_grad():
             weight.copy_(was)
+
+
+@pytest.mark.parametrize("ragged", [False, True], ids=["dense", "ragged"])
+@pytest.mark.parametrize("graph", [True, False], ids=["graph", "eager"])
+def test_root_alone_is_a_decode_step(model, ragged, graph):
+    """Trees of one node take the decode step's kernels: its tokens, bit by bit; sequences that
+    are done wait for the others."""
+    prompts = prompts_of([5, 17, 17, 40])
+    want = BatchedGreedyDecoder(model, cache_of(model, ragged, 4), 4, use_cuda_graph=graph).generate(prompts, 20)
+    kv = cache_of(model, ragged, 4)
+    dec = BatchedTreeDecoder(model, kv, 4, DraftTree([-1]), use_cuda_graph=graph)
+    for _ in range(2):
+        assert torch.equal(dec.generate(prompts, 20), want)
+        assert kv.seq_lens[:4].tolist() == [len(p) + 19 for p in prompts]
+    dec.prefill(prompts)
+    dec.active[1] = 0  # stays where it is
+    for _ in range(3):
+        dec.step()
+    assert kv.seq_lens[:4].tolist() == [8, 17, 20, 43]
+    dec.release()
