@@ -309,6 +309,22 @@ def test_many_short_items(batch, most, dim, heads, kv, nodes, ragged):
     c.check(sequences=[0, 1, batch - 1] + r.sample(range(batch), 12))
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(8, 4, 64), (16, 4, 128), (32, 2, 128)])
+@pytest.mark.parametrize("most", [60, 300])
+def test_values_that_are_not_finite_stay_with_their_sequence(most, heads, kv, dim):
+    """Many short items after one another in a CTA, every third with an infinite value that some of
+    its nodes see: what is kept about one item's values is not taken for the next one's."""
+    r = random.Random(most)
+    c = Case([r.randint(0, most) for _ in range(200)], 20, heads, kv, dim, BF, False)
+    for b in range(0, 200, 3):
+        c.rows(c.v, b)[:, c.lens[b] + r.randint(0, 19), r.randrange(dim)] = r.choice([math.inf, -math.inf, math.nan])
+    for _ in range(3):
+        out = c.run()
+        clean = [b for b in range(200) if b % 3]
+        assert not out[clean].isnan().any() and not out[clean].isinf().any()
+        c.check(out, sequences=range(0, 200, 7))
+
+
 def test_views_of_q_and_masks():
     c = Case([50, 7], 6, 4, 2, 64, BF, False)
     want = c.run().clone()

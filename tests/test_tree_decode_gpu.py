@@ -332,3 +332,16 @@ def test_root_alone_is_a_decode_step(model, ragged, graph):
         dec.step()
     assert kv.seq_lens[:4].tolist() == [8, 17, 20, 43]
     dec.release()
+
+
+@pytest.mark.parametrize("ragged", [False, True], ids=["dense", "ragged"])
+def test_root_alone_with_the_fused_projection(ragged):
+    """head_dim 128: the decode step projects, rotates and appends in one kernel."""
+    shape = dict(SHAPE, num_heads=2, num_kv_heads=1)
+    cfg = LlamaModelConfig(**shape)
+    m = LlamaForCausalLM.from_state_dict(cfg, make_state_dict(shape, 5), device=DEV, dtype=torch.bfloat16)
+    prompts = prompts_of([7, 30, 12])
+    want = BatchedGreedyDecoder(m, cache_of(m, ragged, 3), 3).generate(prompts, 15)
+    dec = BatchedTreeDecoder(m, cache_of(m, ragged, 3), 3, DraftTree([-1]))
+    assert torch.equal(dec.generate(prompts, 15), want)
+    dec.release()
