@@ -13,7 +13,7 @@
 // cheaper than a second launch that waits for the first.  The bound is latency: the
 // rows of a branch are a few kilobytes a layer.  One sequence, 16 nodes, 32 layers
 // 3.1 us; 64 sequences of 64 nodes, whose branches move 207 rows of 32 layers (54 MB in
-// and out, 8.3 us at the copy rate), 14 us.
+// and out, 8.3 us at the copy rate), 12.7 us.
 #include "lpc_common.cuh"
 
 LPC_DECLARE_STATUS(g_accept_status)
@@ -33,7 +33,10 @@ namespace {
 constexpr int MAX_NODES = 64;
 constexpr int MAX_LAYERS = 128;  // a launch
 constexpr int THREADS = 128;
-constexpr int BATCH = 8;         // rows in flight a thread
+// Rows in flight a thread, and CTAs an SM: four and twelve take 12.7 us where eight, whose
+// registers leave room for seven CTAs, took 13.9 (64 sequences, 207 rows of 32 layers).
+constexpr int BATCH = 4;
+constexpr int BLOCKS = 12;
 
 template <int LAYERS>
 struct Caches {
@@ -56,7 +59,7 @@ struct Args {
 };
 
 template <int LAYERS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, BLOCKS)
     tree_accept_kernel(const Args a, const __grid_constant__ Caches<LAYERS> caches) {
   __shared__ int32_t s_path[MAX_NODES];
   __shared__ int s_count;
