@@ -148,7 +148,8 @@ class TreeCache:
                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """``tree_accept`` in every layer; the sequences' lengths grow by what was
         accepted (times ``active``, int32 [B], if given: 0 leaves a sequence where it
-        is).  Returns (accepted, tokens, path)."""
+        is, and its next root has to stay the one it had).  Returns (accepted, tokens,
+        path), of a sequence that stays too what its tree would have given."""
         got = tree_accept(drafted, self.tree.parents, sampled, self.lens, self.layers)
         self.lens.add_(got[0] if active is None else got[0] * active)
         if self._ids is not None:
@@ -165,7 +166,11 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
     ``temperature``, ``top_k``, ``top_p`` and ``min_p`` are those of
     ``sample_tokens`` (temperature 0: greedy); ``generator`` makes the random
     numbers, one a sequence and position.  A token of -1: the model's logits left
-    nothing to draw; the sequence goes on as after token 0."""
+    nothing to draw; the sequence goes on as after token 0.
+
+    ``active`` (int32 [B], device; 1 after a prefill): a sequence whose entry is set to
+    0 waits.  Steps leave its tokens and its length as they are and give 0 accepted
+    tokens for it."""
 
     def __init__(self, model: torch.nn.Module, kv_cache: Union[KVCacheManager, RaggedKVCache],
                  batch_size: int, tree: DraftTree,
@@ -219,9 +224,11 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
         u = self.uniforms.gather(1, (self.positions + 1).clamp_(max=self.rows))
         sampled = sample_tokens(logits, u, **self.settings)
         accepted, tokens, _ = cache.accept(self.tokens, sampled, self.active)
-        self.accepted.copy_(accepted)
-        self.new_tokens.copy_(tokens)
-        self.tokens[:, :1].copy_(tokens.gather(1, (accepted[:, None] - 1).long()).clamp_(min=0))
+        waits = self.active[:, None] == 0
+        roots = tokens.gather(1, (accepted[:, None] - 1).long()).clamp_(min=0)
+        self.tokens[:, :1].copy_(torch.where(waits, self.tokens[:, :1], roots))
+        self.accepted.copy_(accepted.masked_fill_(waits[:, 0], 0))
+        self.new_tokens.copy_(tokens.masked_fill_(waits, -1))
 
     @torch.inference_mode()
     def capture(self) -> None:

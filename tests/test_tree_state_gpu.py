@@ -1,0 +1,73 @@
+"""What a BatchedTreeDecoder and its caches hold between steps."""
+import pytest
+import torch
+
+from llama_pure_compute_b200 import BatchedTreeDecoder, DraftTree, _lib
+from test_tree_decode_gpu import DEV, TIE, TREE, Guesses, cache_of, model, prompts_of  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+LAYOUTS = pytest.mark.parametrize("ragged", [False, True], ids=["dense", "ragged"])
+GRAPHS = pytest.mark.parametrize("graph", [True, False], ids=["graph", "eager"])
+
+
+@pytest.fixture(autouse=True)
+def _clean_status():
+    yield
+    assert _lib.device_status() == 0
+
+
+def greedy_by_the_oracle(model, prompts, texts):  # noqa: F811
+    for p, tokens in zip(prompts, texts):
+        forced = torch.tensor([tokens])
+        mine, gap, _ = model.oracle.greedy(torch.tensor([p]), len(tokens), forced=forced)
+        assert ((mine == forced) | (gap <= TIE)).all()
+
+
+def steps(dec, got, n, guesses=None):
+    """n steps; the new tokens go behind `got`."""
+    for _ in range(n):
+        tokens, accepted = dec.step()
+        for b, (row, count) in enumerate(zip(tokens.tolist(), accepted.tolist())):
+            assert row[count:] == [-1] * (len(row) - count)
+            got[b] += row[:count]
+            if guesses is not None:
+                guesses.at[b] += count
+
+
+@LAYOUTS
+@GRAPHS
+@pytest.mark.parametrize("temperature", [0.0, 1.2])
+@pytest.mark.parametrize("parents", [[-1], TREE], ids=["root", "tree"])
+def test_a_sequence_that_waits_goes_on_where_it_was(model, ragged, graph, parents, temperature):  # noqa: F811
+    """active 0: no tokens, the same length and the same root; afterwards the text goes on, and the
+    cache holds what a plain run over that text holds."""
+    prompts = prompts_of([5, 17, 9])
+    texts = [model.oracle.greedy(torch.tensor([p]), 40)[0][0].tolist() for p in prompts]
+    guesses = Guesses(parents, texts, 0.7)
+    dec = BatchedTreeDecoder(model, cache_of(model, ragged, 3), 3, DraftTree(parents),
+                             guesses if len(parents) > 1 else None, use_cuda_graph=graph, temperature=temperature,
+                             generator=torch.Generator(device=DEV).manual_seed(2))
+    got = [[t] for t in dec.prefill(prompts).tolist()]
+    guesses.at = [1, 1, 1]
+    for active, n in (([1, 1, 1], 2), ([1, 0, 1], 3), ([0, 1, 0], 3), ([1, 1, 1], 2)):
+        dec.active.copy_(torch.tensor(active))
+        had = [list(g) for g in got]
+        for _ in range(n):
+            steps(dec, got, 1, guesses)
+            assert dec.tokens[:, 0].tolist() == [g[-1] for g in got]
+        for b in range(3):
+            assert len(got[b]) >= len(had[b]) + n if active[b] else got[b] == had[b]
+    lens = [len(p) + len(g) - 1 for p, g in zip(prompts, got)]
+    assert dec.kv.seq_lens[:3].tolist() == lens
+    if temperature == 0:
+        greedy_by_the_oracle(model, prompts, got)
+    for b, (p, tokens) in enumerate(zip(prompts, got)):
+        one = cache_of(model, False, 1)
+        ids = torch.tensor([p + tokens[:-1]], device=DEV)
+        model(ids, positions=torch.arange(ids.shape[1], device=DEV)[None], kv_cache=one)
+        for mine, theirs in ((dec.kv.k_cache, one.k_cache), (dec.kv.v_cache, one.v_cache)):
+            for x, y in zip(mine, theirs):
+                x = x[:, dec.kv.bases[b]:][:, :lens[b]] if ragged else x[b, :, :lens[b]]
+                y = y[0, :, :lens[b]]
+                assert (x.float() - y.float()).abs().max() <= 2 ** -5 * y.float().abs().max()
+    dec.release()
