@@ -203,6 +203,7 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
     @torch.inference_mode()
     def prefill(self, prompts: Union[torch.Tensor, List[List[int]]]) -> torch.Tensor:
         """Returns the first generated token of each sequence (device, [B])."""
+        self.started = False
         self.uniforms.uniform_(generator=self.generator)
         first = super().prefill(prompts)
         self.active.fill_(1)
@@ -232,6 +233,8 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
 
     @torch.inference_mode()
     def capture(self) -> None:
+        if not self.started:
+            raise RuntimeError("prefill first")
         lens0 = self.cache.lens.clone()
         tok0 = self.tokens.clone()
         s = torch.cuda.Stream(self.device)
@@ -252,7 +255,8 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
     def step(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """One forward: (tokens [B, T], accepted [B]) on the device -- sequence b goes on
         by ``tokens[b, :accepted[b]]``.  Its cache needs T free rows.  After ``generate``,
-        whose sequences end at different steps, a prefill comes first."""
+        whose sequences end at different steps, and after a prefill that failed, a prefill
+        comes first."""
         if not self.started:
             raise RuntimeError("prefill first")
         if self.tree.nodes > 1:
@@ -287,13 +291,15 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
         out = torch.empty(self.B, max_new_tokens, dtype=torch.long, device=self.device)
         out[:, 0] = self.prefill(rows)
         have = [1] * self.B
-        while min(have) < max_new_tokens:
-            tokens, accepted = self.step()
-            for b, n in enumerate(accepted.tolist()):
-                if have[b] < max_new_tokens:
-                    n = min(n, max_new_tokens - have[b])
-                    out[b, have[b]:have[b] + n] = tokens[b, :n]
-                    have[b] += n
-            self.active.copy_(torch.tensor([int(h < max_new_tokens) for h in have], dtype=torch.int32))
-        self.started = False
+        try:
+            while min(have) < max_new_tokens:
+                tokens, accepted = self.step()
+                for b, n in enumerate(accepted.tolist()):
+                    if have[b] < max_new_tokens:
+                        n = min(n, max_new_tokens - have[b])
+                        out[b, have[b]:have[b] + n] = tokens[b, :n]
+                        have[b] += n
+                self.active.copy_(torch.tensor([int(h < max_new_tokens) for h in have], dtype=torch.int32))
+        finally:
+            self.started = False
         return out

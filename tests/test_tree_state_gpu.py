@@ -71,3 +71,33 @@ def test_a_sequence_that_waits_goes_on_where_it_was(model, ragged, graph, parent
                 y = y[0, :, :lens[b]]
                 assert (x.float() - y.float()).abs().max() <= 2 ** -5 * y.float().abs().max()
     dec.release()
+
+
+def test_no_steps_after_a_run_that_was_broken_off(model):  # noqa: F811
+    """A drafter that raises, a prompt that does not fit: sequences stand anywhere, a prefill comes first."""
+    prompts = prompts_of([6, 9])
+    tree = DraftTree.chain(3)
+    calls = []
+
+    def drafter(roots):
+        calls.append(1)
+        if len(calls) == 3:
+            raise KeyError("no more")
+        return torch.zeros(2, 2, dtype=torch.long, device=DEV)
+    dec = BatchedTreeDecoder(model, cache_of(model, False, 2), 2, tree, drafter)
+    with pytest.raises(KeyError):
+        dec.generate(prompts, 12)
+    with pytest.raises(RuntimeError, match="prefill"):
+        dec.step()
+    dec.prefill(prompts)
+    dec.step()
+    with pytest.raises(ValueError):
+        dec.prefill(prompts_of([6, 400]))
+    with pytest.raises(RuntimeError, match="prefill"):
+        dec.step()
+    with pytest.raises(RuntimeError, match="prefill"):
+        dec.capture()
+    dec.release()
+    fresh = BatchedTreeDecoder(model, cache_of(model, False, 2), 2, tree, drafter)
+    with pytest.raises(RuntimeError, match="prefill"):
+        fresh.capture()
