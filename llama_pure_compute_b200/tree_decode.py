@@ -78,8 +78,10 @@ class TreeCache:
                 raise ValueError(f"batch of {batch} rows but {len(kv_cache.active_ids)} selected "
                                  "sequences")
             # the selection of now: a captured step stays with it
-            self.lens, self._ids = kv_cache.active_lens, kv_cache._idx
+            self._ids = kv_cache._idx
             self.base, self.cap = kv_cache.active_base, kv_cache.active_cap
+            # the selection's lengths may be older than the sequences': as if selected again
+            self.lens = kv_cache.active_lens = kv_cache.seq_lens[self._ids]
         else:
             if not 0 < batch <= kv_cache.max_batch_size:
                 raise ValueError("batch size exceeds cache capacity")
@@ -99,6 +101,8 @@ class TreeCache:
             raise ValueError(f"forward of {B} x {T} tokens over {self.batch} trees of "
                              f"{self.tree.nodes} nodes")
         ctx.decode = True
+        if self._ids is not None:  # where the sequences stand, whoever moved them
+            torch.index_select(self.kv.seq_lens, 0, self._ids, out=self.lens)
         if T == 1:
             self.place.copy_(self.lens[:, None])
             ctx.seq_lens = torch.add(self.lens, 1, out=self.keys)
@@ -211,6 +215,7 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
             self.cache = TreeCache(self.kv, self.B, self.tree)
         elif self.ragged:  # the captured step has the lengths of its own selection
             self.cache.lens.copy_(self.kv.active_lens)
+            self.kv.active_lens = self.cache.lens
         self.started = True
         return first
 
@@ -219,7 +224,7 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
 
     def _step_body(self) -> None:
         cache = self.cache
-        torch.add(cache.lens[:, None], self.tree.depths, out=self.positions)
+        torch.add(self.kv.seq_lens[:self.B, None], self.tree.depths, out=self.positions)
         logits = self.model(self.tokens, positions=self.positions, kv_cache=cache)
         # the token after a node stands one further
         u = self.uniforms.gather(1, (self.positions + 1).clamp_(max=self.rows))
@@ -235,14 +240,16 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
     def capture(self) -> None:
         if not self.started:
             raise RuntimeError("prefill first")
-        lens0 = self.cache.lens.clone()
+        lens = self.kv.seq_lens[:self.B]
+        lens0 = lens.clone()
         tok0 = self.tokens.clone()
         s = torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(s):
             self._step_body()
         torch.cuda.current_stream(self.device).wait_stream(s)
-        self.cache.lens.copy_(lens0)
+        for t in (lens, self.cache.lens):
+            t.copy_(lens0)
         self.tokens.copy_(tok0)
         torch.cuda.synchronize(self.device)
         g = torch.cuda.CUDAGraph()

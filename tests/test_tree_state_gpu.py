@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from llama_pure_compute_b200 import BatchedTreeDecoder, DraftTree, _lib
+from llama_pure_compute_b200 import BatchedTreeDecoder, DraftTree, TreeCache, _lib
 from test_tree_decode_gpu import DEV, TIE, TREE, Guesses, cache_of, model, prompts_of  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -101,3 +101,53 @@ def test_no_steps_after_a_run_that_was_broken_off(model):  # noqa: F811
     fresh = BatchedTreeDecoder(model, cache_of(model, False, 2), 2, tree, drafter)
     with pytest.raises(RuntimeError, match="prefill"):
         fresh.capture()
+
+
+@GRAPHS
+def test_lengths_that_other_caches_read(model, graph):  # noqa: F811
+    """Steps of a second run, a selection in between, trees of another shape over the same
+    sequences: every TreeCache goes on from the lengths that the ragged cache has."""
+    prompts = prompts_of([5, 17])
+    kv = cache_of(model, True, 2)
+    texts = [model.oracle.greedy(torch.tensor([p]), 40)[0][0].tolist() for p in prompts]
+    guesses = Guesses(TREE, texts, 0.8)
+    dec = BatchedTreeDecoder(model, kv, 2, DraftTree(TREE), guesses, use_cuda_graph=graph)
+    for _ in range(2):  # the second run replays the first one's graph
+        got = [[t] for t in dec.prefill(prompts).tolist()]
+        guesses.at = [1, 1]
+        steps(dec, got, 3, guesses)
+        lens = [len(p) + len(g) - 1 for p, g in zip(prompts, got)]
+        assert kv.seq_lens.tolist() == kv.active_lens.tolist() == lens
+        assert TreeCache(kv, 2, DraftTree.chain(2)).lens.tolist() == lens
+    with torch.inference_mode():
+        early = TreeCache(kv, 2, DraftTree.chain(3))
+        kv.select([1, 0])
+        turned = TreeCache(kv, 2, DraftTree([-1]))
+        steps(dec, got, 2, guesses)
+        for cache, order in ((turned, [1, 0]), (early, [0, 1])):
+            T = cache.tree.nodes
+            roots = torch.tensor([[got[b][-1]] + [0] * (T - 1) for b in order], device=DEV)
+            logits = model(roots, positions=torch.zeros(2, T, dtype=torch.long, device=DEV), kv_cache=cache)
+            for i, b in enumerate(order):
+                full = model(torch.tensor([prompts[b] + got[b]], device=DEV))
+                assert (logits[i, 0].float() - full[0, -1].float()).abs().max() < TIE
+            accepted, tokens, _ = cache.accept(roots, logits.argmax(-1))
+            for i, b in enumerate(order):
+                got[b] += tokens[i, :accepted[i]].tolist()
+            assert kv.seq_lens.tolist() == [len(p) + len(g) - 1 for p, g in zip(prompts, got)]
+    greedy_by_the_oracle(model, prompts, got)
+    dec.release()
+
+
+@LAYOUTS
+def test_capture_leaves_the_lengths(model, ragged):  # noqa: F811
+    prompts = prompts_of([5, 17])
+    kv = cache_of(model, ragged, 2)
+    dec = BatchedTreeDecoder(model, kv, 2, DraftTree.chain(3),
+                             lambda r: torch.zeros(2, 2, dtype=torch.long, device=DEV))
+    got = [[t] for t in dec.prefill(prompts).tolist()]
+    dec.capture()
+    assert kv.seq_lens[:2].tolist() == dec.cache.lens.tolist() == [5, 17]
+    steps(dec, got, 4)
+    greedy_by_the_oracle(model, prompts, got)
+    dec.release()
