@@ -629,16 +629,21 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       Walk w(p, sh, pos, stop, seq_first, seq);
       while (ok && w.next()) {
         const int tails = w.tails();
-        if (tails) {
-          uint64_t seen = 0;  // by any node
+        // nodes that the sequence has no rows for: looked at where its last tile is, which need
+        // not be a tail (a context that fills its rows and ends with a tile)
+        const bool past = w.s.end - w.s.n < p.nodes && w.kvh == 0 && w.rb == 0 &&
+                          w.j0 + w.count == w.s.tiles;
+        uint64_t seen = 0;  // by any node
+        if (tails || past) {
           for (int t = lane; t < p.nodes; t += 32)
             seen |= (uint64_t)p.masks[w.b * p.masks_stride + t];
 #pragma unroll
           for (int m = 16; m; m >>= 1) seen |= __shfl_xor_sync(~0u, seen, m);
-          if (seen & node_bits(p.nodes) & ~node_bits(w.s.end - w.s.n) && w.kvh == 0 && w.rb == 0 &&
-              lane == 0)
+          if (past && (seen & node_bits(p.nodes) & ~node_bits(w.s.end - w.s.n)) && lane == 0)
             atomicOr(&g_tree_status, LPC_DEV_ERR_BOUNDS);  // a visible node past the rows
           seen &= node_bits(w.s.end - w.s.n);
+        }
+        if (tails) {
           // asked for only once the epilogue before has read sh.bad
           ok = __all_sync(~0u, lpc::mbar_wait(to_fix, fixes & 1u, st));
           if (!ok) break;
