@@ -505,8 +505,8 @@ LPC_API int lpc_rope_kv_append_tree(const void* qkv, const int32_t* seq_lens,
  * nodes], masks_stride elements between sequences, 0: one tree for all; bits from `nodes` on are
  * not read).  q: [batch, heads, nodes, head_dim], heads a multiple of kv_heads, head_dim 32, 64 or
  * 128, bf16 or fp16; out: [batch, nodes, heads, head_dim].  fp32 scores, maxima and sums; weights
- * rounded to the data type before they meet V.  Rows of K and V that a node does not see do not
- * reach it, whatever they hold; a node that sees nothing gives zeros.  A length beyond the
+ * rounded to the data type before they meet V (fp16: or to 2^-32 of the row's largest weight).
+ * Rows of K and V that a node does not see do not reach it, whatever they hold; a node that sees nothing gives zeros.  A length beyond the
  * sequence's rows is cut to them; it and a visible node past them are flagged in
  * lpc_device_status().  sm_scale > 0.  workspace: lpc_tree_attention_workspace_bytes() bytes for
  * the current device (0: NULL); calls that overlap need one each.  One kernel, and one more where

@@ -33,8 +33,9 @@
 //   warps 0-3, 4-7  softmax of stream 0 and 1.  Thread r has row r: its 128 scores in
 //               one read, maximum, exp2 against a reference that moves only when the
 //               maximum has grown by more than 8 (factor 256: no overflow, same
-//               softmax), P rounded to the data type (half a step, 2^-9 or 2^-12 of p;
-//               the sum is of the unrounded), O rescaled in tensor memory when the
+//               softmax), P rounded to the data type, as the product's other operand V has
+//               it (half a step at most, 2^-8 or 2^-11 of p; fp16's range: RAISE; the
+//               sum is of the unrounded), O rescaled in tensor memory when the
 //               reference moves.
 //   warps 10-11 the tiles that hold nodes or end the sequence: V rows that no node
 //               sees are cleared (0 * NaN would reach every row), and so are visible
@@ -82,6 +83,11 @@ constexpr int NTHREADS = 384;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float GROWTH = 8.0f;              // log2 units that a maximum may pass its reference
+// log2 of the weight at the reference.  fp16 holds weights below 2^-14 as subnormals and none
+// below 2^-25: 20,000 keys of 2^-25.5 of the largest each were lost, 3e-4 of the result.  With
+// 2^7 the largest is 2^15 after GROWTH, and a weight is off by 2^-32 of the largest or its half step.
+template <typename T> constexpr float RAISE = 0.0f;
+template <> constexpr float RAISE<__half> = 7.0f;
 constexpr int LAUNCH_REGS = 168, REGS_LOAD = 96, REGS_SOFTMAX = 200;
 static_assert(128 * REGS_LOAD + 256 * REGS_SOFTMAX <= NTHREADS * LAUNCH_REGS,
               "register split exceeds the block's launch allocation");
@@ -779,12 +785,13 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
         const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * p.scale_log2;  // scale > 0
         // S of this tile was issued after PV of the stream's tile before: O is stable
-        const bool grow = top > m_used + GROWTH || (m_used == -INFINITY && top > -INFINITY);
+        const bool grow = top > m_used + (GROWTH + RAISE<T>) || (m_used == -INFINITY && top > -INFINITY);
         if (__any_sync(~0u, grow)) {
           float alpha = 1.f;
           if (grow) {
-            alpha = m_used == -INFINITY ? 0.f : fast_exp2(m_used - top);
-            m_used = top;
+            const float now = top - RAISE<T>;
+            alpha = m_used == -INFINITY ? 0.f : fast_exp2(m_used - now);
+            m_used = now;
             l *= alpha;
           }
           if (mine > 0) {

@@ -1215,7 +1215,7 @@ def tree_attention(
     128, any number of query heads a KV head.
 
     Softmax statistics and sums in fp32, weights rounded to the data type before
-    they meet V.  What a node does not see does not reach it, whatever those rows
+    they meet V (fp16: or to 2^-32 of the row's largest weight).  What a node does not see does not reach it, whatever those rows
     hold; a node that sees nothing gives zeros.  A length beyond the sequence's
     rows is cut to them, which, as a visible node past them, sets the device
     status.  ``sm_scale`` (positive) defaults to ``D ** -0.5``.
