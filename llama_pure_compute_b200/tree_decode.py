@@ -168,7 +168,8 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
     its guesses for nodes 1 to T - 1 (int64 [B, T - 1]; one outside the vocabulary counts
     as its nearest token); it runs between the steps.
     ``temperature``, ``top_k``, ``top_p`` and ``min_p`` are those of
-    ``sample_tokens`` (temperature 0: greedy); ``generator`` makes the random
+    ``sample_tokens`` (temperature 0: greedy), a number or a device tensor with one
+    entry a sequence, which every step reads anew; ``generator`` makes the random
     numbers, one a sequence and position.  A token of -1: the model's logits left
     nothing to draw; the sequence goes on as after token 0.
 
@@ -179,7 +180,8 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
     def __init__(self, model: torch.nn.Module, kv_cache: Union[KVCacheManager, RaggedKVCache],
                  batch_size: int, tree: DraftTree,
                  drafter: Optional[Callable[[torch.Tensor], torch.Tensor]] = None, *,
-                 temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                 temperature: Union[float, torch.Tensor] = 0.0, top_k: Union[int, torch.Tensor] = 0,
+                 top_p: Union[float, torch.Tensor] = 1.0, min_p: Union[float, torch.Tensor] = 0.0,
                  generator: Optional[torch.Generator] = None, use_cuda_graph: bool = True,
                  prefill_chunk: int = 16) -> None:
         if type(kv_cache) not in (KVCacheManager, RaggedKVCache):
@@ -189,6 +191,10 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
             raise ValueError("a tree of more than its root needs a drafter")
         self.tree, self.drafter = tree, drafter
         self.settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        for name, value in self.settings.items():
+            if isinstance(value, torch.Tensor) and (value.get_device() != kv_cache.seq_lens.get_device()
+                                                    or value.numel() != batch_size):
+                raise ValueError(f"{name} must be a number or have one entry a sequence on the cache's device")
         self.generator = generator
         self.rows = model.config.max_seq_len  # of the rotary tables
         self.tokens = torch.zeros(batch_size, tree.nodes, dtype=torch.long, device=self.device)
@@ -201,8 +207,17 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
         self.cache: Optional[TreeCache] = None
         self.started = False  # a prefill's sequences stand where step() takes them on
 
+    def _sample(self, logits: torch.Tensor, uniforms: torch.Tensor, start: int, stop: int) -> torch.Tensor:
+        """Draws of sequences start to stop - 1, uniforms [stop - start, ...] each."""
+        def of(value):
+            if not isinstance(value, torch.Tensor):
+                return value
+            rows = value.reshape(-1)[start:stop]
+            return rows.view(-1, *[1] * (uniforms.dim() - 1)).expand(uniforms.shape)
+        return sample_tokens(logits, uniforms, **{name: of(value) for name, value in self.settings.items()})
+
     def _pick(self, logits: torch.Tensor, start: int, stop: int, length: int) -> torch.Tensor:
-        return sample_tokens(logits, self.uniforms[start:stop, length], **self.settings)
+        return self._sample(logits, self.uniforms[start:stop, length], start, stop)
 
     @torch.inference_mode()
     def prefill(self, prompts: Union[torch.Tensor, List[List[int]]]) -> torch.Tensor:
@@ -228,7 +243,7 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
         logits = self.model(self.tokens, positions=self.positions, kv_cache=cache)
         # the token after a node stands one further
         u = self.uniforms.gather(1, (self.positions + 1).clamp_(max=self.rows))
-        sampled = sample_tokens(logits, u, **self.settings)
+        sampled = self._sample(logits, u, 0, self.B)
         accepted, tokens, _ = cache.accept(self.tokens, sampled, self.active)
         waits = self.active[:, None] == 0
         roots = tokens.gather(1, (accepted[:, None] - 1).long()).clamp_(min=0)

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from llama_pure_compute_b200 import BatchedTreeDecoder, DraftTree, TreeCache, _lib
+from oracle.tree_ref import accept_ref, sample_ref
 from test_tree_decode_gpu import DEV, TIE, TREE, Guesses, cache_of, model, prompts_of  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -151,3 +152,76 @@ def test_capture_leaves_the_lengths(model, ragged):  # noqa: F811
     steps(dec, got, 4)
     greedy_by_the_oracle(model, prompts, got)
     dec.release()
+
+
+PER_SEQUENCE = [
+    dict(temperature=torch.tensor([0.0, 0.8, 1.1])),
+    dict(temperature=0.9, top_k=torch.tensor([1, 4, 0])),
+    dict(temperature=torch.tensor([0.7, 1.0, 0.0], dtype=torch.float64), top_p=torch.tensor([0.5, 1.0, 0.9]),
+         min_p=torch.tensor([0.0, 0.2, 0.0]), top_k=torch.tensor([[30], [0], [2]], dtype=torch.int32)),
+]
+
+
+@LAYOUTS
+@pytest.mark.parametrize("parents", [[-1], TREE], ids=["root", "tree"])
+@pytest.mark.parametrize("settings", PER_SEQUENCE, ids=["temperature", "top-k", "all"])
+def test_settings_of_each_sequence(model, settings, parents, ragged):  # noqa: F811
+    """Entries of B sequences hold for all of a sequence's draws: the first token's, by prefill
+    groups, and its nodes'."""
+    prompts = prompts_of([6, 25, 25])
+    T = len(parents)
+    seen = []
+
+    class Watched(torch.nn.Module):
+        config = model.config
+
+        def forward(self, ids, **kw):
+            out = model(ids, **kw)
+            seen.append((ids.clone(), kw["positions"].clone(), out.clone()))
+            return out
+    mine = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in settings.items()}
+    guesses = Guesses(parents, [[], [], []], 0.9)
+    made = dict(use_cuda_graph=False, generator=torch.Generator(device=DEV).manual_seed(4), **mine)
+    dec = BatchedTreeDecoder(Watched(), cache_of(model, ragged, 3), 3, DraftTree(parents),
+                             guesses if T > 1 else None, **made)
+    got = [[t] for t in dec.prefill(prompts).tolist()]
+    guesses.texts = got
+    steps(dec, got, 5, guesses)
+
+    def one(b):  # settings are 32-bit numbers
+        return {k: torch.as_tensor(v).reshape(-1).expand(3)[b].to(torch.int32 if k == "top_k" else torch.float32).item()
+                for k, v in settings.items()}
+    u = dec.uniforms.cpu()
+    rows = [(0, seen[0][2][0]), (1, seen[1][2][0]), (2, seen[1][2][1])]  # two groups of prompts
+    for b, logits in rows:
+        assert got[b][0] == sample_ref(logits[-1], u[b, len(prompts[b])].item(), **one(b))
+    at = [1, 1, 1]
+    for ids, positions, logits in seen[2:]:
+        for b in range(3):
+            draws = [sample_ref(logits[b, t], u[b, positions[b, t] + 1].item(), **one(b)) for t in range(T)]
+            _, tokens = accept_ref(ids[b].tolist(), parents, draws)
+            assert got[b][at[b]:at[b] + len(tokens)] == tokens
+            at[b] += len(tokens)
+    assert at == [len(g) for g in got]
+
+
+def test_settings_in_a_captured_step(model):  # noqa: F811
+    """The captured step reads the entries when it runs: what a server changes between requests holds."""
+    prompts = prompts_of([6, 25])
+    t = torch.zeros(2, device=DEV)
+    dec = BatchedTreeDecoder(model, cache_of(model, False, 2), 2, DraftTree([-1]), temperature=t, top_k=50)
+    greedy = dec.generate(prompts, 12)
+    greedy_by_the_oracle(model, prompts, greedy.tolist())
+    t[1] = 5.0
+    hot = dec.generate(prompts, 12)
+    greedy_by_the_oracle(model, prompts[:1], hot[:1].tolist())
+    assert not torch.equal(hot[1], greedy[1])
+    dec.release()
+
+
+def test_settings_that_fit_no_sequence(model):  # noqa: F811
+    kv = cache_of(model, False, 3)
+    for kw in (dict(temperature=torch.ones(2, device=DEV)), dict(top_p=torch.ones(6, device=DEV)),
+               dict(min_p=torch.zeros(3)), dict(top_k=torch.zeros((), dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            BatchedTreeDecoder(model, kv, 3, DraftTree([-1]), **kw)
