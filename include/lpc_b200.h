@@ -532,9 +532,10 @@ LPC_API int lpc_tree_attention(const void* q, const void* key_cache, const void*
  * child whose drafted token is the node's sampled one.  accepted: int32 [batch], nodes of the
  * branch, the root among them; path: int32 [batch, nodes], those nodes, then -1; tokens:
  * int64 [batch, nodes], what was sampled after them, then -1.  The K and V rows seq_lens[b] +
- * path[i] of every layer's caches (host arrays of `layers` device pointers; layers 0: none)
- * move to seq_lens[b] + i.  A branch that leaves the sequence's rows is flagged and not moved.
- * seq_lens is not changed.  elem_bytes: 2 or 4; head_dim * elem_bytes a multiple of 16.
+ * path[i] of every layer's caches (host arrays of `layers` device pointers; layers 0: none; no
+ * two of them share memory) move to seq_lens[b] + i.  A branch that leaves the sequence's rows is
+ * flagged and not moved.  seq_lens is not changed.  elem_bytes: 2 or 4; head_dim * elem_bytes a
+ * multiple of 16.
  */
 LPC_API int lpc_tree_accept(const int64_t* drafted, const int32_t* parents, int64_t parents_stride,
                             const int64_t* sampled, const int32_t* seq_lens,

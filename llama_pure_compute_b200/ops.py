@@ -1267,7 +1267,8 @@ class LayerCaches:
     """The K and V caches of a model's layers, checked once and handed to
     ``tree_accept``: dense [max_batch, kv_heads, max_seq_len, head_dim] each, or
     ragged [kv_heads, total_rows, head_dim] with ``seq_base`` (int64) and
-    ``seq_cap`` (int32), one entry a sequence of the batch."""
+    ``seq_cap`` (int32), one entry a sequence of the batch.  Each has its own memory:
+    the rows of all of them move at once."""
 
     __slots__ = ("key_caches", "value_caches", "seq_base", "seq_cap", "kv_heads", "head_dim",
                  "max_batch", "max_seq_len", "total_rows", "elem_bytes", "index", "_k", "_v", "_c")
@@ -1290,6 +1291,9 @@ class LayerCaches:
              self.total_rows) = _tree_caches(k, v, seq_base, seq_cap, batch, self.index)
         if seq_base is not None and seq_base.numel() != seq_cap.numel():
             raise ValueError("LlamaPureComputeError: seq_base and seq_cap must have the same entries.")
+        by_place = sorted((t for t in keys + values if t.numel()), key=torch.Tensor.data_ptr)
+        if any(_overlap(a, b) for a, b in zip(by_place, by_place[1:])):
+            raise ValueError("LlamaPureComputeError: the caches must not share memory.")
         self.elem_bytes = first.element_size()
         if first.numel() == 0 or self.elem_bytes not in (2, 4) or self.head_dim * self.elem_bytes % 16:
             raise TypeError("LlamaPureComputeError: cache rows must be whole 16-byte pieces of 16- or "

@@ -112,3 +112,14 @@ def test_maxima_that_grow_in_fp16(step, sign):
         bound = (h + fp32) * spread + h * want.abs() + len(rows) * 2.0 ** -32 * v.abs().max().item() + 2.0 ** -25
         err = (got[:, t].double() - want).abs()
         assert bool((err <= bound).all()), (err / bound).max().item()
+
+
+def test_a_cache_is_handed_over_once():
+    """tree_accept moves every cache by itself: the same memory twice would be moved twice at once."""
+    a, b, c = (torch.zeros(2, 2, 16, 32, device=DEV, dtype=BF) for _ in range(3))
+    ops.LayerCaches([a, b], [c, a.clone()])
+    both = torch.zeros(3, 2, 16, 32, device=DEV, dtype=BF)
+    for keys, values in (([a], [a]), ([a, b], [c, b]), ([a, a], [b, c]), ([both[:2]], [both[1:]])):
+        with pytest.raises(ValueError, match="memory"):
+            ops.LayerCaches(keys, values)
+    ops.LayerCaches([both[:1]], [both[1:2]])  # side by side
