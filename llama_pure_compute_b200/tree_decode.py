@@ -204,6 +204,7 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
         self.uniforms = torch.zeros(batch_size, self.rows + 1, device=self.device)
         self.accepted = torch.zeros(batch_size, dtype=torch.int32, device=self.device)
         self.new_tokens = torch.zeros(batch_size, tree.nodes, dtype=torch.long, device=self.device)
+        self._none = torch.full((), -1, dtype=torch.long, device=self.device)
         self.cache: Optional[TreeCache] = None
         self.started = False  # a prefill's sequences stand where step() takes them on
 
@@ -245,11 +246,12 @@ class BatchedTreeDecoder(BatchedGreedyDecoder):
         u = self.uniforms.gather(1, (self.positions + 1).clamp_(max=self.rows))
         sampled = self._sample(logits, u, 0, self.B)
         accepted, tokens, _ = cache.accept(self.tokens, sampled, self.active)
-        waits = self.active[:, None] == 0
+        goes = self.active[:, None] != 0
+        had = self.tokens[:, :1]
         roots = tokens.gather(1, (accepted[:, None] - 1).long()).clamp_(min=0)
-        self.tokens[:, :1].copy_(torch.where(waits, self.tokens[:, :1], roots))
-        self.accepted.copy_(accepted.masked_fill_(waits[:, 0], 0))
-        self.new_tokens.copy_(tokens.masked_fill_(waits, -1))
+        torch.where(goes, roots, had, out=had)
+        torch.mul(accepted, self.active, out=self.accepted)
+        torch.where(goes, tokens, self._none, out=self.new_tokens)
 
     @torch.inference_mode()
     def capture(self) -> None:
