@@ -527,8 +527,8 @@ LPC_API int lpc_tree_attention(const void* q, const void* key_cache, const void*
 /*
  * The branch of each tree that the samples agree with.  drafted, sampled: int64 [batch,
  * nodes], the token of a node and the one sampled after it; parents: int32, as depths above
- * (parents[t] < t; the root's is not read; a node whose parent is not before it is nobody's
- * child and flagged in lpc_device_status()).  From the root the branch goes on to the lowest
+ * (parents[t] < t; the root's is not read; a node of negative parent is nobody's child, and so
+ * is one whose parent is not before it, which is flagged in lpc_device_status()).  From the root the branch goes on to the lowest
  * child whose drafted token is the node's sampled one.  accepted: int32 [batch], nodes of the
  * branch, the root among them; path: int32 [batch, nodes], those nodes, then -1; tokens:
  * int64 [batch, nodes], what was sampled after them, then -1.  The K and V rows seq_lens[b] +

@@ -169,10 +169,11 @@ constexpr int RA_THREADS = 256;  // block size at most (chunks * hpb)
 // TREE: the seq tokens of sequence b are the nodes of a drafted tree.  Node s goes to cache row
 // seq_lens[b] + s and is rotated at position seq_lens[b] + depths[s]; a node of negative depth,
 // and one outside the rows or the tables, gives a zero q.  64 trees of 64 nodes, 32 heads on 8
-// (103 MB) 22.6 us, 4.5 TB/s; one of 16 nodes 2.3 us.  A token is a chain of dependent reads, so
-// up to two items a thread leave registers for a fourth CTA an SM (24.9 us with three); with
-// three or four items it would spill (32 x 64 nodes, 32 heads: 19.7 us with three, 20.3 with
-// four CTAs of two items).
+// (103 MB) 22.5 to 23.3 us, 4.4 to 4.6 TB/s; one of 16 nodes 2.5 us.  A token is a chain of
+// dependent reads, so with up to two items a thread registers are capped at 64 for a fourth CTA
+// an SM: two items then spill 28 bytes (44 with fp32 tables), and are faster all the same (24.9
+// us with three CTAs).  Three and four items have three CTAs, 80 registers and 24 to 60 bytes of
+// spills (32 x 64 nodes, 32 heads: 19.7 us; 20.3 with four CTAs of two items).
 struct TreeRows {
   const int32_t* seq_lens;
   const int32_t* depths;

@@ -35,10 +35,11 @@
 //   * The token: sums of each warp's stretch, a scan over the cluster's warps, and
 //     the warp whose stretch holds the border walks it.
 // Bound: issue slots (65 % of them at 512 rows; fp64 17 %).  512 rows of 32,000 bf16 with
-// top-p 59 us, 75 instructions an element: a row takes 40,000 cycles with a second one on its
+// top-p 57 us, 75 instructions an element: a row takes 40,000 cycles with a second one on its
 // SM, 4,000 of them loads, 10,000 the histogram, 14,500 the weights' pass, 5,000 the token.
-// Without filters 37 (43 instructions), top-k 50 39 (33), greedy 16 (17); 256 rows of 128,256
-// 77, with top-p 191, as some rows' lists overflow.
+// Without filters 35 (43 instructions), top-k 50 38 (33), greedy 14 (17); 256 rows of 128,256
+// 77, with top-p 193, as some rows' lists overflow.  Two CTAs an SM leave 64 registers; what
+// does not fit, 44 to 92 bytes of one-CTA rows and 176 to 192 of clusters', is spilled.
 // fp32 weights first and the integers only near a border gained 15 % there and lost 35 % on
 // flat rows (registers, rows that need both); 1024 threads a row were slower.
 #include <atomic>

@@ -43,11 +43,12 @@
 //               to the nodes that do see them.
 // Tensor memory: S0 S1 O0 O1, 128 columns each.
 //
-// Times (us; bytes' or operations' floor): 32 sequences of up to 4096 keys, 8 KV heads of 96
-// rows 63 (45), of 16 rows 58 (42): 0.8 us a tile of 64 KB while all SMs load, 2.5 us a further
-// item of a stretch (pipeline out and in, O), 5 to 6 around (cutting, join).  3 sequences of
-// 60,000 keys, 8 KV heads of 512 rows 322 to 336 (225 at the burst rate of dense products, 271 at the
-// sustained): 1.1 PFLOP/s at the 1.4 GHz that the power cap leaves.  A tile of 256 rows takes
+// Times (us, from a CUDA graph; bytes' or operations' floor): 32 sequences of up to 4096 keys, 8
+// KV heads of 96 rows 62 (45), of 16 rows 58 (43): 0.8 us a tile of 64 KB while all SMs load, 2.5
+// us a further item of a stretch (pipeline out and in, O), 5 to 6 around (cutting, join).  3
+// sequences of 60,000 keys, 8 KV heads of 512 rows 327 to 335 for some milliseconds (225 at the
+// burst rate of dense products), 405 after seconds of it, at the 1.35 GHz that the power cap leaves
+// (271 at the sustained rate): 1.1 and 0.93 PFLOP/s.  A tile of 256 rows takes
 // 3150 cycles, 2048 of them MMA: a stream's softmax 1920 (scores 95, maximum 345, exponentials
 // 1380), 200 to hand P over, 1030 for its PV and next S.  Slower, all measured: S in two
 // buffers of 64 keys (507: Q is read twice as often), two softmax threads a row (383), a

@@ -57,7 +57,9 @@ def sample_next_token(logits: torch.Tensor, *, temperature: float, top_k: int, t
 
     With ``min_p`` (tokens of less than that share of the likeliest one's probability are
     out) or given random numbers ``uniforms`` (fp32, one a row, in [0, 1)) it is
-    ``ops.sample_tokens``; a row of nothing to draw gives token 0, as argmax does."""
+    ``ops.sample_tokens``; a row of nothing to draw gives token 0, as argmax does.  Of logits
+    equal to the k-th, ``ops.sample_tokens`` keeps the first by index, so that exactly ``top_k``
+    stay; without these two all of them stay."""
     if temperature < 0:
         raise ValueError("temperature must be >= 0")
     if uniforms is not None or min_p != 0:

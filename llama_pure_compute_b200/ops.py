@@ -1320,7 +1320,8 @@ def tree_accept(
 
     ``drafted`` (int64 [B, T]): the tokens of the nodes; ``sampled`` (int64 [B, T]):
     what the model draws after each; ``parents`` (int32 [B, T], or [T] for one
-    tree): ``parents[t] < t``, the root's is not read.  From the root the branch
+    tree): ``parents[t] < t``, the root's is not read; a node with a negative one is
+    nobody's child (padding of a smaller tree).  From the root the branch
     goes on, while there is one, to the lowest child whose token is the node's
     sampled one.  Returns
 

@@ -123,3 +123,14 @@ def test_a_cache_is_handed_over_once():
         with pytest.raises(ValueError, match="memory"):
             ops.LayerCaches(keys, values)
     ops.LayerCaches([both[:1]], [both[1:2]])  # side by side
+
+
+def test_nodes_that_only_fill_up_a_smaller_tree():
+    """A negative parent: nobody's child, whatever the token, and no fault of the tree's."""
+    parents = torch.tensor([[-1, 0, 1, -1], [-1, 0, -2 ** 31, -5]], dtype=torch.int32, device=DEV)
+    drafted = torch.tensor([[3, 4, -1, -1], [3, 4, 5, -1]], device=DEV)
+    sampled = torch.tensor([[4, -1, -1, -1], [4, 5, -1, 0]], device=DEV)
+    accepted, tokens, path = ops.tree_accept(drafted, parents, sampled)
+    assert accepted.tolist() == [3, 2] and path.tolist() == [[0, 1, 2, -1], [0, 1, -1, -1]]
+    assert tokens.tolist() == [[4, -1, -1, -1], [4, 5, -1, -1]]
+    assert _lib.device_status() == 0
