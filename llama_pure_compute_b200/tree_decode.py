@@ -102,7 +102,8 @@ class TreeCache:
                              f"{self.tree.nodes} nodes")
         ctx.decode = True
         if self._ids is not None:  # where the sequences stand, whoever moved them
-            torch.index_select(self.kv.seq_lens, 0, self._ids, out=self.lens)
+            with torch.inference_mode():  # the lengths may have been made there
+                torch.index_select(self.kv.seq_lens, 0, self._ids, out=self.lens)
         if T == 1:
             self.place.copy_(self.lens[:, None])
             ctx.seq_lens = torch.add(self.lens, 1, out=self.keys)

@@ -225,3 +225,29 @@ def test_settings_that_fit_no_sequence(model):  # noqa: F811
                dict(min_p=torch.zeros(3)), dict(top_k=torch.zeros((), dtype=torch.int32, device=DEV))):
         with pytest.raises(ValueError, match=next(iter(kw))):
             BatchedTreeDecoder(model, kv, 3, DraftTree([-1]), **kw)
+
+
+@LAYOUTS
+def test_a_cache_made_in_inference_mode_is_read_outside(model, ragged):  # noqa: F811
+    prompts = prompts_of([9, 30])
+    kv = cache_of(model, ragged, 2)
+    tree = DraftTree(TREE)
+    with torch.inference_mode():
+        if ragged:
+            kv.select([0, 1])
+        cache = TreeCache(kv, 2, tree)
+        ids = torch.zeros(2, tree.nodes, dtype=torch.long, device=DEV)
+    for b, p in enumerate(prompts):
+        if ragged:
+            kv.select([b])
+        one = kv if ragged else cache_of(model, False, 1)
+        model(torch.tensor([p], device=DEV), positions=torch.arange(len(p), device=DEV)[None], kv_cache=one)
+        if not ragged:
+            for mine, theirs in zip(kv.k_cache + kv.v_cache, one.k_cache + one.v_cache):
+                mine[b].copy_(theirs[0])
+            kv.seq_lens[b] = len(p)
+    with torch.no_grad():
+        logits = model(ids, positions=torch.zeros_like(ids), kv_cache=cache)
+    for b, p in enumerate(prompts):
+        full = model(torch.tensor([p + [0]], device=DEV))
+        assert (logits[b, 0].float() - full[0, -1].float()).abs().max() < TIE
